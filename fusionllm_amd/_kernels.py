@@ -500,6 +500,89 @@ def dx_reduce_norm(dx_rows, pos, idx, d_logits, gate_w, rows_routed: int, has_sh
     return dx, dnw
 
 
+LAYER_NORM_MAX_DIM = 16384
+
+
+def _row_stride(t, name, dtype=None):
+    """Address and row stride of a [T, D] operand whose rows may lie apart."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a ROCm device tensor (got {t.device})")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name} must be a matrix with adjacent row elements")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise RuntimeError(f"the rows of {name} must not overlap")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype} (got {t.dtype})")
+    return t.data_ptr(), t.stride(0)
+
+
+def _vector(t, name, dim):
+    if t is None:
+        return None
+    p = _req(t, name)
+    if t.numel() != dim:
+        raise RuntimeError(f"{name} must hold {dim} values (got {tuple(t.shape)})")
+    return p
+
+
+@_timed
+def layer_norm_fwd(x, weight, bias, eps: float, out_dtype: torch.dtype, stats: bool = True):
+    """Layer norm of the rows of x [T, D] (rows may lie apart); returns y, mean, rstd (the last two
+    None without stats)."""
+    lib = _lib.load()
+    xp, ldx = _row_stride(x, "x")
+    T, d = x.shape
+    vec = weight if weight is not None else bias
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("weight and bias must have one dtype")
+    y = torch.empty(T, d, dtype=out_dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(T, dtype=torch.float32, device=x.device)
+        rstd = torch.empty(T, dtype=torch.float32, device=x.device)
+    check(lib.fmoe_layer_norm_fwd(xp, _dtype_code(x.dtype), ldx, _vector(weight, "weight", d),
+                                  _vector(bias, "bias", d), F32 if vec is None else _dtype_code(vec.dtype), T, d,
+                                  eps, y.data_ptr(), _dtype_code(out_dtype), _ptr(mean), _ptr(rstd), _stream()),
+          "fmoe_layer_norm_fwd")
+    return y, mean, rstd
+
+
+@_timed
+def layer_norm_bwd(dy, x, mean, rstd, weight, d_residual=None, need_dx: bool = True,
+                   dw_dtype: torch.dtype | None = None, db_dtype: torch.dtype | None = None):
+    """Backward of the layer norm of x [T, D]; returns dx, d_weight, d_bias, each None where it is not
+    wanted (need_dx, dw_dtype, db_dtype).  d_residual (x's dtype, dense) is added to dx."""
+    lib = _lib.load()
+    xp, ldx = _row_stride(x, "x")
+    T, d = x.shape
+    if tuple(dy.shape) != (T, d):
+        raise RuntimeError(f"dy must be {(T, d)} (got {tuple(dy.shape)})")
+    dyp, lddy = _row_stride(dy, "dy")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.numel() != T:
+            raise RuntimeError(f"{name} must hold {T} values (got {tuple(t.shape)})")
+    if d_residual is not None and tuple(d_residual.shape) != (T, d):
+        raise RuntimeError(f"d_residual must be {(T, d)} (got {tuple(d_residual.shape)})")
+    w_dtype = weight.dtype if weight is not None else dw_dtype or db_dtype or torch.float32
+    if any(t is not None and t != w_dtype for t in (dw_dtype, db_dtype)):
+        raise RuntimeError("the weight, its gradient and the bias's gradient must have one dtype")
+    dev = x.device
+    dx = torch.empty(T, d, dtype=x.dtype, device=dev) if need_dx else None
+    dw = None if dw_dtype is None else torch.empty(d, dtype=dw_dtype, device=dev)
+    db = None if db_dtype is None else torch.empty(d, dtype=db_dtype, device=dev)
+    ws, ws_bytes = None, 0
+    if dw is not None or db is not None:
+        ws_bytes = lib.fmoe_layer_norm_bwd_workspace_bytes(T, d)
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+    check(lib.fmoe_layer_norm_bwd(dyp, _dtype_code(dy.dtype), lddy, xp, _dtype_code(x.dtype), ldx,
+                                  _req(mean, "mean", torch.float32), _req(rstd, "rstd", torch.float32),
+                                  _vector(weight, "weight", d), _dtype_code(w_dtype),
+                                  None if d_residual is None else _req(d_residual, "d_residual", x.dtype),
+                                  T, d, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, _stream()),
+          "fmoe_layer_norm_bwd")
+    return dx, dw, db
+
+
 NORMUON_MAX_TENSORS = 32
 
 

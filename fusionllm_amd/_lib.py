@@ -1,4 +1,5 @@
-"""ctypes binding of libfusionmoe.so (declarations in include/fusionmoe.h).
+"""ctypes binding of libfusionmoe.so (declarations in include/fusionmoe.h and
+include/fusiontrain.h).
 
 The library is built in-tree by ``fusionllm_amd.build`` (or
 ``__graft_entry__.build()``).  There is no fallback: if the library is
@@ -13,7 +14,7 @@ from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfusionmoe.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 MAX_EXPERTS = 64
 MAX_TOPK = 8
 
@@ -71,6 +72,15 @@ SIGNATURES = {
                                     _P, _P, _P, _P, _P, _P]),
 }
 
+# the training operators around the block; mirrors include/fusiontrain.h
+TRAIN_SIGNATURES = {
+    "fmoe_layer_norm_fwd": (c_int, [_P, c_int, c_int64, _P, _P, c_int, c_int64, c_int64, c_float, _P, c_int, _P, _P,
+                                    _P]),
+    "fmoe_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "fmoe_layer_norm_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, _P, _P, c_int, _P, c_int64, c_int64,
+                                    _P, _P, _P, _P, c_size_t, _P]),
+}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -95,7 +105,7 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
                 f"{p} is missing: build the HIP extension first "
                 "(python -m fusionllm_amd.build or __graft_entry__.build())")
         lib = ctypes.CDLL(str(p))
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | TRAIN_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

@@ -46,6 +46,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _kernels as K
+from .norm import LayerNorm, check_norm_operands
 
 
 def _as_bf16(t: torch.Tensor) -> torch.Tensor:
@@ -478,6 +479,47 @@ class _NormMoEResidualFunction(torch.autograd.Function):
         return (None, None, dx, dnw, dgw, dgb, *grads_w)
 
 
+class _LayerNormMoEResidualFunction(torch.autograd.Function):
+    """x + DeepSeekMoE(LayerNorm(x)): as _NormMoEResidualFunction, with the layer
+    norm's kernels.  The MoE's input gradient reaches the norm's backward in
+    fp32, and that adds the residual's gradient.
+
+    Inputs: (meta, eps, x[T,d], norm.weight or None, norm.bias or None,
+    gate.weight, gate.bias, *weights).  Outputs as _MoEBlockFunction.
+    """
+
+    @staticmethod
+    def forward(ctx, meta, eps, x, norm_w, norm_b, gate_w, gate_b, *weights):
+        xc = x.contiguous()
+        nw = None if norm_w is None else norm_w.contiguous()
+        nb = None if norm_b is None else norm_b.contiguous()
+        xn, mean, rstd = K.layer_norm_fwd(xc, nw, nb, eps, torch.bfloat16)
+        counts_host = _host_counts(meta)
+        fw = _forward_pass(meta, xn, gate_w, gate_b, weights, residual=xc, counts_host=counts_host)
+        saved = _save_forward(ctx, meta, fw, gate_w, gate_b, weights, counts_host)
+        ctx.norm_dtypes = tuple(None if p is None else p.dtype for p in (norm_w, norm_b))
+        ctx.save_for_backward(xc, mean, rstd, nw, *saved)
+        idx64, w, counts, y = fw[4], fw[5], fw[7], fw[-1]
+        return y, idx64, w, counts
+
+    @staticmethod
+    def backward(ctx, dy, _d_idx, _d_w, _d_counts):
+        n_w = len(ctx.param_dtypes[2])
+        if dy is None:
+            return (None,) * (7 + n_w)
+        xc, mean, rstd, nw, *saved = ctx.saved_tensors
+        E, k, inter, rs, has_shared, out_dtype = ctx.meta
+        gwb, idx, pos = saved[1], saved[2], saved[7]
+        dy = dy.contiguous()
+        dx_rows, d_logits, dgw, dgb, grads_w = _backward_pass(ctx, saved, dy)
+        d_xn = K.dx_reduce(dx_rows, pos, idx, d_logits, gwb, idx.shape[0] * k, has_shared, torch.float32)
+        need_x, need_w, need_b = ctx.needs_input_grad[2:5]
+        dx, dnw, dnb = K.layer_norm_bwd(d_xn, xc, mean, rstd, nw, dy if need_x else None, need_x,
+                                        ctx.norm_dtypes[0] if need_w else None,
+                                        ctx.norm_dtypes[1] if need_b else None)
+        return (None, None, dx, dnw, dnb, dgw, dgb, *grads_w)
+
+
 class DeepSeekMoE(nn.Module):
     """DeepSeekMoE with aux-loss-free biased sigmoid routing (reference: models/moe.py:24-109)."""
 
@@ -576,14 +618,16 @@ class DeepSeekMoE(nn.Module):
             return self._forward_empty(flat, out_dtype).view(shape)
         return self._run(flat, weights, out_dtype).view(shape)
 
-    def forward_norm_residual(self, x: torch.Tensor, norm: nn.RMSNorm) -> torch.Tensor:
+    def forward_norm_residual(self, x: torch.Tensor, norm: nn.RMSNorm | LayerNorm) -> torch.Tensor:
         """``x + self(norm(x))`` in one pass: the FFN half of
         FusionLLMBlock.forward (models/fusionllm.py:52) with its
-        ``norm2 = nn.RMSNorm(dim, eps=1e-6)`` (models/fusionllm.py:48).
+        ``norm2 = nn.RMSNorm(dim, eps=1e-6)`` (models/fusionllm.py:48), or with
+        this package's ``LayerNorm``.
 
-        The norm's parameters stay in ``norm`` (its weight gets its gradient
-        as usual).  Same dtype rules as ``forward``, with x standing for the
-        norm's output; a bf16 x needs a bf16 norm weight.
+        The norm's parameters stay in ``norm`` (they get their gradients as
+        usual).  Same dtype rules as ``forward``, with x standing for the
+        norm's output; a bf16 x needs a bf16 RMSNorm weight.  (A layer norm of a
+        bf16 x under autocast gives fp32: the plain expression.)
         """
         if tuple(norm.normalized_shape) != (self.dim,):
             raise ValueError(f"norm must normalise the last dimension {self.dim} (got {norm.normalized_shape})")
@@ -592,7 +636,12 @@ class DeepSeekMoE(nn.Module):
         if not flat.is_cuda:
             raise RuntimeError("fusionllm_amd.DeepSeekMoE runs on a ROCm device only (got a CPU tensor)")
         nw = norm.weight
-        if nw is not None and flat.dtype == torch.bfloat16 and nw.dtype != torch.bfloat16:
+        layer = isinstance(norm, LayerNorm)
+        if layer:
+            check_norm_operands(flat, nw, norm.bias)
+            if torch.is_autocast_enabled("cuda") and flat.dtype == torch.bfloat16:
+                return x + self.forward(norm(x))
+        elif nw is not None and flat.dtype == torch.bfloat16 and nw.dtype != torch.bfloat16:
             raise NotImplementedError("a bf16 input needs a bf16 RMSNorm weight")
         if nw is not None and nw.device != flat.device:
             raise RuntimeError("the RMSNorm weight must be on the input's device")
@@ -603,9 +652,10 @@ class DeepSeekMoE(nn.Module):
             # around the block's operator
             return x + self.forward(norm(x))
         eps = norm.eps if norm.eps is not None else torch.finfo(flat.dtype).eps
-        return self._run(flat, weights, out_dtype, norm_w=nw, eps=float(eps), fused_norm=True).view(shape)
+        return self._run(flat, weights, out_dtype, norm_w=nw, eps=float(eps), fused_norm=True,
+                         norm_b=norm.bias if layer else None, layer_norm=layer).view(shape)
 
-    def _run(self, flat, weights, out_dtype, norm_w=None, eps=0.0, fused_norm=False):
+    def _run(self, flat, weights, out_dtype, norm_w=None, eps=0.0, fused_norm=False, norm_b=None, layer_norm=False):
         E, k = self.n_routed_experts, self.n_activated_experts
         if torch.compiler.is_compiling():
             # traced (torch.compile): the block as the fusionllm::moe_fwd operator
@@ -625,11 +675,15 @@ class DeepSeekMoE(nn.Module):
         meta = (E, k, self.moe_inter_dim, float(self.route_scale), has_shared, out_dtype)
         needs_grad = torch.is_grad_enabled() and (
             flat.requires_grad or gw.requires_grad or gb.requires_grad
-            or any(t.requires_grad for t in weights) or (norm_w is not None and norm_w.requires_grad))
+            or any(t.requires_grad for t in weights) or (norm_w is not None and norm_w.requires_grad)
+            or (norm_b is not None and norm_b.requires_grad))
         # Switch devices only when needed (the context manager costs host time).
         switch = flat.device.index != torch._C._cuda_getDevice()
         with torch.cuda.device(flat.device) if switch else contextlib.nullcontext():
-            if needs_grad and fused_norm:
+            if needs_grad and layer_norm:
+                y, idx64, w, counts = _LayerNormMoEResidualFunction.apply(meta, eps, flat, norm_w, norm_b, gw, gb,
+                                                                          *weights)
+            elif needs_grad and fused_norm:
                 y, idx64, w, counts = _NormMoEResidualFunction.apply(meta, eps, flat, norm_w, gw, gb, *weights)
             elif needs_grad:
                 y, idx64, w, counts = _MoEBlockFunction.apply(meta, flat, gw, gb, *weights)
@@ -638,7 +692,12 @@ class DeepSeekMoE(nn.Module):
                 x_in, residual = flat, None
                 if fused_norm:
                     residual = flat.contiguous()
-                    x_in, _ = K.rmsnorm_fwd(residual, None if norm_w is None else norm_w.contiguous(), eps)
+                    nw = None if norm_w is None else norm_w.contiguous()
+                    if layer_norm:
+                        nb = None if norm_b is None else norm_b.contiguous()
+                        x_in = K.layer_norm_fwd(residual, nw, nb, eps, torch.bfloat16, stats=False)[0]
+                    else:
+                        x_in, _ = K.rmsnorm_fwd(residual, nw, eps)
                 fw = _forward_pass(meta, x_in, gw, gb, weights, residual)
                 idx64, w, counts, y = fw[4], fw[5], fw[7], fw[-1]
         # plain attributes (not parameters, buffers or submodules)
@@ -717,8 +776,8 @@ class DeepSeekMoE(nn.Module):
 def moe_residual(x: torch.Tensor, norm: nn.Module, moe: nn.Module) -> torch.Tensor:
     """``x + moe(norm(x))``, the FFN half of FusionLLMBlock.forward
     (models/fusionllm.py:52).  A fusionllm_amd ``DeepSeekMoE`` after an
-    ``nn.RMSNorm`` runs fused (norm, MoE and residual add in the kernels);
-    any other pair runs as the plain expression."""
-    if isinstance(moe, DeepSeekMoE) and isinstance(norm, nn.RMSNorm) and x.is_cuda:
+    ``nn.RMSNorm`` or a fusionllm_amd ``LayerNorm`` runs fused (norm, MoE and
+    residual add in the kernels); any other pair runs as the plain expression."""
+    if isinstance(moe, DeepSeekMoE) and isinstance(norm, (nn.RMSNorm, LayerNorm)) and x.is_cuda:
         return moe.forward_norm_residual(x, norm)
     return x + moe(norm(x))

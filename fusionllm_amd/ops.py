@@ -23,6 +23,10 @@ moe_bwd returns [dx, d_gate_w, d_gate_b, *d_weights] in the inputs' dtypes.
 (models/moe.py:11-21 used alone, the DenseFFN of models/fusionllm.py:17-27):
 outputs y [T,d] bf16, ab [T,2I] bf16, h [T,I] bf16; gradients [dx, dw1,
 dw3, dw2] in the inputs' dtypes.
+
+``fusionllm::layer_norm_fwd`` / ``layer_norm_bwd`` do the same for ``layer_norm``:
+outputs y [T,d] (out_dtype), mean [T] and rstd [T] fp32; gradients [dx, dw, db],
+without those of a weight or bias that is not there.
 """
 from __future__ import annotations
 
@@ -32,6 +36,7 @@ import torch
 from torch import Tensor
 
 from . import _kernels as K
+from . import norm as _norm
 from .moe import _backward_pass, _bf16_operands, _dense_backward, _dense_offsets, _forward_pass, gathers_rows
 
 
@@ -156,3 +161,47 @@ def _swiglu_backward(ctx, dy, *unused):
 
 
 swiglu_fwd.register_autograd(_swiglu_backward, setup_context=_swiglu_setup)
+
+
+@torch.library.custom_op("fusionllm::layer_norm_fwd", mutates_args=())
+def layer_norm_fwd(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                   out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    return _norm._forward(x, weight, bias, eps, out_dtype, True)[2:]
+
+
+@layer_norm_fwd.register_fake
+def _(x, weight, bias, eps, out_dtype):
+    T = x.shape[0]
+    return (x.new_empty(x.shape, dtype=out_dtype), x.new_empty((T,), dtype=torch.float32),
+            x.new_empty((T,), dtype=torch.float32))
+
+
+@torch.library.custom_op("fusionllm::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, weight: Tensor | None,
+                   bias: Tensor | None) -> list[Tensor]:
+    grads = _norm._backward(dy, _norm._rows(x), None if weight is None else weight.contiguous(), mean, rstd, None, True,
+                            None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+    return [g for g in grads if g is not None]
+
+
+@layer_norm_bwd.register_fake
+def _(dy, x, mean, rstd, weight, bias):
+    return [x.new_empty(x.shape), *[p.new_empty(p.shape) for p in (weight, bias) if p is not None]]
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, eps, out_dtype = inputs
+    y, mean, rstd = output
+    ctx.save_for_backward(x, weight, bias, mean, rstd)
+
+
+def _layer_norm_backward(ctx, dy, *unused):
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    if dy is None:
+        return None, None, None, None, None
+    grads = iter(torch.ops.fusionllm.layer_norm_bwd(dy, x, mean, rstd, weight, bias))
+    dx = next(grads)
+    return (dx, None if weight is None else next(grads), None if bias is None else next(grads), None, None)
+
+
+layer_norm_fwd.register_autograd(_layer_norm_backward, setup_context=_layer_norm_setup)

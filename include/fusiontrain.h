@@ -1,0 +1,58 @@
+/*
+ * fusiontrain.h — C ABI of libfusionmoe.so, continued: the training operators
+ * around the feed-forward block that fusionmoe.h does not declare (layer norm
+ * with its backward pass).
+ *
+ * The conventions, status codes and dtype codes are those of fusionmoe.h:
+ * borrowed device pointers, asynchronous on `stream`, no allocation, no
+ * synchronisation, a status instead of an exception.
+ */
+#ifndef FUSIONTRAIN_H
+#define FUSIONTRAIN_H
+
+#include "fusionmoe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FMOE_LAYER_NORM_MAX_DIM 16384
+
+/* ---------------------------------------------------------------------------
+ * Layer norm of the rows of x [T, dim] (dim <= FMOE_LAYER_NORM_MAX_DIM):
+ *   mean[t] = sum_c x[t,c] / dim
+ *   rstd[t] = 1 / sqrt(sum_c (x[t,c] - mean[t])^2 / dim + eps)
+ *   y[t,c]  = ((x[t,c] - mean[t]) * rstd[t]) * weight[c] + bias[c]
+ * fp32 arithmetic, the sums over a row in a fixed order; y is rounded once, to
+ * y_dtype.  Row t of x starts at x + t * ldx (elements, ldx >= dim unless T <=
+ * 1); y is dense.  weight and bias: [dim] of w_dtype, either may be NULL (1, 0).
+ * mean and rstd [T] fp32 are kept for the backward pass; both may be NULL.
+ * Pointers need the alignment of their element type only.
+ * ------------------------------------------------------------------------- */
+int fmoe_layer_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* weight,
+                        const void* bias, int w_dtype, int64_t T, int64_t dim, float eps,
+                        void* y, int y_dtype, float* mean, float* rstd, void* stream);
+
+/* Workspace of fmoe_layer_norm_bwd when d_weight or d_bias is wanted: two fp32
+ * rows of dim for every workgroup of its launch. */
+size_t fmoe_layer_norm_bwd_workspace_bytes(int64_t T, int64_t dim);
+
+/* Backward of the layer norm, with g = dy * weight and xh = (x - mean) * rstd:
+ *   dx = rstd * (g - sum_c(g) / dim - xh * sum_c(g * xh) / dim) + d_residual
+ *   d_weight[c] = sum_t dy[t,c] * xh[t,c],   d_bias[c] = sum_t dy[t,c]
+ * x, d_residual ([T, dim] dense, or NULL: the gradient that reaches x past the
+ * norm) and dx (dense) have x_dtype, dy dy_dtype, weight, d_weight and d_bias
+ * w_dtype.  dx, d_weight and d_bias may each be NULL (not wanted).  The sums
+ * over the rows run in a fixed order (no atomics): fp32 per workgroup, then
+ * over the workgroups.  No output may overlap an input. */
+int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* x, int x_dtype,
+                        int64_t ldx, const float* mean, const float* rstd, const void* weight,
+                        int w_dtype, const void* d_residual, int64_t T, int64_t dim, void* dx,
+                        void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* FUSIONTRAIN_H */
