@@ -618,6 +618,67 @@ def normuon_step(params, grads, exp_avgs, exp_avg_sqs, lr: float, beta1: float, 
           "fmoe_normuon_step")
 
 
+MUON_MAX_TENSORS = 64
+MUON_MAX_SIDE = 65536
+MUON_MAX_ELEMENTS = 1 << 30  # of a matrix whose sides are rounded up to multiples of 64
+MUON_MAX_STEPS = 64
+
+
+def _matrices(groups, names):
+    """Addresses, row and column counts of lists of equally shaped matrices (one list per name), all of
+    one dtype and device, with one pair of sides."""
+    first = groups[0][0]
+    n = len(groups[0])
+    if n > MUON_MAX_TENSORS:
+        raise RuntimeError(f"at most {MUON_MAX_TENSORS} matrices per launch (got {n})")
+    for ts, name in zip(groups, names):
+        if len(ts) != n:
+            raise RuntimeError(f"one {name} per matrix is needed (got {len(ts)} for {n})")
+        for t, like in zip(ts, groups[0]):
+            _req(t, name, first.dtype)
+            if t.device != first.device:
+                raise RuntimeError("all matrices must be on one device")
+            if t.dim() != 2 or t.shape != like.shape:
+                raise RuntimeError(f"{name} must be a matrix of shape {tuple(like.shape)} (got {tuple(t.shape)})")
+    rows = (ctypes.c_int64 * n)(*[t.shape[0] for t in groups[0]])
+    cols = (ctypes.c_int64 * n)(*[t.shape[1] for t in groups[0]])
+    return [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in groups], rows, cols
+
+
+def _muon_workspace(lib, like, n):
+    nbytes = lib.fmoe_orthogonalize_workspace_bytes(like.shape[0], like.shape[1], n, _dtype_code(like.dtype))
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=like.device)
+    return ws, nbytes
+
+
+@_timed
+def orthogonalize(mats, outs, steps: int, coefficients, eps: float):
+    """Newton-Schulz orthogonalisation of up to 64 matrices (one dtype, one pair of sides) into outs."""
+    lib = _lib.load()
+    if not mats:
+        return
+    (src, dst), rows, cols = _matrices((mats, outs), ("matrix", "output"))
+    ws, nbytes = _muon_workspace(lib, mats[0], len(mats))
+    check(lib.fmoe_orthogonalize(src, dst, rows, cols, len(mats), _dtype_code(mats[0].dtype), int(steps),
+                                 (ctypes.c_double * 3)(*coefficients), float(eps), ws.data_ptr(), nbytes, _stream()),
+          "fmoe_orthogonalize")
+
+
+@_timed
+def muon_step(params, grads, bufs, lr_tall: float, lr_wide: float, decay: float, momentum: float, nesterov: bool,
+              steps: int, coefficients, eps: float):
+    """One Muon update of up to 64 matrices (one dtype, one pair of sides), in place."""
+    lib = _lib.load()
+    if not params:
+        return
+    (p, g, b), rows, cols = _matrices((params, grads, bufs), ("param", "grad", "momentum buffer"))
+    ws, nbytes = _muon_workspace(lib, params[0], len(params))
+    check(lib.fmoe_muon_step(p, g, b, rows, cols, len(params), _dtype_code(params[0].dtype), float(lr_tall),
+                             float(lr_wide), float(decay), float(momentum), int(bool(nesterov)), int(steps),
+                             (ctypes.c_double * 3)(*coefficients), float(eps), ws.data_ptr(), nbytes, _stream()),
+          "fmoe_muon_step")
+
+
 CAST_MAX_TENSORS = 64
 
 

@@ -79,6 +79,11 @@ TRAIN_SIGNATURES = {
     "fmoe_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "fmoe_layer_norm_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, _P, _P, c_int, _P, c_int64, c_int64,
                                     _P, _P, _P, _P, c_size_t, _P]),
+    "fmoe_orthogonalize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
+    "fmoe_orthogonalize": (c_int, [_PP, _PP, POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_int,
+                                   POINTER(c_double), c_double, _P, c_size_t, _P]),
+    "fmoe_muon_step": (c_int, [_PP, _PP, _PP, POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_double, c_double,
+                               c_double, c_double, c_int, c_int, POINTER(c_double), c_double, _P, c_size_t, _P]),
 }
 
 _lock = threading.Lock()

@@ -17,6 +17,9 @@ extern "C" const char* fmoe_status_string(int status) {
       return "workload larger than the static scratch of the allocation-free entry point "
              "(fmoe_dispatch_noalloc: fmoe_dispatch_workspace_bytes(T, E, k) must be <= 1 MiB); "
              "use fmoe_dispatch with a workspace";
+    case FMOE_ERR_COEFFICIENTS:
+      return "Newton-Schulz coefficients whose iterates leave the stored range "
+             "(singular values must stay below 2.8 and |b t + c t^2| below 7.9)";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,543 @@
+// newton_schulz.hip — orthogonalised updates of weight matrices by Newton-Schulz
+// products, many matrices of one size at once, and the Muon step around them.
+//
+// For a matrix G (its smaller side first: m x n, m <= n, so a tall matrix is
+// taken transposed):
+//   X = G / max(|G|_F, eps);  steps times:  A = X X^T,  B = b A + c A^2,  X = a X + B X
+// (an odd polynomial of G's singular values, with its singular vectors kept).
+// Muon: u = momentum's combination of the gradient, p = p (1 - lr wd) - lr' X(u).
+//
+// Arithmetic.  The products run on v_mfma_f32_16x16x32_f16: fp16 carries 11 bits
+// where bf16 carries 8 at the same rate, and the iterates' range is known: singular
+// values of X stay below a bound that the host computes from the coefficients,
+// so X, A and B are stored with the power-of-two factors below and neither
+// overflow nor leave the normal range early.  Sums are fp32 throughout.  X is kept
+// as two fp16 numbers (hi + lo, 22 bits) and a X is formed from both: small
+// singular values are carried by that term (times a per step, some hundredfold
+// over five steps), and what a rounding of X adds to it would grow with them.
+// Rounding X in the other products only acts within the row space that X
+// spans already.  Relative error of the result on gradients of full and low rank
+// (768 x 2048, simulated in 64 bits): bf16 products 1e-2 .. 1.6e-1, fp16 without
+// lo 1.3e-3 .. 1.9e-2, this form 3e-4 .. 1.5e-3 (half a step of a bf16 result: 3.9e-3).
+// fp32 matrices take every operand as hi + lo (three products: hi hi, hi lo, lo hi;
+// relative error 2e-6), and so do matrices of a small side up to kSplitSmall, whose
+// few rounding errors average out less and whose products cost nothing next to
+// the launches.
+//
+// A and B are symmetric: only the tiles on and below the diagonal are computed
+// and stored twice.  3 m^2 n + m^3 flops a step, bound by the matrix units; a
+// few matrices are bound by the launches (3 per step and 2 before them).
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/fusiontrain.h"
+#include "fmoe_common.h"
+#include "gemm_core.h"
+
+namespace fmoe {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
+constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
+constexpr int64_t kSplitSmall = 128;
+constexpr int kNormParts_ = 64;     // partial sums of squares per matrix, at most
+constexpr int kNormChunk = 8192;    // elements per partial sum, at least
+// Stored values: X 2^14, A 2^13, B 2^13 (singular values of X below 2.8, |B| below 7.9).
+constexpr float kXScale = 16384.0f, kAScale = 8192.0f;
+constexpr double kMaxSigma = 2.8, kMaxPoly = 7.9;
+
+struct NsArgs {
+  const void* src[kNsMax];  // matrix, or gradient
+  void* buf[kNsMax];        // momentum (Muon)
+  void* dst[kNsMax];        // result, or parameter (Muon)
+  uint64_t tall;            // bit i: matrix i has more rows than columns
+  int count, dtype, muon, nesterov;
+  int m, n, mp, np;         // sides (m <= n) and padded sides
+  int parts;                // partial sums per matrix
+  float mom, om;            // momentum, 1 - momentum
+  float decay;              // 1 - lr * weight_decay
+  float lr_tall, lr_wide;   // step sizes with their size adjustment
+  double eps;
+  float ca, cb, cc;         // the polynomial's coefficients
+  double* norm;             // [count][parts]
+  // fp16, hi and lo: X [count][mp][np] twice (the step reads one and writes the other; lo of
+  // the second only where the products take it), A and B [count][mp][mp]
+  _Float16 *xh[2], *xl[2], *ah, *al, *bh, *bl;
+};
+
+// ---- the source: elements and the value that is orthogonalised ---------------------
+
+__device__ __forceinline__ float ns_elem(const void* p, int dtype, int64_t e) {
+  return dtype == FMOE_BF16 ? bf2f(static_cast<const uint16_t*>(p)[e]) : static_cast<const float*>(p)[e];
+}
+__device__ __forceinline__ void ns_put(void* p, int dtype, int64_t e, float v) {
+  if (dtype == FMOE_BF16) static_cast<uint16_t*>(p)[e] = f2bf(v);
+  else static_cast<float*>(p)[e] = v;
+}
+// Muon: the momentum after this step, from the one before it (fp32, not yet rounded to its type).
+__device__ __forceinline__ float ns_momentum(const NsArgs& a, float g, float buf) { return fmaf(a.mom, buf, a.om * g); }
+__device__ __forceinline__ float ns_update(const NsArgs& a, float g, float newbuf) {
+  return a.nesterov ? fmaf(a.mom, newbuf, a.om * g) : newbuf;
+}
+
+// Sum of squares of each matrix in fp64 (no overflow of large values, no loss over
+// millions of terms): one partial sum per workgroup, in a fixed order.
+__global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
+  __shared__ double red[4];
+  const int mat = blockIdx.y, part = blockIdx.x;
+  const int64_t total = static_cast<int64_t>(a.m) * a.n;
+  const void* g = a.src[mat];
+  const void* b = a.buf[mat];
+  double s = 0.0;
+  for (int64_t e = part * 256 + threadIdx.x; e < total; e += static_cast<int64_t>(a.parts) * 256) {
+    float u = ns_elem(g, a.dtype, e);
+    if (a.muon) u = ns_update(a, u, ns_momentum(a, u, ns_elem(b, a.dtype, e)));
+    s += static_cast<double>(u) * static_cast<double>(u);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) s = s + __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) a.norm[mat * a.parts + part] = ((red[0] + red[1]) + red[2]) + red[3];
+}
+
+// X = u / max(|u|, eps) as hi + lo, its smaller side first, zeros in the padding; Muon: the
+// new momentum.  One 64 x 64 tile of X per workgroup, through LDS (tall matrices arrive transposed).
+__global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
+  __shared__ float tile[64][65];
+  const int mat = blockIdx.z;
+  const bool tall = (a.tall >> mat) & 1;
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;  // of X
+  const int rows = tall ? a.n : a.m, cols = tall ? a.m : a.n;  // of the matrix as it lies
+  const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
+  double ss = 0.0;
+  for (int p = 0; p < a.parts; ++p) ss += a.norm[mat * a.parts + p];
+  // NaN (of a matrix that holds NaN or infinities) stays NaN
+  const double nrm = sqrt(ss);
+  const double scale = static_cast<double>(kXScale) / (nrm < a.eps ? a.eps : nrm);
+  const void* g = a.src[mat];
+  void* b = a.buf[mat];
+  const int c = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = (threadIdx.x >> 6) + 4 * k;
+    float v = 0.0f;
+    if (r0 + r < rows && c0 + c < cols) {
+      const int64_t e = static_cast<int64_t>(r0 + r) * cols + c0 + c;
+      float u = ns_elem(g, a.dtype, e);
+      if (a.muon) {
+        const float nb = ns_momentum(a, u, ns_elem(b, a.dtype, e));
+        ns_put(b, a.dtype, e, nb);
+        u = ns_update(a, u, nb);
+      }
+      v = static_cast<float>(static_cast<double>(u) * scale);
+    }
+    if (tall) tile[c][r] = v;
+    else tile[r][c] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = (threadIdx.x >> 3) + 32 * k, q = (threadIdx.x & 7) * 8;
+    half8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = tile[r][q + e];
+      h[e] = static_cast<_Float16>(v);
+      l[e] = static_cast<_Float16>(v - static_cast<float>(h[e]));
+    }
+    const int64_t o = (static_cast<int64_t>(mat) * a.mp + i0 + r) * a.np + j0 + q;
+    *reinterpret_cast<half8*>(a.xh[0] + o) = h;
+    *reinterpret_cast<half8*>(a.xl[0] + o) = l;
+  }
+}
+
+// ---- the products ------------------------------------------------------------------------
+
+enum NsMode { NS_GRAM = 0, NS_POLY = 1, NS_STEP = 2, NS_LAST = 3 };
+
+// Tile (row, column) of a symmetric product's t-th tile on or below the diagonal, row major.
+__device__ __forceinline__ void triangle(int t, int& i, int& j) {
+  i = static_cast<int>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+  while (i * (i + 1) / 2 > t) --i;
+  while ((i + 1) * (i + 2) / 2 <= t) ++i;
+  j = t - i * (i + 1) / 2;
+}
+
+// TM x TN outputs per workgroup of four waves (2 x 2), K in steps of 64 through two LDS stages:
+// the copies of the next stage (global -> LDS, no registers) run while this one is multiplied.
+// The row operand, and the column operand of the symmetric products, are K-contiguous;
+// the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
+// (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
+template <int MODE, int TM, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
+  using namespace core;
+  constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+  constexpr int TN = SYM ? TM : 128;
+  constexpr int WTM = TM / 2, WTN = TN / 2, FM = WTM / 16, FN = WTN / 16;
+  constexpr int A_ST = TM * RB, STAGE = A_ST + TN * RB;
+  constexpr int CA = TM / 32, CB = TN / 32;  // copies per wave and stage
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = w >> 1, wn = w & 1;
+  const uint32_t sbase = lds_addr(smem);
+
+  // Workgroup b runs on XCD b % 8: each takes a contiguous run of tiles.
+  const int tm_n = (a.mp + TM - 1) / TM, tn_n = SYM ? tm_n : (a.np + TN - 1) / TN;
+  const int per = SYM ? tm_n * (tm_n + 1) / 2 : tm_n * tn_n;
+  const int total = per * a.count, run = (total + 7) / 8;
+  const int item = (static_cast<int>(blockIdx.x) % 8) * run + static_cast<int>(blockIdx.x) / 8;
+  if (static_cast<int>(blockIdx.x) / 8 >= run || item >= total) return;
+  const int mat = __builtin_amdgcn_readfirstlane(item / per), t = item - mat * per;
+  int ti, tj;
+  if constexpr (SYM) triangle(t, ti, tj);
+  else ti = t / tn_n, tj = t - ti * tn_n;
+  ti = __builtin_amdgcn_readfirstlane(ti);
+  tj = __builtin_amdgcn_readfirstlane(tj);
+
+  const int K = MODE == NS_GRAM ? a.np : a.mp;
+  const int lda = K, ldb = SYM ? K : a.np;
+  const int nk = K / BK, steps = nk * (SPLIT ? 3 : 1);
+  const int64_t msq = static_cast<int64_t>(mat) * a.mp * a.mp, mx = static_cast<int64_t>(mat) * a.mp * a.np;
+  const _Float16* ph = MODE == NS_GRAM ? a.xh[cur] + mx : MODE == NS_POLY ? a.ah + msq : a.bh + msq;
+  const _Float16* pl = MODE == NS_GRAM ? a.xl[cur] + mx : MODE == NS_POLY ? a.al + msq : a.bl + msq;
+  const _Float16* qh = SYM ? ph : a.xh[cur] + mx;
+  const _Float16* ql = SYM ? pl : a.xl[cur] + mx;
+
+  // this lane's byte offsets from the operands' bases (rows and columns past the padded end: the last)
+  uint32_t aoff[CA], boff[CB];
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 8;
+#pragma unroll
+  for (int q = 0; q < CA; ++q)
+    aoff[q] = static_cast<uint32_t>(min(ti * TM + 8 * (w + 4 * q) + (lane >> 3), a.mp - 1) * lda + chunk) * 2u;
+#pragma unroll
+  for (int q = 0; q < CB; ++q) {
+    if constexpr (SYM) {
+      boff[q] = static_cast<uint32_t>(min(tj * TN + 8 * (w + 4 * q) + (lane >> 3), a.mp - 1) * ldb + chunk) * 2u;
+    } else {
+      const int krow = 4 * (w + 4 * q) + (lane >> 4);
+      const int cb = ((((lane & 15) >> 1) ^ wsw(krow)) << 1) | (lane & 1);
+      boff[q] = static_cast<uint32_t>(krow * ldb + min(tj * TN + 8 * cb, a.np - 8)) * 2u;
+    }
+  }
+  // SPLIT: hi lo, lo hi, then hi hi, so that the small terms are summed while the sum is small
+  const uint8_t *pa = reinterpret_cast<const uint8_t*>(ph), *pb = reinterpret_cast<const uint8_t*>(SPLIT ? ql : qh);
+  const int64_t bstep = SYM ? RB : static_cast<int64_t>(BK) * ldb * 2;
+  int kt = 0, seg = 0;
+  auto issue = [&](int st) __attribute__((always_inline)) {
+    const uint32_t la = sbase + st * STAGE + w * 1024, lb = la + A_ST;
+#pragma unroll
+    for (int q = 0; q < CA; ++q) copy16(la + q * 4096, pa, aoff[q]);
+#pragma unroll
+    for (int q = 0; q < CB; ++q) copy16(lb + q * 4096, pb, boff[q]);
+    pa += RB;
+    pb += bstep;
+    if (SPLIT && ++kt == nk) {
+      kt = 0;
+      ++seg;
+      pa = reinterpret_cast<const uint8_t*>(seg == 1 ? pl : ph);
+      pb = reinterpret_cast<const uint8_t*>(qh);
+    }
+  };
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t xa = frag_base(wm * WTM, lane);
+  const uint32_t xb = A_ST + (SYM ? frag_base(wn * WTN, lane) : tr_base(4 * wn, lane));
+  typedef __attribute__((address_space(3))) half8 lds_half8;
+  issue(0);
+  for (int it = 0; it < steps; ++it) {
+    wait_vm_barrier<0>();  // this stage is there, and every wave is done with the other
+    if (it + 1 < steps) issue((it + 1) & 1);
+    const uint32_t src = sbase + (it & 1) * STAGE;
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      half8 fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        if constexpr (SYM) fb[j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
+        else fb[j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+    }
+  }
+
+  // acc[i][j] of this lane: row 16 i + l % 16, columns 16 j + 4 (l / 16) + 0..3 of the wave's block.
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int r = ti * TM + wm * WTM + 16 * i + (lane & 15);
+    if (r >= a.mp) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int c = tj * TN + wn * WTN + 16 * j + 4 * (lane >> 4);
+      if (c >= (SYM ? a.mp : a.np)) continue;
+      float v[4];
+      if constexpr (SYM) {
+        const int64_t o = msq + static_cast<int64_t>(r) * a.mp + c;
+        if constexpr (MODE == NS_GRAM) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (kAScale / (kXScale * kXScale));
+        } else {
+          const half4 h = *reinterpret_cast<const half4*>(a.ah + o);
+          half4 l = {0, 0, 0, 0};
+          if constexpr (SPLIT) l = *reinterpret_cast<const half4*>(a.al + o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (acc[i][j][e] / kAScale));
+        }
+        _Float16* oh = MODE == NS_GRAM ? a.ah : a.bh;
+        _Float16* ol = MODE == NS_GRAM ? a.al : a.bl;
+        half4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[e] = static_cast<_Float16>(v[e]);
+          l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+        }
+        *reinterpret_cast<half4*>(oh + o) = h;
+        if constexpr (SPLIT) *reinterpret_cast<half4*>(ol + o) = l;
+        if (ti != tj) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t ot = msq + static_cast<int64_t>(c + e) * a.mp + r;
+            oh[ot] = h[e];
+            if constexpr (SPLIT) ol[ot] = l[e];
+          }
+        }
+      } else {
+        const int64_t o = mx + static_cast<int64_t>(r) * a.np + c;
+        const half4 xh = *reinterpret_cast<const half4*>(a.xh[cur] + o);
+        const half4 xl = *reinterpret_cast<const half4*>(a.xl[cur] + o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = fmaf(a.ca, static_cast<float>(xh[e]) + static_cast<float>(xl[e]), acc[i][j][e] / kAScale);
+        if constexpr (MODE == NS_STEP) {
+          half4 h, l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[e] = static_cast<_Float16>(v[e]);
+            l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+          }
+          *reinterpret_cast<half4*>(a.xh[1 - cur] + o) = h;
+          *reinterpret_cast<half4*>(a.xl[1 - cur] + o) = l;
+        } else {
+          const bool tall = (a.tall >> mat) & 1;
+          if (r >= a.m) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (c + e >= a.n) continue;
+            const int64_t q = tall ? static_cast<int64_t>(c + e) * a.m + r : static_cast<int64_t>(r) * a.n + c + e;
+            float out = v[e] * (1.0f / kXScale);
+            if (a.muon) out = fmaf(tall ? -a.lr_tall : -a.lr_wide, out, ns_elem(a.dst[mat], a.dtype, q) * a.decay);
+            ns_put(a.dst[mat], a.dtype, q, out);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+inline int64_t ns_pad(int64_t v) { return ceil_div(v, kNsPad) * kNsPad; }
+inline bool ns_split(int64_t m, int dtype) { return dtype == FMOE_F32 || m <= kSplitSmall; }
+
+struct NsLayout {
+  size_t norm, x, sq, total;  // bytes of the partial sums, of one X, of one A
+  int parts;
+};
+inline NsLayout ns_layout(int64_t m, int64_t n, int count, bool split) {
+  NsLayout l;
+  l.parts = static_cast<int>(std::min<int64_t>(kNormParts_, ceil_div(m * n, kNormChunk)));
+  l.norm = (static_cast<size_t>(count) * l.parts * sizeof(double) + 255) / 256 * 256;
+  l.x = static_cast<size_t>(count) * ns_pad(m) * ns_pad(n) * 2;
+  l.sq = static_cast<size_t>(count) * ns_pad(m) * ns_pad(m) * 2;
+  l.total = l.norm + 4 * l.x + (split ? 4 : 2) * l.sq;
+  return l;
+}
+
+// Whether the iterates stay within the stored range: the largest singular value after each
+// step, from the polynomial's extrema over [0, s], and the largest |b t + c t^2| over t <= s^2.
+inline bool ns_bounded(double a, double b, double c, int steps) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  double s = 1.0 + 1e-6;
+  for (int k = 0; k < steps; ++k) {
+    if (!(s < kMaxSigma)) return false;
+    const double t1 = s * s;
+    double poly = std::fabs(b * t1 + c * t1 * t1);
+    if (c != 0.0) {
+      const double t = -b / (2.0 * c);
+      if (t > 0.0 && t < t1) poly = std::max(poly, std::fabs(b * t + c * t * t));
+    }
+    if (!(poly < kMaxPoly)) return false;
+    auto p = [&](double v) { return std::fabs(v * (a + v * v * (b + c * v * v))); };
+    double next = p(s);
+    // extrema: 5 c t^2 + 3 b t + a = 0, t = v^2
+    double roots[2];
+    int n = 0;
+    if (c != 0.0) {
+      const double d = 9.0 * b * b - 20.0 * a * c;
+      if (d >= 0.0) {
+        roots[n++] = (-3.0 * b + std::sqrt(d)) / (10.0 * c);
+        roots[n++] = (-3.0 * b - std::sqrt(d)) / (10.0 * c);
+      }
+    } else if (b != 0.0) {
+      roots[n++] = -a / (3.0 * b);
+    }
+    for (int i = 0; i < n; ++i)
+      if (roots[i] > 0.0 && roots[i] < t1) next = std::max(next, p(std::sqrt(roots[i])));
+    s = next * (1.0 + 1e-3);  // room for the roundings
+  }
+  return s < kMaxSigma;
+}
+
+template <int MODE>
+inline void ns_product(const NsArgs& a, int cur, bool split, hipStream_t s) {
+  constexpr bool sym = MODE == NS_GRAM || MODE == NS_POLY;
+  auto tiles = [&](int tm) {
+    const int64_t r = ceil_div(a.mp, tm);
+    return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, 128)) * a.count;
+  };
+  const bool big = tiles(128) >= 256;
+  const dim3 grid(static_cast<unsigned>(8 * ceil_div(tiles(big ? 128 : 64), 8))), block(256);
+  if (big) {
+    if (split) ns_product_kernel<MODE, 128, true><<<grid, block, 0, s>>>(a, cur);
+    else ns_product_kernel<MODE, 128, false><<<grid, block, 0, s>>>(a, cur);
+  } else {
+    if (split) ns_product_kernel<MODE, 64, true><<<grid, block, 0, s>>>(a, cur);
+    else ns_product_kernel<MODE, 64, false><<<grid, block, 0, s>>>(a, cur);
+  }
+}
+
+// Sizes of a call, checked: sets m, n and the tall bits.
+inline int ns_sizes(const int64_t* rows, const int64_t* cols, int count, NsArgs& a) {
+  for (int i = 0; i < count; ++i) {
+    if (rows[i] <= 0 || cols[i] <= 0) return FMOE_ERR_INVALID_ARG;
+    const int64_t m = std::min(rows[i], cols[i]), n = std::max(rows[i], cols[i]);
+    if (n > FMOE_MUON_MAX_SIDE || (i > 0 && (m != a.m || n != a.n))) return FMOE_ERR_SHAPE;
+    a.m = static_cast<int>(m);
+    a.n = static_cast<int>(n);
+    if (rows[i] > cols[i]) a.tall |= uint64_t(1) << i;
+  }
+  a.mp = static_cast<int>(ns_pad(a.m));
+  a.np = static_cast<int>(ns_pad(a.n));
+  // 32-bit byte offsets within a matrix
+  return static_cast<int64_t>(a.mp) * a.np <= FMOE_MUON_MAX_ELEMENTS ? FMOE_OK : FMOE_ERR_SHAPE;
+}
+
+inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* workspace, size_t workspace_bytes,
+                  hipStream_t s) {
+  const bool split = ns_split(a.m, a.dtype);
+  const NsLayout l = ns_layout(a.m, a.n, a.count, split);
+  if (!workspace || workspace_bytes < l.total) return FMOE_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return FMOE_ERR_ALIGN;
+  a.ca = static_cast<float>(coeffs[0]);
+  a.cb = static_cast<float>(coeffs[1]);
+  a.cc = static_cast<float>(coeffs[2]);
+  a.eps = eps;
+  a.parts = l.parts;
+  uint8_t* p = static_cast<uint8_t*>(workspace);
+  a.norm = reinterpret_cast<double*>(p);
+  p += l.norm;
+  auto take = [&](size_t n) {
+    _Float16* q = reinterpret_cast<_Float16*>(p);
+    p += n;
+    return q;
+  };
+  for (int i = 0; i < 2; ++i) a.xh[i] = take(l.x);
+  for (int i = 0; i < 2; ++i) a.xl[i] = take(l.x);
+  a.ah = take(l.sq);
+  a.bh = take(l.sq);
+  if (split) a.al = take(l.sq), a.bl = take(l.sq);
+  ns_norm_kernel<<<dim3(a.parts, a.count), dim3(256), 0, s>>>(a);
+  ns_load_kernel<<<dim3(a.np / 64, a.mp / 64, a.count), dim3(256), 0, s>>>(a);
+  for (int k = 0; k < steps; ++k) {
+    ns_product<NS_GRAM>(a, k & 1, split, s);
+    ns_product<NS_POLY>(a, k & 1, split, s);
+    if (k + 1 < steps) ns_product<NS_STEP>(a, k & 1, split, s);
+    else ns_product<NS_LAST>(a, k & 1, split, s);
+  }
+  return launch_status();
+}
+
+inline bool ns_elem_aligned(const void* p, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == FMOE_BF16 ? 1u : 3u)) == 0;
+}
+
+}  // namespace fmoe
+
+using namespace fmoe;
+
+extern "C" size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype) {
+  if (rows <= 0 || cols <= 0 || rows > FMOE_MUON_MAX_SIDE || cols > FMOE_MUON_MAX_SIDE || n_tensors <= 0 ||
+      n_tensors > kNsMax)
+    return 0;
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  if (ns_pad(m) * ns_pad(n) > FMOE_MUON_MAX_ELEMENTS) return 0;
+  return ns_layout(m, n, n_tensors, ns_split(m, dtype)).total;
+}
+
+extern "C" int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows, const int64_t* cols,
+                                  int n_tensors, int dtype, int steps, const double* coeffs, double eps,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (n_tensors < 0 || n_tensors > kNsMax || steps < 1 || steps > FMOE_MUON_MAX_STEPS) return FMOE_ERR_INVALID_ARG;
+  if (dtype != FMOE_BF16 && dtype != FMOE_F32) return FMOE_ERR_DTYPE;
+  if (n_tensors == 0) return FMOE_OK;
+  if (!src || !dst || !rows || !cols || !coeffs || !(eps > 0.0)) return FMOE_ERR_INVALID_ARG;
+  if (!ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps)) return FMOE_ERR_COEFFICIENTS;
+  NsArgs a = {};
+  a.count = n_tensors;
+  a.dtype = dtype;
+  if (const int rc = ns_sizes(rows, cols, n_tensors, a)) return rc;
+  for (int i = 0; i < n_tensors; ++i) {
+    if (!src[i] || !dst[i]) return FMOE_ERR_INVALID_ARG;
+    if (!ns_elem_aligned(src[i], dtype) || !ns_elem_aligned(dst[i], dtype)) return FMOE_ERR_ALIGN;
+    a.src[i] = src[i];
+    a.dst[i] = dst[i];
+  }
+  return ns_run(a, steps, coeffs, eps, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int fmoe_muon_step(void* const* params, const void* const* grads, void* const* momentum_bufs,
+                              const int64_t* rows, const int64_t* cols, int n_tensors, int dtype, double lr_tall,
+                              double lr_wide, double decay, double momentum, int nesterov, int steps,
+                              const double* coeffs, double eps, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  if (n_tensors < 0 || n_tensors > kNsMax || steps < 1 || steps > FMOE_MUON_MAX_STEPS) return FMOE_ERR_INVALID_ARG;
+  if (dtype != FMOE_BF16 && dtype != FMOE_F32) return FMOE_ERR_DTYPE;
+  if (n_tensors == 0) return FMOE_OK;
+  if (!params || !grads || !momentum_bufs || !rows || !cols || !coeffs || !(eps > 0.0)) return FMOE_ERR_INVALID_ARG;
+  if (!ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps)) return FMOE_ERR_COEFFICIENTS;
+  NsArgs a = {};
+  a.count = n_tensors;
+  a.dtype = dtype;
+  a.muon = 1;
+  a.nesterov = nesterov != 0;
+  a.mom = static_cast<float>(momentum);
+  a.om = static_cast<float>(1.0 - momentum);
+  a.decay = static_cast<float>(decay);
+  a.lr_tall = static_cast<float>(lr_tall);
+  a.lr_wide = static_cast<float>(lr_wide);
+  if (const int rc = ns_sizes(rows, cols, n_tensors, a)) return rc;
+  for (int i = 0; i < n_tensors; ++i) {
+    if (!params[i] || !grads[i] || !momentum_bufs[i]) return FMOE_ERR_INVALID_ARG;
+    if (!ns_elem_aligned(params[i], dtype) || !ns_elem_aligned(grads[i], dtype) ||
+        !ns_elem_aligned(momentum_bufs[i], dtype))
+      return FMOE_ERR_ALIGN;
+    a.dst[i] = params[i];
+    a.src[i] = grads[i];
+    a.buf[i] = momentum_bufs[i];
+  }
+  return ns_run(a, steps, coeffs, eps, workspace, workspace_bytes, as_stream(stream));
+}

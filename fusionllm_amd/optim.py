@@ -1,6 +1,6 @@
-"""Drop-in NorMuon for the weight matrices (reference: training/optimizer.py:11-58).
+"""Optimizers of the weight matrices: NorMuon, Muon and the orthogonalisation it uses.
 
-Same constructor (params, lr, betas, eps, weight_decay, cautious_wd), the
+``NorMuon``: drop-in for the reference's (training/optimizer.py:11-58).  Same constructor (params, lr, betas, eps, weight_decay, cautious_wd), the
 same per-parameter state ("step", "exp_avg", "exp_avg_sq", so optimizer
 checkpoints (training/checkpoint.py:19-40) load either way) and the same
 update.  ``step()`` runs the update as fused kernels
@@ -10,8 +10,18 @@ updated tensors once, where the reference issues about fifteen tensor
 operations per parameter.  Parameters must be ROCm tensors in bf16 or fp32
 with a last dimension that is a multiple of 4 and at most 4096 (every weight
 matrix of the reference model); anything else raises.
+
+``orthogonalize`` replaces matrices by their orthogonalised form (an odd
+polynomial of the singular values, by Newton-Schulz products), every matrix of
+one pair of sides in the same launches.  ``Muon`` is momentum, that form of the
+update, decoupled weight decay and the parameter's update in the same launches,
+with the constructor and state of ``torch.optim.Muon``.  Matrices are bf16 or
+fp32; the products of bf16 matrices run on fp16 operands with fp32 sums, those of
+fp32 matrices on pairs of fp16 operands (22 bits).
 """
 from __future__ import annotations
+
+import math
 
 import torch
 from torch.optim import Optimizer
@@ -65,4 +75,160 @@ class NorMuon(Optimizer):
                         K.normuon_step([t[0] for t in chunk], [t[1] for t in chunk], [t[2] for t in chunk],
                                        [t[3] for t in chunk], lr, beta1, beta2, eps, wd, cautious,
                                        bias_corr1, bias_corr2)
+        return loss
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _launches(items, key, distinct):
+    """Lists of items for one launch each: the same key, at most MUON_MAX_TENSORS, and no two that
+    write the same storage (distinct(item): addresses); in order where they do."""
+    open_: dict = {}
+    out = []
+    for it in items:
+        k = key(it)
+        cur = open_.get(k)
+        addr = distinct(it)
+        if cur is None or len(cur[0]) == K.MUON_MAX_TENSORS or not cur[1].isdisjoint(addr):
+            cur = open_[k] = ([], set())
+            out.append(cur[0])
+        cur[0].append(it)
+        cur[1].update(addr)
+    return out
+
+
+def _sides(t):
+    r, c = t.shape
+    return (r, c) if r <= c else (c, r)
+
+
+def _check_ns(steps, coefficients, eps):
+    if len(coefficients) != 3:
+        raise ValueError(f"three coefficients are needed (got {len(coefficients)})")
+    if not 1 <= steps <= K.MUON_MAX_STEPS:
+        raise ValueError(f"the number of Newton-Schulz steps must be 1 to {K.MUON_MAX_STEPS} (got {steps})")
+    if not eps > 0:
+        raise ValueError(f"eps must be positive (got {eps})")
+
+
+def _check_matrix(what, t):
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs on a ROCm device only (got a {t.device.type} tensor)")
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise NotImplementedError(f"{what} supports bf16 and fp32 matrices (got {t.dtype})")
+    if max(t.shape[-2:]) > K.MUON_MAX_SIDE:
+        raise NotImplementedError(f"{what} takes sides up to {K.MUON_MAX_SIDE} (got {tuple(t.shape)})")
+    r, c = (-(-s // 64) * 64 for s in t.shape[-2:])
+    if r * c > K.MUON_MAX_ELEMENTS:
+        raise NotImplementedError(f"{what} takes matrices of up to {K.MUON_MAX_ELEMENTS} elements (got "
+                                  f"{tuple(t.shape)})")
+
+
+def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7):
+    """Orthogonalised matrices: X = G / max(|G|_F, eps), then ``steps`` times X = a X + (b A + c A^2) X
+    with A = X X^T, on the shorter side.
+
+    mats: a tensor [..., rows, cols] (every matrix of the stack), or a list of such tensors; the result
+    has the same structure, shapes and dtypes.  No backward pass.  The coefficients must keep the
+    singular values below 2.8 (the defaults do)."""
+    single = isinstance(mats, torch.Tensor)
+    stacks = [mats] if single else list(mats)
+    _check_ns(steps, coefficients, eps)
+    for t in stacks:
+        if t.dim() < 2:
+            raise ValueError(f"orthogonalize takes matrices (got shape {tuple(t.shape)})")
+        _check_matrix("orthogonalize", t)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("orthogonalize has no backward pass: call it under no_grad or on detached matrices")
+    outs, items = [], []
+    for t in stacks:
+        t = t.detach().contiguous()
+        out = torch.empty_like(t)
+        outs.append(out)
+        if t.numel():
+            items += zip(t.view(-1, *t.shape[-2:]), out.view(-1, *t.shape[-2:]))
+    for chunk in _launches(items, lambda it: (it[0].device, it[0].dtype, _sides(it[0])),
+                           lambda it: (it[1].data_ptr(),)):
+        with torch.cuda.device(chunk[0][0].device):
+            K.orthogonalize([c[0] for c in chunk], [c[1] for c in chunk], steps, coefficients, eps)
+    return outs[0] if single else outs
+
+
+class Muon(Optimizer):
+    """Muon: momentum, the update orthogonalised by Newton-Schulz products, decoupled weight decay.
+
+        buf = momentum buf + (1 - momentum) grad
+        u   = (1 - momentum) grad + momentum buf  if nesterov else buf
+        p   = p (1 - lr weight_decay) - lr' orthogonalize(u)
+
+    with lr' = lr sqrt(max(1, rows / cols)) (adjust_lr_fn None or "original") or
+    lr 0.2 sqrt(max(rows, cols)) ("match_rms_adamw").  The constructor and the
+    state ("momentum_buffer") are those of ``torch.optim.Muon``.  Parameters are
+    matrices on a ROCm device, bf16 or fp32, with gradients of their own dtype;
+    every matrix of one dtype and pair of sides is updated in the same launches."""
+
+    def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
+                 nesterov: bool = True, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
+                 adjust_lr_fn: str | None = None):
+        if lr < 0:
+            raise ValueError(f"the learning rate must not be negative (got {lr})")
+        if weight_decay < 0:
+            raise ValueError(f"the weight decay must not be negative (got {weight_decay})")
+        if not 0 <= momentum < 1:
+            raise ValueError(f"the momentum must be in [0, 1) (got {momentum})")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"unknown learning rate adjustment {adjust_lr_fn!r}")
+        _check_ns(ns_steps, ns_coefficients, eps)
+        defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                        ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps,
+                        adjust_lr_fn=adjust_lr_fn)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        ps = self.param_groups[-1]["params"]
+        try:
+            if len(set(ps)) != len(ps):
+                raise ValueError("a parameter is given twice")
+            for p in ps:
+                if p.dim() != 2:
+                    raise ValueError(f"Muon takes matrices (got a parameter of shape {tuple(p.shape)})")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            items = []
+            for p in group["params"]:
+                g = p.grad
+                if g is None or p.numel() == 0:
+                    continue
+                _check_matrix("fusionllm_amd.optim.Muon", p)
+                if g.dtype != p.dtype or g.layout != torch.strided:
+                    raise NotImplementedError(f"Muon step for a {p.dtype} parameter with a {g.dtype} {g.layout} grad")
+                if not p.is_contiguous():
+                    raise NotImplementedError("Muon step needs contiguous parameters")
+                state = self.state[p]
+                if len(state) == 0:
+                    state["momentum_buffer"] = torch.zeros_like(p)
+                items.append((p, g.contiguous(), state["momentum_buffer"]))
+            lr, wd = float(group["lr"]), float(group["weight_decay"])
+            for chunk in _launches(items, lambda it: (it[0].device, it[0].dtype, _sides(it[0])),
+                                   lambda it: (it[0].data_ptr(), it[2].data_ptr())):
+                small, large = _sides(chunk[0][0])
+                if group["adjust_lr_fn"] == "match_rms_adamw":
+                    tall = wide = lr * 0.2 * math.sqrt(large)
+                else:
+                    tall, wide = lr * math.sqrt(large / small), lr
+                with torch.cuda.device(chunk[0][0].device):
+                    K.muon_step([c[0] for c in chunk], [c[1] for c in chunk], [c[2] for c in chunk], tall, wide,
+                                1.0 - lr * wd, group["momentum"], group["nesterov"], group["ns_steps"],
+                                group["ns_coefficients"], group["eps"])
         return loss

@@ -58,7 +58,8 @@ enum fmoe_status {
   FMOE_ERR_LAUNCH = 5,        /* hipGetLastError after a launch */
   FMOE_ERR_WORKSPACE = 6,     /* workspace smaller than the size query returned */
   FMOE_ERR_TOO_MANY_EXPERTS = 7,
-  FMOE_ERR_SCRATCH = 8        /* workload beyond the static scratch of an allocation-free entry point */
+  FMOE_ERR_SCRATCH = 8,       /* workload beyond the static scratch of an allocation-free entry point */
+  FMOE_ERR_COEFFICIENTS = 9   /* Newton-Schulz coefficients whose iterates leave the stored range */
 };
 
 enum fmoe_dtype { FMOE_BF16 = 0, FMOE_F32 = 1 };

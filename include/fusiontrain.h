@@ -1,7 +1,7 @@
 /*
  * fusiontrain.h — C ABI of libfusionmoe.so, continued: the training operators
  * around the feed-forward block that fusionmoe.h does not declare (layer norm
- * with its backward pass).
+ * with its backward pass, orthogonalised updates and the Muon step).
  *
  * The conventions, status codes and dtype codes are those of fusionmoe.h:
  * borrowed device pointers, asynchronous on `stream`, no allocation, no
@@ -17,6 +17,10 @@ extern "C" {
 #endif
 
 #define FMOE_LAYER_NORM_MAX_DIM 16384
+#define FMOE_MUON_MAX_TENSORS 64
+#define FMOE_MUON_MAX_SIDE 65536
+#define FMOE_MUON_MAX_ELEMENTS 1073741824 /* of a matrix, its sides rounded up to multiples of 64 */
+#define FMOE_MUON_MAX_STEPS 64
 
 /* ---------------------------------------------------------------------------
  * Layer norm of the rows of x [T, dim] (dim <= FMOE_LAYER_NORM_MAX_DIM):
@@ -50,6 +54,44 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
                         int w_dtype, const void* d_residual, int64_t T, int64_t dim, void* dx,
                         void* d_weight, void* d_bias, void* workspace, size_t workspace_bytes,
                         void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Orthogonalised updates by Newton-Schulz products, for up to
+ * FMOE_MUON_MAX_TENSORS matrices of one dtype whose sides are the same up to
+ * their order (rows[i] x cols[i], row-major and dense; sides up to
+ * FMOE_MUON_MAX_SIDE, FMOE_MUON_MAX_ELEMENTS elements).  For each matrix G, with its smaller side first:
+ *   X = G / max(|G|_F, eps)
+ *   steps times:  A = X X^T,  B = coeffs[1] A + coeffs[2] A^2,  X = coeffs[0] X + B X
+ * and dst = X in G's own orientation (dst may be G's storage).  The norm is
+ * summed in fp64, the products run on fp16 operands with fp32 sums, X held in
+ * 22 bits, the result is rounded once, to dtype; for fp32 matrices (and small
+ * sides up to 128) every operand is held in 22 bits.  A matrix that holds NaN or
+ * infinities gives NaN; a zero matrix gives zeros.  Coefficients whose iterates
+ * leave the stored range (singular values up to 2.8, |b t + c t^2| up to 7.9)
+ * return FMOE_ERR_COEFFICIENTS.  Deterministic.
+ * workspace: 256-byte aligned, of the size query's bytes (a pair of sides in
+ * either order); calls that share one must not overlap.
+ * ------------------------------------------------------------------------- */
+size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype);
+int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows,
+                       const int64_t* cols, int n_tensors, int dtype, int steps,
+                       const double* coeffs, double eps, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* One Muon step of up to FMOE_MUON_MAX_TENSORS matrices (sizes and workspace as
+ * fmoe_orthogonalize), in place:
+ *   buf = momentum * buf + (1 - momentum) * grad
+ *   u   = nesterov ? (1 - momentum) * grad + momentum * buf : buf   (buf before its rounding)
+ *   param = decay * param - lr * X(u)
+ * with lr = lr_tall for matrices of more rows than columns, lr_wide otherwise
+ * (the caller's size adjustment), decay = 1 - learning rate * weight decay.
+ * Arithmetic in fp32; buf and param are rounded once, to dtype.  Params, grads
+ * and buffers must not overlap. */
+int fmoe_muon_step(void* const* params, const void* const* grads, void* const* momentum_bufs,
+                   const int64_t* rows, const int64_t* cols, int n_tensors, int dtype,
+                   double lr_tall, double lr_wide, double decay, double momentum, int nesterov,
+                   int steps, const double* coeffs, double eps, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -102,3 +102,118 @@ def test_layer_norm_operator_fake_shapes():
         assert mean.shape == rstd.shape == (7,) and mean.dtype == rstd.dtype == torch.float32
         dx, dw = torch.ops.fusionllm.layer_norm_bwd(y, x, mean, rstd, w, None)
         assert (dx.shape, dx.dtype, dw.shape, dw.dtype) == ((7, 96), torch.bfloat16, (96,), torch.float32)
+
+
+def _ns(lib, call="ortho", p=FAKE, rows=768, cols=2048, n=1, dtype=0, steps=5, co=(3.4445, -4.775, 2.0315), eps=1e-7,
+        ws=FAKE, nbytes=None, second=None):
+    import ctypes
+    pp = _lib.ptr_array([p] * max(n, 1))
+    good = _lib.ptr_array([FAKE] * max(n, 1))
+    r = (ctypes.c_int64 * max(n, 1))(*[rows] * max(n, 1))
+    c = (ctypes.c_int64 * max(n, 1))(*[cols] * max(n, 1))
+    if second:
+        r[1], c[1] = second
+    if nbytes is None:
+        nbytes = lib.fmoe_orthogonalize_workspace_bytes(rows, cols, n, dtype) - 1  # stops before the launches
+    co = (ctypes.c_double * 3)(*co)
+    if call == "ortho":
+        return lib.fmoe_orthogonalize(pp, good, r, c, n, dtype, steps, co, eps, ws, nbytes, None)
+    return lib.fmoe_muon_step(good, pp, good, r, c, n, dtype, 0.1, 0.1, 0.9, 0.95, 1, steps, co, eps, ws, nbytes,
+                              None)
+
+
+@pytest.mark.parametrize("call", ["ortho", "muon"])
+def test_newton_schulz_argument_errors_without_gpu(call):
+    lib = _lib.load()
+    f = lambda **kw: _ns(lib, call, **kw)
+    assert f() == 6 and f(ws=None) == 6 and f(nbytes=0) == 6  # admitted up to the workspace
+    assert f(n=65) == 1 and f(n=-1) == 1 and f(n=0) == 0
+    assert f(steps=0) == 1 and f(steps=65) == 1
+    assert f(dtype=2) == 4 and f(p=None) == 1 and f(p=FAKE + 1) == 3 and f(p=FAKE + 2, dtype=1) == 3
+    assert f(rows=0) == 1 and f(rows=-4) == 1 and f(cols=0) == 1 and f(cols=65537) == 2
+    assert f(rows=32769, cols=32768, nbytes=0) == 2 and f(rows=32768, cols=32768, nbytes=0) == 6
+    assert f(eps=0.0) == 1 and f(eps=-1.0) == 1 and f(eps=float("nan")) == 1
+    # one pair of sides per call, in either order
+    assert f(n=2, second=(2048, 768)) == 6 and f(n=2, second=(768, 2047)) == 2
+    # coefficients: those of the literature's cubic and quintic stay in range, these do not
+    assert f(co=(1.5, -0.5, 0.0), steps=20) == 6 and f(co=(2.0, -1.5, 0.5), steps=20) == 6
+    assert f(steps=64) == 6
+    assert f(co=(4.0, -4.775, 2.0315)) == 9 and f(co=(3.0, 0.0, 0.0)) == 9 and f(co=(1.0, 9.0, -9.5)) == 9
+    assert f(co=(float("nan"), 0.0, 0.0)) == 9 and f(co=(float("inf"), 0.0, 0.0)) == 9
+    assert b"coefficients" in lib.fmoe_status_string(9)
+
+
+def test_newton_schulz_range_check_covers_the_iterates():
+    # the host's bound of the singular values against the polynomial on a fine grid
+    import numpy as np
+    lib = _lib.load()
+    rng = np.random.default_rng(0)
+    admitted = 0
+    for _ in range(400):
+        a, b, c = rng.uniform(0.5, 4), rng.uniform(-6, 1), rng.uniform(-1, 4)
+        s = np.linspace(0, 1, 20001)
+        worst, poly = 1.0, 0.0
+        for _ in range(5):
+            t = s * s
+            poly = max(poly, np.abs(b * t + c * t * t).max())
+            s = np.abs(s * (a + t * (b + c * t)))
+            s = np.linspace(0, s.max(), 20001)
+            worst = max(worst, s.max())
+            if worst > 1e3:
+                break
+        rc = _ns(lib, co=(a, b, c))
+        if rc == 6:
+            admitted += 1
+            assert worst < 2.8 and poly < 7.9, (a, b, c)
+        else:
+            assert rc == 9 and (worst > 2.7 or poly > 7.7), (a, b, c)
+    assert 20 < admitted < 380
+
+
+def test_newton_schulz_workspace_size():
+    lib = _lib.load()
+    q = lib.fmoe_orthogonalize_workspace_bytes
+    # partial sums; X twice as hi and lo; A and B (hi, and lo for fp32 and small sides); sides padded to 64
+    assert q(768, 2048, 3, 0) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (4 * 768 * 2048 + 2 * 768 * 768)
+    assert q(768, 2048, 3, 1) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (4 * 768 * 2048 + 4 * 768 * 768)
+    assert q(2048, 768, 3, 0) == q(768, 2048, 3, 0)
+    assert q(5, 70, 1, 0) == 256 + 2 * (4 * 64 * 128 + 4 * 64 * 64)
+    assert q(0, 5, 1, 0) == q(5, 5, 0, 0) == q(5, 5, 65, 0) == q(65537, 5, 1, 0) == q(32769, 32768, 1, 0) == 0
+
+
+def test_muon_and_orthogonalize_refusals():
+    from fusionllm_amd.optim import Muon, orthogonalize
+    P = torch.nn.Parameter
+    with pytest.raises(ValueError, match="matrices"):
+        Muon([P(torch.zeros(4))])
+    with pytest.raises(ValueError, match="matrices"):
+        Muon([P(torch.zeros(2, 2, 2))])
+    p = P(torch.zeros(4, 4))
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="twice"):
+        Muon([p, p])
+    for kw in (dict(lr=-1.0), dict(weight_decay=-0.1), dict(momentum=1.0), dict(momentum=-0.1), dict(eps=0.0),
+               dict(ns_steps=0), dict(ns_steps=65), dict(ns_coefficients=(1.0, 2.0)), dict(adjust_lr_fn="other")):
+        with pytest.raises(ValueError):
+            Muon([p], **kw)
+    opt = Muon([p])
+    assert opt.defaults["ns_steps"] == 5 and opt.defaults["lr"] == 1e-3 and opt.defaults["momentum"] == 0.95
+    opt.step()  # no gradient: nothing to do
+    p.grad = torch.zeros(4, 4)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        opt.step()
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="matrices"):
+        orthogonalize(torch.zeros(4))
+    with pytest.raises(ValueError, match="steps"):
+        orthogonalize(torch.zeros(4, 4), steps=0)
+    with FakeTensorMode():
+        x = torch.empty(4, 6, device="cuda")
+        with pytest.raises(NotImplementedError, match="bf16 and fp32"):
+            orthogonalize(x.half())
+        with pytest.raises(RuntimeError, match="no backward"):
+            orthogonalize(x.requires_grad_())
+        with pytest.raises(NotImplementedError, match="65536"):
+            orthogonalize(torch.empty(2, 65537, device="cuda"))
+        with pytest.raises(NotImplementedError, match="elements"):
+            orthogonalize(torch.empty(32769, 32768, device="cuda"))
