@@ -31,18 +31,18 @@
 #include <cmath>
 
 #include "../../include/fusiontrain.h"
+#include "elements.h"
 #include "fmoe_common.h"
 #include "gemm_core.h"
 
 namespace fmoe {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
 constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
 constexpr int64_t kSplitSmall = 128;
-constexpr int kNormParts_ = 64;     // partial sums of squares per matrix, at most
+constexpr int kNsParts = 64;        // partial sums of squares per matrix, at most (a wave adds them)
 constexpr int kNormChunk = 8192;    // elements per partial sum, at least
 // Stored values: X 2^14, A 2^13, B 2^13 (singular values of X below 2.8, |B| below 7.9).
 constexpr float kXScale = 16384.0f, kAScale = 8192.0f;
@@ -69,14 +69,31 @@ struct NsArgs {
 
 // ---- the source: elements and the value that is orthogonalised ---------------------
 
-__device__ __forceinline__ float ns_elem(const void* p, int dtype, int64_t e) {
-  return dtype == FMOE_BF16 ? bf2f(static_cast<const uint16_t*>(p)[e]) : static_cast<const float*>(p)[e];
+// N (8, or fewer at an edge) consecutive elements from e on; the rest zero.
+template <int DT>
+__device__ __forceinline__ void ns_load8(const void* p, int64_t e, int n, float* v) {
+  if (n >= 8) {
+    unpack<DT, 8>(load_raw<DT, 8>(p, e), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = 0.0f;
+      if (i < n) unpack<DT, 1>(load_raw<DT, 1>(p, e + i), v + i);
+    }
+  }
 }
-__device__ __forceinline__ void ns_put(void* p, int dtype, int64_t e, float v) {
-  if (dtype == FMOE_BF16) static_cast<uint16_t*>(p)[e] = f2bf(v);
-  else static_cast<float*>(p)[e] = v;
+template <int DT>
+__device__ __forceinline__ void ns_store8(void* p, int64_t e, int n, const float* v) {
+  if (n >= 8) {
+    store_chunk<DT, 8>(p, e, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) store_chunk<DT, 1>(p, e + i, v + i);
+  }
 }
-// Muon: the momentum after this step, from the one before it (fp32, not yet rounded to its type).
+
+// Muon: the momentum after this step (fp32, not yet rounded to its type) and the update.
 __device__ __forceinline__ float ns_momentum(const NsArgs& a, float g, float buf) { return fmaf(a.mom, buf, a.om * g); }
 __device__ __forceinline__ float ns_update(const NsArgs& a, float g, float newbuf) {
   return a.nesterov ? fmaf(a.mom, newbuf, a.om * g) : newbuf;
@@ -84,6 +101,7 @@ __device__ __forceinline__ float ns_update(const NsArgs& a, float g, float newbu
 
 // Sum of squares of each matrix in fp64 (no overflow of large values, no loss over
 // millions of terms): one partial sum per workgroup, in a fixed order.
+template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
   __shared__ double red[4];
   const int mat = blockIdx.y, part = blockIdx.x;
@@ -91,10 +109,18 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
   const void* g = a.src[mat];
   const void* b = a.buf[mat];
   double s = 0.0;
-  for (int64_t e = part * 256 + threadIdx.x; e < total; e += static_cast<int64_t>(a.parts) * 256) {
-    float u = ns_elem(g, a.dtype, e);
-    if (a.muon) u = ns_update(a, u, ns_momentum(a, u, ns_elem(b, a.dtype, e)));
-    s += static_cast<double>(u) * static_cast<double>(u);
+  for (int64_t e = (part * 256 + static_cast<int>(threadIdx.x)) * 8; e < total;
+       e += static_cast<int64_t>(a.parts) * 256 * 8) {
+    const int n = static_cast<int>(min(total - e, int64_t(8)));
+    float u[8], v[8];
+    ns_load8<DT>(g, e, n, u);
+    if constexpr (MUON) {
+      ns_load8<DT>(b, e, n, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = ns_update(a, u[i], ns_momentum(a, u[i], v[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fma(static_cast<double>(u[i]), static_cast<double>(u[i]), s);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) s = s + __shfl_xor(s, off, 64);
@@ -105,42 +131,61 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const NsArgs a) {
 
 // X = u / max(|u|, eps) as hi + lo, its smaller side first, zeros in the padding; Muon: the
 // new momentum.  One 64 x 64 tile of X per workgroup, through LDS (tall matrices arrive transposed).
+template <int DT, bool MUON>
 __global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
   __shared__ float tile[64][65];
+  __shared__ double scale_s;
   const int mat = blockIdx.z;
   const bool tall = (a.tall >> mat) & 1;
   const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;  // of X
   const int rows = tall ? a.n : a.m, cols = tall ? a.m : a.n;  // of the matrix as it lies
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
-  double ss = 0.0;
-  for (int p = 0; p < a.parts; ++p) ss += a.norm[mat * a.parts + p];
-  // NaN (of a matrix that holds NaN or infinities) stays NaN
-  const double nrm = sqrt(ss);
-  const double scale = static_cast<double>(kXScale) / (nrm < a.eps ? a.eps : nrm);
+  const int q = (threadIdx.x & 7) * 8;
   const void* g = a.src[mat];
   void* b = a.buf[mat];
-  const int c = threadIdx.x & 63;
+  const int n = min(cols - (c0 + q), 8);
+  float u[2][8];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int r = (threadIdx.x >> 6) + 4 * k;
-    float v = 0.0f;
-    if (r0 + r < rows && c0 + c < cols) {
-      const int64_t e = static_cast<int64_t>(r0 + r) * cols + c0 + c;
-      float u = ns_elem(g, a.dtype, e);
-      if (a.muon) {
-        const float nb = ns_momentum(a, u, ns_elem(b, a.dtype, e));
-        ns_put(b, a.dtype, e, nb);
-        u = ns_update(a, u, nb);
+  for (int k = 0; k < 2; ++k) {
+    const int r = r0 + (threadIdx.x >> 3) + 32 * k;
+    const int64_t e = static_cast<int64_t>(r) * cols + c0 + q;
+    const int valid = r < rows ? n : 0;
+    ns_load8<DT>(g, e, valid, u[k]);
+    if constexpr (MUON) {
+      float v[8];
+      ns_load8<DT>(b, e, valid, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = ns_momentum(a, u[k][i], v[i]);
+        u[k][i] = ns_update(a, u[k][i], v[i]);
       }
-      v = static_cast<float>(static_cast<double>(u) * scale);
+      ns_store8<DT>(b, e, valid, v);
     }
-    if (tall) tile[c][r] = v;
-    else tile[r][c] = v;
+  }
+  if (threadIdx.x < 64) {  // the partial sums, in a fixed order
+    double ss = static_cast<int>(threadIdx.x) < a.parts ? a.norm[mat * a.parts + threadIdx.x] : 0.0;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
+    const double nrm = sqrt(ss);
+    // the norm of a matrix that holds NaN or infinities is none, and its X is NaN
+    if (threadIdx.x == 0) scale_s = static_cast<double>(kXScale) / (nrm < a.eps ? a.eps : nrm);
+  }
+  __syncthreads();
+  const double scale = scale_s;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = (threadIdx.x >> 3) + 32 * k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = static_cast<float>(static_cast<double>(u[k][i]) * scale);
+      if (tall) tile[q + i][r] = v;
+      else tile[r][q + i] = v;
+    }
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int r = (threadIdx.x >> 3) + 32 * k, q = (threadIdx.x & 7) * 8;
+    const int r = (threadIdx.x >> 3) + 32 * k;
     half8 h, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -166,8 +211,23 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// TM x TN outputs per workgroup of four waves (2 x 2), K in steps of 64 through two LDS stages:
-// the copies of the next stage (global -> LDS, no registers) run while this one is multiplied.
+// The result: n (up to 8) consecutive elements of the matrix, or of the parameter's update.
+template <int DT>
+__device__ __forceinline__ void ns_finish(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr) {
+  if (n <= 0) return;
+  if (a.muon) {
+    float p[8];
+    ns_load8<DT>(dst, o, n, p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], p[e] * a.decay);
+  }
+  ns_store8<DT>(dst, o, n, v);
+}
+
+// TM x TN outputs per workgroup of four waves (2 x 2), K in steps of 64 through two LDS stages.
+// A step reads its whole stage into registers, and the copies (global -> LDS, no registers) of the
+// stage after the next go into its slot while it is multiplied: one to two stages are in
+// flight, and of the two workgroups of a CU one reads LDS while the other multiplies.
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
@@ -252,96 +312,160 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   const uint32_t xb = A_ST + (SYM ? frag_base(wn * WTN, lane) : tr_base(4 * wn, lane));
   typedef __attribute__((address_space(3))) half8 lds_half8;
   issue(0);
+  if (steps > 1) issue(1);
   for (int it = 0; it < steps; ++it) {
-    wait_vm_barrier<0>();  // this stage is there, and every wave is done with the other
-    if (it + 1 < steps) issue((it + 1) & 1);
+    // this stage is there (the next may be in flight)
+    if (it + 1 < steps) wait_vm_barrier<CA + CB>();
+    else wait_vm_barrier<0>();
     const uint32_t src = sbase + (it & 1) * STAGE;
+    half8 fa[2][FM], fb[2][FN];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
-      half8 fa[FM], fb[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
+      for (int i = 0; i < FM; ++i) fa[kh][i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        if constexpr (SYM) fb[j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
-        else fb[j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
+        if constexpr (SYM) fb[kh][j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
+        else fb[kh][j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
       }
+    }
+    wait_lds_barrier();  // every wave has this stage in registers: its slot takes the stage after the next
+    if (it + 2 < steps) issue(it & 1);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
-    }
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[kh][j], fa[kh][i], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_s_setprio(0);
   }
 
-  // acc[i][j] of this lane: row 16 i + l % 16, columns 16 j + 4 (l / 16) + 0..3 of the wave's block.
+  // Epilogue: the wave's block goes through its part of LDS as fp32 (16-byte chunk c of row r at
+  // slot c ^ f(r): no bank conflicts by rows or by columns) and comes back as 8 consecutive elements
+  // of a row, or of a column for a transposed store, so that global memory sees 16-byte accesses of
+  // full lines.  (Storing from the accumulators' layout, 8 bytes or less per lane in
+  // 16 rows at once, took as long as the multiplication.)
+  constexpr int MASK = WTN / 4 - 1;
+  static_assert(4 * WTM * WTN * 4 <= 2 * STAGE);
+  float* ep = reinterpret_cast<float*>(smem) + w * (WTM * WTN);
+  auto slot = [](int r, int c) { return r * WTN + ((c ^ ((r & 15) ^ ((r >> 3) & 7))) & MASK) * 4; };
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int r = ti * TM + wm * WTM + 16 * i + (lane & 15);
-    if (r >= a.mp) continue;
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int c = tj * TN + wn * WTN + 16 * j + 4 * (lane >> 4);
-      if (c >= (SYM ? a.mp : a.np)) continue;
-      float v[4];
-      if constexpr (SYM) {
-        const int64_t o = msq + static_cast<int64_t>(r) * a.mp + c;
-        if constexpr (MODE == NS_GRAM) {
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<f32x4*>(ep + slot(16 * i + (lane & 15), 4 * j + (lane >> 4))) = acc[i][j];
+  __builtin_amdgcn_wave_barrier();
+  const int row0 = ti * TM + wm * WTM, col0 = tj * TN + wn * WTN;  // of the wave's block
+  auto by_row = [&](int r, int c, float* v) {  // elements c .. c + 7 of row r
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + slot(r, c >> 2));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(ep + slot(r, (c >> 2) + 1));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * (kAScale / (kXScale * kXScale));
-        } else {
-          const half4 h = *reinterpret_cast<const half4*>(a.ah + o);
-          half4 l = {0, 0, 0, 0};
-          if constexpr (SPLIT) l = *reinterpret_cast<const half4*>(a.al + o);
+    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+  };
+  auto put_parts = [](_Float16* ph_, _Float16* pl_, int64_t o, const float* v, bool lo) {
+    half8 h, l;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (acc[i][j][e] / kAScale));
-        }
-        _Float16* oh = MODE == NS_GRAM ? a.ah : a.bh;
-        _Float16* ol = MODE == NS_GRAM ? a.al : a.bl;
-        half4 h, l;
+    for (int e = 0; e < 8; ++e) {
+      h[e] = static_cast<_Float16>(v[e]);
+      l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+    }
+    *reinterpret_cast<half8*>(ph_ + o) = h;
+    if (lo) *reinterpret_cast<half8*>(pl_ + o) = l;
+  };
+  constexpr int LPR = WTN / 8, RPP = 64 / LPR;  // lanes per row, rows per pass
+  constexpr int LPC = WTM / 8, CPP = 64 / LPC;  // the same by columns
+  const int lc = (lane % LPR) * 8, lr = lane / LPR;
+  const int tr = (lane % LPC) * 8, tc = lane / LPC;
+
+  if constexpr (SYM) {
+    _Float16* oh = MODE == NS_GRAM ? a.ah : a.bh;
+    _Float16* ol = MODE == NS_GRAM ? a.al : a.bl;
+    // the value to store, for the element that the wave's sum at this place belongs to
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[e] = static_cast<_Float16>(v[e]);
-          l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
-        }
-        *reinterpret_cast<half4*>(oh + o) = h;
-        if constexpr (SPLIT) *reinterpret_cast<half4*>(ol + o) = l;
-        if (ti != tj) {
+    for (int p = 0; p < WTM / RPP; ++p) {
+      const int r = p * RPP + lr;
+      float v[8];
+      by_row(r, lc, v);
+      const bool on = row0 + r < a.mp && col0 + lc < a.mp;
+      const int64_t o = msq + static_cast<int64_t>(on ? row0 + r : 0) * a.mp + (on ? col0 + lc : 0);
+      if constexpr (MODE == NS_GRAM) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t ot = msq + static_cast<int64_t>(c + e) * a.mp + r;
-            oh[ot] = h[e];
-            if constexpr (SPLIT) ol[ot] = l[e];
-          }
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
+      } else {
+        const half8 h = *reinterpret_cast<const half8*>(a.ah + o);
+        half8 l = {0, 0, 0, 0, 0, 0, 0, 0};
+        if constexpr (SPLIT) l = *reinterpret_cast<const half8*>(a.al + o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (v[e] * (1.0f / kAScale)));
+      }
+      if (on) put_parts(oh, ol, o, v, SPLIT);
+      if (ti != tj) {  // back into LDS for the mirrored tile
+        *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+    if (ti == tj) return;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < WTN / CPP; ++p) {
+      const int c = p * CPP + tc;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
+      if (row0 + tr < a.mp && col0 + c < a.mp)
+        put_parts(oh, ol, msq + static_cast<int64_t>(col0 + c) * a.mp + row0 + tr, v, SPLIT);
+    }
+  } else {
+    // X' = a X + B X, X from hi and lo
+#pragma unroll
+    for (int p = 0; p < WTM / RPP; ++p) {
+      const int r = p * RPP + lr;
+      float v[8];
+      by_row(r, lc, v);
+      const bool on = row0 + r < a.mp && col0 + lc < a.np;
+      const int64_t o = mx + static_cast<int64_t>(on ? row0 + r : 0) * a.np + (on ? col0 + lc : 0);
+      const half8 xh = *reinterpret_cast<const half8*>(a.xh[cur] + o);
+      const half8 xl = *reinterpret_cast<const half8*>(a.xl[cur] + o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = fmaf(a.ca, static_cast<float>(xh[e]) + static_cast<float>(xl[e]), v[e] * (1.0f / kAScale));
+      if constexpr (MODE == NS_STEP) {
+        if (on) put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
+      } else {
+        *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+    if constexpr (MODE == NS_LAST) {
+      __builtin_amdgcn_wave_barrier();
+      void* const dst = a.dst[mat];
+      auto put = [&](int64_t o, int n, float* v, float lr_) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kXScale);
+        if (a.dtype == FMOE_BF16) ns_finish<FMOE_BF16>(a, dst, o, n, v, lr_);
+        else ns_finish<FMOE_F32>(a, dst, o, n, v, lr_);
+      };
+      if ((a.tall >> mat) & 1) {
+#pragma unroll 2
+        for (int p = 0; p < WTN / CPP; ++p) {
+          const int c = p * CPP + tc;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
+          const int n = col0 + c < a.n ? min(a.m - (row0 + tr), 8) : 0;
+          put(static_cast<int64_t>(col0 + c) * a.m + row0 + tr, n, v, a.lr_tall);
         }
       } else {
-        const int64_t o = mx + static_cast<int64_t>(r) * a.np + c;
-        const half4 xh = *reinterpret_cast<const half4*>(a.xh[cur] + o);
-        const half4 xl = *reinterpret_cast<const half4*>(a.xl[cur] + o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = fmaf(a.ca, static_cast<float>(xh[e]) + static_cast<float>(xl[e]), acc[i][j][e] / kAScale);
-        if constexpr (MODE == NS_STEP) {
-          half4 h, l;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            h[e] = static_cast<_Float16>(v[e]);
-            l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
-          }
-          *reinterpret_cast<half4*>(a.xh[1 - cur] + o) = h;
-          *reinterpret_cast<half4*>(a.xl[1 - cur] + o) = l;
-        } else {
-          const bool tall = (a.tall >> mat) & 1;
-          if (r >= a.m) continue;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (c + e >= a.n) continue;
-            const int64_t q = tall ? static_cast<int64_t>(c + e) * a.m + r : static_cast<int64_t>(r) * a.n + c + e;
-            float out = v[e] * (1.0f / kXScale);
-            if (a.muon) out = fmaf(tall ? -a.lr_tall : -a.lr_wide, out, ns_elem(a.dst[mat], a.dtype, q) * a.decay);
-            ns_put(a.dst[mat], a.dtype, q, out);
-          }
+#pragma unroll 2
+        for (int p = 0; p < WTM / RPP; ++p) {
+          const int r = p * RPP + lr;
+          float v[8];
+          by_row(r, lc, v);
+          const int n = row0 + r < a.m ? min(a.n - (col0 + lc), 8) : 0;
+          put(static_cast<int64_t>(row0 + r) * a.n + col0 + lc, n, v, a.lr_wide);
         }
       }
     }
@@ -359,7 +483,7 @@ struct NsLayout {
 };
 inline NsLayout ns_layout(int64_t m, int64_t n, int count, bool split) {
   NsLayout l;
-  l.parts = static_cast<int>(std::min<int64_t>(kNormParts_, ceil_div(m * n, kNormChunk)));
+  l.parts = static_cast<int>(std::min<int64_t>(kNsParts, ceil_div(m * n, kNormChunk)));
   l.norm = (static_cast<size_t>(count) * l.parts * sizeof(double) + 255) / 256 * 256;
   l.x = static_cast<size_t>(count) * ns_pad(m) * ns_pad(n) * 2;
   l.sq = static_cast<size_t>(count) * ns_pad(m) * ns_pad(m) * 2;
@@ -460,8 +584,16 @@ inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* 
   a.ah = take(l.sq);
   a.bh = take(l.sq);
   if (split) a.al = take(l.sq), a.bl = take(l.sq);
-  ns_norm_kernel<<<dim3(a.parts, a.count), dim3(256), 0, s>>>(a);
-  ns_load_kernel<<<dim3(a.np / 64, a.mp / 64, a.count), dim3(256), 0, s>>>(a);
+#define FMOE_NS_LOAD(DT, MUON)                                                                   \
+  do {                                                                                           \
+    ns_norm_kernel<DT, MUON><<<dim3(a.parts, a.count), dim3(256), 0, s>>>(a);                    \
+    ns_load_kernel<DT, MUON><<<dim3(a.np / 64, a.mp / 64, a.count), dim3(256), 0, s>>>(a);       \
+  } while (0)
+  if (a.dtype == FMOE_BF16 && a.muon) FMOE_NS_LOAD(FMOE_BF16, true);
+  else if (a.dtype == FMOE_BF16) FMOE_NS_LOAD(FMOE_BF16, false);
+  else if (a.muon) FMOE_NS_LOAD(FMOE_F32, true);
+  else FMOE_NS_LOAD(FMOE_F32, false);
+#undef FMOE_NS_LOAD
   for (int k = 0; k < steps; ++k) {
     ns_product<NS_GRAM>(a, k & 1, split, s);
     ns_product<NS_POLY>(a, k & 1, split, s);
