@@ -39,6 +39,7 @@ namespace fmoe {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
+constexpr int kNsCus = 256;         // CUs of the chip: workgroups of the persistent products
 constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
 constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
 constexpr int64_t kSplitSmall = 128;
@@ -211,6 +212,37 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
+// The values to store from sums of 8 consecutive elements of a row (offset o in A or X).
+__device__ __forceinline__ void ns_gram8(float* v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
+}
+template <bool SPLIT>
+__device__ __forceinline__ void ns_poly8(const NsArgs& a, int64_t o, float* v) {  // b A + c A^2
+  const half8 h = *reinterpret_cast<const half8*>(a.ah + o);
+  half8 l = {0, 0, 0, 0, 0, 0, 0, 0};
+  if constexpr (SPLIT) l = *reinterpret_cast<const half8*>(a.al + o);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (v[e] * (1.0f / kAScale)));
+}
+__device__ __forceinline__ void ns_step8(const NsArgs& a, int cur, int64_t o, float* v) {  // a X + B X
+  const half8 h = *reinterpret_cast<const half8*>(a.xh[cur] + o);
+  const half8 l = *reinterpret_cast<const half8*>(a.xl[cur] + o);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    v[e] = fmaf(a.ca, static_cast<float>(h[e]) + static_cast<float>(l[e]), v[e] * (1.0f / kAScale));
+}
+__device__ __forceinline__ void ns_put_parts(_Float16* hi, _Float16* lo, int64_t o, const float* v, bool with_lo) {
+  half8 h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    h[e] = static_cast<_Float16>(v[e]);
+    l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+  }
+  *reinterpret_cast<half8*>(hi + o) = h;
+  if (with_lo) *reinterpret_cast<half8*>(lo + o) = l;
+}
 // The result: n (up to 8) consecutive elements of the matrix, or of the parameter's update.
 template <int DT>
 __device__ __forceinline__ void ns_finish(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr) {
@@ -222,6 +254,13 @@ __device__ __forceinline__ void ns_finish(const NsArgs& a, void* dst, int64_t o,
     for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], p[e] * a.decay);
   }
   ns_store8<DT>(dst, o, n, v);
+}
+
+__device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kXScale);
+  if (a.dtype == FMOE_BF16) ns_finish<FMOE_BF16>(a, dst, o, n, v, lr);
+  else ns_finish<FMOE_F32>(a, dst, o, n, v, lr);
 }
 
 // TM x TN outputs per workgroup of four waves (2 x 2), K in steps of 64 through two LDS stages.
@@ -364,16 +403,6 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
   };
-  auto put_parts = [](_Float16* ph_, _Float16* pl_, int64_t o, const float* v, bool lo) {
-    half8 h, l;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      h[e] = static_cast<_Float16>(v[e]);
-      l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
-    }
-    *reinterpret_cast<half8*>(ph_ + o) = h;
-    if (lo) *reinterpret_cast<half8*>(pl_ + o) = l;
-  };
   constexpr int LPR = WTN / 8, RPP = 64 / LPR;  // lanes per row, rows per pass
   constexpr int LPC = WTM / 8, CPP = 64 / LPC;  // the same by columns
   const int lc = (lane % LPR) * 8, lr = lane / LPR;
@@ -390,18 +419,9 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
       by_row(r, lc, v);
       const bool on = row0 + r < a.mp && col0 + lc < a.mp;
       const int64_t o = msq + static_cast<int64_t>(on ? row0 + r : 0) * a.mp + (on ? col0 + lc : 0);
-      if constexpr (MODE == NS_GRAM) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
-      } else {
-        const half8 h = *reinterpret_cast<const half8*>(a.ah + o);
-        half8 l = {0, 0, 0, 0, 0, 0, 0, 0};
-        if constexpr (SPLIT) l = *reinterpret_cast<const half8*>(a.al + o);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (v[e] * (1.0f / kAScale)));
-      }
-      if (on) put_parts(oh, ol, o, v, SPLIT);
+      if constexpr (MODE == NS_GRAM) ns_gram8(v);
+      else ns_poly8<SPLIT>(a, o, v);
+      if (on) ns_put_parts(oh, ol, o, v, SPLIT);
       if (ti != tj) {  // back into LDS for the mirrored tile
         *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
@@ -416,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
       if (row0 + tr < a.mp && col0 + c < a.mp)
-        put_parts(oh, ol, msq + static_cast<int64_t>(col0 + c) * a.mp + row0 + tr, v, SPLIT);
+        ns_put_parts(oh, ol, msq + static_cast<int64_t>(col0 + c) * a.mp + row0 + tr, v, SPLIT);
     }
   } else {
     // X' = a X + B X, X from hi and lo
@@ -427,13 +447,9 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
       by_row(r, lc, v);
       const bool on = row0 + r < a.mp && col0 + lc < a.np;
       const int64_t o = mx + static_cast<int64_t>(on ? row0 + r : 0) * a.np + (on ? col0 + lc : 0);
-      const half8 xh = *reinterpret_cast<const half8*>(a.xh[cur] + o);
-      const half8 xl = *reinterpret_cast<const half8*>(a.xl[cur] + o);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = fmaf(a.ca, static_cast<float>(xh[e]) + static_cast<float>(xl[e]), v[e] * (1.0f / kAScale));
+      ns_step8(a, cur, o, v);
       if constexpr (MODE == NS_STEP) {
-        if (on) put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
+        if (on) ns_put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
       } else {
         *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
@@ -442,12 +458,6 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     if constexpr (MODE == NS_LAST) {
       __builtin_amdgcn_wave_barrier();
       void* const dst = a.dst[mat];
-      auto put = [&](int64_t o, int n, float* v, float lr_) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kXScale);
-        if (a.dtype == FMOE_BF16) ns_finish<FMOE_BF16>(a, dst, o, n, v, lr_);
-        else ns_finish<FMOE_F32>(a, dst, o, n, v, lr_);
-      };
       if ((a.tall >> mat) & 1) {
 #pragma unroll 2
         for (int p = 0; p < WTN / CPP; ++p) {
@@ -456,7 +466,7 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
           const int n = col0 + c < a.n ? min(a.m - (row0 + tr), 8) : 0;
-          put(static_cast<int64_t>(col0 + c) * a.m + row0 + tr, n, v, a.lr_tall);
+          ns_result8(a, dst, static_cast<int64_t>(col0 + c) * a.m + row0 + tr, n, v, a.lr_tall);
         }
       } else {
 #pragma unroll 2
@@ -465,11 +475,334 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
           float v[8];
           by_row(r, lc, v);
           const int n = row0 + r < a.m ? min(a.n - (col0 + lc), 8) : 0;
-          put(static_cast<int64_t>(row0 + r) * a.n + col0 + lc, n, v, a.lr_wide);
+          ns_result8(a, dst, static_cast<int64_t>(row0 + r) * a.n + col0 + lc, n, v, a.lr_wide);
         }
       }
     }
   }
+}
+
+// ---- the products in 256 x 256 tiles -------------------------------------------------------
+// The main loop of gemm_core.h with fp16 operands: persistent workgroups of 8 waves (64 x 128 each)
+// walk the tiles; the copies run as one ring over all K steps of all of a workgroup's tiles, so
+// the next tile's first operands arrive during an epilogue.  A 256 x 256 tile reads half as
+// much through L2 as four of 128 x 128, which is what bounds those.
+
+#define FMOE_NS_MF(c, a, b) "v_mfma_f32_16x16x32_f16 " c ", " a ", " b ", " c "\n"
+__device__ __forceinline__ void ns_mfma4(f32x4& c00, f32x4& c10, f32x4& c01, f32x4& c11, const bf16x8& p0,
+                                         const bf16x8& p1, const bf16x8& q0, const bf16x8& q1) {
+  asm volatile(FMOE_NS_MF("%[c00]", "%[p0]", "%[q0]") FMOE_NS_MF("%[c10]", "%[p0]", "%[q1]")
+               FMOE_NS_MF("%[c01]", "%[p1]", "%[q0]") FMOE_NS_MF("%[c11]", "%[p1]", "%[q1]")
+               : [c00] "+v"(c00), [c10] "+v"(c10), [c01] "+v"(c01), [c11] "+v"(c11)
+               : [p0] "v"(p0), [p1] "v"(p1), [q0] "v"(q0), [q1] "v"(q1)
+               : "memory");
+}
+#undef FMOE_NS_MF
+
+// Quarter (I, J) of the wave's block (core::quarter with fp16 operands).
+template <int I, int J>
+__device__ __forceinline__ void ns_quarter(f32x4 (&acc)[core::FM][core::FN], const core::AFrag& a,
+                                           const core::BFrag& b) {
+  __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int kh = x >> 1, n = (x & 1) * 2;
+    ns_mfma4(acc[2 * I][4 * J + n], acc[2 * I + 1][4 * J + n], acc[2 * I][4 * J + n + 1],
+             acc[2 * I + 1][4 * J + n + 1], b[kh][n], b[kh][n + 1], a[kh][0], a[kh][1]);
+  }
+  __builtin_amdgcn_s_setprio(0);
+  core::barrier();
+}
+
+struct NsTile {
+  int mat, ti, tj;
+};
+
+template <int MODE, bool SPLIT>
+__global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, const int cur) {
+  using namespace core;
+  constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = w / WN, wn = w % WN;
+  const uint32_t sbase = lds_addr(smem);
+  const int tiles_m = (a.mp + BM - 1) / BM, tiles_n = SYM ? tiles_m : (a.np + BN - 1) / BN;
+  const int per = SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+  const int items = per * a.count;
+  // Workgroup b runs on XCD b % 8: its XCD takes a contiguous run of each round's tiles.
+  const int NP = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
+  const int b = NP % 8 == 0 ? (bid % 8) * (NP / 8) + bid / 8 : bid;
+  const int my_items = (items - b + NP - 1) / NP;
+  if (my_items <= 0) return;
+  const int K = MODE == NS_GRAM ? a.np : a.mp;
+  const int ld = K, ldb = SYM ? K : a.np;
+  const int nk = K / BK, steps = SPLIT ? 3 * nk : nk;
+  const int total = my_items * steps;
+
+  auto locate = [&](int item) __attribute__((always_inline)) {
+    NsTile t;
+    t.mat = item / per;
+    const int q = item - t.mat * per;
+    if constexpr (SYM) triangle(q, t.ti, t.tj);
+    else t.ti = q / tiles_n, t.tj = q - t.ti * tiles_n;
+    t.mat = __builtin_amdgcn_readfirstlane(t.mat);
+    t.ti = __builtin_amdgcn_readfirstlane(t.ti);
+    t.tj = __builtin_amdgcn_readfirstlane(t.tj);
+    return t;
+  };
+
+  // ---- copy cursor (the units of a stage and their LDS layout as in gemm_core.h)
+  const uint32_t lds_a = sbase + (64 * (w >> 2) + 8 * (w & 3)) * RB;
+  const uint32_t lds_b = sbase + A_BYTES + w * 1024;
+  int c_ti = 0, c_kt = 0, c_seg = 0;
+  const uint8_t *c_a = nullptr, *c_b = nullptr;
+  uint32_t a_off[4], b_off[4];
+  const int64_t bstep = SYM ? RB : static_cast<int64_t>(2) * BK * ldb;
+  // operand bases of the tile being copied, for segment c_seg (SPLIT: hi lo, lo hi, hi hi)
+  auto bases = [&](const NsTile& t) __attribute__((always_inline)) {
+    const int64_t msq = static_cast<int64_t>(t.mat) * a.mp * a.mp, mx = static_cast<int64_t>(t.mat) * a.mp * a.np;
+    const bool alo = SPLIT && c_seg == 1, blo = SPLIT && c_seg == 0;
+    const _Float16 *p, *q;
+    if constexpr (MODE == NS_GRAM) {
+      p = (alo ? a.xl[cur] : a.xh[cur]) + mx;
+      q = (blo ? a.xl[cur] : a.xh[cur]) + mx;
+    } else if constexpr (MODE == NS_POLY) {
+      p = (alo ? a.al : a.ah) + msq;
+      q = (blo ? a.al : a.ah) + msq;
+    } else {
+      p = (alo ? a.bl : a.bh) + msq;
+      q = (blo ? a.xl[cur] : a.xh[cur]) + mx;
+    }
+    c_a = reinterpret_cast<const uint8_t*>(p + static_cast<int64_t>(t.ti) * BM * ld);
+    c_b = reinterpret_cast<const uint8_t*>(SYM ? q + static_cast<int64_t>(t.tj) * BN * ld : q);
+  };
+  auto copy_tile = [&](int ti) __attribute__((always_inline)) {
+    const NsTile t = locate(b + ti * NP);
+    c_seg = 0;
+    bases(t);
+    // the lane as an opaque value: what follows is formed here, not kept through the main loop
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int dchunk = (l & 7) ^ swzk(l >> 3);
+    const int last_m = min(a.mp - t.ti * BM, BM) - 1, last_n = min(a.mp - t.tj * BN, BN) - 1;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = min(64 * (w >> 2) + 8 * (w & 3) + (l >> 3) + 128 * (q & 1) + 32 * (q >> 1), last_m);
+      a_off[q] = static_cast<uint32_t>(r * ld + dchunk * 8) * 2u;
+      if constexpr (SYM) {
+        const int n = min(128 * (q & 1) + 64 * (q >> 1) + 8 * w + (l >> 3), last_n);
+        b_off[q] = static_cast<uint32_t>(n * ldb + dchunk * 8) * 2u;
+      } else {
+        const int krow = 4 * w + (l >> 4);
+        const int cb = ((((l & 15) >> 1) ^ wsw(krow)) << 1) | (l & 1);
+        const int col = 128 * (cb >> 3) + 8 * (cb & 7) + 64 * (q >> 1);
+        b_off[q] = static_cast<uint32_t>((32 * (q & 1) + krow) * ldb + min(t.tj * BN + col, a.np - 8)) * 2u;
+      }
+    }
+  };
+  copy_tile(0);
+  // A stage's units are issued in the order A0, B0, B1, A1; A1 moves the cursor on.  Past the last
+  // step the last stage is copied again (into slots that are free and not read any more).
+  auto issue_a = [&](int it, int u) __attribute__((always_inline)) {
+    const uint32_t st = lds_a + (it & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) copy16(st + (128 * i + 32 * u) * RB, c_a, a_off[2 * u + i]);
+    if (u == 0) return;
+    c_a += RB;
+    c_b += bstep;
+    if (__builtin_expect(++c_kt == nk, 0)) {
+      if (SPLIT && c_seg < 2) {
+        c_kt = 0;
+        ++c_seg;
+        bases(locate(b + c_ti * NP));
+      } else if (c_ti + 1 < my_items) {
+        c_kt = 0;
+        copy_tile(++c_ti);
+      } else {
+        --c_kt;
+        c_a -= RB;
+        c_b -= bstep;
+      }
+    }
+  };
+  auto issue_b = [&](int it, int u) __attribute__((always_inline)) {
+    const uint32_t st = lds_b + (it & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      copy16(SYM ? st + (128 * i + 64 * u) * RB : st + u * UNIT + i * 8192, c_b, b_off[2 * u + i]);
+  };
+
+  uint32_t xa = frag_base(wm * WTM, lane);
+  uint32_t xb = A_BYTES + (SYM ? frag_base(wn * WTN, lane) : tr_base(4 * wn, lane));
+  AFrag a0, a1;
+  BFrag b0, b1;
+  typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
+  auto lds_frag = [&](uint32_t x, uint32_t src, int kh, int f) {
+    return *(const lds_bf16x8*)(uintptr_t)((x ^ (kh * 64u)) + src + 2048u * f);
+  };
+  auto read_a = [&](AFrag& f, int u, uint32_t src, int kh, int m) { f[kh][m] = lds_frag(xa, src, kh, 2 * u + m); };
+  auto read_b = [&](BFrag& f, int u, uint32_t src, int kh, int n) {
+    if constexpr (SYM) f[kh][n] = lds_frag(xb, src, kh, 4 * u + n);
+    else f[kh][n] = tr_frag(((src + xb) ^ (n << 5)) + u * UNIT + kh * TR_KHALF);
+  };
+  auto read_first = [&](uint32_t src) {
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) read_a(a0, 0, src, kh, m);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) read_b(b0, 0, src, 0, n);
+  };
+
+  issue_a(0, 0);
+  issue_b(0, 0);
+  issue_b(0, 1);
+  issue_a(0, 1);
+  issue_a(1, 0);
+  issue_b(1, 0);
+  issue_b(1, 1);
+  wait_vm_barrier<5 * LU>();
+  read_first(sbase);
+  const bool late = w >= 4;  // this wave's SIMD partner is one phase ahead
+  if (late) barrier();
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float* ep = reinterpret_cast<float*>(smem + 2 * STAGE + w * EPI);  // this wave's staging (4 KB)
+  int e_ti = 0, e_kt = 0;
+  for (int it = 0; it < total; ++it) {
+    // keep the per-step fragment addresses from being hoisted out of the loop
+    asm volatile("" : "+v"(xa), "+v"(xb));
+    const uint32_t st = sbase + (it & 1) * STAGE, nxt = sbase + ((it + 1) & 1) * STAGE;
+    // (0, 0)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) read_b(b0, 0, st, 1, n);
+    issue_a(it + 1, 1);
+    wait_vm_barrier<5 * LU>();  // B1 of this stage
+    ns_quarter<0, 0>(acc, a0, b0);
+    // (0, 1)
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) read_b(b1, 1, st, kh, n);
+    issue_a(it + 2, 0);
+    wait_vm_barrier<5 * LU>();  // A1 of this stage
+    ns_quarter<0, 1>(acc, a0, b1);
+    // (1, 0)
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) read_a(a1, 1, st, kh, m);
+    issue_b(it + 2, 0);
+    wait_vm_barrier<4 * LU>();  // A0, B0 of the next stage
+    ns_quarter<1, 0>(acc, a1, b0);
+    // (1, 1): the next step's first fragments (at a tile's end they are read again after its epilogue)
+    read_first(nxt);
+    issue_b(it + 2, 1);
+    wait_lds_barrier();
+    ns_quarter<1, 1>(acc, a1, b1);
+
+    if (++e_kt < steps) continue;
+    // ---- tile epilogue: this wave's 64 x 128 block (both wave groups together)
+    if (!late) barrier();
+    e_kt = 0;
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3\n" ::: "memory");  // MFMA results -> VALU reads
+    int el = lane;
+    asm volatile("" : "+v"(el));  // the address arithmetic below stays out of the main loop
+    {
+      const NsTile t = locate(b + e_ti * NP);
+      const int row0 = t.ti * BM + wm * WTM, col0 = t.tj * BN + wn * WTN;
+      const int64_t msq = static_cast<int64_t>(t.mat) * a.mp * a.mp, mx = static_cast<int64_t>(t.mat) * a.mp * a.np;
+      const bool tall = (a.tall >> t.mat) & 1;
+      const bool by_columns = SYM ? t.ti != t.tj : (MODE == NS_LAST && tall);
+      void* const dst = MODE == NS_LAST ? a.dst[t.mat] : nullptr;
+      const int lr = el >> 3, lc = (el & 7) * 8;
+      // Rows: 16 x 64 values at a time (chunk c of row r at slot c ^ r)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int jh = 0; jh < 2; ++jh) {
+          auto at = [&](int r, int c) { return reinterpret_cast<f32x4*>(ep + r * 64 + ((c ^ r) & 15) * 4); };
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *at(el & 15, 4 * j + (el >> 4)) = acc[i][4 * jh + j];
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int r = 8 * p + lr, row = row0 + 16 * i + r, col = col0 + 64 * jh + lc;
+            f32x4 lo4 = *at(r, lc >> 2), hi4 = *at(r, (lc >> 2) + 1);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = lo4[e], v[4 + e] = hi4[e];
+            const bool on = row < a.mp && col < (SYM ? a.mp : a.np);
+            const int64_t o = SYM ? msq + static_cast<int64_t>(on ? row : 0) * a.mp + (on ? col : 0)
+                                  : mx + static_cast<int64_t>(on ? row : 0) * a.np + (on ? col : 0);
+            if constexpr (MODE == NS_GRAM) ns_gram8(v);
+            else if constexpr (MODE == NS_POLY) ns_poly8<SPLIT>(a, o, v);
+            else ns_step8(a, cur, o, v);
+            if constexpr (SYM) {
+              if (on) ns_put_parts(MODE == NS_GRAM ? a.ah : a.bh, MODE == NS_GRAM ? a.al : a.bl, o, v, SPLIT);
+            } else if constexpr (MODE == NS_STEP) {
+              if (on) ns_put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
+            } else if (!tall) {
+              const int n = row < a.m ? min(a.n - col, 8) : 0;
+              ns_result8(a, dst, static_cast<int64_t>(row) * a.n + col, n, v, a.lr_wide);
+            }
+            if (by_columns) {
+              *at(r, lc >> 2) = f32x4{v[0], v[1], v[2], v[3]};
+              *at(r, (lc >> 2) + 1) = f32x4{v[4], v[5], v[6], v[7]};
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+          if (by_columns)  // the finished values, back in the accumulators' layout
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][4 * jh + j] = *at(el & 15, 4 * j + (el >> 4));
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      // Columns: 64 x 16 values at a time (chunk c of row r at slot c ^ (r / 2) ^ (r / 8))
+      if (by_columns) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          auto at = [&](int r, int c) { return ep + r * 16 + ((c ^ (r >> 1) ^ (r >> 3)) & 3) * 4; };
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+            *reinterpret_cast<f32x4*>(at(16 * i + (el & 15), el >> 4)) = acc[i][j];
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int c = 8 * p + lr, col = col0 + 16 * j + c, row = row0 + lc;  // rows row .. row + 7
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = at(lc + e, c >> 2)[c & 3];
+            if constexpr (SYM) {
+              if (row < a.mp && col < a.mp)
+                ns_put_parts(MODE == NS_GRAM ? a.ah : a.bh, MODE == NS_GRAM ? a.al : a.bl,
+                             msq + static_cast<int64_t>(col) * a.mp + row, v, SPLIT);
+            } else if constexpr (MODE == NS_LAST) {
+              const int n = col < a.n ? min(a.m - row, 8) : 0;
+              ns_result8(a, dst, static_cast<int64_t>(col) * a.m + row, n, v, a.lr_tall);
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    asm volatile("s_nop 1" ::: "memory");  // VALU writes -> MFMA reads of the accumulators
+    ++e_ti;
+    // the next tile's first fragments (after the last tile a harmless re-read)
+    read_first(sbase + ((it + 1) & 1) * STAGE);
+    if (late && it + 1 < total) barrier();
+  }
+  // the copies past the end have landed before the workgroup's LDS is given back
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -533,6 +866,14 @@ inline void ns_product(const NsArgs& a, int cur, bool split, hipStream_t s) {
     const int64_t r = ceil_div(a.mp, tm);
     return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, 128)) * a.count;
   };
+  const int64_t t256 = sym ? ceil_div(a.mp, 256) * (ceil_div(a.mp, 256) + 1) / 2 * a.count
+                           : ceil_div(a.mp, 256) * ceil_div(a.np, 256) * a.count;
+  if (t256 >= 128) {
+    const dim3 g(static_cast<unsigned>(std::min<int64_t>(t256, kNsCus))), blk(core::NT);
+    if (split) ns_big_kernel<MODE, true><<<g, blk, 0, s>>>(a, cur);
+    else ns_big_kernel<MODE, false><<<g, blk, 0, s>>>(a, cur);
+    return;
+  }
   const bool big = tiles(128) >= 256;
   const dim3 grid(static_cast<unsigned>(8 * ceil_div(tiles(big ? 128 : 64), 8))), block(256);
   if (big) {
