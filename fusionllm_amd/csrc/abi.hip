@@ -19,7 +19,7 @@ extern "C" const char* fmoe_status_string(int status) {
              "use fmoe_dispatch with a workspace";
     case FMOE_ERR_COEFFICIENTS:
       return "Newton-Schulz coefficients whose iterates leave the stored range "
-             "(singular values must stay below 2.8 and |b t + c t^2| below 7.9)";
+             "(singular values must stay below 2.8 and |a + b t + c t^2| below 7.9)";
     default: return "unknown status";
   }
 }

@@ -11,16 +11,18 @@
 // where bf16 carries 8 at the same rate, and the iterates' range is known: singular
 // values of X stay below a bound that the host computes from the coefficients,
 // so X, A and B are stored with the power-of-two factors below and neither
-// overflow nor leave the normal range early.  Sums are fp32 throughout.  X is kept
-// as two fp16 numbers (hi + lo, 22 bits) and a X is formed from both: small
-// singular values are carried by that term (times a per step, some hundredfold
-// over five steps), and what a rounding of X adds to it would grow with them.
-// Rounding X in the other products only acts within the row space that X
-// spans already.  Relative error of the result on gradients of full and low rank
-// (768 x 2048, simulated in 64 bits): bf16 products 1e-2 .. 1.6e-1, fp16 without
-// lo 1.3e-3 .. 1.9e-2, this form 3e-4 .. 1.5e-3 (half a step of a bf16 result: 3.9e-3).
-// fp32 matrices take every operand as hi + lo (three products: hi hi, hi lo, lo hi;
-// relative error 2e-6), and so do matrices of a small side up to kSplitSmall, whose
+// overflow nor leave the normal range early.  Sums are fp32 throughout.
+// A step is X = (a I + B) X: one product, whose rounded operand a I + B costs errors
+// within the row space that X spans already.  A rounding of X would not: small
+// singular values grow by a per step (some hundredfold over five steps), and so would
+// what the rounding adds to them.  So X is kept as two numbers, hi (fp16, the
+// operand) and lo = X - hi (fp8 e4m3), and a lo is added to the step's product in
+// fp32 (not to the last one's, whose result grows no further).  Relative error of
+// the result on gradients of full and low rank (768 x 2048, simulated in 64 bits):
+// bf16 products 1e-2 .. 1.6e-1, fp16 without lo 1.2e-3 .. 4.9e-2, this form
+// 6e-4 .. 1.9e-3 (half a step of a bf16 result: 3.9e-3).
+// fp32 matrices take every operand as hi + lo, both fp16 (three products: hi lo, lo hi,
+// hi hi; relative error 2e-6), and so do matrices of a small side up to kSplitSmall, whose
 // few rounding errors average out less and whose products cost nothing next to
 // the launches.
 //
@@ -45,8 +47,9 @@ constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a m
 constexpr int64_t kSplitSmall = 128;
 constexpr int kNsParts = 64;        // partial sums of squares per matrix, at most (a wave adds them)
 constexpr int kNormChunk = 8192;    // elements per partial sum, at least
-// Stored values: X 2^14, A 2^13, B 2^13 (singular values of X below 2.8, |B| below 7.9).
-constexpr float kXScale = 16384.0f, kAScale = 8192.0f;
+// Stored values: X 2^14, A 2^13, a I + B 2^13 (singular values of X below 2.8, those of a I + B
+// below 7.9), lo of X as fp8 2^4 more: |lo| <= 16 fills e4m3 to 256 of 448.
+constexpr float kXScale = 16384.0f, kAScale = 8192.0f, kLoScale = 16.0f;
 constexpr double kMaxSigma = 2.8, kMaxPoly = 7.9;
 
 struct NsArgs {
@@ -63,10 +66,33 @@ struct NsArgs {
   double eps;
   float ca, cb, cc;         // the polynomial's coefficients
   double* norm;             // [count][parts]
-  // fp16, hi and lo: X [count][mp][np] twice (the step reads one and writes the other; lo of
-  // the second only where the products take it), A and B [count][mp][mp]
+  // fp16, hi and lo: X [count][mp][np] twice (the step reads one and writes the other), A and
+  // B [count][mp][mp]; where operands are hi alone, lo of X is fp8 and there once (each
+  // tile reads and writes its own), and A and B have none
   _Float16 *xh[2], *xl[2], *ah, *al, *bh, *bl;
+  uint8_t* x8;
 };
+
+// lo of X as fp8, 8 elements.
+__device__ __forceinline__ uint2 pack_lo8(const float* l) {
+  int d[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i] * kLoScale, l[4 * i + 1] * kLoScale, 0, false);
+    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i + 2] * kLoScale, l[4 * i + 3] * kLoScale, d[i], true);
+  }
+  return make_uint2(d[0], d[1]);
+}
+__device__ __forceinline__ void unpack_lo8(const uint2& u, float* l) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = static_cast<int>(i == 0 ? u.x : u.y);
+    const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8(d, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(d, true);
+    l[4 * i] = p[0] * (1.0f / kLoScale), l[4 * i + 1] = p[1] * (1.0f / kLoScale);
+    l[4 * i + 2] = q[0] * (1.0f / kLoScale), l[4 * i + 3] = q[1] * (1.0f / kLoScale);
+  }
+}
 
 // ---- the source: elements and the value that is orthogonalised ---------------------
 
@@ -188,15 +214,18 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
   for (int k = 0; k < 2; ++k) {
     const int r = (threadIdx.x >> 3) + 32 * k;
     half8 h, l;
+    float lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float v = tile[r][q + e];
       h[e] = static_cast<_Float16>(v);
-      l[e] = static_cast<_Float16>(v - static_cast<float>(h[e]));
+      lo[e] = v - static_cast<float>(h[e]);
+      l[e] = static_cast<_Float16>(lo[e]);
     }
     const int64_t o = (static_cast<int64_t>(mat) * a.mp + i0 + r) * a.np + j0 + q;
     *reinterpret_cast<half8*>(a.xh[0] + o) = h;
-    *reinterpret_cast<half8*>(a.xl[0] + o) = l;
+    if (a.x8) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(lo);
+    else *reinterpret_cast<half8*>(a.xl[0] + o) = l;
   }
 }
 
@@ -212,76 +241,278 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// The values to store from sums of 8 consecutive elements of a row (offset o in A or X).
-__device__ __forceinline__ void ns_gram8(float* v) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
-}
-template <bool SPLIT>
-__device__ __forceinline__ void ns_poly8(const NsArgs& a, int64_t o, float* v) {  // b A + c A^2
-  const half8 h = *reinterpret_cast<const half8*>(a.ah + o);
-  half8 l = {0, 0, 0, 0, 0, 0, 0, 0};
-  if constexpr (SPLIT) l = *reinterpret_cast<const half8*>(a.al + o);
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e] = fmaf(a.cb, static_cast<float>(h[e]) + static_cast<float>(l[e]), a.cc * (v[e] * (1.0f / kAScale)));
-}
-__device__ __forceinline__ void ns_step8(const NsArgs& a, int cur, int64_t o, float* v) {  // a X + B X
-  const half8 h = *reinterpret_cast<const half8*>(a.xh[cur] + o);
-  const half8 l = *reinterpret_cast<const half8*>(a.xl[cur] + o);
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e] = fmaf(a.ca, static_cast<float>(h[e]) + static_cast<float>(l[e]), v[e] * (1.0f / kAScale));
-}
-__device__ __forceinline__ void ns_put_parts(_Float16* hi, _Float16* lo, int64_t o, const float* v, bool with_lo) {
-  half8 h, l;
+enum NsOut { NS_BF16 = 0, NS_F32 = 1, NS_MUON_BF16 = 2, NS_MUON_F32 = 3 };  // of the last product
+
+// hi and lo of 8 values.
+__device__ __forceinline__ void ns_parts(const float* v, half8& h, float* lo) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     h[e] = static_cast<_Float16>(v[e]);
-    l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+    lo[e] = v[e] - static_cast<float>(h[e]);
   }
-  *reinterpret_cast<half8*>(hi + o) = h;
-  if (with_lo) *reinterpret_cast<half8*>(lo + o) = l;
 }
-// The result: n (up to 8) consecutive elements of the matrix, or of the parameter's update.
-template <int DT>
-__device__ __forceinline__ void ns_finish(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr) {
+__device__ __forceinline__ half8 ns_half8(const float* v) {
+  half8 h;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = static_cast<_Float16>(v[e]);
+  return h;
+}
+
+// The last product's values, n (up to 8) consecutive elements of the matrix: its result, or the
+// parameter's update (p: the parameter's elements, loaded before where all 8 are there).
+template <int OUT>
+__device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr,
+                                           const Raw<OUT & 1, 8>& raw) {
+  constexpr int DT = OUT & 1;
   if (n <= 0) return;
-  if (a.muon) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kXScale);
+  if constexpr (OUT >= NS_MUON_BF16) {
     float p[8];
-    ns_load8<DT>(dst, o, n, p);
+    if (n >= 8) unpack<DT, 8>(raw, p);
+    else ns_load8<DT>(dst, o, n, p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], p[e] * a.decay);
   }
   ns_store8<DT>(dst, o, n, v);
 }
 
-__device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o, int n, float* v, float lr) {
+// Epilogue of a wave's block of 16 FM rows x 16 FN columns (FN a multiple of 4) at (row0, col0) of
+// the padded result: acc[i][j] of lane l holds row 16 i + l % 16, columns 16 j + 4 (l / 16) + 0..3.
+// Every global access is 16 bytes (lo of X: 8) of full lines: the block goes through
+// the wave's 4 KB of LDS, 16 rows x 64 columns at a time, into registers as 8 consecutive
+// elements of a row per lane, and for a transposed store (the mirrored tile of a symmetric product,
+// the result of a tall matrix) once more, as fp16 hi and lo, with transposing reads that
+// return 8 consecutive elements of a column.  What the epilogue reads is asked for first, so
+// that its latency is not paid per slice.  (Epilogues straight from the accumulators, 8 bytes
+// per lane in 16 rows at once, or with the reads slice by slice, took two thirds of a step:
+// 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone.)
+template <int MODE, bool SPLIT, int OUT, int FM, int FN>
+__device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&acc)[FM][FN], uint8_t* ep, int lane,
+                                            int mat, int row0, int col0, bool mirror) {
+  constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+  constexpr bool LO8 = !SPLIT && MODE == NS_STEP;  // a lo, of fp8, is added
+  constexpr int JH = FN / 4;                       // 64-column parts
+  constexpr int SR = FM >= 2 ? 32 : 16;            // rows per transposed slice
+  const int64_t msq = static_cast<int64_t>(mat) * a.mp * a.mp, mx = static_cast<int64_t>(mat) * a.mp * a.np;
+  const int lim = SYM ? a.mp : a.np, ld = lim;
+  const int lr = lane >> 3, lc = (lane & 7) * 8;
+  const bool tall = MODE == NS_LAST && ((a.tall >> mat) & 1);
+  void* const dst = MODE == NS_LAST ? a.dst[mat] : nullptr;
+  // piece (i, jh, p) of this lane: row 16 i + 8 p + lr, columns 64 jh + lc .. + 7
+  auto on = [&](int i, int jh, int p) { return row0 + 16 * i + 8 * p + lr < a.mp && col0 + 64 * jh + lc < lim; };
+  auto offset = [&](int i, int jh, int p) {
+    return (SYM ? msq : mx) + static_cast<int64_t>(row0 + 16 * i + 8 * p + lr) * ld + col0 + 64 * jh + lc;
+  };
+  // A of this block (POLY: a part of it at a time, all would spill), lo of X (STEP)
+  constexpr bool POLY = MODE == NS_POLY;
+  constexpr int H = POLY ? (SPLIT ? 1 : (FM + 1) / 2) : FM;
+  half8 ah[POLY ? H : 1][JH][2], al[POLY && SPLIT ? H : 1][JH][2];
+  uint2 x8[LO8 ? FM : 1][JH][2];
+  auto load_aux = [&](int i0) {
+    if constexpr (POLY || LO8) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kXScale);
-  if (a.dtype == FMOE_BF16) ns_finish<FMOE_BF16>(a, dst, o, n, v, lr);
-  else ns_finish<FMOE_F32>(a, dst, o, n, v, lr);
+      for (int i = 0; i < H; ++i)
+#pragma unroll
+        for (int jh = 0; jh < JH; ++jh)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            if (i0 + i < FM && on(i0 + i, jh, p)) {
+              const int64_t o = offset(i0 + i, jh, p);
+              if constexpr (POLY) ah[i][jh][p] = *reinterpret_cast<const half8*>(a.ah + o);
+              if constexpr (POLY && SPLIT) al[i][jh][p] = *reinterpret_cast<const half8*>(a.al + o);
+              if constexpr (LO8) x8[i][jh][p] = *reinterpret_cast<const uint2*>(a.x8 + o);
+            }
+    }
+  };
+  load_aux(0);
+  // accumulators -> 8 consecutive elements of a row (in the same registers); chunk c of row r at slot c ^ r
+  auto at = [&](int r, int c) { return reinterpret_cast<f32x4*>(ep + r * 256 + ((c ^ r) & 15) * 16); };
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int jh = 0; jh < JH; ++jh) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *at(lane & 15, 4 * j + (lane >> 4)) = acc[i][4 * jh + j];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        acc[i][4 * jh + 2 * p] = *at(8 * p + lr, lc >> 2);
+        acc[i][4 * jh + 2 * p + 1] = *at(8 * p + lr, (lc >> 2) + 1);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  auto value = [&](int i, int jh, int p, float* v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * jh + 2 * p][e], v[4 + e] = acc[i][4 * jh + 2 * p + 1][e];
+    if constexpr (MODE == NS_GRAM) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
+    } else if constexpr (MODE == NS_POLY) {  // a I + b A + c A^2
+      const int d = row0 + 16 * i + 8 * p + lr - (col0 + 64 * jh + lc);  // the diagonal's element
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float x = static_cast<float>(ah[i % H][jh][p][e]);
+        if constexpr (SPLIT) x = x + static_cast<float>(al[i % H][jh][p][e]);
+        v[e] = fmaf(a.cb, x, a.cc * (v[e] * (1.0f / kAScale)));
+        if (d == e) v[e] = v[e] + a.ca * kAScale;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kAScale);
+      if constexpr (LO8) {
+        float l[8];
+        unpack_lo8(x8[i][jh][p], l);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(a.ca, l[e], v[e]);
+      }
+    }
+  };
+  _Float16* const oh = MODE == NS_GRAM ? a.ah : MODE == NS_POLY ? a.bh : a.xh[1 - cur];
+  _Float16* const ol = MODE == NS_GRAM ? a.al : MODE == NS_POLY ? a.bl : a.xl[1 - cur];
+  const bool turn = SYM ? mirror : tall;
+  constexpr bool TURN_LO = SPLIT || MODE == NS_LAST;  // the transposed values need their lo
+  // hi and lo of the pieces, kept in the accumulators' registers for the transposed store
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    if (i > 0 && i % H == 0) load_aux(i);
+    if constexpr (MODE == NS_LAST) {
+      if (!tall) {
+        Raw<OUT & 1, 8> raw[JH][2];
+#pragma unroll
+        for (int jh = 0; jh < JH; ++jh)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int r = row0 + 16 * i + 8 * p + lr, c = col0 + 64 * jh + lc;
+            if (OUT >= NS_MUON_BF16 && r < a.m && c + 8 <= a.n)
+              raw[jh][p] = load_raw<OUT & 1, 8>(dst, static_cast<int64_t>(r) * a.n + c);
+          }
+#pragma unroll
+        for (int jh = 0; jh < JH; ++jh)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int r = row0 + 16 * i + 8 * p + lr, c = col0 + 64 * jh + lc;
+            float v[8];
+            value(i, jh, p, v);
+            ns_result8<OUT>(a, dst, static_cast<int64_t>(r) * a.n + c, r < a.m ? min(a.n - c, 8) : 0, v, a.lr_wide,
+                            raw[jh][p]);
+          }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int jh = 0; jh < JH; ++jh)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float v[8], lo[8];
+        half8 h;
+        value(i, jh, p, v);
+        ns_parts(v, h, lo);
+        if constexpr (MODE != NS_LAST) {
+          if (on(i, jh, p)) {
+            const int64_t o = offset(i, jh, p);
+            *reinterpret_cast<half8*>(oh + o) = h;
+            if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o) = ns_half8(lo);
+            else if constexpr (MODE == NS_STEP) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(lo);
+          }
+        }
+        if constexpr (MODE != NS_STEP) {
+          acc[i][4 * jh + 2 * p] = __builtin_bit_cast(f32x4, h);
+          if constexpr (TURN_LO) acc[i][4 * jh + 2 * p + 1] = __builtin_bit_cast(f32x4, ns_half8(lo));
+        }
+      }
+  }
+  if constexpr (MODE != NS_STEP) {
+    if (!turn) return;
+    // SR rows x 64 columns of fp16: 32-byte window c of row r at window c ^ (r % 4), so that the four rows
+    // of a transposing read fall into different banks; a group of 16 lanes takes 8 rows x 16 columns
+    constexpr int RG = SR / 8, STEPS = RG;  // row groups; windows per group: 4 RG / 4
+    const int g = lane >> 4, sj = (lane >> 2) & 3, sq = lane & 3;
+    const int rg = g % RG, cw0 = g / RG;
+    const uint32_t base = core::lds_addr(ep);
+#pragma unroll
+    for (int i0 = 0; i0 < FM; i0 += SR / 16)
+#pragma unroll
+      for (int jh = 0; jh < JH; ++jh) {
+        half8 t[TURN_LO ? 2 : 1][STEPS];
+#pragma unroll
+        for (int part = 0; part < (TURN_LO ? 2 : 1); ++part) {
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < SR / 16; ++i)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const int r = 16 * i + 8 * p + lr;
+              *reinterpret_cast<f32x4*>(ep + r * 128 + ((((lane & 7) >> 1) ^ (r & 3)) << 5) + ((lane & 1) << 4)) =
+                  acc[i0 + i][4 * jh + 2 * p + part];
+            }
+          __builtin_amdgcn_wave_barrier();
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            const int cw = cw0 + (4 / RG) * k;
+            typedef __attribute__((address_space(3))) core::s16x4 lds_s16x4;
+            const int r = 8 * rg + sj;
+            const uint32_t x = base + r * 128 + ((cw ^ (r & 3)) << 5) + 8 * sq;
+            const core::s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)x);
+            const core::s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(x + 512));
+            t[part][k] = __builtin_bit_cast(half8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+          }
+          __builtin_amdgcn_wave_barrier();
+          asm volatile("" ::: "memory");
+        }
+        Raw<OUT & 1, 8> raw[STEPS];
+        const int row = row0 + 16 * i0 + 8 * rg;  // rows row .. + 7 of column col
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+          const int col = col0 + 64 * jh + 16 * (cw0 + (4 / RG) * k) + (lane & 15);
+          if constexpr (SYM) {
+            if (row < a.mp && col < a.mp) {
+              const int64_t o = msq + static_cast<int64_t>(col) * a.mp + row;
+              *reinterpret_cast<half8*>(oh + o) = t[0][k];
+              if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o) = t[TURN_LO ? 1 : 0][k];
+            }
+          } else if (OUT >= NS_MUON_BF16 && col < a.n && row + 8 <= a.m) {
+            raw[k] = load_raw<OUT & 1, 8>(dst, static_cast<int64_t>(col) * a.m + row);
+          }
+        }
+        if constexpr (MODE == NS_LAST) {
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            const int col = col0 + 64 * jh + 16 * (cw0 + (4 / RG) * k) + (lane & 15);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              v[e] = static_cast<float>(t[0][k][e]) + static_cast<float>(t[TURN_LO ? 1 : 0][k][e]);
+            ns_result8<OUT>(a, dst, static_cast<int64_t>(col) * a.m + row, col < a.n ? min(a.m - row, 8) : 0, v,
+                            a.lr_tall, raw[k]);
+          }
+        }
+      }
+  }
 }
 
-// TM x TN outputs per workgroup of four waves (2 x 2), K in steps of 64 through two LDS stages.
+// TM x TN outputs per workgroup of four waves, K in steps of 64 through two LDS stages.
 // A step reads its whole stage into registers, and the copies (global -> LDS, no registers) of the
 // stage after the next go into its slot while it is multiplied: one to two stages are in
 // flight, and of the two workgroups of a CU one reads LDS while the other multiplies.
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
-template <int MODE, int TM, bool SPLIT>
+template <int MODE, int TM, bool SPLIT, int OUT = NS_BF16>
 __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
   constexpr int TN = SYM ? TM : 128;
-  constexpr int WTM = TM / 2, WTN = TN / 2, FM = WTM / 16, FN = WTN / 16;
+  // 2 x 2 waves; 4 x 1 for 64 x 64 tiles (a wave's columns: 64 for the epilogue)
+  constexpr int WGN = TN / 64, WGM = 4 / WGN;
+  constexpr int WTM = TM / WGM, WTN = 64, FM = WTM / 16, FN = 4;
   constexpr int A_ST = TM * RB, STAGE = A_ST + TN * RB;
   constexpr int CA = TM / 32, CB = TN / 32;  // copies per wave and stage
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = w >> 1, wn = w & 1;
+  const int wm = w / WGN, wn = w % WGN;
   const uint32_t sbase = lds_addr(smem);
 
   // Workgroup b runs on XCD b % 8: each takes a contiguous run of tiles.
@@ -381,105 +612,8 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     __builtin_amdgcn_s_setprio(0);
   }
 
-  // Epilogue: the wave's block goes through its part of LDS as fp32 (16-byte chunk c of row r at
-  // slot c ^ f(r): no bank conflicts by rows or by columns) and comes back as 8 consecutive elements
-  // of a row, or of a column for a transposed store, so that global memory sees 16-byte accesses of
-  // full lines.  (Storing from the accumulators' layout, 8 bytes or less per lane in
-  // 16 rows at once, took as long as the multiplication.)
-  constexpr int MASK = WTN / 4 - 1;
-  static_assert(4 * WTM * WTN * 4 <= 2 * STAGE);
-  float* ep = reinterpret_cast<float*>(smem) + w * (WTM * WTN);
-  auto slot = [](int r, int c) { return r * WTN + ((c ^ ((r & 15) ^ ((r >> 3) & 7))) & MASK) * 4; };
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-      *reinterpret_cast<f32x4*>(ep + slot(16 * i + (lane & 15), 4 * j + (lane >> 4))) = acc[i][j];
-  __builtin_amdgcn_wave_barrier();
-  const int row0 = ti * TM + wm * WTM, col0 = tj * TN + wn * WTN;  // of the wave's block
-  auto by_row = [&](int r, int c, float* v) {  // elements c .. c + 7 of row r
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + slot(r, c >> 2));
-    const f32x4 hi = *reinterpret_cast<const f32x4*>(ep + slot(r, (c >> 2) + 1));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-  };
-  constexpr int LPR = WTN / 8, RPP = 64 / LPR;  // lanes per row, rows per pass
-  constexpr int LPC = WTM / 8, CPP = 64 / LPC;  // the same by columns
-  const int lc = (lane % LPR) * 8, lr = lane / LPR;
-  const int tr = (lane % LPC) * 8, tc = lane / LPC;
-
-  if constexpr (SYM) {
-    _Float16* oh = MODE == NS_GRAM ? a.ah : a.bh;
-    _Float16* ol = MODE == NS_GRAM ? a.al : a.bl;
-    // the value to store, for the element that the wave's sum at this place belongs to
-#pragma unroll
-    for (int p = 0; p < WTM / RPP; ++p) {
-      const int r = p * RPP + lr;
-      float v[8];
-      by_row(r, lc, v);
-      const bool on = row0 + r < a.mp && col0 + lc < a.mp;
-      const int64_t o = msq + static_cast<int64_t>(on ? row0 + r : 0) * a.mp + (on ? col0 + lc : 0);
-      if constexpr (MODE == NS_GRAM) ns_gram8(v);
-      else ns_poly8<SPLIT>(a, o, v);
-      if (on) ns_put_parts(oh, ol, o, v, SPLIT);
-      if (ti != tj) {  // back into LDS for the mirrored tile
-        *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
-      }
-    }
-    if (ti == tj) return;
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int p = 0; p < WTN / CPP; ++p) {
-      const int c = p * CPP + tc;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
-      if (row0 + tr < a.mp && col0 + c < a.mp)
-        ns_put_parts(oh, ol, msq + static_cast<int64_t>(col0 + c) * a.mp + row0 + tr, v, SPLIT);
-    }
-  } else {
-    // X' = a X + B X, X from hi and lo
-#pragma unroll
-    for (int p = 0; p < WTM / RPP; ++p) {
-      const int r = p * RPP + lr;
-      float v[8];
-      by_row(r, lc, v);
-      const bool on = row0 + r < a.mp && col0 + lc < a.np;
-      const int64_t o = mx + static_cast<int64_t>(on ? row0 + r : 0) * a.np + (on ? col0 + lc : 0);
-      ns_step8(a, cur, o, v);
-      if constexpr (MODE == NS_STEP) {
-        if (on) ns_put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
-      } else {
-        *reinterpret_cast<f32x4*>(ep + slot(r, lc >> 2)) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(ep + slot(r, (lc >> 2) + 1)) = f32x4{v[4], v[5], v[6], v[7]};
-      }
-    }
-    if constexpr (MODE == NS_LAST) {
-      __builtin_amdgcn_wave_barrier();
-      void* const dst = a.dst[mat];
-      if ((a.tall >> mat) & 1) {
-#pragma unroll 2
-        for (int p = 0; p < WTN / CPP; ++p) {
-          const int c = p * CPP + tc;
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = ep[slot(tr + e, c >> 2) + (c & 3)];
-          const int n = col0 + c < a.n ? min(a.m - (row0 + tr), 8) : 0;
-          ns_result8(a, dst, static_cast<int64_t>(col0 + c) * a.m + row0 + tr, n, v, a.lr_tall);
-        }
-      } else {
-#pragma unroll 2
-        for (int p = 0; p < WTM / RPP; ++p) {
-          const int r = p * RPP + lr;
-          float v[8];
-          by_row(r, lc, v);
-          const int n = row0 + r < a.m ? min(a.n - (col0 + lc), 8) : 0;
-          ns_result8(a, dst, static_cast<int64_t>(row0 + r) * a.n + col0 + lc, n, v, a.lr_wide);
-        }
-      }
-    }
-  }
+  ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, smem + w * EPI, lane, mat, ti * TM + wm * WTM, tj * TN + wn * WTN,
+                                ti != tj);
 }
 
 // ---- the products in 256 x 256 tiles -------------------------------------------------------
@@ -518,7 +652,7 @@ struct NsTile {
   int mat, ti, tj;
 };
 
-template <int MODE, bool SPLIT>
+template <int MODE, bool SPLIT, int OUT = NS_BF16>
 __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, const int cur) {
   using namespace core;
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
@@ -672,7 +806,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float* ep = reinterpret_cast<float*>(smem + 2 * STAGE + w * EPI);  // this wave's staging (4 KB)
+  uint8_t* ep = smem + 2 * STAGE + w * EPI;  // this wave's staging (4 KB)
   int e_ti = 0, e_kt = 0;
   for (int it = 0; it < total; ++it) {
     // keep the per-step fragment addresses from being hoisted out of the loop
@@ -715,81 +849,8 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
     asm volatile("" : "+v"(el));  // the address arithmetic below stays out of the main loop
     {
       const NsTile t = locate(b + e_ti * NP);
-      const int row0 = t.ti * BM + wm * WTM, col0 = t.tj * BN + wn * WTN;
-      const int64_t msq = static_cast<int64_t>(t.mat) * a.mp * a.mp, mx = static_cast<int64_t>(t.mat) * a.mp * a.np;
-      const bool tall = (a.tall >> t.mat) & 1;
-      const bool by_columns = SYM ? t.ti != t.tj : (MODE == NS_LAST && tall);
-      void* const dst = MODE == NS_LAST ? a.dst[t.mat] : nullptr;
-      const int lr = el >> 3, lc = (el & 7) * 8;
-      // Rows: 16 x 64 values at a time (chunk c of row r at slot c ^ r)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-#pragma unroll
-        for (int jh = 0; jh < 2; ++jh) {
-          auto at = [&](int r, int c) { return reinterpret_cast<f32x4*>(ep + r * 64 + ((c ^ r) & 15) * 4); };
-#pragma unroll
-          for (int j = 0; j < 4; ++j) *at(el & 15, 4 * j + (el >> 4)) = acc[i][4 * jh + j];
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const int r = 8 * p + lr, row = row0 + 16 * i + r, col = col0 + 64 * jh + lc;
-            f32x4 lo4 = *at(r, lc >> 2), hi4 = *at(r, (lc >> 2) + 1);
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = lo4[e], v[4 + e] = hi4[e];
-            const bool on = row < a.mp && col < (SYM ? a.mp : a.np);
-            const int64_t o = SYM ? msq + static_cast<int64_t>(on ? row : 0) * a.mp + (on ? col : 0)
-                                  : mx + static_cast<int64_t>(on ? row : 0) * a.np + (on ? col : 0);
-            if constexpr (MODE == NS_GRAM) ns_gram8(v);
-            else if constexpr (MODE == NS_POLY) ns_poly8<SPLIT>(a, o, v);
-            else ns_step8(a, cur, o, v);
-            if constexpr (SYM) {
-              if (on) ns_put_parts(MODE == NS_GRAM ? a.ah : a.bh, MODE == NS_GRAM ? a.al : a.bl, o, v, SPLIT);
-            } else if constexpr (MODE == NS_STEP) {
-              if (on) ns_put_parts(a.xh[1 - cur], a.xl[1 - cur], o, v, true);
-            } else if (!tall) {
-              const int n = row < a.m ? min(a.n - col, 8) : 0;
-              ns_result8(a, dst, static_cast<int64_t>(row) * a.n + col, n, v, a.lr_wide);
-            }
-            if (by_columns) {
-              *at(r, lc >> 2) = f32x4{v[0], v[1], v[2], v[3]};
-              *at(r, (lc >> 2) + 1) = f32x4{v[4], v[5], v[6], v[7]};
-            }
-          }
-          __builtin_amdgcn_wave_barrier();
-          if (by_columns)  // the finished values, back in the accumulators' layout
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][4 * jh + j] = *at(el & 15, 4 * j + (el >> 4));
-          __builtin_amdgcn_wave_barrier();
-        }
-      }
-      // Columns: 64 x 16 values at a time (chunk c of row r at slot c ^ (r / 2) ^ (r / 8))
-      if (by_columns) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          auto at = [&](int r, int c) { return ep + r * 16 + ((c ^ (r >> 1) ^ (r >> 3)) & 3) * 4; };
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-            *reinterpret_cast<f32x4*>(at(16 * i + (el & 15), el >> 4)) = acc[i][j];
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const int c = 8 * p + lr, col = col0 + 16 * j + c, row = row0 + lc;  // rows row .. row + 7
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = at(lc + e, c >> 2)[c & 3];
-            if constexpr (SYM) {
-              if (row < a.mp && col < a.mp)
-                ns_put_parts(MODE == NS_GRAM ? a.ah : a.bh, MODE == NS_GRAM ? a.al : a.bl,
-                             msq + static_cast<int64_t>(col) * a.mp + row, v, SPLIT);
-            } else if constexpr (MODE == NS_LAST) {
-              const int n = col < a.n ? min(a.m - row, 8) : 0;
-              ns_result8(a, dst, static_cast<int64_t>(col) * a.m + row, n, v, a.lr_tall);
-            }
-          }
-          __builtin_amdgcn_wave_barrier();
-        }
-      }
+      ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, ep, el, t.mat, t.ti * BM + wm * WTM, t.tj * BN + wn * WTN,
+                                    t.ti != t.tj);
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -820,22 +881,23 @@ inline NsLayout ns_layout(int64_t m, int64_t n, int count, bool split) {
   l.norm = (static_cast<size_t>(count) * l.parts * sizeof(double) + 255) / 256 * 256;
   l.x = static_cast<size_t>(count) * ns_pad(m) * ns_pad(n) * 2;
   l.sq = static_cast<size_t>(count) * ns_pad(m) * ns_pad(m) * 2;
-  l.total = l.norm + 4 * l.x + (split ? 4 : 2) * l.sq;
+  // X twice; lo of each where operands are hi + lo, else once and half as wide
+  l.total = l.norm + 2 * l.x + (split ? 2 * l.x : l.x / 2) + (split ? 4 : 2) * l.sq;
   return l;
 }
 
 // Whether the iterates stay within the stored range: the largest singular value after each
-// step, from the polynomial's extrema over [0, s], and the largest |b t + c t^2| over t <= s^2.
+// step, from the polynomial's extrema over [0, s], and the largest |a + b t + c t^2| over t <= s^2.
 inline bool ns_bounded(double a, double b, double c, int steps) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
   double s = 1.0 + 1e-6;
   for (int k = 0; k < steps; ++k) {
     if (!(s < kMaxSigma)) return false;
     const double t1 = s * s;
-    double poly = std::fabs(b * t1 + c * t1 * t1);
+    double poly = std::max(std::fabs(a), std::fabs(a + b * t1 + c * t1 * t1));
     if (c != 0.0) {
       const double t = -b / (2.0 * c);
-      if (t > 0.0 && t < t1) poly = std::max(poly, std::fabs(b * t + c * t * t));
+      if (t > 0.0 && t < t1) poly = std::max(poly, std::fabs(a + b * t + c * t * t));
     }
     if (!(poly < kMaxPoly)) return false;
     auto p = [&](double v) { return std::fabs(v * (a + v * v * (b + c * v * v))); };
@@ -859,29 +921,36 @@ inline bool ns_bounded(double a, double b, double c, int steps) {
   return s < kMaxSigma;
 }
 
+template <int MODE, bool SPLIT, int OUT>
+inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
+  constexpr bool sym = MODE == NS_GRAM || MODE == NS_POLY;
+  auto tiles = [&](int tm, int tn) {
+    const int64_t r = ceil_div(a.mp, tm);
+    return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, tn)) * a.count;
+  };
+  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128);
+  if (t256 >= 128) {
+    ns_big_kernel<MODE, SPLIT, OUT>
+        <<<dim3(static_cast<unsigned>(std::min<int64_t>(t256, kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
+  } else if (t128 >= 256) {
+    ns_product_kernel<MODE, 128, SPLIT, OUT>
+        <<<dim3(static_cast<unsigned>(8 * ceil_div(t128, 8))), dim3(256), 0, s>>>(a, cur);
+  } else {
+    ns_product_kernel<MODE, 64, SPLIT, OUT>
+        <<<dim3(static_cast<unsigned>(8 * ceil_div(tiles(64, 128), 8))), dim3(256), 0, s>>>(a, cur);
+  }
+}
 template <int MODE>
 inline void ns_product(const NsArgs& a, int cur, bool split, hipStream_t s) {
-  constexpr bool sym = MODE == NS_GRAM || MODE == NS_POLY;
-  auto tiles = [&](int tm) {
-    const int64_t r = ceil_div(a.mp, tm);
-    return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, 128)) * a.count;
-  };
-  const int64_t t256 = sym ? ceil_div(a.mp, 256) * (ceil_div(a.mp, 256) + 1) / 2 * a.count
-                           : ceil_div(a.mp, 256) * ceil_div(a.np, 256) * a.count;
-  if (t256 >= 128) {
-    const dim3 g(static_cast<unsigned>(std::min<int64_t>(t256, kNsCus))), blk(core::NT);
-    if (split) ns_big_kernel<MODE, true><<<g, blk, 0, s>>>(a, cur);
-    else ns_big_kernel<MODE, false><<<g, blk, 0, s>>>(a, cur);
-    return;
-  }
-  const bool big = tiles(128) >= 256;
-  const dim3 grid(static_cast<unsigned>(8 * ceil_div(tiles(big ? 128 : 64), 8))), block(256);
-  if (big) {
-    if (split) ns_product_kernel<MODE, 128, true><<<grid, block, 0, s>>>(a, cur);
-    else ns_product_kernel<MODE, 128, false><<<grid, block, 0, s>>>(a, cur);
+  if constexpr (MODE == NS_LAST) {
+    const int out = (a.dtype == FMOE_BF16 ? NS_BF16 : NS_F32) + (a.muon ? 2 : 0);
+    if (out == NS_BF16) split ? ns_launch<MODE, true, NS_BF16>(a, cur, s) : ns_launch<MODE, false, NS_BF16>(a, cur, s);
+    else if (out == NS_MUON_BF16)
+      split ? ns_launch<MODE, true, NS_MUON_BF16>(a, cur, s) : ns_launch<MODE, false, NS_MUON_BF16>(a, cur, s);
+    else if (out == NS_F32) ns_launch<MODE, true, NS_F32>(a, cur, s);  // fp32 matrices are always split
+    else ns_launch<MODE, true, NS_MUON_F32>(a, cur, s);
   } else {
-    if (split) ns_product_kernel<MODE, 64, true><<<grid, block, 0, s>>>(a, cur);
-    else ns_product_kernel<MODE, 64, false><<<grid, block, 0, s>>>(a, cur);
+    split ? ns_launch<MODE, true, NS_BF16>(a, cur, s) : ns_launch<MODE, false, NS_BF16>(a, cur, s);
   }
 }
 
@@ -921,7 +990,9 @@ inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* 
     return q;
   };
   for (int i = 0; i < 2; ++i) a.xh[i] = take(l.x);
-  for (int i = 0; i < 2; ++i) a.xl[i] = take(l.x);
+  if (split)
+    for (int i = 0; i < 2; ++i) a.xl[i] = take(l.x);
+  else a.x8 = reinterpret_cast<uint8_t*>(take(l.x / 2));
   a.ah = take(l.sq);
   a.bh = take(l.sq);
   if (split) a.al = take(l.sq), a.bl = take(l.sq);

@@ -63,11 +63,11 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  *   X = G / max(|G|_F, eps)
  *   steps times:  A = X X^T,  B = coeffs[1] A + coeffs[2] A^2,  X = coeffs[0] X + B X
  * and dst = X in G's own orientation (dst may be G's storage).  The norm is
- * summed in fp64, the products run on fp16 operands with fp32 sums, X held in
- * 22 bits, the result is rounded once, to dtype; for fp32 matrices (and small
+ * summed in fp64, the products run on fp16 operands with fp32 sums, X held as
+ * fp16 and an fp8 remainder, the result is rounded once, to dtype; for fp32 matrices (and small
  * sides up to 128) every operand is held in 22 bits.  A matrix that holds NaN or
  * infinities gives NaN; a zero matrix gives zeros.  Coefficients whose iterates
- * leave the stored range (singular values up to 2.8, |b t + c t^2| up to 7.9)
+ * leave the stored range (singular values up to 2.8, |a + b t + c t^2| up to 7.9)
  * return FMOE_ERR_COEFFICIENTS.  Deterministic.
  * workspace: 256-byte aligned, of the size query's bytes (a pair of sides in
  * either order); calls that share one must not overlap.

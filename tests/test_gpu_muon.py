@@ -1,7 +1,7 @@
 """Orthogonalised updates and the Muon step against their formulas in 64 bits.
 
-Tolerances.  The kernels round to fp16 at stated places (X, A and B; hi + lo where
-an operand is held in 22 bits) and sum in fp32.  ``emulate`` does the same roundings
+Tolerances.  The kernels round to fp16 at stated places (X with an fp8 remainder, A and
+a I + B; hi + lo where an operand is held in 22 bits) and sum in fp32.  ``emulate`` does the same roundings
 in 64 bits, so |emulate - exact| is the error that the scheme makes on this very
 matrix.  The kernel's roundings fall elsewhere in their last place (its sums are
 fp32, in another order), so its error is another draw of the same size: bound 3 x,
@@ -61,11 +61,14 @@ def emulate(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7, split=False, cut=False):
     x = g.double()
     x = x.t().contiguous() if flip else x
     x = x / max(float(x.norm()), eps)
-    for _ in range(steps):
+    eye = torch.eye(x.shape[0], dtype=torch.float64, device=x.device)
+    for k in range(steps):
         xs = parts(x, 14)
         a = parts(mul(xs, tr(xs)), 13)
-        b = parts(co[1] * (a[0] + a[1] if split else a[0]) + co[2] * mul(a, tr(a)), 13)
-        x = co[0] * (xs[0] + xs[1]) + mul(b, xs)
+        b = parts(co[0] * eye + co[1] * (a[0] + a[1] if split else a[0]) + co[2] * mul(a, tr(a)), 13)
+        # the remainder of X, where it is no operand: fp8, and not in the last step
+        lo = ((x - xs[0]) * 2.0 ** 18).float().to(torch.float8_e4m3fn).double() * 2.0 ** -18
+        x = mul(b, xs) + (0 if split or k == steps - 1 else co[0] * lo)
     return x.t() if flip else x
 
 

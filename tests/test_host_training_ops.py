@@ -138,7 +138,7 @@ def test_newton_schulz_argument_errors_without_gpu(call):
     # coefficients: those of the literature's cubic and quintic stay in range, these do not
     assert f(co=(1.5, -0.5, 0.0), steps=20) == 6 and f(co=(2.0, -1.5, 0.5), steps=20) == 6
     assert f(steps=64) == 6
-    assert f(co=(4.0, -4.775, 2.0315)) == 9 and f(co=(3.0, 0.0, 0.0)) == 9 and f(co=(1.0, 9.0, -9.5)) == 9
+    assert f(co=(4.0, -4.775, 2.0315)) == 9 and f(co=(3.0, 0.0, 0.0)) == 9 and f(co=(8.0, -9.0, 1.5)) == 9
     assert f(co=(float("nan"), 0.0, 0.0)) == 9 and f(co=(float("inf"), 0.0, 0.0)) == 9
     assert b"coefficients" in lib.fmoe_status_string(9)
 
@@ -155,7 +155,7 @@ def test_newton_schulz_range_check_covers_the_iterates():
         worst, poly = 1.0, 0.0
         for _ in range(5):
             t = s * s
-            poly = max(poly, np.abs(b * t + c * t * t).max())
+            poly = max(poly, np.abs(a + b * t + c * t * t).max())
             s = np.abs(s * (a + t * (b + c * t)))
             s = np.linspace(0, s.max(), 20001)
             worst = max(worst, s.max())
@@ -173,8 +173,9 @@ def test_newton_schulz_range_check_covers_the_iterates():
 def test_newton_schulz_workspace_size():
     lib = _lib.load()
     q = lib.fmoe_orthogonalize_workspace_bytes
-    # partial sums; X twice as hi and lo; A and B (hi, and lo for fp32 and small sides); sides padded to 64
-    assert q(768, 2048, 3, 0) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (4 * 768 * 2048 + 2 * 768 * 768)
+    # partial sums; X twice, with an fp8 remainder once or (fp32 and small sides) lo twice; A and B with the
+    # same lo; sides padded to 64
+    assert q(768, 2048, 3, 0) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (5 * 768 * 2048 // 2 + 2 * 768 * 768)
     assert q(768, 2048, 3, 1) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (4 * 768 * 2048 + 4 * 768 * 768)
     assert q(2048, 768, 3, 0) == q(768, 2048, 3, 0)
     assert q(5, 70, 1, 0) == 256 + 2 * (4 * 64 * 128 + 4 * 64 * 64)
