@@ -68,8 +68,10 @@ def build_host_module() -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            "-DTORCH_EXTENSION_NAME=_block_host",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{i}" for i in includes], str(CSRC / "block_host.cpp"), "-o", str(tmp),
-           f"-L{libdir}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",  # the current stream's handle: torch's HIP headers
+           *[f"-I{i}" for i in includes], f"-I{Path(HIPCC).resolve().parents[1] / 'include'}",
+           str(CSRC / "block_host.cpp"), "-o", str(tmp),
+           f"-L{libdir}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_hip", "-lc10"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on block_host.cpp:\n{res.stdout}\n{res.stderr}")

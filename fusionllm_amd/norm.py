@@ -52,6 +52,8 @@ def _backward(dy, x, w, mean, rstd, d_residual, need_dx, w_dtype, b_dtype):
 
 
 class _LayerNormFunction(torch.autograd.Function):
+    """The layer norm through the Python wrappers (the native form, csrc/block_host.cpp, runs the same entry points)."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
         with _on_device(x):
@@ -104,12 +106,17 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if torch.compiler.is_compiling():
         # traced (torch.compile): the fusionllm::layer_norm_fwd operator
         y = torch.ops.fusionllm.layer_norm_fwd(flat, weight, bias, float(eps), out_dtype)[0]
-    elif torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                      or (bias is not None and bias.requires_grad)):
-        y = _LayerNormFunction.apply(flat, weight, bias, float(eps), out_dtype)
     else:
-        with _on_device(flat):
-            y = _forward(flat, weight, bias, float(eps), out_dtype, False)[2]
+        grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                            or (bias is not None and bias.requires_grad))
+        host = K.block_host()
+        if host is not None:
+            y = host.layer_norm(flat, weight, bias, eps, out_dtype, grad)
+        elif grad:  # through the wrappers, which time their calls
+            y = _LayerNormFunction.apply(flat, weight, bias, float(eps), out_dtype)
+        else:
+            with _on_device(flat):
+                y = _forward(flat, weight, bias, float(eps), out_dtype, False)[2]
     return y if x.dim() == 2 else y.view(x.shape)
 
 

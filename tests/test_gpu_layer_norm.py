@@ -239,10 +239,15 @@ def test_module_and_autocast(gpu_device):
 
 
 def test_second_derivatives_are_refused(gpu_device):
-    x = torch.randn(3, 64, device=gpu_device, requires_grad=True)
-    (g,) = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    # refused where they are asked for, not before: a graph of the backward may be built around it
+    w = torch.randn(64, device=gpu_device, requires_grad=True)
+    for weight in (None, w):
+        x = torch.randn(3, 64, device=gpu_device, requires_grad=True)
+        (want,) = torch.autograd.grad(layer_norm(x, weight).square().sum(), x)
+        (g,) = torch.autograd.grad(layer_norm(x, weight).square().sum(), x, create_graph=True)
+        assert torch.equal(g, want)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
 
 
 def test_side_stream_and_two_streams(gpu_device):
@@ -370,3 +375,25 @@ def test_moe_residual_of_a_bf16_input_under_autocast_is_the_plain_expression(gpu
         y = moe_residual(x, norm, moe)
         want = x + moe(norm(x))
     assert y.dtype == want.dtype == F32 and torch.equal(y, want)
+
+
+def test_timed_wrappers_give_the_same_bits(gpu_device):
+    # with per-entry-point timing on, the Python form around the same entry points runs
+    x, w, b, dy = inputs(130, 777, BF, F32, gpu_device)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def run():
+        y = layer_norm(*leaves)
+        with torch.no_grad():
+            z = layer_norm(*leaves)
+        return (y.detach(), z, *torch.autograd.grad(y, leaves, dy.to(BF)))
+
+    want = run()
+    store = {}
+    K.set_timer(store)
+    try:
+        got = run()
+    finally:
+        K.set_timer(None)
+    assert set(store) == {"layer_norm_fwd", "layer_norm_bwd"} and len(store["layer_norm_fwd"]) == 2
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
