@@ -71,6 +71,11 @@ struct NsArgs {
   // tile reads and writes its own), and A and B have none
   _Float16 *xh[2], *xl[2], *ah, *al, *bh, *bl;
   uint8_t* x8;
+  // small matrices: X [count][panels][64][128] fp32, partial Gram matrices [2][count][panels][10][256],
+  // and the panels' exponents
+  float *xs, *sparts;
+  int* exps;
+  int panels;
 };
 
 // lo of X as fp8, 8 elements.
@@ -866,6 +871,268 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// ---- matrices of a small side up to 64 ---------------------------------------------------------
+// (router weights): one launch per step instead of three, fp32 operands on
+// v_mfma_f32_16x16x4_f32 (rounding fp32 to fp32 only; the products are small next to the latency of
+// a launch).  A workgroup has 128 columns of X.  It adds the workgroups' partial Gram
+// matrices of the launch before (in a fixed order), forms a I + b A + c A^2 for itself, multiplies
+// its columns and writes the partial Gram matrix of the result for the next launch.  64 x 2048,
+// bf16: three launches a step (28 us of them the Gram matrix's one tile) 190 us.
+
+constexpr int kSmallSide = 64;        // the small side, at most (and the padded one)
+constexpr int kSmallPanel = 128;      // columns per workgroup
+constexpr int kSmallMaxPanels = 32;   // every workgroup adds the partial matrices of all
+constexpr int kSmallBlocks = 10;      // 16 x 16 blocks of a Gram matrix on or below the diagonal
+constexpr int kLdA = 68, kLdX = 132;  // LDS strides
+
+struct SmallLds {
+  float a[kSmallSide * kLdA], b[kSmallSide * kLdA], x[kSmallSide * kLdX];
+  double red[4];
+  int e;
+};
+
+__device__ __forceinline__ f32x4 mfma_f32(float p, float q, f32x4 c) {
+  // D[4 (l / 16) + 0..3][l % 16] += A[l % 16][l / 16] B[l / 16][l % 16] over the lanes l
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(p, q, c, 0, 0, 0);
+}
+// Block (row, column) of the t-th block on or below the diagonal.
+__device__ __forceinline__ void small_block(int t, int& i, int& j) {
+  i = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+  j = t - i * (i + 1) / 2;
+}
+
+// Partial Gram matrix of the panel in LDS: blocks w, w + 4, w + 8 by wave w.
+__device__ __forceinline__ void small_gram(const NsArgs& a, const SmallLds& s, int mat, int panel, int parity) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int mb = (a.m + 15) / 16, cols = min(a.n - panel * kSmallPanel, kSmallPanel);  // zeros after them
+  float* out = a.sparts + ((static_cast<int64_t>(parity) * a.count + mat) * a.panels + panel) * (kSmallBlocks * 256);
+  for (int t = w; t < kSmallBlocks; t += 4) {
+    int i, j;
+    small_block(t, i, j);
+    if (i >= mb) break;  // blocks come in rows
+    const float* p = s.x + (16 * i + (lane & 15)) * kLdX + (lane >> 4);
+    const float* q = s.x + (16 * j + (lane & 15)) * kLdX + (lane >> 4);
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < cols; k0 += 32)
+#pragma unroll
+      for (int k = 0; k < 32; k += 4) c = mfma_f32(p[k0 + k], q[k0 + k], c);
+    *reinterpret_cast<f32x4*>(out + t * 256 + lane * 4) = c;
+  }
+}
+
+// The panel's elements as they lie in the matrix, 8 at a time: F(offset in the matrix, valid elements,
+// row and column of the first in X, whether the 8 go down a column of X).
+template <typename F>
+__device__ __forceinline__ void small_chunks(const NsArgs& a, int mat, int panel, F f) {
+  const int c0 = panel * kSmallPanel;
+  if ((a.tall >> mat) & 1) {
+    const int per = (a.m + 7) / 8;
+    for (int t = threadIdx.x; t < per * kSmallPanel; t += 256) {
+      const int c = t / per, r = (t - c * per) * 8;
+      const int n = c0 + c < a.n ? min(a.m - r, 8) : 0;
+      f(static_cast<int64_t>(c0 + c) * a.m + r, n, r, c, true);
+    }
+  } else {
+    for (int t = threadIdx.x; t < a.m * (kSmallPanel / 8); t += 256) {
+      const int r = t / (kSmallPanel / 8), c = (t % (kSmallPanel / 8)) * 8;
+      f(static_cast<int64_t>(r) * a.n + c0 + c, min(a.n - (c0 + c), 8), r, c, false);
+    }
+  }
+}
+
+// X of the panel, still without the norm (times a power of two that brings the panel's
+// norm to 1/2 .. 1), its sum of squares in fp64 and its partial Gram matrix; Muon: the new momentum.
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void ns_small_load_kernel(const NsArgs a) {
+  __shared__ SmallLds s;
+  const int panel = blockIdx.x, mat = blockIdx.y;
+  for (int t = threadIdx.x; t < kSmallSide * kLdX; t += 256) s.x[t] = 0.0f;
+  __syncthreads();
+  double ss = 0.0;
+  small_chunks(a, mat, panel, [&](int64_t o, int n, int r, int c, bool down) {
+    float u[8];
+    ns_load8<DT>(a.src[mat], o, n, u);
+    if constexpr (MUON) {
+      float v[8];
+      ns_load8<DT>(a.buf[mat], o, n, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = ns_momentum(a, u[i], v[i]);
+        u[i] = ns_update(a, u[i], v[i]);
+      }
+      ns_store8<DT>(a.buf[mat], o, n, v);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) {
+        ss = fma(static_cast<double>(u[i]), static_cast<double>(u[i]), ss);
+        s.x[down ? (r + i) * kLdX + c : r * kLdX + c + i] = u[i];
+      }
+  });
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
+  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = ss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    ss = ((s.red[0] + s.red[1]) + s.red[2]) + s.red[3];
+    int e = 0;
+    if (ss > 0.0 && ss < 1e300) {
+      frexp(sqrt(ss), &e);
+      e = max(-126, min(e, 126));  // 2^-e a normal fp32 number (a panel beyond that stays within 2^15 of 1)
+    }
+    s.e = e;
+    a.norm[mat * a.panels + panel] = ss;
+    a.exps[mat * a.panels + panel] = e;
+  }
+  __syncthreads();
+  const float f = fm_pow2i(-s.e);
+  float* x = a.xs + static_cast<int64_t>(mat) * a.panels * (kSmallSide * kSmallPanel) + panel * (kSmallSide * kSmallPanel);
+  for (int t = threadIdx.x; t < kSmallSide * kSmallPanel; t += 256) {
+    const int r = t / kSmallPanel, c = t % kSmallPanel;
+    const float v = s.x[r * kLdX + c] * f;
+    s.x[r * kLdX + c] = v;
+    x[t] = v;
+  }
+  __syncthreads();
+  small_gram(a, s, mat, panel, 0);
+}
+
+// One step of a panel (step k reads the partial matrices of parity k % 2 and writes the others).
+template <bool LAST, int OUT>
+__global__ __launch_bounds__(256) void ns_small_step_kernel(const NsArgs a, const int k) {
+  __shared__ SmallLds s;
+  const int panel = blockIdx.x, mat = blockIdx.y;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int mb = (a.m + 15) / 16;
+  float* x = a.xs + static_cast<int64_t>(mat) * a.panels * (kSmallSide * kSmallPanel) + panel * (kSmallSide * kSmallPanel);
+  float xv[kSmallSide * kSmallPanel / 256];
+#pragma unroll
+  for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) xv[t] = x[t * 256 + threadIdx.x];
+  // the first step's X and A still lack the norm
+  double inv = 1.0;
+  if (k == 0) {
+    double ss = lane < a.panels ? a.norm[mat * a.panels + lane] : 0.0;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
+    const double nrm = sqrt(ss);
+    inv = 1.0 / (nrm < a.eps ? a.eps : nrm);
+  }
+  auto factor = [&](int p) {  // of panel p: 2^e / |u|
+    return k == 0 ? static_cast<float>(ldexp(inv, a.exps[mat * a.panels + p])) : 1.0f;
+  };
+  // A
+  const float* parts = a.sparts + (static_cast<int64_t>(k & 1) * a.count + mat) * a.panels * (kSmallBlocks * 256);
+  for (int t = w; t < kSmallBlocks; t += 4) {
+    int i, j;
+    small_block(t, i, j);
+    if (i >= mb) break;
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < a.panels; p0 += 8) {
+      f32x4 v[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        v[p] = *reinterpret_cast<const f32x4*>(parts + static_cast<int64_t>(min(p0 + p, a.panels - 1)) * (kSmallBlocks * 256) +
+                                               t * 256 + lane * 4);
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        if (p0 + p < a.panels) {
+          const float f = factor(p0 + p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = c[e] + (v[p][e] * f) * f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 16 * i + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
+      s.a[r * kLdA + q] = c[e];
+      s.a[q * kLdA + r] = c[e];  // (a diagonal block writes the same values twice)
+    }
+  }
+  const float f = factor(panel);
+#pragma unroll
+  for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) {
+    const int q = t * 256 + threadIdx.x;
+    s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel] = xv[t] * f;
+  }
+  __syncthreads();
+  // B = a I + b A + c A^2: rows 16 w .. + 15 by wave w
+  if (w < mb) {
+    f32x4 c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < 16 * mb; q += 4) {
+      const float p = s.a[(16 * w + (lane & 15)) * kLdA + q + (lane >> 4)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < mb) c[j] = mfma_f32(p, s.a[(16 * j + (lane & 15)) * kLdA + q + (lane >> 4)], c[j]);  // A is symmetric
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < mb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 16 * w + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
+          const float v = fmaf(a.cb, s.a[r * kLdA + q], a.cc * c[j][e]);
+          s.b[r * kLdA + q] = r == q ? v + a.ca : v;
+        }
+  }
+  __syncthreads();
+  // X = B X: columns 32 w .. + 31 by wave w (in place after the last read of its own columns)
+  {
+    f32x4 c[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < 16 * mb; q += 4) {
+      float y[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) y[j] = s.x[(q + (lane >> 4)) * kLdX + 32 * w + 16 * j + (lane & 15)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < mb) {
+          const float p = s.b[(16 * i + (lane & 15)) * kLdA + q + (lane >> 4)];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) c[i][j] = mfma_f32(p, y[j], c[i][j]);
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < mb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s.x[(16 * i + 4 * (lane >> 4) + e) * kLdX + 32 * w + 16 * j + (lane & 15)] = c[i][j][e];
+  }
+  __syncthreads();
+  if constexpr (LAST) {
+    small_chunks(a, mat, panel, [&](int64_t o, int n, int r, int c, bool down) {
+      if (n <= 0) return;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? s.x[down ? (r + i) * kLdX + c : r * kLdX + c + i] : 0.0f;
+      if constexpr (OUT >= NS_MUON_BF16) {
+        float p[8];
+        ns_load8<OUT & 1>(a.dst[mat], o, n, p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(down ? -a.lr_tall : -a.lr_wide, v[i], p[i] * a.decay);
+      }
+      ns_store8<OUT & 1>(a.dst[mat], o, n, v);
+    });
+  } else {
+    for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) {
+      const int q = t * 256 + threadIdx.x;
+      x[q] = s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel];
+    }
+    small_gram(a, s, mat, panel, (k + 1) & 1);
+  }
+}
+
+inline int ns_panels(int64_t n) { return static_cast<int>(ceil_div(n, kSmallPanel)); }
+inline bool ns_is_small(int64_t m, int64_t n) { return m <= kSmallSide && ns_panels(n) <= kSmallMaxPanels; }
+
 // ---- host -----------------------------------------------------------------------------------
 
 inline int64_t ns_pad(int64_t v) { return ceil_div(v, kNsPad) * kNsPad; }
@@ -970,16 +1237,58 @@ inline int ns_sizes(const int64_t* rows, const int64_t* cols, int count, NsArgs&
   return static_cast<int64_t>(a.mp) * a.np <= FMOE_MUON_MAX_ELEMENTS ? FMOE_OK : FMOE_ERR_SHAPE;
 }
 
+struct NsSmallLayout {
+  size_t norm, exps, x, parts, total;
+};
+inline NsSmallLayout ns_small_layout(int64_t n, int count) {
+  const size_t panels = static_cast<size_t>(ns_panels(n)) * count;
+  NsSmallLayout l;
+  l.norm = (panels * sizeof(double) + 255) / 256 * 256;
+  l.exps = (panels * sizeof(int) + 255) / 256 * 256;
+  l.x = panels * kSmallSide * kSmallPanel * sizeof(float);
+  l.parts = 2 * panels * kSmallBlocks * 256 * sizeof(float);
+  l.total = l.norm + l.exps + l.x + l.parts;
+  return l;
+}
+
+template <int DT, bool MUON>
+inline int ns_run_small(NsArgs& a, int steps, void* workspace, hipStream_t s) {
+  const NsSmallLayout l = ns_small_layout(a.n, a.count);
+  uint8_t* p = static_cast<uint8_t*>(workspace);
+  a.panels = ns_panels(a.n);
+  a.norm = reinterpret_cast<double*>(p);
+  a.exps = reinterpret_cast<int*>(p + l.norm);
+  a.xs = reinterpret_cast<float*>(p + l.norm + l.exps);
+  a.sparts = reinterpret_cast<float*>(p + l.norm + l.exps + l.x);
+  const dim3 grid(a.panels, a.count), block(256);
+  constexpr int out = DT + (MUON ? 2 : 0);
+  ns_small_load_kernel<DT, MUON><<<grid, block, 0, s>>>(a);
+  for (int k = 0; k + 1 < steps; ++k) ns_small_step_kernel<false, NS_BF16><<<grid, block, 0, s>>>(a, k);
+  ns_small_step_kernel<true, out><<<grid, block, 0, s>>>(a, steps - 1);
+  return launch_status();
+}
+
+inline size_t ns_workspace(int64_t m, int64_t n, int count, int dtype) {
+  return ns_is_small(m, n) ? ns_small_layout(n, count).total : ns_layout(m, n, count, ns_split(m, dtype)).total;
+}
+
 inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* workspace, size_t workspace_bytes,
                   hipStream_t s) {
-  const bool split = ns_split(a.m, a.dtype);
-  const NsLayout l = ns_layout(a.m, a.n, a.count, split);
-  if (!workspace || workspace_bytes < l.total) return FMOE_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < ns_workspace(a.m, a.n, a.count, a.dtype)) return FMOE_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return FMOE_ERR_ALIGN;
   a.ca = static_cast<float>(coeffs[0]);
   a.cb = static_cast<float>(coeffs[1]);
   a.cc = static_cast<float>(coeffs[2]);
   a.eps = eps;
+  if (ns_is_small(a.m, a.n)) {
+    if (a.dtype == FMOE_BF16)
+      return a.muon ? ns_run_small<FMOE_BF16, true>(a, steps, workspace, s)
+                    : ns_run_small<FMOE_BF16, false>(a, steps, workspace, s);
+    return a.muon ? ns_run_small<FMOE_F32, true>(a, steps, workspace, s)
+                  : ns_run_small<FMOE_F32, false>(a, steps, workspace, s);
+  }
+  const bool split = ns_split(a.m, a.dtype);
+  const NsLayout l = ns_layout(a.m, a.n, a.count, split);
   a.parts = l.parts;
   uint8_t* p = static_cast<uint8_t*>(workspace);
   a.norm = reinterpret_cast<double*>(p);
@@ -1029,7 +1338,7 @@ extern "C" size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols,
     return 0;
   const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
   if (ns_pad(m) * ns_pad(n) > FMOE_MUON_MAX_ELEMENTS) return 0;
-  return ns_layout(m, n, n_tensors, ns_split(m, dtype)).total;
+  return ns_workspace(m, n, n_tensors, dtype);
 }
 
 extern "C" int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows, const int64_t* cols,

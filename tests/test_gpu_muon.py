@@ -43,7 +43,15 @@ def exact(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7):
     return x.t() if flip else x
 
 
+def is_small(g):
+    """Whether the fp32 kernels of small matrices run: a side up to 64, 32 panels of 128 columns."""
+    return min(g.shape) <= 64 and max(g.shape) <= 4096
+
+
 def emulate(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7, split=False, cut=False):
+    if is_small(g):
+        return emulate_small(g, steps, co, eps, cut)
+
     def parts(v, scale):
         s = v * 2.0 ** scale
         h = s.half().double()
@@ -69,6 +77,28 @@ def emulate(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7, split=False, cut=False):
         # the remainder of X, where it is no operand: fp8, and not in the last step
         lo = ((x - xs[0]) * 2.0 ** 18).float().to(torch.float8_e4m3fn).double() * 2.0 ** -18
         x = mul(b, xs) + (0 if split or k == steps - 1 else co[0] * lo)
+    return x.t() if flip else x
+
+
+def emulate_small(g, steps, co, eps, cut):
+    """fp32 operands: X, A and a I + b A + c A^2 rounded to fp32.  The sums: a product over K takes K / 4
+    accumulations, the Gram matrix in panels of 128 columns whose sums are added in a chain."""
+    r = lambda v: v.float().double()
+
+    def mul(p, q, panels=0):
+        k = p.shape[1] / 4 if not panels else 32 + panels
+        return p @ q * (1 - k * 2.0 ** -23 if cut else 1)
+
+    flip = g.shape[0] > g.shape[1]
+    x = g.double()
+    x = x.t().contiguous() if flip else x
+    panels = -(-x.shape[1] // 128)
+    x = x / max(float(x.norm()), eps)
+    eye = torch.eye(x.shape[0], dtype=torch.float64, device=x.device)
+    for _ in range(steps):
+        x = r(x)
+        a = r(mul(x, x.t().contiguous(), panels))
+        x = mul(r(co[0] * eye + co[1] * a + co[2] * mul(a, a)), x)
     return x.t() if flip else x
 
 
@@ -107,7 +137,7 @@ def gradient(rows, cols, dev, seed, rank=None, fall=0.5):
 
 
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 3), (8, 768), (64, 64), (63, 65), (65, 64), (5, 200), (128, 130), (129, 129),
-          (130, 700), (257, 191), (300, 301), (512, 512), (768, 2048), (2048, 768), (1001, 1503)]
+          (130, 700), (64, 4096), (4097, 64), (48, 4097), (17, 129), (257, 191), (300, 301), (512, 512), (768, 2048), (2048, 768), (1001, 1503)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
@@ -138,23 +168,28 @@ def test_other_polynomials_and_steps(gpu_device, co, steps):
 def test_scale_of_the_input(gpu_device):
     # values near the ends of the type's range: the norm is summed in fp64; below eps it is eps
     g = gradient(70, 90, gpu_device, 1)
-    for scale in (1e30, 1e-3, 1e-20):
-        x = g * scale
-        check_ortho(orthogonalize(x, eps=1e-30), x, F32, eps=1e-30)
-    x = g * 1e-9
-    check_ortho(orthogonalize(x, eps=1e-3), x, F32, eps=1e-3)
+    for g in (g, gradient(40, 300, gpu_device, 2)):
+        for scale in (1e30, 1e-3, 1e-20):
+            x = g * scale
+            check_ortho(orthogonalize(x, eps=1e-30), x, F32, eps=1e-30)
+        x = g * 1e-9
+        check_ortho(orthogonalize(x, eps=1e-3), x, F32, eps=1e-3)
+        # columns of very different size (panels of a small matrix have factors of their own)
+        x = g * torch.exp2(torch.linspace(-40, 40, g.shape[1], device=gpu_device)).round()
+        check_ortho(orthogonalize(x), x, F32)
 
 
 def test_zero_nan_and_infinite_matrices(gpu_device):
     # in one launch with a clean one, which they leave alone
-    g = gradient(96, 160, gpu_device, 3)
-    stack = torch.stack([g, torch.zeros_like(g), g, g, g])
-    stack[2, 5, 7] = float("nan")
-    stack[3, 95, 159] = float("inf")
-    out = orthogonalize(stack)
-    assert torch.equal(out[0], out[4]) and torch.equal(out[0], orthogonalize(g))
-    assert not out[1].any()
-    assert torch.isnan(out[2]).all() and torch.isnan(out[3]).all()
+    for rows, cols in ((96, 160), (30, 260), (260, 30)):
+        g = gradient(rows, cols, gpu_device, 3)
+        stack = torch.stack([g, torch.zeros_like(g), g, g, g])
+        stack[2, 5, 7] = float("nan")
+        stack[3, rows - 1, cols - 1] = float("inf")
+        out = orthogonalize(stack)
+        assert torch.equal(out[0], out[4]) and torch.equal(out[0], orthogonalize(g))
+        assert not out[1].any()
+        assert torch.isnan(out[2]).all() and torch.isnan(out[3]).all()
 
 
 def test_stacks_lists_and_mixed_sizes(gpu_device):
@@ -190,7 +225,7 @@ def test_many_matrices_take_the_large_tiles(gpu_device):
 
 
 def test_output_is_written_whole_and_nothing_else(gpu_device):
-    for r, c in ((65, 129), (129, 65)):
+    for r, c in ((65, 129), (129, 65), (33, 130), (130, 33)):
         g = gradient(r, c, gpu_device, 2)
         buf = torch.full((r * c + 64,), 7.0, device=gpu_device)
         out = buf[32:32 + r * c].view(r, c)

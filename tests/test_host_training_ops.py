@@ -178,7 +178,10 @@ def test_newton_schulz_workspace_size():
     assert q(768, 2048, 3, 0) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (5 * 768 * 2048 // 2 + 2 * 768 * 768)
     assert q(768, 2048, 3, 1) == (3 * 64 * 8 + 255) // 256 * 256 + 3 * 2 * (4 * 768 * 2048 + 4 * 768 * 768)
     assert q(2048, 768, 3, 0) == q(768, 2048, 3, 0)
-    assert q(5, 70, 1, 0) == 256 + 2 * (4 * 64 * 128 + 4 * 64 * 64)
+    assert q(65, 70, 1, 0) == 256 + 2 * (4 * 128 * 128 + 4 * 128 * 128)
+    # small sides: per panel of 128 columns the norm, the exponent, X and two partial Gram matrices
+    assert q(5, 129, 3, 0) == 256 + 256 + 3 * 2 * 4 * (64 * 128 + 2 * 10 * 256)
+    assert q(64, 4097, 1, 0) > 4 * 2 * 64 * 4096  # 33 panels: the general form
     assert q(0, 5, 1, 0) == q(5, 5, 0, 0) == q(5, 5, 65, 0) == q(65537, 5, 1, 0) == q(32769, 32768, 1, 0) == 0
 
 
