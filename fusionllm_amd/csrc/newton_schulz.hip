@@ -901,232 +901,255 @@ __device__ __forceinline__ void small_block(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// Partial Gram matrix of the panel in LDS: blocks w, w + 4, w + 8 by wave w.
+// Partial Gram matrix of the panel in LDS: blocks w, w + 4, w + 8 by wave w.  MB: 16-row blocks of X.
+template <int MB>
 __device__ __forceinline__ void small_gram(const NsArgs& a, const SmallLds& s, int mat, int panel, int parity) {
+  constexpr int BLOCKS = MB * (MB + 1) / 2, PER = (BLOCKS + 3) / 4;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int mb = (a.m + 15) / 16, cols = min(a.n - panel * kSmallPanel, kSmallPanel);  // zeros after them
+  const int cols = min(a.n - panel * kSmallPanel, kSmallPanel);  // zeros after them
   float* out = a.sparts + ((static_cast<int64_t>(parity) * a.count + mat) * a.panels + panel) * (kSmallBlocks * 256);
-  for (int t = w; t < kSmallBlocks; t += 4) {
-    int i, j;
-    small_block(t, i, j);
-    if (i >= mb) break;  // blocks come in rows
-    const float* p = s.x + (16 * i + (lane & 15)) * kLdX + (lane >> 4);
-    const float* q = s.x + (16 * j + (lane & 15)) * kLdX + (lane >> 4);
-    f32x4 c = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < cols; k0 += 32)
+  const float *p[PER], *q[PER];
+  f32x4 c[PER];
 #pragma unroll
-      for (int k = 0; k < 32; k += 4) c = mfma_f32(p[k0 + k], q[k0 + k], c);
-    *reinterpret_cast<f32x4*>(out + t * 256 + lane * 4) = c;
+  for (int u = 0; u < PER; ++u) {
+    int i, j;
+    small_block(min(w + 4 * u, BLOCKS - 1), i, j);
+    p[u] = s.x + (16 * i + (lane & 15)) * kLdX + (lane >> 4);
+    q[u] = s.x + (16 * j + (lane & 15)) * kLdX + (lane >> 4);
+    c[u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  for (int k0 = 0; k0 < cols; k0 += 32)
+#pragma unroll
+    for (int k = 0; k < 32; k += 4)
+#pragma unroll
+      for (int u = 0; u < PER; ++u) c[u] = mfma_f32(p[u][k0 + k], q[u][k0 + k], c[u]);
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    if (w + 4 * u < BLOCKS) *reinterpret_cast<f32x4*>(out + (w + 4 * u) * 256 + lane * 4) = c[u];
 }
 
-// The panel's elements as they lie in the matrix, 8 at a time: F(offset in the matrix, valid elements,
-// row and column of the first in X, whether the 8 go down a column of X).
-template <typename F>
-__device__ __forceinline__ void small_chunks(const NsArgs& a, int mat, int panel, F f) {
-  const int c0 = panel * kSmallPanel;
-  if ((a.tall >> mat) & 1) {
-    const int per = (a.m + 7) / 8;
-    for (int t = threadIdx.x; t < per * kSmallPanel; t += 256) {
-      const int c = t / per, r = (t - c * per) * 8;
-      const int n = c0 + c < a.n ? min(a.m - r, 8) : 0;
-      f(static_cast<int64_t>(c0 + c) * a.m + r, n, r, c, true);
-    }
-  } else {
-    for (int t = threadIdx.x; t < a.m * (kSmallPanel / 8); t += 256) {
-      const int r = t / (kSmallPanel / 8), c = (t % (kSmallPanel / 8)) * 8;
-      f(static_cast<int64_t>(r) * a.n + c0 + c, min(a.n - (c0 + c), 8), r, c, false);
+// A thread's share of the panel's elements as they lie in the matrix: chunk t of 8 (t < kSmallChunks).
+constexpr int kSmallChunks = kSmallSide * kSmallPanel / 8 / 256;
+struct SmallChunk {
+  int64_t o;       // offset in the matrix
+  int n, r, c;     // valid elements; row and column of X of the first
+  bool down;       // the 8 go down a column of X
+  __device__ __forceinline__ SmallChunk(const NsArgs& a, int mat, int panel, int t) {
+    const int c0 = panel * kSmallPanel, id = t * 256 + threadIdx.x;
+    down = (a.tall >> mat) & 1;
+    if (down) {
+      const int per = (a.m + 7) / 8;
+      c = id / per;
+      r = (id - c * per) * 8;
+      n = c < kSmallPanel && c0 + c < a.n ? min(a.m - r, 8) : 0;
+      o = static_cast<int64_t>(c0 + c) * a.m + r;
+    } else {
+      r = id / (kSmallPanel / 8);
+      c = (id % (kSmallPanel / 8)) * 8;
+      n = r < a.m ? min(a.n - (c0 + c), 8) : 0;
+      o = static_cast<int64_t>(r) * a.n + c0 + c;
     }
   }
-}
+  __device__ __forceinline__ int lds(int i) const { return down ? (r + i) * kLdX + c : r * kLdX + c + i; }
+};
 
 // X of the panel, still without the norm (times a power of two that brings the panel's
 // norm to 1/2 .. 1), its sum of squares in fp64 and its partial Gram matrix; Muon: the new momentum.
-template <int DT, bool MUON>
-__global__ __launch_bounds__(256) void ns_small_load_kernel(const NsArgs a) {
+template <int DT, bool MUON, int MB>
+__global__ __launch_bounds__(256, 2) void ns_small_load_kernel(const NsArgs a) {
   __shared__ SmallLds s;
   const int panel = blockIdx.x, mat = blockIdx.y;
+  float u[kSmallChunks][8], v[MUON ? kSmallChunks : 1][8];
+#pragma unroll
+  for (int t = 0; t < kSmallChunks; ++t) {
+    const SmallChunk k(a, mat, panel, t);
+    ns_load8<DT>(a.src[mat], k.o, k.n, u[t]);
+    if constexpr (MUON) ns_load8<DT>(a.buf[mat], k.o, k.n, v[t]);
+  }
   for (int t = threadIdx.x; t < kSmallSide * kLdX; t += 256) s.x[t] = 0.0f;
-  __syncthreads();
   double ss = 0.0;
-  small_chunks(a, mat, panel, [&](int64_t o, int n, int r, int c, bool down) {
-    float u[8];
-    ns_load8<DT>(a.src[mat], o, n, u);
+#pragma unroll
+  for (int t = 0; t < kSmallChunks; ++t) {
+    const SmallChunk k(a, mat, panel, t);
     if constexpr (MUON) {
-      float v[8];
-      ns_load8<DT>(a.buf[mat], o, n, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = ns_momentum(a, u[i], v[i]);
-        u[i] = ns_update(a, u[i], v[i]);
+        v[t][i] = ns_momentum(a, u[t][i], v[t][i]);
+        u[t][i] = ns_update(a, u[t][i], v[t][i]);
       }
-      ns_store8<DT>(a.buf[mat], o, n, v);
+      if (k.n > 0) ns_store8<DT>(a.buf[mat], k.o, k.n, v[t]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) {
-        ss = fma(static_cast<double>(u[i]), static_cast<double>(u[i]), ss);
-        s.x[down ? (r + i) * kLdX + c : r * kLdX + c + i] = u[i];
-      }
-  });
+      if (i < k.n) ss = fma(static_cast<double>(u[t][i]), static_cast<double>(u[t][i]), ss);
+  }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
   if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = ss;
   __syncthreads();
+  ss = ((s.red[0] + s.red[1]) + s.red[2]) + s.red[3];
+  int e = 0;
+  if (ss > 0.0 && ss < 1e300) {
+    frexp(sqrt(ss), &e);
+    e = max(-126, min(e, 126));  // 2^-e a normal fp32 number (a panel beyond that stays within 2^15 of 1)
+  }
   if (threadIdx.x == 0) {
-    ss = ((s.red[0] + s.red[1]) + s.red[2]) + s.red[3];
-    int e = 0;
-    if (ss > 0.0 && ss < 1e300) {
-      frexp(sqrt(ss), &e);
-      e = max(-126, min(e, 126));  // 2^-e a normal fp32 number (a panel beyond that stays within 2^15 of 1)
-    }
-    s.e = e;
     a.norm[mat * a.panels + panel] = ss;
     a.exps[mat * a.panels + panel] = e;
   }
-  __syncthreads();
-  const float f = fm_pow2i(-s.e);
-  float* x = a.xs + static_cast<int64_t>(mat) * a.panels * (kSmallSide * kSmallPanel) + panel * (kSmallSide * kSmallPanel);
-  for (int t = threadIdx.x; t < kSmallSide * kSmallPanel; t += 256) {
-    const int r = t / kSmallPanel, c = t % kSmallPanel;
-    const float v = s.x[r * kLdX + c] * f;
-    s.x[r * kLdX + c] = v;
-    x[t] = v;
+  const float f = fm_pow2i(-e);
+#pragma unroll
+  for (int t = 0; t < kSmallChunks; ++t) {
+    const SmallChunk k(a, mat, panel, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < k.n) s.x[k.lds(i)] = u[t][i] * f;
   }
   __syncthreads();
-  small_gram(a, s, mat, panel, 0);
+  float* x = a.xs + (static_cast<int64_t>(mat) * a.panels + panel) * (kSmallSide * kSmallPanel);
+#pragma unroll 4
+  for (int t = threadIdx.x; t < 16 * MB * kSmallPanel; t += 256) x[t] = s.x[(t / kSmallPanel) * kLdX + t % kSmallPanel];
+  small_gram<MB>(a, s, mat, panel, 0);
 }
 
 // One step of a panel (step k reads the partial matrices of parity k % 2 and writes the others).
-template <bool LAST, int OUT>
-__global__ __launch_bounds__(256) void ns_small_step_kernel(const NsArgs a, const int k) {
+template <bool LAST, int OUT, int MB>
+__global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, const int k) {
+  constexpr int BLOCKS = MB * (MB + 1) / 2, PER = (BLOCKS + 3) / 4, XV = 16 * MB * kSmallPanel / 256;
+  constexpr int BATCH = 16;  // partial matrices in flight
   __shared__ SmallLds s;
   const int panel = blockIdx.x, mat = blockIdx.y;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int mb = (a.m + 15) / 16;
-  float* x = a.xs + static_cast<int64_t>(mat) * a.panels * (kSmallSide * kSmallPanel) + panel * (kSmallSide * kSmallPanel);
-  float xv[kSmallSide * kSmallPanel / 256];
+  float* x = a.xs + (static_cast<int64_t>(mat) * a.panels + panel) * (kSmallSide * kSmallPanel);
+  float xv[XV];
 #pragma unroll
-  for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) xv[t] = x[t * 256 + threadIdx.x];
-  // the first step's X and A still lack the norm
-  double inv = 1.0;
+  for (int t = 0; t < XV; ++t) xv[t] = x[t * 256 + threadIdx.x];
+  // the first step's X and A still lack the norm: panel p's X the factor 2^e / |u| (lane p has it)
+  float mine = 1.0f;
   if (k == 0) {
     double ss = lane < a.panels ? a.norm[mat * a.panels + lane] : 0.0;
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
     const double nrm = sqrt(ss);
-    inv = 1.0 / (nrm < a.eps ? a.eps : nrm);
+    mine = static_cast<float>(ldexp(1.0 / (nrm < a.eps ? a.eps : nrm), lane < a.panels ? a.exps[mat * a.panels + lane] : 0));
   }
-  auto factor = [&](int p) {  // of panel p: 2^e / |u|
-    return k == 0 ? static_cast<float>(ldexp(inv, a.exps[mat * a.panels + p])) : 1.0f;
-  };
-  // A
+  // A: blocks w, w + 4, w + 8 by wave w, the panels in order
   const float* parts = a.sparts + (static_cast<int64_t>(k & 1) * a.count + mat) * a.panels * (kSmallBlocks * 256);
-  for (int t = w; t < kSmallBlocks; t += 4) {
-    int i, j;
-    small_block(t, i, j);
-    if (i >= mb) break;
-    f32x4 c = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < a.panels; p0 += 8) {
-      f32x4 v[8];
+  f32x4 sum[PER];
 #pragma unroll
-      for (int p = 0; p < 8; ++p)
-        v[p] = *reinterpret_cast<const f32x4*>(parts + static_cast<int64_t>(min(p0 + p, a.panels - 1)) * (kSmallBlocks * 256) +
-                                               t * 256 + lane * 4);
+  for (int u = 0; u < PER; ++u) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < a.panels; p0 += BATCH) {
+    f32x4 v[PER][BATCH];
 #pragma unroll
-      for (int p = 0; p < 8; ++p)
-        if (p0 + p < a.panels) {
-          const float f = factor(p0 + p);
+    for (int p = 0; p < BATCH; ++p)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = c[e] + (v[p][e] * f) * f;
-        }
-    }
+      for (int u = 0; u < PER; ++u)
+        v[u][p] = *reinterpret_cast<const f32x4*>(parts + min(p0 + p, a.panels - 1) * (kSmallBlocks * 256) +
+                                                  min(w + 4 * u, BLOCKS - 1) * 256 + lane * 4);
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 16 * i + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
-      s.a[r * kLdA + q] = c[e];
-      s.a[q * kLdA + r] = c[e];  // (a diagonal block writes the same values twice)
+    for (int p = 0; p < BATCH; ++p) {
+      // a panel past the last adds nothing (its load repeats the last one's)
+      const float g = __shfl(mine, (p0 + p) & 63, 64), f = p0 + p < a.panels ? g : 0.0f;
+#pragma unroll
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[u][e] = sum[u][e] + (v[u][p][e] * f) * f;
     }
   }
-  const float f = factor(panel);
 #pragma unroll
-  for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) {
+  for (int u = 0; u < PER; ++u)
+    if (w + 4 * u < BLOCKS) {
+      int i, j;
+      small_block(w + 4 * u, i, j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * i + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
+        s.a[r * kLdA + q] = sum[u][e];
+        s.a[q * kLdA + r] = sum[u][e];  // (a diagonal block writes the same values twice)
+      }
+    }
+  const float f = __shfl(mine, panel, 64);
+#pragma unroll
+  for (int t = 0; t < XV; ++t) {
     const int q = t * 256 + threadIdx.x;
     s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel] = xv[t] * f;
   }
   __syncthreads();
   // B = a I + b A + c A^2: rows 16 w .. + 15 by wave w
-  if (w < mb) {
-    f32x4 c[4];
+  if (w < MB) {
+    f32x4 c[MB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < 16 * mb; q += 4) {
-      const float p = s.a[(16 * w + (lane & 15)) * kLdA + q + (lane >> 4)];
+    for (int j = 0; j < MB; ++j) c[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* p = s.a + (lane & 15) * kLdA + (lane >> 4);  // (A is symmetric)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < mb) c[j] = mfma_f32(p, s.a[(16 * j + (lane & 15)) * kLdA + q + (lane >> 4)], c[j]);  // A is symmetric
-    }
+    for (int q = 0; q < 16 * MB; q += 4)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < mb)
+      for (int j = 0; j < MB; ++j) c[j] = mfma_f32(p[16 * w * kLdA + q], p[16 * j * kLdA + q], c[j]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 16 * w + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
-          const float v = fmaf(a.cb, s.a[r * kLdA + q], a.cc * c[j][e]);
-          s.b[r * kLdA + q] = r == q ? v + a.ca : v;
-        }
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * w + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
+        const float v = fmaf(a.cb, s.a[r * kLdA + q], a.cc * c[j][e]);
+        s.b[r * kLdA + q] = r == q ? v + a.ca : v;
+      }
   }
   __syncthreads();
   // X = B X: columns 32 w .. + 31 by wave w (in place after the last read of its own columns)
   {
-    f32x4 c[4][2];
+    f32x4 c[MB][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < 16 * mb; q += 4) {
-      float y[2];
+    const float* p = s.b + (lane & 15) * kLdA + (lane >> 4);
+    const float* y = s.x + (lane >> 4) * kLdX + 32 * w + (lane & 15);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) y[j] = s.x[(q + (lane >> 4)) * kLdX + 32 * w + 16 * j + (lane & 15)];
+    for (int q = 0; q < 16 * MB; q += 4)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < mb) {
-          const float p = s.b[(16 * i + (lane & 15)) * kLdA + q + (lane >> 4)];
+      for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) c[i][j] = mfma_f32(p, y[j], c[i][j]);
-        }
-    }
+        for (int j = 0; j < 2; ++j) c[i][j] = mfma_f32(p[16 * i * kLdA + q], y[q * kLdX + 16 * j], c[i][j]);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < mb)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s.x[(16 * i + 4 * (lane >> 4) + e) * kLdX + 32 * w + 16 * j + (lane & 15)] = c[i][j][e];
+        for (int e = 0; e < 4; ++e)
+          s.x[(16 * i + 4 * (lane >> 4) + e) * kLdX + 32 * w + 16 * j + (lane & 15)] = c[i][j][e];
   }
   __syncthreads();
   if constexpr (LAST) {
-    small_chunks(a, mat, panel, [&](int64_t o, int n, int r, int c, bool down) {
-      if (n <= 0) return;
+    constexpr int DT = OUT & 1;
+    constexpr bool MUON = OUT >= NS_MUON_BF16;
+    float p[MUON ? kSmallChunks : 1][8];
+    if constexpr (MUON)
+#pragma unroll
+      for (int t = 0; t < kSmallChunks; ++t) {
+        const SmallChunk q(a, mat, panel, t);
+        ns_load8<DT>(a.dst[mat], q.o, q.n, p[t]);
+      }
+#pragma unroll
+    for (int t = 0; t < kSmallChunks; ++t) {
+      const SmallChunk q(a, mat, panel, t);
+      if (q.n <= 0) continue;
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < n ? s.x[down ? (r + i) * kLdX + c : r * kLdX + c + i] : 0.0f;
-      if constexpr (OUT >= NS_MUON_BF16) {
-        float p[8];
-        ns_load8<OUT & 1>(a.dst[mat], o, n, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(down ? -a.lr_tall : -a.lr_wide, v[i], p[i] * a.decay);
+      for (int i = 0; i < 8; ++i) {
+        v[i] = i < q.n ? s.x[q.lds(i)] : 0.0f;
+        if constexpr (MUON) v[i] = fmaf(q.down ? -a.lr_tall : -a.lr_wide, v[i], p[t][i] * a.decay);
       }
-      ns_store8<OUT & 1>(a.dst[mat], o, n, v);
-    });
+      ns_store8<DT>(a.dst[mat], q.o, q.n, v);
+    }
   } else {
-    for (int t = 0; t < kSmallSide * kSmallPanel / 256; ++t) {
+#pragma unroll 4
+    for (int t = 0; t < XV; ++t) {
       const int q = t * 256 + threadIdx.x;
       x[q] = s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel];
     }
-    small_gram(a, s, mat, panel, (k + 1) & 1);
+    small_gram<MB>(a, s, mat, panel, (k + 1) & 1);
   }
 }
 
@@ -1251,7 +1274,7 @@ inline NsSmallLayout ns_small_layout(int64_t n, int count) {
   return l;
 }
 
-template <int DT, bool MUON>
+template <int DT, bool MUON, int MB>
 inline int ns_run_small(NsArgs& a, int steps, void* workspace, hipStream_t s) {
   const NsSmallLayout l = ns_small_layout(a.n, a.count);
   uint8_t* p = static_cast<uint8_t*>(workspace);
@@ -1262,9 +1285,9 @@ inline int ns_run_small(NsArgs& a, int steps, void* workspace, hipStream_t s) {
   a.sparts = reinterpret_cast<float*>(p + l.norm + l.exps + l.x);
   const dim3 grid(a.panels, a.count), block(256);
   constexpr int out = DT + (MUON ? 2 : 0);
-  ns_small_load_kernel<DT, MUON><<<grid, block, 0, s>>>(a);
-  for (int k = 0; k + 1 < steps; ++k) ns_small_step_kernel<false, NS_BF16><<<grid, block, 0, s>>>(a, k);
-  ns_small_step_kernel<true, out><<<grid, block, 0, s>>>(a, steps - 1);
+  ns_small_load_kernel<DT, MUON, MB><<<grid, block, 0, s>>>(a);
+  for (int k = 0; k + 1 < steps; ++k) ns_small_step_kernel<false, NS_BF16, MB><<<grid, block, 0, s>>>(a, k);
+  ns_small_step_kernel<true, out, MB><<<grid, block, 0, s>>>(a, steps - 1);
   return launch_status();
 }
 
@@ -1281,11 +1304,11 @@ inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* 
   a.cc = static_cast<float>(coeffs[2]);
   a.eps = eps;
   if (ns_is_small(a.m, a.n)) {
-    if (a.dtype == FMOE_BF16)
-      return a.muon ? ns_run_small<FMOE_BF16, true>(a, steps, workspace, s)
-                    : ns_run_small<FMOE_BF16, false>(a, steps, workspace, s);
-    return a.muon ? ns_run_small<FMOE_F32, true>(a, steps, workspace, s)
-                  : ns_run_small<FMOE_F32, false>(a, steps, workspace, s);
+#define FMOE_NS_SMALL(DT, MUON)                                             \
+  (a.m <= 16 ? ns_run_small<DT, MUON, 1>(a, steps, workspace, s) : ns_run_small<DT, MUON, 4>(a, steps, workspace, s))
+    if (a.dtype == FMOE_BF16) return a.muon ? FMOE_NS_SMALL(FMOE_BF16, true) : FMOE_NS_SMALL(FMOE_BF16, false);
+    return a.muon ? FMOE_NS_SMALL(FMOE_F32, true) : FMOE_NS_SMALL(FMOE_F32, false);
+#undef FMOE_NS_SMALL
   }
   const bool split = ns_split(a.m, a.dtype);
   const NsLayout l = ns_layout(a.m, a.n, a.count, split);
