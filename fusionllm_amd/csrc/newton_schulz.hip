@@ -41,6 +41,7 @@ namespace fmoe {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
+#define NS_T128 1000
 constexpr int kNsCus = 256;         // CUs of the chip: workgroups of the persistent products
 constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
 constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
@@ -78,13 +79,16 @@ struct NsArgs {
   int panels;
 };
 
-// lo of X as fp8, 8 elements.
-__device__ __forceinline__ uint2 pack_lo8(const float* l) {
+// lo of X as fp8 (times kLoScale), 8 elements: of values v and their hi; and back, still times kLoScale.
+__device__ __forceinline__ uint2 pack_lo8(const float* v, const half8& h) {
   int d[2];
+  float l[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) l[e] = fmaf(static_cast<float>(h[e]), -kLoScale, v[e] * kLoScale);  // exact
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i] * kLoScale, l[4 * i + 1] * kLoScale, 0, false);
-    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i + 2] * kLoScale, l[4 * i + 3] * kLoScale, d[i], true);
+    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i], l[4 * i + 1], 0, false);
+    d[i] = __builtin_amdgcn_cvt_pk_fp8_f32(l[4 * i + 2], l[4 * i + 3], d[i], true);
   }
   return make_uint2(d[0], d[1]);
 }
@@ -94,8 +98,7 @@ __device__ __forceinline__ void unpack_lo8(const uint2& u, float* l) {
   for (int i = 0; i < 2; ++i) {
     const int d = static_cast<int>(i == 0 ? u.x : u.y);
     const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8(d, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(d, true);
-    l[4 * i] = p[0] * (1.0f / kLoScale), l[4 * i + 1] = p[1] * (1.0f / kLoScale);
-    l[4 * i + 2] = q[0] * (1.0f / kLoScale), l[4 * i + 3] = q[1] * (1.0f / kLoScale);
+    l[4 * i] = p[0], l[4 * i + 1] = p[1], l[4 * i + 2] = q[0], l[4 * i + 3] = q[1];
   }
 }
 
@@ -218,18 +221,17 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = (threadIdx.x >> 3) + 32 * k;
+    float v[8];
     half8 h, l;
-    float lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = tile[r][q + e];
-      h[e] = static_cast<_Float16>(v);
-      lo[e] = v - static_cast<float>(h[e]);
-      l[e] = static_cast<_Float16>(lo[e]);
+      v[e] = tile[r][q + e];
+      h[e] = static_cast<_Float16>(v[e]);
+      l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
     }
     const int64_t o = (static_cast<int64_t>(mat) * a.mp + i0 + r) * a.np + j0 + q;
     *reinterpret_cast<half8*>(a.xh[0] + o) = h;
-    if (a.x8) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(lo);
+    if (a.x8) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(v, h);
     else *reinterpret_cast<half8*>(a.xl[0] + o) = l;
   }
 }
@@ -248,14 +250,6 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
 
 enum NsOut { NS_BF16 = 0, NS_F32 = 1, NS_MUON_BF16 = 2, NS_MUON_F32 = 3 };  // of the last product
 
-// hi and lo of 8 values.
-__device__ __forceinline__ void ns_parts(const float* v, half8& h, float* lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    h[e] = static_cast<_Float16>(v[e]);
-    lo[e] = v[e] - static_cast<float>(h[e]);
-  }
-}
 __device__ __forceinline__ half8 ns_half8(const float* v) {
   half8 h;
 #pragma unroll
@@ -292,24 +286,31 @@ __device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o
 // that its latency is not paid per slice.  (Epilogues straight from the accumulators, 8 bytes
 // per lane in 16 rows at once, or with the reads slice by slice, took two thirds of a step:
 // 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone.)
+//
+// Pieces of 8 elements sit at a uniform address plus one offset per lane, and whether they are inside
+// the padded result is uniform too (its sides, and a block's place, are multiples of 64, or of the
+// block's 16 rows): the vector instructions are what an epilogue takes.
 template <int MODE, bool SPLIT, int OUT, int FM, int FN>
 __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&acc)[FM][FN], uint8_t* ep, int lane,
-                                            int mat, int row0, int col0, bool mirror) {
+                                               int mat, int row0, int col0, bool mirror) {
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
   constexpr bool LO8 = !SPLIT && MODE == NS_STEP;  // a lo, of fp8, is added
   constexpr int JH = FN / 4;                       // 64-column parts
   constexpr int SR = FM >= 2 ? 32 : 16;            // rows per transposed slice
-  const int64_t msq = static_cast<int64_t>(mat) * a.mp * a.mp, mx = static_cast<int64_t>(mat) * a.mp * a.np;
   const int lim = SYM ? a.mp : a.np, ld = lim;
+  const int64_t base = static_cast<int64_t>(mat) * a.mp * lim + static_cast<int64_t>(row0) * ld + col0;
   const int lr = lane >> 3, lc = (lane & 7) * 8;
+  const uint32_t voff = static_cast<uint32_t>(lr * ld + lc);
   const bool tall = MODE == NS_LAST && ((a.tall >> mat) & 1);
   void* const dst = MODE == NS_LAST ? a.dst[mat] : nullptr;
+  static_assert(kNsPad % 64 == 0);
+  if (row0 >= a.mp) return;
   // piece (i, jh, p) of this lane: row 16 i + 8 p + lr, columns 64 jh + lc .. + 7
-  auto on = [&](int i, int jh, int p) { return row0 + 16 * i + 8 * p + lr < a.mp && col0 + 64 * jh + lc < lim; };
-  auto offset = [&](int i, int jh, int p) {
-    return (SYM ? msq : mx) + static_cast<int64_t>(row0 + 16 * i + 8 * p + lr) * ld + col0 + 64 * jh + lc;
+  auto on = [&](int jh) { return col0 + 64 * jh < lim; };
+  auto piece = [&](auto* array, int i, int jh, int p) {
+    return array + (base + static_cast<int64_t>(16 * i + 8 * p) * ld + 64 * jh) + voff;
   };
-  // A of this block (POLY: a part of it at a time, all would spill), lo of X (STEP)
+  // A of this block (POLY; a part of it at a time, all would spill), lo of X (STEP)
   constexpr bool POLY = MODE == NS_POLY;
   constexpr int H = POLY ? (SPLIT ? 1 : (FM + 1) / 2) : FM;
   half8 ah[POLY ? H : 1][JH][2], al[POLY && SPLIT ? H : 1][JH][2];
@@ -322,11 +323,10 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
         for (int jh = 0; jh < JH; ++jh)
 #pragma unroll
           for (int p = 0; p < 2; ++p)
-            if (i0 + i < FM && on(i0 + i, jh, p)) {
-              const int64_t o = offset(i0 + i, jh, p);
-              if constexpr (POLY) ah[i][jh][p] = *reinterpret_cast<const half8*>(a.ah + o);
-              if constexpr (POLY && SPLIT) al[i][jh][p] = *reinterpret_cast<const half8*>(a.al + o);
-              if constexpr (LO8) x8[i][jh][p] = *reinterpret_cast<const uint2*>(a.x8 + o);
+            if (i0 + i < FM && on(jh)) {
+              if constexpr (POLY) ah[i][jh][p] = *reinterpret_cast<const half8*>(piece(a.ah, i0 + i, jh, p));
+              if constexpr (POLY && SPLIT) al[i][jh][p] = *reinterpret_cast<const half8*>(piece(a.al, i0 + i, jh, p));
+              if constexpr (LO8) x8[i][jh][p] = *reinterpret_cast<const uint2*>(piece(a.x8, i0 + i, jh, p));
             }
     }
   };
@@ -354,23 +354,28 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = v[e] * (kAScale / (kXScale * kXScale));
     } else if constexpr (MODE == NS_POLY) {  // a I + b A + c A^2
-      const int d = row0 + 16 * i + 8 * p + lr - (col0 + 64 * jh + lc);  // the diagonal's element
+      const float c = a.cc * (1.0f / kAScale);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float x = static_cast<float>(ah[i % H][jh][p][e]);
         if constexpr (SPLIT) x = x + static_cast<float>(al[i % H][jh][p][e]);
-        v[e] = fmaf(a.cb, x, a.cc * (v[e] * (1.0f / kAScale)));
-        if (d == e) v[e] = v[e] + a.ca * kAScale;
+        v[e] = fmaf(a.cb, x, c * v[e]);
       }
+      if (!mirror) {  // the diagonal is in tiles that have no mirror
+        const int d = row0 + 16 * i + 8 * p + lr - (col0 + 64 * jh + lc);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (d == e) v[e] = v[e] + a.ca * kAScale;
+      }
+    } else if constexpr (LO8) {
+      float l[8];
+      unpack_lo8(x8[i][jh][p], l);
+      const float c = a.ca * (1.0f / kLoScale);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], 1.0f / kAScale, c * l[e]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = v[e] * (1.0f / kAScale);
-      if constexpr (LO8) {
-        float l[8];
-        unpack_lo8(x8[i][jh][p], l);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(a.ca, l[e], v[e]);
-      }
     }
   };
   _Float16* const oh = MODE == NS_GRAM ? a.ah : MODE == NS_POLY ? a.bh : a.xh[1 - cur];
@@ -409,21 +414,24 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
     for (int jh = 0; jh < JH; ++jh)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        float v[8], lo[8];
-        half8 h;
+        float v[8];
         value(i, jh, p, v);
-        ns_parts(v, h, lo);
+        const half8 h = ns_half8(v);
+        half8 l;
+        if constexpr (SPLIT || MODE == NS_LAST) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
+        }
         if constexpr (MODE != NS_LAST) {
-          if (on(i, jh, p)) {
-            const int64_t o = offset(i, jh, p);
-            *reinterpret_cast<half8*>(oh + o) = h;
-            if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o) = ns_half8(lo);
-            else if constexpr (MODE == NS_STEP) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(lo);
+          if (on(jh)) {
+            *reinterpret_cast<half8*>(piece(oh, i, jh, p)) = h;
+            if constexpr (SPLIT) *reinterpret_cast<half8*>(piece(ol, i, jh, p)) = l;
+            else if constexpr (MODE == NS_STEP) *reinterpret_cast<uint2*>(piece(a.x8, i, jh, p)) = pack_lo8(v, h);
           }
         }
         if constexpr (MODE != NS_STEP) {
           acc[i][4 * jh + 2 * p] = __builtin_bit_cast(f32x4, h);
-          if constexpr (TURN_LO) acc[i][4 * jh + 2 * p + 1] = __builtin_bit_cast(f32x4, ns_half8(lo));
+          if constexpr (TURN_LO) acc[i][4 * jh + 2 * p + 1] = __builtin_bit_cast(f32x4, l);
         }
       }
   }
@@ -434,7 +442,9 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
     constexpr int RG = SR / 8, STEPS = RG;  // row groups; windows per group: 4 RG / 4
     const int g = lane >> 4, sj = (lane >> 2) & 3, sq = lane & 3;
     const int rg = g % RG, cw0 = g / RG;
-    const uint32_t base = core::lds_addr(ep);
+    const uint32_t lds = core::lds_addr(ep);
+    const int64_t tbase = static_cast<int64_t>(mat) * a.mp * a.mp + static_cast<int64_t>(col0) * a.mp + row0;
+    const uint32_t tvoff = static_cast<uint32_t>((16 * cw0 + (lane & 15)) * a.mp + 8 * rg);
 #pragma unroll
     for (int i0 = 0; i0 < FM; i0 += SR / 16)
 #pragma unroll
@@ -458,7 +468,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
             const int cw = cw0 + (4 / RG) * k;
             typedef __attribute__((address_space(3))) core::s16x4 lds_s16x4;
             const int r = 8 * rg + sj;
-            const uint32_t x = base + r * 128 + ((cw ^ (r & 3)) << 5) + 8 * sq;
+            const uint32_t x = lds + r * 128 + ((cw ^ (r & 3)) << 5) + 8 * sq;
             const core::s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)x);
             const core::s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(x + 512));
             t[part][k] = __builtin_bit_cast(half8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -472,10 +482,10 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
         for (int k = 0; k < STEPS; ++k) {
           const int col = col0 + 64 * jh + 16 * (cw0 + (4 / RG) * k) + (lane & 15);
           if constexpr (SYM) {
-            if (row < a.mp && col < a.mp) {
-              const int64_t o = msq + static_cast<int64_t>(col) * a.mp + row;
-              *reinterpret_cast<half8*>(oh + o) = t[0][k];
-              if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o) = t[TURN_LO ? 1 : 0][k];
+            if (on(jh)) {
+              const int64_t o = tbase + static_cast<int64_t>(64 * jh + 16 * (4 / RG) * k) * a.mp + 16 * i0;
+              *reinterpret_cast<half8*>(oh + o + tvoff) = t[0][k];
+              if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o + tvoff) = t[TURN_LO ? 1 : 0][k];
             }
           } else if (OUT >= NS_MUON_BF16 && col < a.n && row + 8 <= a.m) {
             raw[k] = load_raw<OUT & 1, 8>(dst, static_cast<int64_t>(col) * a.m + row);
@@ -497,15 +507,15 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
   }
 }
 
-// TM x TN outputs per workgroup of four waves, K in steps of 64 through two LDS stages.
+// TM x TN outputs per workgroup of four waves, K in steps of 64 through NST LDS stages.
 // A step reads its whole stage into registers, and the copies (global -> LDS, no registers) of the
-// stage after the next go into its slot while it is multiplied: one to two stages are in
-// flight, and of the two workgroups of a CU one reads LDS while the other multiplies.
+// stage NST steps on go into its slot while it is multiplied: NST - 1 to NST stages are in
+// flight, and of the workgroups of a CU one reads LDS while another multiplies.
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
-template <int MODE, int TM, bool SPLIT, int OUT = NS_BF16>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
+template <int MODE, int TM, int NST, bool SPLIT, int OUT = NS_BF16>
+__global__ __launch_bounds__(256, NST * TM <= 256 ? 2 : 1) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
   constexpr int TN = SYM ? TM : 128;
@@ -514,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   constexpr int WTM = TM / WGM, WTN = 64, FM = WTM / 16, FN = 4;
   constexpr int A_ST = TM * RB, STAGE = A_ST + TN * RB;
   constexpr int CA = TM / 32, CB = TN / 32;  // copies per wave and stage
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NST * STAGE];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / WGN, wn = w % WGN;
@@ -561,13 +571,16 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   // SPLIT: hi lo, lo hi, then hi hi, so that the small terms are summed while the sum is small
   const uint8_t *pa = reinterpret_cast<const uint8_t*>(ph), *pb = reinterpret_cast<const uint8_t*>(SPLIT ? ql : qh);
   const int64_t bstep = SYM ? RB : static_cast<int64_t>(BK) * ldb * 2;
-  int kt = 0, seg = 0;
+  int kt = 0, seg = 0, left = steps;
+  // the next stage's copies; past the last step the last stage again (into a slot that is free and
+  // not read any more), so that every wait counts the same operations
   auto issue = [&](int st) __attribute__((always_inline)) {
     const uint32_t la = sbase + st * STAGE + w * 1024, lb = la + A_ST;
 #pragma unroll
     for (int q = 0; q < CA; ++q) copy16(la + q * 4096, pa, aoff[q]);
 #pragma unroll
     for (int q = 0; q < CB; ++q) copy16(lb + q * 4096, pb, boff[q]);
+    if (--left <= 0) return;
     pa += RB;
     pb += bstep;
     if (SPLIT && ++kt == nk) {
@@ -586,13 +599,12 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   const uint32_t xa = frag_base(wm * WTM, lane);
   const uint32_t xb = A_ST + (SYM ? frag_base(wn * WTN, lane) : tr_base(4 * wn, lane));
   typedef __attribute__((address_space(3))) half8 lds_half8;
-  issue(0);
-  if (steps > 1) issue(1);
+#pragma unroll
+  for (int st = 0; st < NST; ++st) issue(st);
+  int slot = 0;
   for (int it = 0; it < steps; ++it) {
-    // this stage is there (the next may be in flight)
-    if (it + 1 < steps) wait_vm_barrier<CA + CB>();
-    else wait_vm_barrier<0>();
-    const uint32_t src = sbase + (it & 1) * STAGE;
+    wait_vm_barrier<(NST - 1) * (CA + CB)>();  // this stage is there
+    const uint32_t src = sbase + slot * STAGE;
     half8 fa[2][FM], fb[2][FN];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
@@ -605,7 +617,8 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
       }
     }
     wait_lds_barrier();  // every wave has this stage in registers: its slot takes the stage after the next
-    if (it + 2 < steps) issue(it & 1);
+    issue(slot);
+    slot = slot + 1 == NST ? 0 : slot + 1;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -617,6 +630,7 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     __builtin_amdgcn_s_setprio(0);
   }
 
+  wait_vm_barrier<0>();  // the copies past the end have landed: the epilogue takes their LDS
   ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, smem + w * EPI, lane, mat, ti * TM + wm * WTM, tj * TN + wn * WTN,
                                 ti != tj);
 }
@@ -1218,16 +1232,17 @@ inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
     const int64_t r = ceil_div(a.mp, tm);
     return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, tn)) * a.count;
   };
-  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128);
+  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 128);
+  auto grid = [](int64_t t) { return dim3(static_cast<unsigned>(8 * ceil_div(t, 8))); };
   if (t256 >= 128) {
     ns_big_kernel<MODE, SPLIT, OUT>
         <<<dim3(static_cast<unsigned>(std::min<int64_t>(t256, kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
   } else if (t128 >= 256) {
-    ns_product_kernel<MODE, 128, SPLIT, OUT>
-        <<<dim3(static_cast<unsigned>(8 * ceil_div(t128, 8))), dim3(256), 0, s>>>(a, cur);
+    ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
+  } else if (t128 >= NS_T128) {
+    ns_product_kernel<MODE, 128, 4, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
   } else {
-    ns_product_kernel<MODE, 64, SPLIT, OUT>
-        <<<dim3(static_cast<unsigned>(8 * ceil_div(tiles(64, 128), 8))), dim3(256), 0, s>>>(a, cur);
+    ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<grid(t64), dim3(256), 0, s>>>(a, cur);
   }
 }
 template <int MODE>
