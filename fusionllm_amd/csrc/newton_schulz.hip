@@ -42,7 +42,7 @@ namespace fmoe {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
 #define NS_T128 1000
-constexpr int kNsCus = 256;         // CUs of the chip: workgroups of the persistent products
+constexpr int kNsCus = 256;         // CUs of the chip (a multiple of its 8 XCDs): workgroups of the persistent products
 constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
 constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
 constexpr int64_t kSplitSmall = 128;
@@ -683,10 +683,13 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
   const int tiles_m = (a.mp + BM - 1) / BM, tiles_n = SYM ? tiles_m : (a.np + BN - 1) / BN;
   const int per = SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
   const int items = per * a.count;
-  // Workgroup b runs on XCD b % 8: its XCD takes a contiguous run of each round's tiles.
-  const int NP = static_cast<int>(gridDim.x), bid = static_cast<int>(blockIdx.x);
-  const int b = NP % 8 == 0 ? (bid % 8) * (NP / 8) + bid / 8 : bid;
-  const int my_items = (items - b + NP - 1) / NP;
+  // Workgroup b runs on XCD b % 8.  Each XCD takes an eighth of the tiles, a contiguous run (few
+  // matrices per L2), and its workgroups take them in turn: every XCD writes as much in every
+  // round.  (With runs per round the tiles of a last, partial round fell on few XCDs.)
+  const int xcd = static_cast<int>(blockIdx.x) % 8, step = static_cast<int>(gridDim.x) / 8;
+  const int first = static_cast<int>(static_cast<int64_t>(items) * xcd / 8) + static_cast<int>(blockIdx.x) / 8;
+  const int end = static_cast<int>(static_cast<int64_t>(items) * (xcd + 1) / 8);
+  const int my_items = (end - first + step - 1) / step;
   if (my_items <= 0) return;
   const int K = MODE == NS_GRAM ? a.np : a.mp;
   const int ld = K, ldb = SYM ? K : a.np;
@@ -731,7 +734,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
     c_b = reinterpret_cast<const uint8_t*>(SYM ? q + static_cast<int64_t>(t.tj) * BN * ld : q);
   };
   auto copy_tile = [&](int ti) __attribute__((always_inline)) {
-    const NsTile t = locate(b + ti * NP);
+    const NsTile t = locate(first + ti * step);
     c_seg = 0;
     bases(t);
     // the lane as an opaque value: what follows is formed here, not kept through the main loop
@@ -768,7 +771,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
       if (SPLIT && c_seg < 2) {
         c_kt = 0;
         ++c_seg;
-        bases(locate(b + c_ti * NP));
+        bases(locate(first + c_ti * step));
       } else if (c_ti + 1 < my_items) {
         c_kt = 0;
         copy_tile(++c_ti);
@@ -867,7 +870,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
     int el = lane;
     asm volatile("" : "+v"(el));  // the address arithmetic below stays out of the main loop
     {
-      const NsTile t = locate(b + e_ti * NP);
+      const NsTile t = locate(first + e_ti * step);
       ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, ep, el, t.mat, t.ti * BM + wm * WTM, t.tj * BN + wn * WTN,
                                     t.ti != t.tj);
     }
@@ -1236,7 +1239,7 @@ inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
   auto grid = [](int64_t t) { return dim3(static_cast<unsigned>(8 * ceil_div(t, 8))); };
   if (t256 >= 128) {
     ns_big_kernel<MODE, SPLIT, OUT>
-        <<<dim3(static_cast<unsigned>(std::min<int64_t>(t256, kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
+        <<<dim3(static_cast<unsigned>(std::min<int64_t>(8 * ceil_div(t256, 8), kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
   } else if (t128 >= 256) {
     ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
   } else if (t128 >= NS_T128) {
