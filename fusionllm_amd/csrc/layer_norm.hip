@@ -30,10 +30,15 @@
 namespace fmoe {
 
 constexpr int kLnMaxWaves = 16;   // waves per row
-constexpr int kLnMaxChunks = 2;   // chunks per lane
+// Chunks per lane, at most: 2; up to 4 in the forward of fp32 rows that one wave then holds (no barrier
+// between the waves of a row: 32768 x 2048 113 -> 102 us, 16384 x 1500 45 -> 41; longer rows over half the waves
+// 8192 x 4096 57 -> 60, 4000 x 10240 75 -> 85; bf16 16384 x 2048 34 -> 36).
+constexpr int kLnMaxChunks = 2, kLnMaxChunksOneWave = 4;
 constexpr int kLnRowsPerGroup = 4;  // rows a workgroup works on at once where a wave holds a row
-// Workgroups of the backward: 16 waves for each of the 256 CUs.
-constexpr int kLnWaves = 256 * 16;
+// Waves of the backward's launch: 8 for each of the 256 CUs, whose partial rows cost half as much as
+// 16 (32768 x 2048 fp32 159 against 171 us with their reduction, 4099 x 1023 bf16 15 against 19); 16 for
+// bf16 rows where each still gets 16 of them (65536 x 768: 62 against 66 us).
+constexpr int kLnWaves = 256 * 8, kLnManyRows = 16;
 
 static_assert(kLnMaxWaves * 64 * 8 * kLnMaxChunks == FMOE_LAYER_NORM_MAX_DIM);
 
@@ -290,20 +295,22 @@ __global__ __launch_bounds__(kLnReduceWaves * 64) void layer_norm_reduce_kernel(
 }
 
 // How a row is spread: the fewest waves that hold it with at most kLnMaxChunks
-// chunks per lane, and the chunks that takes.
+// chunks per lane (one_wave: one wave where kLnMaxChunksOneWave suffice), and the chunks that takes.
 struct LnShape {
   int vec, waves, nch;
 };
-inline LnShape ln_shape(int64_t dim) {
+inline LnShape ln_shape(int64_t dim, bool one_wave = false) {
   if (dim < 8) return {1, 1, 1};
   const int64_t chunks = ceil_div(dim, 8);
+  if (one_wave && chunks <= 64 * kLnMaxChunksOneWave) return {8, 1, static_cast<int>(ceil_div(chunks, 64))};
   const int waves = static_cast<int>(ceil_div(chunks, 64 * kLnMaxChunks));
   return {8, waves, static_cast<int>(ceil_div(chunks, 64 * waves))};
 }
 inline int ln_rows(const LnShape& s) { return s.waves == 1 ? kLnRowsPerGroup : 1; }
 inline int ln_threads(const LnShape& s) { return 64 * (s.waves == 1 ? kLnRowsPerGroup : s.waves); }
-inline int64_t ln_bwd_groups(int64_t T, const LnShape& s) {
-  return std::min<int64_t>(ceil_div(T, ln_rows(s)), kLnWaves * 64 / ln_threads(s));
+inline int64_t ln_bwd_groups(int64_t T, const LnShape& s, int x_dtype) {
+  const int64_t many = x_dtype == FMOE_BF16 && T * s.waves >= int64_t(kLnManyRows) * 2 * kLnWaves ? 2 : 1;
+  return std::min<int64_t>(ceil_div(T, ln_rows(s)), many * kLnWaves * 64 / ln_threads(s));
 }
 
 inline bool ln_dtype(int d) { return d == FMOE_BF16 || d == FMOE_F32; }
@@ -326,6 +333,12 @@ using namespace fmoe;
     else if ((s).nch == 1) F(8, 1);   \
     else F(8, 2);                     \
   } while (0)
+#define FMOE_LN_SHAPES_F32(s, F)      \
+  do {                                \
+    if ((s).nch == 3) F(8, 3);        \
+    else if ((s).nch == 4) F(8, 4);   \
+    else FMOE_LN_SHAPES(s, F);        \
+  } while (0)
 
 extern "C" int fmoe_layer_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* weight, const void* bias,
                                    int w_dtype, int64_t T, int64_t dim, float eps, void* y, int y_dtype, float* mean,
@@ -338,7 +351,7 @@ extern "C" int fmoe_layer_norm_fwd(const void* x, int x_dtype, int64_t ldx, cons
   if (!ln_aligned(x, x_dtype) || !ln_aligned(y, y_dtype) || !ln_aligned(weight, w_dtype) ||
       !ln_aligned(bias, w_dtype) || !ln_aligned(mean, FMOE_F32) || !ln_aligned(rstd, FMOE_F32))
     return FMOE_ERR_ALIGN;
-  const LnShape s = ln_shape(dim);
+  const LnShape s = ln_shape(dim, x_dtype == FMOE_F32);
   const dim3 grid(ceil_div(T, ln_rows(s))), block(ln_threads(s));
   hipStream_t st = as_stream(stream);
 #define FMOE_LN_FWD(XT, YT, V, N)                                                                                   \
@@ -350,14 +363,14 @@ extern "C" int fmoe_layer_norm_fwd(const void* x, int x_dtype, int64_t ldx, cons
 #define FMOE_LN_FWD_FF(V, N) FMOE_LN_FWD(FMOE_F32, FMOE_F32, V, N)
   if (x_dtype == FMOE_BF16 && y_dtype == FMOE_BF16) FMOE_LN_SHAPES(s, FMOE_LN_FWD_BB);
   else if (x_dtype == FMOE_BF16) FMOE_LN_SHAPES(s, FMOE_LN_FWD_BF);
-  else if (y_dtype == FMOE_BF16) FMOE_LN_SHAPES(s, FMOE_LN_FWD_FB);
-  else FMOE_LN_SHAPES(s, FMOE_LN_FWD_FF);
+  else if (y_dtype == FMOE_BF16) FMOE_LN_SHAPES_F32(s, FMOE_LN_FWD_FB);
+  else FMOE_LN_SHAPES_F32(s, FMOE_LN_FWD_FF);
   return launch_status();
 }
 
 extern "C" size_t fmoe_layer_norm_bwd_workspace_bytes(int64_t T, int64_t dim) {
   if (T <= 0 || dim <= 0 || dim > FMOE_LAYER_NORM_MAX_DIM) return 0;
-  return static_cast<size_t>(ln_bwd_groups(T, ln_shape(dim))) * 2 * static_cast<size_t>(dim) * sizeof(float);
+  return static_cast<size_t>(ln_bwd_groups(T, ln_shape(dim), FMOE_BF16)) * 2 * static_cast<size_t>(dim) * sizeof(float);
 }
 
 extern "C" int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* x, int x_dtype, int64_t ldx,
@@ -382,7 +395,7 @@ extern "C" int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, c
         !ln_aligned(rstd, FMOE_F32) || !ln_aligned(weight, w_dtype) || !ln_aligned(d_residual, x_dtype) ||
         !ln_aligned(dx, x_dtype) || (vectors && !ln_aligned(workspace, FMOE_F32)))
       return FMOE_ERR_ALIGN;
-    groups = static_cast<int>(ln_bwd_groups(T, s));
+    groups = static_cast<int>(ln_bwd_groups(T, s, x_dtype));
     const dim3 grid(groups), block(ln_threads(s));
     float* parts = vectors ? static_cast<float*>(workspace) : nullptr;
 #define FMOE_LN_BWD(XT, DT, V, N)                                                                              \

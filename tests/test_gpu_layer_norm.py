@@ -61,8 +61,9 @@ def truth(x, w, b, dy, eps):
     g = dy * w
     m = lambda t: t.mean(-1, keepdim=True)
     dx = r * (g - m(g) - xh * m(g * xh))
-    groups = 1024 if T > 4096 else max(1, T)
-    chain = T // groups + 4 + groups // 16 + 16 + 16
+    # rows per wave where there are fewer waves than rows (at least 128 workgroups of the longest
+    # rows, 512 of four rows), or the fewer additions of a larger launch
+    chain = T // 128 + 4 + 1024 // 16 + 16
     tol = {"y": w.abs() * E + N * ((xh * w).abs() + b.abs()),
            "dx": N * r * (g.abs() + m(g.abs()) + xh.abs() * m((g * xh).abs()))
            + r * (E * m((g * xh).abs()) + xh.abs() * m(g.abs() * E)) + N * dx.abs(),
@@ -100,10 +101,12 @@ def test_forward_and_backward_against_64_bits(gpu_device, T, dim, xd, wd):
         assert torch.equal(layer_norm(x, w, b, eps), y)
 
 
-@pytest.mark.parametrize("T,dim", [(5000, 768), (4097, 2048), (9001, 65)])
-def test_many_rows(gpu_device, T, dim):
-    # more rows than the backward's launch has waves: each adds several
-    x, w, b, dy = inputs(T, dim, BF, F32, gpu_device, seed=4)
+@pytest.mark.parametrize("T,dim,xd", [(5000, 768, BF), (4097, 2048, F32), (9001, 65, BF), (66001, 40, BF),
+                                      (65600, 24, F32), (3000, 2051, F32)])
+def test_many_rows(gpu_device, T, dim, xd):
+    # more rows than the backward's launch has waves (and, for bf16, enough for the larger launch): each adds several
+    x, w, b, dy = inputs(T, dim, xd, F32, gpu_device, seed=4)
+    BF = xd
     for p in (x, w, b):
         p.requires_grad_(True)
     y = layer_norm(x, w, b)

@@ -48,8 +48,10 @@ def test_layer_norm_argument_errors_without_gpu():
     assert bwd(dx=FAKE + 2) == 3 and bwd(dw=FAKE + 2) == 3 and bwd(db=FAKE + 1) == 3 and bwd(ws=FAKE + 2) == 3
     assert bwd(res=FAKE + 2) == 3 and bwd(m=FAKE + 1) == 3
     assert bwd(dx=None, dw=None, db=None) == 0  # nothing wanted
-    # one partial row pair per workgroup: 4 rows each below dim 1025, at most 4096 waves in all
+    # one partial row pair per workgroup: 4 rows each below dim 1025, at most 2048 waves in all (4096
+    # where each has 16 rows)
     assert lib.fmoe_layer_norm_bwd_workspace_bytes(4, 64) == 2 * 64 * 4
+    assert lib.fmoe_layer_norm_bwd_workspace_bytes(1 << 15, 768) == 512 * 2 * 768 * 4
     assert lib.fmoe_layer_norm_bwd_workspace_bytes(1 << 20, 768) == 1024 * 2 * 768 * 4
     assert lib.fmoe_layer_norm_bwd_workspace_bytes(1 << 20, 16384) == 256 * 2 * 16384 * 4
     assert lib.fmoe_layer_norm_bwd_workspace_bytes(0, 64) == lib.fmoe_layer_norm_bwd_workspace_bytes(4, 0) == 0
