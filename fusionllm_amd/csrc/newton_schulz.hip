@@ -41,7 +41,6 @@ namespace fmoe {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
-#define NS_T128 1000
 constexpr int kNsCus = 256;         // CUs of the chip (a multiple of its 8 XCDs): workgroups of the persistent products
 constexpr int kNsMax = FMOE_MUON_MAX_TENSORS;
 constexpr int kNsPad = 64;          // both sides are padded (with zeros) to a multiple of this
@@ -508,14 +507,14 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
 }
 
 // TM x TN outputs per workgroup of four waves, K in steps of 64 through NST LDS stages.
-// A step reads its whole stage into registers, and the copies (global -> LDS, no registers) of the
-// stage NST steps on go into its slot while it is multiplied: NST - 1 to NST stages are in
-// flight, and of the workgroups of a CU one reads LDS while another multiplies.
+// A step multiplies the stage that is in registers while it reads the next one from LDS and the copies
+// (global -> LDS, no registers) of the stage NST steps on go into the slot that has been read: one barrier
+// a step, and no latency in its way.
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
 template <int MODE, int TM, int NST, bool SPLIT, int OUT = NS_BF16>
-__global__ __launch_bounds__(256, NST * TM <= 256 ? 2 : 1) void ns_product_kernel(const NsArgs a, const int cur) {
+__global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
   constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
   constexpr int TN = SYM ? TM : 128;
@@ -599,26 +598,34 @@ __global__ __launch_bounds__(256, NST * TM <= 256 ? 2 : 1) void ns_product_kerne
   const uint32_t xa = frag_base(wm * WTM, lane);
   const uint32_t xb = A_ST + (SYM ? frag_base(wn * WTN, lane) : tr_base(4 * wn, lane));
   typedef __attribute__((address_space(3))) half8 lds_half8;
-#pragma unroll
-  for (int st = 0; st < NST; ++st) issue(st);
-  int slot = 0;
-  for (int it = 0; it < steps; ++it) {
-    wait_vm_barrier<(NST - 1) * (CA + CB)>();  // this stage is there
+  struct Frags {
+    half8 a[2][FM], b[2][FN];
+  };
+  auto read = [&](Frags& f, int slot) __attribute__((always_inline)) {
     const uint32_t src = sbase + slot * STAGE;
-    half8 fa[2][FM], fb[2][FN];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[kh][i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
+      for (int i = 0; i < FM; ++i) f.a[kh][i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        if constexpr (SYM) fb[kh][j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
-        else fb[kh][j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
+        if constexpr (SYM) f.b[kh][j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
+        else f.b[kh][j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
       }
     }
-    wait_lds_barrier();  // every wave has this stage in registers: its slot takes the stage after the next
+  };
+#pragma unroll
+  for (int st = 0; st < NST; ++st) issue(st);
+  Frags f0, f1;
+  wait_vm_barrier<(NST - 1) * (CA + CB)>();
+  read(f0, 0);
+  int slot = 0;
+  auto step = [&](const Frags& now, Frags& next) __attribute__((always_inline)) {
+    // the next stage is there, and every wave has this one in registers: its slot takes the stage NST on
+    wait_vm_barrier<(NST - 2) * (CA + CB)>();
     issue(slot);
     slot = slot + 1 == NST ? 0 : slot + 1;
+    read(next, slot);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -626,10 +633,13 @@ __global__ __launch_bounds__(256, NST * TM <= 256 ? 2 : 1) void ns_product_kerne
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[kh][j], fa[kh][i], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.b[kh][j], now.a[kh][i], acc[i][j], 0, 0, 0);
     __builtin_amdgcn_s_setprio(0);
+  };
+  for (int it = 0; it < steps; it += 2) {
+    step(f0, f1);
+    if (it + 1 < steps) step(f1, f0);
   }
-
   wait_vm_barrier<0>();  // the copies past the end have landed: the epilogue takes their LDS
   ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, smem + w * EPI, lane, mat, ti * TM + wm * WTM, tj * TN + wn * WTN,
                                 ti != tj);
@@ -1242,8 +1252,6 @@ inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
         <<<dim3(static_cast<unsigned>(std::min<int64_t>(8 * ceil_div(t256, 8), kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
   } else if (t128 >= 256) {
     ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
-  } else if (t128 >= NS_T128) {
-    ns_product_kernel<MODE, 128, 4, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
   } else {
     ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<grid(t64), dim3(256), 0, s>>>(a, cur);
   }
