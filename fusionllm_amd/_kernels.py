@@ -620,7 +620,7 @@ def normuon_step(params, grads, exp_avgs, exp_avg_sqs, lr: float, beta1: float, 
 
 MUON_MAX_TENSORS = 64
 MUON_MAX_SIDE = 65536
-MUON_MAX_ELEMENTS = 1 << 30  # of a matrix whose sides are rounded up to multiples of 64
+MUON_MAX_ELEMENTS = 1 << 29  # of a matrix whose sides are rounded up to multiples of 64
 MUON_MAX_STEPS = 64
 
 

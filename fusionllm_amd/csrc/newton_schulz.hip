@@ -66,10 +66,12 @@ struct NsArgs {
   double eps;
   float ca, cb, cc;         // the polynomial's coefficients
   double* norm;             // [count][parts]
-  // fp16, hi and lo: X [count][mp][np] twice (the step reads one and writes the other), A and
-  // B [count][mp][mp]; where operands are hi alone, lo of X is fp8 and there once (each
-  // tile reads and writes its own), and A and B have none
-  _Float16 *xh[2], *xl[2], *ah, *al, *bh, *bl;
+  // fp16: X [count][mp][np] twice (the step reads one and writes the other), A and B
+  // [count][mp][mp].  Where operands are hi + lo, the rows are twice as long: 32 elements' hi, their lo,
+  // the next 32 elements' hi, ... (ns_at), so that a K step of a product has both from one
+  // 128-byte piece per row.  Elsewhere lo of X is fp8 (x8, null otherwise) and there once (each
+  // tile reads and writes its own), and A and B have none.
+  _Float16 *xh[2], *ah, *bh;
   uint8_t* x8;
   // small matrices: X [count][panels][64][128] fp32, partial Gram matrices [2][count][panels][10][256],
   // and the panels' exponents
@@ -77,6 +79,13 @@ struct NsArgs {
   int* exps;
   int panels;
 };
+
+// Index in a row of element c's hi, and the distance of its lo, where a row holds both.
+template <bool SPLIT>
+__host__ __device__ __forceinline__ int ns_at(int c) {
+  return SPLIT ? ((c >> 5) << 6) + (c & 31) : c;
+}
+constexpr int kLoAt = 32;
 
 // lo of X as fp8 (times kLoScale), 8 elements: of values v and their hi; and back, still times kLoScale.
 __device__ __forceinline__ uint2 pack_lo8(const float* v, const half8& h) {
@@ -228,10 +237,16 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
       h[e] = static_cast<_Float16>(v[e]);
       l[e] = static_cast<_Float16>(v[e] - static_cast<float>(h[e]));
     }
-    const int64_t o = (static_cast<int64_t>(mat) * a.mp + i0 + r) * a.np + j0 + q;
-    *reinterpret_cast<half8*>(a.xh[0] + o) = h;
-    if (a.x8) *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(v, h);
-    else *reinterpret_cast<half8*>(a.xl[0] + o) = l;
+    const int64_t row = static_cast<int64_t>(mat) * a.mp + i0 + r;
+    if (a.x8) {
+      const int64_t o = row * a.np + j0 + q;
+      *reinterpret_cast<half8*>(a.xh[0] + o) = h;
+      *reinterpret_cast<uint2*>(a.x8 + o) = pack_lo8(v, h);
+    } else {
+      const int64_t o = row * 2 * a.np + ns_at<true>(j0 + q);
+      *reinterpret_cast<half8*>(a.xh[0] + o) = h;
+      *reinterpret_cast<half8*>(a.xh[0] + o + kLoAt) = l;
+    }
   }
 }
 
@@ -296,10 +311,11 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
   constexpr bool LO8 = !SPLIT && MODE == NS_STEP;  // a lo, of fp8, is added
   constexpr int JH = FN / 4;                       // 64-column parts
   constexpr int SR = FM >= 2 ? 32 : 16;            // rows per transposed slice
-  const int lim = SYM ? a.mp : a.np, ld = lim;
-  const int64_t base = static_cast<int64_t>(mat) * a.mp * lim + static_cast<int64_t>(row0) * ld + col0;
+  constexpr int W = SPLIT ? 2 : 1;                 // row length per element
+  const int lim = SYM ? a.mp : a.np, ld = W * lim;
+  const int64_t base = (static_cast<int64_t>(mat) * a.mp + row0) * ld + W * col0;
   const int lr = lane >> 3, lc = (lane & 7) * 8;
-  const uint32_t voff = static_cast<uint32_t>(lr * ld + lc);
+  const uint32_t voff = static_cast<uint32_t>(lr * ld + ns_at<SPLIT>(lc));
   const bool tall = MODE == NS_LAST && ((a.tall >> mat) & 1);
   void* const dst = MODE == NS_LAST ? a.dst[mat] : nullptr;
   static_assert(kNsPad % 64 == 0);
@@ -307,7 +323,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
   // piece (i, jh, p) of this lane: row 16 i + 8 p + lr, columns 64 jh + lc .. + 7
   auto on = [&](int jh) { return col0 + 64 * jh < lim; };
   auto piece = [&](auto* array, int i, int jh, int p) {
-    return array + (base + static_cast<int64_t>(16 * i + 8 * p) * ld + 64 * jh) + voff;
+    return array + (base + static_cast<int64_t>(16 * i + 8 * p) * ld + W * 64 * jh) + voff;
   };
   // A of this block (POLY; a part of it at a time, all would spill), lo of X (STEP)
   constexpr bool POLY = MODE == NS_POLY;
@@ -324,7 +340,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
           for (int p = 0; p < 2; ++p)
             if (i0 + i < FM && on(jh)) {
               if constexpr (POLY) ah[i][jh][p] = *reinterpret_cast<const half8*>(piece(a.ah, i0 + i, jh, p));
-              if constexpr (POLY && SPLIT) al[i][jh][p] = *reinterpret_cast<const half8*>(piece(a.al, i0 + i, jh, p));
+              if constexpr (POLY && SPLIT) al[i][jh][p] = *reinterpret_cast<const half8*>(piece(a.ah, i0 + i, jh, p) + kLoAt);
               if constexpr (LO8) x8[i][jh][p] = *reinterpret_cast<const uint2*>(piece(a.x8, i0 + i, jh, p));
             }
     }
@@ -378,7 +394,6 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
     }
   };
   _Float16* const oh = MODE == NS_GRAM ? a.ah : MODE == NS_POLY ? a.bh : a.xh[1 - cur];
-  _Float16* const ol = MODE == NS_GRAM ? a.al : MODE == NS_POLY ? a.bl : a.xl[1 - cur];
   const bool turn = SYM ? mirror : tall;
   constexpr bool TURN_LO = SPLIT || MODE == NS_LAST;  // the transposed values need their lo
   // hi and lo of the pieces, kept in the accumulators' registers for the transposed store
@@ -424,7 +439,7 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
         if constexpr (MODE != NS_LAST) {
           if (on(jh)) {
             *reinterpret_cast<half8*>(piece(oh, i, jh, p)) = h;
-            if constexpr (SPLIT) *reinterpret_cast<half8*>(piece(ol, i, jh, p)) = l;
+            if constexpr (SPLIT) *reinterpret_cast<half8*>(piece(oh, i, jh, p) + kLoAt) = l;
             else if constexpr (MODE == NS_STEP) *reinterpret_cast<uint2*>(piece(a.x8, i, jh, p)) = pack_lo8(v, h);
           }
         }
@@ -442,8 +457,8 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
     const int g = lane >> 4, sj = (lane >> 2) & 3, sq = lane & 3;
     const int rg = g % RG, cw0 = g / RG;
     const uint32_t lds = core::lds_addr(ep);
-    const int64_t tbase = static_cast<int64_t>(mat) * a.mp * a.mp + static_cast<int64_t>(col0) * a.mp + row0;
-    const uint32_t tvoff = static_cast<uint32_t>((16 * cw0 + (lane & 15)) * a.mp + 8 * rg);
+    const int64_t tbase = (static_cast<int64_t>(mat) * a.mp + col0) * (W * a.mp);
+    const uint32_t tvoff = static_cast<uint32_t>((16 * cw0 + (lane & 15)) * (W * a.mp) + 8 * rg);
 #pragma unroll
     for (int i0 = 0; i0 < FM; i0 += SR / 16)
 #pragma unroll
@@ -482,9 +497,11 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
           const int col = col0 + 64 * jh + 16 * (cw0 + (4 / RG) * k) + (lane & 15);
           if constexpr (SYM) {
             if (on(jh)) {
-              const int64_t o = tbase + static_cast<int64_t>(64 * jh + 16 * (4 / RG) * k) * a.mp + 16 * i0;
+              // (the 8 rows of a group stay within 32 of a multiple of 32)
+              const int64_t o = tbase + static_cast<int64_t>(64 * jh + 16 * (4 / RG) * k) * (W * a.mp) +
+                                ns_at<SPLIT>(row0 + 16 * i0);
               *reinterpret_cast<half8*>(oh + o + tvoff) = t[0][k];
-              if constexpr (SPLIT) *reinterpret_cast<half8*>(ol + o + tvoff) = t[TURN_LO ? 1 : 0][k];
+              if constexpr (SPLIT) *reinterpret_cast<half8*>(oh + o + tvoff + kLoAt) = t[TURN_LO ? 1 : 0][k];
             }
           } else if (OUT >= NS_MUON_BF16 && col < a.n && row + 8 <= a.m) {
             raw[k] = load_raw<OUT & 1, 8>(dst, static_cast<int64_t>(col) * a.m + row);
@@ -512,7 +529,9 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
 // a step, and no latency in its way.
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
-// (gemm_core.h has both layouts and their swizzles).  SPLIT: hi lo + lo hi + hi hi.
+// (gemm_core.h has both layouts and their swizzles).  SPLIT: a stage is hi and lo of 32 k, and a step
+// adds hi lo + lo hi + hi hi (three passes over K instead read each operand again: 3 matrices of 768 x
+// 2048, Gram product 32 us).
 template <int MODE, int TM, int NST, bool SPLIT, int OUT = NS_BF16>
 __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
@@ -542,14 +561,12 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   ti = __builtin_amdgcn_readfirstlane(ti);
   tj = __builtin_amdgcn_readfirstlane(tj);
 
-  const int K = MODE == NS_GRAM ? a.np : a.mp;
-  const int lda = K, ldb = SYM ? K : a.np;
-  const int nk = K / BK, steps = nk * (SPLIT ? 3 : 1);
-  const int64_t msq = static_cast<int64_t>(mat) * a.mp * a.mp, mx = static_cast<int64_t>(mat) * a.mp * a.np;
-  const _Float16* ph = MODE == NS_GRAM ? a.xh[cur] + mx : MODE == NS_POLY ? a.ah + msq : a.bh + msq;
-  const _Float16* pl = MODE == NS_GRAM ? a.xl[cur] + mx : MODE == NS_POLY ? a.al + msq : a.bl + msq;
-  const _Float16* qh = SYM ? ph : a.xh[cur] + mx;
-  const _Float16* ql = SYM ? pl : a.xl[cur] + mx;
+  constexpr int W = SPLIT ? 2 : 1;  // row length per element
+  const int lda = W * (MODE == NS_GRAM ? a.np : a.mp), ldb = SYM ? lda : W * a.np;
+  const int steps = lda / BK;
+  const int64_t msq = static_cast<int64_t>(mat) * a.mp * W * a.mp, mx = static_cast<int64_t>(mat) * a.mp * W * a.np;
+  const _Float16* p = MODE == NS_GRAM ? a.xh[cur] + mx : MODE == NS_POLY ? a.ah + msq : a.bh + msq;
+  const _Float16* q = SYM ? p : a.xh[cur] + mx;
 
   // this lane's byte offsets from the operands' bases (rows and columns past the padded end: the last)
   uint32_t aoff[CA], boff[CB];
@@ -562,15 +579,15 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     if constexpr (SYM) {
       boff[q] = static_cast<uint32_t>(min(tj * TN + 8 * (w + 4 * q) + (lane >> 3), a.mp - 1) * ldb + chunk) * 2u;
     } else {
-      const int krow = 4 * (w + 4 * q) + (lane >> 4);
+      const int krow = 4 * (w + 4 * q) + (lane >> 4);  // SPLIT: rows 0 .. 31's hi, then their lo
       const int cb = ((((lane & 15) >> 1) ^ wsw(krow)) << 1) | (lane & 1);
-      boff[q] = static_cast<uint32_t>(krow * ldb + min(tj * TN + 8 * cb, a.np - 8)) * 2u;
+      const int at = ns_at<SPLIT>(min(tj * TN + 8 * cb, a.np - 8));
+      boff[q] = static_cast<uint32_t>((SPLIT ? krow % 32 : krow) * ldb + at + (SPLIT && krow >= 32 ? kLoAt : 0)) * 2u;
     }
   }
-  // SPLIT: hi lo, lo hi, then hi hi, so that the small terms are summed while the sum is small
-  const uint8_t *pa = reinterpret_cast<const uint8_t*>(ph), *pb = reinterpret_cast<const uint8_t*>(SPLIT ? ql : qh);
-  const int64_t bstep = SYM ? RB : static_cast<int64_t>(BK) * ldb * 2;
-  int kt = 0, seg = 0, left = steps;
+  const uint8_t *pa = reinterpret_cast<const uint8_t*>(p), *pb = reinterpret_cast<const uint8_t*>(q);
+  const int64_t bstep = SYM ? RB : static_cast<int64_t>(BK / W) * ldb * 2;
+  int left = steps;
   // the next stage's copies; past the last step the last stage again (into a slot that is free and
   // not read any more), so that every wait counts the same operations
   auto issue = [&](int st) __attribute__((always_inline)) {
@@ -582,12 +599,6 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     if (--left <= 0) return;
     pa += RB;
     pb += bstep;
-    if (SPLIT && ++kt == nk) {
-      kt = 0;
-      ++seg;
-      pa = reinterpret_cast<const uint8_t*>(seg == 1 ? pl : ph);
-      pb = reinterpret_cast<const uint8_t*>(qh);
-    }
   };
 
   f32x4 acc[FM][FN];
@@ -627,13 +638,15 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     slot = slot + 1 == NST ? 0 : slot + 1;
     read(next, slot);
     __builtin_amdgcn_s_setprio(1);
+    // the halves of a stage: k 0 .. 31 and 32 .. 63, or hi and lo of 32 k
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh)
+    for (int x = 0; x < (SPLIT ? 3 : 2); ++x)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.b[kh][j], now.a[kh][i], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.b[SPLIT ? x == 0 : x][j], now.a[SPLIT ? x == 1 : x][i],
+                                                             acc[i][j], 0, 0, 0);
     __builtin_amdgcn_s_setprio(0);
   };
   for (int it = 0; it < steps; it += 2) {
@@ -663,15 +676,16 @@ __device__ __forceinline__ void ns_mfma4(f32x4& c00, f32x4& c10, f32x4& c01, f32
 #undef FMOE_NS_MF
 
 // Quarter (I, J) of the wave's block (core::quarter with fp16 operands).
-template <int I, int J>
+template <int I, int J, bool SPLIT>
 __device__ __forceinline__ void ns_quarter(f32x4 (&acc)[core::FM][core::FN], const core::AFrag& a,
                                            const core::BFrag& b) {
   __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int kh = x >> 1, n = (x & 1) * 2;
+  for (int x = 0; x < (SPLIT ? 6 : 4); ++x) {
+    const int h = x >> 1, n = (x & 1) * 2;
+    const int ka = SPLIT ? h == 1 : h, kb = SPLIT ? h == 0 : h;  // hi lo, lo hi, hi hi
     ns_mfma4(acc[2 * I][4 * J + n], acc[2 * I + 1][4 * J + n], acc[2 * I][4 * J + n + 1],
-             acc[2 * I + 1][4 * J + n + 1], b[kh][n], b[kh][n + 1], a[kh][0], a[kh][1]);
+             acc[2 * I + 1][4 * J + n + 1], b[kb][n], b[kb][n + 1], a[ka][0], a[ka][1]);
   }
   __builtin_amdgcn_s_setprio(0);
   core::barrier();
@@ -701,9 +715,9 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
   const int end = static_cast<int>(static_cast<int64_t>(items) * (xcd + 1) / 8);
   const int my_items = (end - first + step - 1) / step;
   if (my_items <= 0) return;
-  const int K = MODE == NS_GRAM ? a.np : a.mp;
-  const int ld = K, ldb = SYM ? K : a.np;
-  const int nk = K / BK, steps = SPLIT ? 3 * nk : nk;
+  constexpr int W = SPLIT ? 2 : 1;  // row length per element
+  const int ld = W * (MODE == NS_GRAM ? a.np : a.mp), ldb = SYM ? ld : W * a.np;
+  const int steps = ld / BK;
   const int total = my_items * steps;
 
   auto locate = [&](int item) __attribute__((always_inline)) {
@@ -721,32 +735,17 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
   // ---- copy cursor (the units of a stage and their LDS layout as in gemm_core.h)
   const uint32_t lds_a = sbase + (64 * (w >> 2) + 8 * (w & 3)) * RB;
   const uint32_t lds_b = sbase + A_BYTES + w * 1024;
-  int c_ti = 0, c_kt = 0, c_seg = 0;
+  int c_ti = 0, c_kt = 0;
   const uint8_t *c_a = nullptr, *c_b = nullptr;
   uint32_t a_off[4], b_off[4];
-  const int64_t bstep = SYM ? RB : static_cast<int64_t>(2) * BK * ldb;
-  // operand bases of the tile being copied, for segment c_seg (SPLIT: hi lo, lo hi, hi hi)
-  auto bases = [&](const NsTile& t) __attribute__((always_inline)) {
-    const int64_t msq = static_cast<int64_t>(t.mat) * a.mp * a.mp, mx = static_cast<int64_t>(t.mat) * a.mp * a.np;
-    const bool alo = SPLIT && c_seg == 1, blo = SPLIT && c_seg == 0;
-    const _Float16 *p, *q;
-    if constexpr (MODE == NS_GRAM) {
-      p = (alo ? a.xl[cur] : a.xh[cur]) + mx;
-      q = (blo ? a.xl[cur] : a.xh[cur]) + mx;
-    } else if constexpr (MODE == NS_POLY) {
-      p = (alo ? a.al : a.ah) + msq;
-      q = (blo ? a.al : a.ah) + msq;
-    } else {
-      p = (alo ? a.bl : a.bh) + msq;
-      q = (blo ? a.xl[cur] : a.xh[cur]) + mx;
-    }
-    c_a = reinterpret_cast<const uint8_t*>(p + static_cast<int64_t>(t.ti) * BM * ld);
-    c_b = reinterpret_cast<const uint8_t*>(SYM ? q + static_cast<int64_t>(t.tj) * BN * ld : q);
-  };
+  const int64_t bstep = SYM ? RB : static_cast<int64_t>(BK / W) * ldb * 2;
   auto copy_tile = [&](int ti) __attribute__((always_inline)) {
     const NsTile t = locate(first + ti * step);
-    c_seg = 0;
-    bases(t);
+    const int64_t msq = static_cast<int64_t>(t.mat) * a.mp * W * a.mp, mx = static_cast<int64_t>(t.mat) * a.mp * W * a.np;
+    const _Float16* p = MODE == NS_GRAM ? a.xh[cur] + mx : MODE == NS_POLY ? a.ah + msq : a.bh + msq;
+    const _Float16* q = SYM ? p : a.xh[cur] + mx;
+    c_a = reinterpret_cast<const uint8_t*>(p + static_cast<int64_t>(t.ti) * BM * ld);
+    c_b = reinterpret_cast<const uint8_t*>(SYM ? q + static_cast<int64_t>(t.tj) * BN * ld : q);
     // the lane as an opaque value: what follows is formed here, not kept through the main loop
     int l = lane;
     asm volatile("" : "+v"(l));
@@ -763,7 +762,9 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
         const int krow = 4 * w + (l >> 4);
         const int cb = ((((l & 15) >> 1) ^ wsw(krow)) << 1) | (l & 1);
         const int col = 128 * (cb >> 3) + 8 * (cb & 7) + 64 * (q >> 1);
-        b_off[q] = static_cast<uint32_t>((32 * (q & 1) + krow) * ldb + min(t.tj * BN + col, a.np - 8)) * 2u;
+        const int at = ns_at<SPLIT>(min(t.tj * BN + col, a.np - 8));
+        // SPLIT: the second 32 rows of a stage are the first ones' lo
+        b_off[q] = static_cast<uint32_t>((SPLIT ? krow : 32 * (q & 1) + krow) * ldb + at + (SPLIT && (q & 1) ? kLoAt : 0)) * 2u;
       }
     }
   };
@@ -777,12 +778,8 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
     if (u == 0) return;
     c_a += RB;
     c_b += bstep;
-    if (__builtin_expect(++c_kt == nk, 0)) {
-      if (SPLIT && c_seg < 2) {
-        c_kt = 0;
-        ++c_seg;
-        bases(locate(first + c_ti * step));
-      } else if (c_ti + 1 < my_items) {
+    if (__builtin_expect(++c_kt == steps, 0)) {
+      if (c_ti + 1 < my_items) {
         c_kt = 0;
         copy_tile(++c_ti);
       } else {
@@ -849,7 +846,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
     for (int n = 0; n < 4; ++n) read_b(b0, 0, st, 1, n);
     issue_a(it + 1, 1);
     wait_vm_barrier<5 * LU>();  // B1 of this stage
-    ns_quarter<0, 0>(acc, a0, b0);
+    ns_quarter<0, 0, SPLIT>(acc, a0, b0);
     // (0, 1)
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -857,7 +854,7 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
       for (int n = 0; n < 4; ++n) read_b(b1, 1, st, kh, n);
     issue_a(it + 2, 0);
     wait_vm_barrier<5 * LU>();  // A1 of this stage
-    ns_quarter<0, 1>(acc, a0, b1);
+    ns_quarter<0, 1, SPLIT>(acc, a0, b1);
     // (1, 0)
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -865,12 +862,12 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
       for (int m = 0; m < 2; ++m) read_a(a1, 1, st, kh, m);
     issue_b(it + 2, 0);
     wait_vm_barrier<4 * LU>();  // A0, B0 of the next stage
-    ns_quarter<1, 0>(acc, a1, b0);
+    ns_quarter<1, 0, SPLIT>(acc, a1, b0);
     // (1, 1): the next step's first fragments (at a tile's end they are read again after its epilogue)
     read_first(nxt);
     issue_b(it + 2, 1);
     wait_lds_barrier();
-    ns_quarter<1, 1>(acc, a1, b1);
+    ns_quarter<1, 1, SPLIT>(acc, a1, b1);
 
     if (++e_kt < steps) continue;
     // ---- tile epilogue: this wave's 64 x 128 block (both wave groups together)
@@ -1347,13 +1344,11 @@ inline int ns_run(NsArgs& a, int steps, const double* coeffs, double eps, void* 
     p += n;
     return q;
   };
-  for (int i = 0; i < 2; ++i) a.xh[i] = take(l.x);
-  if (split)
-    for (int i = 0; i < 2; ++i) a.xl[i] = take(l.x);
-  else a.x8 = reinterpret_cast<uint8_t*>(take(l.x / 2));
-  a.ah = take(l.sq);
-  a.bh = take(l.sq);
-  if (split) a.al = take(l.sq), a.bl = take(l.sq);
+  const size_t w = split ? 2 : 1;
+  for (int i = 0; i < 2; ++i) a.xh[i] = take(w * l.x);
+  a.ah = take(w * l.sq);
+  a.bh = take(w * l.sq);
+  if (!split) a.x8 = reinterpret_cast<uint8_t*>(take(l.x / 2));
 #define FMOE_NS_LOAD(DT, MUON)                                                                   \
   do {                                                                                           \
     ns_norm_kernel<DT, MUON><<<dim3(a.parts, a.count), dim3(256), 0, s>>>(a);                    \

@@ -19,7 +19,7 @@ extern "C" {
 #define FMOE_LAYER_NORM_MAX_DIM 16384
 #define FMOE_MUON_MAX_TENSORS 64
 #define FMOE_MUON_MAX_SIDE 65536
-#define FMOE_MUON_MAX_ELEMENTS 1073741824 /* of a matrix, its sides rounded up to multiples of 64 */
+#define FMOE_MUON_MAX_ELEMENTS 536870912 /* of a matrix, its sides rounded up to multiples of 64 */
 #define FMOE_MUON_MAX_STEPS 64
 
 /* ---------------------------------------------------------------------------

@@ -8,8 +8,7 @@ fp32, in another order), so its error is another draw of the same size: bound 3 
 plus the fp32 sums themselves: a product over K is a chain of K / 32 accumulations
 (K padded to 64) whose running sum loses at most 2^-23 of itself each, even where the
 matrix unit cuts instead of rounding, so K / 32 2^-23 of the product in one direction
-(the two small products of the 22-bit form come first and add 2^-11 of that, counted as
-one more accumulation each).  How far such a loss in every product moves the result is
+(three accumulations for every 32 in the 22-bit form).  How far such a loss in every product moves the result is
 computed too: ``emulate`` with every product scaled by it, against the one without.
 Plus half a step of the result's type.  An element is within 8 standard deviations (the bound's root mean square)
 of its value, plus half a step of it."""
@@ -61,7 +60,7 @@ def emulate(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7, split=False, cut=False):
     def mul(p, q):
         r = p[0] @ q[0]
         r = r + p[0] @ q[1] + p[1] @ q[0] if split else r
-        k = -(-p[0].shape[1] // 64) * 2 + 2
+        k = -(-p[0].shape[1] // 64) * 2 * (3 if split else 1)
         return r * (1 - k * 2.0 ** -23) if cut else r
 
     tr = lambda p: tuple(t.t().contiguous() for t in p)

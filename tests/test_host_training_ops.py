@@ -133,7 +133,7 @@ def test_newton_schulz_argument_errors_without_gpu(call):
     assert f(steps=0) == 1 and f(steps=65) == 1
     assert f(dtype=2) == 4 and f(p=None) == 1 and f(p=FAKE + 1) == 3 and f(p=FAKE + 2, dtype=1) == 3
     assert f(rows=0) == 1 and f(rows=-4) == 1 and f(cols=0) == 1 and f(cols=65537) == 2
-    assert f(rows=32769, cols=32768, nbytes=0) == 2 and f(rows=32768, cols=32768, nbytes=0) == 6
+    assert f(rows=16385, cols=32768, nbytes=0) == 2 and f(rows=16384, cols=32768, nbytes=0) == 6
     assert f(eps=0.0) == 1 and f(eps=-1.0) == 1 and f(eps=float("nan")) == 1
     # one pair of sides per call, in either order
     assert f(n=2, second=(2048, 768)) == 6 and f(n=2, second=(768, 2047)) == 2
@@ -184,7 +184,7 @@ def test_newton_schulz_workspace_size():
     # small sides: per panel of 128 columns the norm, the exponent, X and two partial Gram matrices
     assert q(5, 129, 3, 0) == 256 + 256 + 3 * 2 * 4 * (64 * 128 + 2 * 10 * 256)
     assert q(64, 4097, 1, 0) > 4 * 2 * 64 * 4096  # 33 panels: the general form
-    assert q(0, 5, 1, 0) == q(5, 5, 0, 0) == q(5, 5, 65, 0) == q(65537, 5, 1, 0) == q(32769, 32768, 1, 0) == 0
+    assert q(0, 5, 1, 0) == q(5, 5, 0, 0) == q(5, 5, 65, 0) == q(65537, 5, 1, 0) == q(16385, 32768, 1, 0) == 0
 
 
 def test_muon_and_orthogonalize_refusals():
@@ -222,4 +222,4 @@ def test_muon_and_orthogonalize_refusals():
         with pytest.raises(NotImplementedError, match="65536"):
             orthogonalize(torch.empty(2, 65537, device="cuda"))
         with pytest.raises(NotImplementedError, match="elements"):
-            orthogonalize(torch.empty(32769, 32768, device="cuda"))
+            orthogonalize(torch.empty(16385, 32768, device="cuda"))
