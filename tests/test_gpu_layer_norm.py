@@ -400,3 +400,70 @@ def test_timed_wrappers_give_the_same_bits(gpu_device):
         K.set_timer(None)
     assert set(store) == {"layer_norm_fwd", "layer_norm_bwd"} and len(store["layer_norm_fwd"]) == 2
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_autograd_under_graph_capture(gpu_device):
+    # forward and backward through autograd, captured with leaves of its own and replayed on new inputs
+    T, dim = 70, 300
+    x, w, b, dy = inputs(T, dim, BF, F32, gpu_device)
+    dy = dy.to(BF)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = layer_norm(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for rep in range(3):
+        nx, _, _, nd = inputs(T, dim, BF, F32, gpu_device, seed=50 + rep)
+        with torch.no_grad():
+            leaves[0].copy_(nx)
+        dy.copy_(nd.to(BF))
+        g.replay()
+        torch.cuda.synchronize()
+        y, mean, rstd = K.layer_norm_fwd(nx, w, b, 1e-5, BF)
+        want = (y, *K.layer_norm_bwd(nd.to(BF), nx, mean, rstd, w, None, True, F32, F32))
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), rep
+
+
+def test_input_changed_before_the_backward_is_an_error(gpu_device):
+    x = torch.randn(4, 64, device=gpu_device, requires_grad=True)
+    y = layer_norm(x * 1.0, torch.ones(64, device=gpu_device))
+    h = x * 1.0
+    z = layer_norm(h, torch.ones(64, device=gpu_device))
+    h.add_(1.0)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+
+def test_wrappers_refuse_what_the_kernels_do_not_take(gpu_device):
+    x = torch.randn(8, 64, device=gpu_device)
+    w = torch.ones(64, device=gpu_device)
+    m = torch.zeros(8, device=gpu_device)
+    with pytest.raises(RuntimeError, match="overlap"):
+        K.layer_norm_fwd(x[:1].expand(8, 64), w, None, 1e-5, F32)
+    with pytest.raises(RuntimeError, match="adjacent"):
+        K.layer_norm_fwd(torch.randn(64, 8, device=gpu_device).t(), w, None, 1e-5, F32)
+    with pytest.raises(RuntimeError, match="one dtype"):
+        K.layer_norm_fwd(x, w, w.bfloat16(), 1e-5, F32)
+    with pytest.raises(RuntimeError, match="hold 64"):
+        K.layer_norm_fwd(x, w[:32], None, 1e-5, F32)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        K.layer_norm_fwd(x, w, None, 1e-5, torch.float16)
+    with pytest.raises(RuntimeError, match="dy must be"):
+        K.layer_norm_bwd(x[:4], x, m, m, w)
+    with pytest.raises(RuntimeError, match="mean must hold"):
+        K.layer_norm_bwd(x, x, m[:4], m, w)
+    with pytest.raises(RuntimeError, match="d_residual"):
+        K.layer_norm_bwd(x, x, m, m, w, x[:4])
+    with pytest.raises(RuntimeError, match="one dtype"):
+        K.layer_norm_bwd(x, x, m, m, w, None, True, BF, None)

@@ -434,3 +434,61 @@ def test_a_block_trains_with_layer_norm_and_muon(gpu_device):
             tol = lr_ * (ortho_bound(u, o, BF)[1] + 8 * 2.0 ** -20 * rms) + 1e-9
             err = (p.detach().double() - want).abs()
             assert (err <= tol + half(BF) * (want.abs() + tol)).all()
+
+
+def test_wrappers_refuse_what_the_kernels_do_not_take(gpu_device):
+    a, b = torch.randn(2, 32, 48, device=gpu_device)
+    out = torch.empty_like(a)
+    go = lambda m, o: K.orthogonalize(m, o, 5, NS_COEFFICIENTS, 1e-7)
+    with pytest.raises(RuntimeError, match="one output per matrix"):
+        go([a, b], [out])
+    with pytest.raises(RuntimeError, match="matrix of shape"):
+        go([a], [out.t().contiguous()])
+    with pytest.raises(RuntimeError, match="contiguous"):
+        go([a.t()], [out.t()])
+    with pytest.raises(RuntimeError, match="float32"):
+        go([a], [out.bfloat16()])
+    with pytest.raises(RuntimeError, match="unsupported shape"):
+        go([a, torch.randn(32, 40, device=gpu_device)], [out, torch.empty(32, 40, device=gpu_device)])
+    with pytest.raises(RuntimeError, match="at most 64"):
+        go([a] * 65, [out] * 65)
+    with pytest.raises(RuntimeError, match="coefficients"):
+        K.orthogonalize([a], [out], 5, (4.0, -4.775, 2.0315), 1e-7)
+    with pytest.raises(RuntimeError, match="coefficients"):
+        orthogonalize(a, coefficients=(3.0, 0.0, 0.0))
+    p = torch.nn.Parameter(a.clone())
+    p.grad = b.clone()
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="coefficients"):
+        Muon([p], ns_coefficients=(8.0, -9.0, 1.5)).step()
+    q = torch.nn.Parameter(torch.randn(48, 32, device=gpu_device).t())
+    q.grad = b.clone()
+    with pytest.raises(NotImplementedError, match="contiguous"):
+        Muon([q]).step()
+    assert torch.equal(p, before)
+
+
+def test_muon_takes_gradients_of_any_stride(gpu_device):
+    p = torch.nn.Parameter(gradient(40, 70, gpu_device, 1))
+    q = torch.nn.Parameter(p.detach().clone())
+    g = gradient(70, 40, gpu_device, 2)
+    p.grad, q.grad = g.t(), g.t().contiguous()
+    Muon([p], lr=0.1).step()
+    Muon([q], lr=0.1).step()
+    assert torch.equal(p, q)
+
+
+def test_muon_on_a_side_stream(gpu_device):
+    ps, twin = model(gpu_device, BF), model(gpu_device, BF)
+    set_grads(ps, 4)
+    set_grads(twin, 4)
+    a, b = Muon(ps, lr=0.1), Muon(twin, lr=0.1)
+    b.step()
+    b.step()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        a.step()
+        a.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(ps, twin))

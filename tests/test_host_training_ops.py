@@ -223,3 +223,50 @@ def test_muon_and_orthogonalize_refusals():
             orthogonalize(torch.empty(2, 65537, device="cuda"))
         with pytest.raises(NotImplementedError, match="elements"):
             orthogonalize(torch.empty(16385, 32768, device="cuda"))
+
+
+def test_training_kernels_read_no_register_a_load_is_still_filling():
+    # The Newton-Schulz products issue their global -> LDS copies (and, in 256 x 256 tiles, their
+    # MFMAs) from inline assembly with explicit waits, which the compiler does not see.
+    from tests import isa_check as ic
+    build = ROOT / "fusionllm_amd" / "_build"
+    objs = [build / "newton_schulz.o", build / "layer_norm.o"]
+    if not (ic.ROCM_LLVM / "llvm-objdump").exists() or not all(o.exists() for o in objs):
+        pytest.skip("no built objects or no llvm-objdump")
+    checked = 0
+    for o in objs:
+        n, hazards = ic.check_object(o)
+        assert not hazards, "\n".join(hazards[:10])
+        checked += n
+    assert checked >= 80
+
+
+def test_training_kernels_keep_their_values_in_registers(tmp_path):
+    # A product that needs scratch memory pays for it in every tile, a norm in every row.
+    import shutil
+    import subprocess
+
+    from fusionllm_amd import build
+    from tests import isa_check as ic
+    if not ic.ROCM_LLVM.exists():
+        pytest.skip("no LLVM tools here")
+    seen = 0
+    for name in ("newton_schulz", "layer_norm"):
+        obj = build.BUILD_DIR / f"{name}.o"
+        if not obj.exists():
+            pytest.skip("no built objects")
+        work = tmp_path / name
+        work.mkdir()
+        shutil.copy(obj, work / obj.name)
+        subprocess.run([str(ic.ROCM_LLVM / "llvm-objdump"), "--offloading", obj.name], check=True,
+                       capture_output=True, cwd=work)
+        dev = next(p for p in work.iterdir() if "gfx950" in p.name)
+        notes = subprocess.run([str(ic.ROCM_LLVM / "llvm-readelf"), "--notes", str(dev)], check=True,
+                               capture_output=True, text=True).stdout
+        for entry in notes.split("  - .agpr_count:")[1:]:
+            kernel = re.search(r"\.name:\s+(\S+)", entry).group(1)
+            seen += 1
+            spilled = int(re.search(r"\.vgpr_spill_count:\s*(\d+)", entry).group(1))
+            # the backward of bf16 rows of two chunks per lane is one register over
+            assert spilled <= (1 if "layer_norm_bwd" in kernel else 0), kernel
+    assert seen >= 80
