@@ -81,26 +81,34 @@ class NorMuon(Optimizer):
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def _launches(items, key, distinct):
-    """Lists of items for one launch each: the same key, at most MUON_MAX_TENSORS, and no two that
-    write the same storage (distinct(item): addresses); in order where they do."""
-    open_: dict = {}
-    out = []
-    for it in items:
-        k = key(it)
-        cur = open_.get(k)
-        addr = distinct(it)
-        if cur is None or len(cur[0]) == K.MUON_MAX_TENSORS or not cur[1].isdisjoint(addr):
-            cur = open_[k] = ([], set())
-            out.append(cur[0])
-        cur[0].append(it)
-        cur[1].update(addr)
-    return out
+# Elements of one launch's matrices, at most (one matrix may have more): its workspace takes 5 to 8 bytes
+# for each and as much again for square ones, and this many fill the chip many times over.
+LAUNCH_ELEMENTS = 1 << 28
 
 
 def _sides(t):
     r, c = t.shape
     return (r, c) if r <= c else (c, r)
+
+
+def _launches(items, written):
+    """Lists of items (tuples whose first tensor is the matrix) for one launch each: one device, dtype and
+    pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two that write the same storage
+    (written(item): addresses); in order where they do."""
+    open_: dict = {}
+    out = []
+    for it in items:
+        t = it[0]
+        key = (t.device, t.dtype, _sides(t))
+        most = min(K.MUON_MAX_TENSORS, max(1, LAUNCH_ELEMENTS // t.numel()))
+        addr = written(it)
+        cur = open_.get(key)
+        if cur is None or len(cur[0]) >= most or not cur[1].isdisjoint(addr):
+            cur = open_[key] = ([], set())
+            out.append(cur[0])
+        cur[0].append(it)
+        cur[1].update(addr)
+    return out
 
 
 def _check_ns(steps, coefficients, eps):
@@ -131,7 +139,8 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
 
     mats: a tensor [..., rows, cols] (every matrix of the stack), or a list of such tensors; the result
     has the same structure, shapes and dtypes.  No backward pass.  The coefficients must keep the
-    singular values below 2.8 (the defaults do)."""
+    singular values below 2.8 (the defaults do).  The result of a matrix whose norm is far below eps is
+    nearly zero, and precise to 2^-36 of the size that it would have with a norm of eps or more."""
     single = isinstance(mats, torch.Tensor)
     stacks = [mats] if single else list(mats)
     _check_ns(steps, coefficients, eps)
@@ -148,8 +157,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
         outs.append(out)
         if t.numel():
             items += zip(t.view(-1, *t.shape[-2:]), out.view(-1, *t.shape[-2:]))
-    for chunk in _launches(items, lambda it: (it[0].device, it[0].dtype, _sides(it[0])),
-                           lambda it: (it[1].data_ptr(),)):
+    for chunk in _launches(items, lambda it: (it[1].data_ptr(),)):
         with torch.cuda.device(chunk[0][0].device):
             K.orthogonalize([c[0] for c in chunk], [c[1] for c in chunk], steps, coefficients, eps)
     return outs[0] if single else outs
@@ -216,12 +224,11 @@ class Muon(Optimizer):
                 if not p.is_contiguous():
                     raise NotImplementedError("Muon step needs contiguous parameters")
                 state = self.state[p]
-                if len(state) == 0:
+                if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p)
                 items.append((p, g.contiguous(), state["momentum_buffer"]))
             lr, wd = float(group["lr"]), float(group["weight_decay"])
-            for chunk in _launches(items, lambda it: (it[0].device, it[0].dtype, _sides(it[0])),
-                                   lambda it: (it[0].data_ptr(), it[2].data_ptr())):
+            for chunk in _launches(items, lambda it: (it[0].data_ptr(), it[2].data_ptr())):
                 small, large = _sides(chunk[0][0])
                 if group["adjust_lr_fn"] == "match_rms_adamw":
                     tall = wide = lr * 0.2 * math.sqrt(large)

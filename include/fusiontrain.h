@@ -66,7 +66,8 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  * summed in fp64, the products run on fp16 operands with fp32 sums, X held as
  * fp16 and an fp8 remainder, the result is rounded once, to dtype; for fp32 matrices (and small
  * sides up to 128) every operand is held in 22 bits.  A matrix that holds NaN or
- * infinities gives NaN; a zero matrix gives zeros.  Coefficients whose iterates
+ * infinities gives NaN; a zero matrix gives zeros; the nearly zero result of one
+ * whose norm is far below eps is precise to 2^-36 of the usual size.  Coefficients whose iterates
  * leave the stored range (singular values up to 2.8, |a + b t + c t^2| up to 7.9)
  * return FMOE_ERR_COEFFICIENTS.  Deterministic.
  * workspace: 256-byte aligned, of the size query's bytes (a pair of sides in

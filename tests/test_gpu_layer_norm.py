@@ -467,3 +467,21 @@ def test_wrappers_refuse_what_the_kernels_do_not_take(gpu_device):
         K.layer_norm_bwd(x, x, m, m, w, x[:4])
     with pytest.raises(RuntimeError, match="one dtype"):
         K.layer_norm_bwd(x, x, m, m, w, None, True, BF, None)
+
+
+def test_moe_residual_with_layer_norm_compiles(gpu_device):
+    # traced: the plain expression around the block's and the norm's operators
+    cfg = configs.BlockConfig("t", 40, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=3)
+    moe = build_module(cfg, data, gpu_device, BF)
+    norm = LayerNorm(128).to(gpu_device, BF)
+    x = data.x.to(gpu_device, BF).requires_grad_(True)
+    x2 = x.detach().clone().requires_grad_(True)
+    y = torch.compile(lambda t: moe_residual(t, norm, moe), fullgraph=True, backend="aot_eager")(x)
+    want = x2 + moe(norm(x2))
+    assert torch.equal(y, want)
+    y.backward(data.dy.to(gpu_device, BF))
+    gw = norm.weight.grad.clone()
+    norm.zero_grad()
+    want.backward(data.dy.to(gpu_device, BF))
+    assert torch.equal(x.grad, x2.grad) and torch.equal(gw, norm.weight.grad)

@@ -178,6 +178,15 @@ def test_scale_of_the_input(gpu_device):
         check_ortho(orthogonalize(x), x, F32)
 
 
+def test_norms_far_below_eps(gpu_device):
+    # X is stored in steps of at least 2^-24 / 2^14 (fp16's smallest, times X's factor), and five steps multiply
+    # what is that small by a each: the error of an element is below steps a^5 2^-38, some 2^-27
+    for dtype in (BF, F32):
+        g = (gradient(150, 260, gpu_device, 8) * 1e-14).to(dtype)
+        err = orthogonalize(g).double() - exact(g)
+        assert float(err.abs().max()) <= 5 * NS_COEFFICIENTS[0] ** 5 * 2.0 ** -38
+
+
 def test_zero_nan_and_infinite_matrices(gpu_device):
     # in one launch with a clean one, which they leave alone
     for rows, cols in ((96, 160), (30, 260), (260, 30)):
@@ -220,6 +229,11 @@ def test_many_matrices_take_the_large_tiles(gpu_device):
         out = orthogonalize(stack)
         for i in (0, 17, 63):
             check_ortho(out[i], stack[i], dtype)
+            if dtype == BF:
+                # every tile size sums in the same order.  (With operands hi + lo, the two small products of an
+                # element above the diagonal come in one order where a tile has it and in the other where
+                # a tile below mirrors it.)
+                assert torch.equal(out[i], orthogonalize(stack[i]))
         assert torch.equal(out, orthogonalize(stack))
 
 
@@ -300,6 +314,47 @@ def test_muon_is_the_pieces_one_after_the_other(gpu_device):
     Muon([p], lr=0.5, weight_decay=0.0, momentum=0.0, nesterov=False).step()
     want = p0.double() - 0.5 * orthogonalize(p.grad).double()
     torch.testing.assert_close(p.detach().double(), want, rtol=1e-6, atol=1e-7)
+
+
+def test_launches_are_split_by_their_workspace(gpu_device, monkeypatch):
+    from fusionllm_amd import optim
+    mats = torch.stack([gradient(70, 80, gpu_device, i) for i in range(6)])
+    want = orthogonalize(mats)
+    calls = []
+    launch = K.orthogonalize
+    monkeypatch.setattr(K, "orthogonalize", lambda m, *a: (calls.append(len(m)), launch(m, *a)))
+    monkeypatch.setattr(optim, "LAUNCH_ELEMENTS", 4 * 70 * 80 + 1)
+    assert torch.equal(orthogonalize(mats), want) and calls == [4, 2]
+    monkeypatch.setattr(optim, "LAUNCH_ELEMENTS", 1)
+    assert torch.equal(orthogonalize(mats), want) and calls[2:] == [1] * 6
+
+
+@pytest.mark.parametrize("nesterov,adjust", [(True, None), (False, "match_rms_adamw")])
+def test_muon_is_a_drop_in_for_torchs(gpu_device, nesterov, adjust):
+    # the same two steps by torch.optim.Muon on the CPU, whose products are bf16: its updates are within
+    # 1 - 2 % (bf16 products, simulated: 1.0e-2 .. 1.4e-2) of the exact ones; a wrong scale,
+    # momentum or decay is not within 5 %
+    if not hasattr(torch.optim, "Muon"):
+        pytest.skip("this torch has no Muon")
+    ps = [torch.nn.Parameter(0.05 * torch.randn(s)) for s in ((48, 200), (200, 48), (96, 96))]
+    mine = [torch.nn.Parameter(p.detach().to(gpu_device)) for p in ps]
+    kw = dict(lr=0.05, weight_decay=0.2, momentum=0.9, nesterov=nesterov, adjust_lr_fn=adjust)
+    a, b = torch.optim.Muon(ps, **kw), Muon(mine, **kw)
+    for step in range(2):
+        for i, (p, q) in enumerate(zip(ps, mine)):
+            g = gradient(*p.shape, "cpu", 10 * step + i, fall=0.2)
+            p.grad, q.grad = g, g.to(gpu_device)
+        before = [p.detach().clone() for p in ps]
+        for p, q in zip(ps, mine):
+            with torch.no_grad():
+                q.copy_(p)
+        a.step()
+        b.step()
+        for p, q, p0 in zip(ps, mine, before):
+            moved = p.detach() - p0
+            assert (q.detach().cpu() - p.detach()).norm() <= 0.05 * moved.norm()
+            torch.testing.assert_close(b.state[q]["momentum_buffer"].cpu(), a.state[p]["momentum_buffer"],
+                                       rtol=1e-6, atol=1e-9)
 
 
 def test_muon_skips_groups_and_state(gpu_device):

@@ -270,3 +270,15 @@ def test_training_kernels_keep_their_values_in_registers(tmp_path):
             # the backward of bf16 rows of two chunks per lane is one register over
             assert spilled <= (1 if "layer_norm_bwd" in kernel else 0), kernel
     assert seen >= 80
+
+
+def test_muon_has_torchs_constructor():
+    import inspect
+
+    from fusionllm_amd.optim import Muon
+    if not hasattr(torch.optim, "Muon"):
+        pytest.skip("this torch has no Muon")
+    args = lambda cls: [(p.name, p.default) for p in inspect.signature(cls).parameters.values()]
+    assert args(Muon) == args(torch.optim.Muon)
+    p = torch.nn.Parameter(torch.zeros(2, 3))
+    assert Muon([p]).defaults == torch.optim.Muon([p]).defaults
