@@ -22,9 +22,10 @@
 // bf16 products 1e-2 .. 1.6e-1, fp16 without lo 1.2e-3 .. 4.9e-2, this form
 // 6e-4 .. 1.9e-3 (half a step of a bf16 result: 3.9e-3).
 // fp32 matrices take every operand as hi + lo, both fp16 (three products: hi lo, lo hi,
-// hi hi; relative error 2e-6), and so do matrices of a small side up to kSplitSmall, whose
-// few rounding errors average out less and whose products cost nothing next to
-// the launches.
+// hi hi; relative error 3e-6), and so do matrices of a small side up to kSplitSmall: their
+// products cost little next to the launches, and a bf16 result is then as near as its
+// own rounding allows (96 x 2048: 1.7e-3 off in 162 us against 2.0e-3 .. 2.4e-3 in 105).  Those of a small side up to 64 run in fp32 altogether, one launch per step,
+// unless they are very long (below, ns_is_small).
 //
 // A and B are symmetric: only the tiles on and below the diagonal are computed
 // and stored twice.  3 m^2 n + m^3 flops a step, bound by the matrix units; a
@@ -299,7 +300,8 @@ __device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o
 // return 8 consecutive elements of a column.  What the epilogue reads is asked for first, so
 // that its latency is not paid per slice.  (Epilogues straight from the accumulators, 8 bytes
 // per lane in 16 rows at once, or with the reads slice by slice, took two thirds of a step:
-// 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone.)
+// 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone; now 98, of which
+// the stores are 32.)
 //
 // Pieces of 8 elements sit at a uniform address plus one offset per lane, and whether they are inside
 // the padded result is uniform too (its sides, and a block's place, are multiples of 64, or of the
@@ -526,12 +528,13 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
 // TM x TN outputs per workgroup of four waves, K in steps of 64 through NST LDS stages.
 // A step multiplies the stage that is in registers while it reads the next one from LDS and the copies
 // (global -> LDS, no registers) of the stage NST steps on go into the slot that has been read: one barrier
-// a step, and no latency in its way.
+// a step, and no latency in its way.  (64-row tiles: three stages, Gram product of 3 of 768 x 2048
+// 12.4 us against 17.0 with two; four were no faster.  128-row tiles: two, two workgroups per CU.)
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: a stage is hi and lo of 32 k, and a step
 // adds hi lo + lo hi + hi hi (three passes over K instead read each operand again: 3 matrices of 768 x
-// 2048, Gram product 32 us).
+// 2048, Gram product 32 us against 24).
 template <int MODE, int TM, int NST, bool SPLIT, int OUT = NS_BF16>
 __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
@@ -900,12 +903,17 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
 // v_mfma_f32_16x16x4_f32 (rounding fp32 to fp32 only; the products are small next to the latency of
 // a launch).  A workgroup has 128 columns of X.  It adds the workgroups' partial Gram
 // matrices of the launch before (in a fixed order), forms a I + b A + c A^2 for itself, multiplies
-// its columns and writes the partial Gram matrix of the result for the next launch.  64 x 2048,
-// bf16: three launches a step (28 us of them the Gram matrix's one tile) 190 us.
+// its columns and writes the partial Gram matrix of the result for the next launch.  Five steps, bf16,
+// against three launches a step (most of them the Gram matrix's one tile), in a graph: 64 x 2048 72 us
+// against 145, 8 of 32 x 2048 79 against 147, 27 of 64 x 768 86 against 105.  Where many long ones go
+// together every workgroup's sum over the partial matrices counts: 64 of 64 x 2048 237 us
+// against 215, 64 of 64 x 4096 515 against 359.  The rule leaves their number out all the same, so that a
+// matrix's result is the same whatever goes with it.
 
 constexpr int kSmallSide = 64;        // the small side, at most (and the padded one)
 constexpr int kSmallPanel = 128;      // columns per workgroup
-constexpr int kSmallMaxPanels = 32;   // every workgroup adds the partial matrices of all
+constexpr int kSmallMaxPanels = 32;   // every workgroup adds the partial matrices of all (64 x 4096: 88 us
+                                      // against 228)
 constexpr int kSmallBlocks = 10;      // 16 x 16 blocks of a Gram matrix on or below the diagonal
 constexpr int kLdA = 68, kLdX = 132;  // LDS strides
 
@@ -1244,10 +1252,16 @@ inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
   };
   const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 128);
   auto grid = [](int64_t t) { return dim3(static_cast<unsigned>(8 * ceil_div(t, 8))); };
-  if (t256 >= 128) {
+  // 256 x 256 tiles, persistent, where they fill the chip and pad little (their area is at most 1.5 times
+  // the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 56 us against 65, of 22
+  // (132 tiles) 52 against 47; of 64 of 384 x 2048 (twice the area) 56 against 45.  Then 128 x
+  // 128 tiles where there is one per CU: Gram product of 5 of 1408 x 2048 (330 tiles) 39 us
+  // against 44, of 5 of 1001 x 1503 (180 tiles) 24 against 20; 48 rows would leave
+  // most of a 128-row tile empty.
+  if (t256 >= 160 && 8 * t256 < 3 * t128) {
     ns_big_kernel<MODE, SPLIT, OUT>
         <<<dim3(static_cast<unsigned>(std::min<int64_t>(8 * ceil_div(t256, 8), kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
-  } else if (t128 >= 256) {
+  } else if (t128 >= 256 && t64 > t128) {
     ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
   } else {
     ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<grid(t64), dim3(256), 0, s>>>(a, cur);

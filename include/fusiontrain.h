@@ -65,7 +65,8 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  * and dst = X in G's own orientation (dst may be G's storage).  The norm is
  * summed in fp64, the products run on fp16 operands with fp32 sums, X held as
  * fp16 and an fp8 remainder, the result is rounded once, to dtype; for fp32 matrices (and small
- * sides up to 128) every operand is held in 22 bits.  A matrix that holds NaN or
+ * sides up to 128) every operand is held in 22 bits, and small sides up to 64 with at most
+ * 4096 columns run in fp32.  A matrix that holds NaN or
  * infinities gives NaN; a zero matrix gives zeros; the nearly zero result of one
  * whose norm is far below eps is precise to 2^-36 of the usual size.  Coefficients whose iterates
  * leave the stored range (singular values up to 2.8, |a + b t + c t^2| up to 7.9)
