@@ -314,6 +314,7 @@ inline int64_t ln_bwd_groups(int64_t T, const LnShape& s, int x_dtype) {
 }
 
 inline bool ln_dtype(int d) { return d == FMOE_BF16 || d == FMOE_F32; }
+constexpr int ln_bytes(int d) { return d == FMOE_BF16 ? 2 : 4; }
 inline bool ln_aligned(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == FMOE_BF16 ? 1u : 3u)) == 0;
 }
@@ -352,11 +353,17 @@ extern "C" int fmoe_layer_norm_fwd(const void* x, int x_dtype, int64_t ldx, cons
       !ln_aligned(bias, w_dtype) || !ln_aligned(mean, FMOE_F32) || !ln_aligned(rstd, FMOE_F32))
     return FMOE_ERR_ALIGN;
   const LnShape s = ln_shape(dim, x_dtype == FMOE_F32);
-  const dim3 grid(ceil_div(T, ln_rows(s))), block(ln_threads(s));
+  const dim3 block(ln_threads(s));
   hipStream_t st = as_stream(stream);
-#define FMOE_LN_FWD(XT, YT, V, N)                                                                                   \
-  layer_norm_fwd_kernel<XT, YT, V, N><<<grid, block, 0, st>>>(x, ldx, weight, bias, w_dtype, T, (int)dim, s.waves, eps, \
-                                                              y, mean, rstd)
+  // a launch has fewer than 2^32 threads: 2^31 at once
+  const int64_t most = (int64_t(1) << 31) / ln_threads(s) * ln_rows(s);
+#define FMOE_LN_FWD(XT, YT, V, N)                                                                                  \
+  do for (int64_t t0 = 0; t0 < T; t0 += most) {                                                                       \
+    const int64_t rows = std::min(T - t0, most);                                                                   \
+    layer_norm_fwd_kernel<XT, YT, V, N><<<dim3(ceil_div(rows, ln_rows(s))), block, 0, st>>>(                       \
+        static_cast<const char*>(x) + t0 * ldx * ln_bytes(XT), ldx, weight, bias, w_dtype, rows, (int)dim, s.waves, eps, \
+        static_cast<char*>(y) + t0 * dim * ln_bytes(YT), mean ? mean + t0 : nullptr, rstd ? rstd + t0 : nullptr);  \
+  } while (0)
 #define FMOE_LN_FWD_BB(V, N) FMOE_LN_FWD(FMOE_BF16, FMOE_BF16, V, N)
 #define FMOE_LN_FWD_BF(V, N) FMOE_LN_FWD(FMOE_BF16, FMOE_F32, V, N)
 #define FMOE_LN_FWD_FB(V, N) FMOE_LN_FWD(FMOE_F32, FMOE_BF16, V, N)

@@ -166,7 +166,8 @@ swiglu_fwd.register_autograd(_swiglu_backward, setup_context=_swiglu_setup)
 @torch.library.custom_op("fusionllm::layer_norm_fwd", mutates_args=())
 def layer_norm_fwd(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
                    out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
-    return _norm._forward(x, weight, bias, eps, out_dtype, True)[2:]
+    with _norm._on_device(x):
+        return _norm._forward(x, weight, bias, eps, out_dtype, True)[2:]
 
 
 @layer_norm_fwd.register_fake
@@ -179,8 +180,9 @@ def _(x, weight, bias, eps, out_dtype):
 @torch.library.custom_op("fusionllm::layer_norm_bwd", mutates_args=())
 def layer_norm_bwd(dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, weight: Tensor | None,
                    bias: Tensor | None) -> list[Tensor]:
-    grads = _norm._backward(dy, _norm._rows(x), None if weight is None else weight.contiguous(), mean, rstd, None, True,
-                            None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+    with _norm._on_device(x):
+        grads = _norm._backward(dy, _norm._rows(x), None if weight is None else weight.contiguous(), mean, rstd, None,
+                                True, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
     return [g for g in grads if g is not None]
 
 

@@ -485,3 +485,39 @@ def test_moe_residual_with_layer_norm_compiles(gpu_device):
     norm.zero_grad()
     want.backward(data.dy.to(gpu_device, BF))
     assert torch.equal(x.grad, x2.grad) and torch.equal(gw, norm.weight.grad)
+
+
+def test_more_rows_than_one_launch_and_32_bit_offsets_take(gpu_device):
+    # 2^26 + 3 rows: more than 2^32 threads with a wave per row, and more than 2^31 elements.  y and dx in
+    # rows around the places where a launch ends and an offset passes 31 bits; dw and db over all rows, with
+    # a chain of T / 4096 rows per wave (1024 workgroups of four), 4 waves, 64 partial rows and 16 sums.
+    T, dim = 2 ** 26 + 3, 40
+    gen = torch.Generator(gpu_device).manual_seed(9)
+    x = torch.randn(T, dim, dtype=BF, device=gpu_device, generator=gen)
+    dy = torch.randn(T, dim, dtype=BF, device=gpu_device, generator=gen)
+    w = (1 + 0.3 * torch.randn(dim, device=gpu_device, generator=gen))
+    b = torch.randn(dim, device=gpu_device, generator=gen)
+    for p in (x, w, b):
+        p.requires_grad_(True)
+    y = layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x, y, w, b = x.detach(), y.detach(), w.detach(), b.detach()
+    for mid in (0, 2 ** 25, 2 ** 31 // dim, T):
+        rows = slice(max(mid - 600, 0), mid + 600)
+        want, tol = truth(x[rows], w, b, dy[rows], 1e-5)
+        check(y[rows], want, tol, "y")
+        check(dx[rows], want, tol, "dx")
+    total, bound = {"dw": 0.0, "db": 0.0}, {"dw": 0.0, "db": 0.0}
+    chain = T // 4096 + 1 + 4 + 64 + 16
+    for t in range(0, T, 2 ** 22):
+        xs, d = x[t:t + 2 ** 22].double(), dy[t:t + 2 ** 22].double()
+        xs -= xs.mean(-1, keepdim=True)
+        r = 1 / (xs.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+        ax = x[t:t + 2 ** 22].double().abs().mean(-1, keepdim=True)
+        xs *= r
+        total["dw"] += (d * xs).sum(0)
+        total["db"] += d.sum(0)
+        bound["dw"] += (d.abs() * N * (r * ax + xs.abs())).sum(0) + (chain + 2) * U * (d * xs).abs().sum(0)
+        bound["db"] += (chain + 2) * U * d.abs().sum(0)
+    check(dw, total, bound, "dw")
+    check(db, total, bound, "db")

@@ -547,3 +547,50 @@ def test_muon_on_a_side_stream(gpu_device):
         a.step()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(ps, twin))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("tall", [False, True], ids=["wide", "tall"])
+def test_largest_matrix(gpu_device, tall, dtype):
+    # 8192 x 65536, offsets up to 2^31 bytes; one step, every 13th column against 64 bits.  X = P X0: the
+    # error of P is at most its operands' roundings and its sums' losses, each relative to the Frobenius norm of
+    # what is rounded or summed, and a column of X is off by at most that times its X0's norm.
+    m, n = 8192, 65536
+    g = torch.Generator(gpu_device).manual_seed(5)
+    x = (torch.randn(m, 8, device=gpu_device, generator=g) @ torch.randn(8, n, device=gpu_device, generator=g)
+         + 0.01 * torch.randn(m, n, device=gpu_device, generator=g)).to(dtype)
+    got = orthogonalize(x.t().contiguous() if tall else x, steps=1)
+    got = (got.t() if tall else got)[:, ::13].double()
+    x0 = x.double()
+    del x
+    x0 /= x0.norm()
+    a = torch.zeros(m, m, dtype=torch.float64, device=gpu_device)
+    for part in x0.split(8192, 1):
+        a += part.contiguous() @ part.t().contiguous()
+    ca, cb, cc = NS_COEFFICIENTS
+    sq = a @ a
+    xs = x0[:, ::13].contiguous()
+    want = ca * xs + (cb * a + cc * sq) @ xs
+    f = lambda t: float(t.norm())
+    operand = 2.0 ** -11 if dtype == BF else 2.0 ** -21
+    step = 2.0 ** -23 * (1 if dtype == BF else 3)  # lost per accumulation of 32 (three of them in the 22-bit form)
+    top = float(torch.linalg.vector_norm(a @ xs[:, 0]) / torch.linalg.vector_norm(xs[:, 0])) * 1.5  # > largest value of A
+    err_a = (3 * operand + n / 32 * step) * f(a)          # X twice and A itself
+    err_p = (abs(cb) + 2 * abs(cc) * top) * err_a + m / 32 * step * abs(cc) * f(sq)
+    err_p += operand * (ca + f(cb * a + cc * sq))         # P's rounding
+    err = err_p + (operand + m / 32 * step) * (ca + f(cb * a + cc * sq))  # the last product
+    off = (got - want).norm(dim=0)
+    allowed = err * xs.norm(dim=0) + half(dtype) * want.norm(dim=0)
+    assert bool((off <= allowed).all()), (float((off / allowed).max()), int((off / allowed).argmax()))
+
+
+def test_many_large_matrices_in_one_launch(gpu_device):
+    # 20 of 8192 x 8192 in fp32: 5 GiB of X.  The same kernels run for one of them: the same bits.
+    g = torch.Generator(gpu_device).manual_seed(6)
+    x = torch.randn(20, 8192, 8192, device=gpu_device, generator=g)
+    out = torch.empty_like(x)
+    K.orthogonalize(list(x), list(out), 1, NS_COEFFICIENTS, 1e-7)
+    one = torch.empty_like(x[0])
+    for i in (0, 1, 7, 8, 13, 19):
+        K.orthogonalize([x[i]], [one], 1, NS_COEFFICIENTS, 1e-7)
+        assert torch.equal(one, out[i]), i
