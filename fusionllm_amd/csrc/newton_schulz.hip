@@ -529,12 +529,12 @@ __device__ __forceinline__ void ns_epilogue(const NsArgs& a, int cur, f32x4 (&ac
 // A step multiplies the stage that is in registers while it reads the next one from LDS and the copies
 // (global -> LDS, no registers) of the stage NST steps on go into the slot that has been read: one barrier
 // a step, and no latency in its way.  (64-row tiles: three stages, Gram product of 3 of 768 x 2048
-// 12.4 us against 17.0 with two; four were no faster.  128-row tiles: two, two workgroups per CU.)
+// 11.1 us against 16.8 with two; four were no faster.  128-row tiles: two, two workgroups per CU.)
 // The row operand, and the column operand of the symmetric products, are K-contiguous;
 // the step's column operand is X as it lies ([K, N]), read with transposing LDS reads
 // (gemm_core.h has both layouts and their swizzles).  SPLIT: a stage is hi and lo of 32 k, and a step
 // adds hi lo + lo hi + hi hi (three passes over K instead read each operand again: 3 matrices of 768 x
-// 2048, Gram product 32 us against 24).
+// 2048, Gram product 32 us against 21).
 template <int MODE, int TM, int NST, bool SPLIT, int OUT = NS_BF16>
 __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, const int cur) {
   using namespace core;
@@ -593,13 +593,11 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
   int left = steps;
   // the next stage's copies; past the last step the last stage again (into a slot that is free and
   // not read any more), so that every wait counts the same operations
-  auto issue = [&](int st) __attribute__((always_inline)) {
-    const uint32_t la = sbase + st * STAGE + w * 1024, lb = la + A_ST;
-#pragma unroll
-    for (int q = 0; q < CA; ++q) copy16(la + q * 4096, pa, aoff[q]);
-#pragma unroll
-    for (int q = 0; q < CB; ++q) copy16(lb + q * 4096, pb, boff[q]);
-    if (--left <= 0) return;
+  auto copy = [&](int st, int q) __attribute__((always_inline)) {
+    const uint32_t la = sbase + st * STAGE + w * 1024;
+    if (q < CA) copy16(la + q * 4096, pa, aoff[q < CA ? q : 0]);
+    else copy16(la + A_ST + (q - CA) * 4096, pb, boff[q < CA ? 0 : q - CA]);
+    if (q + 1 < CA + CB || --left <= 0) return;
     pa += RB;
     pb += bstep;
   };
@@ -619,25 +617,37 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
     const uint32_t src = sbase + slot * STAGE;
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
+      // opaque, so that what is added to them goes into the reads' offsets
+      uint32_t ra = src + (xa ^ (kh * 64u)), rb = src + (xb ^ (kh * 64u));
+      asm volatile("" : "+v"(ra), "+v"(rb));
 #pragma unroll
-      for (int i = 0; i < FM; ++i) f.a[kh][i] = *(const lds_half8*)(uintptr_t)(src + (xa ^ (kh * 64u)) + 2048u * i);
+      for (int i = 0; i < FM; ++i) f.a[kh][i] = *(const lds_half8*)(uintptr_t)(ra + 2048u * i);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        if constexpr (SYM) f.b[kh][j] = *(const lds_half8*)(uintptr_t)(src + (xb ^ (kh * 64u)) + 2048u * j);
+        if constexpr (SYM) f.b[kh][j] = *(const lds_half8*)(uintptr_t)(rb + 2048u * j);
         else f.b[kh][j] = __builtin_bit_cast(half8, tr_frag(((src + xb) ^ (j << 5)) + kh * TR_KHALF));
       }
     }
   };
 #pragma unroll
-  for (int st = 0; st < NST; ++st) issue(st);
+  for (int st = 0; st < NST; ++st)
+#pragma unroll
+    for (int q = 0; q < CA + CB; ++q) copy(st, q);
   Frags f0, f1;
   wait_vm_barrier<(NST - 1) * (CA + CB)>();
   read(f0, 0);
   int slot = 0;
+  // products between two copies, 0: all copies first.  (Update of 3 of 768 x 2048, hi + lo: 33 us with the
+  // copies first, 30 so; fp16 alone, two thirds of the products: 22.7 and 22.6, its Gram product 19.8 and 21.5.)
+  constexpr int EVERY = SPLIT && TM == 128 ? 4 : 0;
   auto step = [&](const Frags& now, Frags& next) __attribute__((always_inline)) {
     // the next stage is there, and every wave has this one in registers: its slot takes the stage NST on
     wait_vm_barrier<(NST - 2) * (CA + CB)>();
-    issue(slot);
+    const int free = slot;
+    if constexpr (EVERY == 0) {
+#pragma unroll
+      for (int q = 0; q < CA + CB; ++q) copy(free, q);
+    }
     slot = slot + 1 == NST ? 0 : slot + 1;
     read(next, slot);
     __builtin_amdgcn_s_setprio(1);
@@ -647,15 +657,27 @@ __global__ __launch_bounds__(256, 2) void ns_product_kernel(const NsArgs a, cons
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
+        for (int j = 0; j < FN; ++j) {
+          const int n = (x * FM + i) * FN + j;
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.b[SPLIT ? x == 0 : x][j], now.a[SPLIT ? x == 1 : x][i],
                                                              acc[i][j], 0, 0, 0);
+          if constexpr (EVERY > 0) {
+            if (n % EVERY == 0 && n / EVERY < CA + CB) {
+              __builtin_amdgcn_sched_barrier(0);
+              copy(free, n / EVERY);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        }
     __builtin_amdgcn_s_setprio(0);
   };
-  for (int it = 0; it < steps; it += 2) {
+  // two steps without a branch between them (a branch lets the compiler move the first one's reads past
+  // its products, to where they are used)
+  for (int it = 0; it + 1 < steps; it += 2) {
     step(f0, f1);
-    if (it + 1 < steps) step(f1, f0);
+    step(f1, f0);
   }
+  if (steps & 1) step(f0, f1);
   wait_vm_barrier<0>();  // the copies past the end have landed: the epilogue takes their LDS
   ns_epilogue<MODE, SPLIT, OUT>(a, cur, acc, smem + w * EPI, lane, mat, ti * TM + wm * WTM, tj * TN + wn * WTN,
                                 ti != tj);
@@ -1255,13 +1277,13 @@ inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
   // 256 x 256 tiles, persistent, where they fill the chip and pad little (their area is at most 1.5 times
   // the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 56 us against 65, of 22
   // (132 tiles) 52 against 47; of 64 of 384 x 2048 (twice the area) 56 against 45.  Then 128 x
-  // 128 tiles where there is one per CU: Gram product of 5 of 1408 x 2048 (330 tiles) 39 us
-  // against 44, of 5 of 1001 x 1503 (180 tiles) 24 against 20; 48 rows would leave
+  // 128 tiles where there is one for most CUs: Gram product of 12 of 768 x 2048 (252 tiles) 27 us
+  // against 31, of 5 of 1001 x 1503 (180 tiles) 20 against 19; 48 rows would leave
   // most of a 128-row tile empty.
   if (t256 >= 160 && 8 * t256 < 3 * t128) {
     ns_big_kernel<MODE, SPLIT, OUT>
         <<<dim3(static_cast<unsigned>(std::min<int64_t>(8 * ceil_div(t256, 8), kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
-  } else if (t128 >= 256 && t64 > t128) {
+  } else if (t128 >= 192 && t64 > t128) {
     ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
   } else {
     ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<grid(t64), dim3(256), 0, s>>>(a, cur);
