@@ -926,22 +926,25 @@ __global__ __launch_bounds__(core::NT, 1) void ns_big_kernel(const NsArgs a, con
 // a launch).  A workgroup has 128 columns of X.  It adds the workgroups' partial Gram
 // matrices of the launch before (in a fixed order), forms a I + b A + c A^2 for itself, multiplies
 // its columns and writes the partial Gram matrix of the result for the next launch.  Five steps, bf16,
-// against three launches a step (most of them the Gram matrix's one tile), in a graph: 64 x 2048 72 us
-// against 145, 8 of 32 x 2048 79 against 147, 27 of 64 x 768 86 against 105.  Where many long ones go
-// together every workgroup's sum over the partial matrices counts: 64 of 64 x 2048 237 us
-// against 215, 64 of 64 x 4096 515 against 359.  The rule leaves their number out all the same, so that a
+// against three launches a step (most of them the Gram matrix's one tile), in a graph: 64 x 2048 64 us
+// against 145, 8 of 32 x 2048 72 against 147, 27 of 64 x 768 72 against 105.  Where many long ones go
+// together every workgroup's sum over the partial matrices counts: 64 of 64 x 2048 235 us
+// against 215, 64 of 64 x 4096 529 against 359.  The rule leaves their number out all the same, so that a
 // matrix's result is the same whatever goes with it.
 
 constexpr int kSmallSide = 64;        // the small side, at most (and the padded one)
 constexpr int kSmallPanel = 128;      // columns per workgroup
-constexpr int kSmallMaxPanels = 32;   // every workgroup adds the partial matrices of all (64 x 4096: 88 us
+constexpr int kSmallMaxPanels = 32;   // every workgroup adds the partial matrices of all (64 x 4096: 76 us
                                       // against 228)
 constexpr int kSmallBlocks = 10;      // 16 x 16 blocks of a Gram matrix on or below the diagonal
+// Waves per workgroup, by the 16-row blocks of X: 8 (64 x 2048 64 us, 27 of 64 x 768 72; four waves 72 and 86), 4
+// for one block, which leaves the others little (64 of 16 x 4096 152 us, with eight 184).
+constexpr int small_waves(int mb) { return mb > 1 ? 8 : 4; }
 constexpr int kLdA = 68, kLdX = 132;  // LDS strides
 
 struct SmallLds {
   float a[kSmallSide * kLdA], b[kSmallSide * kLdA], x[kSmallSide * kLdX];
-  double red[4];
+  double red[8];
   int e;
 };
 
@@ -955,10 +958,10 @@ __device__ __forceinline__ void small_block(int t, int& i, int& j) {
   j = t - i * (i + 1) / 2;
 }
 
-// Partial Gram matrix of the panel in LDS: blocks w, w + 4, w + 8 by wave w.  MB: 16-row blocks of X.
+// Partial Gram matrix of the panel in LDS: blocks w, w + 8 by wave w (of eight).  MB: 16-row blocks of X.
 template <int MB>
 __device__ __forceinline__ void small_gram(const NsArgs& a, const SmallLds& s, int mat, int panel, int parity) {
-  constexpr int BLOCKS = MB * (MB + 1) / 2, PER = (BLOCKS + 3) / 4;
+  constexpr int BLOCKS = MB * (MB + 1) / 2, NW = small_waves(MB), PER = (BLOCKS + NW - 1) / NW;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int cols = min(a.n - panel * kSmallPanel, kSmallPanel);  // zeros after them
   float* out = a.sparts + ((static_cast<int64_t>(parity) * a.count + mat) * a.panels + panel) * (kSmallBlocks * 256);
@@ -967,7 +970,7 @@ __device__ __forceinline__ void small_gram(const NsArgs& a, const SmallLds& s, i
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     int i, j;
-    small_block(min(w + 4 * u, BLOCKS - 1), i, j);
+    small_block(min(w + NW * u, BLOCKS - 1), i, j);
     p[u] = s.x + (16 * i + (lane & 15)) * kLdX + (lane >> 4);
     q[u] = s.x + (16 * j + (lane & 15)) * kLdX + (lane >> 4);
     c[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -979,17 +982,18 @@ __device__ __forceinline__ void small_gram(const NsArgs& a, const SmallLds& s, i
       for (int u = 0; u < PER; ++u) c[u] = mfma_f32(p[u][k0 + k], q[u][k0 + k], c[u]);
 #pragma unroll
   for (int u = 0; u < PER; ++u)
-    if (w + 4 * u < BLOCKS) *reinterpret_cast<f32x4*>(out + (w + 4 * u) * 256 + lane * 4) = c[u];
+    if (w + NW * u < BLOCKS) *reinterpret_cast<f32x4*>(out + (w + NW * u) * 256 + lane * 4) = c[u];
 }
 
-// A thread's share of the panel's elements as they lie in the matrix: chunk t of 8 (t < kSmallChunks).
-constexpr int kSmallChunks = kSmallSide * kSmallPanel / 8 / 256;
+// A thread's share (one of NT) of the panel's elements as they lie in the matrix: chunk t of 8 (t < COUNT).
+template <int NT>
 struct SmallChunk {
+  static constexpr int COUNT = kSmallSide * kSmallPanel / 8 / NT;
   int64_t o;       // offset in the matrix
   int n, r, c;     // valid elements; row and column of X of the first
   bool down;       // the 8 go down a column of X
   __device__ __forceinline__ SmallChunk(const NsArgs& a, int mat, int panel, int t) {
-    const int c0 = panel * kSmallPanel, id = t * 256 + threadIdx.x;
+    const int c0 = panel * kSmallPanel, id = t * NT + threadIdx.x;
     down = (a.tall >> mat) & 1;
     if (down) {
       const int per = (a.m + 7) / 8;
@@ -1010,21 +1014,22 @@ struct SmallChunk {
 // X of the panel, still without the norm (times a power of two that brings the panel's
 // norm to 1/2 .. 1), its sum of squares in fp64 and its partial Gram matrix; Muon: the new momentum.
 template <int DT, bool MUON, int MB>
-__global__ __launch_bounds__(256, 2) void ns_small_load_kernel(const NsArgs a) {
+__global__ __launch_bounds__(64 * small_waves(MB), 2) void ns_small_load_kernel(const NsArgs a) {
+  constexpr int NW = small_waves(MB), NT = 64 * NW;
   __shared__ SmallLds s;
   const int panel = blockIdx.x, mat = blockIdx.y;
-  float u[kSmallChunks][8], v[MUON ? kSmallChunks : 1][8];
+  float u[SmallChunk<NT>::COUNT][8], v[MUON ? SmallChunk<NT>::COUNT : 1][8];
 #pragma unroll
-  for (int t = 0; t < kSmallChunks; ++t) {
-    const SmallChunk k(a, mat, panel, t);
+  for (int t = 0; t < SmallChunk<NT>::COUNT; ++t) {
+    const SmallChunk<NT> k(a, mat, panel, t);
     ns_load8<DT>(a.src[mat], k.o, k.n, u[t]);
     if constexpr (MUON) ns_load8<DT>(a.buf[mat], k.o, k.n, v[t]);
   }
-  for (int t = threadIdx.x; t < kSmallSide * kLdX; t += 256) s.x[t] = 0.0f;
+  for (int t = threadIdx.x; t < kSmallSide * kLdX; t += NT) s.x[t] = 0.0f;
   double ss = 0.0;
 #pragma unroll
-  for (int t = 0; t < kSmallChunks; ++t) {
-    const SmallChunk k(a, mat, panel, t);
+  for (int t = 0; t < SmallChunk<NT>::COUNT; ++t) {
+    const SmallChunk<NT> k(a, mat, panel, t);
     if constexpr (MUON) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1041,7 +1046,8 @@ __global__ __launch_bounds__(256, 2) void ns_small_load_kernel(const NsArgs a) {
   for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
   if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = ss;
   __syncthreads();
-  ss = ((s.red[0] + s.red[1]) + s.red[2]) + s.red[3];
+  ss = s.red[0];
+  for (int i = 1; i < NW; ++i) ss = ss + s.red[i];
   int e = 0;
   if (ss > 0.0 && ss < 1e300) {
     frexp(sqrt(ss), &e);
@@ -1053,8 +1059,8 @@ __global__ __launch_bounds__(256, 2) void ns_small_load_kernel(const NsArgs a) {
   }
   const float f = fm_pow2i(-e);
 #pragma unroll
-  for (int t = 0; t < kSmallChunks; ++t) {
-    const SmallChunk k(a, mat, panel, t);
+  for (int t = 0; t < SmallChunk<NT>::COUNT; ++t) {
+    const SmallChunk<NT> k(a, mat, panel, t);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < k.n) s.x[k.lds(i)] = u[t][i] * f;
@@ -1062,22 +1068,24 @@ __global__ __launch_bounds__(256, 2) void ns_small_load_kernel(const NsArgs a) {
   __syncthreads();
   float* x = a.xs + (static_cast<int64_t>(mat) * a.panels + panel) * (kSmallSide * kSmallPanel);
 #pragma unroll 4
-  for (int t = threadIdx.x; t < 16 * MB * kSmallPanel; t += 256) x[t] = s.x[(t / kSmallPanel) * kLdX + t % kSmallPanel];
+  for (int t = threadIdx.x; t < 16 * MB * kSmallPanel; t += NT) x[t] = s.x[(t / kSmallPanel) * kLdX + t % kSmallPanel];
   small_gram<MB>(a, s, mat, panel, 0);
 }
 
 // One step of a panel (step k reads the partial matrices of parity k % 2 and writes the others).
 template <bool LAST, int OUT, int MB>
-__global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, const int k) {
-  constexpr int BLOCKS = MB * (MB + 1) / 2, PER = (BLOCKS + 3) / 4, XV = 16 * MB * kSmallPanel / 256;
-  constexpr int BATCH = 16;  // partial matrices in flight
+__global__ __launch_bounds__(64 * small_waves(MB), small_waves(MB) / 2) void ns_small_step_kernel(const NsArgs a, const int k) {
+  constexpr int BLOCKS = MB * (MB + 1) / 2, NW = small_waves(MB), NT = 64 * NW, PER = (BLOCKS + NW - 1) / NW;
+  constexpr int XV = 16 * MB * kSmallPanel / NT;
+  constexpr int BATCH = 8;  // partial matrices in flight (sixteen take the registers of a second workgroup: 64 of 64 x 2048
+                            // 295 us against 235)
   __shared__ SmallLds s;
   const int panel = blockIdx.x, mat = blockIdx.y;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   float* x = a.xs + (static_cast<int64_t>(mat) * a.panels + panel) * (kSmallSide * kSmallPanel);
   float xv[XV];
 #pragma unroll
-  for (int t = 0; t < XV; ++t) xv[t] = x[t * 256 + threadIdx.x];
+  for (int t = 0; t < XV; ++t) xv[t] = x[t * NT + threadIdx.x];
   // the first step's X and A still lack the norm: panel p's X the factor 2^e / |u| (lane p has it)
   float mine = 1.0f;
   if (k == 0) {
@@ -1087,7 +1095,7 @@ __global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, c
     const double nrm = sqrt(ss);
     mine = static_cast<float>(ldexp(1.0 / (nrm < a.eps ? a.eps : nrm), lane < a.panels ? a.exps[mat * a.panels + lane] : 0));
   }
-  // A: blocks w, w + 4, w + 8 by wave w, the panels in order
+  // A: blocks w, w + NW by wave w, the panels in order
   const float* parts = a.sparts + (static_cast<int64_t>(k & 1) * a.count + mat) * a.panels * (kSmallBlocks * 256);
   f32x4 sum[PER];
 #pragma unroll
@@ -1099,7 +1107,7 @@ __global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, c
 #pragma unroll
       for (int u = 0; u < PER; ++u)
         v[u][p] = *reinterpret_cast<const f32x4*>(parts + min(p0 + p, a.panels - 1) * (kSmallBlocks * 256) +
-                                                  min(w + 4 * u, BLOCKS - 1) * 256 + lane * 4);
+                                                  min(w + NW * u, BLOCKS - 1) * 256 + lane * 4);
     __builtin_amdgcn_sched_barrier(0);  // all of them in flight
 #pragma unroll
     for (int p = 0; p < BATCH; ++p) {
@@ -1113,9 +1121,9 @@ __global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, c
   }
 #pragma unroll
   for (int u = 0; u < PER; ++u)
-    if (w + 4 * u < BLOCKS) {
+    if (w + NW * u < BLOCKS) {
       int i, j;
-      small_block(w + 4 * u, i, j);
+      small_block(w + NW * u, i, j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 16 * i + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
@@ -1126,68 +1134,71 @@ __global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, c
   const float f = __shfl(mine, panel, 64);
 #pragma unroll
   for (int t = 0; t < XV; ++t) {
-    const int q = t * 256 + threadIdx.x;
+    const int q = t * NT + threadIdx.x;
     s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel] = xv[t] * f;
   }
   __syncthreads();
-  // B = a I + b A + c A^2: rows 16 w .. + 15 by wave w
-  if (w < MB) {
-    f32x4 c[MB];
+  // B = a I + b A + c A^2: two waves for 16 rows
+  constexpr int JB = MB > 1 ? MB / 2 : 1;
+  const int bi = w >> 1, bj = (w & 1) * JB;
+  if (bi < MB && bj < MB) {
+    f32x4 c[JB];
 #pragma unroll
-    for (int j = 0; j < MB; ++j) c[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < JB; ++j) c[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* p = s.a + (lane & 15) * kLdA + (lane >> 4);  // (A is symmetric)
 #pragma unroll
     for (int q = 0; q < 16 * MB; q += 4)
 #pragma unroll
-      for (int j = 0; j < MB; ++j) c[j] = mfma_f32(p[16 * w * kLdA + q], p[16 * j * kLdA + q], c[j]);
+      for (int j = 0; j < JB; ++j) c[j] = mfma_f32(p[16 * bi * kLdA + q], p[16 * (bj + j) * kLdA + q], c[j]);
 #pragma unroll
-    for (int j = 0; j < MB; ++j)
+    for (int j = 0; j < JB; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = 16 * w + 4 * (lane >> 4) + e, q = 16 * j + (lane & 15);
+        const int r = 16 * bi + 4 * (lane >> 4) + e, q = 16 * (bj + j) + (lane & 15);
         const float v = fmaf(a.cb, s.a[r * kLdA + q], a.cc * c[j][e]);
         s.b[r * kLdA + q] = r == q ? v + a.ca : v;
       }
   }
   __syncthreads();
-  // X = B X: columns 32 w .. + 31 by wave w (in place after the last read of its own columns)
+  // X = B X: a column block or two by each wave (in place after the last read of its own columns)
   {
-    f32x4 c[MB][2];
+    constexpr int JX = kSmallPanel / 16 / NW;
+    f32x4 c[MB][JX];
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < JX; ++j) c[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* p = s.b + (lane & 15) * kLdA + (lane >> 4);
-    const float* y = s.x + (lane >> 4) * kLdX + 32 * w + (lane & 15);
+    const float* y = s.x + (lane >> 4) * kLdX + 16 * JX * w + (lane & 15);
 #pragma unroll
     for (int q = 0; q < 16 * MB; q += 4)
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) c[i][j] = mfma_f32(p[16 * i * kLdA + q], y[q * kLdX + 16 * j], c[i][j]);
+        for (int j = 0; j < JX; ++j) c[i][j] = mfma_f32(p[16 * i * kLdA + q], y[q * kLdX + 16 * j], c[i][j]);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < JX; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s.x[(16 * i + 4 * (lane >> 4) + e) * kLdX + 32 * w + 16 * j + (lane & 15)] = c[i][j][e];
+          s.x[(16 * i + 4 * (lane >> 4) + e) * kLdX + 16 * (JX * w + j) + (lane & 15)] = c[i][j][e];
   }
   __syncthreads();
   if constexpr (LAST) {
     constexpr int DT = OUT & 1;
     constexpr bool MUON = OUT >= NS_MUON_BF16;
-    float p[MUON ? kSmallChunks : 1][8];
+    float p[MUON ? SmallChunk<NT>::COUNT : 1][8];
     if constexpr (MUON)
 #pragma unroll
-      for (int t = 0; t < kSmallChunks; ++t) {
-        const SmallChunk q(a, mat, panel, t);
+      for (int t = 0; t < SmallChunk<NT>::COUNT; ++t) {
+        const SmallChunk<NT> q(a, mat, panel, t);
         ns_load8<DT>(a.dst[mat], q.o, q.n, p[t]);
       }
 #pragma unroll
-    for (int t = 0; t < kSmallChunks; ++t) {
-      const SmallChunk q(a, mat, panel, t);
+    for (int t = 0; t < SmallChunk<NT>::COUNT; ++t) {
+      const SmallChunk<NT> q(a, mat, panel, t);
       if (q.n <= 0) continue;
       float v[8];
 #pragma unroll
@@ -1200,7 +1211,7 @@ __global__ __launch_bounds__(256, 2) void ns_small_step_kernel(const NsArgs a, c
   } else {
 #pragma unroll 4
     for (int t = 0; t < XV; ++t) {
-      const int q = t * 256 + threadIdx.x;
+      const int q = t * NT + threadIdx.x;
       x[q] = s.x[(q / kSmallPanel) * kLdX + q % kSmallPanel];
     }
     small_gram<MB>(a, s, mat, panel, (k + 1) & 1);
@@ -1342,7 +1353,7 @@ inline int ns_run_small(NsArgs& a, int steps, void* workspace, hipStream_t s) {
   a.exps = reinterpret_cast<int*>(p + l.norm);
   a.xs = reinterpret_cast<float*>(p + l.norm + l.exps);
   a.sparts = reinterpret_cast<float*>(p + l.norm + l.exps + l.x);
-  const dim3 grid(a.panels, a.count), block(256);
+  const dim3 grid(a.panels, a.count), block(64 * small_waves(MB));
   constexpr int out = DT + (MUON ? 2 : 0);
   ns_small_load_kernel<DT, MUON, MB><<<grid, block, 0, s>>>(a);
   for (int k = 0; k + 1 < steps; ++k) ns_small_step_kernel<false, NS_BF16, MB><<<grid, block, 0, s>>>(a, k);
