@@ -300,7 +300,7 @@ __device__ __forceinline__ void ns_result8(const NsArgs& a, void* dst, int64_t o
 // return 8 consecutive elements of a column.  What the epilogue reads is asked for first, so
 // that its latency is not paid per slice.  (Epilogues straight from the accumulators, 8 bytes
 // per lane in 16 rows at once, or with the reads slice by slice, took two thirds of a step:
-// 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone; now 98, of which
+// 27 matrices of 768 x 2048, 141 - 182 us against 53 for the product alone; now 92 .. 98, of which
 // the stores are 32.)
 //
 // Pieces of 8 elements sit at a uniform address plus one offset per lane, and whether they are inside
