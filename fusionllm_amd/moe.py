@@ -44,6 +44,7 @@ import contextlib
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _kernels as K
 from .norm import LayerNorm, check_norm_operands
@@ -503,6 +504,7 @@ class _LayerNormMoEResidualFunction(torch.autograd.Function):
         return y, idx64, w, counts
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, _d_idx, _d_w, _d_counts):
         n_w = len(ctx.param_dtypes[2])
         if dy is None:

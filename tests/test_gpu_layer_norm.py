@@ -521,3 +521,37 @@ def test_more_rows_than_one_launch_and_32_bit_offsets_take(gpu_device):
         bound["db"] += (chain + 2) * U * d.abs().sum(0)
     check(dw, total, bound, "dw")
     check(db, total, bound, "db")
+
+
+def test_second_derivatives_of_the_fused_form_are_refused(gpu_device):
+    # not left out in silence, also where another term of the sum has one
+    cfg = configs.BlockConfig("t", 9, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=3)
+    moe = build_module(cfg, data, gpu_device, BF)
+    norm = LayerNorm(128).to(gpu_device, BF)
+    x = data.x.to(gpu_device, BF).requires_grad_(True)
+    (want,) = torch.autograd.grad(moe_residual(x, norm, moe).float().square().sum(), x)
+    (g,) = torch.autograd.grad(moe_residual(x, norm, moe).float().square().sum(), x, create_graph=True)
+    assert torch.equal(g, want)
+    with pytest.raises(RuntimeError):
+        (g.float().sum() + x.float().square().sum()).backward()
+
+
+def test_moe_residual_of_fp32_outside_autocast(gpu_device):
+    cfg = configs.BlockConfig("t", 33, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=3)
+    moe = build_module(cfg, data, gpu_device, F32)
+    norm = LayerNorm(128).to(gpu_device)
+    moe2, norm2 = copy.deepcopy(moe), copy.deepcopy(norm)
+    x = data.x.to(gpu_device, F32).requires_grad_(True)
+    x2 = x.detach().clone().requires_grad_(True)
+    dy = data.dy.to(gpu_device, F32)
+    y, y2 = moe_residual(x, norm, moe), x2 + moe2(norm2(x2))
+    y.backward(dy)
+    y2.backward(dy)
+    assert y.dtype == F32 and torch.equal(moe._last_indices, moe2._last_indices)
+    # the block takes bf16 copies of the norm's output either way; its fp32 results are added in fp32
+    tol = 2.0 ** -7
+    for got, want in ((y, y2), (x.grad, x2.grad), (norm.weight.grad, norm2.weight.grad),
+                      (norm.bias.grad, norm2.bias.grad)):
+        assert float((got.double() - want.double()).norm()) <= tol * float(want.double().norm())
