@@ -21,6 +21,7 @@ fp32 matrices on pairs of fp16 operands (22 bits).
 """
 from __future__ import annotations
 
+import bisect
 import math
 
 import torch
@@ -93,22 +94,29 @@ def _sides(t):
 
 def _launches(items, written):
     """Lists of items (tuples whose first tensor is the matrix) for one launch each: one device, dtype and
-    pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two that write the same storage
-    (written(item): addresses); in order where they do."""
+    pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two that write the same memory
+    (written(item): tensors); in order where they do."""
     open_: dict = {}
     out = []
     for it in items:
         t = it[0]
         key = (t.device, t.dtype, _sides(t))
         most = min(K.MUON_MAX_TENSORS, max(1, LAUNCH_ELEMENTS // t.numel()))
-        addr = written(it)
+        spans = [(w.data_ptr(), w.data_ptr() + w.numel() * w.element_size()) for w in written(it)]
         cur = open_.get(key)
-        if cur is None or len(cur[0]) >= most or not cur[1].isdisjoint(addr):
-            cur = open_[key] = ([], set())
+        if cur is None or len(cur[0]) >= most or any(_overlaps(cur[1], s) for s in spans):
+            cur = open_[key] = ([], [])
             out.append(cur[0])
         cur[0].append(it)
-        cur[1].update(addr)
+        for s in spans:
+            bisect.insort(cur[1], s)
     return out
+
+
+def _overlaps(spans, span):
+    """Whether a span of addresses meets one of the sorted, disjoint spans."""
+    i = bisect.bisect(spans, span)
+    return (i > 0 and spans[i - 1][1] > span[0]) or (i < len(spans) and spans[i][0] < span[1])
 
 
 def _check_ns(steps, coefficients, eps):
@@ -157,7 +165,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
         outs.append(out)
         if t.numel():
             items += zip(t.view(-1, *t.shape[-2:]), out.view(-1, *t.shape[-2:]))
-    for chunk in _launches(items, lambda it: (it[1].data_ptr(),)):
+    for chunk in _launches(items, lambda it: it[1:]):
         with torch.cuda.device(chunk[0][0].device):
             K.orthogonalize([c[0] for c in chunk], [c[1] for c in chunk], steps, coefficients, eps)
     return outs[0] if single else outs
@@ -228,7 +236,7 @@ class Muon(Optimizer):
                     state["momentum_buffer"] = torch.zeros_like(p)
                 items.append((p, g.contiguous(), state["momentum_buffer"]))
             lr, wd = float(group["lr"]), float(group["weight_decay"])
-            for chunk in _launches(items, lambda it: (it[0].data_ptr(), it[2].data_ptr())):
+            for chunk in _launches(items, lambda it: (it[0], it[2])):
                 small, large = _sides(chunk[0][0])
                 if group["adjust_lr_fn"] == "match_rms_adamw":
                     tall = wide = lr * 0.2 * math.sqrt(large)

@@ -594,3 +594,20 @@ def test_many_large_matrices_in_one_launch(gpu_device):
     for i in (0, 1, 7, 8, 13, 19):
         K.orthogonalize([x[i]], [one], 1, NS_COEFFICIENTS, 1e-7)
         assert torch.equal(one, out[i]), i
+
+
+def test_muon_of_overlapping_parameters(gpu_device):
+    # rows 0 .. 39 and 20 .. 59 of one matrix, given together: one after the other, as the formulas say
+    g = torch.Generator(gpu_device).manual_seed(3)
+    base = torch.randn(60, 96, device=gpu_device, generator=g)
+    grads = [torch.randn(40, 96, device=gpu_device, generator=g) for _ in range(2)]
+
+    def run(groups, t):
+        ps = [torch.nn.Parameter(t[:40]), torch.nn.Parameter(t[20:])]
+        for p, q in zip(ps, grads):
+            p.grad = q
+        for group in groups:
+            Muon([ps[i] for i in group], lr=0.1).step()
+        return t
+
+    assert torch.equal(run([(0, 1)], base.clone()), run([(0,), (1,)], base.clone()))
