@@ -92,31 +92,64 @@ def _sides(t):
     return (r, c) if r <= c else (c, r)
 
 
-def _launches(items, written):
+class _Spans:
+    """Ranges of addresses, kept sorted and disjoint (those that meet become one)."""
+
+    def __init__(self):
+        self.lo, self.hi = [], []
+
+    def _meeting(self, lo, hi):
+        return bisect.bisect_right(self.hi, lo), bisect.bisect_left(self.lo, hi)
+
+    def meets(self, lo, hi):
+        i, j = self._meeting(lo, hi)
+        return i < j
+
+    def add(self, lo, hi):
+        i, j = self._meeting(lo, hi)
+        if i < j:
+            lo, hi = min(lo, self.lo[i]), max(hi, self.hi[j - 1])
+        self.lo[i:j], self.hi[i:j] = [lo], [hi]
+
+
+def _span(t):
+    """Addresses from a tensor's first element to the end of its last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+class _Launch:
+    def __init__(self):
+        self.items, self.written, self.read = [], _Spans(), _Spans()
+
+    def conflicts(self, written, read):
+        return (any(self.written.meets(*s) or self.read.meets(*s) for s in written)
+                or any(self.written.meets(*s) for s in read))
+
+
+def _launches(items, written, read=lambda it: ()):
     """Lists of items (tuples whose first tensor is the matrix) for one launch each: one device, dtype and
-    pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two that write the same memory
-    (written(item): tensors); in order where they do."""
-    open_: dict = {}
-    out = []
+    pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two of which one writes
+    memory that the other writes or reads (written(item), read(item): tensors).  Two such items, of whatever
+    sides, are in launches of their order: an item joins its sides' last launch only if it conflicts
+    neither with that nor with any launch behind it."""
+    last: dict = {}  # place of the last launch of each device, dtype and sides
+    out: list = []
     for it in items:
         t = it[0]
         key = (t.device, t.dtype, _sides(t))
         most = min(K.MUON_MAX_TENSORS, max(1, LAUNCH_ELEMENTS // t.numel()))
-        spans = [(w.data_ptr(), w.data_ptr() + w.numel() * w.element_size()) for w in written(it)]
-        cur = open_.get(key)
-        if cur is None or len(cur[0]) >= most or any(_overlaps(cur[1], s) for s in spans):
-            cur = open_[key] = ([], [])
-            out.append(cur[0])
-        cur[0].append(it)
-        for s in spans:
-            bisect.insort(cur[1], s)
-    return out
-
-
-def _overlaps(spans, span):
-    """Whether a span of addresses meets one of the sorted, disjoint spans."""
-    i = bisect.bisect(spans, span)
-    return (i > 0 and spans[i - 1][1] > span[0]) or (i < len(spans) and spans[i][0] < span[1])
+        w, r = [_span(x) for x in written(it)], [_span(x) for x in read(it)]
+        at = last.get(key)
+        if at is None or len(out[at].items) >= most or any(c.conflicts(w, r) for c in out[at:]):
+            at = last[key] = len(out)
+            out.append(_Launch())
+        out[at].items.append(it)
+        for s in w:
+            out[at].written.add(*s)
+        for s in r:
+            out[at].read.add(*s)
+    return [c.items for c in out]
 
 
 def _check_ns(steps, coefficients, eps):
@@ -234,16 +267,16 @@ class Muon(Optimizer):
                 state = self.state[p]
                 if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p)
-                items.append((p, g.contiguous(), state["momentum_buffer"]))
+                items.append((p, g, state["momentum_buffer"]))
             lr, wd = float(group["lr"]), float(group["weight_decay"])
-            for chunk in _launches(items, lambda it: (it[0], it[2])):
+            for chunk in _launches(items, lambda it: (it[0], it[2]), lambda it: (it[1],)):
                 small, large = _sides(chunk[0][0])
                 if group["adjust_lr_fn"] == "match_rms_adamw":
                     tall = wide = lr * 0.2 * math.sqrt(large)
                 else:
                     tall, wide = lr * math.sqrt(large / small), lr
                 with torch.cuda.device(chunk[0][0].device):
-                    K.muon_step([c[0] for c in chunk], [c[1] for c in chunk], [c[2] for c in chunk], tall, wide,
-                                1.0 - lr * wd, group["momentum"], group["nesterov"], group["ns_steps"],
+                    K.muon_step([c[0] for c in chunk], [c[1].contiguous() for c in chunk], [c[2] for c in chunk],
+                                tall, wide, 1.0 - lr * wd, group["momentum"], group["nesterov"], group["ns_steps"],
                                 group["ns_coefficients"], group["eps"])
         return loss

@@ -611,3 +611,21 @@ def test_muon_of_overlapping_parameters(gpu_device):
         return t
 
     assert torch.equal(run([(0, 1)], base.clone()), run([(0,), (1,)], base.clone()))
+
+
+def test_muon_of_overlapping_parameters_of_other_sides(gpu_device):
+    # rows 0 .. 19, 15 .. 44 and 40 .. 59 of one matrix: each update as if it were alone, in their order
+    g = torch.Generator(gpu_device).manual_seed(4)
+    base = torch.randn(60, 96, device=gpu_device, generator=g)
+    cuts = ((0, 20), (15, 45), (40, 60))
+    grads = [torch.randn(b - a, 96, device=gpu_device, generator=g) for a, b in cuts]
+
+    def run(groups, t):
+        ps = [torch.nn.Parameter(t[a:b]) for a, b in cuts]
+        for p, q in zip(ps, grads):
+            p.grad = q
+        for group in groups:
+            Muon([ps[i] for i in group], lr=0.1).step()
+        return t
+
+    assert torch.equal(run([(0, 1, 2)], base.clone()), run([(0,), (1,), (2,)], base.clone()))
