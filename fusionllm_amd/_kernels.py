@@ -645,6 +645,12 @@ def _matrices(groups, names):
     return [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in groups], rows, cols
 
 
+def check_newton_schulz(steps: int, coefficients) -> None:
+    """Raises what a launch with these would (host only)."""
+    check(_lib.load().fmoe_newton_schulz_check(int(steps), (ctypes.c_double * 3)(*coefficients)),
+          "fmoe_newton_schulz_check")
+
+
 def _muon_workspace(lib, like, n):
     nbytes = lib.fmoe_orthogonalize_workspace_bytes(like.shape[0], like.shape[1], n, _dtype_code(like.dtype))
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=like.device)

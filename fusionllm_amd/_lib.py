@@ -14,7 +14,7 @@ from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfusionmoe.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 MAX_EXPERTS = 64
 MAX_TOPK = 8
 
@@ -79,6 +79,7 @@ TRAIN_SIGNATURES = {
     "fmoe_layer_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "fmoe_layer_norm_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, _P, _P, c_int, _P, c_int64, c_int64,
                                     _P, _P, _P, _P, c_size_t, _P]),
+    "fmoe_newton_schulz_check": (c_int, [c_int, POINTER(c_double)]),
     "fmoe_orthogonalize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "fmoe_orthogonalize": (c_int, [_PP, _PP, POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_int,
                                    POINTER(c_double), c_double, _P, c_size_t, _P]),

@@ -1423,6 +1423,11 @@ inline bool ns_elem_aligned(const void* p, int dtype) {
 
 using namespace fmoe;
 
+extern "C" int fmoe_newton_schulz_check(int steps, const double* coeffs) {
+  if (steps < 1 || steps > FMOE_MUON_MAX_STEPS || !coeffs) return FMOE_ERR_INVALID_ARG;
+  return ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps) ? FMOE_OK : FMOE_ERR_COEFFICIENTS;
+}
+
 extern "C" size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype) {
   if (rows <= 0 || cols <= 0 || rows > FMOE_MUON_MAX_SIDE || cols > FMOE_MUON_MAX_SIDE || n_tensors <= 0 ||
       n_tensors > kNsMax)
@@ -1439,7 +1444,7 @@ extern "C" int fmoe_orthogonalize(const void* const* src, void* const* dst, cons
   if (dtype != FMOE_BF16 && dtype != FMOE_F32) return FMOE_ERR_DTYPE;
   if (n_tensors == 0) return FMOE_OK;
   if (!src || !dst || !rows || !cols || !coeffs || !(eps > 0.0)) return FMOE_ERR_INVALID_ARG;
-  if (!ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps)) return FMOE_ERR_COEFFICIENTS;
+  if (const int rc = fmoe_newton_schulz_check(steps, coeffs)) return rc;
   NsArgs a = {};
   a.count = n_tensors;
   a.dtype = dtype;
@@ -1462,7 +1467,7 @@ extern "C" int fmoe_muon_step(void* const* params, const void* const* grads, voi
   if (dtype != FMOE_BF16 && dtype != FMOE_F32) return FMOE_ERR_DTYPE;
   if (n_tensors == 0) return FMOE_OK;
   if (!params || !grads || !momentum_bufs || !rows || !cols || !coeffs || !(eps > 0.0)) return FMOE_ERR_INVALID_ARG;
-  if (!ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps)) return FMOE_ERR_COEFFICIENTS;
+  if (const int rc = fmoe_newton_schulz_check(steps, coeffs)) return rc;
   NsArgs a = {};
   a.count = n_tensors;
   a.dtype = dtype;

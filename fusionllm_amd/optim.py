@@ -215,7 +215,8 @@ class Muon(Optimizer):
     lr 0.2 sqrt(max(rows, cols)) ("match_rms_adamw").  The constructor and the
     state ("momentum_buffer") are those of ``torch.optim.Muon``.  Parameters are
     matrices on a ROCm device, bf16 or fp32, with gradients of their own dtype;
-    every matrix of one dtype and pair of sides is updated in the same launches."""
+    every matrix of one dtype and pair of sides is updated in the same launches.
+    What a step refuses it refuses before anything is updated."""
 
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
@@ -236,16 +237,45 @@ class Muon(Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        ps = self.param_groups[-1]["params"]
+        group = self.param_groups[-1]
+        ps = group["params"]
         try:
             if len(set(ps)) != len(ps):
                 raise ValueError("a parameter is given twice")
             for p in ps:
                 if p.dim() != 2:
                     raise ValueError(f"Muon takes matrices (got a parameter of shape {tuple(p.shape)})")
-        except ValueError:
+            self._check_group(group)
+        except Exception:
             self.param_groups.pop()
             raise
+
+    @staticmethod
+    def _check_group(group):
+        _check_ns(group["ns_steps"], group["ns_coefficients"], group["eps"])
+        K.check_newton_schulz(group["ns_steps"], group["ns_coefficients"])
+
+    def _group_items(self, group):
+        """(parameter, gradient, momentum or None) of a group's matrices that have something to do, checked."""
+        self._check_group(group)
+        items = []
+        for p in group["params"]:
+            g = p.grad
+            if g is None or p.numel() == 0:
+                continue
+            _check_matrix("fusionllm_amd.optim.Muon", p)
+            if g.dtype != p.dtype or g.layout != torch.strided or g.device != p.device:
+                raise NotImplementedError(f"Muon step for a {p.dtype} parameter on {p.device} with a {g.dtype} {g.layout} "
+                                          f"grad on {g.device}")
+            if not p.is_contiguous():
+                raise NotImplementedError("Muon step needs contiguous parameters")
+            buf = self.state[p].get("momentum_buffer") if p in self.state else None
+            if buf is not None and (buf.shape != p.shape or buf.dtype != p.dtype or buf.device != p.device
+                                    or not buf.is_contiguous()):
+                raise RuntimeError("the momentum buffer must be contiguous, with its parameter's shape, dtype and device "
+                                   f"(got {tuple(buf.shape)}, {buf.dtype}, {buf.device})")
+            items.append((p, g, buf))
+        return items
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -253,22 +283,15 @@ class Muon(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            items = []
-            for p in group["params"]:
-                g = p.grad
-                if g is None or p.numel() == 0:
-                    continue
-                _check_matrix("fusionllm_amd.optim.Muon", p)
-                if g.dtype != p.dtype or g.layout != torch.strided:
-                    raise NotImplementedError(f"Muon step for a {p.dtype} parameter with a {g.dtype} {g.layout} grad")
-                if not p.is_contiguous():
-                    raise NotImplementedError("Muon step needs contiguous parameters")
+        # every group is checked before any is updated: a step that is refused has changed nothing
+        todo = [(group, float(group["lr"]), float(group["weight_decay"]), float(group["momentum"]),
+                 self._group_items(group)) for group in self.param_groups]
+        for group, lr, wd, momentum, items in todo:
+            for i, (p, g, _) in enumerate(items):
                 state = self.state[p]
-                if "momentum_buffer" not in state:
+                if state.get("momentum_buffer") is None:
                     state["momentum_buffer"] = torch.zeros_like(p)
-                items.append((p, g, state["momentum_buffer"]))
-            lr, wd = float(group["lr"]), float(group["weight_decay"])
+                items[i] = (p, g, state["momentum_buffer"])
             for chunk in _launches(items, lambda it: (it[0], it[2]), lambda it: (it[1],)):
                 small, large = _sides(chunk[0][0])
                 if group["adjust_lr_fn"] == "match_rms_adamw":
@@ -277,6 +300,6 @@ class Muon(Optimizer):
                     tall, wide = lr * math.sqrt(large / small), lr
                 with torch.cuda.device(chunk[0][0].device):
                     K.muon_step([c[0] for c in chunk], [c[1].contiguous() for c in chunk], [c[2] for c in chunk],
-                                tall, wide, 1.0 - lr * wd, group["momentum"], group["nesterov"], group["ns_steps"],
+                                tall, wide, 1.0 - lr * wd, momentum, group["nesterov"], group["ns_steps"],
                                 group["ns_coefficients"], group["eps"])
         return loss

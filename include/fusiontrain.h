@@ -74,6 +74,10 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  * workspace: 256-byte aligned, of the size query's bytes (a pair of sides in
  * either order); calls that share one must not overlap.
  * ------------------------------------------------------------------------- */
+/* FMOE_OK where the two entry points below take this number of steps and these coefficients,
+ * the status that they would return otherwise.  Host only. */
+int fmoe_newton_schulz_check(int steps, const double* coeffs);
+
 size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype);
 int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows,
                        const int64_t* cols, int n_tensors, int dtype, int steps,

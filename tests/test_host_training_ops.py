@@ -347,3 +347,67 @@ def test_a_gradient_on_anothers_memory_is_read_in_order():
     g = new()
     items = [(p, g, new()), (q, g, new())]
     assert [len(c) for c in optim._launches(items, lambda it: (it[0], it[2]), lambda it: (it[1],))] == [2]
+
+
+def test_coefficients_are_checked_on_the_host_and_by_the_constructor():
+    from fusionllm_amd.optim import Muon
+    lib = _lib.load()
+    import ctypes
+    f = lambda *co, steps=5: lib.fmoe_newton_schulz_check(steps, (ctypes.c_double * 3)(*co))
+    good = (3.4445, -4.775, 2.0315)
+    assert f(*good) == 0 and f(*good, steps=64) == 0 and f(1.5, -0.5, 0.0, steps=20) == 0
+    assert f(*good, steps=0) == 1 and f(*good, steps=65) == 1 and lib.fmoe_newton_schulz_check(5, None) == 1
+    assert f(4.0, -4.775, 2.0315) == 9 and f(float("nan"), 0.0, 0.0) == 9
+    P = lambda: torch.nn.Parameter(torch.zeros(4, 4))
+    with pytest.raises(RuntimeError, match="coefficients"):
+        Muon([P()], ns_coefficients=(8.0, -9.0, 1.5))
+    # a group's own values too, and the group is not taken
+    opt = Muon([P()])
+    for own, error in ((dict(ns_coefficients=(8.0, -9.0, 1.5)), RuntimeError), (dict(ns_steps=0), ValueError),
+                       (dict(eps=0.0), ValueError), (dict(ns_coefficients=(1.0,)), ValueError)):
+        with pytest.raises(error):
+            opt.add_param_group({"params": [P()], **own})
+        assert len(opt.param_groups) == 1
+
+
+def test_muon_checks_every_group_before_it_updates_any(monkeypatch):
+    # what a second group is refused for leaves the first one's parameters and state alone
+    from fusionllm_amd import optim
+    from fusionllm_amd.optim import Muon
+    launched = []
+    monkeypatch.setattr(optim.K, "muon_step", lambda *a: launched.append(a))
+
+    def make(shape=(4, 6), dtype=torch.float32, device="cuda"):
+        p = torch.nn.Parameter(torch.empty(shape, dtype=dtype, device=device))
+        p.grad = torch.empty(shape, dtype=dtype, device=device)
+        return p
+
+    def bad_buffer(opt, p, buf):
+        opt.state[p]["momentum_buffer"] = buf
+
+    cases = [
+        (lambda opt, p: bad_buffer(opt, p, torch.empty(6, 4, device="cuda").t()), RuntimeError, "contiguous"),
+        (lambda opt, p: bad_buffer(opt, p, torch.empty(4, 6, device="cuda", dtype=torch.bfloat16)), RuntimeError,
+         "momentum"),
+        (lambda opt, p: bad_buffer(opt, p, torch.empty(4, 6, device="cpu")), RuntimeError, "momentum"),
+        (lambda opt, p: bad_buffer(opt, p, torch.empty(4, 5, device="cuda")), RuntimeError, "momentum"),
+        (lambda opt, p: opt.param_groups[1].update(ns_coefficients=(8.0, -9.0, 1.5)), RuntimeError, "coefficients"),
+        (lambda opt, p: opt.param_groups[1].update(ns_steps=0), ValueError, "steps"),
+        (lambda opt, p: opt.param_groups[1].update(eps=-1.0), ValueError, "eps"),
+    ]
+    with FakeTensorMode():
+        for spoil, error, match in cases:
+            first, second = make(), make()
+            opt = Muon([{"params": [first]}, {"params": [second]}])
+            spoil(opt, second)
+            with pytest.raises(error, match=match):
+                opt.step()
+            assert not launched and first not in opt.state, match
+        for shape, dtype, device, error in (((4, 6), torch.float16, "cuda", NotImplementedError),
+                                            ((4, 6), torch.float32, "cpu", RuntimeError),
+                                            ((2, 65537), torch.float32, "cuda", NotImplementedError)):
+            first, second = make(), make(shape, dtype, device)
+            opt = Muon([{"params": [first]}, {"params": [second]}])
+            with pytest.raises(error):
+                opt.step()
+            assert not launched and first not in opt.state and second not in opt.state
