@@ -216,7 +216,8 @@ class Muon(Optimizer):
     state ("momentum_buffer") are those of ``torch.optim.Muon``.  Parameters are
     matrices on a ROCm device, bf16 or fp32, with gradients of their own dtype;
     every matrix of one dtype and pair of sides is updated in the same launches.
-    What a step refuses it refuses before anything is updated."""
+    What a step refuses it refuses before anything is updated.  A step can be captured into a
+    graph once every matrix has its momentum; the graph keeps the step sizes of the capture."""
 
     def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
                  nesterov: bool = True, ns_coefficients=NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
@@ -286,6 +287,10 @@ class Muon(Optimizer):
         # every group is checked before any is updated: a step that is refused has changed nothing
         todo = [(group, float(group["lr"]), float(group["weight_decay"]), float(group["momentum"]),
                  self._group_items(group)) for group in self.param_groups]
+        if any(it[2] is None for t in todo for it in t[-1]) and torch.cuda.is_current_stream_capturing():
+            # the zeros would be part of the graph and clear the momentum in every replay
+            raise RuntimeError("Muon: a step that creates momentum buffers cannot be captured into a graph; run one "
+                               "before the capture")
         for group, lr, wd, momentum, items in todo:
             for i, (p, g, _) in enumerate(items):
                 state = self.state[p]

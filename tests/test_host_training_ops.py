@@ -411,3 +411,26 @@ def test_muon_checks_every_group_before_it_updates_any(monkeypatch):
             with pytest.raises(error):
                 opt.step()
             assert not launched and first not in opt.state and second not in opt.state
+
+
+def test_muon_refuses_to_create_momentum_in_a_capture(monkeypatch):
+    # the captured zeros would clear the momentum in every replay
+    from fusionllm_amd import optim
+    from fusionllm_amd.optim import Muon
+    launched = []
+    monkeypatch.setattr(optim.K, "muon_step", lambda *a: launched.append(a))
+    with FakeTensorMode():
+        ps = [torch.nn.Parameter(torch.empty(4, 6, device="cuda")) for _ in range(2)]
+        for p in ps:
+            p.grad = torch.empty(4, 6, device="cuda")
+        opt = Muon(ps)
+        opt.state[ps[0]]["momentum_buffer"] = torch.empty(4, 6, device="cuda")
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captur"):
+            opt.step()
+        assert not launched and ps[1] not in opt.state
+        ps[1].grad = None  # every matrix of this step has its momentum
+        monkeypatch.setattr(optim, "_launches", lambda items, *a: [items])
+        monkeypatch.setattr(torch.cuda, "device", lambda d: __import__("contextlib").nullcontext())
+        opt.step()
+        assert len(launched) == 1
