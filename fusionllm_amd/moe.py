@@ -47,7 +47,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _kernels as K
-from .norm import LayerNorm, check_norm_operands
+from .norm import LayerNorm, check_norm_operands, refuse_tangents
 
 
 def _as_bf16(t: torch.Tensor) -> torch.Tensor:
@@ -674,6 +674,7 @@ class DeepSeekMoE(nn.Module):
         gate = mods["gate"]._parameters
         gw, gb = gate["weight"], gate["bias"]
         has_shared = mods.get("shared_expert") is not None  # None is a plain attribute, not in _modules
+        refuse_tangents("fusionllm_amd.DeepSeekMoE", flat, norm_w, norm_b, gw, gb, *weights)
         meta = (E, k, self.moe_inter_dim, float(self.route_scale), has_shared, out_dtype)
         needs_grad = torch.is_grad_enabled() and (
             flat.requires_grad or gw.requires_grad or gb.requires_grad

@@ -19,6 +19,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
@@ -73,6 +74,14 @@ class _LayerNormFunction(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
+def refuse_tangents(what, *tensors):
+    """A tensor with a tangent (forward-mode derivatives) need not require a gradient: without this
+    the result would come without one."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def check_norm_operands(x, weight, bias):
     what = "fusionllm_amd.layer_norm"
     if not x.is_cuda:
@@ -107,6 +116,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         # traced (torch.compile): the fusionllm::layer_norm_fwd operator
         y = torch.ops.fusionllm.layer_norm_fwd(flat, weight, bias, float(eps), out_dtype)[0]
     else:
+        refuse_tangents("fusionllm_amd.layer_norm", x, weight, bias)
         grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                             or (bias is not None and bias.requires_grad))
         host = K.block_host()

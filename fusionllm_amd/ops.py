@@ -166,6 +166,7 @@ swiglu_fwd.register_autograd(_swiglu_backward, setup_context=_swiglu_setup)
 @torch.library.custom_op("fusionllm::layer_norm_fwd", mutates_args=())
 def layer_norm_fwd(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
                    out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    _norm.refuse_tangents("fusionllm::layer_norm_fwd", x, weight, bias)
     with _norm._on_device(x):
         return _norm._forward(x, weight, bias, eps, out_dtype, True)[2:]
 

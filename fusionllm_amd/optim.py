@@ -28,6 +28,7 @@ import torch
 from torch.optim import Optimizer
 
 from . import _kernels as K
+from .norm import refuse_tangents
 
 
 class NorMuon(Optimizer):
@@ -191,6 +192,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
         _check_matrix("orthogonalize", t)
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("orthogonalize has no backward pass: call it under no_grad or on detached matrices")
+        refuse_tangents("orthogonalize", t)
     outs, items = [], []
     for t in stacks:
         t = t.detach().contiguous()

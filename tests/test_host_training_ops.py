@@ -434,3 +434,36 @@ def test_muon_refuses_to_create_momentum_in_a_capture(monkeypatch):
         monkeypatch.setattr(torch.cuda, "device", lambda d: __import__("contextlib").nullcontext())
         opt.step()
         assert len(launched) == 1
+
+
+def _duals(n, *tensors):
+    """The tensors, the n-th of them with a tangent (inside a dual level)."""
+    import torch.autograd.forward_ad as fw
+    return [fw.make_dual(t, torch.ones_like(t)) if i == n else t for i, t in enumerate(tensors)]
+
+
+def test_forward_mode_derivatives_are_refused():
+    # not lost without a word: a tensor with a tangent need not require a gradient
+    import torch.autograd.forward_ad as fw
+
+    from fusionllm_amd import DeepSeekMoE, moe_residual
+    from fusionllm_amd.optim import orthogonalize
+    with FakeTensorMode(), torch.device("cuda"):
+        x, w, b = torch.empty(4, 64), torch.empty(64), torch.empty(64)
+        moe = DeepSeekMoE(dict(dim=64, n_routed_experts=4, n_shared_experts=1, n_activated_experts=2,
+                               moe_inter_dim=64)).requires_grad_(False)
+        norm = LayerNorm(64).requires_grad_(False)
+        with fw.dual_level():
+            for i in range(3):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    layer_norm(*_duals(i, x, w, b))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.func.functional_call(norm, {"bias": _duals(0, b)[0]}, x)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                moe_residual(_duals(0, x)[0], norm, moe)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                moe(_duals(0, x)[0])
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                orthogonalize(_duals(0, x)[0])
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                orthogonalize([x, _duals(0, x)[0]])
