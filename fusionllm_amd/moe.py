@@ -44,6 +44,7 @@ import contextlib
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+import torch.nn.modules.module as nn_module
 from torch.autograd.function import once_differentiable
 
 from . import _kernels as K
@@ -776,11 +777,23 @@ class DeepSeekMoE(nn.Module):
         return (frac * prob).sum() * E
 
 
+def _as_defined(module: nn.Module, cls: type) -> bool:
+    """Whether calling the module runs cls.forward and nothing else: no forward of a subclass or of the
+    instance, no hooks."""
+    d = module.__dict__
+    return (type(module).forward is cls.forward and "forward" not in d
+            and not (d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"]
+                     or nn_module._global_forward_hooks or nn_module._global_forward_pre_hooks
+                     or nn_module._global_backward_hooks or nn_module._global_backward_pre_hooks))
+
+
 def moe_residual(x: torch.Tensor, norm: nn.Module, moe: nn.Module) -> torch.Tensor:
     """``x + moe(norm(x))``, the FFN half of FusionLLMBlock.forward
     (models/fusionllm.py:52).  A fusionllm_amd ``DeepSeekMoE`` after an
     ``nn.RMSNorm`` or a fusionllm_amd ``LayerNorm`` runs fused (norm, MoE and
-    residual add in the kernels); any other pair runs as the plain expression."""
+    residual add in the kernels); any other pair, and modules with hooks or a
+    forward of their own, run as the plain expression."""
     if isinstance(moe, DeepSeekMoE) and isinstance(norm, (nn.RMSNorm, LayerNorm)) and x.is_cuda:
-        return moe.forward_norm_residual(x, norm)
+        if _as_defined(norm, LayerNorm if isinstance(norm, LayerNorm) else nn.RMSNorm) and _as_defined(moe, DeepSeekMoE):
+            return moe.forward_norm_residual(x, norm)
     return x + moe(norm(x))

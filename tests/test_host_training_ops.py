@@ -467,3 +467,64 @@ def test_forward_mode_derivatives_are_refused():
                 orthogonalize(_duals(0, x)[0])
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 orthogonalize([x, _duals(0, x)[0]])
+
+
+def test_moe_residual_fuses_only_what_it_knows(monkeypatch):
+    """A norm or a block with a forward of its own, or with hooks, is called; the fused form would pass it by."""
+    from torch.nn.modules import module as nnm
+
+    from fusionllm_amd import DeepSeekMoE, moe_residual
+
+    fused = []
+    monkeypatch.setattr(DeepSeekMoE, "forward_norm_residual", lambda self, x, norm: fused.append(norm) or x)
+    monkeypatch.setattr(DeepSeekMoE, "forward", lambda self, x: x)
+    for cls in (LayerNorm, torch.nn.RMSNorm):
+        monkeypatch.setattr(cls, "forward", lambda self, x: x)
+    cfg = dict(dim=64, n_routed_experts=4, n_shared_experts=1, n_activated_experts=2, moe_inter_dim=64)
+
+    class Own(LayerNorm):
+        def forward(self, x):
+            return 2 * x
+
+    class OwnRMS(torch.nn.RMSNorm):
+        def forward(self, x):
+            return 2 * x
+
+    class OwnMoE(DeepSeekMoE):
+        def forward(self, x):
+            return 2 * x
+
+    class Named(LayerNorm):
+        pass
+
+    with FakeTensorMode(), torch.device("cuda"):
+        x = torch.empty(4, 64)
+
+        def takes(norm, moe):
+            del fused[:]
+            moe_residual(x, norm, moe)
+            return bool(fused)
+
+        moe = DeepSeekMoE(cfg)
+        assert takes(LayerNorm(64), moe) and takes(torch.nn.RMSNorm(64), moe) and takes(Named(64), moe)
+        assert not takes(torch.nn.LayerNorm(64), moe)
+        assert not takes(Own(64), moe) and not takes(OwnRMS(64), moe) and not takes(LayerNorm(64), OwnMoE(cfg))
+        for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                         "register_full_backward_pre_hook"):
+            for cls in (LayerNorm, torch.nn.RMSNorm):
+                norm = cls(64)
+                handle = getattr(norm, register)(lambda *a: None)
+                assert not takes(norm, moe), register
+                handle.remove()
+                assert takes(norm, moe), register
+            handle = getattr(moe, register)(lambda *a: None)
+            assert not takes(LayerNorm(64), moe), register
+            handle.remove()
+        for register in (nnm.register_module_forward_hook, nnm.register_module_forward_pre_hook):
+            handle = register(lambda *a: None)
+            assert not takes(LayerNorm(64), moe)
+            handle.remove()
+        # a forward put on the instance
+        norm = LayerNorm(64)
+        norm.forward = lambda t: 2 * t
+        assert not takes(norm, moe)
