@@ -211,8 +211,9 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsArgs a) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
     const double nrm = sqrt(ss);
-    // the norm of a matrix that holds NaN or infinities is none, and its X is NaN
-    if (threadIdx.x == 0) scale_s = static_cast<double>(kXScale) / (nrm < a.eps ? a.eps : nrm);
+    // the norm of a matrix that holds NaN or infinities is none, and its X is NaN; zeros stay zeros
+    // (1 / eps need not be finite)
+    if (threadIdx.x == 0) scale_s = ss == 0.0 ? 0.0 : static_cast<double>(kXScale) / (nrm < a.eps ? a.eps : nrm);
   }
   __syncthreads();
   const double scale = scale_s;
@@ -1089,11 +1090,14 @@ __global__ __launch_bounds__(64 * small_waves(MB), small_waves(MB) / 2) void ns_
   // the first step's X and A still lack the norm: panel p's X the factor 2^e / |u| (lane p has it)
   float mine = 1.0f;
   if (k == 0) {
-    double ss = lane < a.panels ? a.norm[mat * a.panels + lane] : 0.0;
+    const double own = lane < a.panels ? a.norm[mat * a.panels + lane] : 0.0;
+    double ss = own;
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) ss = ss + __shfl_xor(ss, off, 64);
     const double nrm = sqrt(ss);
-    mine = static_cast<float>(ldexp(1.0 / (nrm < a.eps ? a.eps : nrm), lane < a.panels ? a.exps[mat * a.panels + lane] : 0));
+    // (a panel of zeros, whose exponent is 0, stays zero: 1 / |u| may be beyond fp32)
+    mine = own == 0.0 ? 0.0f
+                      : static_cast<float>(ldexp(1.0 / (nrm < a.eps ? a.eps : nrm), a.exps[mat * a.panels + lane]));
   }
   // A: blocks w, w + NW by wave w, the panels in order
   const float* parts = a.sparts + (static_cast<int64_t>(k & 1) * a.count + mat) * a.panels * (kSmallBlocks * 256);

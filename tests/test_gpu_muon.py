@@ -629,3 +629,16 @@ def test_muon_of_overlapping_parameters_of_other_sides(gpu_device):
         return t
 
     assert torch.equal(run([(0, 1, 2)], base.clone()), run([(0,), (1,), (2,)], base.clone()))
+
+
+@pytest.mark.parametrize("eps", [1e-7, 1e-30, 1e-40, 1e-310, 5e-324])
+def test_zero_parts_under_any_eps(gpu_device, eps):
+    # zeros stay zeros whatever they are divided by: a whole matrix, and 128 columns of one whose norm is as
+    # small as eps (1 / eps is beyond fp32, or beyond fp64)
+    for rows, cols in ((96, 160), (30, 300), (300, 30)):
+        z = torch.zeros(rows, cols, device=gpu_device)
+        assert not orthogonalize(z, eps=eps).any()
+        assert not orthogonalize(z.bfloat16(), eps=eps).any()
+        z[3, 5] = 2.0 ** -140
+        z[5, 3] = -2.0 ** -140
+        check_ortho(orthogonalize(z, eps=eps), z, F32, eps=eps)
