@@ -80,6 +80,7 @@ TRAIN_SIGNATURES = {
     "fmoe_layer_norm_bwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, _P, _P, c_int, _P, c_int64, c_int64,
                                     _P, _P, _P, _P, c_size_t, _P]),
     "fmoe_newton_schulz_check": (c_int, [c_int, POINTER(c_double)]),
+    "fmoe_newton_schulz_tile": (c_int, [c_int64, c_int64, c_int, c_int]),
     "fmoe_orthogonalize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "fmoe_orthogonalize": (c_int, [_PP, _PP, POINTER(c_int64), POINTER(c_int64), c_int, c_int, c_int,
                                    POINTER(c_double), c_double, _P, c_size_t, _P]),

@@ -1280,29 +1280,34 @@ inline bool ns_bounded(double a, double b, double c, int steps) {
   return s < kMaxSigma;
 }
 
+// Output tiles of a product of `count` matrices: their number for tiles of tm x tn.
+inline int64_t ns_tiles(bool sym, int64_t mp, int64_t np, int count, int tm, int tn) {
+  const int64_t r = ceil_div(mp, tm);
+  return (sym ? r * (r + 1) / 2 : r * ceil_div(np, tn)) * count;
+}
+// Rows of the output tiles.  256 x 256 tiles, persistent, where they fill the chip and pad little (their area is at most
+// 1.5 times the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 56 us against 65, of 22
+// (132 tiles) 52 against 47; of 64 of 384 x 2048 (twice the area) 56 against 45.  Then 128 x
+// 128 tiles where there is one for most CUs: Gram product of 12 of 768 x 2048 (252 tiles) 27 us
+// against 31, of 5 of 1001 x 1503 (180 tiles) 20 against 19; 48 rows would leave
+// most of a 128-row tile empty.
+inline int ns_tile_rows(bool sym, int64_t mp, int64_t np, int count) {
+  const int64_t t256 = ns_tiles(sym, mp, np, count, 256, 256), t128 = ns_tiles(sym, mp, np, count, 128, 128);
+  if (t256 >= 160 && 8 * t256 < 3 * t128) return 256;
+  return t128 >= 192 && ns_tiles(sym, mp, np, count, 64, 128) > t128 ? 128 : 64;
+}
+
 template <int MODE, bool SPLIT, int OUT>
 inline void ns_launch(const NsArgs& a, int cur, hipStream_t s) {
   constexpr bool sym = MODE == NS_GRAM || MODE == NS_POLY;
-  auto tiles = [&](int tm, int tn) {
-    const int64_t r = ceil_div(a.mp, tm);
-    return (sym ? r * (r + 1) / 2 : r * ceil_div(a.np, tn)) * a.count;
-  };
-  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 128);
-  auto grid = [](int64_t t) { return dim3(static_cast<unsigned>(8 * ceil_div(t, 8))); };
-  // 256 x 256 tiles, persistent, where they fill the chip and pad little (their area is at most 1.5 times
-  // the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 56 us against 65, of 22
-  // (132 tiles) 52 against 47; of 64 of 384 x 2048 (twice the area) 56 against 45.  Then 128 x
-  // 128 tiles where there is one for most CUs: Gram product of 12 of 768 x 2048 (252 tiles) 27 us
-  // against 31, of 5 of 1001 x 1503 (180 tiles) 20 against 19; 48 rows would leave
-  // most of a 128-row tile empty.
-  if (t256 >= 160 && 8 * t256 < 3 * t128) {
-    ns_big_kernel<MODE, SPLIT, OUT>
-        <<<dim3(static_cast<unsigned>(std::min<int64_t>(8 * ceil_div(t256, 8), kNsCus))), dim3(core::NT), 0, s>>>(a, cur);
-  } else if (t128 >= 192 && t64 > t128) {
-    ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<grid(t128), dim3(256), 0, s>>>(a, cur);
-  } else {
-    ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<grid(t64), dim3(256), 0, s>>>(a, cur);
-  }
+  const int rows = ns_tile_rows(sym, a.mp, a.np, a.count);
+  const int64_t tiles = ns_tiles(sym, a.mp, a.np, a.count, rows, rows == 64 ? 128 : rows);
+  // workgroups: a multiple of the XCDs
+  const unsigned groups = static_cast<unsigned>(8 * ceil_div(tiles, 8));
+  if (rows == 256)
+    ns_big_kernel<MODE, SPLIT, OUT><<<dim3(std::min<unsigned>(groups, kNsCus)), dim3(core::NT), 0, s>>>(a, cur);
+  else if (rows == 128) ns_product_kernel<MODE, 128, 2, SPLIT, OUT><<<dim3(groups), dim3(256), 0, s>>>(a, cur);
+  else ns_product_kernel<MODE, 64, 3, SPLIT, OUT><<<dim3(groups), dim3(256), 0, s>>>(a, cur);
 }
 template <int MODE>
 inline void ns_product(const NsArgs& a, int cur, bool split, hipStream_t s) {
@@ -1430,6 +1435,12 @@ using namespace fmoe;
 extern "C" int fmoe_newton_schulz_check(int steps, const double* coeffs) {
   if (steps < 1 || steps > FMOE_MUON_MAX_STEPS || !coeffs) return FMOE_ERR_INVALID_ARG;
   return ns_bounded(coeffs[0], coeffs[1], coeffs[2], steps) ? FMOE_OK : FMOE_ERR_COEFFICIENTS;
+}
+
+extern "C" int fmoe_newton_schulz_tile(int64_t rows, int64_t cols, int n_tensors, int symmetric) {
+  if (fmoe_orthogonalize_workspace_bytes(rows, cols, n_tensors, FMOE_BF16) == 0) return 0;
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  return ns_is_small(m, n) ? 0 : ns_tile_rows(symmetric != 0, ns_pad(m), ns_pad(n), n_tensors);
 }
 
 extern "C" size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype) {

@@ -78,6 +78,11 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  * the status that they would return otherwise.  Host only. */
 int fmoe_newton_schulz_check(int steps, const double* coeffs);
 
+/* Rows of the output tiles (256, 128 or 64) that a launch of n_tensors matrices of these sides takes for
+ * its symmetric products (A and A^2), or for its updates of X; 0 where the form of small sides runs, or for
+ * sizes that are not taken.  Host only, for tests and profiles. */
+int fmoe_newton_schulz_tile(int64_t rows, int64_t cols, int n_tensors, int symmetric);
+
 size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype);
 int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows,
                        const int64_t* cols, int n_tensors, int dtype, int steps,

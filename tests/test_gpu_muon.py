@@ -642,3 +642,120 @@ def test_zero_parts_under_any_eps(gpu_device, eps):
         z[3, 5] = 2.0 ** -140
         z[5, 3] = -2.0 ** -140
         check_ortho(orthogonalize(z, eps=eps), z, F32, eps=eps)
+
+
+# Launches that take every tile size, none with sides that are multiples of it: sides, matrices, tile rows of
+# the symmetric products and of the updates (checked on the host: test_host_training_ops.py has the same table)
+LAUNCHES = [(700, 1030, 27, 256, 256), (700, 1030, 10, 128, 128), (400, 600, 56, 256, 256), (1400, 1500, 24, 256, 256),
+            (320, 450, 64, 128, 256), (321, 449, 20, 64, 128), (700, 1030, 3, 64, 64)]
+LAUNCH_IDS = [f"{c}x{m}x{n}" for m, n, c, _, _ in LAUNCHES]
+
+
+def mixed(m, n, count, dev, dtype, seed=0, rank=None):
+    """count matrices, wide and tall ones in turn; every one another (rows and columns rolled)."""
+    base = [gradient(m, n, dev, seed + i, rank) for i in range(3)]
+    mats = [base[i % 3].roll((7 * i, 11 * i), (0, 1)) * (1 + i % 5) for i in range(count)]
+    return [(x.t().contiguous() if i % 2 else x).to(dtype) for i, x in enumerate(mats)]
+
+
+def emulate_chain(g, steps=5, co=NS_COEFFICIENTS, eps=1e-7):
+    """The 22-bit form with its sums as they are formed: a chain of accumulations, hi lo, lo hi and hi hi of every
+    32 products, each cut to 24 bits.
+
+    ``emulate(cut=True)`` scales a product as a whole and so takes a sum's loss to be a share of what it ends
+    as.  Off the diagonal of A it is more: K products of mixed sign that end near zero stand at up to sqrt(K) of
+    their size on the way, and each of the 3 K / 32 accumulations loses up to 2^-23 of where the sum stands.
+    Cutting loses 2^-23 / sqrt(3) of the running sum in the root mean square, rounding half as much; over
+    3 K / 32 = 132 accumulations of 1408 products, sqrt(132) 2^-23 / sqrt(3) = 7.9e-7 of a running sum of
+    about half of sqrt(1408) products.  Of 1400 x 1500 the operands' roundings move the result by 1.0e-8 (root mean
+    square, of values of 2.2e-2), the chain with rounding by 3.9e-8, the chain with cuts by twice that: at sides
+    beyond some hundred the sums are what the error is made of."""
+    def parts(v, scale):
+        s = v.float().double() * 2.0 ** scale
+        h = s.half().double()
+        return h * 2.0 ** -scale, (s - h).half().double() * 2.0 ** -scale
+
+    def cut(v):
+        f = v.float()
+        return torch.where(f.double().abs() > v.abs(), torch.nextafter(f, torch.zeros_like(f)), f)
+
+    def mul(p, q):
+        acc = torch.zeros(p[0].shape[0], q[0].shape[1], dtype=torch.float32, device=p[0].device)
+        for k in range(0, p[0].shape[1], 32):
+            for x, y in ((0, 1), (1, 0), (0, 0)):
+                acc = cut(acc.double() + p[x][:, k:k + 32].contiguous() @ q[y][k:k + 32])
+        return acc.double()
+
+    tr = lambda p: tuple(t.t().contiguous() for t in p)
+    flip = g.shape[0] > g.shape[1]
+    x = g.double()
+    x = x.t().contiguous() if flip else x
+    x = x / max(float(x.norm()), eps)
+    eye = torch.eye(x.shape[0], dtype=torch.float64, device=x.device)
+    for _ in range(steps):
+        xs = parts(x, 14)
+        a = parts(mul(xs, tr(xs)), 13)
+        x = mul(parts(co[0] * eye + co[1] * (a[0] + a[1]) + co[2] * mul(a, tr(a)), 13), xs)
+    return x.t() if flip else x
+
+
+def launch_bound(g, want, dtype):
+    """ortho_bound, with the sums' chain emulated where operands are held in 22 bits: the same multiples of
+    its error (3 x, 8 standard deviations)."""
+    if dtype == BF:
+        return ortho_bound(g, want, dtype)
+    d = emulate_chain(g) - want
+    rms = lambda t, dim=None: (t * t).mean(dim, keepdim=dim is not None).sqrt()
+    size = rms(d, 1) * rms(d, 0) / rms(d) + rms(d)
+    return 3 * float(d.norm()) / float(want.norm()) + 2.0 ** -22, 24 * size + 2.0 ** -20 * want.abs()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,count,sym,update", LAUNCHES, ids=LAUNCH_IDS)
+def test_every_tile_size_at_its_edges(gpu_device, m, n, count, sym, update, dtype):
+    lib = K._lib.load()
+    assert [lib.fmoe_newton_schulz_tile(m, n, count, s) for s in (1, 0)] == [sym, update]
+    mats = mixed(m, n, count, gpu_device, dtype)
+    outs = orthogonalize(mats)
+    for x, o in zip(mats, outs):
+        want = exact(x)
+        rel, tol = launch_bound(x, want, dtype)
+        err = o.double() - want
+        assert o.dtype == dtype and float(err.norm()) <= (rel + half(dtype)) * float(want.norm()), tuple(x.shape)
+        assert (err.abs() <= tol + half(dtype) * (want.abs() + tol)).all(), tuple(x.shape)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,count,sym,update", LAUNCHES, ids=LAUNCH_IDS)
+def test_muon_in_every_tile_size(gpu_device, m, n, count, sym, update, dtype):
+    """The parameters' update in the last product's epilogue, tall and wide, bounds as above; memory
+    between the parameters stays as it was."""
+    lib = K._lib.load()
+    assert [lib.fmoe_newton_schulz_tile(n, m, count, s) for s in (1, 0)] == [sym, update]
+    lr, wd, mom = 0.03, 0.1, 0.9
+    grads = mixed(m, n, count, gpu_device, dtype, 10)
+    gap = 5
+    store = torch.randn(count * (m * n + gap), generator=torch.Generator(gpu_device).manual_seed(1),
+                        device=gpu_device).mul_(0.05).to(dtype)
+    ps, gaps = [], []
+    for i, g in enumerate(grads):
+        o = i * (m * n + gap)
+        ps.append(torch.nn.Parameter(store[o:o + m * n].view(g.shape)))
+        gaps.append((store[o + m * n:o + m * n + gap], store[o + m * n:o + m * n + gap].clone()))
+        ps[-1].grad = g
+    opt = Muon(ps, lr=lr, weight_decay=wd, momentum=mom)
+    bufs = [b.mul_(0.5) for b in mixed(m, n, count, gpu_device, dtype, 20)]
+    before = [(p.detach().clone(), b.clone()) for p, b in zip(ps, bufs)]
+    for p, b in zip(ps, bufs):
+        opt.state[p]["momentum_buffer"] = b
+    opt.step()
+    for p, g, b, (p0, b0) in zip(ps, grads, bufs, before):
+        want, buf, lr_, o, u = expect_step(p0, g, b0, lr, wd, mom, True, None)
+        size = mom * b0.double().abs() + (1 - mom) * g.double().abs()
+        assert ((b.double() - buf).abs() <= 4 * 2.0 ** -24 * size + half(dtype) * buf.abs() * (1 + 2.0 ** -20)).all()
+        rms = float(o.norm()) / math.sqrt(o.numel())
+        tol = lr_ * (launch_bound(u, o, dtype)[1] + 8 * 2.0 ** -20 * rms)
+        tol = tol + 4 * 2.0 ** -24 * (p0.double().abs() + lr_ * o.abs())
+        err = (p.detach().double() - want).abs()
+        assert (err <= tol + half(dtype) * (want.abs() + tol)).all(), tuple(p.shape)
+    assert all(torch.equal(x, y) for x, y in gaps)

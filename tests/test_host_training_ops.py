@@ -528,3 +528,14 @@ def test_moe_residual_fuses_only_what_it_knows(monkeypatch):
         norm = LayerNorm(64)
         norm.forward = lambda t: 2 * t
         assert not takes(norm, moe)
+
+
+def test_tiles_of_a_launch():
+    # the shapes by which the GPU tests reach every tile size; both sides of the rule
+    tile = _lib.load().fmoe_newton_schulz_tile
+    for m, n, count, sym, update in [(700, 1030, 27, 256, 256), (700, 1030, 10, 128, 128), (400, 600, 56, 256, 256),
+                                     (1400, 1500, 24, 256, 256), (320, 450, 64, 128, 256), (321, 449, 20, 64, 128),
+                                     (700, 1030, 3, 64, 64)]:
+        assert (tile(m, n, count, 1), tile(m, n, count, 0)) == (sym, update) == (tile(n, m, count, 1), tile(n, m, count, 0))
+    assert tile(64, 4096, 64, 1) == 0 and tile(64, 4097, 1, 1) == 64  # the form of small sides
+    assert tile(0, 5, 1, 0) == tile(5, 5, 65, 0) == tile(65537, 5, 1, 0) == tile(16385, 32768, 1, 0) == 0
