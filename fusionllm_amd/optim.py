@@ -182,7 +182,8 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
     mats: a tensor [..., rows, cols] (every matrix of the stack), or a list of such tensors; the result
     has the same structure, shapes and dtypes.  No backward pass.  The coefficients must keep the
     singular values below 2.8 (the defaults do).  The result of a matrix whose norm is far below eps is
-    nearly zero, and precise to 2^-36 of the size that it would have with a norm of eps or more."""
+    nearly zero; beside its relative error, an element of any result is off by up to about
+    steps |a|^steps 2^-38 (2^-27 with the defaults)."""
     single = isinstance(mats, torch.Tensor)
     stacks = [mats] if single else list(mats)
     _check_ns(steps, coefficients, eps)

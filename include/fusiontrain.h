@@ -67,14 +67,22 @@ int fmoe_layer_norm_bwd(const void* dy, int dy_dtype, int64_t lddy, const void* 
  * fp16 and an fp8 remainder, the result is rounded once, to dtype; for fp32 matrices (and small
  * sides up to 128) every operand is held in 22 bits, and small sides up to 64 with at most
  * 4096 columns run in fp32.  A matrix that holds NaN or
- * infinities gives NaN; a zero matrix gives zeros; the nearly zero result of one
- * whose norm is far below eps is precise to 2^-36 of the usual size.  Coefficients whose iterates
+ * infinities gives NaN; a zero matrix gives zeros.  X is stored in steps of 2^-38 at the finest, and a step
+ * multiplies what that loses by up to |coeffs[0]|: beside the relative error an element is off by up to
+ * about steps |coeffs[0]|^steps 2^-38 (2^-27 for five steps with 3.4445), all the precision that the
+ * nearly zero result of a matrix of a norm far below eps has.  Coefficients whose iterates
  * leave the stored range (singular values up to 2.8, |a + b t + c t^2| up to 7.9)
  * return FMOE_ERR_COEFFICIENTS.  Deterministic.
  * workspace: 256-byte aligned, of the size query's bytes (a pair of sides in
  * either order); calls that share one must not overlap.
  * ------------------------------------------------------------------------- */
-/* FMOE_OK where the two entry points below take this number of steps and these coefficients,
+size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype);
+int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows,
+                       const int64_t* cols, int n_tensors, int dtype, int steps,
+                       const double* coeffs, double eps, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* FMOE_OK where fmoe_orthogonalize and fmoe_muon_step take this number of steps and these coefficients,
  * the status that they would return otherwise.  Host only. */
 int fmoe_newton_schulz_check(int steps, const double* coeffs);
 
@@ -82,12 +90,6 @@ int fmoe_newton_schulz_check(int steps, const double* coeffs);
  * its symmetric products (A and A^2), or for its updates of X; 0 where the form of small sides runs, or for
  * sizes that are not taken.  Host only, for tests and profiles. */
 int fmoe_newton_schulz_tile(int64_t rows, int64_t cols, int n_tensors, int symmetric);
-
-size_t fmoe_orthogonalize_workspace_bytes(int64_t rows, int64_t cols, int n_tensors, int dtype);
-int fmoe_orthogonalize(const void* const* src, void* const* dst, const int64_t* rows,
-                       const int64_t* cols, int n_tensors, int dtype, int steps,
-                       const double* coeffs, double eps, void* workspace,
-                       size_t workspace_bytes, void* stream);
 
 /* One Muon step of up to FMOE_MUON_MAX_TENSORS matrices (sizes and workspace as
  * fmoe_orthogonalize), in place:
