@@ -555,3 +555,100 @@ def test_moe_residual_of_fp32_outside_autocast(gpu_device):
     for got, want in ((y, y2), (x.grad, x2.grad), (norm.weight.grad, norm2.weight.grad),
                       (norm.bias.grad, norm2.bias.grad)):
         assert float((got.double() - want.double()).norm()) <= tol * float(want.double().norm())
+
+
+@pytest.mark.parametrize("kw", [dict(bias=False), dict(elementwise_affine=False)], ids=["no_bias", "no_vectors"])
+@pytest.mark.parametrize("mode", ["bf16", "autocast"])
+def test_moe_residual_with_fewer_vectors(gpu_device, kw, mode):
+    # bounds as in test_moe_residual_with_layer_norm
+    cfg = configs.BlockConfig("t", 61, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=5)
+    dt = BF if mode == "bf16" else F32
+    moe = build_module(cfg, data, gpu_device, dt)
+    norm = LayerNorm(128, **kw).to(gpu_device, dt)
+    with torch.no_grad():
+        for p in norm.parameters():
+            p.add_(0.2 * torch.randn_like(p))
+    moe2, norm2 = copy.deepcopy(moe), copy.deepcopy(norm)
+    x = data.x.to(gpu_device, dt).requires_grad_(True)
+    x2 = x.detach().clone().requires_grad_(True)
+    dy = data.dy.to(gpu_device, dt)
+    with torch.autocast("cuda", dtype=BF, enabled=mode == "autocast"):
+        y, y2 = moe_residual(x, norm, moe), x2 + moe2(norm2(x2))
+        with torch.no_grad():
+            assert torch.equal(moe_residual(x, norm, moe), y)
+    y.backward(dy)
+    y2.backward(dy)
+    assert y.dtype == dt and torch.equal(moe._last_indices, moe2._last_indices)
+    pairs = [(y, y2), (x.grad, x2.grad), *((p.grad, q.grad) for p, q in zip(norm.parameters(), norm2.parameters()))]
+    assert len(pairs) == 2 + len(list(norm.parameters()))
+    for got, want in pairs:
+        assert float((got.detach().double() - want.detach().double()).norm()) <= 2.0 ** -7 * float(want.detach().double().norm())
+    for p, q in zip(moe.parameters(), moe2.parameters()):
+        assert (p.grad is None and q.grad is None) or torch.equal(p.grad, q.grad)
+
+
+def test_moe_residual_partial_gradients(gpu_device):
+    # only what is asked for is computed, with the same bits: input, weight, bias, each alone and none of them
+    cfg = configs.BlockConfig("t", 37, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=6)
+    moe = build_module(cfg, data, gpu_device, BF)
+    norm = LayerNorm(128).to(gpu_device, BF)
+    dy = data.dy.to(gpu_device, BF)
+    x = data.x.to(gpu_device, BF)
+
+    def run(pick, block):
+        norm.weight.requires_grad_(1 in pick)
+        norm.bias.requires_grad_(2 in pick)
+        moe.requires_grad_(block)
+        xs = x.clone().requires_grad_(0 in pick)
+        leaves = [t for i, t in enumerate((xs, norm.weight, norm.bias)) if i in pick]
+        leaves += [moe.experts[0].w1.weight] if block else []
+        y = moe_residual(xs, norm, moe)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy)) if leaves else (y.detach(),)
+
+    y, dx, dw, db, d1 = run((0, 1, 2), True)
+    full = (dx, dw, db)
+    for pick in ((), (0,), (1,), (2,), (0, 1), (1, 2), (0, 2)):
+        for block in (True, False):
+            got = run(pick, block)
+            want = (y, *(full[i] for i in pick), *((d1,) if block else ()))
+            assert len(got) == len(want) and all(torch.equal(p, q) for p, q in zip(got, want)), (pick, block)
+
+
+def test_forward_mode_derivatives_are_refused(gpu_device):
+    # eager, traced, through torch.func, and where a parameter requires a gradient; vmap has no rule either
+    import torch.autograd.forward_ad as fw
+    x, w, b, _ = inputs(6, 64, F32, F32, gpu_device)
+    t = torch.ones_like(x)
+    with fw.dual_level():
+        d = fw.make_dual(x, t)
+        for call in (lambda: layer_norm(d, w, b), lambda: layer_norm(d, w.clone().requires_grad_(True), b),
+                     lambda: torch.ops.fusionllm.layer_norm_fwd(d, w, b, 1e-5, F32)):
+            with pytest.raises(NotImplementedError):
+                call()
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            layer_norm(d, w, b)
+        layer_norm(x, w, b)  # no tangent: as ever
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda v: layer_norm(v, w, b), (x,), (t,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: layer_norm(v, w, b))(x)
+
+
+def test_moe_residual_calls_hooks(gpu_device):
+    cfg = configs.BlockConfig("t", 20, dim=128, inter=192, n_experts=4, topk=2)
+    data = configs.make_block(cfg, seed=7)
+    moe = build_module(cfg, data, gpu_device, BF)
+    x = data.x.to(gpu_device, BF)
+    for norm in (LayerNorm(128).to(gpu_device, BF), nn.RMSNorm(128).to(gpu_device, BF)):
+        seen = []
+        handle = norm.register_forward_hook(lambda m, a, out: seen.append(out) or 2 * out)
+        with torch.no_grad():
+            y = moe_residual(x, norm, moe)
+            assert len(seen) == 1
+            handle.remove()
+            assert torch.equal(y, x + moe(2 * norm(x)))
+            # bounds as above: the block's output is rounded before the add, or after it
+            want = (x + moe(norm(x))).double()
+            assert float((moe_residual(x, norm, moe).double() - want).norm()) <= 2.0 ** -7 * float(want.norm())
