@@ -539,3 +539,36 @@ def test_tiles_of_a_launch():
         assert (tile(m, n, count, 1), tile(m, n, count, 0)) == (sym, update) == (tile(n, m, count, 1), tile(n, m, count, 0))
     assert tile(64, 4096, 64, 1) == 0 and tile(64, 4097, 1, 1) == 64  # the form of small sides
     assert tile(0, 5, 1, 0) == tile(5, 5, 65, 0) == tile(65537, 5, 1, 0) == tile(16385, 32768, 1, 0) == 0
+
+
+def test_training_kernels_without_scratch_memory(tmp_path):
+    # none but the backward of bf16 rows of two chunks per lane, which keeps one register of its 128 there
+    import shutil
+    import subprocess
+
+    from fusionllm_amd import build
+    from tests import isa_check as ic
+    if not ic.ROCM_LLVM.exists():
+        pytest.skip("no LLVM tools here")
+    scratch = {}
+    for name in ("newton_schulz", "layer_norm"):
+        obj = build.BUILD_DIR / f"{name}.o"
+        if not obj.exists():
+            pytest.skip("no built objects")
+        work = tmp_path / name
+        work.mkdir()
+        shutil.copy(obj, work / obj.name)
+        subprocess.run([str(ic.ROCM_LLVM / "llvm-objdump"), "--offloading", obj.name], check=True,
+                       capture_output=True, cwd=work)
+        dev = next(p for p in work.iterdir() if "gfx950" in p.name)
+        notes = subprocess.run([str(ic.ROCM_LLVM / "llvm-readelf"), "--notes", str(dev)], check=True,
+                               capture_output=True, text=True).stdout
+        for entry in notes.split("  - .agpr_count:")[1:]:
+            kernel = re.search(r"\.name:\s+_ZN4fmoe\d+(\w+)", entry).group(1)
+            value = lambda key: int(re.search(rf"\.{key}:\s*(\d+)", entry).group(1))
+            if value("private_segment_fixed_size") or value("vgpr_spill_count"):
+                scratch[kernel] = (value("private_segment_fixed_size"), value("vgpr_spill_count"))
+    # x bf16, dy bf16 or fp32, chunks of 8, two per lane
+    assert {k.split("EEEv")[0] for k in scratch} <= {"layer_norm_bwd_kernelILi0ELi0ELi8ELi2",
+                                                     "layer_norm_bwd_kernelILi0ELi1ELi8ELi2"}
+    assert all(size <= 8 and spilled <= 1 for size, spilled in scratch.values())
