@@ -115,8 +115,9 @@ class _Spans:
 
 def _span(t):
     """Addresses from a tensor's first element to the end of its last."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    n = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    lo = t.data_ptr()
+    return lo, lo + n * t.element_size()
 
 
 class _Launch:
@@ -127,29 +128,48 @@ class _Launch:
         return (any(self.written.meets(*s) or self.read.meets(*s) for s in written)
                 or any(self.written.meets(*s) for s in read))
 
+    def add(self, written, read):
+        for s in written:
+            self.written.add(*s)
+        for s in read:
+            self.read.add(*s)
 
-def _launches(items, written, read=lambda it: ()):
+
+def _apart(written, read):
+    """Whether no written span meets another one (read spans may meet each other)."""
+    spans = sorted([(lo, hi, True) for w in written for lo, hi in w] + [(lo, hi, False) for r in read for lo, hi in r])
+    end = end_written = 0
+    for lo, hi, w in spans:
+        if lo < (end if w else end_written):
+            return False
+        if hi > end:
+            end = hi
+        if w and hi > end_written:
+            end_written = hi
+    return True
+
+
+def _launches(items, written=lambda it: (), read=lambda it: ()):
     """Lists of items (tuples whose first tensor is the matrix) for one launch each: one device, dtype and
     pair of sides, at most MUON_MAX_TENSORS and LAUNCH_ELEMENTS, and no two of which one writes
     memory that the other writes or reads (written(item), read(item): tensors).  Two such items, of whatever
     sides, are in launches of their order: an item joins its sides' last launch only if it conflicts
     neither with that nor with any launch behind it."""
+    w, r = [[_span(x) for x in written(it)] for it in items], [[_span(x) for x in read(it)] for it in items]
+    apart = _apart(w, r)  # as ever, but for tied and overlapping parameters
     last: dict = {}  # place of the last launch of each device, dtype and sides
     out: list = []
-    for it in items:
+    for i, it in enumerate(items):
         t = it[0]
         key = (t.device, t.dtype, _sides(t))
-        most = min(K.MUON_MAX_TENSORS, max(1, LAUNCH_ELEMENTS // t.numel()))
-        w, r = [_span(x) for x in written(it)], [_span(x) for x in read(it)]
         at = last.get(key)
-        if at is None or len(out[at].items) >= most or any(c.conflicts(w, r) for c in out[at:]):
+        if (at is None or len(out[at].items) >= min(K.MUON_MAX_TENSORS, max(1, LAUNCH_ELEMENTS // t.numel()))
+                or (not apart and any(c.conflicts(w[i], r[i]) for c in out[at:]))):
             at = last[key] = len(out)
             out.append(_Launch())
         out[at].items.append(it)
-        for s in w:
-            out[at].written.add(*s)
-        for s in r:
-            out[at].read.add(*s)
+        if not apart:
+            out[at].add(w[i], r[i])
     return [c.items for c in out]
 
 
@@ -201,7 +221,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
         outs.append(out)
         if t.numel():
             items += zip(t.view(-1, *t.shape[-2:]), out.view(-1, *t.shape[-2:]))
-    for chunk in _launches(items, lambda it: it[1:]):
+    for chunk in _launches(items):  # (the results' memory is new)
         with torch.cuda.device(chunk[0][0].device):
             K.orthogonalize([c[0] for c in chunk], [c[1] for c in chunk], steps, coefficients, eps)
     return outs[0] if single else outs
@@ -273,7 +293,8 @@ class Muon(Optimizer):
                                           f"grad on {g.device}")
             if not p.is_contiguous():
                 raise NotImplementedError("Muon step needs contiguous parameters")
-            buf = self.state[p].get("momentum_buffer") if p in self.state else None
+            state = self.state.get(p)
+            buf = state.get("momentum_buffer") if state else None
             if buf is not None and (buf.shape != p.shape or buf.dtype != p.dtype or buf.device != p.device
                                     or not buf.is_contiguous()):
                 raise RuntimeError("the momentum buffer must be contiguous, with its parameter's shape, dtype and device "
@@ -295,11 +316,12 @@ class Muon(Optimizer):
             raise RuntimeError("Muon: a step that creates momentum buffers cannot be captured into a graph; run one "
                                "before the capture")
         for group, lr, wd, momentum, items in todo:
-            for i, (p, g, _) in enumerate(items):
-                state = self.state[p]
-                if state.get("momentum_buffer") is None:
-                    state["momentum_buffer"] = torch.zeros_like(p)
-                items[i] = (p, g, state["momentum_buffer"])
+            for i, (p, g, buf) in enumerate(items):
+                if buf is None:
+                    state = self.state[p]
+                    if state.get("momentum_buffer") is None:
+                        state["momentum_buffer"] = torch.zeros_like(p)
+                    items[i] = (p, g, state["momentum_buffer"])
             for chunk in _launches(items, lambda it: (it[0], it[2]), lambda it: (it[1],)):
                 small, large = _sides(chunk[0][0])
                 if group["adjust_lr_fn"] == "match_rms_adamw":
