@@ -1286,8 +1286,11 @@ inline int64_t ns_tiles(bool sym, int64_t mp, int64_t np, int count, int tm, int
   return (sym ? r * (r + 1) / 2 : r * ceil_div(np, tn)) * count;
 }
 // Rows of the output tiles.  256 x 256 tiles, persistent, where they fill the chip and pad little (their area is at most
-// 1.5 times the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 56 us against 65, of 22
-// (132 tiles) 52 against 47; of 64 of 384 x 2048 (twice the area) 56 against 45.  Then 128 x
+// 1.5 times the 128 x 128 tiles'): Gram product of 27 matrices of 768 x 2048 (162 tiles) 58 us against 63, of 22
+// (132 tiles) 52 against 40, of 24 (144) 54 against 41, of 25 (150) 55 against 59, of 26 (156) 56 against 58; of 18 of
+// 1001 x 1503 (180) 46 against 50, of 15 (150) 43 against 44, of 14 (140) 41 against 32; of 64 of 384 x 2048 (twice the
+// area) 56 against 45.  (128 x 128 tiles win while two per CU hold all of them, up to 512 of them; from there to
+// 160 of these the two are within 7 %.)  Then 128 x
 // 128 tiles where there is one for most CUs: Gram product of 12 of 768 x 2048 (252 tiles) 27 us
 // against 31, of 5 of 1001 x 1503 (180 tiles) 20 against 19; 48 rows would leave
 // most of a 128-row tile empty.
