@@ -685,6 +685,119 @@ def muon_step(params, grads, bufs, lr_tall: float, lr_wide: float, decay: float,
           "fmoe_muon_step")
 
 
+VOCAB_MAX_DIM = 16384
+VOCAB_MAX_TOP = 1024
+
+
+def _index(t, name):
+    """Address of an index tensor and whether it is int64."""
+    if t.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name} must be int32 or int64 (got {t.dtype})")
+    return _req(t, name), int(t.dtype == torch.int64)
+
+
+@_timed
+def embedding_fwd(ids, weight, scale: float):
+    """Rows ids [T] of weight [V, D] (rows may lie apart), times scale."""
+    lib = _lib.load()
+    ip, i64 = _index(ids, "ids")
+    wp, ldw = _row_stride(weight, "weight")
+    V, d = weight.shape
+    y = torch.empty(ids.numel(), d, dtype=weight.dtype, device=weight.device)
+    check(lib.fmoe_embedding_fwd(ip, i64, wp, _dtype_code(weight.dtype), ldw, ids.numel(), V, d, scale, y.data_ptr(),
+                                 _stream()), "fmoe_embedding_fwd")
+    return y
+
+
+@_timed
+def embedding_bwd(ids, dy, vocab: int, scale: float, padding_idx: int, dtype: torch.dtype):
+    """Gradient [vocab, D] of the embedding's weight; padding_idx -1: none."""
+    lib = _lib.load()
+    ip, i64 = _index(ids, "ids")
+    dyp, lddy = _row_stride(dy, "dy")
+    T, d = dy.shape
+    if ids.numel() != T:
+        raise RuntimeError(f"ids must hold {T} values (got {tuple(ids.shape)})")
+    dw = torch.empty(vocab, d, dtype=dtype, device=dy.device)
+    nbytes = lib.fmoe_embedding_bwd_workspace_bytes(T, vocab, d)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dy.device)
+    check(lib.fmoe_embedding_bwd(ip, i64, dyp, _dtype_code(dy.dtype), lddy, T, vocab, d, scale, padding_idx,
+                                 dw.data_ptr(), _dtype_code(dtype), ws.data_ptr(), nbytes, _stream()),
+          "fmoe_embedding_bwd")
+    return dw
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def vocab_loss_state_bytes(rows: int, dim: int, top: int, planes: int) -> int:
+    """Bytes of the state that vocab_loss_fwd returns (arithmetic alone, also on symbolic sizes).  In
+    csrc/vocab_loss.hip, VlState: blocks of multiples of 256 bytes."""
+    block = lambda n: (n + 255) // 256 * 256
+    padded = (rows + 63) // 64 * 64
+    padded = torch.sym_max(padded, 64)
+    return (256 + 3 * block(rows * 4) + 3 * block(rows * top * 4) + block(rows * 8) +
+            block(planes * padded * ((dim + 63) // 64 * 64) * 2))
+
+
+@_timed
+def vocab_loss_fwd(hidden, weight, index, teacher, ignore_index: int, logit_scale: float, temperature: float,
+                   planes: int, reduction: str):
+    """Loss over a vocabulary of hidden [T, D] against weight [V, D]; index [T, K] and teacher [T, K] or
+    None (cross entropy, K = 1).  Returns the fp32 loss ([T], or one value) and the state for the backward."""
+    lib = _lib.load()
+    hp, ldh = _row_stride(hidden, "hidden")
+    wp, ldw = _row_stride(weight, "weight")
+    ip, i64 = _index(index, "index")
+    (T, d), V = hidden.shape, weight.shape[0]
+    if weight.shape[1] != d:
+        raise RuntimeError(f"weight must have {d} columns (got {tuple(weight.shape)})")
+    if index.dim() != 2 or index.shape[0] != T or (teacher is not None and teacher.shape != index.shape):
+        raise RuntimeError(f"index and teacher must be [{T}, top]")
+    top = index.shape[1]
+    dev = hidden.device
+    w_code = _dtype_code(weight.dtype)
+    packs = lib.fmoe_vocab_loss_packs(wp, w_code, ldw, d, planes)
+    n_state = lib.fmoe_vocab_loss_state_bytes(T, d, top, planes)
+    n_ws = lib.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, planes, packs)
+    state = torch.empty(n_state, dtype=torch.uint8, device=dev)
+    ws = torch.empty(max(n_ws, 256), dtype=torch.uint8, device=dev)
+    loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    # (an empty tensor has no address; the entry point wants one for its output)
+    lp = loss.data_ptr() or state.data_ptr()
+    tp = None if teacher is None else _req(teacher, "teacher")
+    check(lib.fmoe_vocab_loss_fwd(hp, _dtype_code(hidden.dtype), ldh, wp, w_code, ldw, ip, i64, tp,
+                                  F32 if teacher is None else _dtype_code(teacher.dtype), T, d, V, top, ignore_index,
+                                  logit_scale, temperature, planes, REDUCTIONS[reduction], lp, state.data_ptr(),
+                                  n_state, ws.data_ptr(), n_ws, _stream()), "fmoe_vocab_loss_fwd")
+    return loss, state
+
+
+@_timed
+def vocab_loss_bwd(d_loss, weight, state, rows: int, top: int, distill: bool, logit_scale: float, temperature: float,
+                   planes: int, reduction: str, dh_dtype: torch.dtype | None, dw_dtype: torch.dtype | None):
+    """Backward of vocab_loss_fwd; returns d_hidden and d_weight, each None where its dtype is None."""
+    lib = _lib.load()
+    wp, ldw = _row_stride(weight, "weight")
+    V, d = weight.shape
+    if d_loss.numel() != (rows if reduction == "none" else 1):
+        raise RuntimeError(f"d_loss must hold {rows if reduction == 'none' else 1} values (got {tuple(d_loss.shape)})")
+    dev = weight.device
+    w_code = _dtype_code(weight.dtype)
+    n_ws = lib.fmoe_vocab_loss_bwd_workspace_bytes(rows, d, V, planes,
+                                                   lib.fmoe_vocab_loss_packs(wp, w_code, ldw, d, planes))
+    ws = torch.empty(max(n_ws, 256), dtype=torch.uint8, device=dev)
+    dh = None if dh_dtype is None else torch.empty(rows, d, dtype=dh_dtype, device=dev)
+    dw = None if dw_dtype is None else torch.empty(V, d, dtype=dw_dtype, device=dev)
+    check(lib.fmoe_vocab_loss_bwd(_req(d_loss, "d_loss", torch.float32) or state.data_ptr(), wp, w_code, ldw, rows, d,
+                                  V, top, int(distill), logit_scale, temperature, planes, REDUCTIONS[reduction],
+                                  _req(state, "state", torch.uint8), state.numel(), _ptr(dh),
+                                  _dtype_code(dh_dtype or torch.float32), _ptr(dw),
+                                  _dtype_code(dw_dtype or torch.float32), ws.data_ptr(), n_ws, _stream()),
+          "fmoe_vocab_loss_bwd")
+    return dh, dw
+
+
 CAST_MAX_TENSORS = 64
 
 

@@ -1,5 +1,5 @@
-"""ctypes binding of libfusionmoe.so (declarations in include/fusionmoe.h and
-include/fusiontrain.h).
+"""ctypes binding of libfusionmoe.so (declarations in include/fusionmoe.h,
+include/fusiontrain.h and include/fusionvocab.h).
 
 The library is built in-tree by ``fusionllm_amd.build`` (or
 ``__graft_entry__.build()``).  There is no fallback: if the library is
@@ -14,7 +14,7 @@ from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfusionmoe.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 MAX_EXPERTS = 64
 MAX_TOPK = 8
 
@@ -88,6 +88,23 @@ TRAIN_SIGNATURES = {
                                c_double, c_double, c_int, c_int, POINTER(c_double), c_double, _P, c_size_t, _P]),
 }
 
+# the vocabulary operators at a model's two ends; mirrors include/fusionvocab.h
+VOCAB_SIGNATURES = {
+    "fmoe_embedding_fwd": (c_int, [_P, c_int, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_float, _P, _P]),
+    "fmoe_embedding_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "fmoe_embedding_bwd": (c_int, [_P, c_int, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_float, c_int64, _P,
+                                   c_int, _P, c_size_t, _P]),
+    "fmoe_vocab_loss_state_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "fmoe_vocab_loss_packs": (c_int, [_P, c_int, c_int64, c_int64, c_int]),
+    "fmoe_vocab_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "fmoe_vocab_loss_fwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int, c_int64, c_int64,
+                                    c_int64, c_int64, c_int64, c_double, c_double, c_int, c_int, _P, _P, c_size_t,
+                                    _P, c_size_t, _P]),
+    "fmoe_vocab_loss_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "fmoe_vocab_loss_bwd": (c_int, [_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_double,
+                                    c_double, c_int, c_int, _P, c_size_t, _P, c_int, _P, c_int, _P, c_size_t, _P]),
+}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -112,7 +129,7 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
                 f"{p} is missing: build the HIP extension first "
                 "(python -m fusionllm_amd.build or __graft_entry__.build())")
         lib = ctypes.CDLL(str(p))
-        for name, (res, args) in (SIGNATURES | TRAIN_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | TRAIN_SIGNATURES | VOCAB_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

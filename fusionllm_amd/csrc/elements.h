@@ -79,4 +79,28 @@ __device__ __forceinline__ void store_chunk(void* base, int64_t e, const float* 
   }
 }
 
+// The same for n (up to 8) elements at the end of a row; what is past them reads as zero and is not written.
+template <int DT>
+__device__ __forceinline__ void load_upto8(const void* base, int64_t e, int n, float* v) {
+  if (n >= 8) {
+    unpack<DT, 8>(load_raw<DT, 8>(base, e), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = 0.0f;
+      if (i < n) unpack<DT, 1>(load_raw<DT, 1>(base, e + i), v + i);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_upto8(void* base, int64_t e, int n, const float* v) {
+  if (n >= 8) {
+    store_chunk<DT, 8>(base, e, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) store_chunk<DT, 1>(base, e + i, v + i);
+  }
+}
+
 }  // namespace fmoe

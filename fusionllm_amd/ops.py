@@ -208,3 +208,88 @@ def _layer_norm_backward(ctx, dy, *unused):
 
 
 layer_norm_fwd.register_autograd(_layer_norm_backward, setup_context=_layer_norm_setup)
+
+
+@torch.library.custom_op("fusionllm::embedding_fwd", mutates_args=())
+def embedding_fwd(ids: Tensor, weight: Tensor, scale: float, padding_idx: int) -> Tensor:
+    _norm.refuse_tangents("fusionllm::embedding_fwd", weight)
+    with _norm._on_device(weight):
+        return K.embedding_fwd(ids, _norm._rows(weight), scale)
+
+
+@embedding_fwd.register_fake
+def _(ids, weight, scale, padding_idx):
+    return weight.new_empty((ids.shape[0], weight.shape[1]))
+
+
+@torch.library.custom_op("fusionllm::embedding_bwd", mutates_args=())
+def embedding_bwd(ids: Tensor, dy: Tensor, vocab: int, scale: float, padding_idx: int) -> Tensor:
+    with _norm._on_device(dy):
+        return K.embedding_bwd(ids, _norm._rows(dy), vocab, scale, padding_idx, dy.dtype)
+
+
+@embedding_bwd.register_fake
+def _(ids, dy, vocab, scale, padding_idx):
+    return dy.new_empty((vocab, dy.shape[1]))
+
+
+def _embedding_setup(ctx, inputs, output):
+    ids, weight, scale, padding_idx = inputs
+    ctx.save_for_backward(ids)
+    ctx.args = (weight.shape[0], scale, padding_idx)
+
+
+def _embedding_backward(ctx, dy):
+    ids, = ctx.saved_tensors
+    if dy is None:
+        return None, None, None, None
+    return None, torch.ops.fusionllm.embedding_bwd(ids, dy, *ctx.args), None, None
+
+
+embedding_fwd.register_autograd(_embedding_backward, setup_context=_embedding_setup)
+
+
+@torch.library.custom_op("fusionllm::vocab_loss_fwd", mutates_args=())
+def vocab_loss_fwd(hidden: Tensor, weight: Tensor, index: Tensor, teacher: Tensor | None, ignore_index: int,
+                   logit_scale: float, temperature: float, planes: int, reduction: str) -> tuple[Tensor, Tensor]:
+    _norm.refuse_tangents("fusionllm::vocab_loss_fwd", hidden, weight)
+    with _norm._on_device(weight):
+        return K.vocab_loss_fwd(_norm._rows(hidden), _norm._rows(weight), index, teacher, ignore_index, logit_scale,
+                                temperature, planes, reduction)
+
+
+@vocab_loss_fwd.register_fake
+def _(hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction):
+    T, top = index.shape
+    return (hidden.new_empty((T,) if reduction == "none" else (), dtype=torch.float32),
+            hidden.new_empty((K.vocab_loss_state_bytes(T, hidden.shape[1], top, planes),), dtype=torch.uint8))
+
+
+@torch.library.custom_op("fusionllm::vocab_loss_bwd", mutates_args=())
+def vocab_loss_bwd(d_loss: Tensor, hidden: Tensor, weight: Tensor, state: Tensor, top: int, distill: bool,
+                   logit_scale: float, temperature: float, planes: int, reduction: str) -> list[Tensor]:
+    with _norm._on_device(weight):
+        return list(K.vocab_loss_bwd(d_loss.contiguous(), _norm._rows(weight), state, hidden.shape[0], top, distill,
+                                     logit_scale, temperature, planes, reduction, hidden.dtype, weight.dtype))
+
+
+@vocab_loss_bwd.register_fake
+def _(d_loss, hidden, weight, state, top, distill, logit_scale, temperature, planes, reduction):
+    return [hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)]
+
+
+def _vocab_loss_setup(ctx, inputs, output):
+    hidden, weight, index, teacher, _, logit_scale, temperature, planes, reduction = inputs
+    ctx.save_for_backward(hidden, weight, output[1])
+    ctx.args = (index.shape[1], teacher is not None, logit_scale, temperature, planes, reduction)
+
+
+def _vocab_loss_backward(ctx, d_loss, *unused):
+    hidden, weight, state = ctx.saved_tensors
+    if d_loss is None:
+        return (None,) * 9
+    dh, dw = torch.ops.fusionllm.vocab_loss_bwd(d_loss, hidden, weight, state, *ctx.args)
+    return dh, dw, None, None, None, None, None, None, None
+
+
+vocab_loss_fwd.register_autograd(_vocab_loss_backward, setup_context=_vocab_loss_setup)

@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define FMOE_ABI_VERSION 15
+#define FMOE_ABI_VERSION 16
 #define FMOE_MAX_EXPERTS 64
 #define FMOE_MAX_TOPK 8
 #define FMOE_MAX_CAST 64

@@ -1,0 +1,97 @@
+/*
+ * fusionvocab.h — C ABI of libfusionmoe.so, continued: the vocabulary operators
+ * at the two ends of a model, the token embedding in front of the blocks and the
+ * losses behind them that multiply the hidden states with the vocabulary's weight
+ * and keep no logits.
+ *
+ * The conventions, status codes and dtype codes are those of fusionmoe.h:
+ * borrowed device pointers, asynchronous on `stream`, no allocation, no
+ * synchronisation, a status instead of an exception.  Indices are int32 or int64
+ * (index64 = 0 or 1).
+ */
+#ifndef FUSIONVOCAB_H
+#define FUSIONVOCAB_H
+
+#include "fusionmoe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FMOE_VOCAB_MAX_DIM 16384
+#define FMOE_VOCAB_MAX_TOKENS 16777216 /* rows of one call */
+#define FMOE_VOCAB_MAX_VOCAB 16777216
+#define FMOE_VOCAB_MAX_ELEMENTS 68719476736LL /* of an operand: rows * dim, vocab * dim */
+#define FMOE_VOCAB_MAX_TOP 1024        /* listed logits of a teacher per row */
+
+/* ---------------------------------------------------------------------------
+ * Token embedding: y[t] = scale * weight[ids[t]], one rounding to y's dtype, which
+ * is weight's (dtype).  Row v of weight [vocab, dim] starts at weight + v * ldw; y
+ * [T, dim] is dense.  An id outside 0 .. vocab - 1 gives a row of NaN (nothing is read).
+ * Pointers need the alignment of their element type only.
+ * ------------------------------------------------------------------------- */
+int fmoe_embedding_fwd(const void* ids, int index64, const void* weight, int dtype, int64_t ldw,
+                       int64_t T, int64_t vocab, int64_t dim, float scale, void* y, void* stream);
+
+/* Its backward: d_weight[v] = scale * sum of dy[t] over the t with ids[t] = v, every row
+ * written (zeros where v has no token).  The tokens are sorted by id, stably; a row is summed in
+ * fp32, in a fixed order (pieces of 32 of an id's tokens where it has many), without atomics: the
+ * same bits every run.  Rows of padding_idx (-1: none) stay zero, ids out of range add nothing.
+ * Row t of dy starts at dy + t * lddy.  workspace: 256-byte aligned. */
+size_t fmoe_embedding_bwd_workspace_bytes(int64_t T, int64_t vocab, int64_t dim);
+int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtype, int64_t lddy,
+                       int64_t T, int64_t vocab, int64_t dim, float scale, int64_t padding_idx,
+                       void* d_weight, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Losses over a vocabulary.  With s[t, v] = logit_scale / temperature * sum_c hidden[t, c] weight[v, c]
+ * and log p[t] = s[t] - logsumexp(s[t]):
+ *   cross entropy (teacher NULL, top = 1, temperature 1):  loss[t] = -log p[t, index[t]]
+ *   distillation from a teacher's listed logits:  q[t] = softmax(teacher[t] / temperature) over the row's
+ *     entries,  loss[t] = temperature^2 * sum_k q[t, k] (log q[t, k] - log p[t, index[t, k]])
+ * index [T, top]; an entry whose index is ignore_index, or whose teacher logit is -infinity, is none,
+ * and a row without entries has no loss, no gradient, and its hidden state is not read.  An index listed twice
+ * counts twice.  Any other index outside 0 .. vocab - 1 makes the row's loss NaN (and with it the gradients).
+ * reduction: loss [T] (0 in rows without entries), or one value, the mean over the rows with entries
+ * (NaN where there are none) or their sum.
+ *
+ * The rows with entries are packed, and tiles of the logits are formed on the matrix units, reduced to
+ * a maximum and a sum of exponentials per row and dropped; the backward forms them again, a piece
+ * of the vocabulary at a time, as G = (p - q) times the row's weight, and multiplies
+ *   d_hidden = G weight,  d_weight = G^T hidden.
+ * planes = 1: operands and G are bf16 (fp32 operands are rounded), sums fp32.  planes = 3: fp32
+ * operands and G as three bf16 numbers each, whose six largest products are added: fp32 precision.
+ * Deterministic, no atomics.
+ *
+ * state keeps what the backward needs (fmoe_vocab_loss_state_bytes); it belongs to one forward call.
+ * workspaces and state: 256-byte aligned.  hidden rows lie ldh apart, weight rows ldw.
+ * ------------------------------------------------------------------------- */
+enum fmoe_reduction { FMOE_REDUCE_NONE = 0, FMOE_REDUCE_MEAN = 1, FMOE_REDUCE_SUM = 2 };
+
+size_t fmoe_vocab_loss_state_bytes(int64_t T, int64_t dim, int64_t top, int planes);
+/* 1 where the products read a copy of weight, made a piece at a time, rather than weight as it lies
+ * (bf16 rows of a multiple of 64 elements at 16-byte addresses): an argument of the size queries. */
+int fmoe_vocab_loss_packs(const void* weight, int w_dtype, int64_t ldw, int64_t dim, int planes);
+size_t fmoe_vocab_loss_fwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int planes, int packs);
+int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh, const void* weight, int w_dtype,
+                        int64_t ldw, const void* index, int index64, const void* teacher, int t_dtype,
+                        int64_t T, int64_t dim, int64_t vocab, int64_t top, int64_t ignore_index,
+                        double logit_scale, double temperature, int planes, int reduction, float* loss,
+                        void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Backward of the call that wrote state, whose sizes and options are repeated here.  d_loss: one fp32 value, or T
+ * of them where reduction is none.  d_hidden [T, dim] and d_weight [vocab, dim] are dense and written whole; either may be NULL (not
+ * wanted). */
+size_t fmoe_vocab_loss_bwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int planes, int packs);
+int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int w_dtype, int64_t ldw, int64_t T,
+                        int64_t dim, int64_t vocab, int64_t top, int distill, double logit_scale,
+                        double temperature, int planes, int reduction, const void* state,
+                        size_t state_bytes, void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* FUSIONVOCAB_H */
