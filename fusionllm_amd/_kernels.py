@@ -736,7 +736,7 @@ def vocab_loss_state_bytes(rows: int, dim: int, top: int, planes: int) -> int:
     block = lambda n: (n + 255) // 256 * 256
     padded = (rows + 63) // 64 * 64
     padded = torch.sym_max(padded, 64)
-    return (256 + 3 * block(rows * 4) + 3 * block(rows * top * 4) + block(rows * 8) +
+    return (256 + 2 * block(rows * 4) + 3 * block(rows * top * 4) + block(rows * 8) +
             block(planes * padded * ((dim + 63) // 64 * 64) * 2))
 
 

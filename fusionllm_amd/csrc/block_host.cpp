@@ -25,6 +25,7 @@
 
 #include "../../include/fusionmoe.h"
 #include "../../include/fusiontrain.h"
+#include "../../include/fusionvocab.h"
 
 namespace {
 
@@ -37,7 +38,10 @@ using at::Tensor;
   F(fmoe_route_and_dispatch) F(fmoe_gateup_fwd) F(fmoe_down_fwd) F(fmoe_combine_fwd) F(fmoe_combine_bwd)  \
   F(fmoe_down_bwd_dx) F(fmoe_weight_grad_workspace_bytes) F(fmoe_weight_grad) F(fmoe_gateup_bwd_dx)       \
   F(fmoe_router_bwd_workspace_bytes) F(fmoe_router_bwd)                                                 \
-  F(fmoe_layer_norm_fwd) F(fmoe_layer_norm_bwd_workspace_bytes) F(fmoe_layer_norm_bwd)
+  F(fmoe_layer_norm_fwd) F(fmoe_layer_norm_bwd_workspace_bytes) F(fmoe_layer_norm_bwd)                   \
+  F(fmoe_embedding_fwd) F(fmoe_embedding_bwd_workspace_bytes) F(fmoe_embedding_bwd)                       \
+  F(fmoe_vocab_loss_state_bytes) F(fmoe_vocab_loss_packs) F(fmoe_vocab_loss_fwd_workspace_bytes)          \
+  F(fmoe_vocab_loss_fwd) F(fmoe_vocab_loss_bwd_workspace_bytes) F(fmoe_vocab_loss_bwd)
 struct Api {
 #define F(name) decltype(&::name) name = nullptr;
   FMOE_ENTRY_POINTS(F)
@@ -409,6 +413,187 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
   return norm_fwd(norm_rows(x), vector_or_none(w), vector_or_none(b), eps, out_dtype, false)[0];
 }
 
+// ---- embedding -------------------------------------------------------------------------
+
+int index64(const Tensor& t) { return t.scalar_type() == at::kLong; }
+
+// Operands of the vocabulary operators are checked by the caller (fusionllm_amd/vocab.py).
+Tensor embedding_fwd(const Tensor& ids, const Tensor& weight, double scale) {
+  need_entry_points();
+  const Tensor w = norm_rows(weight);
+  Tensor y = empty({ids.numel(), w.size(1)}, w.scalar_type(), w);
+  check(api.fmoe_embedding_fwd(ids.data_ptr(), index64(ids), w.data_ptr(), dtype_code(w.scalar_type()), w.stride(0),
+                               ids.numel(), w.size(0), w.size(1), static_cast<float>(scale), y.data_ptr(),
+                               current_stream(w)),
+        "fmoe_embedding_fwd");
+  return y;
+}
+
+Tensor embedding_bwd(const Tensor& ids, const Tensor& dy, int64_t vocab, double scale, int64_t pad) {
+  need_entry_points();
+  const Tensor g = norm_rows(dy);
+  const int64_t T = ids.numel(), d = g.size(1);
+  Tensor dw = empty({vocab, d}, g.scalar_type(), g);
+  const Workspace ws(api.fmoe_embedding_bwd_workspace_bytes(T, vocab, d), g);
+  const int code = dtype_code(g.scalar_type());
+  check(api.fmoe_embedding_bwd(ids.data_ptr(), index64(ids), g.data_ptr(), code, g.stride(0), T, vocab, d,
+                               static_cast<float>(scale), pad, dw.data_ptr(), code, ws.ptr(), ws.bytes,
+                               current_stream(g)),
+        "fmoe_embedding_bwd");
+  return dw;
+}
+
+// As LayerNormBackward: what a backward pass returns cannot be differentiated again, and says so.
+struct EmbeddingBackward : torch::autograd::Function<EmbeddingBackward> {
+  static Tensor forward(AutogradContext*, const Tensor& dy, const Tensor& ids, int64_t vocab, double scale, int64_t pad) {
+    return embedding_bwd(ids, dy, vocab, scale, pad);
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    throw std::runtime_error("fusionllm_amd.embedding: second derivatives are not implemented");
+  }
+};
+
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t pad) {
+    const c10::DeviceGuard guard(weight.device());
+    ctx->save_for_backward({ids});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = pad;
+    return embedding_fwd(ids, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(4);
+    const variable_list saved = ctx->get_saved_variables();
+    if (!grads[0].defined() || !ctx->needs_input_grad(1)) return out;
+    const c10::DeviceGuard guard(grads[0].device());
+    const int64_t vocab = ctx->saved_data["vocab"].toInt(), pad = ctx->saved_data["pad"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    out[1] = at::GradMode::is_enabled() ? EmbeddingBackward::apply(grads[0], saved[0], vocab, scale, pad)
+                                        : embedding_bwd(saved[0], grads[0], vocab, scale, pad);
+    return out;
+  }
+};
+
+// scale * weight[ids] for ids [T] (contiguous); differentiable where grad says so.
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, bool grad) {
+  if (grad) return Embedding::apply(ids, weight, scale, pad);
+  const c10::DeviceGuard guard(weight.device());
+  return embedding_fwd(ids, weight, scale);
+}
+
+// ---- losses over the vocabulary -----------------------------------------------------------
+
+struct LossOptions {
+  int64_t ignore_index;
+  double logit_scale, temperature;
+  int64_t planes, reduction;  // FMOE_REDUCE_*
+};
+
+// loss, state
+std::array<Tensor, 2> loss_fwd(const Tensor& h, const Tensor& w, const Tensor& index, const Tensor& teacher,
+                               const LossOptions& o) {
+  need_entry_points();
+  const int64_t T = h.size(0), d = h.size(1), V = w.size(0), top = index.size(1);
+  const int planes = static_cast<int>(o.planes), wc = dtype_code(w.scalar_type());
+  const int packs = api.fmoe_vocab_loss_packs(w.data_ptr(), wc, w.stride(0), d, planes);
+  const size_t bytes = api.fmoe_vocab_loss_state_bytes(T, d, top, planes);
+  Tensor state = empty({static_cast<int64_t>(bytes)}, at::kByte, h);
+  const Workspace ws(api.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, planes, packs), h);
+  Tensor loss = o.reduction == FMOE_REDUCE_NONE ? empty({T}, at::kFloat, h) : empty({}, at::kFloat, h);
+  // (an empty tensor has no address; the entry point wants one for its output)
+  float* lp = static_cast<float*>(T == 0 && o.reduction == FMOE_REDUCE_NONE ? state.data_ptr() : loss.data_ptr());
+  check(api.fmoe_vocab_loss_fwd(h.data_ptr(), dtype_code(h.scalar_type()), h.stride(0), w.data_ptr(), wc, w.stride(0),
+                                index.data_ptr(), index64(index), ptr_or_null(teacher),
+                                teacher.defined() ? dtype_code(teacher.scalar_type()) : FMOE_F32, T, d, V, top,
+                                o.ignore_index, o.logit_scale, o.temperature, planes, static_cast<int>(o.reduction), lp,
+                                state.data_ptr(), bytes, ws.ptr(), ws.bytes, current_stream(h)),
+        "fmoe_vocab_loss_fwd");
+  return {loss, state};
+}
+
+// d_hidden [T, d], d_weight, each undefined where it is not wanted.
+std::array<Tensor, 2> loss_bwd(const Tensor& d_loss, const Tensor& w, const Tensor& state, int64_t T, int64_t top,
+                               bool distill, const LossOptions& o, at::ScalarType h_dtype, bool need_h, bool need_w) {
+  need_entry_points();
+  const Tensor up = d_loss.contiguous();
+  const int64_t V = w.size(0), d = w.size(1);
+  const int planes = static_cast<int>(o.planes), wc = dtype_code(w.scalar_type());
+  std::array<Tensor, 2> out;
+  if (need_h) out[0] = empty({T, d}, h_dtype, w);
+  if (need_w) out[1] = empty({V, d}, w.scalar_type(), w);
+  const int packs = api.fmoe_vocab_loss_packs(w.data_ptr(), wc, w.stride(0), d, planes);
+  const Workspace ws(api.fmoe_vocab_loss_bwd_workspace_bytes(T, d, V, planes, packs), w);
+  const void* upp = up.numel() == 0 ? state.data_ptr() : up.data_ptr();
+  check(api.fmoe_vocab_loss_bwd(static_cast<const float*>(upp), w.data_ptr(), wc, w.stride(0), T, d, V, top, distill,
+                                o.logit_scale, o.temperature, planes, static_cast<int>(o.reduction), state.data_ptr(),
+                                static_cast<size_t>(state.numel()), ptr_or_null(out[0]), dtype_code(h_dtype),
+                                ptr_or_null(out[1]), wc, ws.ptr(), ws.bytes, current_stream(w)),
+        "fmoe_vocab_loss_bwd");
+  return out;
+}
+
+struct VocabLossBackward : torch::autograd::Function<VocabLossBackward> {
+  static variable_list forward(AutogradContext*, const Tensor& d_loss, const Tensor& w, const Tensor& state, int64_t T,
+                               int64_t top, bool distill, const LossOptions& o, at::ScalarType h_dtype, bool need_h,
+                               bool need_w) {
+    variable_list out;
+    for (const Tensor& t : loss_bwd(d_loss, w, state, T, top, distill, o, h_dtype, need_h, need_w))
+      if (t.defined()) out.push_back(t);
+    return out;
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    throw std::runtime_error("fusionllm_amd losses over the vocabulary: second derivatives are not implemented");
+  }
+};
+
+struct VocabLoss : torch::autograd::Function<VocabLoss> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& index,
+                        const OptTensor& teacher, const LossOptions& o) {
+    const c10::DeviceGuard guard(weight.device());
+    const Tensor w = norm_rows(weight);
+    const auto out = loss_fwd(norm_rows(hidden), w, index, vector_or_none(teacher), o);
+    ctx->save_for_backward({w, out[1]});
+    auto& d = ctx->saved_data;
+    d["T"] = hidden.size(0), d["top"] = index.size(1), d["distill"] = teacher.has_value();
+    d["scale"] = o.logit_scale, d["temperature"] = o.temperature, d["planes"] = o.planes, d["reduction"] = o.reduction;
+    d["h_dtype"] = static_cast<int64_t>(hidden.scalar_type());
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(5);
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const variable_list saved = ctx->get_saved_variables();
+    if (!grads[0].defined() || !(need_h || need_w)) return out;
+    const c10::DeviceGuard guard(saved[0].device());
+    auto& d = ctx->saved_data;
+    const LossOptions o{0, d["scale"].toDouble(), d["temperature"].toDouble(), d["planes"].toInt(), d["reduction"].toInt()};
+    const auto h_dtype = static_cast<at::ScalarType>(d["h_dtype"].toInt());
+    const int64_t T = d["T"].toInt(), top = d["top"].toInt();
+    const bool distill = d["distill"].toBool();
+    if (at::GradMode::is_enabled()) {
+      variable_list g = VocabLossBackward::apply(grads[0], saved[0], saved[1], T, top, distill, o, h_dtype, need_h, need_w);
+      size_t i = 0;
+      if (need_h) out[0] = g[i++];
+      if (need_w) out[1] = g[i++];
+      return out;
+    }
+    const auto g = loss_bwd(grads[0], saved[0], saved[1], T, top, distill, o, h_dtype, need_h, need_w);
+    out[0] = g[0], out[1] = g[1];
+    return out;
+  }
+};
+
+// The loss of hidden [T, d] against weight [V, d] over index [T, top] (teacher: its logits, or none).
+Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& index, const OptTensor& teacher,
+                  int64_t ignore_index, double logit_scale, double temperature, int64_t planes, int64_t reduction,
+                  bool grad) {
+  const LossOptions o{ignore_index, logit_scale, temperature, planes, reduction};
+  if (grad) return VocabLoss::apply(hidden, weight, index, teacher, o);
+  const c10::DeviceGuard guard(weight.device());
+  return loss_fwd(norm_rows(hidden), norm_rows(weight), index, vector_or_none(teacher), o)[0];
+}
+
 }  // namespace
 
 // Other Python threads run during a sequence, as they do during a ctypes call.
@@ -425,4 +610,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward", &forward, py::call_guard<py::gil_scoped_release>());
   m.def("backward", &backward, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
+  m.def("vocab_loss", &vocab_loss, py::call_guard<py::gil_scoped_release>());
 }

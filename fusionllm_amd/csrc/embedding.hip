@@ -2,12 +2,14 @@
 // dW[v] = scale * sum of dy[t] over the tokens t of v.
 //
 // Both are bound by memory: the forward reads and writes T rows; the backward reads
-// T rows and writes the V rows of the gradient, most of them zeros.  A row is read in
-// pieces of 512 columns, 8 consecutive elements per lane, one wave per piece.
+// T rows and writes the V rows of the gradient, most of them zeros.  A wave takes 1 KB of a row at a time,
+// 16 bytes per lane.
 //
 // The gradient is summed without atomics, so that the same bits come out every run:
-//   1. embed_sort_kernel sorts the tokens by id, stably, in one launch: a workgroup owns 512 ids and
-//      walks all the tokens itself (T indices from L2), so that no workgroup waits for another.
+//   1. embed_sort_kernel sorts the tokens by id, stably, in one launch: a workgroup owns up to 512 ids and
+//      walks all the tokens itself (T indices from L2), so that no workgroup waits for another.  It owns every
+//      G-th id (G workgroups, a power of two): the frequent ids, which a tokenizer numbers first, fall to
+//      different workgroups.  So "sorted" is by slot, (id mod G) * 512 + id / G.
 //   2. embed_sum_kernel adds the rows of the sorted tokens, kTile at a time per wave: an id whose tokens
 //      lie in one tile is written there; one that crosses tiles leaves an fp32 partial row per tile.
 //   3. embed_rest_kernel writes the ids that cross tiles, from their partial rows in order, and zeros
@@ -18,16 +20,51 @@
 
 namespace fmoe {
 
-constexpr int kSegment = 512;      // columns per wave: 64 lanes of 8
-constexpr int kTile = 32;          // sorted tokens per wave of embed_sum_kernel
-constexpr int kSortIds = 512;      // ids per workgroup of the sort
+constexpr int kTile = 16;          // sorted tokens per wave of embed_sum_kernel
+constexpr int kSortIds = 512;      // ids per workgroup of the sort, at most
 constexpr int kSortWaves = 16;
-constexpr int kRestIds = 8;        // ids per wave of embed_rest_kernel
+constexpr int kRestIds = 8;        // slots per wave of embed_rest_kernel
 constexpr int kRestWaves = 16;
-constexpr int kLongTiles = 32;     // tiles above which a workgroup adds an id's partial rows together
+constexpr int kLongTiles = 8;      // tiles above which a workgroup adds an id's partial rows together
 
-__device__ __forceinline__ int64_t load_index(const void* p, bool index64, int64_t i) {
-  return index64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+// Consecutive elements per lane: 16 bytes.
+template <int DT>
+constexpr int kPer = DT == FMOE_BF16 ? 8 : 4;
+constexpr int segments_of(int64_t D, int dtype) { return static_cast<int>((D + (dtype == FMOE_BF16 ? 511 : 255)) / (dtype == FMOE_BF16 ? 512 : 256)); }
+
+// V elements at any element's address, n of them inside the row.
+template <int DT, int V>
+__device__ __forceinline__ void load_v(const void* base, int64_t e, int n, float* v) {
+  if (n >= V && DT == FMOE_BF16 && V == 8) {
+    unpack<FMOE_BF16, 8>(load_raw<FMOE_BF16, 8>(base, e), v);
+  } else if (n >= V && DT == FMOE_F32 && V % 4 == 0) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const f32x4 x = reinterpret_cast<const f32x4_e4*>(static_cast<const float*>(base) + e)[q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * q + i] = x[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = 0.0f;
+      if (i < n) unpack<DT, 1>(load_raw<DT, 1>(base, e + i), v + i);
+    }
+  }
+}
+template <int DT, int V>
+__device__ __forceinline__ void store_v(void* base, int64_t e, int n, const float* v) {
+  if (n >= V && DT == FMOE_BF16 && V == 8) {
+    store_chunk<FMOE_BF16, 8>(base, e, v);
+  } else if (n >= V && DT == FMOE_F32 && V % 4 == 0) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q)
+      reinterpret_cast<f32x4_e4*>(static_cast<float*>(base) + e)[q] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) store_chunk<DT, 1>(base, e + i, v + i);
+  }
 }
 
 struct EmbedArgs {
@@ -40,67 +77,93 @@ struct EmbedArgs {
   int index64;
   int pad;           // -1: none
   float scale;
-  int *start, *order, *key;  // backward: first sorted position of each id [V + 1], tokens and ids by position
-  float* part;               // [tiles][2][D]: of the id that comes from the tile before, of the one that goes on
+  // backward
+  int shift;         // G = 1 << shift
+  int slots;         // G * kSortIds
+  int* start;        // first sorted position of each slot [slots + 1]
+  int2* sorted;      // token and slot by position
+  float* part;       // [tiles][2][D]: of the id that comes from the tile before, of the one that goes on
 };
 
 // ROWS rows per wave: their loads are in flight together.
 template <int DT, int ROWS>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const EmbedArgs a) {
+  constexpr int V = kPer<DT>;
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t group = item / a.segments;
-  const int c = static_cast<int>(item - group * a.segments) * kSegment + lane * 8;
-  const int n = min(a.D - c, 8);
+  const int c = (static_cast<int>(item - group * a.segments) * 64 + lane) * V;
+  const int n = min(a.D - c, V);
   const int64_t t0 = group * ROWS;
   if (t0 >= a.T) return;
-  float v[ROWS][8];
+  float v[ROWS][V];
   bool bad[ROWS];
+  int64_t id[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int64_t id = load_index(a.ids, a.index64, min(t0 + r, a.T - 1));
-    bad[r] = id < 0 || id >= a.V;
-    load_upto8<DT>(a.src, (bad[r] ? 0 : id) * a.ld + c, bad[r] ? 0 : n, v[r]);
+    const int64_t at = min(t0 + r, a.T - 1);
+    id[r] = a.index64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    bad[r] = id[r] < 0 || id[r] >= a.V;
+    load_v<DT, V>(a.src, (bad[r] ? 0 : id[r]) * a.ld + c, bad[r] ? 0 : n, v[r]);
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     if (t0 + r >= a.T) break;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[r][e] = bad[r] ? __builtin_nanf("") : v[r][e] * a.scale;
-    store_upto8<DT>(a.dst, (t0 + r) * a.D + c, n, v[r]);
+    for (int e = 0; e < V; ++e) v[r][e] = bad[r] ? __builtin_nanf("") : v[r][e] * a.scale;
+    store_v<DT, V>(a.dst, (t0 + r) * a.D + c, n, v[r]);
   }
 }
 
-// Sorted positions of the tokens of ids lo .. lo + 511, after the tokens of smaller ids.  Wave w walks
-// its sixteenth of the tokens twice: counts per id first, then places, where a token's rank among its
-// wave's earlier tokens of the same id comes from ballots over the bits of the id.
+// Sorted positions of the tokens of this workgroup's ids, after the tokens of those of lower workgroups.  Wave w walks
+// its sixteenth of the tokens twice: counts per id first, then places, where a token's rank among the
+// 64 tokens of the same id comes from ballots.  The loads of 16 tokens
+// per lane are in flight together (no branch around them).
+template <bool I64>
 __global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(const EmbedArgs a) {
   __shared__ int hist[kSortWaves][kSortIds];
   __shared__ int below[kSortWaves], waves[kSortIds / 64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int lo = blockIdx.x * kSortIds;
-  for (int i = tid; i < kSortWaves * kSortIds; i += 64 * kSortWaves) (&hist[0][0])[i] = 0;
-  __syncthreads();
-  const int64_t per = ((a.T + 63) / 64 + kSortWaves - 1) / kSortWaves * 64;
-  const int64_t t0 = min(w * per, a.T), t1 = min(t0 + per, a.T);
-  // an id as int: -1 where the token adds nothing
-  auto token_id = [&](int64_t t) {
-    if (t >= t1) return -1;
-    const int64_t id = load_index(a.ids, a.index64, t);
-    return id < 0 || id >= a.V || id == a.pad ? -1 : static_cast<int>(id);
-  };
-  constexpr int U = 8;
-  int less = 0;
-  for (int64_t t = t0; t < t1; t += 64 * U) {
-    int id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) id[u] = token_id(t + 64 * u + lane);
+  const int mine = blockIdx.x, lo = mine * kSortIds;
+  const int per = static_cast<int>(((a.T + 63) / 64 + kSortWaves - 1) / kSortWaves * 64);
+  const int T = static_cast<int>(a.T), t0 = min(w * per, T), t1 = min(t0 + per, T);
+  constexpr int U = 16;
+  // slots of the tokens t + 64 u + lane relative to lo, -1 where a token adds nothing here; less: tokens of
+  // lower workgroups
+  auto load_slots = [&](int t, int (&k)[U], int& less) __attribute__((always_inline)) {
+    uint32_t id[U], high[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      less += id[u] >= 0 && id[u] < lo;
-      const int k = id[u] - lo;
-      if (id[u] >= lo && k < kSortIds) atomicAdd(&hist[w][k], 1);  // counts: any order
+      const int at = min(t + 64 * u + lane, T - 1);
+      if constexpr (I64) {
+        const uint2 raw = static_cast<const uint2*>(a.ids)[at];
+        id[u] = raw.x, high[u] = raw.y;
+      } else {
+        id[u] = static_cast<const uint32_t*>(a.ids)[at], high[u] = 0;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool out = high[u] != 0 || id[u] >= static_cast<uint32_t>(a.V) || id[u] == static_cast<uint32_t>(a.pad) ||
+                       t + 64 * u + lane >= t1;
+      const int owner = out ? INT32_MAX : static_cast<int>(id[u]) & ((1 << a.shift) - 1);
+      less += owner < mine;
+      k[u] = owner == mine ? static_cast<int>(id[u]) >> a.shift : -1;
+    }
+  };
+  int k[U], less = 0, ignored = 0;
+  if (t0 < t1) load_slots(t0, k, less);
+  for (int i = tid; i < kSortWaves * kSortIds / 4; i += 64 * kSortWaves)
+    reinterpret_cast<int4*>(&hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  for (int t = t0; t < t1; t += 64 * U) {
+    if (t > t0) load_slots(t, k, less);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k[u] >= 0) atomicAdd(&hist[w][k[u]], 1);  // counts: any order
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) less += __shfl_xor(less, off, 64);
@@ -119,8 +182,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(const Embed
 #pragma unroll
     for (int q = 0; q < kSortWaves; ++q) at += below[q];
     for (int q = 0; q < w; ++q) at += waves[q];
-    if (lo + tid <= a.V) a.start[lo + tid] = at;  // (of id V: where the last id ends)
-    if (tid == kSortIds - 1 && lo + kSortIds == a.V) a.start[a.V] = at + total;
+    a.start[lo + tid] = at;
+    if (lo + tid + 1 == a.slots) a.start[a.slots] = at + total;
 #pragma unroll
     for (int q = 0; q < kSortWaves; ++q) {
       const int n = hist[q][tid];
@@ -129,167 +192,211 @@ __global__ __launch_bounds__(64 * kSortWaves) void embed_sort_kernel(const Embed
     }
   }
   __syncthreads();
-  for (int64_t t = t0; t < t1; t += 64 * U) {
-    int id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) id[u] = token_id(t + 64 * u + lane);
+  for (int t = t0; t < t1; t += 64 * U) {
+    if (per > 64 * U) load_slots(t, k, ignored);  // (else they are there still)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = id[u] - lo;
-      const bool mine = id[u] >= lo && k < kSortIds;
-      uint64_t same = __ballot(mine);
-      if (same == 0) continue;
+      uint64_t left = __ballot(k[u] >= 0), same = left;
+      if (left == 0) continue;
+      if (__popcll(left) <= 8) {  // few of this workgroup's tokens: one comparison per id among them
+        while (left != 0) {
+          const int first = __builtin_amdgcn_readlane(k[u], __builtin_ctzll(left));
+          const uint64_t equal = __ballot(k[u] == first);
+          if (k[u] == first) same = equal;
+          left &= ~equal;
+        }
+      } else {  // one per bit of the id
 #pragma unroll
-      for (int b = 0; b < 9; ++b) {
-        const bool bit = (k >> b) & 1;
-        const uint64_t on = __ballot(bit);
-        same &= bit ? on : ~on;
+        for (int b = 0; b < 9; ++b) {
+          const bool bit = (k[u] >> b) & 1;
+          const uint64_t on = __ballot(bit);
+          same &= bit ? on : ~on;
+        }
       }
-      if (mine) {
+      if (k[u] >= 0) {
         const int rank = __popcll(same & ((uint64_t(1) << lane) - 1));
-        const int base = hist[w][k];
-        const int at = base + rank;
-        a.order[at] = static_cast<int>(t + 64 * u + lane);
-        a.key[at] = id[u];
+        const int base = hist[w][k[u]];
+        a.sorted[base + rank] = make_int2(t + 64 * u + lane, lo + k[u]);
         // (the wave's reads of base are before this: LDS operations of a wave run in order)
-        if (rank == 0) hist[w][k] = base + __popcll(same);
+        if (rank == 0) hist[w][k[u]] = base + __popcll(same);
       }
     }
   }
 }
 
+// Row of the weight that a slot stands for.
+__device__ __forceinline__ int64_t slot_id(const EmbedArgs& a, int slot) {
+  return (static_cast<int64_t>(slot % kSortIds) << a.shift) + slot / kSortIds;
+}
+
+// 16 bytes of a row as they lie in memory.
+template <int DT>
+struct Row16 {
+  typedef u32x4_e2 type;
+};
+template <>
+struct Row16<FMOE_F32> {
+  typedef f32x4_e4 type;
+};
+
+// A tile's rows are all in flight together.
 template <int DY, int DW>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedArgs a) {
+  constexpr int V = kPer<DY>;
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tile = item / a.segments;
-  const int c = static_cast<int>(item - tile * a.segments) * kSegment + lane * 8;
-  const int n = min(a.D - c, 8);
-  const int total = a.start[a.V];
+  const int c = (static_cast<int>(item - tile * a.segments) * 64 + lane) * V;
+  const int n = min(a.D - c, V);
+  const int total = a.start[a.slots];
   const int64_t p0 = tile * kTile;
   if (p0 >= total) return;
   const int count = static_cast<int>(min(static_cast<int64_t>(total) - p0, int64_t(kTile)));
-  // lane i: the i-th sorted token and its id; the ids before and after the tile
-  const int64_t at = p0 + min(lane, count - 1);
-  const int token = a.order[at], id = a.key[at];
-  const int before = p0 > 0 ? a.key[p0 - 1] : -1;
-  const int after = p0 + count < total ? a.key[p0 + count] : -1;
-  float acc[8];
+  // lane i: the i-th sorted token and its slot, then the slot after the tile; lane 63: the one before
+  const int64_t at = lane == 63 ? p0 - 1 : p0 + lane;
+  int2 ts = make_int2(0, -1);
+  if (at >= 0 && at < total && (lane <= kTile || lane == 63)) ts = a.sorted[at];
+  const int token = ts.x, slot = ts.y;
+  const int before = __builtin_amdgcn_readlane(slot, 63);
+  const bool whole = n >= V;  // of this lane's columns
+  typedef typename Row16<DY>::type Raw16;
+  Raw16 raw[kTile];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-  bool from_before = __builtin_amdgcn_readlane(id, 0) == before;
-  constexpr int U = 8;
-  for (int i0 = 0; i0 < count; i0 += U) {
-    float v[U][8];
+  for (int i = 0; i < kTile; ++i) {
+    const int64_t t = __builtin_amdgcn_readlane(token, min(i, count - 1));
+    if (whole)
+      raw[i] = *reinterpret_cast<const Raw16*>(static_cast<const uint8_t*>(a.src) + (t * a.ld + c) * (16 / V));
+  }
+  float acc[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t t = __builtin_amdgcn_readlane(token, min(i0 + u, count - 1));
-      load_upto8<DY>(a.src, t * a.ld + c, n, v[u]);
+  for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+  bool from_before = __builtin_amdgcn_readlane(slot, 0) == before;
+  auto flush = [&](int cur, bool goes_on) {
+    if (from_before || goes_on) {
+      store_v<FMOE_F32, V>(a.part, (2 * tile + (from_before ? 0 : 1)) * a.D + c, n, acc);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = acc[e] * a.scale;
+      store_v<DW, V>(a.dst, slot_id(a, cur) * a.D + c, n, acc);
     }
+    from_before = false;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      if (i >= count) break;
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+  };
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = acc[e] + v[u][e];
-      const int cur = __builtin_amdgcn_readlane(id, i);
-      const int next = i + 1 < count ? __builtin_amdgcn_readlane(id, min(i + 1, 63)) : after;
-      if (i + 1 < count && next == cur) continue;
-      const bool goes_on = next == cur;
-      if (from_before || goes_on) {
-        store_upto8<FMOE_F32>(a.part, (2 * tile + (from_before ? 0 : 1)) * a.D + c, n, acc);
+  for (int i = 0; i < kTile; ++i) {
+    if (i < count) {
+      float v[V];
+      if (!whole) {
+        load_v<DY, V>(a.src, static_cast<int64_t>(__builtin_amdgcn_readlane(token, i)) * a.ld + c, n, v);
+      } else if constexpr (DY == FMOE_F32) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = raw[i][e];
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = acc[e] * a.scale;
-        store_upto8<DW>(a.dst, static_cast<int64_t>(cur) * a.D + c, n, acc);
+        for (int e = 0; e < V / 2; ++e) {
+          v[2 * e] = __uint_as_float(raw[i][e] << 16);
+          v[2 * e + 1] = __uint_as_float(raw[i][e] & 0xffff0000u);
+        }
       }
-      from_before = false;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+      for (int e = 0; e < V; ++e) acc[e] = acc[e] + v[e];
+      // (past the last token the slot is -1)
+      const int cur = __builtin_amdgcn_readlane(slot, i), next = __builtin_amdgcn_readlane(slot, i + 1);
+      if (i + 1 >= count || next != cur) flush(cur, next == cur);
     }
   }
 }
 
 // Partial rows first .. last of an id's later tiles, stepping by step, added to acc.
+template <int V>
 __device__ __forceinline__ void add_partials(const EmbedArgs& a, int64_t first, int64_t last, int64_t step, int c, int n,
                                              float* acc) {
   constexpr int U = 8;
   for (int64_t q = first; q <= last; q += U * step) {
-    float v[U][8];
+    float v[U][V];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      load_upto8<FMOE_F32>(a.part, 2 * min(q + u * step, last) * a.D + c, n, v[u]);
+      load_v<FMOE_F32, V>(a.part, 2 * min(q + u * step, last) * a.D + c, n, v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = q + u * step <= last ? acc[e] + v[u][e] : acc[e];
+      for (int e = 0; e < V; ++e) acc[e] = q + u * step <= last ? acc[e] + v[u][e] : acc[e];
   }
 }
 
+// Workgroups 0 .. blocks - 1: 128 slots each, those without tokens and those of a few tiles.  The others:
+// 16 tiles each; the ids that begin in them and go on through more than kLongTiles tiles.
 template <int DW>
-__global__ __launch_bounds__(64 * kRestWaves) void embed_rest_kernel(const EmbedArgs a) {
-  __shared__ float sums[kRestWaves][kSegment];
+__global__ __launch_bounds__(64 * kRestWaves) void embed_rest_kernel(const EmbedArgs a, int blocks) {
+  constexpr int V = kPer<DW>;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t group = blockIdx.x / a.segments;
-  const int c = static_cast<int>(blockIdx.x - group * a.segments) * kSegment + lane * 8;
-  const int n = min(a.D - c, 8);
-  const int block0 = static_cast<int>(group) * (kRestIds * kRestWaves);
-  const int v0 = block0 + w * kRestIds;
-  const int starts = a.start[min(v0 + min(lane, kRestIds), a.V)];
-  float zero[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) zero[e] = 0.0f;
-  uint64_t longs = 0;
-#pragma unroll
-  for (int i = 0; i < kRestIds; ++i) {
-    if (v0 + i >= a.V) break;
-    const int s = __builtin_amdgcn_readlane(starts, i), e = __builtin_amdgcn_readlane(starts, i + 1);
-    const int64_t o = static_cast<int64_t>(v0 + i) * a.D + c;
-    if (s == e) {
-      store_upto8<DW>(a.dst, o, n, zero);
-      continue;
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    __shared__ float sums[kRestWaves][64 * V];
+    __shared__ int found[kRestWaves];
+    const int item = blockIdx.x - blocks, group = item / a.segments;
+    const int c = ((item - group * a.segments) * 64 + lane) * V, n = min(a.D - c, V);
+    {
+      // wave w: the id that goes on from its tile into the next one, if it begins in it and is long
+      const int64_t tile = static_cast<int64_t>(group) * kRestWaves + w, next = (tile + 1) * kTile;
+      int slot = -1;
+      if (next < a.start[a.slots]) {
+        slot = a.sorted[next].y;
+        const int64_t ta = a.start[slot] / kTile, tb = (a.start[slot + 1] - 1) / kTile;
+        if (ta != tile || tb - ta <= kLongTiles) slot = -1;
+      }
+      if (lane == 0) found[w] = slot;
     }
-    const int64_t ta = s / kTile, tb = (e - 1) / kTile;
-    if (ta == tb) continue;  // written with its tile
-    if (tb - ta > kLongTiles) {
-      longs |= uint64_t(1) << i;
-      continue;
-    }
-    // first piece: the second partial of its tile, or the first one where the id begins with the tile
-    // and fills it (then nothing comes from the tile before, and it is the one that goes on)
-    float acc[8];
-    load_upto8<FMOE_F32>(a.part, (2 * ta + 1) * a.D + c, n, acc);
-    add_partials(a, ta + 1, tb, 1, c, n, acc);
+    __syncthreads();
+    for (int f = 0; f < kRestWaves; ++f) {
+      const int slot = found[f];
+      if (slot < 0) continue;
+      const int64_t ta = a.start[slot] / kTile, tb = (a.start[slot + 1] - 1) / kTile;
+      // wave w every 16th partial row, then the waves in order
+      float acc[V];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] = acc[q] * a.scale;
-    store_upto8<DW>(a.dst, o, n, acc);
-  }
-  // ids of many tiles: the whole workgroup, wave w every 16th partial row, then the waves in order
-  __shared__ uint64_t long_ids[kRestWaves];
-  if (lane == 0) long_ids[w] = longs;
-  __syncthreads();
-  for (int q = 0; q < kRestWaves; ++q)
-    for (uint64_t left = long_ids[q]; left != 0; left &= left - 1) {
-      const int v = block0 + q * kRestIds + __builtin_ctzll(left);
-      const int64_t ta = a.start[v] / kTile, tb = (a.start[v + 1] - 1) / kTile;
-      float acc[8];
+      for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+      if (w == 0) load_v<FMOE_F32, V>(a.part, (2 * ta + 1) * a.D + c, n, acc);
+      add_partials<V>(a, ta + 1 + w, tb, kRestWaves, c, n, acc);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-      if (w == 0) load_upto8<FMOE_F32>(a.part, (2 * ta + 1) * a.D + c, n, acc);
-      add_partials(a, ta + 1 + w, tb, kRestWaves, c, n, acc);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[w][lane * 8 + e] = acc[e];
+      for (int q = 0; q < V; ++q) sums[w][q * 64 + lane] = acc[q];
       __syncthreads();
       if (w == 0) {
         for (int p = 1; p < kRestWaves; ++p)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] = acc[e] + sums[p][lane * 8 + e];
+          for (int q = 0; q < V; ++q) acc[q] = acc[q] + sums[p][q * 64 + lane];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = acc[e] * a.scale;
-        store_upto8<DW>(a.dst, static_cast<int64_t>(v) * a.D + c, n, acc);
+        for (int q = 0; q < V; ++q) acc[q] = acc[q] * a.scale;
+        store_v<DW, V>(a.dst, slot_id(a, slot) * a.D + c, n, acc);
       }
       __syncthreads();
     }
+    return;
+  }
+  const int group = blockIdx.x / a.segments;
+  const int c = ((static_cast<int>(blockIdx.x) - group * a.segments) * 64 + lane) * V, n = min(a.D - c, V);
+  const int s0 = (group * kRestWaves + w) * kRestIds;
+  const int starts = a.start[min(s0 + min(lane, kRestIds), a.slots)];
+  float zero[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRestIds; ++i) {
+    const int64_t id = slot_id(a, s0 + i);
+    if (id >= a.V) continue;
+    const int s = __builtin_amdgcn_readlane(starts, i), e = __builtin_amdgcn_readlane(starts, i + 1);
+    const int64_t o = id * a.D + c, ta = s / kTile, tb = (e - 1) / kTile;
+    if (s == e) {
+      store_v<DW, V>(a.dst, o, n, zero);
+    } else if (ta < tb && tb - ta <= kLongTiles) {  // (in one tile: written with it)
+      float acc[V];
+      load_v<FMOE_F32, V>(a.part, (2 * ta + 1) * a.D + c, n, acc);
+      add_partials<V>(a, ta + 1, tb, 1, c, n, acc);
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] = acc[q] * a.scale;
+      store_v<DW, V>(a.dst, o, n, acc);
+    }
+  }
 }
 
 inline bool elem_aligned(const void* p, int dtype) {
@@ -300,7 +407,7 @@ int embed_check(const void* ids, int index64, const void* src, int src_dtype, in
                 int64_t vocab, int64_t dim, const void* dst, int dst_dtype) {
   if (T < 0 || vocab <= 0 || dim <= 0 || index64 < 0 || index64 > 1) return FMOE_ERR_INVALID_ARG;
   if (dim > FMOE_VOCAB_MAX_DIM || T > FMOE_VOCAB_MAX_TOKENS || vocab > FMOE_VOCAB_MAX_VOCAB) return FMOE_ERR_SHAPE;
-  // (more elements than the card's memory holds: the launches stay below 2^32 threads)
+  // (the launches stay below 2^32 threads)
   if (T * dim > FMOE_VOCAB_MAX_ELEMENTS || vocab * dim > FMOE_VOCAB_MAX_ELEMENTS) return FMOE_ERR_SHAPE;
   if (src_rows > 1 && (ld < dim || ld > (int64_t(1) << 38))) return FMOE_ERR_SHAPE;
   for (const int d : {src_dtype, dst_dtype})
@@ -314,17 +421,19 @@ int embed_check(const void* ids, int index64, const void* src, int src_dtype, in
 }
 
 struct EmbedSpace {
-  size_t start, order, key, part, bytes;
+  int shift = 0;
+  int64_t slots;
+  size_t start, sorted, part, bytes = 0;
   EmbedSpace(int64_t T, int64_t V, int64_t D) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += (n + 255) & ~size_t(255);
       return at;
     };
-    bytes = 0;
-    start = take((V + 1) * 4);
-    order = take(T * 4);
-    key = take(T * 4);
+    while ((int64_t(kSortIds) << shift) < V) ++shift;
+    slots = int64_t(kSortIds) << shift;
+    start = take((slots + 1) * 4);
+    sorted = take(T * 8);
     part = take(static_cast<size_t>(ceil_div(T, kTile)) * 2 * D * 4);
   }
 };
@@ -341,7 +450,7 @@ extern "C" int fmoe_embedding_fwd(const void* ids, int index64, const void* weig
   EmbedArgs a{};
   a.ids = ids, a.index64 = index64, a.src = weight, a.ld = ldw, a.dst = y, a.T = T;
   a.V = static_cast<int>(vocab), a.D = static_cast<int>(dim), a.scale = scale;
-  a.segments = static_cast<int>(ceil_div(dim, kSegment));
+  a.segments = segments_of(dim, dtype);
   // four rows per wave (their loads overlap) where that still fills every CU with 16 waves
   constexpr int R = 4;
   const bool many = T * a.segments >= R * 256 * 16;
@@ -378,22 +487,30 @@ extern "C" int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, 
   EmbedArgs a{};
   a.ids = ids, a.index64 = index64, a.src = dy, a.ld = lddy, a.dst = d_weight, a.T = T;
   a.V = static_cast<int>(vocab), a.D = static_cast<int>(dim), a.scale = scale, a.pad = static_cast<int>(padding_idx);
-  a.segments = static_cast<int>(ceil_div(dim, kSegment));
+  a.shift = space.shift, a.slots = static_cast<int>(space.slots);
   a.start = reinterpret_cast<int*>(ws + space.start);
-  a.order = reinterpret_cast<int*>(ws + space.order);
-  a.key = reinterpret_cast<int*>(ws + space.key);
+  a.sorted = reinterpret_cast<int2*>(ws + space.sorted);
   a.part = reinterpret_cast<float*>(ws + space.part);
   const hipStream_t s = as_stream(stream);
-  embed_sort_kernel<<<dim3(static_cast<uint32_t>(ceil_div(vocab, kSortIds))), 64 * kSortWaves, 0, s>>>(a);
+  const dim3 sort(1u << space.shift);
+  if (index64) embed_sort_kernel<true><<<sort, 64 * kSortWaves, 0, s>>>(a);
+  else embed_sort_kernel<false><<<sort, 64 * kSortWaves, 0, s>>>(a);
+  const int64_t tiles = ceil_div(T, kTile);
   if (T > 0) {
-    const dim3 grid(static_cast<uint32_t>(ceil_div(ceil_div(T, kTile) * a.segments, 4)));
+    a.segments = segments_of(dim, dy_dtype);
+    const dim3 grid(static_cast<uint32_t>(ceil_div(tiles * a.segments, 4)));
     if (dy_dtype == FMOE_BF16 && dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_BF16><<<grid, 256, 0, s>>>(a);
     else if (dy_dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_F32><<<grid, 256, 0, s>>>(a);
     else if (dtype == FMOE_BF16) embed_sum_kernel<FMOE_F32, FMOE_BF16><<<grid, 256, 0, s>>>(a);
     else embed_sum_kernel<FMOE_F32, FMOE_F32><<<grid, 256, 0, s>>>(a);
   }
-  const dim3 rest(static_cast<uint32_t>(ceil_div(vocab, kRestIds * kRestWaves) * a.segments));
-  if (dtype == FMOE_BF16) embed_rest_kernel<FMOE_BF16><<<rest, 64 * kRestWaves, 0, s>>>(a);
-  else embed_rest_kernel<FMOE_F32><<<rest, 64 * kRestWaves, 0, s>>>(a);
+  a.segments = segments_of(dim, dtype);
+  // (an id of more than kLongTiles tiles needs as many tokens)
+  const int64_t blocks = ceil_div(space.slots, kRestIds * kRestWaves) * a.segments;
+  const int64_t longs = tiles > kLongTiles ? ceil_div(tiles, kRestWaves) * a.segments : 0;
+  const dim3 rest(static_cast<uint32_t>(blocks + longs));
+  const int b = static_cast<int>(blocks);
+  if (dtype == FMOE_BF16) embed_rest_kernel<FMOE_BF16><<<rest, 64 * kRestWaves, 0, s>>>(a, b);
+  else embed_rest_kernel<FMOE_F32><<<rest, 64 * kRestWaves, 0, s>>>(a, b);
   return launch_status();
 }

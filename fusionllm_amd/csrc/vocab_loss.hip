@@ -49,8 +49,7 @@ struct VlState {
   int* inv;       // [T] row -> packed row, or -1
   int* index;     // [T][top] of packed rows; of equal ones all but the first are kNone
   float* q;       // [T][top] target distribution, equal entries added (distillation)
-  float* entropy; // [T] sum of q ln q over the list as it was (distillation)
-  float* picked;  // [T][top] t of the listed entries
+  float* picked;  // [T][top] t of the listed entries; cross entropy: p - 1 of the target
   float2* stat;   // [T] m, l
   uint16_t* h;    // [planes][Tp][Dp] packed rows
   int64_t Tp, Dp, plane;
@@ -68,7 +67,6 @@ struct VlState {
     inv = reinterpret_cast<int*>(take(T * 4));
     index = reinterpret_cast<int*>(take(T * top * 4));
     q = reinterpret_cast<float*>(take(T * top * 4));
-    entropy = reinterpret_cast<float*>(take(T * 4));
     picked = reinterpret_cast<float*>(take(T * top * 4));
     stat = reinterpret_cast<float2*>(take(T * 8));
     h = reinterpret_cast<uint16_t*>(take(planes * plane * 2));
@@ -80,57 +78,59 @@ struct VlState {
 struct RowsArgs {
   const void *hidden, *index, *teacher;
   int64_t ldh, ignore;
-  int h_dtype, index64, t_dtype;  // t_dtype -1: no teacher
-  int T, D, Dp, V, top, planes;
+  int index64, t_dtype;  // t_dtype -1: no teacher
+  int T, D, Dp, V, top;
   int64_t plane;
   float inv_temp;
-  int *counts, *head, *perm, *inv, *out_index;
-  float *q, *entropy, *loss;  // loss: of rows without entries, where it is [T] (else nullptr)
+  uint32_t* masks;       // rows with entries, 32 per word; nullptr: every workgroup finds them itself
+  int *head, *perm, *inv, *out_index;
+  float* loss;           // zeros in rows without entries, where it is [T] (else nullptr)
   uint16_t* h;
 };
+constexpr int kFewEntries = 16384;  // entries of all rows that a workgroup looks at itself: 16 per thread
 
-// Entry k of row t: kNone, kBad or an index; z: its teacher logit over the temperature.
-__device__ __forceinline__ int vl_entry(const RowsArgs& a, int64_t t, int k, float& z) {
-  const int64_t e = t * a.top + k;
+// Entry e = row * top + k: kNone, kBad or an index; z: its teacher logit over the temperature.
+__device__ __forceinline__ int vl_entry(const RowsArgs& a, int64_t e, float& z) {
   const int64_t id = a.index64 ? static_cast<const int64_t*>(a.index)[e] : static_cast<const int32_t*>(a.index)[e];
   z = 0.0f;
-  if (a.t_dtype >= 0) {
-    const float raw = a.t_dtype == FMOE_BF16 ? bf2f(static_cast<const uint16_t*>(a.teacher)[e])
-                                             : static_cast<const float*>(a.teacher)[e];
-    if (raw == -__builtin_inff()) return kNone;
-    z = raw * a.inv_temp;
-  }
-  if (id == a.ignore) return kNone;
+  float raw = 0.0f;
+  if (a.t_dtype >= 0)
+    raw = a.t_dtype == FMOE_BF16 ? bf2f(static_cast<const uint16_t*>(a.teacher)[e])
+                                 : static_cast<const float*>(a.teacher)[e];
+  z = raw * a.inv_temp;
+  if (id == a.ignore || raw == -__builtin_inff()) return kNone;
   return id < 0 || id >= a.V ? kBad : static_cast<int>(id);
 }
 
-// Bit i: row block0 + i of the workgroup's rows has an entry (256 threads, all get the mask).
-__device__ __forceinline__ uint32_t vl_rows_mask(const RowsArgs& a, int block0, uint32_t* shared_mask) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  if (threadIdx.x == 0) *shared_mask = 0;
+// Sets in LDS the bits of the rows row0 .. row1 - 1 that have an entry (1024 threads).
+__device__ __forceinline__ void vl_mark_rows(const RowsArgs& a, int row0, int row1, uint32_t* bits) {
+  const int words = (row1 - row0 + 31) / 32;
+  for (int i = threadIdx.x; i < words; i += 1024) bits[i] = 0;
   __syncthreads();
-  float z;
-  if (a.top == 1) {
-    if (w == 0) {
-      const bool has = lane < kRowBlock && block0 + lane < a.T && vl_entry(a, block0 + lane, 0, z) != kNone;
-      const uint64_t m = __ballot(has);
-      if (lane == 0) *shared_mask = static_cast<uint32_t>(m);
+  const int64_t e0 = static_cast<int64_t>(row0) * a.top, e1 = static_cast<int64_t>(row1) * a.top;
+  constexpr int U = 8;
+  for (int64_t e = e0 + threadIdx.x; e < e1; e += 1024 * U) {
+    bool has[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float z;
+      const int64_t at = e + 1024 * u;
+      has[u] = vl_entry(a, min(at, e1 - 1), z) != kNone && at < e1;
     }
-  } else {
-    for (int i = w; i < kRowBlock && block0 + i < a.T; i += 4) {
-      bool has = false;
-      for (int k = lane; k < a.top; k += 64) has = has || vl_entry(a, block0 + i, k, z) != kNone;
-      if (__ballot(has) != 0 && lane == 0) atomicOr(shared_mask, 1u << i);
-    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (has[u]) {
+        const int r = static_cast<int>(e - e0 + 1024 * u) / a.top;
+        atomicOr(&bits[r >> 5], 1u << (r & 31));
+      }
   }
   __syncthreads();
-  return *shared_mask;
 }
 
-__global__ __launch_bounds__(256) void vl_count_kernel(const RowsArgs a) {
-  __shared__ uint32_t mask;
-  const uint32_t m = vl_rows_mask(a, blockIdx.x * kRowBlock, &mask);
-  if (threadIdx.x == 0) a.counts[blockIdx.x] = __popc(m);
+__global__ __launch_bounds__(1024) void vl_mark_kernel(const RowsArgs a) {
+  __shared__ uint32_t bits[1];
+  vl_mark_rows(a, blockIdx.x * kRowBlock, min(static_cast<int>(blockIdx.x + 1) * kRowBlock, a.T), bits);
+  if (threadIdx.x == 0) a.masks[blockIdx.x] = bits[0];
 }
 
 // hi, mid and lo of fp32 values (planes = 3), or their bf16 rounding alone.
@@ -165,32 +165,33 @@ __device__ __forceinline__ void vl_copy_row(const void* src, int64_t row, int n,
 }
 
 template <int DT, int PLANES>
-__global__ __launch_bounds__(256) void vl_rows_kernel(const RowsArgs a) {
-  __shared__ uint32_t mask_s;
-  __shared__ int before_s[4];
-  __shared__ float tz[4][FMOE_VOCAB_MAX_TOP];
-  __shared__ int ti[4][FMOE_VOCAB_MAX_TOP];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int block0 = blockIdx.x * kRowBlock;
-  const uint32_t mask = vl_rows_mask(a, block0, &mask_s);
+__global__ __launch_bounds__(1024) void vl_rows_kernel(const RowsArgs a) {
+  __shared__ uint32_t bits[kFewEntries / 32];
+  __shared__ int before_s[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, block = blockIdx.x;
+  const int block0 = block * kRowBlock;
+  if (a.masks == nullptr) vl_mark_rows(a, 0, min(block0 + kRowBlock, a.T), bits);
+  const uint32_t* masks = a.masks ? a.masks : bits;
   int before = 0;
-  for (int i = threadIdx.x; i < static_cast<int>(blockIdx.x); i += 256) before += a.counts[i];
+  for (int i = threadIdx.x; i < block; i += 1024) before += __popc(masks[i]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
   if (lane == 0) before_s[w] = before;
+  const uint32_t mask = block0 < a.T ? masks[block] : 0;
   __syncthreads();
-  const int base = before_s[0] + before_s[1] + before_s[2] + before_s[3];
+  int base = 0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) base += before_s[q];
   const int n = base + __popc(mask);
-  const bool last = blockIdx.x + 1 == gridDim.x;
-  if (last) {  // zeros up to the next multiple of 64 rows
+  if (block + 1 == static_cast<int>(gridDim.x)) {  // zeros up to the next multiple of 64 rows
     if (threadIdx.x == 0) a.head[0] = n;
-    for (int r = n + w; r < pad_rows(n); r += 4)
+    for (int r = n + w; r < pad_rows(n); r += 16)
       for (int c = lane * 8; c < a.Dp; c += 512)
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
           *reinterpret_cast<uint4*>(a.h + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
   }
-  for (int i = w; i < kRowBlock && block0 + i < a.T; i += 4) {
+  for (int i = w; i < kRowBlock && block0 + i < a.T; i += 16) {
     const int64_t t = block0 + i;
     if (!((mask >> i) & 1)) {
       if (lane == 0) {
@@ -203,58 +204,8 @@ __global__ __launch_bounds__(256) void vl_rows_kernel(const RowsArgs a) {
     if (lane == 0) {
       a.inv[t] = r;
       a.perm[r] = static_cast<int>(t);
-    }
-    if (a.t_dtype < 0) {
       float z;
-      if (lane == 0) a.out_index[r] = vl_entry(a, t, 0, z);
-    } else {
-      // softmax over the list; entries of one index are added to the first of them
-      float peak = -__builtin_inff();
-      bool nan = false;
-      for (int k = lane; k < a.top; k += 64) {
-        float z;
-        const int id = vl_entry(a, t, k, z);
-        ti[w][k] = id;
-        tz[w][k] = z;
-        if (id != kNone) peak = fmaxf(peak, z), nan = nan || z != z;
-      }
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) peak = fmaxf(peak, __shfl_xor(peak, off, 64));
-      if (__ballot(nan) != 0) peak = __builtin_nanf("");
-      float sum = 0.0f;
-      for (int k = lane; k < a.top; k += 64) {
-        const float e = ti[w][k] == kNone ? 0.0f : expf(tz[w][k] - peak);
-        sum = sum + e;
-      }
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) sum = sum + __shfl_xor(sum, off, 64);
-      const float log_sum = logf(sum);
-      float ent = 0.0f;
-      for (int k = lane; k < a.top; k += 64) {
-        const float lq = (tz[w][k] - peak) - log_sum;
-        const float q = ti[w][k] == kNone ? 0.0f : expf(lq);
-        if (ti[w][k] != kNone && !(q == 0.0f)) ent = fmaf(q, lq, ent);
-        tz[w][k] = q;
-      }
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) ent = ent + __shfl_xor(ent, off, 64);
-      if (lane == 0) a.entropy[r] = ent;
-      __builtin_amdgcn_wave_barrier();
-      for (int k = lane; k < a.top; k += 64) {
-        const int id = ti[w][k];
-        float q = tz[w][k];
-        bool first = true;
-        if (id >= 0) {
-          q = 0.0f;
-          for (int j = 0; j < a.top; ++j)
-            if (ti[w][j] == id) {
-              first = first && j >= k;
-              q = q + tz[w][j];
-            }
-        }
-        a.out_index[static_cast<int64_t>(r) * a.top + k] = first ? id : kNone;
-        a.q[static_cast<int64_t>(r) * a.top + k] = first ? q : 0.0f;
-      }
+      if (a.t_dtype < 0) a.out_index[r] = vl_entry(a, t, z);
     }
     vl_copy_row<DT, PLANES>(a.hidden, t * a.ldh, a.D, a.Dp, a.h + static_cast<int64_t>(r) * a.Dp, a.plane, lane, 64);
   }
@@ -284,38 +235,32 @@ struct VlGemm {
   const uint16_t *a, *b;
   int64_t a_plane, b_plane;
   int lda, ldb;
-  int passes;           // 1, or 6: products of planes
   const int* head;      // rows with entries
   int cols;             // STATS, GRAD: vocabulary rows of the piece; DH, DW: columns (Dp)
   int vocab;            // DH, DW: vocabulary rows of the piece
   int k;                // STATS, GRAD: K (Dp)
-  int ranges;           // DH: ranges of K
-  float c;
+  int v0;               // STATS, GRAD: the piece's first vocabulary row
+  float c;              // t = c * (H W^T)
+  const int* index;     // cross entropy: the rows' targets (else nullptr)
+  float* picked;        // their t; GRAD: p - 1
   // STATS
   float2* part;         // [2 * column tiles][Tp]
   int64_t Tp;
-  const int* index;     // cross entropy: the target's t is picked on the way (else nullptr)
-  float* picked;
-  int v0;               // the piece's first vocabulary row
   // GRAD
   const float2* stat;
   const float* d_loss;
-  const int* perm;
+  const int* perm;      // (and DH)
   float factor;
-  int reduction, planes;
+  int reduction;
   uint16_t* g;
   int64_t g_plane;
   int ldg;              // a multiple of 256
-  // DH
-  float* sum;           // [ranges][Tp][Dp]
-  int add;              // there is a piece before
-  // DW
-  void* dw;
-  int D, dw_dtype;
-};
-
-struct VlItem {
-  int tm, tn, k0, kn, range;
+  // DH, DW: the result, out [.][D] of out_dtype; DH: in rows perm
+  void* out;
+  int D, out_dtype;
+  float* sum;           // DH: [Tp][Dp], the sum over the pieces before (add) and for those after (more)
+  int add, more;
+  float* split;         // fp32 partial tiles
 };
 
 // Planes of a pass, the smallest products first: (0, 2), (1, 1), (2, 0), (0, 1), (1, 0), (0, 0).
@@ -325,10 +270,224 @@ __device__ __forceinline__ void vl_planes(int passes, int pass, int& pa, int& pb
   pb = (0x046 >> i) & 3;
 }
 
+// Split of DH's and DW's K: with T tiles, the T mod 256 ones of the last, partial round are cut into S ranges
+// of K, which leave fp32 partial tiles that a second launch adds in order.  S gives the fewest steps, a
+// round costing its steps and an epilogue, a partial tile its traffic (256 KB written and read), the second launch
+// its own.  (S ranges of one tile are walked range by range, so that the workgroups of an XCD read the same operand
+// rows at a time.)
+struct VlSplit {
+  int whole, rest, ranges;  // tiles computed whole, tiles split, ranges of each
+};
+constexpr int kSplitSlots = 1024;  // partial tiles, at most
+__host__ __device__ inline VlSplit vl_split(int tiles, int units) {
+  const int rest = tiles % kVlCus;
+  VlSplit best{tiles, 0, 1};
+  if (rest == 0) return best;
+  float least = static_cast<float>(units) + 2.0f;
+  for (int s = 2; s <= units / 8 && s * rest <= kSplitSlots; ++s) {
+    const float rounds = static_cast<float>((s * rest + kVlCus - 1) / kVlCus);
+    const float cost = rounds * (static_cast<float>(units) / static_cast<float>(s) + 2.0f) + 0.055f * static_cast<float>(s * rest) + 4.0f;
+    if (cost < least) least = cost, best = VlSplit{tiles - rest, rest, s};
+  }
+  return best;
+}
+
+struct VlItem {
+  int tm, tn, u0, un, slot;  // tile, K steps (of all passes), partial tile (-1: the tile is whole)
+};
+
+// Tile t: groups of kGroup row tiles, in a group column by column.  The 32 workgroups of an XCD
+// share 8 + 4 operand panels instead of 1 + 32.
+__device__ __forceinline__ void vl_tile(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per = kGroup * tiles_n, g = t / per, rem = t - g * per, rows = min(tiles_m - g * kGroup, kGroup);
+  const int col = rem / rows;
+  tm = __builtin_amdgcn_readfirstlane(g * kGroup + rem - col * rows);
+  tn = __builtin_amdgcn_readfirstlane(col);
+}
+
+// 8 consecutive values of a row of the result; DH of several pieces: with the sum so far, or into it.
 template <int MODE>
+__device__ __forceinline__ void vl_result8(const VlGemm& a, int n, int row, int col, float* v) {
+  if (MODE == VL_DW) {
+    if (row >= a.vocab || col >= a.D) return;
+    const int64_t o = static_cast<int64_t>(row) * a.D + col;
+    if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - col, v);
+    else store_upto8<FMOE_F32>(a.out, o, a.D - col, v);
+  } else {
+    if (row >= n || col >= a.D) return;
+    float* const s = a.sum + static_cast<int64_t>(row) * a.cols + col;
+    if (a.add) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(s), hi = *reinterpret_cast<const f32x4*>(s + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = lo[e] + v[e], v[4 + e] = hi[e] + v[4 + e];
+    }
+    if (a.more) {
+      *reinterpret_cast<f32x4*>(s) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(s + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      return;
+    }
+    const int64_t o = static_cast<int64_t>(a.perm[row]) * a.D + col;
+    if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - col, v);
+    else store_upto8<FMOE_F32>(a.out, o, a.D - col, v);
+  }
+}
+
+// What a row's p - q are multiplied with.
+__device__ __forceinline__ float vl_row_weight(const float* d_loss, const int* perm, int reduction, int n, int row, float factor) {
+  const float up = reduction == FMOE_REDUCE_NONE ? d_loss[perm[row]] : d_loss[0];
+  return (reduction == FMOE_REDUCE_MEAN ? up / static_cast<float>(n) : up) * factor;
+}
+
+// (written out: the compiler puts an instruction for quiet NaNs before each operand of its own maximum; a NaN
+// among the logits reaches the sum of exponentials whatever the maximum is)
+__device__ __forceinline__ float vl_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Epilogue of STATS: maximum and sum of exponentials of each row's 128 columns.  c >= 0 here, so that the
+// maximum is taken of the accumulators; the exponent of an element is one multiply-add.  FULL: all columns
+// are inside the vocabulary (128 v_exp_f32 and 320 other instructions a lane; with the bounds and a
+// product of its own 640).
+template <bool FULL>
+__device__ __forceinline__ void vl_stats_epilogue(const VlGemm& a, f32x4 (&acc)[core::FM][core::FN], float c, int n,
+                                                  int row0, int col0, int piece, int el) {
+  using namespace core;
+  const int er = el & 15, eg = el >> 4;
+  float2 mine = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int row = row0 + 16 * i + er;
+    // columns of this lane inside: 16 j + e < lim (opaque, or the comparisons are kept in registers for all rows)
+    int lim = a.cols - col0 - 4 * eg;
+    asm volatile("" : "+v"(lim));
+    if constexpr (!FULL) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 16 * j + e < lim ? acc[i][j][e] : -__builtin_inff();
+    }
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < FN; ++j) m = vl_max3(vl_max3(m, acc[i][j][0], acc[i][j][1]), acc[i][j][2], acc[i][j][3]);
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    // (columns outside, or c = 0: no infinity may meet it)
+    if constexpr (!FULL) {
+      if (m == -__builtin_inff()) m = 0.0f;
+    }
+    m = m * c;
+    const float peak = m == -__builtin_inff() ? 0.0f : m;  // a sum of zero; NaN stays NaN
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -peak));
+        if constexpr (!FULL) x = 16 * j + e < lim ? x : 0.0f;
+        s = s + x;
+      }
+    s = s + __shfl_xor(s, 16, 64);
+    s = s + __shfl_xor(s, 32, 64);
+    if (eg == i) mine = make_float2(!FULL && s == 0.0f ? -__builtin_inff() : m, s);
+    if (a.index) {  // the target's column, where it is in this block
+      const int rel = row < n ? a.index[row] - (a.v0 + col0) : -1;
+      const bool here = rel >= 0 && rel < WTN && col0 + rel < a.cols;
+      if (__ballot(here) != 0) {
+        float t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t = rel == 16 * j + 4 * eg + e ? acc[i][j][e] : t;
+        if (here && ((rel >> 2) & 3) == eg) a.picked[row] = t * c;
+      }
+    }
+  }
+  const int row = row0 + el;  // lane group eg kept block eg
+  if (row < n) a.part[static_cast<int64_t>(piece) * a.Tp + row] = mine;
+}
+
+// Epilogue of GRAD: G, 16 rows at a time through the wave's LDS into 16-byte stores.  With one plane, 2^(t - m -
+// l) takes one multiply-add (m + l rounded: 2^-24 of some tens in the exponent, far below G's own half step of
+// 2^-8); with three, m is subtracted first.
+template <int PLANES, bool FULL>
+__device__ __forceinline__ void vl_grad_epilogue(const VlGemm& a, f32x4 (&acc)[core::FM][core::FN], uint8_t* ep, int n,
+                                                 int np, int row0, int col0, int el) {
+  using namespace core;
+  const int er = el & 15, eg = el >> 4;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    asm volatile("" ::: "memory");  // (the rows' values of all blocks at once would spill)
+    const int row = row0 + 16 * i + er;
+    float2 ml = make_float2(0.0f, 0.0f);
+    float up = 0.0f;
+    int rel = -1;
+    if (row < n) {
+      ml = a.stat[row];
+      up = vl_row_weight(a.d_loss, a.perm, a.reduction, n, row, a.factor);
+      if (a.index) rel = a.index[row] - (a.v0 + col0);
+    }
+    const float off = PLANES == 1 ? -(ml.x + ml.y) : -ml.x;
+    int lim = row < n ? a.cols - col0 - 4 * eg : 0;  // as above; none in rows that are padding
+    asm volatile("" : "+v"(lim));
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = fmaf(acc[i][j][e], a.c, off);
+        if constexpr (PLANES > 1) x = x - ml.y;
+        x = __builtin_amdgcn_exp2f(x) * up;
+        if constexpr (!FULL) x = 16 * j + e < lim ? x : 0.0f;
+        acc[i][j][e] = x;
+      }
+    const bool here = rel >= 0 && rel < WTN && col0 + rel < a.cols;
+    if (__ballot(here) != 0) {  // the target
+      const float v = here ? a.picked[row] * up : 0.0f;
+      const int at = here ? rel : -1;
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = at == 16 * j + 4 * eg + e ? v : acc[i][j][e];
+    }
+#pragma unroll 1  // (three at once would spill)
+    for (int p = 0; p < PLANES; ++p) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int col = j * 16 + eg * 4;
+        uint2 u;
+        u.x = pack2(acc[i][j][0], acc[i][j][1]);
+        u.y = pack2(acc[i][j][2], acc[i][j][3]);
+        *reinterpret_cast<uint2*>(ep + er * 256 + ((((col >> 3) ^ er)) << 4) + (col & 7) * 2) = u;
+        if constexpr (PLANES > 1) {
+          acc[i][j][0] = acc[i][j][0] - __uint_as_float(u.x << 16);
+          acc[i][j][1] = acc[i][j][1] - __uint_as_float(u.x & 0xffff0000u);
+          acc[i][j][2] = acc[i][j][2] - __uint_as_float(u.y << 16);
+          acc[i][j][3] = acc[i][j][3] - __uint_as_float(u.y & 0xffff0000u);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      // uniform addresses, one offset per lane
+      uint8_t* const base = reinterpret_cast<uint8_t*>(a.g + p * a.g_plane + static_cast<int64_t>(row0 + 16 * i) * a.ldg + col0);
+      const uint32_t voff = static_cast<uint32_t>(eg * a.ldg + er * 8) * 2u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int r = t * 4 + eg;
+        const uint4 v = *reinterpret_cast<const uint4*>(ep + r * 256 + ((er ^ r) << 4));
+        if (FULL || row0 + 16 * i + r < np)
+          *reinterpret_cast<uint4*>(base + static_cast<int64_t>(8 * t) * a.ldg + voff) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+    }
+  }
+}
+
+template <int MODE, int PLANES>
 __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   using namespace core;
-  constexpr bool ATR = MODE == VL_DW, BTR = MODE == VL_DH || MODE == VL_DW;
+  constexpr bool ATR = MODE == VL_DW, BTR = MODE == VL_DH || MODE == VL_DW, SPLIT = MODE == VL_DH || MODE == VL_DW;
+  constexpr int PASSES = PLANES == 1 ? 1 : 6;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -339,31 +498,34 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   const int m_rows = MODE == VL_DW ? a.vocab : np;
   const int tiles_m = (m_rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
   const int nk = MODE == VL_DH ? (a.vocab + BK - 1) / BK : MODE == VL_DW ? np / BK : a.k / BK;
-  const int ranges = MODE == VL_DH ? a.ranges : 1;
-  const int tiles = tiles_m * tiles_n, items = tiles * ranges;
-  // Workgroup b runs on XCD b % 8.  Each XCD takes a contiguous eighth of the items.
-  const int xcd = static_cast<int>(blockIdx.x) % 8, step = static_cast<int>(gridDim.x) / 8;
-  const int first = static_cast<int>(static_cast<int64_t>(items) * xcd / 8) + static_cast<int>(blockIdx.x) / 8;
-  const int end = static_cast<int>(static_cast<int64_t>(items) * (xcd + 1) / 8);
-  const int my_items = (end - first + step - 1) / step;
+  const int units = nk * PASSES, tiles = tiles_m * tiles_n;
+  const VlSplit sp = SPLIT ? vl_split(tiles, units) : VlSplit{tiles, 0, 1};
+  // Workgroup b runs on XCD b % 8.  Each XCD takes a contiguous eighth of the whole tiles, then of the ranges.
+  const int xcd = static_cast<int>(blockIdx.x) % 8, slot = static_cast<int>(blockIdx.x) / 8, step = static_cast<int>(gridDim.x) / 8;
+  auto share = [&](int items, int& first) {
+    const int lo = static_cast<int>(static_cast<int64_t>(items) * xcd / 8), hi = static_cast<int>(static_cast<int64_t>(items) * (xcd + 1) / 8);
+    first = lo + slot;
+    return max(hi - first + step - 1, 0) / step;
+  };
+  int first_whole, first_range = 0;
+  const int my_whole = share(sp.whole, first_whole);
+  const int my_items = my_whole + (SPLIT ? share(sp.rest * sp.ranges, first_range) : 0);
   if (my_items <= 0) return;
 
-  // Items in order: K ranges, then groups of kGroup row tiles, in a group column by column: the 32
-  // workgroups of an XCD share 8 + 4 operand panels instead of 1 + 32.
-  auto locate = [&](int item) __attribute__((always_inline)) {
-    VlItem t;
-    t.range = MODE == VL_DH ? item / tiles : 0;
-    const int q = item - t.range * tiles, per = kGroup * tiles_n;
-    const int g = q / per, rem = q - g * per, rows = min(tiles_m - g * kGroup, kGroup);
-    t.tn = rem / rows;
-    t.tm = g * kGroup + rem - t.tn * rows;
-    t.k0 = static_cast<int>(static_cast<int64_t>(nk) * t.range / ranges);
-    t.kn = static_cast<int>(static_cast<int64_t>(nk) * (t.range + 1) / ranges) - t.k0;
-    t.tm = __builtin_amdgcn_readfirstlane(t.tm);
-    t.tn = __builtin_amdgcn_readfirstlane(t.tn);
-    t.k0 = __builtin_amdgcn_readfirstlane(t.k0);
-    t.kn = __builtin_amdgcn_readfirstlane(t.kn);
-    t.range = __builtin_amdgcn_readfirstlane(t.range);
+  auto locate = [&](int i) __attribute__((always_inline)) {
+    VlItem t{0, 0, 0, units, -1};
+    int tile = first_whole + i * step;
+    if (SPLIT && i >= my_whole) {
+      const int q = first_range + (i - my_whole) * step, range = q / sp.rest;
+      tile = sp.whole + q - range * sp.rest;
+      t.u0 = static_cast<int>(static_cast<int64_t>(units) * range / sp.ranges);
+      t.un = static_cast<int>(static_cast<int64_t>(units) * (range + 1) / sp.ranges) - t.u0;
+      t.slot = q;
+    }
+    vl_tile(tile, tiles_m, tiles_n, t.tm, t.tn);
+    t.u0 = __builtin_amdgcn_readfirstlane(t.u0);
+    t.un = __builtin_amdgcn_readfirstlane(t.un);
+    t.slot = __builtin_amdgcn_readfirstlane(t.slot);
     return t;
   };
 
@@ -371,22 +533,12 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   const uint32_t lds_a = ATR ? sbase + w * 1024 : sbase + (64 * (w >> 2) + 8 * (w & 3)) * RB;
   const uint32_t lds_b = sbase + A_BYTES + w * 1024;
   const int lda = a.lda, ldb = a.ldb;
-  VlItem c_t = locate(first);
-  int c_ti = 0, c_pass = 0, c_k = 0, c_left = 0;
+  int c_ti = 0, c_tm, c_tn, c_u, c_end, c_left = 0, c_run;  // item, its tile, the next call's K step and its last one
   const uint8_t *c_a = nullptr, *c_b = nullptr;
   int64_t astep = ATR ? static_cast<int64_t>(2 * BK) * lda : RB, bstep = BTR ? static_cast<int64_t>(2 * BK) * ldb : RB;
   uint32_t a_off[4], b_off[4];
-  // pointers and offsets of step c_k of pass c_pass, and the steps until the next call
-  auto place = [&]() __attribute__((always_inline)) {
-    int pa, pb;
-    vl_planes(a.passes, c_pass, pa, pb);
-    const int k = (c_t.k0 + c_k) * BK;
-    const uint16_t* p = a.a + pa * a.a_plane + (ATR ? static_cast<int64_t>(k) * lda : static_cast<int64_t>(c_t.tm) * BM * lda + k);
-    const uint16_t* q = a.b + pb * a.b_plane + (BTR ? static_cast<int64_t>(k) * ldb : static_cast<int64_t>(c_t.tn) * BN * ldb + k);
-    c_a = reinterpret_cast<const uint8_t*>(p);
-    c_b = reinterpret_cast<const uint8_t*>(q);
-    c_left = c_t.kn - c_k;
-    if (MODE == VL_DH && (a.vocab & (BK - 1)) && c_t.k0 + c_t.kn == nk && c_left > 1) --c_left;  // the last step has clamped rows
+  // this lane's offsets from c_a and c_b; k: the step's first K
+  auto form_offsets = [&](int k) __attribute__((always_inline)) {
     // the lane as an opaque value: what follows is formed here, not kept through the main loop
     int l = lane;
     asm volatile("" : "+v"(l));
@@ -395,13 +547,13 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     const int cb = ((((l & 15) >> 1) ^ wsw(krow)) << 1) | (l & 1);
     if constexpr (ATR) {
       // unit u: rows (of C) 32 u .. + 31 of every wave's 64
-      const int m0 = c_t.tm * BM;
+      const int m0 = c_tm * BM;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         a_off[q] = static_cast<uint32_t>((32 * (q & 1) + krow) * lda +
                                          min(m0 + 64 * (cb >> 2) + 32 * (q >> 1) + 8 * (cb & 3), lda - 8)) * 2u;
     } else {
-      const int last_m = min(m_rows - c_t.tm * BM, BM) - 1;
+      const int last_m = min(m_rows - c_tm * BM, BM) - 1;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = min(64 * (w >> 2) + 8 * (w & 3) + (l >> 3) + 128 * (q & 1) + 32 * (q >> 1), last_m);
@@ -409,13 +561,13 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       }
     }
     if constexpr (BTR) {
-      const int n0 = c_t.tn * BN, last_k = MODE == VL_DH ? a.vocab - 1 - k : BK;
+      const int n0 = c_tn * BN, last_k = MODE == VL_DH ? a.vocab - 1 - k : BK;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         b_off[q] = static_cast<uint32_t>(min(32 * (q & 1) + krow, last_k) * ldb +
                                          min(n0 + 128 * (cb >> 3) + 8 * (cb & 7) + 64 * (q >> 1), a.cols - 8)) * 2u;
     } else {
-      const int last_n = min(a.cols - c_t.tn * BN, BN) - 1;
+      const int last_n = min(a.cols - c_tn * BN, BN) - 1;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = min(128 * (q & 1) + 64 * (q >> 1) + 8 * w + (l >> 3), last_n);
@@ -423,28 +575,46 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       }
     }
   };
+  // pointers and offsets of K step c_u of the item, and the steps until the next call
+  auto place = [&]() __attribute__((always_inline)) {
+    int pa = 0, pb = 0, ku = c_u;
+    if constexpr (PASSES > 1) {
+      const int pass = c_u / nk;
+      ku = c_u - pass * nk;
+      vl_planes(PASSES, pass, pa, pb);
+    }
+    const int k = ku * BK;
+    const uint16_t* p = a.a + pa * a.a_plane + (ATR ? static_cast<int64_t>(k) * lda : static_cast<int64_t>(c_tm) * BM * lda + k);
+    const uint16_t* q = a.b + pb * a.b_plane + (BTR ? static_cast<int64_t>(k) * ldb : static_cast<int64_t>(c_tn) * BN * ldb + k);
+    c_a = reinterpret_cast<const uint8_t*>(p);
+    c_b = reinterpret_cast<const uint8_t*>(q);
+    c_run = min(c_end - c_u, nk - ku);
+    // the last step of a vocabulary that is no multiple of 64 has clamped rows of its own
+    if (MODE == VL_DH && (a.vocab & (BK - 1)) && ku + c_run == nk && c_run > 1) --c_run;
+    c_left = c_run;
+    form_offsets(k);
+  };
+  auto take = [&](int i) __attribute__((always_inline)) {
+    const VlItem t = locate(i);
+    c_tm = t.tm, c_tn = t.tn, c_u = t.u0, c_end = t.u0 + t.un;
+  };
+  take(0);
   place();
-  int c_run = c_left;
   // A stage's units are issued in the order A0, B0, B1, A1; A1 moves the cursor on.  Past the last
   // step the last stage is copied again (into slots that are free and not read any more).
   auto advance = [&]() __attribute__((always_inline)) {
-    c_k += c_run;
-    if (c_k == c_t.kn) {
-      c_k = 0;
-      if (++c_pass == a.passes) {
-        c_pass = 0;
-        if (++c_ti == my_items) {
-          c_a -= astep;
-          c_b -= bstep;
-          astep = bstep = 0;
-          c_left = INT32_MAX;
-          return;
-        }
-        c_t = locate(first + c_ti * step);
+    c_u += c_run;
+    if (c_u == c_end) {
+      if (++c_ti == my_items) {
+        c_a -= astep;
+        c_b -= bstep;
+        astep = bstep = 0;
+        c_left = INT32_MAX;
+        return;
       }
+      take(c_ti);
     }
     place();
-    c_run = c_left;
   };
   auto issue_a = [&](int it, int u) __attribute__((always_inline)) {
     const uint32_t st = lds_a + (it & 1) * STAGE;
@@ -506,9 +676,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   uint8_t* ep = smem + 2 * STAGE + w * EPI;  // this wave's staging (4 KB)
-  int e_ti = 0;
-  VlItem e_t = locate(first);
-  int e_left = e_t.kn * a.passes;
+  int e_ti = 0, e_left = locate(0).un;
   for (int it = 0;; ++it) {
     // keep the per-step fragment addresses from being hoisted out of the loop
     asm volatile("" : "+v"(xa), "+v"(xb));
@@ -547,116 +715,40 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3\n" ::: "memory");  // MFMA results -> VALU reads
     int el = lane;
     asm volatile("" : "+v"(el));  // the address arithmetic below stays out of the main loop
-    const int row0 = e_t.tm * BM + wm * WTM, col0 = e_t.tn * BN + wn * WTN;
+    const VlItem t = locate(e_ti);
+    const int row0 = t.tm * BM + wm * WTM, col0 = t.tn * BN + wn * WTN;
     const int er = el & 15, eg = el >> 4;  // acc[i][j]: row 16 i + er, columns 16 j + 4 eg + 0..3
 
     if constexpr (MODE == VL_STATS) {
-      float2 mine = make_float2(0.0f, 0.0f);
+      float c = a.c;
+      if (c < 0.0f) {
+        c = -c;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int row = row0 + 16 * i + er;
-        float m = -__builtin_inff();
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float t = col0 + 16 * j + 4 * eg + e < a.cols ? acc[i][j][e] * a.c : -__builtin_inff();
-            acc[i][j][e] = t;
-            m = fmaxf(m, t);
-          }
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float peak = m == -__builtin_inff() ? 0.0f : m;  // (no columns: a sum of zero; NaN stays NaN)
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s = s + __builtin_amdgcn_exp2f(acc[i][j][e] - peak);
-        s = s + __shfl_xor(s, 16, 64);
-        s = s + __shfl_xor(s, 32, 64);
-        if (eg == i) mine = make_float2(m, s);
-        if (a.index) {  // the target's column, where it is in this block
-          const int rel = row < n ? a.index[row] - (a.v0 + col0) : -1;
-          const bool here = rel >= 0 && rel < WTN && col0 + rel < a.cols;
-          if (__ballot(here) != 0) {
-            float t = 0.0f;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t = rel == 16 * j + 4 * eg + e ? acc[i][j][e] : t;
-            if (here && ((rel >> 2) & 3) == eg) a.picked[row] = t;
-          }
-        }
+          for (int j = 0; j < FN; ++j) acc[i][j] = -acc[i][j];
       }
-      const int row = row0 + el;  // lane group eg kept block eg
-      if (row < n) a.part[((a.v0 / BN + e_t.tn) * WN + wn) * a.Tp + row] = mine;
+      const int piece = (a.v0 / BN + t.tn) * WN + wn;
+      if (col0 + WTN <= a.cols) vl_stats_epilogue<true>(a, acc, c, n, row0, col0, piece, el);
+      else vl_stats_epilogue<false>(a, acc, c, n, row0, col0, piece, el);
     } else if constexpr (MODE == VL_GRAD) {
+      if (row0 + WTM <= n && col0 + WTN <= a.cols) vl_grad_epilogue<PLANES, true>(a, acc, ep, n, np, row0, col0, el);
+      else vl_grad_epilogue<PLANES, false>(a, acc, ep, n, np, row0, col0, el);
+    } else if (t.slot >= 0) {
+      // a range's partial tile, as it lies in the accumulators; 16-row slices without valid rows left out
+      float* part = a.split + static_cast<int64_t>(t.slot) * (BM * BN);
+      const int valid = (MODE == VL_DW ? a.vocab : n) - t.tm * BM;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int row = row0 + 16 * i + er;
-        float2 ml = make_float2(0.0f, 0.0f);
-        float up = 0.0f;
-        if (row < n) {
-          ml = a.stat[row];
-          up = a.reduction == FMOE_REDUCE_NONE ? a.d_loss[a.perm[row]] : a.d_loss[0];
-          if (a.reduction == FMOE_REDUCE_MEAN) up = up / static_cast<float>(n);
-          up = up * a.factor;
-        }
+      for (int i = 0; i < FM; ++i)
+        if (wm * WTM + 16 * i < valid)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f((acc[i][j][e] * a.c - ml.x) - ml.y);
-            acc[i][j][e] = row < n && col0 + 16 * j + 4 * eg + e < a.cols ? p * up : 0.0f;
-          }
-        for (int p = 0; p < a.planes; ++p) {
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            const int col = j * 16 + eg * 4;
-            const uint32_t off = er * 256 + ((((col >> 3) ^ er)) << 4) + (col & 7) * 2;
-            uint2 u;
-            u.x = pack2(acc[i][j][0], acc[i][j][1]);
-            u.y = pack2(acc[i][j][2], acc[i][j][3]);
-            *reinterpret_cast<uint2*>(ep + off) = u;
-            acc[i][j][0] = acc[i][j][0] - __uint_as_float(u.x << 16);
-            acc[i][j][1] = acc[i][j][1] - __uint_as_float(u.x & 0xffff0000u);
-            acc[i][j][2] = acc[i][j][2] - __uint_as_float(u.y << 16);
-            acc[i][j][3] = acc[i][j][3] - __uint_as_float(u.y & 0xffff0000u);
-          }
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int r = t * 4 + eg, c = er, grow = row0 + 16 * i + r;
-            const uint4 v = *reinterpret_cast<const uint4*>(ep + r * 256 + ((c ^ r) << 4));
-            if (grow < np) *reinterpret_cast<uint4*>(a.g + p * a.g_plane + static_cast<int64_t>(grow) * a.ldg + col0 + c * 8) = v;
-          }
-          __builtin_amdgcn_wave_barrier();
-        }
-      }
-    } else if constexpr (MODE == VL_DH) {
-      float* out = a.sum + static_cast<int64_t>(e_t.range) * a.Tp * a.cols;
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int row = row0 + 16 * i + er;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int col = col0 + 16 * j + 4 * eg;
-          if (row < n && col < a.cols) {
-            f32x4* p = reinterpret_cast<f32x4*>(out + static_cast<int64_t>(row) * a.cols + col);
-            f32x4 v = acc[i][j];
-            if (a.add) {
-              const f32x4 o = *p;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = o[e] + v[e];
-            }
-            *p = v;
-          }
-        }
-      }
+          for (int j = 0; j < FN; ++j)
+            *reinterpret_cast<f32x4*>(part + (wm * WTM + 16 * i + er) * BN + wn * WTN + 16 * j + 4 * eg) = acc[i][j];
     } else {
+      // 16 rows x 64 columns of fp32 at a time through LDS (chunk c of row r at slot c ^ r), 8 consecutive values
+      // of a row per lane
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        // 16 rows x 64 columns of fp32 at a time; chunk c of row r at slot c ^ r
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int jh = 0; jh < FN / 4; ++jh) {
 #pragma unroll
@@ -668,17 +760,11 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
             const int r = 8 * p + (el >> 3), c = (el & 7) * 8;
             const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + r * 256 + (((c >> 2) ^ r) << 4));
             const f32x4 hi = *reinterpret_cast<const f32x4*>(ep + r * 256 + ((((c >> 2) + 1) ^ r) << 4));
-            const int row = row0 + 16 * i + r, col = col0 + 64 * jh + c;
-            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (row < a.vocab && col < a.D) {
-              const int64_t o = static_cast<int64_t>(row) * a.D + col;
-              if (a.dw_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.dw, o, a.D - col, v);
-              else store_upto8<FMOE_F32>(a.dw, o, a.D - col, v);
-            }
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            vl_result8<MODE>(a, n, row0 + 16 * i + r, col0 + 64 * jh + c, v);
           }
           __builtin_amdgcn_wave_barrier();
         }
-      }
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -686,14 +772,76 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     asm volatile("s_nop 1" ::: "memory");  // VALU writes -> MFMA reads of the accumulators
     if (++e_ti == my_items) break;
-    e_t = locate(first + e_ti * step);
-    e_left = e_t.kn * a.passes;
+    e_left = locate(e_ti).un;
+    if constexpr (MODE == VL_GRAD) {
+      // formed again: kept across the epilogue they made it spill
+      form_offsets(0);
+      xa = frag_base(wm * WTM, el);
+      xb = A_BYTES + frag_base(wn * WTN, el);
+    }
     // the next tile's first fragments
     read_first(sbase + ((it + 1) & 1) * STAGE);
     if (late) barrier();
   }
   // the copies past the end have landed before the workgroup's LDS is given back
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// The split tiles: their ranges' partial tiles added in order.  A workgroup adds 16 rows of a tile.  DH's last
+// piece: and zeros in the rows of the result without entries, 64 rows a workgroup behind those.
+template <int MODE, int PLANES>
+__global__ __launch_bounds__(256) void vl_split_kernel(const VlGemm a, const int* inv, int T, int blocks) {
+  using namespace core;
+  const int n = a.head[0];
+  if (MODE == VL_DH && static_cast<int>(blockIdx.x) >= blocks) {
+    const int t0 = (blockIdx.x - blocks) * 64;
+    float zero[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) zero[e] = 0.0f;
+    for (int i = threadIdx.x >> 6; i < 64 && t0 + i < T; i += 4) {
+      if (inv[t0 + i] >= 0) continue;
+      for (int c = (threadIdx.x & 63) * 8; c < a.D; c += 512) {
+        const int64_t o = static_cast<int64_t>(t0 + i) * a.D + c;
+        if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - c, zero);
+        else store_upto8<FMOE_F32>(a.out, o, a.D - c, zero);
+      }
+    }
+    return;
+  }
+  const int np = pad_rows(n);
+  const int m_rows = MODE == VL_DW ? a.vocab : np;
+  const int tiles_m = (m_rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
+  const int nk = MODE == VL_DH ? (a.vocab + BK - 1) / BK : np / BK;
+  const VlSplit sp = vl_split(tiles_m * tiles_n, nk * (PLANES == 1 ? 1 : 6));
+  const int r = blockIdx.x / 16, rows16 = (blockIdx.x % 16) * 16;
+  if (r >= sp.rest) return;
+  int tm, tn;
+  vl_tile(sp.whole + r, tiles_m, tiles_n, tm, tn);
+  if (tm * BM + rows16 >= (MODE == VL_DW ? a.vocab : n)) return;
+  constexpr int U = 8;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = rows16 + half * 8 + (threadIdx.x >> 5), col = (threadIdx.x & 31) * 8;
+    const float* src = a.split + static_cast<int64_t>(r) * (BM * BN) + row * BN + col;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    for (int s0 = 0; s0 < sp.ranges; s0 += U) {
+      f32x4 u[U][2];
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        const float* p = src + static_cast<int64_t>(min(s0 + s, sp.ranges - 1)) * sp.rest * (BM * BN);
+        u[s][0] = *reinterpret_cast<const f32x4*>(p);
+        u[s][1] = *reinterpret_cast<const f32x4*>(p + 4);
+      }
+#pragma unroll
+      for (int s = 0; s < U; ++s)
+        if (s0 + s < sp.ranges)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = v[e] + u[s][0][e], v[4 + e] = v[4 + e] + u[s][1][e];
+    }
+    vl_result8<MODE>(a, n, tm * BM + row, tn * BN + col, v);
+  }
 }
 
 // ---- the rows' statistics and losses -------------------------------------------------------------
@@ -708,13 +856,15 @@ struct LossArgs {
   float* row_loss;    // of packed rows (reductions), or
   float* loss;        // of rows
   // distillation
-  const float *q, *entropy;
   const uint16_t* h;
   int64_t h_plane;
   const void* weight;
   int64_t ldw;
-  int top, D, Dp, w_dtype, planes;
   float c, factor;    // factor: temperature^2
+  int top, planes;    // top 0: cross entropy
+  int *out_index;     // distillation: of the packed rows
+  float* out_q;
+  RowsArgs rows;
 };
 
 __device__ __forceinline__ void vl_store_loss(const LossArgs& a, int row, float v) {
@@ -761,27 +911,49 @@ __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
   for (int q = 1; q < 16; ++q) vl_join(m, s, red[q][lane].x, red[q][lane].y);
   float l = log2f(s);
   if (a.top == 0) {  // cross entropy
-    const int id = a.index[row];
-    if (id == kBad) l = __builtin_nanf("");
-    else vl_store_loss(a, row, ((m - a.picked[row]) + l) * kLn2);
-    if (id == kBad) vl_store_loss(a, row, l);
+    if (a.index[row] == kBad) {
+      l = __builtin_nanf("");
+      vl_store_loss(a, row, l);
+    } else {
+      const float loss = ((m - a.picked[row]) + l) * kLn2;
+      vl_store_loss(a, row, loss);
+      a.picked[row] = expm1f(-loss);  // p - 1 (exact to its own size where p is near 1), for the backward
+    }
   }
   a.stat[row] = make_float2(m, l);
 }
 
-// Distillation: t of a row's listed entries (a dot product of length D each, in fp32), and its loss.
+// Distillation, a workgroup per packed row: the teacher's softmax over its list, t of the listed entries (a dot
+// product of length D each, in fp32, four entries of a wave at a time) and the loss.
+__device__ __forceinline__ float vl_block_max(float v, float* red) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+__device__ __forceinline__ float vl_block_sum(float v, float* red) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = v + __shfl_xor(v, off, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
   extern __shared__ float h[];
-  __shared__ float red[4];
-  __shared__ int bad_s;
+  __shared__ float red[4], tq[FMOE_VOCAB_MAX_TOP];
+  __shared__ int ti[FMOE_VOCAB_MAX_TOP];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x;
   if (row >= a.head[0]) return;
-  if (threadIdx.x == 0) bad_s = 0;
+  const int D = a.rows.D, Dp = a.rows.Dp, top = a.top;
   const bool round = DT == FMOE_F32 && a.planes == 1;
-  for (int c = threadIdx.x * 8; c < a.Dp; c += 2048) {
+  for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
     float v[8];
-    const uint16_t* p = a.h + static_cast<int64_t>(row) * a.Dp + c;
+    const uint16_t* p = a.h + static_cast<int64_t>(row) * Dp + c;
     unpack8(*reinterpret_cast<const uint4*>(p), v);
     for (int q = 1; q < a.planes; ++q) {
       float u[8];
@@ -792,36 +964,101 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[c + e] = v[e];
   }
+  // the list: thread i has entries i, i + 256, ...
+  constexpr int E = FMOE_VOCAB_MAX_TOP / 256;
+  const int64_t list = static_cast<int64_t>(a.perm[row]) * top, out = static_cast<int64_t>(row) * top;
+  float z[E], peak = -__builtin_inff(), any_nan = 0.0f, bad = 0.0f;
+  int id[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int k = threadIdx.x + 256 * i;
+    id[i] = kNone;
+    z[i] = 0.0f;
+    if (k < top) id[i] = vl_entry(a.rows, list + k, z[i]);
+    if (id[i] != kNone) peak = fmaxf(peak, z[i]), any_nan = z[i] != z[i] ? 1.0f : any_nan;
+    if (id[i] == kBad) bad = 1.0f;
+  }
+  peak = vl_block_max(peak, red);
+  if (vl_block_max(any_nan, red) != 0.0f) peak = __builtin_nanf("");
+  const bool row_bad = vl_block_max(bad, red) != 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) sum = id[i] == kNone ? sum : sum + expf(z[i] - peak);
+  const float log_sum = logf(vl_block_sum(sum, red));
+  float ent = 0.0f;  // sum of q ln q
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const float lq = (z[i] - peak) - log_sum, q = id[i] == kNone ? 0.0f : expf(lq);
+    if (!(q == 0.0f)) ent = fmaf(q, lq, ent);
+    z[i] = q;
+    const int k = threadIdx.x + 256 * i;
+    if (k < top) tq[k] = q, ti[k] = id[i];
+  }
+  ent = vl_block_sum(ent, red);
+  // entries of one index are added to the first of them
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int k = threadIdx.x + 256 * i;
+    if (id[i] < 0) continue;
+    float q = 0.0f;
+    bool first = true;
+    for (int j = 0; j < top; ++j)
+      if (ti[j] == id[i]) first = first && j >= k, q = q + tq[j];
+    id[i] = first ? id[i] : kNone;
+    z[i] = first ? q : 0.0f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int k = threadIdx.x + 256 * i;
+    if (k < top) {
+      tq[k] = z[i], ti[k] = id[i];
+      a.out_index[out + k] = id[i];
+      a.out_q[out + k] = z[i];
+    }
+  }
   __syncthreads();
   const float2 ml = a.stat[row];
   float cross = 0.0f;
-  for (int k = w; k < a.top; k += 4) {
-    const int id = __builtin_amdgcn_readfirstlane(a.index[static_cast<int64_t>(row) * a.top + k]);
-    if (id < 0) {
-      if (id == kBad && lane == 0) bad_s = 1;
-      continue;
+  constexpr int U = 4;
+  for (int k0 = w * U; k0 < top; k0 += 4 * U) {
+    float acc[U][4];
+    int64_t at[U];
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = __builtin_amdgcn_readfirstlane(ti[min(k0 + u, top - 1)]);
+      on[u] = k0 + u < top && v >= 0;
+      at[u] = static_cast<int64_t>(max(v, 0)) * a.ldw;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[u][e] = 0.0f;
     }
-    float acc[8];
+    for (int c = lane * 8; c < D; c += 512) {
+      float hv[8], v[U][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    for (int c = lane * 8; c < a.D; c += 512) {
-      float v[8];
-      load_upto8<DT>(a.weight, static_cast<int64_t>(id) * a.ldw + c, a.D - c, v);
+      for (int u = 0; u < U; ++u) load_upto8<DT>(a.weight, at[u] + c, on[u] ? D - c : 0, v[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(round ? bf_round(v[e]) : v[e], h[c + e], acc[e]);
+      for (int e = 0; e < 8; ++e) hv[e] = h[c + e];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[u][e & 3] = fmaf(round ? bf_round(v[u][e]) : v[u][e], hv[e], acc[u][e & 3]);
     }
-    float s = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) s = s + __shfl_xor(s, off, 64);
-    const float t = s * a.c, q = a.q[static_cast<int64_t>(row) * a.top + k];
-    if (lane == 0) a.picked[static_cast<int64_t>(row) * a.top + k] = t;
-    if (!(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
+    for (int u = 0; u < U; ++u) {
+      float s = (acc[u][0] + acc[u][1]) + (acc[u][2] + acc[u][3]);
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) s = s + __shfl_xor(s, off, 64);
+      if (!on[u]) continue;
+      const float t = s * a.c, q = tq[k0 + u];
+      if (lane == 0) a.picked[out + k0 + u] = t;
+      if (!(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
+    }
   }
-  if (lane == 0) red[w] = cross;
-  __syncthreads();
+  cross = vl_block_sum(lane == 0 ? cross : 0.0f, red);
   if (threadIdx.x == 0) {
-    float v = fmaf((red[0] + red[1]) + (red[2] + red[3]), kLn2, a.entropy[row]) * a.factor;
-    if (bad_s) {
+    float v = fmaf(cross, kLn2, ent) * a.factor;
+    if (row_bad) {
       v = __builtin_nanf("");
       a.stat[row] = make_float2(ml.x, v);
     }
@@ -847,36 +1084,30 @@ __global__ __launch_bounds__(1024) void vl_sum_kernel(const int* head, const flo
   }
 }
 
-// ---- backward: the listed entries of G, and dH ------------------------------------------------------
+// ---- backward of distillation: the listed entries of G -----------------------------------------------
 
 struct FixArgs {
   const int *head, *perm, *index;
   const float *q, *picked;
   const float2* stat;
   const float* d_loss;
-  int top, distill, v0, v1, reduction, planes, ldg;
-  int64_t rows_cap;
+  int top, v0, v1, reduction, planes, ldg;
   float factor;
   uint16_t* g;
   int64_t g_plane;
 };
 
-// G at the entries that lie in this piece of the vocabulary: factor * (p - q) in fp32, rounded once.
+// G at the entries that lie in this piece of the vocabulary: the row's weight times p - q in fp32, rounded once.
 __global__ __launch_bounds__(256) void vl_fix_kernel(const FixArgs a) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int n = a.head[0];
-  const int64_t row = i / a.top;
+  const int n = a.head[0], row = static_cast<int>(i / a.top);
   if (row >= n) return;
   const int id = a.index[i];
   if (id < a.v0 || id >= a.v1) return;
   const float2 ml = a.stat[row];
-  const float lp = (a.picked[i] - ml.x) - ml.y;  // log2 p
-  float up = a.reduction == FMOE_REDUCE_NONE ? a.d_loss[a.perm[row]] : a.d_loss[0];
-  if (a.reduction == FMOE_REDUCE_MEAN) up = up / static_cast<float>(n);
-  up = up * a.factor;
-  // (p - 1 where p is near 1: from the logarithm)
-  float v = (a.distill ? __builtin_amdgcn_exp2f(lp) - a.q[i] : expm1f(lp * kLn2)) * up;
-  uint16_t* p = a.g + row * a.ldg + (id - a.v0);
+  float v = (__builtin_amdgcn_exp2f((a.picked[i] - ml.x) - ml.y) - a.q[i]) *
+            vl_row_weight(a.d_loss, a.perm, a.reduction, n, row, a.factor);
+  uint16_t* p = a.g + static_cast<int64_t>(row) * a.ldg + (id - a.v0);
   for (int k = 0; k < a.planes; ++k) {
     const uint16_t b = f2bf(v);
     p[k * a.g_plane] = b;
@@ -884,75 +1115,24 @@ __global__ __launch_bounds__(256) void vl_fix_kernel(const FixArgs a) {
   }
 }
 
-// dH of a row: its partial sums in order; zeros in rows that were not packed.
-template <int DT>
-__global__ __launch_bounds__(256) void vl_dh_kernel(const int* inv, const float* sum, int64_t stride, int ranges, int64_t T,
-                                                    int D, int Dp, void* out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (t >= T) return;
-  const int r = __builtin_amdgcn_readfirstlane(inv[t]);
-  for (int c = lane * 8; c < D; c += 512) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (r >= 0) {
-      const float* p = sum + static_cast<int64_t>(r) * Dp + c;
-      constexpr int U = 4;
-      for (int s0 = 0; s0 < ranges; s0 += U) {
-        f32x4 u[U][2];
-#pragma unroll
-        for (int s = 0; s < U; ++s) {
-          const f32x4* q = reinterpret_cast<const f32x4*>(p + min(s0 + s, ranges - 1) * stride);
-          u[s][0] = q[0], u[s][1] = q[1];
-        }
-#pragma unroll
-        for (int s = 0; s < U; ++s)
-          if (s0 + s < ranges)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = v[e] + u[s][0][e], v[4 + e] = v[4 + e] + u[s][1][e];
-      }
-    }
-    store_upto8<DT>(out, t * D + c, D - c, v);
-  }
-}
-
 // ---- host ------------------------------------------------------------------------------------------
 
-// Pieces of the vocabulary and ranges of dH's K.  The pieces' G is bounded (kPieceBytes); within that, the
-// number of pieces, and of ranges, whose tiles fill the CUs' rounds best: a launch's time is its rounds of
-// tiles, each K steps and an epilogue long.
-constexpr int64_t kPieceBytes = int64_t(1) << 29;
+// Vocabulary rows of a piece of the backward, a multiple of 256: as many as G's bound (kPieceBytes) allows, in
+// pieces of one size.
+constexpr int64_t kPieceBytes = int64_t(1) << 30;
 constexpr int64_t kPackBytes = int64_t(1) << 28;
-constexpr int64_t kSumBytes = int64_t(1) << 30;
 
-struct VlPlan {
-  int64_t piece;  // vocabulary rows of a piece, a multiple of 256 (the last one has fewer)
-  int ranges;
-};
-
-VlPlan vl_plan(int64_t T, int64_t D, int64_t V, int planes) {
-  const int64_t mt = std::max<int64_t>(ceil_div(T, 256), 1), dt = ceil_div(D, 256), vt = ceil_div(V, 256);
-  const int64_t Tp = std::max<int64_t>(pad64(T), 64), Dp = pad64(D);
-  const int passes = planes == 3 ? 6 : 1;
-  // us: a K step of a full chip, a tile's epilogue, a launch
-  const double step = 1.9 * passes, tile = 4.0, launch = 6.0;
+int64_t vl_bwd_piece(int64_t T, int64_t V, int planes) {
+  const int64_t Tp = std::max<int64_t>(pad64(T), 64), vt = ceil_div(V, 256);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>({vt, kPieceBytes / (Tp * 512 * planes), 4096}));
-  const int64_t fewest = ceil_div(vt, most);
-  auto rounds = [](int64_t items) { return static_cast<double>(ceil_div(items, kVlCus)); };
-  VlPlan best{};
-  double best_time = 0.0;
-  for (int64_t pieces = fewest; pieces <= fewest + 12 && pieces <= vt; ++pieces) {
-    const int64_t pt = ceil_div(vt, pieces);
-    for (int s = 1; s <= 64; ++s) {
-      if (s > 1 && (pt * 4 < s * 8 || s * Tp * Dp * 4 > kSumBytes)) break;
-      const double add = static_cast<double>(s) * Tp * Dp * 8.0 / 4e6;  // the partial sums' traffic, us
-      const double time = ceil_div(vt, pt) * (rounds(mt * pt) * (Dp / 64 * step + tile) + rounds(pt * dt) * (Tp / 64 * step + tile) +
-                                    rounds(mt * dt * s) * (4.0 * pt / s * step + tile) + add + 3 * launch);
-      if (best.piece == 0 || time < best_time) best = {pt * 256, s}, best_time = time;
-    }
-  }
-  return best;
+  return ceil_div(vt, ceil_div(vt, most)) * 256;
+}
+
+// Partial tiles of a product of at most so many tiles: the rows that turn out to have entries may be fewer.
+int64_t vl_split_slots(int64_t tiles, int64_t units) {
+  if (units < 16) return 0;
+  const int64_t rest = std::min<int64_t>(tiles, kVlCus - 1);
+  return std::min<int64_t>(kSplitSlots, rest * (units / 8));
 }
 
 // Vocabulary rows of a piece of the forward: all of them, or as many as a packed copy may have.
@@ -962,7 +1142,7 @@ int64_t vl_fwd_piece(int64_t D, int64_t V, int planes, bool packs) {
 }
 
 struct VlFwdSpace {
-  size_t counts, part, row_loss, pack, bytes = 0;
+  size_t masks, part, row_loss, pack, bytes = 0;
   VlFwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
@@ -970,7 +1150,7 @@ struct VlFwdSpace {
       return at;
     };
     const int64_t Tp = std::max<int64_t>(pad64(T), 64);
-    counts = take(ceil_div(T, kRowBlock) * 4);
+    masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
     pack = take(packs ? vl_fwd_piece(D, V, planes, true) * pad64(D) * 2 * planes : 0);
@@ -978,18 +1158,21 @@ struct VlFwdSpace {
 };
 
 struct VlBwdSpace {
-  VlPlan plan;
-  size_t g, sum, pack, bytes = 0;
-  VlBwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) : plan(vl_plan(T, D, V, planes)) {
+  int64_t piece;
+  size_t g, sum, split, pack, bytes = 0;
+  VlBwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) : piece(vl_bwd_piece(T, V, planes)) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += (n + 255) & ~size_t(255);
       return at;
     };
-    const int64_t Tp = std::max<int64_t>(pad64(T), 64), Dp = pad64(D);
-    g = take(Tp * plan.piece * 2 * planes);
-    sum = take(plan.ranges * Tp * Dp * 4);
-    pack = take(packs ? std::min(pad64(V), plan.piece) * Dp * 2 * planes : 0);
+    const int64_t Tp = std::max<int64_t>(pad64(T), 64), Dp = pad64(D), dt = ceil_div(Dp, 256);
+    const int64_t passes = planes == 3 ? 6 : 1;
+    g = take(Tp * piece * 2 * planes);
+    sum = take(V > piece ? Tp * Dp * 4 : 0);
+    split = take(std::max(vl_split_slots(ceil_div(Tp, 256) * dt, ceil_div(std::min(V, piece), 64) * passes),
+                          vl_split_slots(ceil_div(std::min(V, piece), 256) * dt, Tp / 64 * passes)) * (core::BM * core::BN * 4));
+    pack = take(packs ? std::min(pad64(V), piece) * Dp * 2 * planes : 0);
   }
 };
 
@@ -1075,23 +1258,23 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
 
   RowsArgs r{};
   r.hidden = hidden, r.index = index, r.teacher = teacher, r.ldh = ldh, r.ignore = ignore_index;
-  r.h_dtype = h_dtype, r.index64 = index64, r.t_dtype = distill ? t_dtype : -1;
+  r.index64 = index64, r.t_dtype = distill ? t_dtype : -1;
   r.T = static_cast<int>(T), r.D = static_cast<int>(dim), r.Dp = static_cast<int>(st.Dp), r.V = static_cast<int>(vocab);
-  r.top = static_cast<int>(top), r.planes = planes, r.plane = st.plane;
+  r.top = static_cast<int>(top), r.plane = st.plane;
   r.inv_temp = static_cast<float>(1.0 / temperature);
-  r.counts = reinterpret_cast<int*>(ws + space.counts);
-  r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.q = st.q, r.entropy = st.entropy, r.h = st.h;
+  r.masks = T * top <= kFewEntries ? nullptr : reinterpret_cast<uint32_t*>(ws + space.masks);
+  r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.h = st.h;
   r.loss = reduction == FMOE_REDUCE_NONE ? loss : nullptr;
-  if (blocks > 1) vl_count_kernel<<<dim3(static_cast<uint32_t>(blocks)), 256, 0, s>>>(r);
   const dim3 rows_grid(static_cast<uint32_t>(blocks));
-  if (h_dtype == FMOE_BF16 && planes == 1) vl_rows_kernel<FMOE_BF16, 1><<<rows_grid, 256, 0, s>>>(r);
-  else if (h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 3><<<rows_grid, 256, 0, s>>>(r);
-  else if (planes == 1) vl_rows_kernel<FMOE_F32, 1><<<rows_grid, 256, 0, s>>>(r);
-  else vl_rows_kernel<FMOE_F32, 3><<<rows_grid, 256, 0, s>>>(r);
+  if (r.masks) vl_mark_kernel<<<rows_grid, 1024, 0, s>>>(r);
+  if (h_dtype == FMOE_BF16 && planes == 1) vl_rows_kernel<FMOE_BF16, 1><<<rows_grid, 1024, 0, s>>>(r);
+  else if (h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 3><<<rows_grid, 1024, 0, s>>>(r);
+  else if (planes == 1) vl_rows_kernel<FMOE_F32, 1><<<rows_grid, 1024, 0, s>>>(r);
+  else vl_rows_kernel<FMOE_F32, 3><<<rows_grid, 1024, 0, s>>>(r);
 
   VlGemm g{};
   g.a = st.h, g.a_plane = st.plane, g.lda = static_cast<int>(st.Dp);
-  g.passes = planes == 3 ? 6 : 1, g.head = st.head, g.k = static_cast<int>(st.Dp);
+  g.head = st.head, g.k = static_cast<int>(st.Dp);
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
   g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = st.Tp;
   g.index = distill ? nullptr : st.index, g.picked = st.picked;
@@ -1107,7 +1290,9 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
       g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
     }
     g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
-    vl_gemm_kernel<VL_STATS><<<vl_grid(ceil_div(st.Tp, 256) * ceil_div(rows, 256)), core::NT, 0, s>>>(g);
+    const dim3 grid = vl_grid(ceil_div(st.Tp, 256) * ceil_div(rows, 256));
+    if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(g);
+    else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(g);
   }
 
   LossArgs l{};
@@ -1116,9 +1301,9 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   l.stat = st.stat, l.picked = st.picked;
   l.row_loss = reinterpret_cast<float*>(ws + space.row_loss);
   l.loss = r.loss;
-  l.q = st.q, l.entropy = st.entropy, l.h = st.h, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
+  l.h = st.h, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
   l.top = distill ? static_cast<int>(top) : 0;
-  l.D = r.D, l.Dp = r.Dp, l.w_dtype = w_dtype, l.planes = planes, l.c = g.c;
+  l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r;
   l.factor = static_cast<float>(temperature * temperature);
   if (T > 0) {
     if (T >= 8192) vl_stat_kernel<64><<<dim3(static_cast<uint32_t>(ceil_div(T, 64))), 1024, 0, s>>>(l);
@@ -1161,16 +1346,15 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint16_t* const gbuf = reinterpret_cast<uint16_t*>(ws + space.g);
   uint16_t* const pack = reinterpret_cast<uint16_t*>(ws + space.pack);
-  float* const sum = reinterpret_cast<float*>(ws + space.sum);
-  const int64_t piece = space.plan.piece, g_plane = st.Tp * piece;
+  const int64_t piece = space.piece, g_plane = st.Tp * piece;
   const int64_t pack_plane = std::min(pad64(vocab), piece) * st.Dp;
-  const int passes = planes == 3 ? 6 : 1, Dp = static_cast<int>(st.Dp);
-  const float factor = static_cast<float>(temperature * logit_scale);  // temperature^2 times d t / d logit
+  const int Dp = static_cast<int>(st.Dp);
   const int64_t mt = ceil_div(st.Tp, 256), dt = ceil_div(st.Dp, 256);
   for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
-    const int64_t rows = std::min(piece, vocab - v0);
+    const int64_t rows = std::min(piece, vocab - v0), vt = ceil_div(rows, 256);
     VlGemm g{};
-    g.passes = passes, g.head = st.head, g.Tp = st.Tp, g.planes = planes;
+    g.head = st.head, g.Tp = st.Tp, g.perm = st.perm, g.D = static_cast<int>(dim);
+    g.split = reinterpret_cast<float*>(ws + space.split);
     const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ldw;
     int64_t w_plane = 0;
     int w_ld = static_cast<int>(ldw);
@@ -1182,40 +1366,51 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     g.a = st.h, g.a_plane = st.plane, g.lda = Dp, g.k = Dp;
     g.b = w, g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
     g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
-    g.stat = st.stat, g.d_loss = d_loss, g.perm = st.perm, g.factor = factor, g.reduction = reduction;
+    g.index = distill ? nullptr : st.index, g.picked = st.picked;
+    g.stat = st.stat, g.d_loss = d_loss, g.reduction = reduction;
+    g.factor = static_cast<float>(temperature * logit_scale);  // temperature^2 times d t / d logit
     g.g = gbuf, g.g_plane = g_plane, g.ldg = static_cast<int>(piece);
-    vl_gemm_kernel<VL_GRAD><<<vl_grid(mt * ceil_div(rows, 256)), core::NT, 0, s>>>(g);
-    FixArgs f{};
-    f.head = st.head, f.perm = st.perm, f.index = st.index, f.q = st.q, f.picked = st.picked, f.stat = st.stat;
-    f.d_loss = d_loss, f.top = static_cast<int>(top), f.distill = distill;
-    f.v0 = static_cast<int>(v0), f.v1 = static_cast<int>(v0 + rows), f.reduction = reduction, f.planes = planes;
-    f.ldg = g.ldg, f.factor = factor, f.g = gbuf, f.g_plane = g_plane;
-    if (T > 0) vl_fix_kernel<<<dim3(static_cast<uint32_t>(ceil_div(T * top, 256))), 256, 0, s>>>(f);
+    if (planes == 1) vl_gemm_kernel<VL_GRAD, 1><<<vl_grid(mt * vt), core::NT, 0, s>>>(g);
+    else vl_gemm_kernel<VL_GRAD, 3><<<vl_grid(mt * vt), core::NT, 0, s>>>(g);
+    if (distill && T > 0) {
+      FixArgs f{};
+      f.head = st.head, f.perm = st.perm, f.index = st.index, f.q = st.q, f.picked = st.picked, f.stat = st.stat;
+      f.d_loss = d_loss, f.top = static_cast<int>(top);
+      f.v0 = static_cast<int>(v0), f.v1 = static_cast<int>(v0 + rows), f.reduction = reduction, f.planes = planes;
+      f.ldg = g.ldg, f.factor = g.factor, f.g = gbuf, f.g_plane = g_plane;
+      vl_fix_kernel<<<dim3(static_cast<uint32_t>(ceil_div(T * top, 256))), 256, 0, s>>>(f);
+    }
+    VlGemm h = g;
+    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg;
+    h.cols = Dp, h.vocab = static_cast<int>(rows);
     if (d_hidden != nullptr) {
-      VlGemm h = g;
-      h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg;
-      h.cols = Dp, h.vocab = static_cast<int>(rows), h.sum = sum, h.add = v0 > 0;
-      h.ranges = static_cast<int>(std::min<int64_t>(space.plan.ranges, ceil_div(rows, 64)));
-      // (a short last piece may have fewer ranges: the others keep their sums)
-      vl_gemm_kernel<VL_DH><<<vl_grid(mt * dt * h.ranges), core::NT, 0, s>>>(h);
+      h.out = d_hidden, h.out_dtype = dh_dtype, h.sum = reinterpret_cast<float*>(ws + space.sum);
+      h.add = v0 > 0, h.more = v0 + rows < vocab;
+      // the split tiles' number depends on the rows with entries, which the host does not know
+      const int64_t units = ceil_div(rows, 64) * (planes == 3 ? 6 : 1);
+      const int64_t blocks = units < 16 ? 0 : std::min<int64_t>(mt * dt, kVlCus - 1) * 16;
+      const int64_t clear = h.more ? 0 : ceil_div(T, 64);
+      const dim3 grid(static_cast<uint32_t>(blocks + clear));
+      if (planes == 1) vl_gemm_kernel<VL_DH, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
+      else vl_gemm_kernel<VL_DH, 3><<<dim3(kVlCus), core::NT, 0, s>>>(h);
+      if (blocks + clear > 0) {
+        const int b = static_cast<int>(blocks), t = static_cast<int>(T);
+        if (planes == 1) vl_split_kernel<VL_DH, 1><<<grid, 256, 0, s>>>(h, st.inv, t, b);
+        else vl_split_kernel<VL_DH, 3><<<grid, 256, 0, s>>>(h, st.inv, t, b);
+      }
     }
     if (d_weight != nullptr) {
-      VlGemm d = g;
-      d.a = gbuf, d.a_plane = g_plane, d.lda = g.ldg;
-      d.b = st.h, d.b_plane = st.plane, d.ldb = Dp;
-      d.cols = Dp, d.vocab = static_cast<int>(rows), d.D = static_cast<int>(dim), d.dw_dtype = dw_dtype;
-      d.dw = static_cast<uint8_t*>(d_weight) + v0 * dim * (dw_dtype == FMOE_BF16 ? 2 : 4);
-      vl_gemm_kernel<VL_DW><<<vl_grid(ceil_div(rows, 256) * dt), core::NT, 0, s>>>(d);
+      h.b = st.h, h.b_plane = st.plane, h.ldb = Dp;
+      h.out = static_cast<uint8_t*>(d_weight) + v0 * dim * (dw_dtype == FMOE_BF16 ? 2 : 4), h.out_dtype = dw_dtype;
+      const int64_t units = st.Tp / 64 * (planes == 3 ? 6 : 1), rest = vt * dt % kVlCus;
+      if (planes == 1) vl_gemm_kernel<VL_DW, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
+      else vl_gemm_kernel<VL_DW, 3><<<dim3(kVlCus), core::NT, 0, s>>>(h);
+      if (units >= 16 && rest > 0) {
+        const dim3 grid(static_cast<uint32_t>(rest * 16));
+        if (planes == 1) vl_split_kernel<VL_DW, 1><<<grid, 256, 0, s>>>(h, nullptr, 0, 0);
+        else vl_split_kernel<VL_DW, 3><<<grid, 256, 0, s>>>(h, nullptr, 0, 0);
+      }
     }
-  }
-  if (d_hidden != nullptr && T > 0) {
-    const dim3 grid(static_cast<uint32_t>(ceil_div(T, 4)));
-    const int64_t stride = st.Tp * st.Dp;
-    const int d = static_cast<int>(dim);
-    if (dh_dtype == FMOE_BF16)
-      vl_dh_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(st.inv, sum, stride, space.plan.ranges, T, d, Dp, d_hidden);
-    else
-      vl_dh_kernel<FMOE_F32><<<grid, 256, 0, s>>>(st.inv, sum, stride, space.plan.ranges, T, d, Dp, d_hidden);
   }
   return launch_status();
 }

@@ -57,7 +57,7 @@ def _check_index(what, name, t, device):
 
 
 class _EmbeddingFunction(torch.autograd.Function):
-    """The embedding through the Python wrappers."""
+    """The embedding through the Python wrappers (the native form, csrc/block_host.cpp, runs the same entry points)."""
 
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
@@ -89,17 +89,21 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
             raise ValueError(f"{what}: padding_idx must be within the vocabulary (got {padding_idx} of {V})")
         pad = padding_idx % V
     scale = float(scale)
-    flat = ids.reshape(-1).contiguous()
+    flat = ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
     if torch.compiler.is_compiling():
         y = torch.ops.fusionllm.embedding_fwd(flat, weight, scale, pad)
     else:
         refuse_tangents(what, weight)
-        if torch.is_grad_enabled() and weight.requires_grad:
+        grad = torch.is_grad_enabled() and weight.requires_grad
+        host = K.block_host()
+        if host is not None:
+            y = host.embedding(flat, weight, scale, pad, grad)
+        elif grad:
             y = _EmbeddingFunction.apply(flat, weight, scale, pad)
         else:
             with _on_device(weight):
                 y = K.embedding_fwd(flat, _rows(weight), scale)
-    return y.view(*ids.shape, dim)
+    return y if ids.dim() == 1 else y.view(*ids.shape, dim)
 
 
 class Embedding(nn.Embedding):
@@ -124,7 +128,8 @@ class Embedding(nn.Embedding):
 
 
 class _VocabLossFunction(torch.autograd.Function):
-    """A loss over the vocabulary; teacher None: cross entropy."""
+    """A loss over the vocabulary (teacher None: cross entropy) through the Python wrappers (the native form,
+    csrc/block_host.cpp, runs the same entry points)."""
 
     @staticmethod
     def forward(ctx, hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction):
@@ -174,8 +179,8 @@ def _check_loss(what, hidden, weight, reduction, logit_scale):
 def _vocab_loss(what, hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction):
     """index and teacher: hidden's leading shape and the list."""
     shape = hidden.shape[:-1]
-    flat = hidden.reshape(-1, hidden.shape[-1])
-    index = index.reshape(flat.shape[0], -1).contiguous() if flat.shape[0] else index.new_empty((0, index.shape[-1]))
+    flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    index = index.reshape(-1, index.shape[-1]).contiguous()
     if teacher is not None:
         teacher = teacher.detach().reshape(index.shape).contiguous()
     args = (flat, weight, index, teacher, int(ignore_index), float(logit_scale), float(temperature), planes, reduction)
@@ -183,12 +188,16 @@ def _vocab_loss(what, hidden, weight, index, teacher, ignore_index, logit_scale,
         loss = torch.ops.fusionllm.vocab_loss_fwd(*args)[0]
     else:
         refuse_tangents(what, hidden, weight)
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        host = K.block_host()
+        if host is not None:
+            loss = host.vocab_loss(*args[:-1], K.REDUCTIONS[reduction], grad)
+        elif grad:
             loss = _VocabLossFunction.apply(*args)
         else:
             with _on_device(weight):
                 loss = K.vocab_loss_fwd(_rows(flat), _rows(weight), *args[2:])[0]
-    return loss.view(shape) if reduction == "none" else loss
+    return loss.view(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,

@@ -21,7 +21,7 @@ extern "C" {
 #define FMOE_VOCAB_MAX_DIM 16384
 #define FMOE_VOCAB_MAX_TOKENS 16777216 /* rows of one call */
 #define FMOE_VOCAB_MAX_VOCAB 16777216
-#define FMOE_VOCAB_MAX_ELEMENTS 68719476736LL /* of an operand: rows * dim, vocab * dim */
+#define FMOE_VOCAB_MAX_ELEMENTS 8589934592LL /* of an operand: rows * dim, vocab * dim */
 #define FMOE_VOCAB_MAX_TOP 1024        /* listed logits of a teacher per row */
 
 /* ---------------------------------------------------------------------------
@@ -35,7 +35,7 @@ int fmoe_embedding_fwd(const void* ids, int index64, const void* weight, int dty
 
 /* Its backward: d_weight[v] = scale * sum of dy[t] over the t with ids[t] = v, every row
  * written (zeros where v has no token).  The tokens are sorted by id, stably; a row is summed in
- * fp32, in a fixed order (pieces of 32 of an id's tokens where it has many), without atomics: the
+ * fp32, in a fixed order (pieces of 16 of an id's tokens where it has many), without atomics: the
  * same bits every run.  Rows of padding_idx (-1: none) stay zero, ids out of range add nothing.
  * Row t of dy starts at dy + t * lddy.  workspace: 256-byte aligned. */
 size_t fmoe_embedding_bwd_workspace_bytes(int64_t T, int64_t vocab, int64_t dim);
