@@ -271,23 +271,25 @@ __device__ __forceinline__ void vl_planes(int passes, int pass, int& pa, int& pb
 }
 
 // Split of DH's and DW's K: with T tiles, the T mod 256 ones of the last, partial round are cut into S ranges
-// of K, which leave fp32 partial tiles that a second launch adds in order.  S gives the fewest steps, a
-// round costing its steps and an epilogue, a partial tile its traffic (256 KB written and read), the second launch
-// its own.  (S ranges of one tile are walked range by range, so that the workgroups of an XCD read the same operand
-// rows at a time.)
+// of K, which leave fp32 partial tiles that a second launch adds in order.  S fills one to four rounds of
+// workgroups, whichever takes the fewest steps: a round costs its steps and an epilogue, a partial tile its traffic
+// (256 KB written and read), the second launch its own.  (The ranges are walked range by range, so that the
+// workgroups of an XCD read the same operand rows at a time.)
 struct VlSplit {
   int whole, rest, ranges;  // tiles computed whole, tiles split, ranges of each
 };
 constexpr int kSplitSlots = 1024;  // partial tiles, at most
-__host__ __device__ inline VlSplit vl_split(int tiles, int units) {
+__device__ __forceinline__ VlSplit vl_split(int tiles, int units) {
   const int rest = tiles % kVlCus;
   VlSplit best{tiles, 0, 1};
   if (rest == 0) return best;
   float least = static_cast<float>(units) + 2.0f;
-  for (int s = 2; s <= units / 8 && s * rest <= kSplitSlots; ++s) {
-    const float rounds = static_cast<float>((s * rest + kVlCus - 1) / kVlCus);
-    const float cost = rounds * (static_cast<float>(units) / static_cast<float>(s) + 2.0f) + 0.055f * static_cast<float>(s * rest) + 4.0f;
-    if (cost < least) least = cost, best = VlSplit{tiles - rest, rest, s};
+#pragma unroll
+  for (int rounds = 1; rounds <= 4; ++rounds) {
+    const int s = min(rounds * kVlCus / rest, min(units / 8, kSplitSlots / rest));
+    const float cost = static_cast<float>(rounds) * (static_cast<float>(units) / static_cast<float>(max(s, 1)) + 2.0f) +
+                       0.055f * static_cast<float>(s * rest) + 4.0f;
+    if (s >= 2 && cost < least) least = cost, best = VlSplit{tiles - rest, rest, s};
   }
   return best;
 }
@@ -787,8 +789,276 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// The split tiles: their ranges' partial tiles added in order.  A workgroup adds 16 rows of a tile.  DH's last
-// piece: and zeros in the rows of the result without entries, 64 rows a workgroup behind those.
+// Joins the maximum and sum of exponentials of other columns.
+__device__ __forceinline__ void vl_join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), peak = top == -__builtin_inff() ? 0.0f : top;
+  s = s * __builtin_amdgcn_exp2f(m - peak) + s2 * __builtin_amdgcn_exp2f(m2 - peak);
+  m = top;
+}
+
+// ---- logits of few rows ------------------------------------------------------------------------------
+// Up to 64 rows (T, which the host knows): bound by the read of the weight, which a 256-row tile would stream through
+// few workgroups (37 rows, vocab 32768, dim 768: 128 tiles).  A workgroup takes 128 columns, a wave 16 of them and all
+// rows; the wave's part of the weight goes from memory straight into the fragments, 8 loads in flight, as it lies
+// (any dtype, stride and alignment: no packed copy), the rows' K piece through LDS.  planes = 3: the products are
+// v_mfma_f32_16x16x4_f32 on fp32 operands, at up to 64 rows as fast as the weight arrives.
+constexpr int kThinRows = 64;
+constexpr int kThinBytes = 1024;             // of a row's K piece in LDS
+constexpr int kThinRow = kThinBytes + 16;    // (the 16 rows of a fragment in different banks)
+
+struct ThinWeight {
+  const void* p;
+  int64_t ld;
+  int D;
+};
+
+// One lane's operand of a step: E consecutive elements of its weight row.
+template <int WT, int PLANES>
+struct ThinFrag {
+  uint32_t u[WT == FMOE_F32 && PLANES == 1 ? 8 : 4];
+};
+// 16 bytes of a packed row's K piece: bf16, or the three parts of four fp32 numbers.
+template <int PLANES>
+struct ThinRow {
+  uint2 u[PLANES == 3 ? 3 : 2];
+};
+
+template <int MODE, int WT, int PLANES, int MB>
+__global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const ThinWeight wt) {
+  constexpr bool F = PLANES == 3;
+  constexpr int E = F ? 4 : 8;               // elements per lane and step; a step is 4 E of K
+  constexpr int KC = kThinBytes / (F ? 4 : 2), STEPS = KC / (4 * E), RING = WT == FMOE_F32 && PLANES == 1 ? 4 : 8;
+  constexpr int HV = MB * 2;                 // 16-byte pieces of the rows per thread
+  static_assert(STEPS == 16 && HV * 512 == 16 * MB * 64);
+  __shared__ __attribute__((aligned(16))) uint8_t hs[16 * MB * kThinRow];
+  __shared__ float2 red[8][16 * MB];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int er = lane & 15, eg = lane >> 4;
+  const int D = wt.D;
+  const int full = D / (4 * E), total = (D + 4 * E - 1) / (4 * E);
+  const int col0 = blockIdx.x * 128 + 16 * w;  // of the piece
+  const int64_t row_at = static_cast<int64_t>(a.v0 + min(col0 + er, a.cols - 1)) * wt.ld;
+
+  typedef ThinFrag<WT, PLANES> Frag;
+  auto load = [&](int g) __attribute__((always_inline)) {
+    Frag f;
+    const int64_t at = row_at + (g * 4 * E + eg * E);
+    if constexpr (WT == FMOE_BF16) {
+      f = __builtin_bit_cast(Frag, load_raw<FMOE_BF16, 8>(wt.p, at));
+    } else {
+      const f32x4_e4* p = reinterpret_cast<const f32x4_e4*>(static_cast<const float*>(wt.p) + at);
+#pragma unroll
+      for (int q = 0; q < E / 4; ++q) {
+        const f32x4 x = p[q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.u[4 * q + i] = __float_as_uint(x[i]);
+      }
+    }
+    return f;
+  };
+  Frag ring[RING];
+#pragma unroll
+  for (int g = 0; g < RING; ++g)
+    if (g < full) ring[g] = load(g);
+  // the rows' K piece from step g0 on (zeros up to Dp, a multiple of 64; what is past that is not read)
+  ThinRow<PLANES> hv[HV];
+  auto load_rows = [&](int g0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < HV; ++i) {
+      const int r = 8 * i + w, k = g0 * 4 * E + lane * E;
+      if (k < a.lda) {
+        const uint16_t* p = a.a + static_cast<int64_t>(r) * a.lda + k;
+        if constexpr (F) {
+#pragma unroll
+          for (int q = 0; q < 3; ++q) hv[i].u[q] = *reinterpret_cast<const uint2*>(p + q * a.a_plane);
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          hv[i].u[0] = make_uint2(x.x, x.y), hv[i].u[1] = make_uint2(x.z, x.w);
+        }
+      }
+    }
+  };
+  load_rows(0);
+
+  f32x4 acc[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Frag& f, int s) __attribute__((always_inline)) {
+    const uint8_t* hp = hs + er * kThinRow + s * 64 + eg * 16;
+    if constexpr (F) {
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(hp + m * 16 * kThinRow);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.u[i]), x[i], acc[m], 0, 0, 0);
+      }
+    } else {
+      bf16x8 b;
+      if constexpr (WT == FMOE_F32) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(f.u[i]);
+        b = __builtin_bit_cast(bf16x8, pack8(v));
+      } else {
+        b = __builtin_bit_cast(bf16x8, f);
+      }
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(hp + m * 16 * kThinRow);
+        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, x, acc[m], 0, 0, 0);
+      }
+    }
+  };
+  for (int g0 = 0; g0 < total; g0 += STEPS) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HV; ++i) {
+      uint4 v;
+      if constexpr (F) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 2; q >= 0; --q) {  // exact: the parts of one fp32 number
+          const uint2 u = hv[i].u[q];
+          x[0] += __uint_as_float(u.x << 16), x[1] += __uint_as_float(u.x & 0xffff0000u);
+          x[2] += __uint_as_float(u.y << 16), x[3] += __uint_as_float(u.y & 0xffff0000u);
+        }
+        v = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      } else {
+        v = make_uint4(hv[i].u[0].x, hv[i].u[0].y, hv[i].u[1].x, hv[i].u[1].y);
+      }
+      *reinterpret_cast<uint4*>(hs + (8 * i + w) * kThinRow + lane * 16) = v;
+    }
+    __syncthreads();
+    if (g0 + STEPS < total) load_rows(g0 + STEPS);  // under this piece's products
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (g0 + s < full) {
+        const Frag f = ring[s % RING];
+        if (g0 + s + RING < full) ring[s % RING] = load(g0 + s + RING);
+        multiply(f, s);
+      }
+    }
+  }
+  if (full < total) {  // the end of rows whose length is no multiple of a step's
+    const int k = full * 4 * E + eg * E;
+    float v[8];
+    load_upto8<WT>(wt.p, row_at + k, min(max(D - k, 0), E), v);
+    Frag f;
+    if constexpr (WT == FMOE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.u[i] = pack2(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) f.u[i] = __float_as_uint(v[i]);
+    }
+    multiply(f, full % STEPS);
+  }
+  const int n = __builtin_amdgcn_readfirstlane(a.head[0]);
+
+  // acc[m] of lane l: row 16 m + l % 16, columns col0 + 4 (l / 16) + 0..3
+  const int lim = a.cols - col0 - 4 * eg;
+  if constexpr (MODE == VL_STATS) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int row = 16 * m + er;
+      float t[4], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        t[e] = e < lim ? acc[m][e] * a.c : -__builtin_inff();
+        top = fmaxf(top, t[e]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float peak = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = sum + __builtin_amdgcn_exp2f(t[e] - peak);
+      sum = sum + __shfl_xor(sum, 16, 64);
+      sum = sum + __shfl_xor(sum, 32, 64);
+      if (eg == 0) red[w][row] = make_float2(top, sum);
+      if (a.index && row < n) {
+        const int rel = a.index[row] - (a.v0 + col0) - 4 * eg;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (rel == e && e < lim) a.picked[row] = t[e];
+      }
+    }
+    __syncthreads();
+    if (tid < 16 * MB && tid < n) {
+      float2 ms = red[0][tid];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) vl_join(ms.x, ms.y, red[q][tid].x, red[q][tid].y);
+      a.part[static_cast<int64_t>(a.v0 / 128 + blockIdx.x) * a.Tp + tid] = ms;
+    }
+  } else {
+    // 128 columns of G per row, a plane at a time through LDS into whole lines
+    constexpr int LD = 128 * 2 + 16;
+    float v[MB][4];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int row = 16 * m + er;
+      float2 ml = make_float2(0.0f, 0.0f);
+      float up = 0.0f;
+      int rel = -1;
+      if (row < n) {
+        ml = a.stat[row];
+        up = vl_row_weight(a.d_loss, a.perm, a.reduction, n, row, a.factor);
+        if (a.index) rel = a.index[row] - (a.v0 + col0) - 4 * eg;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f((acc[m][e] * a.c - ml.x) - ml.y);
+        v[m][e] = row < n && e < lim ? (rel == e ? a.picked[row] : p) * up : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const uint2 u = make_uint2(pack2(v[m][0], v[m][1]), pack2(v[m][2], v[m][3]));
+        *reinterpret_cast<uint2*>(hs + (16 * m + er) * LD + 32 * w + 8 * eg) = u;
+        v[m][0] = v[m][0] - __uint_as_float(u.x << 16);
+        v[m][1] = v[m][1] - __uint_as_float(u.x & 0xffff0000u);
+        v[m][2] = v[m][2] - __uint_as_float(u.y << 16);
+        v[m][3] = v[m][3] - __uint_as_float(u.y & 0xffff0000u);
+      }
+      __syncthreads();
+      for (int i = tid; i < kThinRows * 16; i += 512) {
+        const int r = i >> 4, c = i & 15;
+        const uint4 x = r < 16 * MB ? *reinterpret_cast<const uint4*>(hs + r * LD + c * 16) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(a.g + p * a.g_plane + static_cast<int64_t>(r) * a.ldg + blockIdx.x * 128 + c * 8) = x;
+      }
+    }
+  }
+}
+
+template <int MODE, int WT, int PLANES>
+void vl_thin_launch(const VlGemm& a, const ThinWeight& w, int64_t T, dim3 grid, hipStream_t s) {
+  if (T <= 16) vl_thin_kernel<MODE, WT, PLANES, 1><<<grid, 512, 0, s>>>(a, w);
+  else if (T <= 32) vl_thin_kernel<MODE, WT, PLANES, 2><<<grid, 512, 0, s>>>(a, w);
+  else vl_thin_kernel<MODE, WT, PLANES, 4><<<grid, 512, 0, s>>>(a, w);
+}
+// Where it is the faster form: T <= kThinRows, but for more than 32 rows against a bf16 weight whose 256-row tiles
+// fill two rounds of workgroups (37 rows, 131072 x 4096: 275 us in tiles against 318; 32768 x 768 21 against 15; one
+// row, 131072 x 768: 40 against 34).
+bool vl_is_thin(int64_t T, int64_t V, bool packs) {
+  return T <= kThinRows && (T <= 32 || packs || ceil_div(V, 256) < 2 * kVlCus);
+}
+// Logits of T <= kThinRows rows: STATS (two workgroups per 256 columns: each writes its partial sums, also of no
+// columns) or GRAD.
+template <int MODE>
+void vl_thin(const VlGemm& a, const void* weight, int w_dtype, int64_t ldw, int64_t D, int planes, int64_t T, hipStream_t s) {
+  const ThinWeight w{weight, ldw, static_cast<int>(D)};
+  const dim3 grid(static_cast<uint32_t>(2 * ceil_div(a.cols, 256)));
+  if (planes == 3) vl_thin_launch<MODE, FMOE_F32, 3>(a, w, T, grid, s);
+  else if (w_dtype == FMOE_BF16) vl_thin_launch<MODE, FMOE_BF16, 1>(a, w, T, grid, s);
+  else vl_thin_launch<MODE, FMOE_F32, 1>(a, w, T, grid, s);
+}
+
+// The split tiles: their ranges' partial tiles added in order, by the first `blocks` workgroups (32 for every tile
+// that can be split).  DH's last piece: and zeros in the rows of the result without entries, 64 rows a workgroup
+// behind those.
 template <int MODE, int PLANES>
 __global__ __launch_bounds__(256) void vl_split_kernel(const VlGemm a, const int* inv, int T, int blocks) {
   using namespace core;
@@ -813,34 +1083,57 @@ __global__ __launch_bounds__(256) void vl_split_kernel(const VlGemm a, const int
   const int tiles_m = (m_rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
   const int nk = MODE == VL_DH ? (a.vocab + BK - 1) / BK : np / BK;
   const VlSplit sp = vl_split(tiles_m * tiles_n, nk * (PLANES == 1 ? 1 : 6));
-  const int r = blockIdx.x / 16, rows16 = (blockIdx.x % 16) * 16;
-  if (r >= sp.rest) return;
-  int tm, tn;
-  vl_tile(sp.whole + r, tiles_m, tiles_n, tm, tn);
-  if (tm * BM + rows16 >= (MODE == VL_DW ? a.vocab : n)) return;
+  const int64_t range = static_cast<int64_t>(sp.rest) * (BM * BN);
+  const int limit = MODE == VL_DW ? a.vocab : n;
   constexpr int U = 8;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int row = rows16 + half * 8 + (threadIdx.x >> 5), col = (threadIdx.x & 31) * 8;
-    const float* src = a.split + static_cast<int64_t>(r) * (BM * BN) + row * BN + col;
-    float v[8];
+  // ranges first, first + step, ... of 8 columns, added in order
+  auto add = [&](const float* src, int first, int step, float* v) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    for (int s0 = 0; s0 < sp.ranges; s0 += U) {
+    for (int s0 = first; s0 < sp.ranges; s0 += U * step) {
       f32x4 u[U][2];
 #pragma unroll
       for (int s = 0; s < U; ++s) {
-        const float* p = src + static_cast<int64_t>(min(s0 + s, sp.ranges - 1)) * sp.rest * (BM * BN);
+        const float* p = src + min(s0 + s * step, sp.ranges - 1) * range;
         u[s][0] = *reinterpret_cast<const f32x4*>(p);
         u[s][1] = *reinterpret_cast<const f32x4*>(p + 4);
       }
 #pragma unroll
       for (int s = 0; s < U; ++s)
-        if (s0 + s < sp.ranges)
+        if (s0 + s * step < sp.ranges)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = v[e] + u[s][0][e], v[4 + e] = v[4 + e] + u[s][1][e];
     }
+  };
+  const int col = (threadIdx.x & 31) * 8, sub = threadIdx.x >> 5;
+  int tm, tn;
+  float v[8];
+  if (sp.ranges < 2 * U) {  // 8 rows of a tile per workgroup
+    const int r = blockIdx.x / 32, row = (blockIdx.x % 32) * 8 + sub;
+    if (r >= sp.rest) return;
+    vl_tile(sp.whole + r, tiles_m, tiles_n, tm, tn);
+    if (tm * BM + (blockIdx.x % 32) * 8 >= limit) return;
+    add(a.split + static_cast<int64_t>(r) * (BM * BN) + row * BN + col, 0, 1, v);
     vl_result8<MODE>(a, n, tm * BM + row, tn * BN + col, v);
+    return;
+  }
+  // many ranges of few tiles: a row per workgroup, eight parts of its ranges side by side
+  __shared__ float sums[8][BN];
+  for (int q = blockIdx.x; q < sp.rest * BM; q += blocks) {
+    const int r = q / BM, row = q % BM;
+    vl_tile(sp.whole + r, tiles_m, tiles_n, tm, tn);
+    if (tm * BM + row >= limit) continue;
+    add(a.split + static_cast<int64_t>(r) * (BM * BN) + row * BN + col, sub, 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[sub][(threadIdx.x & 31) + 32 * e] = v[e];
+    __syncthreads();
+    if (sub == 0) {
+      for (int p = 1; p < 8; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] + sums[p][threadIdx.x + 32 * e];
+      vl_result8<MODE>(a, n, tm * BM + row, tn * BN + col, v);
+    }
+    __syncthreads();
   }
 }
 
@@ -874,12 +1167,6 @@ __device__ __forceinline__ void vl_store_loss(const LossArgs& a, int row, float 
 
 // m and l of R rows per workgroup: each of its 1024 / R threads per row joins every so many of the partial
 // sums, in order; then lanes, then waves.
-__device__ __forceinline__ void vl_join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2), peak = top == -__builtin_inff() ? 0.0f : top;
-  s = s * __builtin_amdgcn_exp2f(m - peak) + s2 * __builtin_amdgcn_exp2f(m2 - peak);
-  m = top;
-}
-
 template <int R>
 __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
   __shared__ float2 red[16][R];
@@ -1153,7 +1440,7 @@ struct VlFwdSpace {
     masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
-    pack = take(packs ? vl_fwd_piece(D, V, planes, true) * pad64(D) * 2 * planes : 0);
+    pack = take(packs && !vl_is_thin(T, V, packs) ? vl_fwd_piece(D, V, planes, true) * pad64(D) * 2 * planes : 0);
   }
 };
 
@@ -1190,8 +1477,7 @@ int vl_pack(const void* weight, int w_dtype, int64_t ldw, int64_t v0, int64_t ro
             int64_t plane, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(ceil_div(rows, 4)));
   const int Dp = static_cast<int>(pad64(D)), r = static_cast<int>(rows), d = static_cast<int>(D);
-  if (w_dtype == FMOE_BF16 && planes == 1) vl_pack_kernel<FMOE_BF16, 1><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
-  else if (w_dtype == FMOE_BF16) vl_pack_kernel<FMOE_BF16, 3><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
+  if (w_dtype == FMOE_BF16) vl_pack_kernel<FMOE_BF16, 1><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
   else if (planes == 1) vl_pack_kernel<FMOE_F32, 1><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
   else vl_pack_kernel<FMOE_F32, 3><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
   return launch_status();
@@ -1239,7 +1525,9 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   if (!vl_sizes_ok(T, dim, vocab, top, planes)) return FMOE_ERR_SHAPE;
   if ((T > 1 && (ldh < dim || ldh > (int64_t(1) << 38))) || (vocab > 1 && (ldw < dim || ldw >= (int64_t(1) << 22))))
     return FMOE_ERR_SHAPE;
-  if (!vl_dtype(h_dtype) || !vl_dtype(w_dtype) || (teacher && !vl_dtype(t_dtype))) return FMOE_ERR_DTYPE;
+  if (!vl_dtype(h_dtype) || !vl_dtype(w_dtype) || (teacher && !vl_dtype(t_dtype)) ||
+      (planes == 3 && (h_dtype != FMOE_F32 || w_dtype != FMOE_F32)))
+    return FMOE_ERR_DTYPE;
   if (weight == nullptr || (T > 0 && (hidden == nullptr || index == nullptr || (distill && teacher == nullptr))) ||
       loss == nullptr)
     return FMOE_ERR_INVALID_ARG;
@@ -1267,8 +1555,7 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   r.loss = reduction == FMOE_REDUCE_NONE ? loss : nullptr;
   const dim3 rows_grid(static_cast<uint32_t>(blocks));
   if (r.masks) vl_mark_kernel<<<rows_grid, 1024, 0, s>>>(r);
-  if (h_dtype == FMOE_BF16 && planes == 1) vl_rows_kernel<FMOE_BF16, 1><<<rows_grid, 1024, 0, s>>>(r);
-  else if (h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 3><<<rows_grid, 1024, 0, s>>>(r);
+  if (h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 1><<<rows_grid, 1024, 0, s>>>(r);
   else if (planes == 1) vl_rows_kernel<FMOE_F32, 1><<<rows_grid, 1024, 0, s>>>(r);
   else vl_rows_kernel<FMOE_F32, 3><<<rows_grid, 1024, 0, s>>>(r);
 
@@ -1278,21 +1565,26 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
   g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = st.Tp;
   g.index = distill ? nullptr : st.index, g.picked = st.picked;
-  const int64_t piece = vl_fwd_piece(dim, vocab, planes, packs);
-  for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
-    const int64_t rows = std::min(piece, vocab - v0);
-    if (packs) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(ws + space.pack);
-      const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, dst, piece * st.Dp, s);
-      if (rc != FMOE_OK) return rc;
-      g.b = dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp);
-    } else {
-      g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
+  if (vl_is_thin(T, vocab, packs)) {
+    g.cols = static_cast<int>(vocab);
+    vl_thin<VL_STATS>(g, weight, w_dtype, ldw, dim, planes, T, s);
+  } else {
+    const int64_t piece = vl_fwd_piece(dim, vocab, planes, packs);
+    for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
+      const int64_t rows = std::min(piece, vocab - v0);
+      if (packs) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(ws + space.pack);
+        const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, dst, piece * st.Dp, s);
+        if (rc != FMOE_OK) return rc;
+        g.b = dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp);
+      } else {
+        g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
+      }
+      g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
+      const dim3 grid = vl_grid(ceil_div(st.Tp, 256) * ceil_div(rows, 256));
+      if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(g);
+      else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(g);
     }
-    g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
-    const dim3 grid = vl_grid(ceil_div(st.Tp, 256) * ceil_div(rows, 256));
-    if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(g);
-    else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(g);
   }
 
   LossArgs l{};
@@ -1331,7 +1623,8 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     return FMOE_ERR_INVALID_ARG;
   if (!vl_sizes_ok(T, dim, vocab, top, planes)) return FMOE_ERR_SHAPE;
   if (vocab > 1 && (ldw < dim || ldw >= (int64_t(1) << 22))) return FMOE_ERR_SHAPE;
-  if (!vl_dtype(w_dtype) || !vl_dtype(dh_dtype) || !vl_dtype(dw_dtype)) return FMOE_ERR_DTYPE;
+  if (!vl_dtype(w_dtype) || !vl_dtype(dh_dtype) || !vl_dtype(dw_dtype) || (planes == 3 && w_dtype != FMOE_F32))
+    return FMOE_ERR_DTYPE;
   if (weight == nullptr || d_loss == nullptr) return FMOE_ERR_INVALID_ARG;
   if (!vl_elem_aligned(weight, w_dtype) || !vl_elem_aligned(d_loss, FMOE_F32) || !vl_elem_aligned(d_hidden, dh_dtype) ||
       !vl_elem_aligned(d_weight, dw_dtype) || !vl_ws_aligned(state) || !vl_ws_aligned(workspace))
@@ -1350,6 +1643,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
   const int64_t pack_plane = std::min(pad64(vocab), piece) * st.Dp;
   const int Dp = static_cast<int>(st.Dp);
   const int64_t mt = ceil_div(st.Tp, 256), dt = ceil_div(st.Dp, 256);
+  const bool thin = vl_is_thin(T, vocab, packs);
   for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
     const int64_t rows = std::min(piece, vocab - v0), vt = ceil_div(rows, 256);
     VlGemm g{};
@@ -1358,7 +1652,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ldw;
     int64_t w_plane = 0;
     int w_ld = static_cast<int>(ldw);
-    if (packs) {
+    if (packs && (!thin || d_hidden != nullptr)) {
       const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, pack, pack_plane, s);
       if (rc != FMOE_OK) return rc;
       w = pack, w_plane = pack_plane, w_ld = Dp;
@@ -1370,7 +1664,8 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     g.stat = st.stat, g.d_loss = d_loss, g.reduction = reduction;
     g.factor = static_cast<float>(temperature * logit_scale);  // temperature^2 times d t / d logit
     g.g = gbuf, g.g_plane = g_plane, g.ldg = static_cast<int>(piece);
-    if (planes == 1) vl_gemm_kernel<VL_GRAD, 1><<<vl_grid(mt * vt), core::NT, 0, s>>>(g);
+    if (thin) vl_thin<VL_GRAD>(g, weight, w_dtype, ldw, dim, planes, T, s);
+    else if (planes == 1) vl_gemm_kernel<VL_GRAD, 1><<<vl_grid(mt * vt), core::NT, 0, s>>>(g);
     else vl_gemm_kernel<VL_GRAD, 3><<<vl_grid(mt * vt), core::NT, 0, s>>>(g);
     if (distill && T > 0) {
       FixArgs f{};
@@ -1388,7 +1683,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
       h.add = v0 > 0, h.more = v0 + rows < vocab;
       // the split tiles' number depends on the rows with entries, which the host does not know
       const int64_t units = ceil_div(rows, 64) * (planes == 3 ? 6 : 1);
-      const int64_t blocks = units < 16 ? 0 : std::min<int64_t>(mt * dt, kVlCus - 1) * 16;
+      const int64_t blocks = units < 16 ? 0 : std::min<int64_t>(mt * dt, kVlCus - 1) * 32;
       const int64_t clear = h.more ? 0 : ceil_div(T, 64);
       const dim3 grid(static_cast<uint32_t>(blocks + clear));
       if (planes == 1) vl_gemm_kernel<VL_DH, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
@@ -1406,9 +1701,9 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
       if (planes == 1) vl_gemm_kernel<VL_DW, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
       else vl_gemm_kernel<VL_DW, 3><<<dim3(kVlCus), core::NT, 0, s>>>(h);
       if (units >= 16 && rest > 0) {
-        const dim3 grid(static_cast<uint32_t>(rest * 16));
-        if (planes == 1) vl_split_kernel<VL_DW, 1><<<grid, 256, 0, s>>>(h, nullptr, 0, 0);
-        else vl_split_kernel<VL_DW, 3><<<grid, 256, 0, s>>>(h, nullptr, 0, 0);
+        const int b = static_cast<int>(rest * 32);
+        if (planes == 1) vl_split_kernel<VL_DW, 1><<<dim3(b), 256, 0, s>>>(h, nullptr, 0, b);
+        else vl_split_kernel<VL_DW, 3><<<dim3(b), 256, 0, s>>>(h, nullptr, 0, b);
       }
     }
   }

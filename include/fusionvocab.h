@@ -60,7 +60,7 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  * of the vocabulary at a time, as G = (p - q) times the row's weight, and multiplies
  *   d_hidden = G weight,  d_weight = G^T hidden.
  * planes = 1: operands and G are bf16 (fp32 operands are rounded), sums fp32.  planes = 3: fp32
- * operands and G as three bf16 numbers each, whose six largest products are added: fp32 precision.
+ * operands (both) and G as three bf16 numbers each, whose six largest products are added: fp32 precision.
  * Deterministic, no atomics.
  *
  * state keeps what the backward needs (fmoe_vocab_loss_state_bytes); it belongs to one forward call.

@@ -191,7 +191,8 @@ def _check(loss, h, w, up, want):
     return gh, gw
 
 
-SIZES = [(1, 2, 8), (1, 300, 64), (1, 32768, 768), (37, 5003, 768), (64, 64, 48), (65, 257, 128), (300, 777, 1001),
+SIZES = [(1, 2, 8), (1, 300, 64), (1, 32768, 768), (16, 900, 4099), (20, 384, 520), (37, 5003, 768), (64, 64, 48),
+         (64, 1281, 1500), (65, 257, 128), (300, 777, 1001),
          (513, 4096, 256), (700, 10007, 192), (1030, 1000, 320)]
 
 
@@ -241,3 +242,310 @@ def test_distillation(gpu_device, T, V, D, K, reduction, tau, dtype):
     up = torch.rand(T, generator=g).to(gpu_device) if reduction == "none" else torch.tensor(2.0, device=gpu_device)
     loss = linear_distillation(h, w, index, z, temperature=tau, reduction=reduction, logit_scale=0.9)
     _check(loss, h, w, up, _reference(h, w, index, z, -100, 0.9, tau, reduction, up))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_lists_with_repeats_infinities_and_lowest_values(gpu_device, dtype):
+    g = _gen(5)
+    T, V, D, K = 40, 500, 128, 12
+    h, w, _ = _operands(g, T, V, D, dtype, gpu_device)
+    index, z = _lists(g, T, V, K, gpu_device, repeat=True)
+    lowest = torch.finfo(torch.float32).min
+    z[1] = lowest                   # equal, so an even distribution
+    z[2, 3:] = lowest               # next to ordinary ones: nothing
+    z[3, :5] = -math.inf            # none
+    z[4] = -math.inf                # a row without entries
+    index[5, 1:] = -100
+    index[6] = -100
+    z[7, 0], index[7, 0] = math.nan, -100  # a value that is not there
+    up = torch.rand(T, generator=g).to(gpu_device)
+    clean = torch.where(index == -100, 0.0, z)
+    loss = linear_distillation(h, w, index, z, reduction="none")
+    assert float(loss[4]) == 0 and float(loss[6]) == 0
+    gh, _ = _check(loss, h, w, up, _reference(h, w, index, clean, -100, 1.0, 1.0, "none", up))
+    assert not gh[4].any() and not gh[6].any()
+
+
+@pytest.mark.parametrize("T", [50, 300])
+def test_what_is_in_rows_without_targets_stays_out(gpu_device, T):
+    # NaN and infinities in hidden states whose target is ignored change nothing
+    g = _gen(T)
+    h, w, t = _operands(g, T, 600, 96, torch.bfloat16, gpu_device)
+    drop = torch.rand(T, generator=g).to(gpu_device) < 0.5
+    t[drop] = -100
+    want = torch.autograd.grad(linear_cross_entropy(h, w, t), [h, w])
+    bad = h.detach().clone()
+    bad[drop] = math.nan
+    bad[int(drop.nonzero()[0])] = math.inf
+    bad.requires_grad_(True)
+    loss = linear_cross_entropy(bad, w, t)
+    got = torch.autograd.grad(loss, [bad, w])
+    assert torch.equal(loss, linear_cross_entropy(h, w, t))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][drop].any()
+
+
+@pytest.mark.parametrize("T", [3, 100])
+def test_no_targets_at_all_and_targets_outside_the_vocabulary(gpu_device, T):
+    g = _gen(T)
+    h, w, t = _operands(g, T, 300, 64, torch.float32, gpu_device)
+    none = torch.full_like(t, -1)
+    for reduction, want in (("mean", math.nan), ("sum", 0.0)):
+        loss = linear_cross_entropy(h, w, none, ignore_index=-1, reduction=reduction)
+        gh, gw = torch.autograd.grad(loss, [h, w])
+        assert torch.equal(loss.detach().cpu(), torch.tensor(want)) or (math.isnan(want) and bool(loss.isnan()))
+        assert not gh.any() and not gw.any()
+    t[1], t[2] = 300, -100
+    loss = linear_cross_entropy(h, w, t, reduction="none")
+    assert bool(loss[1].isnan()) and float(loss[2]) == 0 and not bool(loss[0].isnan())
+    t[0] = -7
+    assert int(linear_cross_entropy(h, w, t, reduction="none").isnan().sum()) == 2
+    assert bool(linear_cross_entropy(h, w, t).isnan())
+    lists = t[:, None].repeat(1, 3)
+    loss = linear_distillation(h, w, lists, torch.zeros(T, 3, device=gpu_device), reduction="none")
+    assert loss.isnan().nonzero().flatten().tolist() == [0, 1]
+
+
+def test_empty_batch(gpu_device):
+    w = torch.randn(100, 64, device=gpu_device, requires_grad=True)
+    h = torch.randn(0, 64, device=gpu_device, requires_grad=True)
+    t = torch.empty(0, dtype=torch.long, device=gpu_device)
+    assert linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+    assert bool(linear_cross_entropy(h, w, t).isnan())
+    gh, gw = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction="sum"), [h, w])
+    assert gh.shape == (0, 64) and not gw.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,D", [(48, 192), (200, 192), (200, 101)])
+def test_strided_operands_leading_shapes_and_frozen_parts(gpu_device, T, D, dtype):
+    # rows inside wider ones at odd addresses, [B, S, D] hidden states, a gradient for one operand only
+    g = _gen(T + D)
+    V = 700
+    h, w, t = _operands(g, T, V, D, dtype, gpu_device)
+    wide_h = torch.randn(T, D + 9, generator=g).to(gpu_device, dtype)
+    wide_h[:, 5:5 + D] = h.detach()
+    wide_w = torch.randn(V, D + 7, generator=g).to(gpu_device, dtype)
+    wide_w[:, 3:3 + D] = w.detach()
+    hs, ws = wide_h[:, 5:5 + D].requires_grad_(True), wide_w[:, 3:3 + D].requires_grad_(True)
+    up = torch.tensor(1.0, device=gpu_device)
+    want = _reference(h, w, t[:, None], None, -100, 1.0, 1.0, "mean", up)
+    grads = _check(linear_cross_entropy(hs, ws, t), hs, ws, up, want)
+    shaped = linear_cross_entropy(hs.view(4, -1, D) if hs.is_contiguous() else hs.unflatten(0, (4, -1)), ws,
+                                  t.view(4, -1), reduction="none")
+    assert shaped.shape == (4, T // 4)
+    only, = torch.autograd.grad(linear_cross_entropy(hs, ws.detach(), t), [hs])
+    assert torch.equal(only, grads[0])
+    only, = torch.autograd.grad(linear_cross_entropy(hs.detach(), ws, t), [ws])
+    assert torch.equal(only, grads[1])
+    # a transposed weight: columns adjacent
+    turned = w.detach().t().contiguous().t().requires_grad_(True)
+    gt = torch.autograd.grad(linear_cross_entropy(h, turned, t), [turned])[0]
+    _within(gt, want[2][0], want[2][1], "d_weight of a transposed weight")
+
+
+@pytest.mark.parametrize("T", [40, 260])
+def test_autocast(gpu_device, T):
+    # the trainer's setting: fp32 parameters, bf16 products; gradients in each operand's dtype
+    g = _gen(T)
+    h, w, t = _operands(g, T, 900, 160, torch.float32, gpu_device)
+    hb, wb = (x.detach().bfloat16().requires_grad_(True) for x in (h, w))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = linear_cross_entropy(h, w, t)
+        mixed = linear_cross_entropy(hb, w, t)
+    want = linear_cross_entropy(hb, wb, t)
+    assert torch.equal(loss, want) and torch.equal(mixed, want)
+    gh, gw = torch.autograd.grad(loss, [h, w])
+    bh, bw = torch.autograd.grad(want, [hb, wb])
+    assert gh.dtype == gw.dtype == torch.float32
+    assert torch.equal(gh.bfloat16(), bh) and torch.equal(gw.bfloat16(), bw)
+    mh, mw = torch.autograd.grad(mixed, [hb, w])
+    assert mh.dtype == torch.bfloat16 and torch.equal(mh, bh) and torch.equal(mw, gw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_against_differences(gpu_device, dtype):
+    # the loss's own differences along random directions: a step s changes it by s <grad, dir> up to s^2 and
+    # what fp32 sums of it are off by
+    g = _gen(3)
+    h, w, t = _operands(g, 30, 200, 64, torch.float32, gpu_device)
+    index, z = _lists(g, 30, 200, 6, gpu_device)
+    for call in (lambda a, b: linear_cross_entropy(a, b, t, reduction="sum"),
+                 lambda a, b: linear_distillation(a, b, index, z, temperature=2.0, reduction="sum")):
+        if dtype == torch.bfloat16:
+            continue  # bf16 operands cannot take a small step; the products are the fp32 path's
+        gh, gw = torch.autograd.grad(call(h, w), [h, w])
+        for x, grad, place in ((h, gh, 0), (w, gw, 1)):
+            d = torch.randn(x.shape, generator=g).to(gpu_device)
+            s = 2.0 ** -8 / float(d.norm())
+            args = [h.detach(), w.detach()]
+            args[place] = x.detach() + s * d
+            up = float(call(*args).double())
+            args[place] = x.detach() - s * d
+            down = float(call(*args).double())
+            slope = (up - down) / (2 * s)
+            # third-order term of 30 rows whose logits move by s |d_t| |w_v| (at most 2^-8 * 16 here), and fp32 sums
+            tol = 30 * (2.0 ** -8 * 16) ** 3 / s + abs(up) * 64 * U / s
+            assert abs(slope - float((grad.double() * d.double()).sum())) <= tol
+
+
+def test_streams_and_two_calls_at_once(gpu_device):
+    g = _gen(11)
+    cases = []
+    for T, V, D in ((300, 2000, 128), (40, 3000, 256)):
+        h, w, t = _operands(g, T, V, D, torch.bfloat16, gpu_device)
+        cases.append((h, w, t, *torch.autograd.grad(linear_cross_entropy(h, w, t), [h, w])))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = []
+    for _ in range(3):
+        for s, (h, w, t, _, _) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                outs.append(torch.autograd.grad(linear_cross_entropy(h, w, t), [h, w]))
+    torch.cuda.synchronize()
+    for i, (gh, gw) in enumerate(outs):
+        assert torch.equal(gh, cases[i % 2][3]) and torch.equal(gw, cases[i % 2][4])
+
+
+@pytest.mark.parametrize("T", [20, 500])
+def test_captured_and_replayed(gpu_device, T):
+    # a step of embedding and loss, forward and backward, in a graph; new tokens written into its inputs
+    g = _gen(T)
+    V, D = 800, 128
+    w = torch.randn(V, D, generator=g).to(gpu_device, torch.bfloat16).requires_grad_(True)
+    ids = torch.randint(0, V, (T,), generator=g).to(gpu_device)
+    t = torch.randint(0, V, (T,), generator=g).to(gpu_device)
+    index, z = _lists(g, T, V, 5, gpu_device)
+
+    def step(ids, t, index, z):
+        # the weight of this step alone: no graph of an earlier step shares its leaf
+        leaf = w.detach().requires_grad_(True)
+        x = embedding(ids, leaf, 2.0)
+        loss = linear_cross_entropy(x, leaf, t) + linear_distillation(x, leaf, index, z)
+        return loss.detach(), *torch.autograd.grad(loss, [leaf])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(ids, t, index, z)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(ids, t, index, z)
+    for rep in range(4):
+        new_ids = torch.randint(0, V, (T,), generator=g).to(gpu_device)
+        new_t = torch.randint(0, V, (T,), generator=g).to(gpu_device)
+        new_t[:rep * 3] = -100
+        ids.copy_(new_ids)
+        t.copy_(new_t)
+        z.add_(0.5 * torch.randn(z.shape, generator=g).to(gpu_device))
+        graph.replay()
+        got = [x.clone() for x in out]
+        torch.cuda.synchronize()
+        want = step(ids, t, index, z)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
+
+
+def test_compiled(gpu_device):
+    torch.manual_seed(0)
+    w = torch.randn(300, 64, device=gpu_device, dtype=torch.bfloat16, requires_grad=True)
+    ids = torch.randint(0, 300, (2, 30), device=gpu_device)
+    z = torch.randn(2, 30, 4, device=gpu_device)
+    index = torch.randint(0, 300, (2, 30, 4), device=gpu_device)
+
+    def step(ids, w):
+        x = embedding(ids, w, 3.0, padding_idx=1)
+        return linear_cross_entropy(x, w, ids) + linear_distillation(x, w, index, z, reduction="none").sum()
+
+    want = torch.autograd.grad(step(ids, w), [w])[0]
+    loss = torch.compile(step, fullgraph=True, backend="aot_eager")(ids, w)
+    assert torch.equal(loss, step(ids, w)) and torch.equal(torch.autograd.grad(loss, [w])[0], want)
+
+
+def test_second_derivatives_are_refused(gpu_device):
+    h, w, t = _operands(_gen(0), 8, 50, 64, torch.float32, gpu_device)
+    gh, = torch.autograd.grad(linear_cross_entropy(h, w, t), [h], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        gh.sum().backward()
+    gw, = torch.autograd.grad(embedding(t, w).pow(2).sum(), [w], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        gw.sum().backward()
+
+
+def test_wrappers_give_the_native_calls_results(gpu_device):
+    # the path of per-entry-point timing
+    from fusionllm_amd import _kernels as K
+    g = _gen(9)
+    h, w, t = _operands(g, 70, 300, 96, torch.bfloat16, gpu_device)
+    index, z = _lists(g, 70, 300, 9, gpu_device)
+
+    def step():
+        loss = linear_cross_entropy(h, w, t) + linear_distillation(h, w, index, z)
+        y = embedding(t, w, 2.0)
+        return loss, *torch.autograd.grad(loss + y.float().sum(), [h, w])
+
+    want = step()
+    times = {}
+    K.set_timer(times)
+    try:
+        got = step()
+    finally:
+        K.set_timer(None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert {"embedding_fwd", "embedding_bwd", "vocab_loss_fwd", "vocab_loss_bwd"} <= set(times)
+
+
+def test_long_offsets(gpu_device):
+    # a weight of more than 2^31 elements (rows at offsets beyond 32 bits), few of them used
+    V, D = 1 << 20, 2064
+    w = torch.zeros(V, D, device=gpu_device, dtype=torch.bfloat16)
+    ids = torch.tensor([0, V - 1, V - 2, V // 2, V - 1], device=gpu_device)
+    rows = torch.randn(5, D, generator=_gen(1)).to(gpu_device, torch.bfloat16)
+    rows[4] = rows[1]
+    w[ids] = rows
+    assert torch.equal(embedding(ids, w, 1.0), rows)
+    w.requires_grad_(True)
+    dw, = torch.autograd.grad(embedding(ids, w, 1.0), [w], rows)
+    assert torch.equal(dw[V - 1], (2 * rows[1].float()).bfloat16()) and torch.equal(dw[V // 2], rows[3])
+    assert int(dw.count_nonzero(dim=1).count_nonzero()) == 4
+    # the other rows' logits are zero: lse and its gradients in closed form
+    h = (rows * 0.05).detach().requires_grad_(True)
+    loss = linear_cross_entropy(h, w, ids, reduction="none")
+    s = h.detach().double() @ w.detach()[ids[:4]].double().T
+    lse = torch.log(torch.exp(s).sum(1) + (V - 4))
+    want = lse - s.gather(1, torch.tensor([[0], [1], [2], [3], [1]], device=gpu_device))[:, 0]
+    torch.testing.assert_close(loss.detach().double(), want, rtol=0, atol=(D + V / 128 + 64) * 8 * U * 4)
+
+
+def test_a_training_step_from_tokens_to_loss(gpu_device):
+    # embedding -> norm, block and residual -> norm -> loss, tied weight, in this package's operators; against torch
+    # operations around the same block, whose own rounding both sides share
+    from fusionllm_amd import DeepSeekMoE, Embedding, configs, layer_norm, moe_residual
+    cfg = configs.C2
+    torch.manual_seed(2)
+    emb = Embedding(1000, cfg.dim, scale=cfg.dim ** 0.5).to(gpu_device, torch.bfloat16)
+    torch.nn.init.normal_(emb.weight, std=0.02)
+    block = DeepSeekMoE(cfg.moe_config())
+    block.load_state_dict({k: v.bfloat16() for k, v in configs.make_block(cfg, seed=1, tokens=8).state_dict().items()})
+    block = block.to(device=gpu_device, dtype=torch.bfloat16)
+    norm = torch.nn.RMSNorm(cfg.dim, eps=1e-6).to(gpu_device, torch.bfloat16)
+    ids = torch.randint(0, 1000, (3, 100), device=gpu_device)
+    target = ids.roll(-1, 1)
+    target[:, -1] = -100
+
+    x = moe_residual(emb(ids), norm, block)
+    hidden = layer_norm(x)
+    loss = linear_cross_entropy(hidden, emb.weight, target)
+    loss.backward()
+    got = emb.weight.grad.clone()
+    emb.weight.grad = None
+
+    y = torch.nn.functional.embedding(ids, emb.weight) * cfg.dim ** 0.5
+    hidden2 = layer_norm(moe_residual(y.bfloat16(), norm, block))
+    logits = hidden2.reshape(-1, cfg.dim).float() @ emb.weight.float().t()
+    ref = torch.nn.functional.cross_entropy(logits, target.flatten())
+    ref.backward()
+    want = emb.weight.grad
+    assert torch.equal(hidden, hidden2)
+    # both losses in fp32 of the same operands; gradients of bf16 roundings at a few places (G, d_hidden, d_weight)
+    assert abs(float(loss) - float(ref)) <= 2 * (cfg.dim + 64) * U * float(logits.abs().max() + 8)
+    assert float((got.float() - want.float()).norm()) <= 4 * 2.0 ** -8 * float(want.float().norm())

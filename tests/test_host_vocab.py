@@ -1,0 +1,257 @@
+"""CPU tests of the vocabulary operators' host side: declared symbols, argument checks before any GPU call,
+the refusals of the Python entry points, operator shapes, and the machine code."""
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import fusionllm_amd
+from fusionllm_amd import Embedding, _lib, embedding, linear_cross_entropy, linear_distillation
+from fusionllm_amd import _kernels as K
+
+ROOT = Path(__file__).resolve().parents[1]
+FAKE = 1 << 20  # a non-null address that is never dereferenced (rejected first)
+
+
+def test_library_exports_the_vocabulary_symbols():
+    lib = _lib.load()
+    text = (ROOT / "include" / "fusionvocab.h").read_text()
+    syms = set(re.findall(r"^\s*(?:int|size_t)\s+(fmoe_\w+)\(", text, re.M))
+    assert syms == set(_lib.VOCAB_SIGNATURES)
+    assert not syms & (set(_lib.SIGNATURES) | set(_lib.TRAIN_SIGNATURES))
+    for s in syms:
+        assert hasattr(lib, s), s
+
+
+def test_embedding_argument_errors_without_gpu():
+    lib = _lib.load()
+
+    def fwd(ids=FAKE, i64=1, w=FAKE, dt=1, ldw=64, T=4, V=10, d=64, y=FAKE):
+        return lib.fmoe_embedding_fwd(ids, i64, w, dt, ldw, T, V, d, 1.0, y, None)
+
+    assert fwd(T=-1) == 1 and fwd(V=0) == 1 and fwd(d=0) == 1 and fwd(i64=2) == 1
+    assert fwd(d=16385, ldw=1 << 20) == 2 and fwd(T=(1 << 24) + 1) == 2 and fwd(V=(1 << 24) + 1) == 2
+    assert fwd(ldw=63) == 2 and fwd(ldw=1 << 40) == 2
+    assert fwd(T=1 << 24, d=1024, ldw=1024) == 2 and fwd(V=1 << 24, d=1024, ldw=1024) == 2  # too many elements
+    assert fwd(dt=2) == 4 and fwd(ids=None) == 1 and fwd(w=None) == 1 and fwd(y=None) == 1
+    assert fwd(ids=FAKE + 4) == 3 and fwd(ids=FAKE + 2, i64=0) == 3 and fwd(w=FAKE + 2) == 3 and fwd(y=FAKE + 1, dt=0) == 3
+    assert fwd(T=0) == 0 and fwd(T=0, ids=None, w=None, y=None) == 0
+
+    size = lib.fmoe_embedding_bwd_workspace_bytes(4, 10, 64)
+
+    def bwd(ids=FAKE, i64=1, dy=FAKE, dyt=1, ld=64, T=4, V=10, d=64, pad=-1, dw=FAKE, dt=1, ws=FAKE, n=size):
+        return lib.fmoe_embedding_bwd(ids, i64, dy, dyt, ld, T, V, d, 1.0, pad, dw, dt, ws, n, None)
+
+    assert bwd(T=-1) == 1 and bwd(pad=10) == 1 and bwd(pad=-2) == 1 and bwd(dw=None) == 1 and bwd(dy=None) == 1
+    assert bwd(ld=63) == 2 and bwd(dyt=5) == 4 and bwd(dt=5) == 4
+    assert bwd(n=size - 1) == 6 and bwd(ws=None) == 6 and bwd(ws=FAKE + 16) == 3 and bwd(dw=FAKE + 2) == 3
+    # slot starts (512 slots and the end), sorted tokens, two partial rows a tile of 16
+    assert size == 513 * 4 // 256 * 256 + 256 + 256 + 2 * 64 * 4
+    assert lib.fmoe_embedding_bwd_workspace_bytes(-1, 10, 64) == lib.fmoe_embedding_bwd_workspace_bytes(4, 0, 64) == 0
+
+
+def test_loss_argument_errors_without_gpu():
+    lib = _lib.load()
+    state = lib.fmoe_vocab_loss_state_bytes(4, 64, 1, 1)
+    fws = lib.fmoe_vocab_loss_fwd_workspace_bytes(4, 64, 100, 1, 0)
+    bws = lib.fmoe_vocab_loss_bwd_workspace_bytes(4, 64, 100, 1, 0)
+    assert state > 0 and fws > 0 and bws > 0
+
+    def fwd(h=FAKE, ht=0, ldh=64, w=FAKE, wt=0, ldw=64, i=FAKE, i64=1, t=None, tt=1, T=4, d=64, V=100, top=1,
+            scale=1.0, temp=1.0, planes=1, red=1, loss=FAKE, st=FAKE, sn=state, ws=FAKE, wn=fws):
+        return lib.fmoe_vocab_loss_fwd(h, ht, ldh, w, wt, ldw, i, i64, t, tt, T, d, V, top, -100, scale, temp, planes,
+                                       red, loss, st, sn, ws, wn, None)
+
+    assert fwd(T=-1) == 1 and fwd(d=0) == 1 and fwd(V=0) == 1 and fwd(top=0) == 1 and fwd(red=3) == 1 and fwd(planes=2) == 1
+    assert fwd(temp=0.0) == 1 and fwd(temp=float("nan")) == 1 and fwd(temp=2.0) == 1 and fwd(i64=-1) == 1
+    assert fwd(top=5) == 1  # a list without a teacher
+    assert fwd(d=16385, ldh=1 << 15, ldw=1 << 15) == 2 and fwd(top=1025, t=FAKE) == 2 and fwd(V=(1 << 24) + 1) == 2
+    assert fwd(ldh=63) == 2 and fwd(ldw=63) == 2 and fwd(ldw=1 << 22) == 2
+    assert fwd(ht=2) == 4 and fwd(wt=2) == 4 and fwd(t=FAKE, tt=7) == 4 and fwd(planes=3) == 4
+    assert fwd(planes=3, ht=1) == 4 and fwd(planes=3, wt=1) == 4
+    assert fwd(h=None) == 1 and fwd(w=None) == 1 and fwd(i=None) == 1 and fwd(loss=None) == 1
+    assert fwd(h=FAKE + 1) == 3 and fwd(w=FAKE + 1) == 3 and fwd(i=FAKE + 4) == 3 and fwd(loss=FAKE + 2) == 3
+    assert fwd(st=FAKE + 8) == 3 and fwd(ws=FAKE + 8) == 3
+    assert fwd(sn=state - 1) == 6 and fwd(wn=fws - 1) == 6 and fwd(st=None) == 6 and fwd(ws=None) == 6
+
+    def bwd(dl=FAKE, w=FAKE, wt=0, ldw=64, T=4, d=64, V=100, top=1, dis=0, temp=1.0, planes=1, red=1, st=FAKE, sn=state,
+            dh=FAKE, dht=0, dw=FAKE, dwt=0, ws=FAKE, wn=bws):
+        return lib.fmoe_vocab_loss_bwd(dl, w, wt, ldw, T, d, V, top, dis, 1.0, temp, planes, red, st, sn, dh, dht, dw, dwt,
+                                       ws, wn, None)
+
+    assert bwd(T=-1) == 1 and bwd(top=2) == 1 and bwd(dis=2) == 1 and bwd(temp=2.0) == 1 and bwd(red=-1) == 1
+    assert bwd(dl=None) == 1 and bwd(w=None) == 1
+    assert bwd(ldw=10) == 2 and bwd(wt=3) == 4 and bwd(dht=3) == 4 and bwd(dwt=3) == 4 and bwd(planes=3) == 4
+    assert bwd(dl=FAKE + 2) == 3 and bwd(dh=FAKE + 1) == 3 and bwd(dw=FAKE + 1) == 3 and bwd(st=FAKE + 4) == 3
+    assert bwd(sn=state - 1) == 6 and bwd(wn=bws - 1) == 6 and bwd(ws=None) == 6
+    assert bwd(dh=None, dw=None) == 0  # nothing wanted
+    for a in [(-1, 64, 1, 1), (4, 0, 1, 1), (4, 64, 0, 1), (4, 64, 1, 2), (4, 64, 1025, 1)]:
+        assert lib.fmoe_vocab_loss_state_bytes(*a) == 0
+
+
+def test_state_size_is_the_librarys():
+    lib = _lib.load()
+    for a in [(0, 1, 1, 1), (1, 1, 1, 1), (5, 7, 3, 3), (64, 64, 64, 1), (65, 65, 1, 3), (16384, 768, 1, 1),
+              (4096, 2048, 1000, 3)]:
+        assert lib.fmoe_vocab_loss_state_bytes(*a) == K.vocab_loss_state_bytes(*a), a
+
+
+def test_workspaces_stay_bounded():
+    # no logits: a piece of the vocabulary in bf16 (1 GiB), partial tiles (256 MiB), the sum of d_hidden between pieces
+    lib = _lib.load()
+    n = lib.fmoe_vocab_loss_bwd_workspace_bytes(32768, 2048, 131072, 1, 0)
+    assert n <= (1 << 30) + (1 << 28) + 32768 * 2048 * 4 + 1024
+    assert n < 32768 * 131072 * 2 // 4
+    # the forward's: a maximum and a sum per row and 128 columns
+    assert lib.fmoe_vocab_loss_fwd_workspace_bytes(32768, 2048, 131072, 1, 0) <= 32768 * 1024 * 8 + (1 << 18)
+    # rows that the products read as they lie
+    assert lib.fmoe_vocab_loss_packs(FAKE, 0, 128, 128, 1) == 0
+    for w, dt, ld, d, planes in [(FAKE + 2, 0, 128, 128, 1), (FAKE, 1, 128, 128, 1), (FAKE, 0, 129, 128, 1),
+                                 (FAKE, 0, 128, 100, 1), (FAKE, 1, 128, 128, 3)]:
+        assert lib.fmoe_vocab_loss_packs(w, dt, ld, d, planes) == 1
+
+
+def test_embedding_refusals():
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        embedding(torch.zeros(3, dtype=torch.long), torch.randn(4, 64))
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        Embedding(10, 64)(torch.zeros(3, dtype=torch.long))
+    for bad in (dict(max_norm=1.0), dict(scale_grad_by_freq=True), dict(sparse=True)):
+        with pytest.raises(NotImplementedError, match="max_norm"):
+            Embedding(10, 64, **bad)
+    with FakeTensorMode():
+        w = torch.empty(10, 64, device="cuda")
+        ids = torch.empty(3, dtype=torch.long, device="cuda")
+        with pytest.raises(ValueError, match=r"\[vocab, dim\]"):
+            embedding(ids, w[0])
+        with pytest.raises(ValueError, match=r"\[vocab, dim\]"):
+            embedding(ids, w[:0])
+        with pytest.raises(NotImplementedError, match="16384"):
+            embedding(ids, torch.empty(2, 16385, device="cuda"))
+        with pytest.raises(NotImplementedError, match="bf16 and fp32"):
+            embedding(ids, w.half())
+        with pytest.raises(ValueError, match="int32 or int64"):
+            embedding(ids.float(), w)
+        with pytest.raises(RuntimeError, match="weight's device"):
+            embedding(torch.empty(3, dtype=torch.long), w)
+        for pad in (10, -11):
+            with pytest.raises(ValueError, match="padding_idx"):
+                embedding(ids, w, padding_idx=pad)
+
+
+def test_loss_refusals():
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        linear_cross_entropy(torch.randn(3, 64), torch.randn(10, 64), torch.zeros(3, dtype=torch.long))
+    with FakeTensorMode():
+        h, w = torch.empty(2, 3, 64, device="cuda"), torch.empty(10, 64, device="cuda")
+        t = torch.empty(2, 3, dtype=torch.long, device="cuda")
+        index = torch.empty(2, 3, 5, dtype=torch.long, device="cuda")
+        z = torch.empty(2, 3, 5, device="cuda")
+        for call in (lambda h=h, w=w, **k: linear_cross_entropy(h, w, t, **k),
+                     lambda h=h, w=w, **k: linear_distillation(h, w, index, z, **k)):
+            with pytest.raises(ValueError, match="columns"):
+                call(h[..., :63])
+            with pytest.raises(RuntimeError, match="one dtype"):
+                call(h.bfloat16())
+            with pytest.raises(NotImplementedError, match="bf16 and fp32"):
+                call(h.half())
+            with pytest.raises(NotImplementedError, match="bf16 and fp32"):
+                call(h, w.double())
+            with pytest.raises(RuntimeError, match="device"):
+                call(torch.empty(2, 3, 64))
+            with pytest.raises(ValueError, match="reduction"):
+                call(reduction="batchmean")
+            for bad in (float("inf"), float("nan")):
+                with pytest.raises(ValueError, match="logit_scale"):
+                    call(logit_scale=bad)
+        with pytest.raises(ValueError, match="shape"):
+            linear_cross_entropy(h, w, t[0])
+        with pytest.raises(ValueError, match="int32 or int64"):
+            linear_cross_entropy(h, w, t.float())
+        with pytest.raises(ValueError, match="shape"):
+            linear_distillation(h, w, index[0], z[0])
+        with pytest.raises(ValueError, match="teacher_logits"):
+            linear_distillation(h, w, index, z[..., :4])
+        with pytest.raises(NotImplementedError, match="bf16 and fp32"):
+            linear_distillation(h, w, index, z.half())
+        with pytest.raises(NotImplementedError, match="1024"):
+            linear_distillation(h, w, index[..., :0], z[..., :0])
+        with pytest.raises(NotImplementedError, match="1024"):
+            linear_distillation(h, w, t[..., None].expand(2, 3, 1025), z[..., :1].expand(2, 3, 1025))
+        with pytest.raises(NotImplementedError, match="teacher"):
+            linear_distillation(h, w, index, z.requires_grad_(True))
+        for bad in (0.0, -1.0, float("inf"), float("nan")):
+            with pytest.raises(ValueError, match="temperature"):
+                linear_distillation(h, w, index, z.detach(), temperature=bad)
+
+
+def test_embedding_module_has_torchs_interface():
+    a, b = Embedding(12, 8, padding_idx=2, scale=3.0), torch.nn.Embedding(12, 8, padding_idx=2)
+    assert isinstance(a, torch.nn.Embedding) and a.scale == 3.0 and a.padding_idx == 2
+    assert not a.weight[2].any() and "scale=3.0" in repr(a)
+    assert {k: tuple(v.shape) for k, v in a.state_dict().items()} == {
+        k: tuple(v.shape) for k, v in b.state_dict().items()}
+    c = Embedding.from_pretrained(b.weight.detach(), freeze=False)
+    assert torch.equal(c.weight, b.weight) and c.scale == 1.0
+    assert fusionllm_amd.Embedding is Embedding
+
+
+def test_operator_fake_shapes():
+    with FakeTensorMode():
+        w = torch.empty(10, 64, device="cuda", dtype=torch.bfloat16)
+        ids = torch.empty(7, dtype=torch.long, device="cuda")
+        y = torch.ops.fusionllm.embedding_fwd(ids, w, 1.0, -1)
+        assert (y.shape, y.dtype) == ((7, 64), torch.bfloat16)
+        dw = torch.ops.fusionllm.embedding_bwd(ids, y, 10, 1.0, -1)
+        assert (dw.shape, dw.dtype) == ((10, 64), torch.bfloat16)
+        for reduction, shape in (("mean", ()), ("none", (7,))):
+            loss, state = torch.ops.fusionllm.vocab_loss_fwd(y, w, ids[:, None], None, -100, 1.0, 1.0, 1, reduction)
+            assert (loss.shape, loss.dtype) == (shape, torch.float32)
+            assert state.shape == (K.vocab_loss_state_bytes(7, 64, 1, 1),)
+            dh, dw = torch.ops.fusionllm.vocab_loss_bwd(loss, y, w, state, 1, False, 1.0, 1.0, 1, reduction)
+            assert (dh.shape, dw.shape, dh.dtype) == ((7, 64), (10, 64), torch.bfloat16)
+
+
+def _objects():
+    from fusionllm_amd import build
+    return [build.BUILD_DIR / "vocab_loss.o", build.BUILD_DIR / "embedding.o"]
+
+
+def test_vocabulary_kernels_read_no_register_a_load_is_still_filling():
+    # The products issue their global -> LDS copies and their MFMAs from inline assembly with explicit waits.
+    from tests import isa_check as ic
+    objs = _objects()
+    if not (ic.ROCM_LLVM / "llvm-objdump").exists() or not all(o.exists() for o in objs):
+        pytest.skip("no built objects or no llvm-objdump")
+    checked = 0
+    for o in objs:
+        n, hazards = ic.check_object(o)
+        assert not hazards, "\n".join(hazards[:10])
+        checked += n
+    assert checked >= 30
+
+
+def test_vocabulary_kernels_keep_their_values_in_registers(tmp_path):
+    from tests import isa_check as ic
+    if not ic.ROCM_LLVM.exists() or not all(o.exists() for o in _objects()):
+        pytest.skip("no built objects or no LLVM tools here")
+    seen = 0
+    for obj in _objects():
+        work = tmp_path / obj.stem
+        work.mkdir()
+        shutil.copy(obj, work / obj.name)
+        subprocess.run([str(ic.ROCM_LLVM / "llvm-objdump"), "--offloading", obj.name], check=True, capture_output=True,
+                       cwd=work)
+        dev = next(p for p in work.iterdir() if "gfx950" in p.name)
+        notes = subprocess.run([str(ic.ROCM_LLVM / "llvm-readelf"), "--notes", str(dev)], check=True,
+                               capture_output=True, text=True).stdout
+        for entry in notes.split("  - .agpr_count:")[1:]:
+            name = re.search(r"\.name:\s+(\S+)", entry).group(1)
+            seen += 1
+            assert re.search(r"\.private_segment_fixed_size:\s*0\s", entry), name
+            assert re.search(r"\.vgpr_spill_count:\s*0\s", entry), name
+    assert seen >= 30
