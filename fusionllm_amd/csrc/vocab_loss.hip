@@ -1231,26 +1231,13 @@ __device__ __forceinline__ float vl_block_sum(float v, float* red) {
 
 template <int DT>
 __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
-  extern __shared__ float h[];
   __shared__ float red[4], tq[FMOE_VOCAB_MAX_TOP];
   __shared__ int ti[FMOE_VOCAB_MAX_TOP];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x;
   if (row >= a.head[0]) return;
-  const int D = a.rows.D, Dp = a.rows.Dp, top = a.top;
+  const int D = a.rows.D, top = a.top;
+  const uint16_t* h = a.h + static_cast<int64_t>(row) * a.rows.Dp;
   const bool round = DT == FMOE_F32 && a.planes == 1;
-  for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
-    float v[8];
-    const uint16_t* p = a.h + static_cast<int64_t>(row) * Dp + c;
-    unpack8(*reinterpret_cast<const uint4*>(p), v);
-    for (int q = 1; q < a.planes; ++q) {
-      float u[8];
-      unpack8(*reinterpret_cast<const uint4*>(p + q * a.h_plane), u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] + u[e];  // exact: the parts of one fp32 number
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[c + e] = v[e];
-  }
   // the list: thread i has entries i, i + 256, ...
   constexpr int E = FMOE_VOCAB_MAX_TOP / 256;
   const int64_t list = static_cast<int64_t>(a.perm[row]) * top, out = static_cast<int64_t>(row) * top;
@@ -1324,8 +1311,13 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
       float hv[8], v[U][8];
 #pragma unroll
       for (int u = 0; u < U; ++u) load_upto8<DT>(a.weight, at[u] + c, on[u] ? D - c : 0, v[u]);
+      unpack8(*reinterpret_cast<const uint4*>(h + c), hv);
+      for (int q = 1; q < a.planes; ++q) {
+        float x[8];
+        unpack8(*reinterpret_cast<const uint4*>(h + q * a.h_plane + c), x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hv[e] = h[c + e];
+        for (int e = 0; e < 8; ++e) hv[e] = hv[e] + x[e];  // exact: the parts of one fp32 number
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -1603,9 +1595,8 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
     else vl_stat_kernel<4><<<dim3(static_cast<uint32_t>(ceil_div(T, 4))), 1024, 0, s>>>(l);
     if (distill) {
       const dim3 grid(static_cast<uint32_t>(T));
-      const size_t lds = st.Dp * 4;
-      if (w_dtype == FMOE_BF16) vl_list_kernel<FMOE_BF16><<<grid, 256, lds, s>>>(l);
-      else vl_list_kernel<FMOE_F32><<<grid, 256, lds, s>>>(l);
+      if (w_dtype == FMOE_BF16) vl_list_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(l);
+      else vl_list_kernel<FMOE_F32><<<grid, 256, 0, s>>>(l);
     }
   }
   if (reduction != FMOE_REDUCE_NONE) vl_sum_kernel<<<1, 1024, 0, s>>>(st.head, l.row_loss, reduction, loss);
