@@ -798,6 +798,68 @@ def vocab_loss_bwd(d_loss, weight, state, rows: int, top: int, distill: bool, lo
     return dh, dw
 
 
+def vocab_loss_takes_gradients(rows: int, dim: int, vocab: int, planes: int, packs: bool) -> bool:
+    """Whether vocab_loss_fwd_grad takes these sizes: arithmetic alone, for traced calls (csrc/vocab_loss.hip,
+    vl_fused_piece)."""
+    wide, tall, cols = (vocab + 255) // 256 * 256, (rows + 255) // 256 * 256, (dim + 63) // 64 * 64
+    if rows <= 64 or vocab > 1 << 22 or (packs and wide * cols * 2 * planes > 1 << 31):
+        return False
+    most = (1 << 30) // (wide * 2 * planes) // 256 * 256
+    return most >= tall or (most >= 2048 and vocab * cols * 4 <= 1 << 31)
+
+
+def vocab_loss_packs(weight, planes: int) -> bool:
+    """Whether the products read a copy of weight."""
+    return bool(_lib.load().fmoe_vocab_loss_packs(weight.data_ptr(), _dtype_code(weight.dtype), weight.stride(0),
+                                                  weight.shape[1], planes))
+
+
+@_timed
+def vocab_loss_fwd_grad(hidden, weight, index, teacher, ignore_index: int, logit_scale: float, temperature: float,
+                        planes: int, reduction: str, need_h: bool, need_w: bool):
+    """vocab_loss_fwd of reduction mean or sum and its gradients for d_loss = 1: loss, d_hidden, d_weight (None where
+    not wanted)."""
+    lib = _lib.load()
+    hp, ldh = _row_stride(hidden, "hidden")
+    wp, ldw = _row_stride(weight, "weight")
+    ip, i64 = _index(index, "index")
+    (T, d), V = hidden.shape, weight.shape[0]
+    if weight.shape[1] != d:
+        raise RuntimeError(f"weight must have {d} columns (got {tuple(weight.shape)})")
+    if index.dim() != 2 or index.shape[0] != T or (teacher is not None and teacher.shape != index.shape):
+        raise RuntimeError(f"index and teacher must be [{T}, top]")
+    top = index.shape[1]
+    dev = hidden.device
+    h_code, w_code = _dtype_code(hidden.dtype), _dtype_code(weight.dtype)
+    n_ws = lib.fmoe_vocab_loss_grad_workspace_bytes(T, d, V, top, planes,
+                                                    lib.fmoe_vocab_loss_packs(wp, w_code, ldw, d, planes))
+    ws = torch.empty(max(n_ws, 256), dtype=torch.uint8, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    dh = torch.empty(T, d, dtype=hidden.dtype, device=dev) if need_h else None
+    dw = torch.empty(V, d, dtype=weight.dtype, device=dev) if need_w else None
+    check(lib.fmoe_vocab_loss_fwd_grad(hp, h_code, ldh, wp, w_code, ldw, ip, i64,
+                                       None if teacher is None else _req(teacher, "teacher"),
+                                       F32 if teacher is None else _dtype_code(teacher.dtype), T, d, V, top,
+                                       ignore_index, logit_scale, temperature, planes, REDUCTIONS[reduction],
+                                       loss.data_ptr(), _ptr(dh), h_code, _ptr(dw), w_code, ws.data_ptr(), n_ws,
+                                       _stream()), "fmoe_vocab_loss_fwd_grad")
+    return loss, dh, dw
+
+
+@_timed
+def scale(factor, src, dst=None):
+    """factor (one fp32 value) times src, into dst (default: a new tensor; src itself: in place)."""
+    lib = _lib.load()
+    sp = _req(src, "src")
+    if dst is None:
+        dst = torch.empty_like(src)
+    if factor.numel() != 1 or dst.shape != src.shape:
+        raise RuntimeError("factor must hold one value, and dst have src's shape")
+    check(lib.fmoe_scale(_req(factor, "factor", torch.float32), sp, _req(dst, "dst", src.dtype), _dtype_code(src.dtype),
+                         src.numel(), _stream()), "fmoe_scale")
+    return dst
+
+
 CAST_MAX_TENSORS = 64
 
 

@@ -103,6 +103,11 @@ VOCAB_SIGNATURES = {
     "fmoe_vocab_loss_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
     "fmoe_vocab_loss_bwd": (c_int, [_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_double,
                                     c_double, c_int, c_int, _P, c_size_t, _P, c_int, _P, c_int, _P, c_size_t, _P]),
+    "fmoe_vocab_loss_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "fmoe_vocab_loss_fwd_grad": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int, c_int64, c_int64,
+                                         c_int64, c_int64, c_int64, c_double, c_double, c_int, c_int, _P, _P, c_int,
+                                         _P, c_int, _P, c_size_t, _P]),
+    "fmoe_scale": (c_int, [_P, _P, _P, c_int, c_int64, _P]),
 }
 
 _lock = threading.Lock()

@@ -16,6 +16,7 @@
 // wrappers took 15 us more of host time for a forward and 60 - 90 for a forward and
 // backward pass, whose kernels take 40 us at 16384 x 768).
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -41,7 +42,8 @@ using at::Tensor;
   F(fmoe_layer_norm_fwd) F(fmoe_layer_norm_bwd_workspace_bytes) F(fmoe_layer_norm_bwd)                   \
   F(fmoe_embedding_fwd) F(fmoe_embedding_bwd_workspace_bytes) F(fmoe_embedding_bwd)                       \
   F(fmoe_vocab_loss_state_bytes) F(fmoe_vocab_loss_packs) F(fmoe_vocab_loss_fwd_workspace_bytes)          \
-  F(fmoe_vocab_loss_fwd) F(fmoe_vocab_loss_bwd_workspace_bytes) F(fmoe_vocab_loss_bwd)
+  F(fmoe_vocab_loss_fwd) F(fmoe_vocab_loss_bwd_workspace_bytes) F(fmoe_vocab_loss_bwd)                    \
+  F(fmoe_vocab_loss_grad_workspace_bytes) F(fmoe_vocab_loss_fwd_grad) F(fmoe_scale)
 struct Api {
 #define F(name) decltype(&::name) name = nullptr;
   FMOE_ENTRY_POINTS(F)
@@ -584,11 +586,85 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
   }
 };
 
+// Gradients formed in the forward (loss of one value): their scaling by the loss's gradient.  In place, where
+// this backward pass is the only one (it frees the graph); nothing is touched where the factor is 1.
+Tensor scaled(const Tensor& factor, const Tensor& g, bool in_place) {
+  const Tensor f = factor.contiguous();
+  Tensor out = in_place ? g : at::empty_like(g);
+  check(api.fmoe_scale(static_cast<const float*>(f.data_ptr()), g.data_ptr(), out.data_ptr(), dtype_code(g.scalar_type()),
+                       g.numel(), current_stream(g)),
+        "fmoe_scale");
+  return out;
+}
+
+struct ScaledGradients : torch::autograd::Function<ScaledGradients> {
+  static variable_list forward(AutogradContext*, const Tensor& d_loss, const OptTensor& dh, const OptTensor& dw) {
+    variable_list out;
+    for (const OptTensor* g : {&dh, &dw})
+      if (g->has_value()) out.push_back(scaled(d_loss, **g, false));
+    return out;
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    throw std::runtime_error("fusionllm_amd losses over the vocabulary: second derivatives are not implemented");
+  }
+};
+
+struct VocabLossGrad : torch::autograd::Function<VocabLossGrad> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& index,
+                        const OptTensor& teacher, const LossOptions& o, size_t workspace_bytes) {
+    const c10::DeviceGuard guard(weight.device());
+    const Tensor h = norm_rows(hidden), w = norm_rows(weight), z = vector_or_none(teacher);
+    const int64_t T = h.size(0), d = h.size(1), V = w.size(0);
+    const int hc = dtype_code(h.scalar_type()), wc = dtype_code(w.scalar_type());
+    const Workspace ws(workspace_bytes, h);
+    Tensor loss = empty({}, at::kFloat, h), dh, dw;
+    if (hidden.requires_grad()) dh = empty({T, d}, h.scalar_type(), h);
+    if (weight.requires_grad()) dw = empty({V, d}, w.scalar_type(), h);
+    check(api.fmoe_vocab_loss_fwd_grad(h.data_ptr(), hc, h.stride(0), w.data_ptr(), wc, w.stride(0), index.data_ptr(),
+                                       index64(index), ptr_or_null(z), z.defined() ? dtype_code(z.scalar_type()) : FMOE_F32,
+                                       T, d, V, index.size(1), o.ignore_index, o.logit_scale, o.temperature,
+                                       static_cast<int>(o.planes), static_cast<int>(o.reduction),
+                                       static_cast<float*>(loss.data_ptr()), ptr_or_null(dh), hc, ptr_or_null(dw), wc,
+                                       ws.ptr(), ws.bytes, current_stream(h)),
+          "fmoe_vocab_loss_fwd_grad");
+    ctx->save_for_backward({dh, dw});
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(6);
+    variable_list saved = ctx->get_saved_variables();
+    const bool need[2] = {ctx->needs_input_grad(0) && saved[0].defined(), ctx->needs_input_grad(1) && saved[1].defined()};
+    if (!grads[0].defined() || !(need[0] || need[1])) return out;
+    const c10::DeviceGuard guard(grads[0].device());
+    if (at::GradMode::is_enabled()) {
+      auto opt = [&](int i) { return need[i] ? OptTensor(saved[i]) : OptTensor(); };
+      const variable_list g = ScaledGradients::apply(grads[0], opt(0), opt(1));
+      size_t k = 0;
+      for (int i = 0; i < 2; ++i)
+        if (need[i]) out[i] = g[k++];
+      return out;
+    }
+    const bool only = !torch::autograd::get_current_graph_task_keep_graph();
+    for (int i = 0; i < 2; ++i)
+      if (need[i]) out[i] = scaled(grads[0], saved[i], only);
+    return out;
+  }
+};
+
 // The loss of hidden [T, d] against weight [V, d] over index [T, top] (teacher: its logits, or none).
 Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& index, const OptTensor& teacher,
                   int64_t ignore_index, double logit_scale, double temperature, int64_t planes, int64_t reduction,
                   bool grad) {
   const LossOptions o{ignore_index, logit_scale, temperature, planes, reduction};
+  if (grad && reduction != FMOE_REDUCE_NONE) {
+    need_entry_points();
+    const c10::DeviceGuard guard(weight.device());
+    const int p = static_cast<int>(planes);
+    const Tensor w = norm_rows(weight);
+    const int packs = api.fmoe_vocab_loss_packs(w.data_ptr(), dtype_code(w.scalar_type()), w.stride(0), w.size(1), p);
+    const size_t n = api.fmoe_vocab_loss_grad_workspace_bytes(hidden.size(0), w.size(1), w.size(0), index.size(1), p, packs);
+    if (n > 0) return VocabLossGrad::apply(hidden, w, index, teacher, o, n);
+  }
   if (grad) return VocabLoss::apply(hidden, weight, index, teacher, o);
   const c10::DeviceGuard guard(weight.device());
   return loss_fwd(norm_rows(hidden), norm_rows(weight), index, vector_or_none(teacher), o)[0];

@@ -8,10 +8,12 @@
 //   G[r, v] = w[r] * (p[r, v] - q[r, v]),  dH = G W,  dW = G^T H
 // with q the row's target distribution: 1 at the target, or the teacher's softmax over its list.
 //
-// The logits [rows, vocab] are never stored: a tile's are reduced to a maximum and a sum of
-// exponentials per row (forward), or turned into G (backward), a piece of the vocabulary at a time.
-// That costs one product more than keeping them would (8 instead of 6 T V d flops), and
-// bounds the extra memory by a piece.  All four products are bound by the matrix units and run on
+// The logits [rows, vocab] are never stored.  A call whose loss is one value (mean or sum), for training, forms
+// its gradients at once (vl_fused, below): a piece of the rows at a time, whose exponentials 2^(t - o) are G
+// up to a factor per row, which is known when the piece's logits are done.  A call with a loss per row, whose weights
+// only the backward brings, reduces a tile's logits to a maximum and a sum of exponentials per row, and forms
+// them again in the backward, a piece of the vocabulary at a time: one product more (8 instead of
+// 6 T V d flops).  Either way the extra memory is bounded by a piece.  All products are bound by the matrix units and run on
 // the main loop of gemm_core.h: 256 x 256 tiles, persistent workgroups, copies in one ring over all
 // of a workgroup's tiles.
 //
@@ -227,15 +229,18 @@ __global__ __launch_bounds__(256) void vl_pack_kernel(const void* src, int64_t l
 // GRAD   t = H W^T of a piece -> G
 // DH     G W of a piece, K split in ranges -> fp32 partial sums, added to the piece's before
 // DW     G^T H                -> the piece's rows of dW
+// PROB   t = H W^T            -> 2^(t - o), and its sum per row and 128 columns
 // H and G are row-major, so A is K-contiguous but for DW (G^T: read with transposing LDS reads), and B is
-// K-contiguous for STATS and GRAD, and read as it lies, transposing, for DH (W) and DW (H).
-enum VlMode { VL_STATS = 0, VL_GRAD = 1, VL_DH = 2, VL_DW = 3 };
+// K-contiguous for STATS, GRAD and PROB, and read as it lies, transposing, for DH (W) and DW (H).
+enum VlMode { VL_STATS = 0, VL_GRAD = 1, VL_DH = 2, VL_DW = 3, VL_PROB = 4 };
 
 struct VlGemm {
   const uint16_t *a, *b;
   int64_t a_plane, b_plane;
   int lda, ldb;
   const int* head;      // rows with entries
+  int row0, rows;       // the rows of this call: row0 .. row0 + rows - 1 of them (pointers to rows start at row0)
+  const int* only_if;   // nothing is done where it holds 0 (nullptr: always)
   int cols;             // STATS, GRAD: vocabulary rows of the piece; DH, DW: columns (Dp)
   int vocab;            // DH, DW: vocabulary rows of the piece
   int k;                // STATS, GRAD: K (Dp)
@@ -246,9 +251,10 @@ struct VlGemm {
   // STATS
   float2* part;         // [2 * column tiles][Tp]
   int64_t Tp;
+  const float* off;     // PROB: o
   // GRAD
   const float2* stat;
-  const float* d_loss;
+  const float* d_loss;  // (nullptr: 1)
   const int* perm;      // (and DH)
   float factor;
   int reduction;
@@ -258,8 +264,9 @@ struct VlGemm {
   // DH, DW: the result, out [.][D] of out_dtype; DH: in rows perm
   void* out;
   int D, out_dtype;
-  float* sum;           // DH: [Tp][Dp], the sum over the pieces before (add) and for those after (more)
+  float* sum;           // DH: [Tp][Dp], DW: [vocab][Dp], the sum over the pieces before (add) and for those after (more)
   int add, more;
+  const float* row_factor;  // DH: the rows' factors (nullptr: 1)
   float* split;         // fp32 partial tiles
 };
 
@@ -294,6 +301,11 @@ __device__ __forceinline__ VlSplit vl_split(int tiles, int units) {
   return best;
 }
 
+// Packed rows among the call's row0 .. row0 + rows - 1.
+__device__ __forceinline__ int vl_rows_here(const int* head, int row0, int rows) {
+  return __builtin_amdgcn_readfirstlane(max(0, min(head[0] - row0, rows)));
+}
+
 struct VlItem {
   int tm, tn, u0, un, slot;  // tile, K steps (of all passes), partial tile (-1: the tile is whole)
 };
@@ -307,17 +319,17 @@ __device__ __forceinline__ void vl_tile(int t, int tiles_m, int tiles_n, int& tm
   tn = __builtin_amdgcn_readfirstlane(col);
 }
 
-// 8 consecutive values of a row of the result; DH of several pieces: with the sum so far, or into it.
+// 8 consecutive values of a row of the result; of several pieces: with the sum so far, or into it.
 template <int MODE>
 __device__ __forceinline__ void vl_result8(const VlGemm& a, int n, int row, int col, float* v) {
-  if (MODE == VL_DW) {
-    if (row >= a.vocab || col >= a.D) return;
-    const int64_t o = static_cast<int64_t>(row) * a.D + col;
-    if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - col, v);
-    else store_upto8<FMOE_F32>(a.out, o, a.D - col, v);
-  } else {
-    if (row >= n || col >= a.D) return;
+  {
+    if (row >= (MODE == VL_DW ? a.vocab : n) || col >= a.D) return;
     float* const s = a.sum + static_cast<int64_t>(row) * a.cols + col;
+    if (MODE == VL_DH && a.row_factor) {
+      const float f = a.row_factor[row];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * f;
+    }
     if (a.add) {
       const f32x4 lo = *reinterpret_cast<const f32x4*>(s), hi = *reinterpret_cast<const f32x4*>(s + 4);
 #pragma unroll
@@ -328,7 +340,7 @@ __device__ __forceinline__ void vl_result8(const VlGemm& a, int n, int row, int 
       *reinterpret_cast<f32x4*>(s + 4) = f32x4{v[4], v[5], v[6], v[7]};
       return;
     }
-    const int64_t o = static_cast<int64_t>(a.perm[row]) * a.D + col;
+    const int64_t o = static_cast<int64_t>(MODE == VL_DW ? row : a.perm[row]) * a.D + col;
     if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - col, v);
     else store_upto8<FMOE_F32>(a.out, o, a.D - col, v);
   }
@@ -336,7 +348,7 @@ __device__ __forceinline__ void vl_result8(const VlGemm& a, int n, int row, int 
 
 // What a row's p - q are multiplied with.
 __device__ __forceinline__ float vl_row_weight(const float* d_loss, const int* perm, int reduction, int n, int row, float factor) {
-  const float up = reduction == FMOE_REDUCE_NONE ? d_loss[perm[row]] : d_loss[0];
+  const float up = d_loss == nullptr ? 1.0f : reduction == FMOE_REDUCE_NONE ? d_loss[perm[row]] : d_loss[0];
   return (reduction == FMOE_REDUCE_MEAN ? up / static_cast<float>(n) : up) * factor;
 }
 
@@ -410,17 +422,55 @@ __device__ __forceinline__ void vl_stats_epilogue(const VlGemm& a, f32x4 (&acc)[
   if (row < n) a.part[static_cast<int64_t>(piece) * a.Tp + row] = mine;
 }
 
-// Epilogue of GRAD: G, 16 rows at a time through the wave's LDS into 16-byte stores.  With one plane, 2^(t - m -
-// l) takes one multiply-add (m + l rounded: 2^-24 of some tens in the exponent, far below G's own half step of
-// 2^-8); with three, m is subtracted first.
+// 16 rows of G (block i of the accumulators) through the wave's LDS into 16-byte stores, plane by plane.
+template <int PLANES, bool FULL>
+__device__ __forceinline__ void vl_store_g(const VlGemm& a, f32x4 (&acc)[core::FN], uint8_t* ep, int np, int row, int col0,
+                                           int el) {
+  using namespace core;
+  const int er = el & 15, eg = el >> 4;
+#pragma unroll 1  // (three at once would spill)
+  for (int p = 0; p < PLANES; ++p) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int col = j * 16 + eg * 4;
+      uint2 u;
+      u.x = pack2(acc[j][0], acc[j][1]);
+      u.y = pack2(acc[j][2], acc[j][3]);
+      *reinterpret_cast<uint2*>(ep + er * 256 + ((((col >> 3) ^ er)) << 4) + (col & 7) * 2) = u;
+      if constexpr (PLANES > 1) {
+        acc[j][0] = acc[j][0] - __uint_as_float(u.x << 16);
+        acc[j][1] = acc[j][1] - __uint_as_float(u.x & 0xffff0000u);
+        acc[j][2] = acc[j][2] - __uint_as_float(u.y << 16);
+        acc[j][3] = acc[j][3] - __uint_as_float(u.y & 0xffff0000u);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    // uniform addresses, one offset per lane
+    uint8_t* const base = reinterpret_cast<uint8_t*>(a.g + p * a.g_plane + static_cast<int64_t>(row) * a.ldg + col0);
+    const uint32_t voff = static_cast<uint32_t>(eg * a.ldg + er * 8) * 2u;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int r = t * 4 + eg;
+      const uint4 v = *reinterpret_cast<const uint4*>(ep + r * 256 + ((er ^ r) << 4));
+      if (FULL || row + r < np)
+        *reinterpret_cast<uint4*>(base + static_cast<int64_t>(8 * t) * a.ldg + voff) = v;
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+  }
+}
+
+// Epilogue of GRAD.  With one plane, 2^(t - m - l) takes one multiply-add (m + l rounded: 2^-24 of some tens in
+// the exponent, far below G's own half step of 2^-8); with three, m is subtracted first.
 template <int PLANES, bool FULL>
 __device__ __forceinline__ void vl_grad_epilogue(const VlGemm& a, f32x4 (&acc)[core::FM][core::FN], uint8_t* ep, int n,
                                                  int np, int row0, int col0, int el) {
   using namespace core;
-  const int er = el & 15, eg = el >> 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     asm volatile("" ::: "memory");  // (the rows' values of all blocks at once would spill)
+    asm volatile("" : "+v"(el));
+    const int er = el & 15, eg = el >> 4;
     const int row = row0 + 16 * i + er;
     float2 ml = make_float2(0.0f, 0.0f);
     float up = 0.0f;
@@ -452,36 +502,49 @@ __device__ __forceinline__ void vl_grad_epilogue(const VlGemm& a, f32x4 (&acc)[c
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = at == 16 * j + 4 * eg + e ? v : acc[i][j][e];
     }
-#pragma unroll 1  // (three at once would spill)
-    for (int p = 0; p < PLANES; ++p) {
+    vl_store_g<PLANES, FULL>(a, acc[i], ep, np, row0 + 16 * i, col0, el);
+  }
+}
+
+// Epilogue of PROB: 2^(t - o), one multiply-add and one exponential an element, and its sum over the row's 128
+// columns (in fp32, before the elements are rounded).
+template <int PLANES, bool FULL>
+__device__ __forceinline__ void vl_prob_epilogue(const VlGemm& a, f32x4 (&acc)[core::FM][core::FN], uint8_t* ep, int n,
+                                                 int np, int row0, int col0, int piece, int el) {
+  using namespace core;
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int col = j * 16 + eg * 4;
-        uint2 u;
-        u.x = pack2(acc[i][j][0], acc[i][j][1]);
-        u.y = pack2(acc[i][j][2], acc[i][j][3]);
-        *reinterpret_cast<uint2*>(ep + er * 256 + ((((col >> 3) ^ er)) << 4) + (col & 7) * 2) = u;
-        if constexpr (PLANES > 1) {
-          acc[i][j][0] = acc[i][j][0] - __uint_as_float(u.x << 16);
-          acc[i][j][1] = acc[i][j][1] - __uint_as_float(u.x & 0xffff0000u);
-          acc[i][j][2] = acc[i][j][2] - __uint_as_float(u.y << 16);
-          acc[i][j][3] = acc[i][j][3] - __uint_as_float(u.y & 0xffff0000u);
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
-      // uniform addresses, one offset per lane
-      uint8_t* const base = reinterpret_cast<uint8_t*>(a.g + p * a.g_plane + static_cast<int64_t>(row0 + 16 * i) * a.ldg + col0);
-      const uint32_t voff = static_cast<uint32_t>(eg * a.ldg + er * 8) * 2u;
+  for (int i = 0; i < FM; ++i) {
+    asm volatile("" ::: "memory");  // (as in GRAD's)
+    asm volatile("" : "+v"(el));
+    const int er = el & 15, eg = el >> 4;
+    const int row = row0 + 16 * i + er;
+    const float off = row < n ? a.off[row] : 0.0f;
+    const int rel = row < n && a.index ? a.index[row] - (a.v0 + col0) : -1;
+    const bool here = rel >= 0 && rel < WTN && col0 + rel < a.cols;
+    if (__ballot(here) != 0) {  // the target's t
+      float t = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int r = t * 4 + eg;
-        const uint4 v = *reinterpret_cast<const uint4*>(ep + r * 256 + ((er ^ r) << 4));
-        if (FULL || row0 + 16 * i + r < np)
-          *reinterpret_cast<uint4*>(base + static_cast<int64_t>(8 * t) * a.ldg + voff) = v;
-      }
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("" ::: "memory");
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = rel == 16 * j + 4 * eg + e ? acc[i][j][e] : t;
+      if (here && ((rel >> 2) & 3) == eg) a.picked[row] = t * a.c;
     }
+    int lim = row < n ? a.cols - col0 - 4 * eg : 0;
+    asm volatile("" : "+v"(lim));
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.c, -off));
+        if constexpr (!FULL) x = 16 * j + e < lim ? x : 0.0f;
+        s = s + x;
+        acc[i][j][e] = x;
+      }
+    s = s + __shfl_xor(s, 16, 64);
+    s = s + __shfl_xor(s, 32, 64);
+    if (eg == 0 && row < n) a.part[static_cast<int64_t>(piece) * a.Tp + row] = make_float2(off, s);
+    vl_store_g<PLANES, FULL>(a, acc[i], ep, np, row0 + 16 * i, col0, el);
   }
 }
 
@@ -495,7 +558,9 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / WN, wn = w % WN;
   const uint32_t sbase = lds_addr(smem);
-  const int n = __builtin_amdgcn_readfirstlane(a.head[0]);
+  if (a.only_if && a.only_if[0] == 0) return;
+  const int n = vl_rows_here(a.head, a.row0, a.rows);
+  if (a.row0 > 0 && n == 0) return;
   const int np = pad_rows(n);
   const int m_rows = MODE == VL_DW ? a.vocab : np;
   const int tiles_m = (m_rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
@@ -733,6 +798,10 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       const int piece = (a.v0 / BN + t.tn) * WN + wn;
       if (col0 + WTN <= a.cols) vl_stats_epilogue<true>(a, acc, c, n, row0, col0, piece, el);
       else vl_stats_epilogue<false>(a, acc, c, n, row0, col0, piece, el);
+    } else if constexpr (MODE == VL_PROB) {
+      const int piece = (a.v0 / BN + t.tn) * WN + wn;
+      if (row0 + WTM <= n && col0 + WTN <= a.cols) vl_prob_epilogue<PLANES, true>(a, acc, ep, n, np, row0, col0, piece, el);
+      else vl_prob_epilogue<PLANES, false>(a, acc, ep, n, np, row0, col0, piece, el);
     } else if constexpr (MODE == VL_GRAD) {
       if (row0 + WTM <= n && col0 + WTN <= a.cols) vl_grad_epilogue<PLANES, true>(a, acc, ep, n, np, row0, col0, el);
       else vl_grad_epilogue<PLANES, false>(a, acc, ep, n, np, row0, col0, el);
@@ -775,7 +844,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     asm volatile("s_nop 1" ::: "memory");  // VALU writes -> MFMA reads of the accumulators
     if (++e_ti == my_items) break;
     e_left = locate(e_ti).un;
-    if constexpr (MODE == VL_GRAD) {
+    if constexpr (MODE == VL_GRAD || MODE == VL_PROB) {
       // formed again: kept across the epilogue they made it spill
       form_offsets(0);
       xa = frag_base(wm * WTM, el);
@@ -954,7 +1023,7 @@ __global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const T
     }
     multiply(f, full % STEPS);
   }
-  const int n = __builtin_amdgcn_readfirstlane(a.head[0]);
+  const int n = vl_rows_here(a.head, 0, kThinRows);
 
   // acc[m] of lane l: row 16 m + l % 16, columns col0 + 4 (l / 16) + 0..3
   const int lim = a.cols - col0 - 4 * eg;
@@ -1062,7 +1131,7 @@ void vl_thin(const VlGemm& a, const void* weight, int w_dtype, int64_t ldw, int6
 template <int MODE, int PLANES>
 __global__ __launch_bounds__(256) void vl_split_kernel(const VlGemm a, const int* inv, int T, int blocks) {
   using namespace core;
-  const int n = a.head[0];
+  const int n = vl_rows_here(a.head, a.row0, a.rows);
   if (MODE == VL_DH && static_cast<int>(blockIdx.x) >= blocks) {
     const int t0 = (blockIdx.x - blocks) * 64;
     float zero[8];
@@ -1078,6 +1147,7 @@ __global__ __launch_bounds__(256) void vl_split_kernel(const VlGemm a, const int
     }
     return;
   }
+  if (a.row0 > 0 && n == 0) return;
   const int np = pad_rows(n);
   const int m_rows = MODE == VL_DW ? a.vocab : np;
   const int tiles_m = (m_rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
@@ -1158,6 +1228,12 @@ struct LossArgs {
   int *out_index;     // distillation: of the packed rows
   float* out_q;
   RowsArgs rows;
+  int row0, n_rows;   // as in VlGemm
+  // gradients at once: o of the rows; distillation: the loss without ln 2 (m - o + l), over the temperature's square;
+  // set where a row's sum is not one that 2^(t - o) can stand for
+  float *off, *row_part;
+  int* flag;
+  const int* only_if;
 };
 
 __device__ __forceinline__ void vl_store_loss(const LossArgs& a, int row, float v) {
@@ -1171,7 +1247,8 @@ template <int R>
 __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
   __shared__ float2 red[16][R];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int n = a.head[0];
+  if (a.only_if && a.only_if[0] == 0) return;
+  const int n = vl_rows_here(a.head, a.row0, a.n_rows);
   const int row0 = blockIdx.x * R;
   if (row0 >= n) return;
   const int row = row0 + lane % R;
@@ -1206,8 +1283,13 @@ __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
       vl_store_loss(a, row, loss);
       a.picked[row] = expm1f(-loss);  // p - 1 (exact to its own size where p is near 1), for the backward
     }
+  } else if (a.row_part) {  // distillation whose lists were read before
+    const float part = a.row_part[row];
+    if (part != part) l = part;
+    vl_store_loss(a, row, fmaf((m - a.off[row]) + l, kLn2, part) * a.factor);
   }
   a.stat[row] = make_float2(m, l);
+  if (a.flag && !(s < 0x1p100f && s > 0x1p-100f)) a.flag[0] = 1;
 }
 
 // Distillation, a workgroup per packed row: the teacher's softmax over its list, t of the listed entries (a dot
@@ -1234,7 +1316,9 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
   __shared__ float red[4], tq[FMOE_VOCAB_MAX_TOP];
   __shared__ int ti[FMOE_VOCAB_MAX_TOP];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x;
-  if (row >= a.head[0]) return;
+  const bool early = a.row_part != nullptr;  // before the logits' statistics: o of the row, and its part of the loss
+  if (early && row == 0 && threadIdx.x == 0) a.flag[0] = 0;
+  if (row >= vl_rows_here(a.head, a.row0, a.n_rows)) return;
   const int D = a.rows.D, top = a.top;
   const uint16_t* h = a.h + static_cast<int64_t>(row) * a.rows.Dp;
   const bool round = DT == FMOE_F32 && a.planes == 1;
@@ -1292,8 +1376,8 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
     }
   }
   __syncthreads();
-  const float2 ml = a.stat[row];
-  float cross = 0.0f;
+  const float2 ml = early ? make_float2(0.0f, 0.0f) : a.stat[row];
+  float cross = 0.0f, most = -__builtin_inff();
   constexpr int U = 4;
   for (int k0 = w * U; k0 < top; k0 += 4 * U) {
     float acc[U][4];
@@ -1330,9 +1414,25 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
       for (int off = 32; off >= 1; off >>= 1) s = s + __shfl_xor(s, off, 64);
       if (!on[u]) continue;
       const float t = s * a.c, q = tq[k0 + u];
+      most = fmaxf(most, t);
       if (lane == 0) a.picked[out + k0 + u] = t;
       if (!(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
     }
+  }
+  if (early) {
+    // o: the largest listed t.  Sum of q (o - t), with o known only now
+    most = vl_block_max(most, red);
+    if (most == -__builtin_inff()) most = 0.0f;
+    __syncthreads();  // (picked, written by this workgroup's lanes 0)
+    cross = 0.0f;
+    for (int k = threadIdx.x; k < top; k += 256)
+      if (ti[k] >= 0 && !(tq[k] == 0.0f)) cross = fmaf(tq[k], most - a.picked[out + k], cross);
+    cross = vl_block_sum(cross, red);
+    if (threadIdx.x == 0) {
+      a.off[row] = most;
+      a.row_part[row] = row_bad ? __builtin_nanf("") : fmaf(cross, kLn2, ent);
+    }
+    return;
   }
   cross = vl_block_sum(lane == 0 ? cross : 0.0f, red);
   if (threadIdx.x == 0) {
@@ -1363,7 +1463,7 @@ __global__ __launch_bounds__(1024) void vl_sum_kernel(const int* head, const flo
   }
 }
 
-// ---- backward of distillation: the listed entries of G -----------------------------------------------
+// ---- the listed entries of G -----------------------------------------------
 
 struct FixArgs {
   const int *head, *perm, *index;
@@ -1374,23 +1474,130 @@ struct FixArgs {
   float factor;
   uint16_t* g;
   int64_t g_plane;
+  // gradients at once: p - q times 2^l, or by itself where flag is set; q nullptr: picked is p - 1
+  int row0, rows;
+  const int* flag;
 };
 
 // G at the entries that lie in this piece of the vocabulary: the row's weight times p - q in fp32, rounded once.
 __global__ __launch_bounds__(256) void vl_fix_kernel(const FixArgs a) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int n = a.head[0], row = static_cast<int>(i / a.top);
+  const int n = vl_rows_here(a.head, a.row0, a.rows), row = static_cast<int>(i / a.top);
   if (row >= n) return;
   const int id = a.index[i];
   if (id < a.v0 || id >= a.v1) return;
   const float2 ml = a.stat[row];
-  float v = (__builtin_amdgcn_exp2f((a.picked[i] - ml.x) - ml.y) - a.q[i]) *
-            vl_row_weight(a.d_loss, a.perm, a.reduction, n, row, a.factor);
+  float v = a.q ? __builtin_amdgcn_exp2f((a.picked[i] - ml.x) - ml.y) - a.q[i] : a.picked[i];
+  if (a.flag) v = a.flag[0] ? v : v * __builtin_amdgcn_exp2f(ml.y);
+  else v = v * vl_row_weight(a.d_loss, a.perm, a.reduction, n, row, a.factor);
   uint16_t* p = a.g + static_cast<int64_t>(row) * a.ldg + (id - a.v0);
   for (int k = 0; k < a.planes; ++k) {
     const uint16_t b = f2bf(v);
     p[k * a.g_plane] = b;
     v = v - bf2f(b);
+  }
+}
+
+// ---- gradients at once ---------------------------------------------------------------------------------
+// For a piece of the rows:  G' = 2^(t - o) (PROB, o: the target's t, or the largest listed one),  l = log2 of its
+// sum per row,  G'[r, listed] = 2^l (p - q),  f[r] = w[r] 2^-l,  dH = f (G' W),  dW += G'^T (f H).
+// bf16 has the exponents of fp32, so o need not be the maximum.  Where a row's sum leaves 2^-100 .. 2^100 all the
+// same (a loss of some 70), or is no number, the piece's flag is set, and STATS and GRAD form its statistics and G in
+// the ordinary way (with f[r] = w[r]); else those launches end at once.
+// f H is rounded once more (planes = 1: half a step of bf16 an element, as G).
+
+// o of cross entropy's rows, a wave each.
+template <int DT>
+__global__ __launch_bounds__(256) void vl_off_kernel(const LossArgs a) {
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.flag[0] = 0;
+  if (row >= vl_rows_here(a.head, a.row0, a.n_rows)) return;
+  const int id = __builtin_amdgcn_readfirstlane(a.index[row]);
+  const int D = a.rows.D;
+  const bool round = DT == FMOE_F32 && a.planes == 1;
+  const uint16_t* h = a.h + static_cast<int64_t>(row) * a.rows.Dp;
+  float acc = 0.0f;
+  for (int c = lane * 8; c < D; c += 512) {
+    float hv[8], v[8];
+    load_upto8<DT>(a.weight, static_cast<int64_t>(max(id, 0)) * a.ldw + c, D - c, v);
+    unpack8(*reinterpret_cast<const uint4*>(h + c), hv);
+    for (int q = 1; q < a.planes; ++q) {
+      float x[8];
+      unpack8(*reinterpret_cast<const uint4*>(h + q * a.h_plane + c), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hv[e] = hv[e] + x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf(round ? bf_round(v[e]) : v[e], hv[e], acc);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) acc = acc + __shfl_xor(acc, off, 64);
+  if (lane == 0) a.off[row] = id < 0 ? 0.0f : acc * a.c;
+}
+
+// f and f H of the piece's rows (zeros in the padding), a wave each.
+template <int PLANES>
+__global__ __launch_bounds__(256) void vl_factor_kernel(const int* head, int row0, int rows, const float2* stat,
+                                                        const int* flag, float factor, int mean, const uint16_t* h,
+                                                        int64_t h_plane, int Dp, float* row_factor, uint16_t* out,
+                                                        int64_t out_plane) {
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int n = vl_rows_here(head, row0, rows);
+  if (row >= pad_rows(n)) return;
+  float f = 0.0f;
+  if (row < n) {
+    f = mean ? factor / static_cast<float>(head[0]) : factor;
+    if (flag[0] == 0) f = f * __builtin_amdgcn_exp2f(-stat[row].y);
+    if (lane == 0) row_factor[row] = f;
+  }
+  for (int c = lane * 8; c < Dp; c += 512) {
+    const int64_t at = static_cast<int64_t>(row) * Dp + c;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row < n) {
+      unpack8(*reinterpret_cast<const uint4*>(h + at), v);
+#pragma unroll
+      for (int q = 1; q < PLANES; ++q) {
+        float x[8];
+        unpack8(*reinterpret_cast<const uint4*>(h + q * h_plane + at), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] + x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * f;
+    }
+    uint4 o[PLANES];
+    vl_split8<PLANES>(v, o);
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4*>(out + p * out_plane + at) = o[p];
+  }
+}
+
+// dW from the sum over the pieces.
+template <int DT>
+__global__ __launch_bounds__(256) void vl_dw_kernel(const float* sum, int64_t vocab, int D, int Dp, void* out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (v >= vocab) return;
+  for (int c = lane * 8; c < D; c += 512) {
+    float x[8];
+    load_upto8<FMOE_F32>(sum, v * Dp + c, 8, x);
+    store_upto8<DT>(out, v * D + c, D - c, x);
+  }
+}
+
+// dst = scale[0] * src; nothing where they are the same and scale[0] is 1.
+template <int DT>
+__global__ __launch_bounds__(256) void vl_scale_kernel(const float* scale, const void* src, void* dst, int64_t n) {
+  const float f = scale[0];
+  if (src == dst && f == 1.0f) return;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256 * 8;
+  for (int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; e < n; e += stride) {
+    const int k = static_cast<int>(min(n - e, int64_t(8)));
+    float v[8];
+    load_upto8<DT>(src, e, k, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] * f;
+    store_upto8<DT>(dst, e, k, v);
   }
 }
 
@@ -1484,6 +1691,128 @@ bool vl_dtype(int d) { return d == FMOE_BF16 || d == FMOE_F32; }
 // Workgroups of a product of so many tiles: one per CU, fewer only in eighths.
 dim3 vl_grid(int64_t items) { return dim3(static_cast<uint32_t>(std::min<int64_t>(kVlCus, ceil_div(items, 8) * 8))); }
 
+// The forward call's arguments.
+struct VlCall {
+  const void *hidden, *weight, *index, *teacher;
+  int h_dtype, w_dtype, index64, t_dtype;
+  int64_t ldh, ldw, T, dim, vocab, top, ignore_index;
+  double logit_scale, temperature;
+  int planes, reduction;
+  float* loss;
+  bool distill() const { return teacher != nullptr || top != 1; }
+};
+
+int vl_check(const VlCall& a, const void* state, const void* workspace) {
+  const bool distill = a.distill();
+  if (a.T < 0 || a.dim <= 0 || a.vocab <= 0 || a.top <= 0 || a.index64 < 0 || a.index64 > 1 || a.reduction < 0 ||
+      a.reduction > 2 || (a.planes != 1 && a.planes != 3) || !(a.temperature > 0.0) || (!distill && a.temperature != 1.0))
+    return FMOE_ERR_INVALID_ARG;
+  if (!vl_sizes_ok(a.T, a.dim, a.vocab, a.top, a.planes)) return FMOE_ERR_SHAPE;
+  if ((a.T > 1 && (a.ldh < a.dim || a.ldh > (int64_t(1) << 38))) ||
+      (a.vocab > 1 && (a.ldw < a.dim || a.ldw >= (int64_t(1) << 22))))
+    return FMOE_ERR_SHAPE;
+  if (!vl_dtype(a.h_dtype) || !vl_dtype(a.w_dtype) || (a.teacher && !vl_dtype(a.t_dtype)) ||
+      (a.planes == 3 && (a.h_dtype != FMOE_F32 || a.w_dtype != FMOE_F32)))
+    return FMOE_ERR_DTYPE;
+  if (a.weight == nullptr || a.loss == nullptr ||
+      (a.T > 0 && (a.hidden == nullptr || a.index == nullptr || (distill && a.teacher == nullptr))))
+    return FMOE_ERR_INVALID_ARG;
+  if (!vl_elem_aligned(a.hidden, a.h_dtype) || !vl_elem_aligned(a.weight, a.w_dtype) || !vl_elem_aligned(a.loss, FMOE_F32) ||
+      (a.teacher && !vl_elem_aligned(a.teacher, a.t_dtype)) ||
+      (reinterpret_cast<uintptr_t>(a.index) & (a.index64 ? 7u : 3u)) != 0 || !vl_ws_aligned(state) || !vl_ws_aligned(workspace))
+    return FMOE_ERR_ALIGN;
+  return FMOE_OK;
+}
+
+// Packs the rows with entries; the arguments for those that read lists later.
+RowsArgs vl_pack_rows(const VlCall& a, const VlState& st, uint32_t* masks, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(std::max<int64_t>(ceil_div(a.T, kRowBlock), 1)));
+  RowsArgs r{};
+  r.hidden = a.hidden, r.index = a.index, r.teacher = a.teacher, r.ldh = a.ldh, r.ignore = a.ignore_index;
+  r.index64 = a.index64, r.t_dtype = a.distill() ? a.t_dtype : -1;
+  r.T = static_cast<int>(a.T), r.D = static_cast<int>(a.dim), r.Dp = static_cast<int>(st.Dp), r.V = static_cast<int>(a.vocab);
+  r.top = static_cast<int>(a.top), r.plane = st.plane;
+  r.inv_temp = static_cast<float>(1.0 / a.temperature);
+  r.masks = a.T * a.top <= kFewEntries ? nullptr : masks;
+  r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.h = st.h;
+  r.loss = a.reduction == FMOE_REDUCE_NONE ? a.loss : nullptr;
+  if (r.masks) vl_mark_kernel<<<grid, 1024, 0, s>>>(r);
+  if (a.h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 1><<<grid, 1024, 0, s>>>(r);
+  else if (a.planes == 1) vl_rows_kernel<FMOE_F32, 1><<<grid, 1024, 0, s>>>(r);
+  else vl_rows_kernel<FMOE_F32, 3><<<grid, 1024, 0, s>>>(r);
+  return r;
+}
+
+// The statistics (and losses) of `rows` rows.
+void vl_stat(const LossArgs& l, int64_t rows, hipStream_t s) {
+  if (rows >= 8192) vl_stat_kernel<64><<<dim3(static_cast<uint32_t>(ceil_div(rows, 64))), 1024, 0, s>>>(l);
+  else if (rows >= 1024) vl_stat_kernel<16><<<dim3(static_cast<uint32_t>(ceil_div(rows, 16))), 1024, 0, s>>>(l);
+  else vl_stat_kernel<4><<<dim3(static_cast<uint32_t>(ceil_div(rows, 4))), 1024, 0, s>>>(l);
+}
+
+void vl_lists(const LossArgs& l, int w_dtype, int64_t rows, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>(rows));
+  if (w_dtype == FMOE_BF16) vl_list_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(l);
+  else vl_list_kernel<FMOE_F32><<<grid, 256, 0, s>>>(l);
+}
+
+// DH and DW with their split tiles; rest of DH's result (rows without entries) with its last piece.
+template <int MODE>
+void vl_product(const VlGemm& g, int planes, int64_t mt, int64_t nt, int64_t units, const int* inv, int64_t T, hipStream_t s) {
+  if (planes == 1) vl_gemm_kernel<MODE, 1><<<dim3(kVlCus), core::NT, 0, s>>>(g);
+  else vl_gemm_kernel<MODE, 3><<<dim3(kVlCus), core::NT, 0, s>>>(g);
+  // the split tiles' number depends on the rows with entries, which the host does not know
+  const int64_t passes = planes == 3 ? 6 : 1;
+  const int64_t blocks = units * passes < 16 ? 0 : std::min<int64_t>(mt * nt, kVlCus - 1) * 32;
+  const int64_t clear = MODE == VL_DH && inv ? ceil_div(T, 64) : 0;
+  if (blocks + clear == 0) return;
+  const dim3 grid(static_cast<uint32_t>(blocks + clear));
+  if (planes == 1) vl_split_kernel<MODE, 1><<<grid, 256, 0, s>>>(g, inv, static_cast<int>(T), static_cast<int>(blocks));
+  else vl_split_kernel<MODE, 3><<<grid, 256, 0, s>>>(g, inv, static_cast<int>(T), static_cast<int>(blocks));
+}
+
+// Gradients at once: rows of a piece, or 0 where that form is not taken.  It needs G of at least kFusedRows rows (or
+// all) within kPieceBytes, since every piece adds to all of dW (fp32: written and read once more a piece), a packed copy of
+// the whole weight where one is needed, and rows enough for the tiles.
+constexpr int64_t kFusedRows = 2048, kFusedBytes = int64_t(1) << 31;
+int64_t vl_fused_piece(int64_t T, int64_t D, int64_t V, int planes, bool packs) {
+  const int64_t Vp = ceil_div(V, 256) * 256, Tp = ceil_div(std::max<int64_t>(T, 1), 256) * 256;
+  if (T <= kThinRows || V > (int64_t(1) << 22) || (packs && Vp * pad64(D) * 2 * planes > kFusedBytes)) return 0;
+  const int64_t most = std::min(Tp, kPieceBytes / (Vp * 2 * planes) / 256 * 256);
+  if (most < std::min(Tp, kFusedRows) || (most < Tp && V * pad64(D) * 4 > kFusedBytes)) return 0;
+  const int64_t pieces = ceil_div(Tp, most);
+  return ceil_div(Tp / 256, pieces) * 256;
+}
+
+struct VlFusedSpace {
+  int64_t piece;
+  size_t state, masks, part, row_loss, row_part, off, factor, flag, g, fh, split, sum, pack, bytes = 0;
+  VlFusedSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
+      : piece(vl_fused_piece(T, D, V, planes, packs)) {
+    if (piece == 0) return;
+    auto take = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) & ~size_t(255);
+      return at;
+    };
+    const int64_t Dp = pad64(D), dt = ceil_div(Dp, 256), vt = ceil_div(V, 256), passes = planes == 3 ? 6 : 1;
+    state = take(VlState(nullptr, T, D, top, planes).bytes);
+    masks = take(ceil_div(T, kRowBlock) * 4);
+    part = take(2 * vt * piece * 8);
+    row_loss = take(T * 4);
+    row_part = take(piece * 4);
+    off = take(piece * 4);
+    factor = take(piece * 4);
+    flag = take(4);
+    g = take(piece * vt * 512 * planes);
+    fh = take(piece * Dp * 2 * planes);
+    split = take(std::max(vl_split_slots(piece / 256 * dt, ceil_div(V, 64) * passes),
+                          vl_split_slots(vt * dt, piece / 64 * passes)) * (core::BM * core::BN * 4));
+    sum = take(piece < T ? V * Dp * 4 : 0);
+    pack = take(packs ? V * Dp * 2 * planes : 0);
+  }
+};
+
 }  // namespace fmoe
 
 using namespace fmoe;
@@ -1510,23 +1839,10 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
                                    double logit_scale, double temperature, int planes, int reduction, float* loss,
                                    void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
                                    void* stream) {
-  const bool distill = teacher != nullptr || top != 1;
-  if (T < 0 || dim <= 0 || vocab <= 0 || top <= 0 || index64 < 0 || index64 > 1 || reduction < 0 || reduction > 2 ||
-      (planes != 1 && planes != 3) || !(temperature > 0.0) || (!distill && temperature != 1.0))
-    return FMOE_ERR_INVALID_ARG;
-  if (!vl_sizes_ok(T, dim, vocab, top, planes)) return FMOE_ERR_SHAPE;
-  if ((T > 1 && (ldh < dim || ldh > (int64_t(1) << 38))) || (vocab > 1 && (ldw < dim || ldw >= (int64_t(1) << 22))))
-    return FMOE_ERR_SHAPE;
-  if (!vl_dtype(h_dtype) || !vl_dtype(w_dtype) || (teacher && !vl_dtype(t_dtype)) ||
-      (planes == 3 && (h_dtype != FMOE_F32 || w_dtype != FMOE_F32)))
-    return FMOE_ERR_DTYPE;
-  if (weight == nullptr || (T > 0 && (hidden == nullptr || index == nullptr || (distill && teacher == nullptr))) ||
-      loss == nullptr)
-    return FMOE_ERR_INVALID_ARG;
-  if (!vl_elem_aligned(hidden, h_dtype) || !vl_elem_aligned(weight, w_dtype) || !vl_elem_aligned(loss, FMOE_F32) ||
-      (teacher && !vl_elem_aligned(teacher, t_dtype)) ||
-      (reinterpret_cast<uintptr_t>(index) & (index64 ? 7u : 3u)) != 0 || !vl_ws_aligned(state) || !vl_ws_aligned(workspace))
-    return FMOE_ERR_ALIGN;
+  const VlCall call{hidden, weight, index, teacher, h_dtype, w_dtype, index64, t_dtype, ldh, ldw, T, dim, vocab, top,
+                    ignore_index, logit_scale, temperature, planes, reduction, loss};
+  const bool distill = call.distill();
+  if (const int rc = vl_check(call, state, workspace); rc != FMOE_OK) return rc;
   const bool packs = vl_packs(weight, w_dtype, ldw, dim, planes);
   const VlFwdSpace space(T, dim, vocab, planes, packs);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1534,26 +1850,11 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   if (state == nullptr || state_bytes < st.bytes || workspace == nullptr || workspace_bytes < space.bytes)
     return FMOE_ERR_WORKSPACE;
   const hipStream_t s = as_stream(stream);
-  const int64_t blocks = std::max<int64_t>(ceil_div(T, kRowBlock), 1);
-
-  RowsArgs r{};
-  r.hidden = hidden, r.index = index, r.teacher = teacher, r.ldh = ldh, r.ignore = ignore_index;
-  r.index64 = index64, r.t_dtype = distill ? t_dtype : -1;
-  r.T = static_cast<int>(T), r.D = static_cast<int>(dim), r.Dp = static_cast<int>(st.Dp), r.V = static_cast<int>(vocab);
-  r.top = static_cast<int>(top), r.plane = st.plane;
-  r.inv_temp = static_cast<float>(1.0 / temperature);
-  r.masks = T * top <= kFewEntries ? nullptr : reinterpret_cast<uint32_t*>(ws + space.masks);
-  r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.h = st.h;
-  r.loss = reduction == FMOE_REDUCE_NONE ? loss : nullptr;
-  const dim3 rows_grid(static_cast<uint32_t>(blocks));
-  if (r.masks) vl_mark_kernel<<<rows_grid, 1024, 0, s>>>(r);
-  if (h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 1><<<rows_grid, 1024, 0, s>>>(r);
-  else if (planes == 1) vl_rows_kernel<FMOE_F32, 1><<<rows_grid, 1024, 0, s>>>(r);
-  else vl_rows_kernel<FMOE_F32, 3><<<rows_grid, 1024, 0, s>>>(r);
+  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), s);
 
   VlGemm g{};
   g.a = st.h, g.a_plane = st.plane, g.lda = static_cast<int>(st.Dp);
-  g.head = st.head, g.k = static_cast<int>(st.Dp);
+  g.head = st.head, g.rows = static_cast<int>(T), g.k = static_cast<int>(st.Dp);
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
   g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = st.Tp;
   g.index = distill ? nullptr : st.index, g.picked = st.picked;
@@ -1587,17 +1888,11 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   l.loss = r.loss;
   l.h = st.h, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
   l.top = distill ? static_cast<int>(top) : 0;
-  l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r;
+  l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r, l.n_rows = g.rows;
   l.factor = static_cast<float>(temperature * temperature);
   if (T > 0) {
-    if (T >= 8192) vl_stat_kernel<64><<<dim3(static_cast<uint32_t>(ceil_div(T, 64))), 1024, 0, s>>>(l);
-    else if (T >= 1024) vl_stat_kernel<16><<<dim3(static_cast<uint32_t>(ceil_div(T, 16))), 1024, 0, s>>>(l);
-    else vl_stat_kernel<4><<<dim3(static_cast<uint32_t>(ceil_div(T, 4))), 1024, 0, s>>>(l);
-    if (distill) {
-      const dim3 grid(static_cast<uint32_t>(T));
-      if (w_dtype == FMOE_BF16) vl_list_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(l);
-      else vl_list_kernel<FMOE_F32><<<grid, 256, 0, s>>>(l);
-    }
+    vl_stat(l, T, s);
+    if (distill) vl_lists(l, w_dtype, T, s);
   }
   if (reduction != FMOE_REDUCE_NONE) vl_sum_kernel<<<1, 1024, 0, s>>>(st.head, l.row_loss, reduction, loss);
   return launch_status();
@@ -1638,7 +1933,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
   for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
     const int64_t rows = std::min(piece, vocab - v0), vt = ceil_div(rows, 256);
     VlGemm g{};
-    g.head = st.head, g.Tp = st.Tp, g.perm = st.perm, g.D = static_cast<int>(dim);
+    g.head = st.head, g.rows = static_cast<int>(T), g.Tp = st.Tp, g.perm = st.perm, g.D = static_cast<int>(dim);
     g.split = reinterpret_cast<float*>(ws + space.split);
     const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ldw;
     int64_t w_plane = 0;
@@ -1661,7 +1956,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     if (distill && T > 0) {
       FixArgs f{};
       f.head = st.head, f.perm = st.perm, f.index = st.index, f.q = st.q, f.picked = st.picked, f.stat = st.stat;
-      f.d_loss = d_loss, f.top = static_cast<int>(top);
+      f.d_loss = d_loss, f.top = static_cast<int>(top), f.rows = g.rows;
       f.v0 = static_cast<int>(v0), f.v1 = static_cast<int>(v0 + rows), f.reduction = reduction, f.planes = planes;
       f.ldg = g.ldg, f.factor = g.factor, f.g = gbuf, f.g_plane = g_plane;
       vl_fix_kernel<<<dim3(static_cast<uint32_t>(ceil_div(T * top, 256))), 256, 0, s>>>(f);
@@ -1672,31 +1967,149 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     if (d_hidden != nullptr) {
       h.out = d_hidden, h.out_dtype = dh_dtype, h.sum = reinterpret_cast<float*>(ws + space.sum);
       h.add = v0 > 0, h.more = v0 + rows < vocab;
-      // the split tiles' number depends on the rows with entries, which the host does not know
-      const int64_t units = ceil_div(rows, 64) * (planes == 3 ? 6 : 1);
-      const int64_t blocks = units < 16 ? 0 : std::min<int64_t>(mt * dt, kVlCus - 1) * 32;
-      const int64_t clear = h.more ? 0 : ceil_div(T, 64);
-      const dim3 grid(static_cast<uint32_t>(blocks + clear));
-      if (planes == 1) vl_gemm_kernel<VL_DH, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
-      else vl_gemm_kernel<VL_DH, 3><<<dim3(kVlCus), core::NT, 0, s>>>(h);
-      if (blocks + clear > 0) {
-        const int b = static_cast<int>(blocks), t = static_cast<int>(T);
-        if (planes == 1) vl_split_kernel<VL_DH, 1><<<grid, 256, 0, s>>>(h, st.inv, t, b);
-        else vl_split_kernel<VL_DH, 3><<<grid, 256, 0, s>>>(h, st.inv, t, b);
-      }
+      vl_product<VL_DH>(h, planes, mt, dt, ceil_div(rows, 64), h.more ? nullptr : st.inv, T, s);
     }
     if (d_weight != nullptr) {
-      h.b = st.h, h.b_plane = st.plane, h.ldb = Dp;
+      h.b = st.h, h.b_plane = st.plane, h.ldb = Dp, h.add = h.more = 0;
       h.out = static_cast<uint8_t*>(d_weight) + v0 * dim * (dw_dtype == FMOE_BF16 ? 2 : 4), h.out_dtype = dw_dtype;
-      const int64_t units = st.Tp / 64 * (planes == 3 ? 6 : 1), rest = vt * dt % kVlCus;
-      if (planes == 1) vl_gemm_kernel<VL_DW, 1><<<dim3(kVlCus), core::NT, 0, s>>>(h);
-      else vl_gemm_kernel<VL_DW, 3><<<dim3(kVlCus), core::NT, 0, s>>>(h);
-      if (units >= 16 && rest > 0) {
-        const int b = static_cast<int>(rest * 32);
-        if (planes == 1) vl_split_kernel<VL_DW, 1><<<dim3(b), 256, 0, s>>>(h, nullptr, 0, b);
-        else vl_split_kernel<VL_DW, 3><<<dim3(b), 256, 0, s>>>(h, nullptr, 0, b);
-      }
+      vl_product<VL_DW>(h, planes, vt, dt, st.Tp / 64, nullptr, 0, s);
     }
   }
+  return launch_status();
+}
+
+extern "C" size_t fmoe_vocab_loss_grad_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes,
+                                                       int packs) {
+  return vl_sizes_ok(T, dim, vocab, top, planes) ? VlFusedSpace(T, dim, vocab, top, planes, packs).bytes : 0;
+}
+
+extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t ldh, const void* weight, int w_dtype,
+                                        int64_t ldw, const void* index, int index64, const void* teacher, int t_dtype,
+                                        int64_t T, int64_t dim, int64_t vocab, int64_t top, int64_t ignore_index,
+                                        double logit_scale, double temperature, int planes, int reduction, float* loss,
+                                        void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const VlCall call{hidden, weight, index, teacher, h_dtype, w_dtype, index64, t_dtype, ldh, ldw, T, dim, vocab, top,
+                    ignore_index, logit_scale, temperature, planes, reduction, loss};
+  const bool distill = call.distill();
+  if (const int rc = vl_check(call, nullptr, workspace); rc != FMOE_OK) return rc;
+  if (reduction == FMOE_REDUCE_NONE) return FMOE_ERR_INVALID_ARG;
+  if (!vl_dtype(dh_dtype) || !vl_dtype(dw_dtype)) return FMOE_ERR_DTYPE;
+  if (!vl_elem_aligned(d_hidden, dh_dtype) || !vl_elem_aligned(d_weight, dw_dtype)) return FMOE_ERR_ALIGN;
+  const bool packs = vl_packs(weight, w_dtype, ldw, dim, planes);
+  const VlFusedSpace space(T, dim, vocab, top, planes, packs);
+  if (space.piece == 0) return FMOE_ERR_SHAPE;
+  if (workspace == nullptr || workspace_bytes < space.bytes) return FMOE_ERR_WORKSPACE;
+  const hipStream_t s = as_stream(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const VlState st(ws + space.state, T, dim, top, planes);
+  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), s);
+
+  const int Dp = static_cast<int>(st.Dp);
+  const int64_t piece = space.piece, vt = ceil_div(vocab, 256), dt = ceil_div(st.Dp, 256), mt = piece / 256;
+  const int64_t g_plane = piece * vt * 256, fh_plane = piece * st.Dp;
+  uint16_t* const gbuf = reinterpret_cast<uint16_t*>(ws + space.g);
+  uint16_t* const fh = reinterpret_cast<uint16_t*>(ws + space.fh);
+  float* const factor = reinterpret_cast<float*>(ws + space.factor);
+  int* const flag = reinterpret_cast<int*>(ws + space.flag);
+  const uint16_t* w = static_cast<const uint16_t*>(weight);
+  int64_t w_plane = 0;
+  int w_ld = static_cast<int>(ldw);
+  if (packs) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(ws + space.pack);
+    const int rc = vl_pack(weight, w_dtype, ldw, 0, vocab, dim, planes, dst, vocab * st.Dp, s);
+    if (rc != FMOE_OK) return rc;
+    w = dst, w_plane = vocab * st.Dp, w_ld = Dp;
+  }
+  for (int64_t r0 = 0; r0 < std::max<int64_t>(T, 1); r0 += piece) {
+    const int64_t rows = std::min(piece, T - r0);
+    VlGemm g{};
+    g.head = st.head, g.row0 = static_cast<int>(r0), g.rows = static_cast<int>(rows);
+    g.a = st.h + r0 * st.Dp, g.a_plane = st.plane, g.lda = Dp, g.k = Dp;
+    g.b = w, g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(vocab);
+    g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
+    g.index = distill ? nullptr : st.index + r0, g.picked = st.picked + r0 * top;
+    g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = piece;
+    g.off = reinterpret_cast<float*>(ws + space.off);
+    g.stat = st.stat + r0, g.perm = st.perm + r0, g.factor = 1.0f, g.reduction = FMOE_REDUCE_SUM;
+    g.g = gbuf, g.g_plane = g_plane, g.ldg = static_cast<int>(vt * 256);
+    g.D = static_cast<int>(dim), g.split = reinterpret_cast<float*>(ws + space.split);
+
+    LossArgs l{};
+    l.head = st.head, l.row0 = g.row0, l.n_rows = g.rows, l.perm = g.perm, l.index = st.index + r0;
+    l.part = g.part, l.Tp = piece, l.pieces = static_cast<int>(2 * vt), l.stat = st.stat + r0, l.picked = g.picked;
+    l.row_loss = reinterpret_cast<float*>(ws + space.row_loss) + r0;
+    l.h = g.a, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
+    l.top = distill ? static_cast<int>(top) : 0;
+    l.planes = planes, l.c = g.c, l.out_index = st.index + r0 * top, l.out_q = st.q + r0 * top, l.rows = r;
+    l.factor = static_cast<float>(temperature * temperature);
+    l.off = reinterpret_cast<float*>(ws + space.off), l.flag = flag;
+    if (distill) l.row_part = reinterpret_cast<float*>(ws + space.row_part);
+
+    const dim3 grid = vl_grid(mt * vt);
+    if (distill) vl_lists(l, w_dtype, std::max<int64_t>(rows, 1), s);
+    else if (w_dtype == FMOE_BF16) vl_off_kernel<FMOE_BF16><<<dim3(static_cast<uint32_t>(ceil_div(std::max<int64_t>(rows, 1), 4))), 256, 0, s>>>(l);
+    else vl_off_kernel<FMOE_F32><<<dim3(static_cast<uint32_t>(ceil_div(std::max<int64_t>(rows, 1), 4))), 256, 0, s>>>(l);
+    if (planes == 1) vl_gemm_kernel<VL_PROB, 1><<<grid, core::NT, 0, s>>>(g);
+    else vl_gemm_kernel<VL_PROB, 3><<<grid, core::NT, 0, s>>>(g);
+    vl_stat(l, std::max<int64_t>(rows, 1), s);
+    // the ordinary way, where a row asks for it
+    VlGemm q = g;
+    LossArgs lq = l;
+    q.only_if = lq.only_if = flag;
+    lq.flag = nullptr;
+    if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(q);
+    else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(q);
+    vl_stat(lq, std::max<int64_t>(rows, 1), s);
+    q.index = nullptr;  // (the listed entries follow)
+    if (planes == 1) vl_gemm_kernel<VL_GRAD, 1><<<grid, core::NT, 0, s>>>(q);
+    else vl_gemm_kernel<VL_GRAD, 3><<<grid, core::NT, 0, s>>>(q);
+
+    FixArgs f{};
+    f.head = st.head, f.index = l.out_index, f.q = distill ? l.out_q : nullptr, f.picked = g.picked, f.stat = g.stat;
+    f.top = static_cast<int>(top), f.v1 = static_cast<int>(vocab), f.planes = planes, f.ldg = g.ldg, f.g = gbuf;
+    f.g_plane = g_plane, f.row0 = g.row0, f.rows = g.rows, f.flag = flag;
+    if (rows > 0) vl_fix_kernel<<<dim3(static_cast<uint32_t>(ceil_div(rows * top, 256))), 256, 0, s>>>(f);
+    const float fac = static_cast<float>(temperature * logit_scale);  // temperature^2 times d t / d logit
+    const dim3 wave_rows(static_cast<uint32_t>(ceil_div(pad64(std::max<int64_t>(rows, 1)), 4)));
+    if (planes == 1)
+      vl_factor_kernel<1><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
+                                                   g.a, st.plane, Dp, factor, fh, fh_plane);
+    else
+      vl_factor_kernel<3><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
+                                                   g.a, st.plane, Dp, factor, fh, fh_plane);
+    VlGemm h = g;
+    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg, h.cols = Dp, h.vocab = static_cast<int>(vocab);
+    if (d_hidden != nullptr) {
+      h.out = d_hidden, h.out_dtype = dh_dtype, h.row_factor = factor;
+      // (rows without entries: once)
+      vl_product<VL_DH>(h, planes, mt, dt, ceil_div(vocab, 64), r0 + piece >= T ? st.inv : nullptr, T, s);
+    }
+    if (d_weight != nullptr) {
+      h.b = fh, h.b_plane = fh_plane, h.ldb = Dp, h.out = d_weight, h.out_dtype = dw_dtype;
+      h.sum = reinterpret_cast<float*>(ws + space.sum), h.add = r0 > 0, h.more = piece < T;
+      vl_product<VL_DW>(h, planes, vt, dt, ceil_div(rows, 64), nullptr, 0, s);
+    }
+  }
+  if (d_weight != nullptr && piece < T) {
+    const dim3 grid(static_cast<uint32_t>(ceil_div(vocab, 4)));
+    const float* sum = reinterpret_cast<const float*>(ws + space.sum);
+    const int d = static_cast<int>(dim);
+    if (dw_dtype == FMOE_BF16) vl_dw_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(sum, vocab, d, Dp, d_weight);
+    else vl_dw_kernel<FMOE_F32><<<grid, 256, 0, s>>>(sum, vocab, d, Dp, d_weight);
+  }
+  vl_sum_kernel<<<1, 1024, 0, s>>>(st.head, reinterpret_cast<const float*>(ws + space.row_loss), reduction, loss);
+  return launch_status();
+}
+
+extern "C" int fmoe_scale(const float* scale, const void* src, void* dst, int dtype, int64_t n, void* stream) {
+  if (n < 0) return FMOE_ERR_INVALID_ARG;
+  if (!vl_dtype(dtype)) return FMOE_ERR_DTYPE;
+  if (n == 0) return FMOE_OK;
+  if (scale == nullptr || src == nullptr || dst == nullptr) return FMOE_ERR_INVALID_ARG;
+  if (!vl_elem_aligned(scale, FMOE_F32) || !vl_elem_aligned(src, dtype) || !vl_elem_aligned(dst, dtype)) return FMOE_ERR_ALIGN;
+  const dim3 grid(static_cast<uint32_t>(std::min<int64_t>(ceil_div(n, 2048), 2048)));
+  if (dtype == FMOE_BF16) vl_scale_kernel<FMOE_BF16><<<grid, 256, 0, as_stream(stream)>>>(scale, src, dst, n);
+  else vl_scale_kernel<FMOE_F32><<<grid, 256, 0, as_stream(stream)>>>(scale, src, dst, n);
   return launch_status();
 }

@@ -27,6 +27,10 @@ dw3, dw2] in the inputs' dtypes.
 ``fusionllm::layer_norm_fwd`` / ``layer_norm_bwd`` do the same for ``layer_norm``:
 outputs y [T,d] (out_dtype), mean [T] and rstd [T] fp32; gradients [dx, dw, db],
 without those of a weight or bias that is not there.
+
+``fusionllm::embedding_fwd`` / ``embedding_bwd`` and the losses over a vocabulary:
+``vocab_loss_fwd`` (loss, the state for the backward) / ``vocab_loss_bwd`` (d_hidden, d_weight),
+and ``vocab_loss_fwd_grad`` (loss, and the gradients that are wanted, formed at once) with ``scale``.
 """
 from __future__ import annotations
 
@@ -293,3 +297,48 @@ def _vocab_loss_backward(ctx, d_loss, *unused):
 
 
 vocab_loss_fwd.register_autograd(_vocab_loss_backward, setup_context=_vocab_loss_setup)
+
+
+@torch.library.custom_op("fusionllm::vocab_loss_fwd_grad", mutates_args=())
+def vocab_loss_fwd_grad(hidden: Tensor, weight: Tensor, index: Tensor, teacher: Tensor | None, ignore_index: int,
+                        logit_scale: float, temperature: float, planes: int, reduction: str, need_h: bool,
+                        need_w: bool) -> list[Tensor]:
+    _norm.refuse_tangents("fusionllm::vocab_loss_fwd_grad", hidden, weight)
+    with _norm._on_device(weight):
+        out = K.vocab_loss_fwd_grad(_norm._rows(hidden), _norm._rows(weight), index, teacher, ignore_index, logit_scale,
+                                    temperature, planes, reduction, need_h, need_w)
+    return [t for t in out if t is not None]
+
+
+@vocab_loss_fwd_grad.register_fake
+def _(hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction, need_h, need_w):
+    out = [hidden.new_empty((), dtype=torch.float32)]
+    return out + ([hidden.new_empty(hidden.shape)] if need_h else []) + ([weight.new_empty(weight.shape)] if need_w else [])
+
+
+@torch.library.custom_op("fusionllm::scale", mutates_args=())
+def scale(factor: Tensor, src: Tensor) -> Tensor:
+    with _norm._on_device(src):
+        return K.scale(factor.contiguous(), src)
+
+
+@scale.register_fake
+def _(factor, src):
+    return torch.empty_like(src)
+
+
+def _vocab_loss_grad_setup(ctx, inputs, output):
+    ctx.need = inputs[-2:]
+    ctx.save_for_backward(*output[1:])
+
+
+def _vocab_loss_grad_backward(ctx, d_outs):
+    d_loss = d_outs[0]
+    if d_loss is None:
+        return (None,) * 11
+    grads = iter(ctx.saved_tensors)
+    dh, dw = (torch.ops.fusionllm.scale(d_loss, next(grads)) if need else None for need in ctx.need)
+    return dh, dw, *(None,) * 9
+
+
+vocab_loss_fwd_grad.register_autograd(_vocab_loss_grad_backward, setup_context=_vocab_loss_grad_setup)

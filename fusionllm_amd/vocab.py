@@ -7,8 +7,11 @@ the tokens by id and adds each id's rows in fp32 in a fixed order: the same
 bits every run, no atomics.
 
 The losses are those of the logits ``s = logit_scale * hidden @ weight.T``,
-which are never stored: the forward reduces them tile by tile, the backward
-forms them again, a piece of the vocabulary at a time.  Rows without a target
+which are never stored.  A loss of one value (mean, sum) that needs gradients forms them in
+its forward, a piece of the rows at a time (up to 1 GiB), and its backward scales
+them by the loss's gradient.  A loss per row (none), and one of up to 64 rows or of a vocabulary too
+large for such pieces, reduces the logits tile by tile in the forward and forms
+them again in the backward.  Rows without a target
 (``ignore_index``) are left out of every product.
 
     linear_cross_entropy   -log softmax(s)[target]
@@ -18,7 +21,8 @@ forms them again, a piece of the vocabulary at a time.  Rows without a target
 
 hidden and weight are both bf16 (bf16 products, fp32 sums) or both fp32 (fp32 precision throughout);
 under bf16 autocast either may be either, and both are taken as bf16.  Losses
-are fp32, gradients have their operand's dtype.  ROCm tensors only.
+are fp32, gradients have their operand's dtype.  fp32 operands that hold infinities may give NaN
+where sums of infinities would be infinite.  ROCm tensors only.
 """
 from __future__ import annotations
 
@@ -153,6 +157,34 @@ class _VocabLossFunction(torch.autograd.Function):
         return dh, dw, None, None, None, None, None, None, None
 
 
+class _VocabLossGradFunction(torch.autograd.Function):
+    """A loss of one value whose gradients are formed in the forward, through the Python wrappers."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction):
+        with _on_device(weight):
+            loss, dh, dw = K.vocab_loss_fwd_grad(_rows(hidden), _rows(weight), index, teacher, ignore_index, logit_scale,
+                                                 temperature, planes, reduction, *ctx.needs_input_grad[:2])
+        ctx.save_for_backward(dh, dw)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_loss):
+        grads = []
+        for g, need in zip(ctx.saved_tensors, ctx.needs_input_grad):
+            with _on_device(d_loss):
+                grads.append(K.scale(d_loss.contiguous(), g) if need else None)
+        return *grads, None, None, None, None, None, None, None
+
+
+def _gradients_at_once(flat, weight, planes, reduction):
+    """Whether the forward forms the gradients.  A contiguous copy of a weight that is none starts at an aligned
+    address."""
+    return reduction != "none" and K.vocab_loss_takes_gradients(
+        flat.shape[0], flat.shape[1], weight.shape[0], planes, K.vocab_loss_packs(_rows(weight), planes))
+
+
 def _check_loss(what, hidden, weight, reduction, logit_scale):
     """Checks the operands; the planes of the products (1: bf16, 3: fp32)."""
     _check_weight(what, weight)
@@ -185,7 +217,13 @@ def _vocab_loss(what, hidden, weight, index, teacher, ignore_index, logit_scale,
         teacher = teacher.detach().reshape(index.shape).contiguous()
     args = (flat, weight, index, teacher, int(ignore_index), float(logit_scale), float(temperature), planes, reduction)
     if torch.compiler.is_compiling():
-        loss = torch.ops.fusionllm.vocab_loss_fwd(*args)[0]
+        # (the traced form sees no addresses: a weight as it lies in a module)
+        packs = planes != 1 or weight.dtype != torch.bfloat16 or weight.shape[1] % 64 != 0 or not weight.is_contiguous()
+        if (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) and reduction != "none" and
+                K.vocab_loss_takes_gradients(flat.shape[0], flat.shape[1], weight.shape[0], planes, packs)):
+            loss = torch.ops.fusionllm.vocab_loss_fwd_grad(*args, hidden.requires_grad, weight.requires_grad)[0]
+        else:
+            loss = torch.ops.fusionllm.vocab_loss_fwd(*args)[0]
     else:
         refuse_tangents(what, hidden, weight)
         grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
@@ -193,7 +231,9 @@ def _vocab_loss(what, hidden, weight, index, teacher, ignore_index, logit_scale,
         if host is not None:
             loss = host.vocab_loss(*args[:-1], K.REDUCTIONS[reduction], grad)
         elif grad:
-            loss = _VocabLossFunction.apply(*args)
+            with _on_device(weight):
+                at_once = _gradients_at_once(flat, weight, planes, reduction)
+            loss = (_VocabLossGradFunction if at_once else _VocabLossFunction).apply(*args)
         else:
             with _on_device(weight):
                 loss = K.vocab_loss_fwd(_rows(flat), _rows(weight), *args[2:])[0]

@@ -56,7 +56,7 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  * (NaN where there are none) or their sum.
  *
  * The rows with entries are packed, and tiles of the logits are formed on the matrix units, reduced to
- * a maximum and a sum of exponentials per row and dropped; the backward forms them again, a piece
+ * a maximum and a sum of exponentials per row and dropped; fmoe_vocab_loss_bwd forms them again, a piece
  * of the vocabulary at a time, as G = (p - q) times the row's weight, and multiplies
  *   d_hidden = G weight,  d_weight = G^T hidden.
  * planes = 1: operands and G are bf16 (fp32 operands are rounded), sums fp32.  planes = 3: fp32
@@ -89,6 +89,25 @@ int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int w_dtype, in
                         double temperature, int planes, int reduction, const void* state,
                         size_t state_bytes, void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype,
                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* The forward and the gradients of a loss of one value (mean or sum, for d_loss = 1) in one call, without
+ * forming the logits twice: a piece of the rows at a time, whose exponentials 2^(s - o), o the logit of the row's
+ * target (or the largest listed one), are G up to a factor per row.  Those factors go into d_hidden, and with hidden into
+ * the product of d_weight: with planes = 1 the scaled hidden states are rounded to bf16 once more.  Rows whose
+ * sum of such exponentials leaves 2^-100 .. 2^100 (or is no number) make their piece be formed in the ordinary way.
+ * d_hidden and d_weight as in fmoe_vocab_loss_bwd.  The size query returns 0 where this form is not taken (up to 64
+ * rows; vocabularies of which no piece of 2048 rows fits 1 GiB): FMOE_ERR_SHAPE.  There is no state. */
+size_t fmoe_vocab_loss_grad_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes, int packs);
+int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t ldh, const void* weight, int w_dtype,
+                             int64_t ldw, const void* index, int index64, const void* teacher, int t_dtype,
+                             int64_t T, int64_t dim, int64_t vocab, int64_t top, int64_t ignore_index,
+                             double logit_scale, double temperature, int planes, int reduction, float* loss,
+                             void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* dst = scale[0] * src, n elements of dtype (fp32 arithmetic, one rounding); src == dst: in place, and nothing is
+ * touched where scale[0] is 1 (gradients whose loss's gradient arrives later). */
+int fmoe_scale(const float* scale, const void* src, void* dst, int dtype, int64_t n, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,8 @@ u = 2^-24 is half a step of fp32 and h half a step of the operands' and results'
   lane, 6 joins, then one per 128 columns, each with up to 4 roundings.
 * p = exp(s - lse) has the relative error of both, d; G = up (p - q) the error d up p, and half a step h of its own.
 * dH = G W and dW = G^T H: what G is off by times |W| or |H|, the dot product's own error and the result's rounding.
+* Where a loss of one value forms its gradients at once (more than 64 rows), the rows' factors go into H before
+  dW's product: one more rounding of each of its terms, half a step h.
 """
 import math
 
@@ -168,7 +170,8 @@ def _reference(hidden, weight, lists, teacher, ignore, scale, tau, reduction, up
     out_h, out_w = HALF[hidden.dtype], HALF[weight.dtype]
     dH, dW = G @ W, G.T @ H
     bH = dG @ W.abs() + (dot(V) + 80 * U) * (G.abs() @ W.abs()) + out_h * dH.abs()
-    bW = dG.T @ H.abs() + dot(T) * (G.abs().T @ H.abs()) + out_w * dW.abs()
+    again = g_half if reduction != "none" and T > 64 else 0.0
+    bW = dG.T @ H.abs() + (dot(T) + again) * (G.abs().T @ H.abs()) + out_w * dW.abs()
     return (loss, bound * 1.0001 + 1e-30), (dH, bH * 1.01 + 1e-30), (dW, bW * 1.01 + 1e-30)
 
 
@@ -213,7 +216,12 @@ def test_cross_entropy(gpu_device, T, V, D, reduction, dtype):
     again = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale), [h, w], up)
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
     with torch.no_grad():
-        assert torch.equal(linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale), loss)
+        only = linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale)
+    if reduction == "none" or T <= 64:
+        assert torch.equal(only, loss)
+    else:  # (with gradients, the exponentials are relative to another logit: other roundings within the same bound)
+        want = _reference(h, w, t[:, None], None, -100, scale, 1.0, reduction, up)[0]
+        _within(only, *want, "loss without gradients")
 
 
 def _lists(g, T, V, K, device, repeat=False):
@@ -255,12 +263,76 @@ def test_several_pieces_wide_rows_and_split_products(gpu_device, T, V, D, K, dty
     up = torch.tensor(3.0, device=gpu_device)
     want = _reference(h, w, t[:, None], None, -100, 1.0, 1.0, "mean", up)
     _check(linear_cross_entropy(h, w, t), h, w, up, want)
+    ups = torch.rand(T, generator=g).to(gpu_device)
+    want = _reference(h, w, t[:, None], None, -100, 1.0, 1.0, "none", ups)
+    _check(linear_cross_entropy(h, w, t, reduction="none"), h, w, ups, want)
     del want
     index = torch.randint(0, V, (T, K), generator=g).to(gpu_device)
     index[::5] = -100
     z = torch.randn(T, K, generator=g).to(gpu_device)
     want = _reference(h, w, index, z, -100, 1.0, 2.0, "sum", up)
     _check(linear_distillation(h, w, index, z, temperature=2.0, reduction="sum"), h, w, up, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far", [60.0, 90.0, 400.0])
+def test_rows_far_from_their_targets(gpu_device, far, dtype):
+    # targets (and all listed tokens) whose logits lie far below the others': the exponentials relative to them
+    # leave the range that stands for probabilities, in one row (90: beyond 2^100; 400: beyond fp32)
+    g = _gen(int(far))
+    T, V, D = 200, 700, 64
+    h, w, t = _operands(g, T, V, D, torch.float32, gpu_device, pull=False)
+    with torch.no_grad():
+        h[17] = -far * w[t[17]] / w[t[17]].square().sum()
+    h, w = (x.detach().to(dtype).requires_grad_(True) for x in (h, w))
+    up = torch.tensor(1.0, device=gpu_device)
+    for reduction in ("mean", "sum"):
+        loss = linear_cross_entropy(h, w, t, reduction=reduction)
+        _check(loss, h, w, up, _reference(h, w, t[:, None], None, -100, 1.0, 1.0, reduction, up))
+    index = t[:, None].repeat(1, 2)
+    z = torch.randn(T, 2, generator=g).to(gpu_device)
+    loss = linear_distillation(h, w, index, z)
+    _check(loss, h, w, up, _reference(h, w, index, z, -100, 1.0, 1.0, "mean", up))
+
+
+def test_infinite_operands(gpu_device):
+    # a vocabulary row of -infinity (a token that is never taken) against positive hidden states: torch's results
+    # from bf16 operands; NaN from fp32 operands, whose parts (infinity less infinity) are no numbers
+    g = _gen(4)
+    T, V, D = 100, 300, 64
+    h = torch.rand(T, D, generator=g).to(gpu_device)
+    w = torch.randn(V, D, generator=g).to(gpu_device)
+    w[7] = -math.inf
+    t = torch.randint(8, V, (T,), generator=g).to(gpu_device)
+    for rows in (slice(None), slice(0, 50)):  # (up to 64 rows run on fp32 products)
+        got = linear_cross_entropy(h[rows], w, t[rows], reduction="none")
+        assert bool(got.isnan().all()) or (rows.stop == 50 and bool(got.isfinite().all()))
+    hb, wb = h.bfloat16() + 0.25, w.bfloat16()
+    for reduction in ("none", "mean"):
+        got = linear_cross_entropy(hb.requires_grad_(True), wb, t, reduction=reduction)
+        want = torch.nn.functional.cross_entropy(hb.detach().double() @ wb.double().T, t, reduction=reduction)
+        torch.testing.assert_close(got.detach().double(), want, rtol=0, atol=(D + 100) * U * 128)
+    t[3] = 7
+    assert float(linear_cross_entropy(hb, wb, t, reduction="none")[3].detach()) == math.inf
+    assert float(linear_cross_entropy(hb, wb, t).detach()) == math.inf
+
+
+@pytest.mark.parametrize("T", [40, 300])
+def test_backward_passes_of_a_graph_that_is_kept(gpu_device, T):
+    # gradients formed in the forward are handed out scaled; a second pass gets its own
+    g = _gen(T)
+    h, w, t = _operands(g, T, 500, 96, torch.bfloat16, gpu_device)
+    one = torch.autograd.grad(linear_cross_entropy(h, w, t), [h, w])
+    loss = linear_cross_entropy(h, w, t)
+    first = torch.autograd.grad(loss, [h, w], torch.tensor(0.5, device=gpu_device), retain_graph=True)
+    second = torch.autograd.grad(loss, [h, w], torch.tensor(-2.0, device=gpu_device), retain_graph=True)
+    third = torch.autograd.grad(loss, [h, w])
+    for a, b, c, d in zip(one, first, second, third):  # (powers of two: exact)
+        assert torch.equal(b, 0.5 * a) and torch.equal(c, -2 * a) and torch.equal(d, a)
+        assert len({x.data_ptr() for x in (b, c, d)}) == 3
+    (linear_cross_entropy(h, w, t) * 4).backward()
+    (linear_cross_entropy(h, w, t) * 4).backward()
+    assert torch.equal(h.grad, 8 * one[0]) and torch.equal(w.grad, 8 * one[1])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -315,6 +387,7 @@ def test_no_targets_at_all_and_targets_outside_the_vocabulary(gpu_device, T):
         assert not gh.any() and not gw.any()
     t[1], t[2] = 300, -100
     loss = linear_cross_entropy(h, w, t, reduction="none")
+    loss = loss.detach()
     assert bool(loss[1].isnan()) and float(loss[2]) == 0 and not bool(loss[0].isnan())
     t[0] = -7
     assert int(linear_cross_entropy(h, w, t, reduction="none").isnan().sum()) == 2
@@ -464,12 +537,13 @@ def test_captured_and_replayed(gpu_device, T):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
 
 
-def test_compiled(gpu_device):
+@pytest.mark.parametrize("S", [30, 70])
+def test_compiled(gpu_device, S):
     torch.manual_seed(0)
     w = torch.randn(300, 64, device=gpu_device, dtype=torch.bfloat16, requires_grad=True)
-    ids = torch.randint(0, 300, (2, 30), device=gpu_device)
-    z = torch.randn(2, 30, 4, device=gpu_device)
-    index = torch.randint(0, 300, (2, 30, 4), device=gpu_device)
+    ids = torch.randint(0, 300, (2, S), device=gpu_device)
+    z = torch.randn(2, S, 4, device=gpu_device)
+    index = torch.randint(0, 300, (2, S, 4), device=gpu_device)
 
     def step(ids, w):
         x = embedding(ids, w, 3.0, padding_idx=1)
@@ -498,7 +572,7 @@ def test_wrappers_give_the_native_calls_results(gpu_device):
     index, z = _lists(g, 70, 300, 9, gpu_device)
 
     def step():
-        loss = linear_cross_entropy(h, w, t) + linear_distillation(h, w, index, z)
+        loss = linear_cross_entropy(h, w, t) + linear_distillation(h, w, index, z, reduction="none").sum()
         y = embedding(t, w, 2.0)
         return loss, *torch.autograd.grad(loss + y.float().sum(), [h, w])
 
@@ -510,7 +584,8 @@ def test_wrappers_give_the_native_calls_results(gpu_device):
     finally:
         K.set_timer(None)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
-    assert {"embedding_fwd", "embedding_bwd", "vocab_loss_fwd", "vocab_loss_bwd"} <= set(times)
+    assert {"embedding_fwd", "embedding_bwd", "vocab_loss_fwd", "vocab_loss_bwd", "vocab_loss_fwd_grad",
+            "scale"} <= set(times)
 
 
 def test_long_offsets(gpu_device):

@@ -93,11 +93,45 @@ def test_loss_argument_errors_without_gpu():
         assert lib.fmoe_vocab_loss_state_bytes(*a) == 0
 
 
+def test_gradients_at_once_and_scale_argument_errors_without_gpu():
+    lib = _lib.load()
+    ws = lib.fmoe_vocab_loss_grad_workspace_bytes(100, 64, 100, 1, 1, 0)
+
+    def call(h=FAKE, T=100, V=100, d=64, top=1, red=1, planes=1, loss=FAKE, dh=FAKE, dht=0, dw=FAKE, dwt=0, w=FAKE,
+             n=ws, t=None):
+        return lib.fmoe_vocab_loss_fwd_grad(h, 0, 64, FAKE, 0, 64, FAKE, 1, t, 1, T, d, V, top, -100, 1.0, 1.0, planes,
+                                            red, loss, dh, dht, dw, dwt, w, n, None)
+
+    assert call(red=0) == 1 and call(T=-1) == 1 and call(loss=None) == 1 and call(h=None) == 1 and call(planes=3) == 4
+    assert call(dht=2) == 4 and call(dwt=-1) == 4 and call(dh=FAKE + 1) == 3 and call(dw=FAKE + 1) == 3 and call(w=FAKE + 1) == 3
+    assert call(T=64) == 2 and call(n=ws - 1) == 6 and call(w=None) == 6 and call(top=3) == 1
+
+    def scale(f=FAKE, a=FAKE, b=FAKE, dt=1, n=4):
+        return lib.fmoe_scale(f, a, b, dt, n, None)
+
+    assert scale(n=-1) == 1 and scale(dt=9) == 4 and scale(f=None) == 1 and scale(a=None) == 1 and scale(b=None) == 1
+    assert scale(f=FAKE + 2) == 3 and scale(a=FAKE + 2) == 3 and scale(b=FAKE + 1, dt=0) == 3 and scale(n=0, a=None) == 0
+
+
 def test_state_size_is_the_librarys():
     lib = _lib.load()
     for a in [(0, 1, 1, 1), (1, 1, 1, 1), (5, 7, 3, 3), (64, 64, 64, 1), (65, 65, 1, 3), (16384, 768, 1, 1),
               (4096, 2048, 1000, 3)]:
         assert lib.fmoe_vocab_loss_state_bytes(*a) == K.vocab_loss_state_bytes(*a), a
+
+
+def test_rule_of_gradients_at_once_is_the_librarys():
+    lib = _lib.load()
+    taken = 0
+    for T in (0, 1, 64, 65, 256, 257, 2000, 2049, 5000, 32768, 100000):
+        for V in (1, 255, 257, 32768, 50021, 131072, 262145, 1 << 22, (1 << 22) + 1):
+            for d in (1, 768, 2048, 4096):
+                for planes in (1, 3):
+                    for packs in (0, 1):
+                        want = lib.fmoe_vocab_loss_grad_workspace_bytes(T, d, V, 1, planes, packs) > 0
+                        assert K.vocab_loss_takes_gradients(T, d, V, planes, packs) == want, (T, V, d, planes, packs)
+                        taken += want
+    assert 0 < taken < 11 * 9 * 4 * 4
 
 
 def test_workspaces_stay_bounded():
@@ -108,6 +142,13 @@ def test_workspaces_stay_bounded():
     assert n < 32768 * 131072 * 2 // 4
     # the forward's: a maximum and a sum per row and 128 columns
     assert lib.fmoe_vocab_loss_fwd_workspace_bytes(32768, 2048, 131072, 1, 0) <= 32768 * 1024 * 8 + (1 << 18)
+    # gradients at once: a piece of 4096 rows, d_weight's sum, partial tiles, packed and scaled rows
+    n = lib.fmoe_vocab_loss_grad_workspace_bytes(32768, 2048, 131072, 1, 1, 0)
+    assert 0 < n <= (1 << 30) + 131072 * 2048 * 4 + (1 << 28) + 33792 * 2048 * 2 + 4096 * (2048 * 2 + 1024 * 8) + (1 << 20)
+    # not for few rows, nor vocabularies whose pieces would have few rows
+    assert lib.fmoe_vocab_loss_grad_workspace_bytes(64, 2048, 131072, 1, 1, 0) == 0
+    assert lib.fmoe_vocab_loss_grad_workspace_bytes(32768, 2048, 300000, 1, 1, 0) == 0
+    assert lib.fmoe_vocab_loss_grad_workspace_bytes(1000, 2048, 300000, 1, 1, 0) > 0
     # rows that the products read as they lie
     assert lib.fmoe_vocab_loss_packs(FAKE, 0, 128, 128, 1) == 0
     for w, dt, ld, d, planes in [(FAKE + 2, 0, 128, 128, 1), (FAKE, 1, 128, 128, 1), (FAKE, 0, 129, 128, 1),
