@@ -802,9 +802,10 @@ def vocab_loss_takes_gradients(rows: int, dim: int, vocab: int, planes: int, pac
     """Whether vocab_loss_fwd_grad takes these sizes: arithmetic alone, for traced calls (csrc/vocab_loss.hip,
     vl_fused_piece)."""
     wide, tall, cols = (vocab + 255) // 256 * 256, (rows + 255) // 256 * 256, (dim + 63) // 64 * 64
-    if rows <= 64 or vocab > 1 << 22 or (packs and wide * cols * 2 * planes > 1 << 31):
+    if rows <= 64 or vocab > 1 << 22 or max(vocab, rows) * dim > 1 << 33 or (
+            packs and wide * cols * 2 * planes > 1 << 31):
         return False
-    most = (1 << 30) // (wide * 2 * planes) // 256 * 256
+    most = (1 << 31) // (wide * 2 * planes) // 256 * 256
     return most >= tall or (most >= 2048 and vocab * cols * 4 <= 1 << 31)
 
 
@@ -847,17 +848,20 @@ def vocab_loss_fwd_grad(hidden, weight, index, teacher, ignore_index: int, logit
 
 
 @_timed
-def scale(factor, src, dst=None):
-    """factor (one fp32 value) times src, into dst (default: a new tensor; src itself: in place)."""
+def scale(factor, tensors):
+    """factor (one fp32 value) times each of up to 8 tensors, as new ones; None stays None."""
     lib = _lib.load()
-    sp = _req(src, "src")
-    if dst is None:
-        dst = torch.empty_like(src)
-    if factor.numel() != 1 or dst.shape != src.shape:
-        raise RuntimeError("factor must hold one value, and dst have src's shape")
-    check(lib.fmoe_scale(_req(factor, "factor", torch.float32), sp, _req(dst, "dst", src.dtype), _dtype_code(src.dtype),
-                         src.numel(), _stream()), "fmoe_scale")
-    return dst
+    src = [t for t in tensors if t is not None]
+    dst = [torch.empty_like(t) for t in src]
+    if factor.numel() != 1:
+        raise RuntimeError(f"factor must hold one value (got {tuple(factor.shape)})")
+    n = len(src)
+    check(lib.fmoe_scale(_req(factor, "factor", torch.float32), (ctypes.c_void_p * n)(*[_req(t, "src") for t in src]),
+                         (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst]),
+                         (ctypes.c_int * n)(*[_dtype_code(t.dtype) for t in src]),
+                         (ctypes.c_int64 * n)(*[t.numel() for t in src]), n, _stream()), "fmoe_scale")
+    out = iter(dst)
+    return [None if t is None else next(out) for t in tensors]
 
 
 CAST_MAX_TENSORS = 64

@@ -107,7 +107,7 @@ VOCAB_SIGNATURES = {
     "fmoe_vocab_loss_fwd_grad": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int, c_int64, c_int64,
                                          c_int64, c_int64, c_int64, c_double, c_double, c_int, c_int, _P, _P, c_int,
                                          _P, c_int, _P, c_size_t, _P]),
-    "fmoe_scale": (c_int, [_P, _P, _P, c_int, c_int64, _P]),
+    "fmoe_scale": (c_int, [_P, _PP, _PP, POINTER(c_int), POINTER(c_int64), c_int, _P]),
 }
 
 _lock = threading.Lock()

@@ -588,21 +588,30 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
 
 // Gradients formed in the forward (loss of one value): their scaling by the loss's gradient.  In place, where
 // this backward pass is the only one (it frees the graph); nothing is touched where the factor is 1.
-Tensor scaled(const Tensor& factor, const Tensor& g, bool in_place) {
+variable_list scaled(const Tensor& factor, const variable_list& src, bool in_place) {
   const Tensor f = factor.contiguous();
-  Tensor out = in_place ? g : at::empty_like(g);
-  check(api.fmoe_scale(static_cast<const float*>(f.data_ptr()), g.data_ptr(), out.data_ptr(), dtype_code(g.scalar_type()),
-                       g.numel(), current_stream(g)),
+  variable_list out;
+  std::vector<const void*> from;
+  std::vector<void*> to;
+  std::vector<int> codes;
+  std::vector<int64_t> n;
+  for (const Tensor& t : src) {
+    out.push_back(in_place ? t : at::empty_like(t));
+    from.push_back(t.data_ptr()), to.push_back(out.back().data_ptr());
+    codes.push_back(dtype_code(t.scalar_type())), n.push_back(t.numel());
+  }
+  check(api.fmoe_scale(static_cast<const float*>(f.data_ptr()), from.data(), to.data(), codes.data(), n.data(),
+                       static_cast<int>(src.size()), current_stream(f)),
         "fmoe_scale");
   return out;
 }
 
 struct ScaledGradients : torch::autograd::Function<ScaledGradients> {
   static variable_list forward(AutogradContext*, const Tensor& d_loss, const OptTensor& dh, const OptTensor& dw) {
-    variable_list out;
+    variable_list src;
     for (const OptTensor* g : {&dh, &dw})
-      if (g->has_value()) out.push_back(scaled(d_loss, **g, false));
-    return out;
+      if (g->has_value()) src.push_back(**g);
+    return scaled(d_loss, src, false);
   }
   static variable_list backward(AutogradContext*, const variable_list&) {
     throw std::runtime_error("fusionllm_amd losses over the vocabulary: second derivatives are not implemented");
@@ -644,9 +653,13 @@ struct VocabLossGrad : torch::autograd::Function<VocabLossGrad> {
         if (need[i]) out[i] = g[k++];
       return out;
     }
-    const bool only = !torch::autograd::get_current_graph_task_keep_graph();
+    variable_list src;
     for (int i = 0; i < 2; ++i)
-      if (need[i]) out[i] = scaled(grads[0], saved[i], only);
+      if (need[i]) src.push_back(saved[i]);
+    const variable_list g = scaled(grads[0], src, !torch::autograd::get_current_graph_task_keep_graph());
+    size_t k = 0;
+    for (int i = 0; i < 2; ++i)
+      if (need[i]) out[i] = g[k++];
     return out;
   }
 };

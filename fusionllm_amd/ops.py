@@ -317,14 +317,14 @@ def _(hidden, weight, index, teacher, ignore_index, logit_scale, temperature, pl
 
 
 @torch.library.custom_op("fusionllm::scale", mutates_args=())
-def scale(factor: Tensor, src: Tensor) -> Tensor:
-    with _norm._on_device(src):
-        return K.scale(factor.contiguous(), src)
+def scale(factor: Tensor, tensors: list[Tensor]) -> list[Tensor]:
+    with _norm._on_device(factor):
+        return K.scale(factor.contiguous(), tensors)
 
 
 @scale.register_fake
-def _(factor, src):
-    return torch.empty_like(src)
+def _(factor, tensors):
+    return [torch.empty_like(t) for t in tensors]
 
 
 def _vocab_loss_grad_setup(ctx, inputs, output):
@@ -336,8 +336,8 @@ def _vocab_loss_grad_backward(ctx, d_outs):
     d_loss = d_outs[0]
     if d_loss is None:
         return (None,) * 11
-    grads = iter(ctx.saved_tensors)
-    dh, dw = (torch.ops.fusionllm.scale(d_loss, next(grads)) if need else None for need in ctx.need)
+    grads = iter(torch.ops.fusionllm.scale(d_loss, list(ctx.saved_tensors)))
+    dh, dw = (next(grads) if need else None for need in ctx.need)
     return dh, dw, *(None,) * 9
 
 

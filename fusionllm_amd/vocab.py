@@ -8,7 +8,7 @@ bits every run, no atomics.
 
 The losses are those of the logits ``s = logit_scale * hidden @ weight.T``,
 which are never stored.  A loss of one value (mean, sum) that needs gradients forms them in
-its forward, a piece of the rows at a time (up to 1 GiB), and its backward scales
+its forward, a piece of the rows at a time (up to 2 GiB), and its backward scales
 them by the loss's gradient.  A loss per row (none), and one of up to 64 rows or of a vocabulary too
 large for such pieces, reduces the logits tile by tile in the forward and forms
 them again in the backward.  Rows without a target
@@ -171,10 +171,9 @@ class _VocabLossGradFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        grads = []
-        for g, need in zip(ctx.saved_tensors, ctx.needs_input_grad):
-            with _on_device(d_loss):
-                grads.append(K.scale(d_loss.contiguous(), g) if need else None)
+        grads = [g if need else None for g, need in zip(ctx.saved_tensors, ctx.needs_input_grad)]
+        with _on_device(d_loss):
+            grads = K.scale(d_loss.contiguous(), grads)
         return *grads, None, None, None, None, None, None, None
 
 

@@ -22,6 +22,7 @@ extern "C" {
 #define FMOE_VOCAB_MAX_TOKENS 16777216 /* rows of one call */
 #define FMOE_VOCAB_MAX_VOCAB 16777216
 #define FMOE_VOCAB_MAX_ELEMENTS 8589934592LL /* of an operand: rows * dim, vocab * dim */
+#define FMOE_SCALE_MAX_TENSORS 8
 #define FMOE_VOCAB_MAX_TOP 1024        /* listed logits of a teacher per row */
 
 /* ---------------------------------------------------------------------------
@@ -96,7 +97,7 @@ int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int w_dtype, in
  * the product of d_weight: with planes = 1 the scaled hidden states are rounded to bf16 once more.  Rows whose
  * sum of such exponentials leaves 2^-100 .. 2^100 (or is no number) make their piece be formed in the ordinary way.
  * d_hidden and d_weight as in fmoe_vocab_loss_bwd.  The size query returns 0 where this form is not taken (up to 64
- * rows; vocabularies of which no piece of 2048 rows fits 1 GiB): FMOE_ERR_SHAPE.  There is no state. */
+ * rows; vocabularies of which no piece of 2048 rows fits 2 GiB): FMOE_ERR_SHAPE.  There is no state. */
 size_t fmoe_vocab_loss_grad_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes, int packs);
 int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t ldh, const void* weight, int w_dtype,
                              int64_t ldw, const void* index, int index64, const void* teacher, int t_dtype,
@@ -105,9 +106,11 @@ int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t ldh, const
                              void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype, void* workspace,
                              size_t workspace_bytes, void* stream);
 
-/* dst = scale[0] * src, n elements of dtype (fp32 arithmetic, one rounding); src == dst: in place, and nothing is
- * touched where scale[0] is 1 (gradients whose loss's gradient arrives later). */
-int fmoe_scale(const float* scale, const void* src, void* dst, int dtype, int64_t n, void* stream);
+/* dst[i] = scale[0] * src[i] for up to FMOE_SCALE_MAX_TENSORS tensors of n[i] elements of dtype[i] (host arrays; fp32
+ * arithmetic, one rounding).  src[i] == dst[i]: in place, and nothing is touched where scale[0] is 1 (gradients
+ * whose loss's gradient arrives later). */
+int fmoe_scale(const float* scale, const void* const* src, void* const* dst, const int* dtype, const int64_t* n,
+               int n_tensors, void* stream);
 
 #ifdef __cplusplus
 }

@@ -252,7 +252,7 @@ def test_distillation(gpu_device, T, V, D, K, reduction, tau, dtype):
     _check(loss, h, w, up, _reference(h, w, index, z, -100, 0.9, tau, reduction, up))
 
 
-@pytest.mark.parametrize("T,V,D,K,dtype", [(12000, 46000, 64, 3, torch.bfloat16), (4200, 45000, 96, 2, torch.float32),
+@pytest.mark.parametrize("T,V,D,K,dtype", [(24000, 46000, 64, 3, torch.bfloat16), (8200, 45000, 96, 2, torch.float32),
                                            (70, 600, 16384, 20, torch.float32), (9, 300, 16384, 20, torch.bfloat16),
                                            (2100, 9000, 640, 1, torch.bfloat16)])
 def test_several_pieces_wide_rows_and_split_products(gpu_device, T, V, D, K, dtype):
