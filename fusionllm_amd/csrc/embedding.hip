@@ -11,9 +11,9 @@
 //      G-th id (G workgroups, a power of two): the frequent ids, which a tokenizer numbers first, fall to
 //      different workgroups.  So "sorted" is by slot, (id mod G) * 512 + id / G.
 //   2. embed_sum_kernel adds the rows of the sorted tokens, kTile at a time per wave: an id whose tokens
-//      lie in one tile is written there; one that crosses tiles leaves an fp32 partial row per tile.
-//   3. embed_rest_kernel writes the ids that cross tiles, from their partial rows in order, and zeros
-//      for the ids without tokens.
+//      lie in one tile is written there; one that crosses tiles leaves an fp32 partial row per tile.  Workgroups
+//      behind those write zeros for the ids without tokens.
+//   3. embed_join_kernel writes the ids that cross tiles, from their partial rows in order.
 #include "../../include/fusionvocab.h"
 #include "elements.h"
 #include "fmoe_common.h"
@@ -23,8 +23,8 @@ namespace fmoe {
 constexpr int kTile = 16;          // sorted tokens per wave of embed_sum_kernel
 constexpr int kSortIds = 512;      // ids per workgroup of the sort, at most
 constexpr int kSortWaves = 16;
-constexpr int kRestIds = 8;        // slots per wave of embed_rest_kernel
-constexpr int kRestWaves = 16;
+constexpr int kZeroIds = 8;        // slots per wave that looks for ids without tokens
+constexpr int kJoinWaves = 16;     // waves, and tiles, per workgroup of embed_join_kernel
 constexpr int kLongTiles = 8;      // tiles above which a workgroup adds an id's partial rows together
 
 // Consecutive elements per lane: 16 bytes.
@@ -239,10 +239,35 @@ struct Row16<FMOE_F32> {
   typedef f32x4_e4 type;
 };
 
-// A tile's rows are all in flight together.
+// Zeros in the rows of 8 slots without tokens, per wave.
+template <int DW>
+__device__ __forceinline__ void embed_zero(const EmbedArgs& a, int64_t item) {
+  constexpr int V = kPer<DW>;
+  const int segments = (a.D + 64 * V - 1) / (64 * V);
+  const int lane = threadIdx.x & 63, group = static_cast<int>(item / segments);
+  const int c = (static_cast<int>(item - static_cast<int64_t>(group) * segments) * 64 + lane) * V, n = min(a.D - c, V);
+  const int s0 = group * kZeroIds;
+  if (s0 >= a.slots) return;
+  const int starts = a.start[min(s0 + min(lane, kZeroIds), a.slots)];
+  float zero[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kZeroIds; ++i) {
+    const int64_t id = slot_id(a, s0 + i);
+    if (id < a.V && __builtin_amdgcn_readlane(starts, i) == __builtin_amdgcn_readlane(starts, i + 1))
+      store_v<DW, V>(a.dst, id * a.D + c, n, zero);
+  }
+}
+
+// A tile's rows are all in flight together.  Workgroups from `blocks` on: zeros.
 template <int DY, int DW>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedArgs a) {
+__global__ __launch_bounds__(256) void embed_sum_kernel(const EmbedArgs a, int blocks) {
   constexpr int V = kPer<DY>;
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    embed_zero<DW>(a, static_cast<int64_t>(blockIdx.x - blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    return;
+  }
   const int lane = threadIdx.x & 63;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tile = item / a.segments;
@@ -325,77 +350,56 @@ __device__ __forceinline__ void add_partials(const EmbedArgs& a, int64_t first, 
   }
 }
 
-// Workgroups 0 .. blocks - 1: 128 slots each, those without tokens and those of a few tiles.  The others:
-// 16 tiles each; the ids that begin in them and go on through more than kLongTiles tiles.
+// Wave w: the id that goes on from its tile into the next one, if it begins in that tile; one of many tiles is the
+// whole workgroup's.
 template <int DW>
-__global__ __launch_bounds__(64 * kRestWaves) void embed_rest_kernel(const EmbedArgs a, int blocks) {
+__global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(const EmbedArgs a) {
   constexpr int V = kPer<DW>;
+  __shared__ float sums[kJoinWaves][64 * V];
+  __shared__ int found[kJoinWaves];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (static_cast<int>(blockIdx.x) >= blocks) {
-    __shared__ float sums[kRestWaves][64 * V];
-    __shared__ int found[kRestWaves];
-    const int item = blockIdx.x - blocks, group = item / a.segments;
-    const int c = ((item - group * a.segments) * 64 + lane) * V, n = min(a.D - c, V);
-    {
-      // wave w: the id that goes on from its tile into the next one, if it begins in it and is long
-      const int64_t tile = static_cast<int64_t>(group) * kRestWaves + w, next = (tile + 1) * kTile;
-      int slot = -1;
-      if (next < a.start[a.slots]) {
-        slot = a.sorted[next].y;
-        const int64_t ta = a.start[slot] / kTile, tb = (a.start[slot + 1] - 1) / kTile;
-        if (ta != tile || tb - ta <= kLongTiles) slot = -1;
-      }
-      if (lane == 0) found[w] = slot;
-    }
-    __syncthreads();
-    for (int f = 0; f < kRestWaves; ++f) {
-      const int slot = found[f];
-      if (slot < 0) continue;
-      const int64_t ta = a.start[slot] / kTile, tb = (a.start[slot + 1] - 1) / kTile;
-      // wave w every 16th partial row, then the waves in order
-      float acc[V];
-#pragma unroll
-      for (int q = 0; q < V; ++q) acc[q] = 0.0f;
-      if (w == 0) load_v<FMOE_F32, V>(a.part, (2 * ta + 1) * a.D + c, n, acc);
-      add_partials<V>(a, ta + 1 + w, tb, kRestWaves, c, n, acc);
-#pragma unroll
-      for (int q = 0; q < V; ++q) sums[w][q * 64 + lane] = acc[q];
-      __syncthreads();
-      if (w == 0) {
-        for (int p = 1; p < kRestWaves; ++p)
-#pragma unroll
-          for (int q = 0; q < V; ++q) acc[q] = acc[q] + sums[p][q * 64 + lane];
-#pragma unroll
-        for (int q = 0; q < V; ++q) acc[q] = acc[q] * a.scale;
-        store_v<DW, V>(a.dst, slot_id(a, slot) * a.D + c, n, acc);
-      }
-      __syncthreads();
-    }
-    return;
-  }
   const int group = blockIdx.x / a.segments;
   const int c = ((static_cast<int>(blockIdx.x) - group * a.segments) * 64 + lane) * V, n = min(a.D - c, V);
-  const int s0 = (group * kRestWaves + w) * kRestIds;
-  const int starts = a.start[min(s0 + min(lane, kRestIds), a.slots)];
-  float zero[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) zero[e] = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kRestIds; ++i) {
-    const int64_t id = slot_id(a, s0 + i);
-    if (id >= a.V) continue;
-    const int s = __builtin_amdgcn_readlane(starts, i), e = __builtin_amdgcn_readlane(starts, i + 1);
-    const int64_t o = id * a.D + c, ta = s / kTile, tb = (e - 1) / kTile;
-    if (s == e) {
-      store_v<DW, V>(a.dst, o, n, zero);
-    } else if (ta < tb && tb - ta <= kLongTiles) {  // (in one tile: written with it)
+  const int64_t tile = static_cast<int64_t>(group) * kJoinWaves + w, next = (tile + 1) * kTile;
+  int slot = -1;
+  if (next < a.start[a.slots]) {
+    const int s = a.sorted[next].y;
+    const int64_t ta = a.start[s] / kTile, tb = (a.start[s + 1] - 1) / kTile;
+    if (ta == tile && tb - ta > kLongTiles) {
+      slot = s;
+    } else if (ta == tile && tb > ta) {
       float acc[V];
       load_v<FMOE_F32, V>(a.part, (2 * ta + 1) * a.D + c, n, acc);
       add_partials<V>(a, ta + 1, tb, 1, c, n, acc);
 #pragma unroll
       for (int q = 0; q < V; ++q) acc[q] = acc[q] * a.scale;
-      store_v<DW, V>(a.dst, o, n, acc);
+      store_v<DW, V>(a.dst, slot_id(a, s) * a.D + c, n, acc);
     }
+  }
+  if (lane == 0) found[w] = slot;
+  __syncthreads();
+  for (int f = 0; f < kJoinWaves; ++f) {
+    const int s = found[f];
+    if (s < 0) continue;
+    const int64_t ta = a.start[s] / kTile, tb = (a.start[s + 1] - 1) / kTile;
+    // wave w every 16th partial row, then the waves in order
+    float acc[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+    if (w == 0) load_v<FMOE_F32, V>(a.part, (2 * ta + 1) * a.D + c, n, acc);
+    add_partials<V>(a, ta + 1 + w, tb, kJoinWaves, c, n, acc);
+#pragma unroll
+    for (int q = 0; q < V; ++q) sums[w][q * 64 + lane] = acc[q];
+    __syncthreads();
+    if (w == 0) {
+      for (int p = 1; p < kJoinWaves; ++p)
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] = acc[q] + sums[p][q * 64 + lane];
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] = acc[q] * a.scale;
+      store_v<DW, V>(a.dst, slot_id(a, s) * a.D + c, n, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -496,21 +500,20 @@ extern "C" int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, 
   if (index64) embed_sort_kernel<true><<<sort, 64 * kSortWaves, 0, s>>>(a);
   else embed_sort_kernel<false><<<sort, 64 * kSortWaves, 0, s>>>(a);
   const int64_t tiles = ceil_div(T, kTile);
-  if (T > 0) {
-    a.segments = segments_of(dim, dy_dtype);
-    const dim3 grid(static_cast<uint32_t>(ceil_div(tiles * a.segments, 4)));
-    if (dy_dtype == FMOE_BF16 && dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_BF16><<<grid, 256, 0, s>>>(a);
-    else if (dy_dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_F32><<<grid, 256, 0, s>>>(a);
-    else if (dtype == FMOE_BF16) embed_sum_kernel<FMOE_F32, FMOE_BF16><<<grid, 256, 0, s>>>(a);
-    else embed_sum_kernel<FMOE_F32, FMOE_F32><<<grid, 256, 0, s>>>(a);
-  }
-  a.segments = segments_of(dim, dtype);
-  // (an id of more than kLongTiles tiles needs as many tokens)
-  const int64_t blocks = ceil_div(space.slots, kRestIds * kRestWaves) * a.segments;
-  const int64_t longs = tiles > kLongTiles ? ceil_div(tiles, kRestWaves) * a.segments : 0;
-  const dim3 rest(static_cast<uint32_t>(blocks + longs));
+  a.segments = segments_of(dim, dy_dtype);
+  const int64_t blocks = ceil_div(tiles * a.segments, 4);
+  const int64_t zeros = ceil_div(ceil_div(space.slots, kZeroIds) * segments_of(dim, dtype), 4);
+  const dim3 grid(static_cast<uint32_t>(blocks + zeros));
   const int b = static_cast<int>(blocks);
-  if (dtype == FMOE_BF16) embed_rest_kernel<FMOE_BF16><<<rest, 64 * kRestWaves, 0, s>>>(a, b);
-  else embed_rest_kernel<FMOE_F32><<<rest, 64 * kRestWaves, 0, s>>>(a, b);
+  if (dy_dtype == FMOE_BF16 && dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_BF16><<<grid, 256, 0, s>>>(a, b);
+  else if (dy_dtype == FMOE_BF16) embed_sum_kernel<FMOE_BF16, FMOE_F32><<<grid, 256, 0, s>>>(a, b);
+  else if (dtype == FMOE_BF16) embed_sum_kernel<FMOE_F32, FMOE_BF16><<<grid, 256, 0, s>>>(a, b);
+  else embed_sum_kernel<FMOE_F32, FMOE_F32><<<grid, 256, 0, s>>>(a, b);
+  if (tiles > 1) {
+    a.segments = segments_of(dim, dtype);
+    const dim3 join(static_cast<uint32_t>(ceil_div(tiles, kJoinWaves) * a.segments));
+    if (dtype == FMOE_BF16) embed_join_kernel<FMOE_BF16><<<join, 64 * kJoinWaves, 0, s>>>(a);
+    else embed_join_kernel<FMOE_F32><<<join, 64 * kJoinWaves, 0, s>>>(a);
+  }
   return launch_status();
 }
