@@ -736,8 +736,9 @@ def vocab_loss_state_bytes(rows: int, dim: int, top: int, planes: int) -> int:
     block = lambda n: (n + 255) // 256 * 256
     padded = (rows + 63) // 64 * 64
     padded = torch.sym_max(padded, 64)
-    return (256 + 2 * block(rows * 4) + 3 * block(rows * top * 4) + block(rows * 8) +
-            block(planes * padded * ((dim + 63) // 64 * 64) * 2))
+    plane = padded * ((dim + 63) // 64 * 64) * 2
+    return (256 + 2 * block(rows * 4) + 3 * block(rows * top * 4) + block(rows * 8) + block(planes * plane) +
+            (block(2 * plane) + block(padded * 4) if planes == 3 else 0))
 
 
 @_timed
@@ -803,7 +804,7 @@ def vocab_loss_takes_gradients(rows: int, dim: int, vocab: int, planes: int, pac
     vl_fused_piece)."""
     wide, tall, cols = (vocab + 255) // 256 * 256, (rows + 255) // 256 * 256, (dim + 63) // 64 * 64
     if rows <= 64 or vocab > 1 << 22 or max(vocab, rows) * dim > 1 << 33 or (
-            packs and wide * cols * 2 * planes > 1 << 31):
+            packs and wide * cols * (10 if planes == 3 else 2) > 1 << 31):
         return False
     most = (1 << 31) // (wide * 2 * planes) // 256 * 256
     return most >= tall or (most >= 2048 and vocab * cols * 4 <= 1 << 31)

@@ -21,11 +21,15 @@
 // order, with zeros up to a multiple of 64 rows and columns, so that they cost nothing and what is in
 // them (also NaN) stays out of the products.
 //
-// Operands are bf16 (planes = 1), or fp32 as three bf16 numbers, hi + mid + lo (planes = 3): 24
-// bits.  Of the nine products of such numbers the six largest are added, the smallest first, as six passes over K
-// in one ring; what is left out is below 2^-22 of the largest.  G is rounded the same way: half a step of bf16,
+// Operands are bf16 (planes = 1) or fp32 (planes = 3).  The logits of fp32 operands are products of rows that are scaled
+// by a power of two each (their largest element to 2^13 .. 2^14) and held as two fp16 numbers, hi + lo: 22 bits of every
+// element down to 2^-17 of its row's largest, and 2^-39 of that below.  lo hi + hi lo + hi hi are added, as three passes
+// over K in one ring.  G spans more: a row's gradient is as precise in its smallest elements, which make up whole rows of dW, so
+// the products with it take three bf16 numbers, hi + mid + lo: 24 bits at any size.  Of the nine products of
+// such numbers the six largest are added, the smallest first; what is left out is below 2^-22 of the largest.  G is rounded the same way: half a step of bf16,
 // 2^-8 of an element at most, before the elements of a row or column are summed in fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/fusionvocab.h"
 #include "elements.h"
@@ -54,6 +58,8 @@ struct VlState {
   float* picked;  // [T][top] t of the listed entries; cross entropy: p - 1 of the target
   float2* stat;   // [T] m, l
   uint16_t* h;    // [planes][Tp][Dp] packed rows
+  uint16_t* h16;  // planes = 3: [2][Tp][Dp] them as fp16, hi and lo of the scaled rows,
+  float* h_scale; // [Tp] and what undoes the scaling
   int64_t Tp, Dp, plane;
   size_t bytes;
   VlState(uint8_t* base, int64_t T, int64_t D, int64_t top, int planes) {
@@ -72,6 +78,8 @@ struct VlState {
     picked = reinterpret_cast<float*>(take(T * top * 4));
     stat = reinterpret_cast<float2*>(take(T * 8));
     h = reinterpret_cast<uint16_t*>(take(planes * plane * 2));
+    h16 = reinterpret_cast<uint16_t*>(take(planes == 3 ? 2 * plane * 2 : 0));
+    h_scale = reinterpret_cast<float*>(take(planes == 3 ? Tp * 4 : 0));
   }
 };
 
@@ -87,7 +95,8 @@ struct RowsArgs {
   uint32_t* masks;       // rows with entries, 32 per word; nullptr: every workgroup finds them itself
   int *head, *perm, *inv, *out_index;
   float* loss;           // zeros in rows without entries, where it is [T] (else nullptr)
-  uint16_t* h;
+  uint16_t *h, *h16;
+  float* h_scale;
 };
 constexpr int kFewEntries = 4096;  // entries of all rows that a workgroup looks at itself: 4 per thread
 
@@ -166,6 +175,40 @@ __device__ __forceinline__ void vl_copy_row(const void* src, int64_t row, int n,
   }
 }
 
+// An fp32 row of n elements as fp16 hi and lo, scaled so that its largest element lies in 2^13 .. 2^14 (infinities
+// and NaN: as they are); *undo: the inverse of the scale.
+__device__ __forceinline__ void vl_half_row(const float* src, int n, int np, uint16_t* dst, int64_t plane, float* undo,
+                                            int lane) {
+  float most = 0.0f;
+  for (int c = lane * 8; c < n; c += 512) {
+    float v[8];
+    load_upto8<FMOE_F32>(src, c, n - c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+  // 2^shift, shift = 13 - floor(log2(most)), up to 126 (subnormal rows are not scaled up further)
+  const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+  const int shift = most == 0.0f || exponent == 128 ? 0 : min(13 - exponent, 126);
+  const float scale = fm_pow2i(shift);
+  if (lane == 0) *undo = fm_pow2i(-shift);
+  typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  for (int c = lane * 8; c < np; c += 512) {
+    float v[8];
+    load_upto8<FMOE_F32>(src, c, n - c, v);
+    half8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = v[e] * scale;
+      hi[e] = static_cast<_Float16>(x);
+      lo[e] = static_cast<_Float16>(x - static_cast<float>(hi[e]));
+    }
+    *reinterpret_cast<half8*>(dst + c) = hi;
+    *reinterpret_cast<half8*>(dst + plane + c) = lo;
+  }
+}
+
 template <int DT, int PLANES>
 __global__ __launch_bounds__(1024) void vl_rows_kernel(const RowsArgs a) {
   __shared__ uint32_t bits[kFewEntries / 32];
@@ -192,6 +235,14 @@ __global__ __launch_bounds__(1024) void vl_rows_kernel(const RowsArgs a) {
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
           *reinterpret_cast<uint4*>(a.h + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
+    if constexpr (PLANES == 3)
+      for (int r = n + w; r < pad_rows(n); r += 16) {
+        if (lane == 0) a.h_scale[r] = 1.0f;
+        for (int c = lane * 8; c < a.Dp; c += 512)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            *reinterpret_cast<uint4*>(a.h16 + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
+      }
   }
   for (int i = w; i < kRowBlock && block0 + i < a.T; i += 16) {
     const int64_t t = block0 + i;
@@ -210,6 +261,9 @@ __global__ __launch_bounds__(1024) void vl_rows_kernel(const RowsArgs a) {
       if (a.t_dtype < 0) a.out_index[r] = vl_entry(a, t, z);
     }
     vl_copy_row<DT, PLANES>(a.hidden, t * a.ldh, a.D, a.Dp, a.h + static_cast<int64_t>(r) * a.Dp, a.plane, lane, 64);
+    if constexpr (PLANES == 3)
+      vl_half_row(static_cast<const float*>(a.hidden) + t * a.ldh, a.D, a.Dp, a.h16 + static_cast<int64_t>(r) * a.Dp, a.plane,
+                  a.h_scale + r, lane);
   }
 }
 
@@ -222,6 +276,17 @@ __global__ __launch_bounds__(256) void vl_pack_kernel(const void* src, int64_t l
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   vl_copy_row<DT, PLANES>(src, (v0 + r) * ld, D, Dp, dst + static_cast<int64_t>(r) * Dp, plane, lane, 64);
+}
+
+// fp32 rows, as bf16 planes (dst, where wanted) and as scaled fp16 (dst16, where wanted).
+__global__ __launch_bounds__(256) void vl_pack32_kernel(const float* src, int64_t ld, int64_t v0, int rows, int D, int Dp,
+                                                        uint16_t* dst, uint16_t* dst16, float* undo, int64_t plane) {
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int64_t at = static_cast<int64_t>(r) * Dp;
+  if (dst16) vl_half_row(src + (v0 + r) * ld, D, Dp, dst16 + at, plane, undo + r, lane);
+  if (dst) vl_copy_row<FMOE_F32, 3>(src, (v0 + r) * ld, D, Dp, dst + at, plane, lane, 64);
 }
 
 // ---- the products ----------------------------------------------------------------------------
@@ -238,6 +303,7 @@ struct VlGemm {
   const uint16_t *a, *b;
   int64_t a_plane, b_plane;
   int lda, ldb;
+  const float *a_scale, *b_scale;  // logits of fp32 operands: what undoes the scaling of the rows of a and of b
   const int* head;      // rows with entries
   int row0, rows;       // the rows of this call: row0 .. row0 + rows - 1 of them (pointers to rows start at row0)
   const int* only_if;   // nothing is done where it holds 0 (nullptr: always)
@@ -270,11 +336,33 @@ struct VlGemm {
   float* split;         // fp32 partial tiles
 };
 
-// Planes of a pass, the smallest products first: (0, 2), (1, 1), (2, 0), (0, 1), (1, 0), (0, 0).
+// Planes of a pass, the smallest products first: (0, 2), (1, 1), (2, 0), (0, 1), (1, 0), (0, 0); of two planes the last
+// three.
 __device__ __forceinline__ void vl_planes(int passes, int pass, int& pa, int& pb) {
-  const int i = 2 * (pass + 6 - passes);  // (a single pass: the last)
+  const int i = 2 * (pass + 6 - passes);
   pa = (0x124 >> i) & 3;
   pb = (0x046 >> i) & 3;
+}
+
+// core::quarter of fp16 operands.
+template <int I, int J>
+__device__ __forceinline__ void vl_half_quarter(f32x4 (&acc)[core::FM][core::FN], const core::AFrag& a, const core::BFrag& b) {
+  __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int k = x >> 1, n = (x & 1) * 2;
+    asm volatile(
+        "v_mfma_f32_16x16x32_f16 %[c00], %[p0], %[q0], %[c00]\n"
+        "v_mfma_f32_16x16x32_f16 %[c10], %[p0], %[q1], %[c10]\n"
+        "v_mfma_f32_16x16x32_f16 %[c01], %[p1], %[q0], %[c01]\n"
+        "v_mfma_f32_16x16x32_f16 %[c11], %[p1], %[q1], %[c11]\n"
+        : [c00] "+v"(acc[2 * I][4 * J + n]), [c10] "+v"(acc[2 * I + 1][4 * J + n]), [c01] "+v"(acc[2 * I][4 * J + n + 1]),
+          [c11] "+v"(acc[2 * I + 1][4 * J + n + 1])
+        : [p0] "v"(b[k][n]), [p1] "v"(b[k][n + 1]), [q0] "v"(a[k][0]), [q1] "v"(a[k][1])
+        : "memory");
+  }
+  __builtin_amdgcn_s_setprio(0);
+  core::barrier();
 }
 
 // Split of DH's and DW's K: with T tiles, the T mod 256 ones of the last, partial round are cut into S ranges
@@ -552,7 +640,8 @@ template <int MODE, int PLANES>
 __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   using namespace core;
   constexpr bool ATR = MODE == VL_DW, BTR = MODE == VL_DH || MODE == VL_DW, SPLIT = MODE == VL_DH || MODE == VL_DW;
-  constexpr int PASSES = PLANES == 1 ? 1 : 6;
+  constexpr bool HALF = PLANES == 3 && !BTR;  // logits of fp32 operands: fp16 hi and lo
+  constexpr int PASSES = PLANES == 1 ? 1 : HALF ? 3 : 6;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -742,6 +831,10 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step_quarter = [&](auto i, auto j, const AFrag& x, const BFrag& y) __attribute__((always_inline)) {
+    if constexpr (HALF) vl_half_quarter<decltype(i)::value, decltype(j)::value>(acc, x, y);
+    else quarter<decltype(i)::value, decltype(j)::value>(acc, x, y);
+  };
   uint8_t* ep = smem + 2 * STAGE + w * EPI;  // this wave's staging (4 KB)
   int e_ti = 0, e_left = locate(0).un;
   for (int it = 0;; ++it) {
@@ -753,7 +846,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     for (int q = 0; q < 4; ++q) read_b(b0, 0, st, 1, q);
     issue_a(it + 1, 1);
     wait_vm_barrier<5 * LU>();  // B1 of this stage
-    quarter<0, 0>(acc, a0, b0);
+    step_quarter(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, a0, b0);
     // (0, 1)
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -761,7 +854,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       for (int q = 0; q < 4; ++q) read_b(b1, 1, st, kh, q);
     issue_a(it + 2, 0);
     wait_vm_barrier<5 * LU>();  // A1 of this stage
-    quarter<0, 1>(acc, a0, b1);
+    step_quarter(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, a0, b1);
     // (1, 0)
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
@@ -769,12 +862,12 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
       for (int m = 0; m < 2; ++m) read_a(a1, 1, st, kh, m);
     issue_b(it + 2, 0);
     wait_vm_barrier<4 * LU>();  // A0, B0 of the next stage
-    quarter<1, 0>(acc, a1, b0);
+    step_quarter(std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{}, a1, b0);
     // (1, 1): the next step's first fragments (at a tile's end they are read again after its epilogue)
     read_first(nxt);
     issue_b(it + 2, 1);
     wait_lds_barrier();
-    quarter<1, 1>(acc, a1, b1);
+    step_quarter(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, a1, b1);
 
     if (--e_left > 0) continue;
     // ---- tile epilogue: this wave's 64 x 128 block (both wave groups together)
@@ -786,6 +879,21 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     const int row0 = t.tm * BM + wm * WTM, col0 = t.tn * BN + wn * WTN;
     const int er = el & 15, eg = el >> 4;  // acc[i][j]: row 16 i + er, columns 16 j + 4 eg + 0..3
 
+    if constexpr (HALF) {
+      float rs[FM];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) rs[i] = a.a_scale[min(row0 + 16 * i + er, np - 1)];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float cs = a.b_scale[min(col0 + 16 * j + 4 * eg + e, a.cols - 1)];
+#pragma unroll
+          for (int i = 0; i < FM; ++i) acc[i][j][e] = (acc[i][j][e] * rs[i]) * cs;
+        }
+      }
+    }
     if constexpr (MODE == VL_STATS) {
       float c = a.c;
       if (c < 0.0f) {
@@ -1644,11 +1752,24 @@ int64_t vl_split_slots(int64_t tiles, int64_t units) {
 // Vocabulary rows of a piece of the forward: all of them, or as many as a packed copy may have.
 int64_t vl_fwd_piece(int64_t D, int64_t V, int planes, bool packs) {
   if (!packs) return V;
-  return std::min(V, std::max<int64_t>(kPackBytes / (pad64(D) * 2 * planes) / 256, 1) * 256);
+  return std::min(V, std::max<int64_t>(kPackBytes / (pad64(D) * (planes == 3 ? 4 : 2)) / 256, 1) * 256);
 }
 
+// Copies of weight rows: bf16 planes, and for fp32 scaled fp16 with its scales.
+struct VlPackSpace {
+  size_t planes = 0, half = 0, scale = 0;
+  template <typename Take>
+  VlPackSpace(Take take, int64_t rows, int64_t Dp, int n_planes, bool bf16) {
+    planes = take(bf16 ? rows * Dp * 2 * n_planes : 0);
+    half = take(n_planes == 3 ? rows * Dp * 4 : 0);
+    scale = take(n_planes == 3 ? rows * 4 : 0);
+  }
+  VlPackSpace() = default;
+};
+
 struct VlFwdSpace {
-  size_t masks, part, row_loss, pack, bytes = 0;
+  size_t masks, part, row_loss, bytes = 0;
+  VlPackSpace pack;
   VlFwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
@@ -1659,13 +1780,14 @@ struct VlFwdSpace {
     masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
-    pack = take(packs && !vl_is_thin(T, V, packs) ? vl_fwd_piece(D, V, planes, true) * pad64(D) * 2 * planes : 0);
+    if (packs && !vl_is_thin(T, V, packs)) pack = VlPackSpace(take, vl_fwd_piece(D, V, planes, true), pad64(D), planes, planes == 1);
   }
 };
 
 struct VlBwdSpace {
   int64_t piece;
-  size_t g, sum, split, pack, bytes = 0;
+  size_t g, sum, split, bytes = 0;
+  VlPackSpace pack;
   VlBwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) : piece(vl_bwd_piece(T, V, planes)) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
@@ -1678,7 +1800,7 @@ struct VlBwdSpace {
     sum = take(V > piece ? Tp * Dp * 4 : 0);
     split = take(std::max(vl_split_slots(ceil_div(Tp, 256) * dt, ceil_div(std::min(V, piece), 64) * passes),
                           vl_split_slots(ceil_div(std::min(V, piece), 256) * dt, Tp / 64 * passes)) * (core::BM * core::BN * 4));
-    pack = take(packs ? std::min(pad64(V), piece) * Dp * 2 * planes : 0);
+    if (packs) pack = VlPackSpace(take, std::min(pad64(V), piece), Dp, planes, true);
   }
 };
 
@@ -1692,13 +1814,23 @@ bool vl_packs(const void* weight, int w_dtype, int64_t ldw, int64_t dim, int pla
   return planes != 1 || w_dtype != FMOE_BF16 || dim % 64 != 0 || ldw % 8 != 0 || !aligned16(weight);
 }
 
-int vl_pack(const void* weight, int w_dtype, int64_t ldw, int64_t v0, int64_t rows, int64_t D, int planes, uint16_t* dst,
+// A copy of rows v0 .. v0 + rows - 1 of the weight: planes at dst, for fp32 (planes = 3) fp16 at half and its scales
+// (each where it is not null); plane: elements of a plane of either.
+struct VlPacked {
+  uint16_t *dst, *half;
+  float* scale;
+  VlPacked(uint8_t* ws, const VlPackSpace& p)
+      : dst(reinterpret_cast<uint16_t*>(ws + p.planes)), half(reinterpret_cast<uint16_t*>(ws + p.half)),
+        scale(reinterpret_cast<float*>(ws + p.scale)) {}
+};
+int vl_pack(const void* weight, int w_dtype, int64_t ldw, int64_t v0, int64_t rows, int64_t D, int planes, VlPacked p,
             int64_t plane, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(ceil_div(rows, 4)));
   const int Dp = static_cast<int>(pad64(D)), r = static_cast<int>(rows), d = static_cast<int>(D);
+  uint16_t* const dst = p.dst;
   if (w_dtype == FMOE_BF16) vl_pack_kernel<FMOE_BF16, 1><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
   else if (planes == 1) vl_pack_kernel<FMOE_F32, 1><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
-  else vl_pack_kernel<FMOE_F32, 3><<<grid, 256, 0, s>>>(weight, ldw, v0, r, d, Dp, dst, plane);
+  else vl_pack32_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(weight), ldw, v0, r, d, Dp, dst, p.half, p.scale, plane);
   return launch_status();
 }
 
@@ -1755,6 +1887,7 @@ RowsArgs vl_pack_rows(const VlCall& a, const VlState& st, uint32_t* masks, hipSt
   r.inv_temp = static_cast<float>(1.0 / a.temperature);
   r.masks = a.T * a.top <= kFewEntries ? nullptr : masks;
   r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.h = st.h;
+  r.h16 = st.h16, r.h_scale = st.h_scale;
   r.loss = a.reduction == FMOE_REDUCE_NONE ? a.loss : nullptr;
   if (r.masks) vl_mark_kernel<<<grid, 1024, 0, s>>>(r);
   if (a.h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 1><<<grid, 1024, 0, s>>>(r);
@@ -1797,7 +1930,7 @@ void vl_product(const VlGemm& g, int planes, int64_t mt, int64_t nt, int64_t uni
 constexpr int64_t kFusedRows = 2048, kFusedBytes = int64_t(1) << 31;
 int64_t vl_fused_piece(int64_t T, int64_t D, int64_t V, int planes, bool packs) {
   const int64_t Vp = ceil_div(V, 256) * 256, Tp = ceil_div(std::max<int64_t>(T, 1), 256) * 256;
-  if (T <= kThinRows || V > (int64_t(1) << 22) || (packs && Vp * pad64(D) * 2 * planes > kFusedBytes)) return 0;
+  if (T <= kThinRows || V > (int64_t(1) << 22) || (packs && Vp * pad64(D) * (planes == 3 ? 10 : 2) > kFusedBytes)) return 0;
   const int64_t most = std::min(Tp, kPieceBytes / (Vp * 2 * planes) / 256 * 256);
   if (most < std::min(Tp, kFusedRows) || (most < Tp && V * pad64(D) * 4 > kFusedBytes)) return 0;
   const int64_t pieces = ceil_div(Tp, most);
@@ -1806,7 +1939,8 @@ int64_t vl_fused_piece(int64_t T, int64_t D, int64_t V, int planes, bool packs) 
 
 struct VlFusedSpace {
   int64_t piece;
-  size_t state, masks, part, row_loss, row_part, off, factor, flag, g, fh, split, sum, pack, bytes = 0;
+  size_t state, masks, part, row_loss, row_part, off, factor, flag, g, fh, split, sum, bytes = 0;
+  VlPackSpace pack;
   VlFusedSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
       : piece(vl_fused_piece(T, D, V, planes, packs)) {
     if (piece == 0) return;
@@ -1829,7 +1963,7 @@ struct VlFusedSpace {
     split = take(std::max(vl_split_slots(piece / 256 * dt, ceil_div(V, 64) * passes),
                           vl_split_slots(vt * dt, piece / 64 * passes)) * (core::BM * core::BN * 4));
     sum = take(piece < T ? V * Dp * 4 : 0);
-    pack = take(packs ? V * Dp * 2 * planes : 0);
+    if (packs) pack = VlPackSpace(take, V, Dp, planes, true);
   }
 };
 
@@ -1873,12 +2007,14 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), s);
 
   VlGemm g{};
-  g.a = st.h, g.a_plane = st.plane, g.lda = static_cast<int>(st.Dp);
+  // (the tiles' operands of fp32 are fp16; the form of few rows reads the planes)
+  const bool thin = vl_is_thin(T, vocab, packs), half = planes == 3 && !thin;
+  g.a = half ? st.h16 : st.h, g.a_plane = st.plane, g.lda = static_cast<int>(st.Dp), g.a_scale = st.h_scale;
   g.head = st.head, g.rows = static_cast<int>(T), g.k = static_cast<int>(st.Dp);
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
   g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = st.Tp;
   g.index = distill ? nullptr : st.index, g.picked = st.picked;
-  if (vl_is_thin(T, vocab, packs)) {
+  if (thin) {
     g.cols = static_cast<int>(vocab);
     vl_thin<VL_STATS>(g, weight, w_dtype, ldw, dim, planes, T, s);
   } else {
@@ -1886,10 +2022,11 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
     for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
       const int64_t rows = std::min(piece, vocab - v0);
       if (packs) {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(ws + space.pack);
-        const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, dst, piece * st.Dp, s);
+        VlPacked copy(ws, space.pack);
+        if (half) copy.dst = nullptr;
+        const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, copy, piece * st.Dp, s);
         if (rc != FMOE_OK) return rc;
-        g.b = dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp);
+        g.b = half ? copy.half : copy.dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp), g.b_scale = copy.scale;
       } else {
         g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
       }
@@ -1944,12 +2081,11 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
   const hipStream_t s = as_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint16_t* const gbuf = reinterpret_cast<uint16_t*>(ws + space.g);
-  uint16_t* const pack = reinterpret_cast<uint16_t*>(ws + space.pack);
   const int64_t piece = space.piece, g_plane = st.Tp * piece;
   const int64_t pack_plane = std::min(pad64(vocab), piece) * st.Dp;
   const int Dp = static_cast<int>(st.Dp);
   const int64_t mt = ceil_div(st.Tp, 256), dt = ceil_div(st.Dp, 256);
-  const bool thin = vl_is_thin(T, vocab, packs);
+  const bool thin = vl_is_thin(T, vocab, packs), half = planes == 3 && !thin;
   for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
     const int64_t rows = std::min(piece, vocab - v0), vt = ceil_div(rows, 256);
     VlGemm g{};
@@ -1959,12 +2095,17 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     int64_t w_plane = 0;
     int w_ld = static_cast<int>(ldw);
     if (packs && (!thin || d_hidden != nullptr)) {
-      const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, pack, pack_plane, s);
+      VlPacked copy(ws, space.pack);
+      if (!half) copy.half = nullptr;
+      else g.b = copy.half, g.b_scale = copy.scale;
+      if (planes == 3 && d_hidden == nullptr) copy.dst = nullptr;
+      const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, copy, pack_plane, s);
       if (rc != FMOE_OK) return rc;
-      w = pack, w_plane = pack_plane, w_ld = Dp;
+      w = copy.dst, w_plane = pack_plane, w_ld = Dp;
     }
-    g.a = st.h, g.a_plane = st.plane, g.lda = Dp, g.k = Dp;
-    g.b = w, g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
+    g.a = half ? st.h16 : st.h, g.a_plane = st.plane, g.lda = Dp, g.k = Dp, g.a_scale = st.h_scale;
+    if (!half) g.b = w;
+    g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
     g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
     g.index = distill ? nullptr : st.index, g.picked = st.picked;
     g.stat = st.stat, g.d_loss = d_loss, g.reduction = reduction;
@@ -1982,7 +2123,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
       vl_fix_kernel<<<dim3(static_cast<uint32_t>(ceil_div(T * top, 256))), 256, 0, s>>>(f);
     }
     VlGemm h = g;
-    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg;
+    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg, h.b = w;
     h.cols = Dp, h.vocab = static_cast<int>(rows);
     if (d_hidden != nullptr) {
       h.out = d_hidden, h.out_dtype = dh_dtype, h.sum = reinterpret_cast<float*>(ws + space.sum);
@@ -2032,21 +2173,27 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
   uint16_t* const fh = reinterpret_cast<uint16_t*>(ws + space.fh);
   float* const factor = reinterpret_cast<float*>(ws + space.factor);
   int* const flag = reinterpret_cast<int*>(ws + space.flag);
-  const uint16_t* w = static_cast<const uint16_t*>(weight);
+  const uint16_t *w = static_cast<const uint16_t*>(weight), *w16 = nullptr;
+  const float* w_scale = nullptr;
+  const bool half = planes == 3;
   int64_t w_plane = 0;
   int w_ld = static_cast<int>(ldw);
   if (packs) {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(ws + space.pack);
-    const int rc = vl_pack(weight, w_dtype, ldw, 0, vocab, dim, planes, dst, vocab * st.Dp, s);
+    VlPacked copy(ws, space.pack);
+    if (!half) copy.half = nullptr;
+    w16 = copy.half, w_scale = copy.scale;
+    const int rc = vl_pack(weight, w_dtype, ldw, 0, vocab, dim, planes, copy, vocab * st.Dp, s);
     if (rc != FMOE_OK) return rc;
-    w = dst, w_plane = vocab * st.Dp, w_ld = Dp;
+    w = copy.dst, w_plane = vocab * st.Dp, w_ld = Dp;
   }
   for (int64_t r0 = 0; r0 < std::max<int64_t>(T, 1); r0 += piece) {
     const int64_t rows = std::min(piece, T - r0);
     VlGemm g{};
     g.head = st.head, g.row0 = static_cast<int>(r0), g.rows = static_cast<int>(rows);
-    g.a = st.h + r0 * st.Dp, g.a_plane = st.plane, g.lda = Dp, g.k = Dp;
-    g.b = w, g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(vocab);
+    const uint16_t* const rows_h = st.h + r0 * st.Dp;
+    g.a = half ? st.h16 + r0 * st.Dp : rows_h, g.a_plane = st.plane, g.lda = Dp, g.k = Dp;
+    if (half) g.a_scale = st.h_scale + r0, g.b_scale = w_scale;
+    g.b = half ? w16 : w, g.b_plane = w_plane, g.ldb = w_ld, g.cols = static_cast<int>(vocab);
     g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
     g.index = distill ? nullptr : st.index + r0, g.picked = st.picked + r0 * top;
     g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = piece;
@@ -2059,7 +2206,7 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
     l.head = st.head, l.row0 = g.row0, l.n_rows = g.rows, l.perm = g.perm, l.index = st.index + r0;
     l.part = g.part, l.Tp = piece, l.pieces = static_cast<int>(2 * vt), l.stat = st.stat + r0, l.picked = g.picked;
     l.row_loss = reinterpret_cast<float*>(ws + space.row_loss) + r0;
-    l.h = g.a, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
+    l.h = rows_h, l.h_plane = st.plane, l.weight = weight, l.ldw = ldw;
     l.top = distill ? static_cast<int>(top) : 0;
     l.planes = planes, l.c = g.c, l.out_index = st.index + r0 * top, l.out_q = st.q + r0 * top, l.rows = r;
     l.factor = static_cast<float>(temperature * temperature);
@@ -2094,12 +2241,12 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
     const dim3 wave_rows(static_cast<uint32_t>(ceil_div(pad64(std::max<int64_t>(rows, 1)), 4)));
     if (planes == 1)
       vl_factor_kernel<1><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
-                                                   g.a, st.plane, Dp, factor, fh, fh_plane);
+                                                   rows_h, st.plane, Dp, factor, fh, fh_plane);
     else
       vl_factor_kernel<3><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
-                                                   g.a, st.plane, Dp, factor, fh, fh_plane);
+                                                   rows_h, st.plane, Dp, factor, fh, fh_plane);
     VlGemm h = g;
-    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg, h.cols = Dp, h.vocab = static_cast<int>(vocab);
+    h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg, h.b = w, h.cols = Dp, h.vocab = static_cast<int>(vocab);
     if (d_hidden != nullptr) {
       h.out = d_hidden, h.out_dtype = dh_dtype, h.row_factor = factor;
       // (rows without entries: once)
