@@ -760,7 +760,7 @@ def vocab_loss_fwd(hidden, weight, index, teacher, ignore_index: int, logit_scal
     w_code = _dtype_code(weight.dtype)
     packs = lib.fmoe_vocab_loss_packs(wp, w_code, ldw, d, planes)
     n_state = lib.fmoe_vocab_loss_state_bytes(T, d, top, planes)
-    n_ws = lib.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, planes, packs)
+    n_ws = lib.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, top, planes, packs)
     state = torch.empty(n_state, dtype=torch.uint8, device=dev)
     ws = torch.empty(max(n_ws, 256), dtype=torch.uint8, device=dev)
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)

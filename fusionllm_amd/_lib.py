@@ -96,7 +96,7 @@ VOCAB_SIGNATURES = {
                                    c_int, _P, c_size_t, _P]),
     "fmoe_vocab_loss_state_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "fmoe_vocab_loss_packs": (c_int, [_P, c_int, c_int64, c_int64, c_int]),
-    "fmoe_vocab_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "fmoe_vocab_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
     "fmoe_vocab_loss_fwd": (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int, c_int64, c_int64,
                                     c_int64, c_int64, c_int64, c_double, c_double, c_int, c_int, _P, _P, c_size_t,
                                     _P, c_size_t, _P]),

@@ -501,7 +501,7 @@ std::array<Tensor, 2> loss_fwd(const Tensor& h, const Tensor& w, const Tensor& i
   const int packs = api.fmoe_vocab_loss_packs(w.data_ptr(), wc, w.stride(0), d, planes);
   const size_t bytes = api.fmoe_vocab_loss_state_bytes(T, d, top, planes);
   Tensor state = empty({static_cast<int64_t>(bytes)}, at::kByte, h);
-  const Workspace ws(api.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, planes, packs), h);
+  const Workspace ws(api.fmoe_vocab_loss_fwd_workspace_bytes(T, d, V, top, planes, packs), h);
   Tensor loss = o.reduction == FMOE_REDUCE_NONE ? empty({T}, at::kFloat, h) : empty({}, at::kFloat, h);
   // (an empty tensor has no address; the entry point wants one for its output)
   float* lp = static_cast<float*>(T == 0 && o.reduction == FMOE_REDUCE_NONE ? state.data_ptr() : loss.data_ptr());

@@ -8,7 +8,8 @@
 //   G[r, v] = w[r] * (p[r, v] - q[r, v]),  dH = G W,  dW = G^T H
 // with q the row's target distribution: 1 at the target, or the teacher's softmax over its list.
 //
-// The logits [rows, vocab] are never stored.  A call whose loss is one value (mean or sum), for training, forms
+// The logits [rows, vocab] are not kept (long lists of a distillation read them from a piece of at most 256 MB,
+// vl_stores_logits below).  A call whose loss is one value (mean or sum), for training, forms
 // its gradients at once (vl_fused, below): a piece of the rows at a time, whose exponentials 2^(t - o) are G
 // up to a factor per row, which is known when the piece's logits are done.  A call with a loss per row, whose weights
 // only the backward brings, reduces a tile's logits to a maximum and a sum of exponentials per row, and forms
@@ -295,9 +296,10 @@ __global__ __launch_bounds__(256) void vl_pack32_kernel(const float* src, int64_
 // DH     G W of a piece, K split in ranges -> fp32 partial sums, added to the piece's before
 // DW     G^T H                -> the piece's rows of dW
 // PROB   t = H W^T            -> 2^(t - o), and its sum per row and 128 columns
+// LOGITS as STATS, and t of the rows
 // H and G are row-major, so A is K-contiguous but for DW (G^T: read with transposing LDS reads), and B is
 // K-contiguous for STATS, GRAD and PROB, and read as it lies, transposing, for DH (W) and DW (H).
-enum VlMode { VL_STATS = 0, VL_GRAD = 1, VL_DH = 2, VL_DW = 3, VL_PROB = 4 };
+enum VlMode { VL_STATS = 0, VL_GRAD = 1, VL_DH = 2, VL_DW = 3, VL_PROB = 4, VL_LOGITS = 5 };
 
 struct VlGemm {
   const uint16_t *a, *b;
@@ -316,6 +318,8 @@ struct VlGemm {
   float* picked;        // their t; GRAD: p - 1
   // STATS
   float2* part;         // [2 * column tiles][Tp]
+  float* logits;        // LOGITS: t, [rows][ldt]
+  int ldt;              // a multiple of 256
   int64_t Tp;
   const float* off;     // PROB: o
   // GRAD
@@ -894,7 +898,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
         }
       }
     }
-    if constexpr (MODE == VL_STATS) {
+    if constexpr (MODE == VL_STATS || MODE == VL_LOGITS) {
       float c = a.c;
       if (c < 0.0f) {
         c = -c;
@@ -902,6 +906,23 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j) acc[i][j] = -acc[i][j];
+      }
+      if constexpr (MODE == VL_LOGITS) {
+        // 16 bytes a lane, 64 of a row; the next store takes the other half of its 128
+        float* const out = a.logits + static_cast<int64_t>(row0) * a.ldt + col0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          int l = el;
+          asm volatile("" : "+v"(l));
+          const int r = 16 * i + (l & 15);
+          if (row0 + r >= n) continue;
+          float* const p = out + r * a.ldt + 4 * (l >> 4);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            asm volatile("" ::: "memory");
+            *reinterpret_cast<f32x4*>(p + 16 * j) = acc[i][j] * c;
+          }
+        }
       }
       const int piece = (a.v0 / BN + t.tn) * WN + wn;
       if (col0 + WTN <= a.cols) vl_stats_epilogue<true>(a, acc, c, n, row0, col0, piece, el);
@@ -952,7 +973,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     asm volatile("s_nop 1" ::: "memory");  // VALU writes -> MFMA reads of the accumulators
     if (++e_ti == my_items) break;
     e_left = locate(e_ti).un;
-    if constexpr (MODE == VL_GRAD || MODE == VL_PROB) {
+    if constexpr (MODE == VL_GRAD || MODE == VL_PROB || MODE == VL_LOGITS) {
       // formed again: kept across the epilogue they made it spill
       form_offsets(0);
       xa = frag_base(wm * WTM, el);
@@ -1334,6 +1355,8 @@ struct LossArgs {
   float c, factor;    // factor: temperature^2
   int top, planes;    // top 0: cross entropy
   int *out_index;     // distillation: of the packed rows
+  const float* logits;  // t of the rows, [n_rows][ldt] (nullptr: the listed ones are formed here)
+  int ldt;
   float* out_q;
   RowsArgs rows;
   int row0, n_rows;   // as in VlGemm
@@ -1401,7 +1424,7 @@ __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
 }
 
 // Distillation, a workgroup per packed row: the teacher's softmax over its list, t of the listed entries (a dot
-// product of length D each, in fp32, four entries of a wave at a time) and the loss.
+// product of length D each, in fp32, four entries of a wave at a time; or read from the stored logits) and the loss.
 __device__ __forceinline__ float vl_block_max(float v, float* red) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
@@ -1486,8 +1509,18 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
   __syncthreads();
   const float2 ml = early ? make_float2(0.0f, 0.0f) : a.stat[row];
   float cross = 0.0f, most = -__builtin_inff();
+  if (a.logits) {
+    const float* t_row = a.logits + static_cast<int64_t>(row) * a.ldt;
+    for (int k = threadIdx.x; k < top; k += 256) {
+      if (ti[k] < 0) continue;
+      const float t = t_row[ti[k]], q = tq[k];
+      most = fmaxf(most, t);
+      a.picked[out + k] = t;
+      if (!(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
+    }
+  }
   constexpr int U = 4;
-  for (int k0 = w * U; k0 < top; k0 += 4 * U) {
+  for (int k0 = w * U; k0 < (a.logits ? 0 : top); k0 += 4 * U) {
     float acc[U][4];
     int64_t at[U];
     bool on[U];
@@ -1524,14 +1557,14 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
       const float t = s * a.c, q = tq[k0 + u];
       most = fmaxf(most, t);
       if (lane == 0) a.picked[out + k0 + u] = t;
-      if (!(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
+      if (lane == 0 && !(q == 0.0f)) cross = fmaf(q, (ml.x - t) + ml.y, cross);
     }
   }
   if (early) {
     // o: the largest listed t.  Sum of q (o - t), with o known only now
     most = vl_block_max(most, red);
     if (most == -__builtin_inff()) most = 0.0f;
-    __syncthreads();  // (picked, written by this workgroup's lanes 0)
+    __syncthreads();  // (picked, written by this workgroup)
     cross = 0.0f;
     for (int k = threadIdx.x; k < top; k += 256)
       if (ti[k] >= 0 && !(tq[k] == 0.0f)) cross = fmaf(tq[k], most - a.picked[out + k], cross);
@@ -1542,7 +1575,7 @@ __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
     }
     return;
   }
-  cross = vl_block_sum(lane == 0 ? cross : 0.0f, red);
+  cross = vl_block_sum(cross, red);
   if (threadIdx.x == 0) {
     float v = fmaf(cross, kLn2, ent) * a.factor;
     if (row_bad) {
@@ -1755,6 +1788,24 @@ int64_t vl_fwd_piece(int64_t D, int64_t V, int planes, bool packs) {
   return std::min(V, std::max<int64_t>(kPackBytes / (pad64(D) * (planes == 3 ? 4 : 2)) / 256, 1) * 256);
 }
 
+// Listed logits of a distillation: dot products, which read top * D elements of the weight a row (4 .. 9 TB/s out of the
+// caches), or their product with all of the vocabulary, stored a piece of the rows at a time (4 V bytes a row written,
+// a line read for each listed one).  Where the statistics come first the product is there anyhow (8192 rows x 2944, vocab
+// 1664, 156 listed: 993 us with dot products, 205 stored; 4096 x 768 x 32768: 64 listed 301 and 321, 256 listed 591 and
+// 386); gradients at once need the lists before their product, and so one more (8192 x 2944 x 1664, 156 listed: 1243 and
+// 526; 4096 x 2048 x 32768: 64 listed 1543 and 1954, 256 listed 2075 and 1970; fp32, 2000 x 1024 x 8192, 128 listed: 689
+// and 673).
+constexpr int64_t kLogitBytes = int64_t(1) << 28;
+bool vl_stores_logits(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool once_more) {
+  const int64_t read = top * D * (planes == 3 ? 4 : 2);
+  if (top == 1 || T <= kThinRows || V * 4 * 1024 > kLogitBytes) return false;  // (top 1: also cross entropy)
+  return once_more ? T >= 1024 && read > 5 * V + planes * V * D / 80 : read > 5 * V;
+}
+// Rows whose logits are stored at a time.
+int64_t vl_logit_rows(int64_t T, int64_t V) {
+  return std::min(ceil_div(T, 256), kLogitBytes / (ceil_div(V, 256) * 1024) / 256) * 256;
+}
+
 // Copies of weight rows: bf16 planes, and for fp32 scaled fp16 with its scales.
 struct VlPackSpace {
   size_t planes = 0, half = 0, scale = 0;
@@ -1768,9 +1819,12 @@ struct VlPackSpace {
 };
 
 struct VlFwdSpace {
-  size_t masks, part, row_loss, bytes = 0;
+  size_t masks, part, row_loss, logits, bytes = 0;
+  bool stored;  // the logits, a piece of the rows at a time
   VlPackSpace pack;
-  VlFwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) {
+  VlFwdSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
+      : stored(!vl_is_thin(T, V, packs) && vl_fwd_piece(D, V, planes, packs) >= V &&
+               vl_stores_logits(T, D, V, top, planes, false)) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += (n + 255) & ~size_t(255);
@@ -1780,6 +1834,7 @@ struct VlFwdSpace {
     masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
+    logits = take(stored ? vl_logit_rows(T, V) * ceil_div(V, 256) * 1024 : 0);
     if (packs && !vl_is_thin(T, V, packs)) pack = VlPackSpace(take, vl_fwd_piece(D, V, planes, true), pad64(D), planes, planes == 1);
   }
 };
@@ -1909,6 +1964,36 @@ void vl_lists(const LossArgs& l, int w_dtype, int64_t rows, hipStream_t s) {
   else vl_list_kernel<FMOE_F32><<<grid, 256, 0, s>>>(l);
 }
 
+// STATS or LOGITS of up to so many rows.
+template <int MODE>
+void vl_stats(const VlGemm& g, int planes, int64_t rows, hipStream_t s) {
+  const dim3 grid = vl_grid(ceil_div(rows, 256) * ceil_div(g.cols, 256));
+  if (planes == 1) vl_gemm_kernel<MODE, 1><<<grid, core::NT, 0, s>>>(g);
+  else vl_gemm_kernel<MODE, 3><<<grid, core::NT, 0, s>>>(g);
+}
+
+// The lists of g's and l's `rows` rows from stored logits, `most` rows at a time; stat: with the rows' statistics between.
+void vl_stored_lists(const VlGemm& g, const LossArgs& l, int w_dtype, int64_t rows, int64_t most, int64_t Dp, int top,
+                     bool stat, hipStream_t s) {
+  for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    const int64_t here = std::min(most, rows - r0);
+    VlGemm q = g;
+    q.row0 += static_cast<int>(r0), q.rows = static_cast<int>(here);
+    q.a += r0 * Dp, q.part += r0;
+    if (l.planes == 3) q.a_scale += r0;
+    vl_stats<VL_LOGITS>(q, l.planes, here, s);
+    LossArgs m = l;
+    m.row0 = q.row0, m.n_rows = q.rows, m.perm += r0, m.part += r0, m.stat += r0, m.index += r0, m.h += r0 * Dp;
+    m.picked += r0 * top, m.out_index += r0 * top, m.out_q += r0 * top;
+    if (m.row_loss) m.row_loss += r0;
+    if (m.off) m.off += r0;
+    if (m.row_part) m.row_part += r0;
+    m.logits = g.logits, m.ldt = g.ldt;
+    if (stat) vl_stat(m, here, s);
+    vl_lists(m, w_dtype, here, s);
+  }
+}
+
 // DH and DW with their split tiles; rest of DH's result (rows without entries) with its last piece.
 template <int MODE>
 void vl_product(const VlGemm& g, int planes, int64_t mt, int64_t nt, int64_t units, const int* inv, int64_t T, hipStream_t s) {
@@ -1939,7 +2024,8 @@ int64_t vl_fused_piece(int64_t T, int64_t D, int64_t V, int planes, bool packs) 
 
 struct VlFusedSpace {
   int64_t piece;
-  size_t state, masks, part, row_loss, row_part, off, factor, flag, g, fh, split, sum, bytes = 0;
+  size_t state, masks, part, row_loss, row_part, off, factor, flag, logits, g, fh, split, sum, bytes = 0;
+  bool stored;  // the logits, for the lists: of a part of the piece at a time
   VlPackSpace pack;
   VlFusedSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
       : piece(vl_fused_piece(T, D, V, planes, packs)) {
@@ -1958,6 +2044,8 @@ struct VlFusedSpace {
     off = take(piece * 4);
     factor = take(piece * 4);
     flag = take(4);
+    stored = vl_stores_logits(T, D, V, top, planes, true);
+    logits = take(stored ? vl_logit_rows(piece, V) * vt * 1024 : 0);
     g = take(piece * vt * 512 * planes);
     fh = take(piece * Dp * 2 * planes);
     split = take(std::max(vl_split_slots(piece / 256 * dt, ceil_div(V, 64) * passes),
@@ -1979,8 +2067,9 @@ extern "C" int fmoe_vocab_loss_packs(const void* weight, int w_dtype, int64_t ld
   return vl_packs(weight, w_dtype, ldw, dim, planes);
 }
 
-extern "C" size_t fmoe_vocab_loss_fwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int planes, int packs) {
-  return vl_sizes_ok(T, dim, vocab, 1, planes) ? VlFwdSpace(T, dim, vocab, planes, packs).bytes : 0;
+extern "C" size_t fmoe_vocab_loss_fwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes,
+                                                      int packs) {
+  return vl_sizes_ok(T, dim, vocab, top, planes) ? VlFwdSpace(T, dim, vocab, top, planes, packs).bytes : 0;
 }
 
 extern "C" size_t fmoe_vocab_loss_bwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int planes, int packs) {
@@ -1998,7 +2087,7 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   const bool distill = call.distill();
   if (const int rc = vl_check(call, state, workspace); rc != FMOE_OK) return rc;
   const bool packs = vl_packs(weight, w_dtype, ldw, dim, planes);
-  const VlFwdSpace space(T, dim, vocab, planes, packs);
+  const VlFwdSpace space(T, dim, vocab, top, planes, packs);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const VlState st(static_cast<uint8_t*>(state), T, dim, top, planes);
   if (state == nullptr || state_bytes < st.bytes || workspace == nullptr || workspace_bytes < space.bytes)
@@ -2014,29 +2103,6 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
   g.part = reinterpret_cast<float2*>(ws + space.part), g.Tp = st.Tp;
   g.index = distill ? nullptr : st.index, g.picked = st.picked;
-  if (thin) {
-    g.cols = static_cast<int>(vocab);
-    vl_thin<VL_STATS>(g, weight, w_dtype, ldw, dim, planes, T, s);
-  } else {
-    const int64_t piece = vl_fwd_piece(dim, vocab, planes, packs);
-    for (int64_t v0 = 0; v0 < vocab; v0 += piece) {
-      const int64_t rows = std::min(piece, vocab - v0);
-      if (packs) {
-        VlPacked copy(ws, space.pack);
-        if (half) copy.dst = nullptr;
-        const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, copy, piece * st.Dp, s);
-        if (rc != FMOE_OK) return rc;
-        g.b = half ? copy.half : copy.dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp), g.b_scale = copy.scale;
-      } else {
-        g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
-      }
-      g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
-      const dim3 grid = vl_grid(ceil_div(st.Tp, 256) * ceil_div(rows, 256));
-      if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(g);
-      else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(g);
-    }
-  }
-
   LossArgs l{};
   l.head = st.head, l.perm = st.perm, l.index = st.index, l.part = g.part, l.Tp = st.Tp;
   l.pieces = static_cast<int>(2 * ceil_div(vocab, 256));
@@ -2047,7 +2113,31 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   l.top = distill ? static_cast<int>(top) : 0;
   l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r, l.n_rows = g.rows;
   l.factor = static_cast<float>(temperature * temperature);
-  if (T > 0) {
+
+  if (thin) {
+    g.cols = static_cast<int>(vocab);
+    vl_thin<VL_STATS>(g, weight, w_dtype, ldw, dim, planes, T, s);
+  }
+  const int64_t piece = vl_fwd_piece(dim, vocab, planes, packs);
+  for (int64_t v0 = 0; v0 < vocab && !thin; v0 += piece) {
+    const int64_t rows = std::min(piece, vocab - v0);
+    if (packs) {
+      VlPacked copy(ws, space.pack);
+      if (half) copy.dst = nullptr;
+      const int rc = vl_pack(weight, w_dtype, ldw, v0, rows, dim, planes, copy, piece * st.Dp, s);
+      if (rc != FMOE_OK) return rc;
+      g.b = half ? copy.half : copy.dst, g.b_plane = piece * st.Dp, g.ldb = static_cast<int>(st.Dp), g.b_scale = copy.scale;
+    } else {
+      g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
+    }
+    g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
+    if (space.stored) break;  // (one piece of the vocabulary)
+    vl_stats<VL_STATS>(g, planes, st.Tp, s);
+  }
+  if (space.stored) {
+    g.logits = reinterpret_cast<float*>(ws + space.logits), g.ldt = static_cast<int>(ceil_div(vocab, 256) * 256);
+    vl_stored_lists(g, l, w_dtype, T, vl_logit_rows(T, vocab), st.Dp, static_cast<int>(top), true, s);
+  } else if (T > 0) {
     vl_stat(l, T, s);
     if (distill) vl_lists(l, w_dtype, T, s);
   }
@@ -2214,7 +2304,11 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
     if (distill) l.row_part = reinterpret_cast<float*>(ws + space.row_part);
 
     const dim3 grid = vl_grid(mt * vt);
-    if (distill) vl_lists(l, w_dtype, std::max<int64_t>(rows, 1), s);
+    if (space.stored) {
+      VlGemm q = g;
+      q.logits = reinterpret_cast<float*>(ws + space.logits), q.ldt = g.ldg;
+      vl_stored_lists(q, l, w_dtype, std::max<int64_t>(rows, 1), vl_logit_rows(piece, vocab), st.Dp, static_cast<int>(top), false, s);
+    } else if (distill) vl_lists(l, w_dtype, std::max<int64_t>(rows, 1), s);
     else if (w_dtype == FMOE_BF16) vl_off_kernel<FMOE_BF16><<<dim3(static_cast<uint32_t>(ceil_div(std::max<int64_t>(rows, 1), 4))), 256, 0, s>>>(l);
     else vl_off_kernel<FMOE_F32><<<dim3(static_cast<uint32_t>(ceil_div(std::max<int64_t>(rows, 1), 4))), 256, 0, s>>>(l);
     if (planes == 1) vl_gemm_kernel<VL_PROB, 1><<<grid, core::NT, 0, s>>>(g);
@@ -2225,8 +2319,7 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
     LossArgs lq = l;
     q.only_if = lq.only_if = flag;
     lq.flag = nullptr;
-    if (planes == 1) vl_gemm_kernel<VL_STATS, 1><<<grid, core::NT, 0, s>>>(q);
-    else vl_gemm_kernel<VL_STATS, 3><<<grid, core::NT, 0, s>>>(q);
+    vl_stats<VL_STATS>(q, planes, piece, s);
     vl_stat(lq, std::max<int64_t>(rows, 1), s);
     q.index = nullptr;  // (the listed entries follow)
     if (planes == 1) vl_gemm_kernel<VL_GRAD, 1><<<grid, core::NT, 0, s>>>(q);

@@ -73,7 +73,7 @@ size_t fmoe_vocab_loss_state_bytes(int64_t T, int64_t dim, int64_t top, int plan
 /* 1 where the products read a copy of weight, made a piece at a time, rather than weight as it lies
  * (bf16 rows of a multiple of 64 elements at 16-byte addresses): an argument of the size queries. */
 int fmoe_vocab_loss_packs(const void* weight, int w_dtype, int64_t ldw, int64_t dim, int planes);
-size_t fmoe_vocab_loss_fwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int planes, int packs);
+size_t fmoe_vocab_loss_fwd_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes, int packs);
 int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh, const void* weight, int w_dtype,
                         int64_t ldw, const void* index, int index64, const void* teacher, int t_dtype,
                         int64_t T, int64_t dim, int64_t vocab, int64_t top, int64_t ignore_index,

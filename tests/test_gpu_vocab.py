@@ -252,6 +252,21 @@ def test_distillation(gpu_device, T, V, D, K, reduction, tau, dtype):
     _check(loss, h, w, up, _reference(h, w, index, z, -100, 0.9, tau, reduction, up))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("T,V,D,K", [(1500, 60000, 512, 800), (1030, 130, 96, 50)])
+def test_long_lists(gpu_device, T, V, D, K, reduction, dtype):
+    # lists read from stored logits, the first in two parts of the rows
+    g = _gen(T + K)
+    h, w, _ = _operands(g, T, V, D, dtype, gpu_device, pull=False)
+    index, z = _lists(g, T, V, K, gpu_device, repeat=True)
+    index[::6] = -100
+    z = z.to(dtype)
+    up = torch.rand(T, generator=g).to(gpu_device) if reduction == "none" else torch.tensor(1.0, device=gpu_device)
+    loss = linear_distillation(h, w, index, z, temperature=2.0, reduction=reduction)
+    _check(loss, h, w, up, _reference(h, w, index, z, -100, 1.0, 2.0, reduction, up))
+
+
 @pytest.mark.parametrize("T,V,D,K,dtype", [(24000, 46000, 64, 3, torch.bfloat16), (8200, 45000, 96, 2, torch.float32),
                                            (70, 600, 16384, 20, torch.float32), (9, 300, 16384, 20, torch.bfloat16),
                                            (2100, 9000, 640, 1, torch.bfloat16)])

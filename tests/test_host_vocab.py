@@ -58,7 +58,7 @@ def test_embedding_argument_errors_without_gpu():
 def test_loss_argument_errors_without_gpu():
     lib = _lib.load()
     state = lib.fmoe_vocab_loss_state_bytes(4, 64, 1, 1)
-    fws = lib.fmoe_vocab_loss_fwd_workspace_bytes(4, 64, 100, 1, 0)
+    fws = lib.fmoe_vocab_loss_fwd_workspace_bytes(4, 64, 100, 1, 1, 0)
     bws = lib.fmoe_vocab_loss_bwd_workspace_bytes(4, 64, 100, 1, 0)
     assert state > 0 and fws > 0 and bws > 0
 
@@ -145,7 +145,7 @@ def test_workspaces_stay_bounded():
     assert n <= (1 << 31) + (1 << 28) + 32768 * 2048 * 4 + 1024
     assert n < 32768 * 131072 * 2 // 3
     # the forward's: a maximum and a sum per row and 128 columns
-    assert lib.fmoe_vocab_loss_fwd_workspace_bytes(32768, 2048, 131072, 1, 0) <= 32768 * 1024 * 8 + (1 << 18)
+    assert lib.fmoe_vocab_loss_fwd_workspace_bytes(32768, 2048, 131072, 1, 1, 0) <= 32768 * 1024 * 8 + (1 << 18)
     # gradients at once: a piece of 8192 rows, d_weight's sum, partial tiles, packed and scaled rows
     n = lib.fmoe_vocab_loss_grad_workspace_bytes(32768, 2048, 131072, 1, 1, 0)
     assert 0 < n <= (1 << 31) + 131072 * 2048 * 4 + (1 << 28) + 33792 * 2048 * 2 + 8192 * (2048 * 2 + 1024 * 8) + (1 << 20)
