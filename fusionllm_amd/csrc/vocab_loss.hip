@@ -41,7 +41,7 @@ namespace fmoe {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kVlCus = 256;        // workgroups of the persistent products: one per CU
-constexpr int kRowBlock = 32;      // rows per workgroup of the packing
+constexpr int kRowBlock = 32;      // rows of a mask
 constexpr int kGroup = 4;          // row tiles that are walked together, column by column (8: 0.5 % slower, 16: 4 %)
 // index of a listed entry: none, or outside the vocabulary
 constexpr int kNone = -1, kBad = -2;
@@ -210,62 +210,75 @@ __device__ __forceinline__ void vl_half_row(const float* src, int n, int np, uin
   }
 }
 
-template <int DT, int PLANES>
+// RB rows per workgroup: 32, two a wave; or 4, four waves each, where that leaves few workgroups.  The zeros up to the next
+// multiple of 64 rows are shared out (5 rows x 3832 in fp32: 31 us by one workgroup of 32 rows, 7 us by 16 of 4).
+template <int DT, int PLANES, int RB>
 __global__ __launch_bounds__(1024) void vl_rows_kernel(const RowsArgs a) {
+  constexpr int WAVES = RB < 16 ? 16 / RB : 1;  // per row
   __shared__ uint32_t bits[kFewEntries / 32];
-  __shared__ int before_s[16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, block = blockIdx.x;
-  const int block0 = block * kRowBlock;
-  if (a.masks == nullptr) vl_mark_rows(a, 0, min(block0 + kRowBlock, a.T), bits);
+  __shared__ int2 before_s[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int block0 = static_cast<int>(blockIdx.x) * RB, word = block0 / 32;
+  if (a.masks == nullptr) vl_mark_rows(a, 0, a.T, bits);
   const uint32_t* masks = a.masks ? a.masks : bits;
-  int before = 0;
-  for (int i = threadIdx.x; i < block; i += 1024) before += __popc(masks[i]);
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < (a.T + 31) / 32; i += 1024) {
+    const int c = __popc(masks[i]);
+    all += c;
+    if (i < word) before += c;
+  }
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64);
-  if (lane == 0) before_s[w] = before;
-  const uint32_t mask = block0 < a.T ? masks[block] : 0;
+  for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off, 64), all += __shfl_xor(all, off, 64);
+  if (lane == 0) before_s[w] = make_int2(before, all);
+  const uint32_t mask = block0 < a.T ? masks[word] : 0;
   __syncthreads();
-  int base = 0;
+  int base = 0, n = 0;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) base += before_s[q];
-  const int n = base + __popc(mask);
-  if (block + 1 == static_cast<int>(gridDim.x)) {  // zeros up to the next multiple of 64 rows
-    if (threadIdx.x == 0) a.head[0] = n;
-    for (int r = n + w; r < pad_rows(n); r += 16)
+  for (int q = 0; q < 16; ++q) base += before_s[q].x, n += before_s[q].y;
+  if (block0 == 0 && threadIdx.x == 0) a.head[0] = n;
+  for (int r = n + static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) * w; r < pad_rows(n); r += gridDim.x * 16) {
+    for (int c = lane * 8; c < a.Dp; c += 512)
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p)
+        *reinterpret_cast<uint4*>(a.h + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
+    if (PLANES == 3 && a.h16) {
+      if (lane == 0) a.h_scale[r] = 1.0f;
       for (int c = lane * 8; c < a.Dp; c += 512)
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-          *reinterpret_cast<uint4*>(a.h + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
-    if constexpr (PLANES == 3)
-      for (int r = n + w; r < pad_rows(n); r += 16) {
-        if (lane == 0) a.h_scale[r] = 1.0f;
-        for (int c = lane * 8; c < a.Dp; c += 512)
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-            *reinterpret_cast<uint4*>(a.h16 + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
-      }
+        for (int p = 0; p < 2; ++p)
+          *reinterpret_cast<uint4*>(a.h16 + p * a.plane + static_cast<int64_t>(r) * a.Dp + c) = make_uint4(0, 0, 0, 0);
+    }
   }
-  for (int i = w; i < kRowBlock && block0 + i < a.T; i += 16) {
+  for (int i = w / WAVES; i < RB && block0 + i < a.T; i += 16 / WAVES) {
     const int64_t t = block0 + i;
-    if (!((mask >> i) & 1)) {
-      if (lane == 0) {
+    const int bit = t & 31;
+    const bool first = lane == 0 && w % WAVES == 0;
+    if (!((mask >> bit) & 1)) {
+      if (first) {
         a.inv[t] = -1;
         if (a.loss) a.loss[t] = 0.0f;
       }
       continue;
     }
-    const int r = base + __popc(mask & ((1u << i) - 1));
-    if (lane == 0) {
+    const int r = base + __popc(mask & ((1u << bit) - 1));
+    if (first) {
       a.inv[t] = r;
       a.perm[r] = static_cast<int>(t);
       float z;
       if (a.t_dtype < 0) a.out_index[r] = vl_entry(a, t, z);
     }
-    vl_copy_row<DT, PLANES>(a.hidden, t * a.ldh, a.D, a.Dp, a.h + static_cast<int64_t>(r) * a.Dp, a.plane, lane, 64);
+    vl_copy_row<DT, PLANES>(a.hidden, t * a.ldh, a.D, a.Dp, a.h + static_cast<int64_t>(r) * a.Dp, a.plane,
+                            (w % WAVES) * 64 + lane, 64 * WAVES);
     if constexpr (PLANES == 3)
-      vl_half_row(static_cast<const float*>(a.hidden) + t * a.ldh, a.D, a.Dp, a.h16 + static_cast<int64_t>(r) * a.Dp, a.plane,
-                  a.h_scale + r, lane);
+      if (a.h16 && w % WAVES == 0)
+        vl_half_row(static_cast<const float*>(a.hidden) + t * a.ldh, a.D, a.Dp, a.h16 + static_cast<int64_t>(r) * a.Dp, a.plane,
+                    a.h_scale + r, lane);
   }
+}
+template <int DT, int PLANES>
+void vl_rows_launch(const RowsArgs& r, hipStream_t s) {
+  if (r.T <= 1024) vl_rows_kernel<DT, PLANES, 4><<<dim3(static_cast<uint32_t>(std::max((r.T + 3) / 4, 16))), 1024, 0, s>>>(r);
+  else vl_rows_kernel<DT, PLANES, 32><<<dim3(static_cast<uint32_t>((r.T + 31) / 32)), 1024, 0, s>>>(r);
 }
 
 // Rows v0 .. v0 + rows - 1 of the weight as padded planes: where its rows are not bf16 of a multiple of 64
@@ -997,9 +1010,12 @@ __device__ __forceinline__ void vl_join(float& m, float& s, float m2, float s2) 
 // ---- logits of few rows ------------------------------------------------------------------------------
 // Up to 64 rows (T, which the host knows): bound by the read of the weight, which a 256-row tile would stream through
 // few workgroups (37 rows, vocab 32768, dim 768: 128 tiles).  A workgroup takes 128 columns, a wave 16 of them and all
-// rows; the wave's part of the weight goes from memory straight into the fragments, 8 loads in flight, as it lies
-// (any dtype, stride and alignment: no packed copy), the rows' K piece through LDS.  planes = 3: the products are
-// v_mfma_f32_16x16x4_f32 on fp32 operands, at up to 64 rows as fast as the weight arrives.
+// rows; the wave's part of the weight goes from memory straight into the fragments, as it lies (any dtype, stride and
+// alignment: no packed copy), the rows' K piece through LDS.  The loads of 8 steps (4 of 64 rows, for registers) are issued at a
+// time, 512 bytes of each weight row: issued one by one, 64 bytes of 32768 rows all over the chip, they reach half of
+// the memory's rate (5 rows x 2048, vocab 131072: 164 us, in groups 116, 4.6 TB/s; 37 x 768 x 32768: 26 and 23).
+// planes = 3: the products are v_mfma_f32_16x16x4_f32 on fp32 operands, which are done as the weight arrives up to 32 rows;
+// 49 rows x 3832, vocab 24448, are bound by them (200 us; 5 rows 97).
 constexpr int kThinRows = 64;
 constexpr int kThinBytes = 1024;             // of a row's K piece in LDS
 constexpr int kThinRow = kThinBytes + 16;    // (the 16 rows of a fragment in different banks)
@@ -1025,7 +1041,8 @@ template <int MODE, int WT, int PLANES, int MB>
 __global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const ThinWeight wt) {
   constexpr bool F = PLANES == 3;
   constexpr int E = F ? 4 : 8;               // elements per lane and step; a step is 4 E of K
-  constexpr int KC = kThinBytes / (F ? 4 : 2), STEPS = KC / (4 * E), RING = WT == FMOE_F32 && PLANES == 1 ? 4 : 8;
+  // (RING steps' loads are issued while RING others are multiplied)
+  constexpr int KC = kThinBytes / (F ? 4 : 2), STEPS = KC / (4 * E), RING = (WT == FMOE_F32 && PLANES == 1 ? 4 : 8) / (MB == 4 ? 2 : 1);
   constexpr int HV = MB * 2;                 // 16-byte pieces of the rows per thread
   static_assert(STEPS == 16 && HV * 512 == 16 * MB * 64);
   __shared__ __attribute__((aligned(16))) uint8_t hs[16 * MB * kThinRow];
@@ -1054,10 +1071,10 @@ __global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const T
     }
     return f;
   };
-  Frag ring[RING];
+  Frag ring[2][RING];
 #pragma unroll
   for (int g = 0; g < RING; ++g)
-    if (g < full) ring[g] = load(g);
+    if (g < full) ring[0][g] = load(g);
   // the rows' K piece from step g0 on (zeros up to Dp, a multiple of 64; what is past that is not read)
   ThinRow<PLANES> hv[HV];
   auto load_rows = [&](int g0) __attribute__((always_inline)) {
@@ -1131,11 +1148,12 @@ __global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const T
     if (g0 + STEPS < total) load_rows(g0 + STEPS);  // under this piece's products
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      if (g0 + s < full) {
-        const Frag f = ring[s % RING];
-        if (g0 + s + RING < full) ring[s % RING] = load(g0 + s + RING);
-        multiply(f, s);
+      if (s % RING == 0) {
+#pragma unroll
+        for (int g = 0; g < RING; ++g)
+          if (g0 + s + RING + g < full) ring[(s / RING + 1) & 1][g] = load(g0 + s + RING + g);
       }
+      if (g0 + s < full) multiply(ring[(s / RING) & 1][s % RING], s);
     }
   }
   if (full < total) {  // the end of rows whose length is no multiple of a step's
@@ -1932,8 +1950,7 @@ int vl_check(const VlCall& a, const void* state, const void* workspace) {
 }
 
 // Packs the rows with entries; the arguments for those that read lists later.
-RowsArgs vl_pack_rows(const VlCall& a, const VlState& st, uint32_t* masks, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(std::max<int64_t>(ceil_div(a.T, kRowBlock), 1)));
+RowsArgs vl_pack_rows(const VlCall& a, const VlState& st, uint32_t* masks, bool half, hipStream_t s) {
   RowsArgs r{};
   r.hidden = a.hidden, r.index = a.index, r.teacher = a.teacher, r.ldh = a.ldh, r.ignore = a.ignore_index;
   r.index64 = a.index64, r.t_dtype = a.distill() ? a.t_dtype : -1;
@@ -1942,12 +1959,12 @@ RowsArgs vl_pack_rows(const VlCall& a, const VlState& st, uint32_t* masks, hipSt
   r.inv_temp = static_cast<float>(1.0 / a.temperature);
   r.masks = a.T * a.top <= kFewEntries ? nullptr : masks;
   r.head = st.head, r.perm = st.perm, r.inv = st.inv, r.out_index = st.index, r.h = st.h;
-  r.h16 = st.h16, r.h_scale = st.h_scale;
+  r.h16 = half ? st.h16 : nullptr, r.h_scale = st.h_scale;
   r.loss = a.reduction == FMOE_REDUCE_NONE ? a.loss : nullptr;
-  if (r.masks) vl_mark_kernel<<<grid, 1024, 0, s>>>(r);
-  if (a.h_dtype == FMOE_BF16) vl_rows_kernel<FMOE_BF16, 1><<<grid, 1024, 0, s>>>(r);
-  else if (a.planes == 1) vl_rows_kernel<FMOE_F32, 1><<<grid, 1024, 0, s>>>(r);
-  else vl_rows_kernel<FMOE_F32, 3><<<grid, 1024, 0, s>>>(r);
+  if (r.masks) vl_mark_kernel<<<dim3(static_cast<uint32_t>(ceil_div(a.T, kRowBlock))), 1024, 0, s>>>(r);
+  if (a.h_dtype == FMOE_BF16) vl_rows_launch<FMOE_BF16, 1>(r, s);
+  else if (a.planes == 1) vl_rows_launch<FMOE_F32, 1>(r, s);
+  else vl_rows_launch<FMOE_F32, 3>(r, s);
   return r;
 }
 
@@ -2093,11 +2110,11 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   if (state == nullptr || state_bytes < st.bytes || workspace == nullptr || workspace_bytes < space.bytes)
     return FMOE_ERR_WORKSPACE;
   const hipStream_t s = as_stream(stream);
-  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), s);
-
-  VlGemm g{};
   // (the tiles' operands of fp32 are fp16; the form of few rows reads the planes)
   const bool thin = vl_is_thin(T, vocab, packs), half = planes == 3 && !thin;
+  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), half, s);
+
+  VlGemm g{};
   g.a = half ? st.h16 : st.h, g.a_plane = st.plane, g.lda = static_cast<int>(st.Dp), g.a_scale = st.h_scale;
   g.head = st.head, g.rows = static_cast<int>(T), g.k = static_cast<int>(st.Dp);
   g.c = static_cast<float>(logit_scale / temperature * static_cast<double>(kLog2e));
@@ -2254,7 +2271,7 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
   const hipStream_t s = as_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const VlState st(ws + space.state, T, dim, top, planes);
-  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), s);
+  const RowsArgs r = vl_pack_rows(call, st, reinterpret_cast<uint32_t*>(ws + space.masks), true, s);
 
   const int Dp = static_cast<int>(st.Dp);
   const int64_t piece = space.piece, vt = ceil_div(vocab, 256), dt = ceil_div(st.Dp, 256), mt = piece / 256;
