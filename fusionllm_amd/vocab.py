@@ -2,12 +2,12 @@
 the blocks, and the losses behind them that take the hidden states and the
 vocabulary's weight, ``linear_cross_entropy`` and ``linear_distillation``.
 
-``embedding(ids, weight, scale)`` is ``scale * weight[ids]``.  Its backward sorts
-the tokens by id and adds each id's rows in fp32 in a fixed order: the same
+``embedding(ids, weight, scale)`` is ``scale * weight[ids]``.  Its backward adds each
+id's rows in fp32 in a fixed order (above 64 tokens they are sorted by id first): the same
 bits every run, no atomics.
 
 The losses are those of the logits ``s = logit_scale * hidden @ weight.T``,
-which are never stored.  A loss of one value (mean, sum) that needs gradients forms them in
+which are not kept (a distillation with long lists forms them a piece of 256 MB at a time).  A loss of one value (mean, sum) that needs gradients forms them in
 its forward, a piece of the rows at a time (up to 2 GiB), and its backward scales
 them by the loss's gradient.  A loss per row (none), and one of up to 64 rows or of a vocabulary too
 large for such pieces, reduces the logits tile by tile in the forward and forms

@@ -35,10 +35,10 @@ int fmoe_embedding_fwd(const void* ids, int index64, const void* weight, int dty
                        int64_t T, int64_t vocab, int64_t dim, float scale, void* y, void* stream);
 
 /* Its backward: d_weight[v] = scale * sum of dy[t] over the t with ids[t] = v, every row
- * written (zeros where v has no token).  The tokens are sorted by id, stably; a row is summed in
- * fp32, in a fixed order (pieces of 16 of an id's tokens where it has many), without atomics: the
- * same bits every run.  Rows of padding_idx (-1: none) stay zero, ids out of range add nothing.
- * Row t of dy starts at dy + t * lddy.  workspace: 256-byte aligned. */
+ * written (zeros where v has no token).  A row is summed in fp32, in a fixed order, without atomics: the
+ * same bits every run (up to 64 tokens in their order; more are sorted by id, stably, and an id with many
+ * is summed in pieces of 16).  Rows of padding_idx (-1: none) stay zero, ids out of range add nothing.
+ * Row t of dy starts at dy + t * lddy.  workspace: 256-byte aligned (up to 64 tokens need none: 0 bytes). */
 size_t fmoe_embedding_bwd_workspace_bytes(int64_t T, int64_t vocab, int64_t dim);
 int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtype, int64_t lddy,
                        int64_t T, int64_t vocab, int64_t dim, float scale, int64_t padding_idx,

@@ -57,6 +57,7 @@ def _embed_bound(ids, dy, w, scale, pad):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,V,D,scale", [(1, 1, 1, 1.0), (1, 32768, 768, 1.0), (7, 3, 5, 2.5), (64, 512, 512, 1.0),
+                                         (64, 1, 1500, 0.5), (63, 4099, 520, 2.0), (65, 2, 300, 1.0),
                                          (601, 513, 2048, 45.25), (1000, 1024, 513, -0.5), (4099, 50021, 1000, 1.0),
                                          (3000, 7, 768, 1.0), (40000, 2, 64, 27.75), (9000, 1, 520, 1.0)])
 def test_embedding_and_its_gradient(gpu_device, T, V, D, scale, dtype):

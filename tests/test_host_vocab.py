@@ -42,16 +42,18 @@ def test_embedding_argument_errors_without_gpu():
     assert fwd(ids=FAKE + 4) == 3 and fwd(ids=FAKE + 2, i64=0) == 3 and fwd(w=FAKE + 2) == 3 and fwd(y=FAKE + 1, dt=0) == 3
     assert fwd(T=0) == 0 and fwd(T=0, ids=None, w=None, y=None) == 0
 
-    size = lib.fmoe_embedding_bwd_workspace_bytes(4, 10, 64)
+    size = lib.fmoe_embedding_bwd_workspace_bytes(100, 10, 64)
 
-    def bwd(ids=FAKE, i64=1, dy=FAKE, dyt=1, ld=64, T=4, V=10, d=64, pad=-1, dw=FAKE, dt=1, ws=FAKE, n=size):
+    def bwd(ids=FAKE, i64=1, dy=FAKE, dyt=1, ld=64, T=100, V=10, d=64, pad=-1, dw=FAKE, dt=1, ws=FAKE, n=size):
         return lib.fmoe_embedding_bwd(ids, i64, dy, dyt, ld, T, V, d, 1.0, pad, dw, dt, ws, n, None)
 
     assert bwd(T=-1) == 1 and bwd(pad=10) == 1 and bwd(pad=-2) == 1 and bwd(dw=None) == 1 and bwd(dy=None) == 1
     assert bwd(ld=63) == 2 and bwd(dyt=5) == 4 and bwd(dt=5) == 4
     assert bwd(n=size - 1) == 6 and bwd(ws=None) == 6 and bwd(ws=FAKE + 16) == 3 and bwd(dw=FAKE + 2) == 3
-    # slot starts (512 slots and the end), sorted tokens, two partial rows a tile of 16
-    assert size == 513 * 4 // 256 * 256 + 256 + 256 + 2 * 64 * 4
+    # slot starts (512 slots and the end), sorted tokens, two partial rows a tile of 16; none up to 64 tokens
+    assert size == 513 * 4 // 256 * 256 + 256 + 1024 + 7 * 2 * 64 * 4
+    assert lib.fmoe_embedding_bwd_workspace_bytes(64, 10, 64) == 0
+    assert bwd(T=64, ws=FAKE + 16, n=0) == 3 and bwd(T=64, ws=None, n=0, dw=None) == 1
     assert lib.fmoe_embedding_bwd_workspace_bytes(-1, 10, 64) == lib.fmoe_embedding_bwd_workspace_bytes(4, 0, 64) == 0
 
 
