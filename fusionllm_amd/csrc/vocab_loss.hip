@@ -331,7 +331,7 @@ struct VlGemm {
   float* picked;        // their t; GRAD: p - 1
   // STATS
   float2* part;         // [2 * column tiles][Tp]
-  float* logits;        // LOGITS: t, [rows][ldt]
+  float* logits;        // LOGITS: t, [rows][ldt]; few rows: as well, where it is not null
   int ldt;              // a multiple of 256
   int64_t Tp;
   const float* off;     // PROB: o
@@ -1192,6 +1192,8 @@ __global__ __launch_bounds__(512, 4) void vl_thin_kernel(const VlGemm a, const T
       sum = sum + __shfl_xor(sum, 16, 64);
       sum = sum + __shfl_xor(sum, 32, 64);
       if (eg == 0) red[w][row] = make_float2(top, sum);
+      if (a.logits && row < n)
+        *reinterpret_cast<f32x4*>(a.logits + static_cast<int64_t>(row) * a.ldt + (col0 + 4 * eg)) = f32x4{t[0], t[1], t[2], t[3]};
       if (a.index && row < n) {
         const int rel = a.index[row] - (a.v0 + col0) - 4 * eg;
 #pragma unroll
@@ -1814,6 +1816,9 @@ int64_t vl_fwd_piece(int64_t D, int64_t V, int planes, bool packs) {
 // 526; 4096 x 2048 x 32768: 64 listed 1543 and 1954, 256 listed 2075 and 1970; fp32, 2000 x 1024 x 8192, 128 listed: 689
 // and 673).
 constexpr int64_t kLogitBytes = int64_t(1) << 28;
+// Up to 64 rows have few workgroups for their lists, and store for lists of more than four (3 rows x 1690, vocab 9699, 150
+// listed, in fp32: 57 us, with dot products 122; 8 rows x 768 x 32768, 8 listed: 25 and 29; 64 x 256 x 65536, 5 listed: 27
+// both).
 bool vl_stores_logits(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool once_more) {
   const int64_t read = top * D * (planes == 3 ? 4 : 2);
   if (top == 1 || T <= kThinRows || V * 4 * 1024 > kLogitBytes) return false;  // (top 1: also cross entropy)
@@ -1841,8 +1846,8 @@ struct VlFwdSpace {
   bool stored;  // the logits, a piece of the rows at a time
   VlPackSpace pack;
   VlFwdSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
-      : stored(!vl_is_thin(T, V, packs) && vl_fwd_piece(D, V, planes, packs) >= V &&
-               vl_stores_logits(T, D, V, top, planes, false)) {
+      : stored(vl_is_thin(T, V, packs) ? top > 4 && V <= kLogitBytes / (4 * kThinRows)
+                                       : vl_fwd_piece(D, V, planes, packs) >= V && vl_stores_logits(T, D, V, top, planes, false)) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += (n + 255) & ~size_t(255);
@@ -1852,7 +1857,7 @@ struct VlFwdSpace {
     masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
-    logits = take(stored ? vl_logit_rows(T, V) * ceil_div(V, 256) * 1024 : 0);
+    logits = take(stored ? std::min(vl_logit_rows(T, V), T) * ceil_div(V, 256) * 1024 : 0);
     if (packs && !vl_is_thin(T, V, packs)) pack = VlPackSpace(take, vl_fwd_piece(D, V, planes, true), pad64(D), planes, planes == 1);
   }
 };
@@ -2131,6 +2136,10 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r, l.n_rows = g.rows;
   l.factor = static_cast<float>(temperature * temperature);
 
+  if (space.stored) {
+    g.logits = reinterpret_cast<float*>(ws + space.logits), g.ldt = static_cast<int>(ceil_div(vocab, 256) * 256);
+    l.logits = g.logits, l.ldt = g.ldt;
+  }
   if (thin) {
     g.cols = static_cast<int>(vocab);
     vl_thin<VL_STATS>(g, weight, w_dtype, ldw, dim, planes, T, s);
@@ -2151,8 +2160,7 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
     if (space.stored) break;  // (one piece of the vocabulary)
     vl_stats<VL_STATS>(g, planes, st.Tp, s);
   }
-  if (space.stored) {
-    g.logits = reinterpret_cast<float*>(ws + space.logits), g.ldt = static_cast<int>(ceil_div(vocab, 256) * 256);
+  if (space.stored && !thin) {
     vl_stored_lists(g, l, w_dtype, T, vl_logit_rows(T, vocab), st.Dp, static_cast<int>(top), true, s);
   } else if (T > 0) {
     vl_stat(l, T, s);
