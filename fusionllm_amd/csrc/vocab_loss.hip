@@ -1274,6 +1274,184 @@ void vl_thin(const VlGemm& a, const void* weight, int w_dtype, int64_t ldw, int6
   else vl_thin_launch<MODE, FMOE_F32, 1>(a, w, T, grid, s);
 }
 
+// ---- dH of few rows, fp32 ----------------------------------------------------------------------------
+// G W of up to 64 rows on the weight as it lies, with v_mfma_f32_16x16x4_f32 on fp32 numbers (G: the sum of its three
+// parts, exact), instead of a packed copy and six products.  Bound by the weight's read up to 32 rows.  A wave takes
+// 64 columns and all rows, 32 vocabulary rows a step: a lane's load is 4 elements of a weight row, which are the A operands
+// of four products (column d0 + 4 m + i is row m of product i, so that a lane ends with 16 consecutive columns), and the
+// step's G comes from LDS, four vocabulary rows a lane at a time.  The vocabulary is split over workgroups, and where the
+// rows are short over the waves of one; vl_thin_join_kernel adds their partial rows in order.  Training, vocab 50021 x 1024:
+// 20 rows 457 us with the packed copy, 308; 60 rows 507 and 421.  (bf16 rows of odd lengths this way: 5 rows x 1001 x 50021
+// 195 and 187 us, 20 rows 197 and 211: not taken.)  17 to 32 rows spill two registers to run two workgroups a CU: 307 us
+// at 20 rows, with one and no spills 318.
+constexpr int kDhRows = 256;  // vocabulary rows whose G is in LDS
+struct ThinDh {
+  int across, ranges;  // waves side by side; parts of the vocabulary
+  int64_t T;
+  ThinDh(int64_t T, int64_t D, int64_t V) : T(T) {
+    across = D > 256 ? 8 : D > 128 ? 4 : D > 64 ? 2 : 1;
+    ranges = static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(V, kDhRows), 512 / ceil_div(D, 64 * across))));
+  }
+  int slots() const { return ranges * (8 / across); }
+  size_t bytes(int64_t Dp) const { return static_cast<size_t>(slots()) * T * Dp * 4; }
+};
+
+template <int MB>
+__global__ __launch_bounds__(512, MB == 4 ? 2 : 4) void vl_thin_dh_kernel(const VlGemm a, const ThinWeight wt, const ThinDh sh) {
+  constexpr int GS = kDhRows + 4;  // (16 rows' reads of 16 bytes in different banks)
+  __shared__ __attribute__((aligned(16))) float gs[16 * MB * GS];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int er = lane & 15, eg = lane >> 4;
+  const int n = vl_rows_here(a.head, 0, kThinRows);
+  const int kw = w / sh.across, parts = 8 / sh.across;
+  const int d0 = (blockIdx.x * sh.across + w % sh.across) * 64, d = d0 + 4 * er, left = wt.D - d;
+  const bool active = d0 < wt.D;
+  const int chunks = (a.vocab + kDhRows - 1) / kDhRows;
+  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * blockIdx.y / sh.ranges);
+  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (blockIdx.y + 1) / sh.ranges);
+
+  struct Step {
+    float v[2][4][4];  // [half][vocabulary row 4 eg + s of its 16][column]
+  };
+  auto load = [&](int v0) __attribute__((always_inline)) {
+    Step f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = static_cast<int64_t>(a.v0 + min(v0 + 16 * h + 4 * eg + q, a.vocab - 1)) * wt.ld + d;
+        if (left >= 4) {
+          const f32x4 x = *reinterpret_cast<const f32x4_e4*>(static_cast<const float*>(wt.p) + at);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f.v[h][q][i] = x[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f.v[h][q][i] = i < left ? static_cast<const float*>(wt.p)[at + i] : 0.0f;
+        }
+      }
+    return f;
+  };
+
+  f32x4 acc[4][MB];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[i][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Step cur;
+  if (active) cur = load(c0 * kDhRows + 32 * kw);
+  for (int c = c0; c < c1; ++c) {
+    __syncthreads();
+    for (int i = tid; i < 16 * MB * 32; i += 512) {
+      const int r = i >> 5, k = (i & 31) * 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+#pragma unroll
+      for (int p = 2; p >= 0; --p) {
+        float y[8];
+        unpack8(*reinterpret_cast<const uint4*>(a.g + p * a.g_plane + static_cast<int64_t>(r) * a.ldg + c * kDhRows + k), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] + y[e];
+      }
+      *reinterpret_cast<f32x4*>(gs + r * GS + k) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(gs + r * GS + k + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    }
+    __syncthreads();
+    if (!active) continue;
+    for (int st = kw; st < kDhRows / 32; st += parts) {
+      const int v = c * kDhRows + 32 * st;
+      const bool same = st + parts < kDhRows / 32;
+      Step next;
+      if (same || c + 1 < c1) next = load(same ? v + 32 * parts : (c + 1) * kDhRows + 32 * kw);
+      if (v + 32 > a.vocab) {  // (what is read again there may be infinite)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cur.v[h][q][i] = v + 16 * h + 4 * eg + q < a.vocab ? cur.v[h][q][i] : 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(gs + (16 * m + er) * GS + 32 * st + 16 * h + 4 * eg);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.v[h][q][i], x[q], acc[i][m], 0, 0, 0);
+        }
+      }
+      cur = next;
+    }
+  }
+  if (!active) return;
+  // acc[i][m][e] of a lane: column d0 + 16 eg + 4 e + i, row 16 m + er
+  float* const part = a.split + static_cast<int64_t>(blockIdx.y * parts + kw) * sh.T * a.cols;
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    if (16 * m + er >= n) continue;
+    float* const p = part + static_cast<int64_t>(16 * m + er) * a.cols + d0 + 16 * eg;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<f32x4*>(p + 4 * e) = f32x4{acc[0][m][e], acc[1][m][e], acc[2][m][e], acc[3][m][e]};
+  }
+}
+
+// A row's partial rows added, 512 columns a workgroup: each wave every fourth, in order; then the waves.
+__global__ __launch_bounds__(256) void vl_thin_join_kernel(const VlGemm a, const int* inv, int T, int slots) {
+  __shared__ float sums[4][512];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = blockIdx.x, col = blockIdx.y * 512 + lane * 8;
+  const int row = inv[t];
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  if (row < 0) {
+    if (w > 0 || a.more || col >= a.D) return;
+    const int64_t o = static_cast<int64_t>(t) * a.D + col;
+    if (a.out_dtype == FMOE_BF16) store_upto8<FMOE_BF16>(a.out, o, a.D - col, v);
+    else store_upto8<FMOE_F32>(a.out, o, a.D - col, v);
+    return;
+  }
+  constexpr int U = 8;
+  if (col < a.cols)
+    for (int s0 = w; s0 < slots; s0 += 4 * U) {
+      f32x4 x[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float* p = a.split + (static_cast<int64_t>(min(s0 + 4 * u, slots - 1)) * T + row) * a.cols + col;
+        x[u][0] = *reinterpret_cast<const f32x4*>(p);
+        x[u][1] = *reinterpret_cast<const f32x4*>(p + 4);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + 4 * u < slots)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = v[e] + x[u][0][e], v[4 + e] = v[4 + e] + x[u][1][e];
+    }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[w][lane + 64 * e] = v[e];
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int q = 1; q < 4; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] + sums[q][lane + 64 * e];
+  vl_result8<VL_DH>(a, kThinRows, row, col, v);
+}
+
+void vl_thin_dh(const VlGemm& a, const void* weight, int64_t ldw, const int* inv, const ThinDh& sh, hipStream_t s) {
+  if (sh.T == 0) return;
+  const ThinWeight w{weight, ldw, a.D};
+  const dim3 grid(static_cast<uint32_t>(ceil_div(a.D, 64 * sh.across)), static_cast<uint32_t>(sh.ranges));
+  if (sh.T <= 16) vl_thin_dh_kernel<1><<<grid, 512, 0, s>>>(a, w, sh);
+  else if (sh.T <= 32) vl_thin_dh_kernel<2><<<grid, 512, 0, s>>>(a, w, sh);
+  else vl_thin_dh_kernel<4><<<grid, 512, 0, s>>>(a, w, sh);
+  const dim3 join(static_cast<uint32_t>(sh.T), static_cast<uint32_t>(ceil_div(a.D, 512)));
+  vl_thin_join_kernel<<<join, 256, 0, s>>>(a, inv, static_cast<int>(sh.T), sh.slots());
+}
+
 // The split tiles: their ranges' partial tiles added in order, by the first `blocks` workgroups (32 for every tile
 // that can be split).  DH's last piece: and zeros in the rows of the result without entries, 64 rows a workgroup
 // behind those.
@@ -1865,6 +2043,7 @@ struct VlFwdSpace {
 struct VlBwdSpace {
   int64_t piece;
   size_t g, sum, split, bytes = 0;
+  bool as_it_lies;  // fp32, few rows: no product reads a packed weight
   VlPackSpace pack;
   VlBwdSpace(int64_t T, int64_t D, int64_t V, int planes, bool packs) : piece(vl_bwd_piece(T, V, planes)) {
     auto take = [&](size_t n) {
@@ -1873,12 +2052,14 @@ struct VlBwdSpace {
       return at;
     };
     const int64_t Tp = std::max<int64_t>(pad64(T), 64), Dp = pad64(D), dt = ceil_div(Dp, 256);
-    const int64_t passes = planes == 3 ? 6 : 1;
+    const int64_t passes = planes == 3 ? 6 : 1, tile = core::BM * core::BN * 4;
+    as_it_lies = planes == 3 && vl_is_thin(T, V, packs);
     g = take(Tp * piece * 2 * planes);
     sum = take(V > piece ? Tp * Dp * 4 : 0);
-    split = take(std::max(vl_split_slots(ceil_div(Tp, 256) * dt, ceil_div(std::min(V, piece), 64) * passes),
-                          vl_split_slots(ceil_div(std::min(V, piece), 256) * dt, Tp / 64 * passes)) * (core::BM * core::BN * 4));
-    if (packs) pack = VlPackSpace(take, std::min(pad64(V), piece), Dp, planes, true);
+    const int64_t dh = as_it_lies ? ThinDh(T, D, std::min(V, piece)).bytes(Dp)
+                                  : vl_split_slots(ceil_div(Tp, 256) * dt, ceil_div(std::min(V, piece), 64) * passes) * tile;
+    split = take(std::max<int64_t>(dh, vl_split_slots(ceil_div(std::min(V, piece), 256) * dt, Tp / 64 * passes) * tile));
+    if (packs && !as_it_lies) pack = VlPackSpace(take, std::min(pad64(V), piece), Dp, planes, true);
   }
 };
 
@@ -2209,7 +2390,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ldw;
     int64_t w_plane = 0;
     int w_ld = static_cast<int>(ldw);
-    if (packs && (!thin || d_hidden != nullptr)) {
+    if (packs && !space.as_it_lies && (!thin || d_hidden != nullptr)) {
       VlPacked copy(ws, space.pack);
       if (!half) copy.half = nullptr;
       else g.b = copy.half, g.b_scale = copy.scale;
@@ -2243,7 +2424,8 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
     if (d_hidden != nullptr) {
       h.out = d_hidden, h.out_dtype = dh_dtype, h.sum = reinterpret_cast<float*>(ws + space.sum);
       h.add = v0 > 0, h.more = v0 + rows < vocab;
-      vl_product<VL_DH>(h, planes, mt, dt, ceil_div(rows, 64), h.more ? nullptr : st.inv, T, s);
+      if (space.as_it_lies) vl_thin_dh(h, weight, ldw, st.inv, ThinDh(T, dim, std::min(vocab, piece)), s);
+      else vl_product<VL_DH>(h, planes, mt, dt, ceil_div(rows, 64), h.more ? nullptr : st.inv, T, s);
     }
     if (d_weight != nullptr) {
       h.b = st.h, h.b_plane = st.plane, h.ldb = Dp, h.add = h.more = 0;

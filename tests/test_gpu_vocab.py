@@ -270,7 +270,8 @@ def test_long_lists(gpu_device, T, V, D, K, reduction, dtype):
 
 @pytest.mark.parametrize("T,V,D,K,dtype", [(24000, 46000, 64, 3, torch.bfloat16), (8200, 45000, 96, 2, torch.float32),
                                            (70, 600, 16384, 20, torch.float32), (9, 300, 16384, 20, torch.bfloat16),
-                                           (2100, 9000, 640, 1, torch.bfloat16)])
+                                           (2100, 9000, 640, 1, torch.bfloat16), (5, 1100000, 8, 6, torch.float32),
+                                           (40, 2000, 333, 6, torch.float32), (17, 5001, 130, 2, torch.float32)])
 def test_several_pieces_wide_rows_and_split_products(gpu_device, T, V, D, K, dtype):
     # the backward in pieces of the vocabulary (the first two), the widest rows, tiles cut along K beside whole ones
     g = _gen(T)
