@@ -3,7 +3,8 @@
 //
 // Both are bound by memory: the forward reads and writes T rows; the backward reads
 // T rows and writes the V rows of the gradient, most of them zeros.  A wave takes 1 KB of a row at a time,
-// 16 bytes per lane.
+// 16 bytes per lane.  32768 tokens x 2048 in fp32, vocab 131072: forward 89 us (6.0 TB/s), backward 281 (the sums and zeros 244:
+// 5.5 TB/s, of a copy's 4.9); 16384 x 768 in bf16, vocab 50021: 10 and 41.
 //
 // The gradient is summed without atomics, so that the same bits come out every run:
 //   1. embed_sort_kernel sorts the tokens by id, stably, in one launch: a workgroup owns up to 512 ids and

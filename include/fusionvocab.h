@@ -2,7 +2,7 @@
  * fusionvocab.h — C ABI of libfusionmoe.so, continued: the vocabulary operators
  * at the two ends of a model, the token embedding in front of the blocks and the
  * losses behind them that multiply the hidden states with the vocabulary's weight
- * and keep no logits.
+ * without keeping the logits.
  *
  * The conventions, status codes and dtype codes are those of fusionmoe.h:
  * borrowed device pointers, asynchronous on `stream`, no allocation, no
@@ -61,7 +61,9 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  * of the vocabulary at a time, as G = (p - q) times the row's weight, and multiplies
  *   d_hidden = G weight,  d_weight = G^T hidden.
  * planes = 1: operands and G are bf16 (fp32 operands are rounded), sums fp32.  planes = 3: fp32
- * operands (both) and G as three bf16 numbers each, whose six largest products are added: fp32 precision.
+ * operands (both), whose rows are taken as two scaled fp16 numbers each for the logits (three products) and, like G, as
+ * three bf16 numbers for the gradients (the six largest products): fp32 precision; up to 64 rows the logits and d_hidden are fp32 products.
+ * Long lists of a distillation read their logits from a piece of at most 256 MB in the workspace.
  * Deterministic, no atomics.
  *
  * state keeps what the backward needs (fmoe_vocab_loss_state_bytes); it belongs to one forward call.
