@@ -1284,9 +1284,9 @@ void vl_thin(const VlGemm& a, const void* weight, int w_dtype, int64_t ldw, int6
 // of four products (column d0 + 4 m + i is row m of product i, so that a lane ends with 16 consecutive columns), and the
 // step's G comes from LDS, four vocabulary rows a lane at a time.  The vocabulary is split over workgroups, and where the
 // rows are short over the waves of one; vl_thin_join_kernel adds their partial rows in order.  Training, vocab 50021 x 1024:
-// 20 rows 457 us with the packed copy, 308; 60 rows 507 and 421.  (bf16 rows of odd lengths this way: 5 rows x 1001 x 50021
-// 195 and 187 us, 20 rows 197 and 211: not taken.)  17 to 32 rows spill two registers to run two workgroups a CU: 307 us
-// at 20 rows, with one and no spills 318.
+// 20 rows 457 us with the packed copy, 318; 60 rows 507 and 421.  (bf16 rows of odd lengths this way: 5 rows x 1001 x 50021
+// 195 and 187 us, 20 rows 197 and 211: not taken.)  One workgroup a CU above 16 rows: two would spill (20 rows: 307
+// with two spilled registers).
 constexpr int kDhRows = 256;  // vocabulary rows whose G is in LDS
 struct ThinDh {
   int across, ranges;  // waves side by side; parts of the vocabulary
@@ -1300,7 +1300,7 @@ struct ThinDh {
 };
 
 template <int MB>
-__global__ __launch_bounds__(512, MB == 4 ? 2 : 4) void vl_thin_dh_kernel(const VlGemm a, const ThinWeight wt, const ThinDh sh) {
+__global__ __launch_bounds__(512, MB == 1 ? 4 : 2) void vl_thin_dh_kernel(const VlGemm a, const ThinWeight wt, const ThinDh sh) {
   constexpr int GS = kDhRows + 4;  // (16 rows' reads of 16 bytes in different banks)
   __shared__ __attribute__((aligned(16))) float gs[16 * MB * GS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
