@@ -7,11 +7,13 @@ id's rows in fp32 in a fixed order (above 64 tokens they are sorted by id first)
 bits every run, no atomics.
 
 The losses are those of the logits ``s = logit_scale * hidden @ weight.T``,
-which are not kept (a distillation with long lists forms them a piece of 256 MB at a time).  A loss of one value (mean, sum) that needs gradients forms them in
+which are not kept (a distillation with long lists forms them a piece of 256 MB
+at a time).  A loss of one value (mean, sum) that needs gradients forms them in
 its forward, a piece of the rows at a time (up to 2 GiB), and its backward scales
-them by the loss's gradient.  A loss per row (none), and one of up to 64 rows or of a vocabulary too
-large for such pieces, reduces the logits tile by tile in the forward and forms
-them again in the backward.  Rows without a target
+them by the loss's gradient (rounded to their dtype a second time, unless that is
+a power of two).  A loss per row (none), and one of up to 64 rows or of a
+vocabulary too large for such pieces, reduces the logits tile by tile in the
+forward and forms them again in the backward.  Rows without a target
 (``ignore_index``) are left out of every product.
 
     linear_cross_entropy   -log softmax(s)[target]

@@ -168,7 +168,11 @@ def _reference(hidden, weight, lists, teacher, ignore, scale, tau, reduction, up
     G = c * (p - target)
     g_half = HALF[torch.bfloat16] if planes == 1 else 4 * U
     dG = c.abs() * ((d + 8 * U) * p + (dq if teacher is None else dq[:, None]) * target + 4 * U * (p + target)) + g_half * G.abs()
-    out_h, out_w = HALF[hidden.dtype], HALF[weight.dtype]
+    # gradients formed in the forward are rounded to their dtype there, as for a loss's gradient of 1, and once more when that
+    # gradient, up, multiplies them: (x (1 + a)) up (1 + b) = x up (1 + a + b + a b) with |a|, |b| up to half a step, and b = 0
+    # where up is a power of two (the 1.01 below covers a b)
+    twice = 2 if reduction != "none" and T > 64 and math.frexp(float(up))[0] != 0.5 else 1
+    out_h, out_w = twice * HALF[hidden.dtype], twice * HALF[weight.dtype]
     dH, dW = G @ W, G.T @ H
     bH = dG @ W.abs() + (dot(V) + 80 * U) * (G.abs() @ W.abs()) + out_h * dH.abs()
     again = g_half if reduction != "none" and T > 64 else 0.0
@@ -266,6 +270,40 @@ def test_long_lists(gpu_device, T, V, D, K, reduction, dtype):
     up = torch.rand(T, generator=g).to(gpu_device) if reduction == "none" else torch.tensor(1.0, device=gpu_device)
     loss = linear_distillation(h, w, index, z, temperature=2.0, reduction=reduction)
     _check(loss, h, w, up, _reference(h, w, index, z, -100, 1.0, 2.0, reduction, up))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction,scale", [("mean", -1.5), ("none", 0.0), ("sum", 3.0)])
+@pytest.mark.parametrize("T,V,D,K", [(64, 1, 1, 6), (65, 1, 1, 3), (33, 130, 65, 1024), (1024, 2, 9, 1), (1025, 33, 9, 1024),
+                                     (2049, 257, 100, 40), (4097, 300, 72, 5)])
+def test_smallest_vocabularies_longest_lists_and_signs(gpu_device, T, V, D, K, reduction, scale, dtype):
+    g = _gen(T + V + K)
+    h, w, t = _operands(g, T, V, D, dtype, gpu_device)
+    t[torch.randperm(T, generator=g)[:T // 4].to(gpu_device)] = -100
+    up = torch.rand(T, generator=g).to(gpu_device) if reduction == "none" else torch.tensor(1.5, device=gpu_device)
+    loss = linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale)
+    _check(loss, h, w, up, _reference(h, w, t[:, None], None, -100, scale, 1.0, reduction, up))
+    index, z = torch.randint(0, V, (T, K), generator=g).to(gpu_device), 3 * torch.randn(T, K, generator=g).to(gpu_device)
+    index[::3, : (K + 1) // 2] = -100
+    loss = linear_distillation(h, w, index, z, temperature=0.75, reduction=reduction, logit_scale=scale)
+    _check(loss, h, w, up, _reference(h, w, index, z, -100, scale, 0.75, reduction, up))
+
+
+@pytest.mark.parametrize("T", [3, 64, 300])
+def test_expanded_operands(gpu_device, T):
+    # rows that are one row in memory, and an incoming gradient that is one value
+    g = _gen(T)
+    row = torch.randn(1, 96, generator=g).to(gpu_device, torch.bfloat16).requires_grad_(True)
+    w = torch.randn(500, 96, generator=g).to(gpu_device, torch.bfloat16).requires_grad_(True)
+    t = torch.randint(0, 500, (T,), generator=g).to(gpu_device)
+    for reduction in ("mean", "none"):
+        got = torch.autograd.grad(linear_cross_entropy(row.expand(T, 96), w, t, reduction=reduction).sum(), [row, w])
+        want = torch.autograd.grad(linear_cross_entropy(row.repeat(T, 1), w, t, reduction=reduction).sum(), [row, w])
+        assert torch.equal(got[1], want[1])
+        torch.testing.assert_close(got[0], want[0])
+    dw, = torch.autograd.grad(embedding(t, w, 2.0).sum(), [w])
+    count = torch.bincount(t, minlength=500).float()[:, None]
+    assert torch.equal(dw, (2 * count).to(torch.bfloat16).expand(500, 96))
 
 
 @pytest.mark.parametrize("T,V,D,K,dtype", [(24000, 46000, 64, 3, torch.bfloat16), (8200, 45000, 96, 2, torch.float32),
