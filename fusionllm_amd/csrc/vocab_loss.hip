@@ -2058,17 +2058,24 @@ int64_t vl_fwd_piece(int64_t D, int64_t V, int planes, bool packs) {
 // 526; 4096 x 2048 x 32768: 64 listed 1543 and 1954, 256 listed 2075 and 1970; fp32, 2000 x 1024 x 8192, 128 listed: 689
 // and 673).
 constexpr int64_t kLogitBytes = int64_t(1) << 28;
-// Up to 64 rows have few workgroups for their lists, and store for lists of more than four (3 rows x 1690, vocab 9699, 150
-// listed, in fp32: 57 us, with dot products 122; 8 rows x 768 x 32768, 8 listed: 25 and 29; 64 x 256 x 65536, 5 listed: 27
-// both).
 bool vl_stores_logits(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool once_more) {
   const int64_t read = top * D * (planes == 3 ? 4 : 2);
   if (top == 1 || T <= kThinRows || V * 4 * 1024 > kLogitBytes) return false;  // (top 1: also cross entropy)
   return once_more ? T >= 1024 && read > 5 * V + planes * V * D / 80 : read > 5 * V;
 }
-// Rows whose logits are stored at a time.
+// Rows whose logits are stored at a time, where vl_stores_logits says so: whole row tiles, 1024 rows and more of the
+// vocabularies that it takes.
 int64_t vl_logit_rows(int64_t T, int64_t V) {
   return std::min(ceil_div(T, 256), kLogitBytes / (ceil_div(V, 256) * 1024) / 256) * 256;
+}
+// Rows whose logits the forward stores at a time (0: none).  The thin form's few rows have few workgroups for their lists,
+// and it stores those of lists of more than four, all rows at once, where 64 rows would fit kLogitBytes (3 rows x 1690,
+// vocab 9699, 150 listed, in fp32: 57 us, with dot products 122; 8 rows x 768 x 32768, 8 listed: 25 and 29; 64 x 256 x 65536,
+// 5 listed: 27 both).  Up to 64 rows that take tiles (vl_is_thin) do not store.
+int64_t vl_fwd_logit_rows(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs) {
+  if (vl_is_thin(T, V, packs)) return top > 4 && ceil_div(V, 256) * 1024 * kThinRows <= kLogitBytes ? T : 0;
+  const bool stored = vl_fwd_piece(D, V, planes, packs) >= V && vl_stores_logits(T, D, V, top, planes, false);
+  return stored ? std::min(vl_logit_rows(T, V), T) : 0;
 }
 
 // Copies of weight rows: bf16 planes, and for fp32 scaled fp16 with its scales.
@@ -2085,11 +2092,10 @@ struct VlPackSpace {
 
 struct VlFwdSpace {
   size_t masks, part, row_loss, logits, bytes = 0;
-  bool stored;  // the logits, a piece of the rows at a time
+  int64_t logit_rows;  // whose logits are stored at a time (0: none)
   VlPackSpace pack;
   VlFwdSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
-      : stored(vl_is_thin(T, V, packs) ? top > 4 && V <= kLogitBytes / (4 * kThinRows)
-                                       : vl_fwd_piece(D, V, planes, packs) >= V && vl_stores_logits(T, D, V, top, planes, false)) {
+      : logit_rows(vl_fwd_logit_rows(T, D, V, top, planes, packs)) {
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += (n + 255) & ~size_t(255);
@@ -2099,7 +2105,7 @@ struct VlFwdSpace {
     masks = take(ceil_div(T, kRowBlock) * 4);
     part = take(2 * ceil_div(V, 256) * Tp * 8);
     row_loss = take(T * 4);
-    logits = take(stored ? std::min(vl_logit_rows(T, V), T) * ceil_div(V, 256) * 1024 : 0);
+    logits = take(logit_rows * ceil_div(V, 256) * 1024);
     if (packs && !vl_is_thin(T, V, packs)) pack = VlPackSpace(take, vl_fwd_piece(D, V, planes, true), pad64(D), planes, planes == 1);
   }
 };
@@ -2383,7 +2389,7 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
   l.planes = planes, l.c = g.c, l.out_index = st.index, l.out_q = st.q, l.rows = r, l.n_rows = g.rows;
   l.factor = static_cast<float>(temperature * temperature);
 
-  if (space.stored) {
+  if (space.logit_rows > 0) {
     g.logits = reinterpret_cast<float*>(ws + space.logits), g.ldt = static_cast<int>(ceil_div(vocab, 256) * 256);
     l.logits = g.logits, l.ldt = g.ldt;
   }
@@ -2405,11 +2411,11 @@ extern "C" int fmoe_vocab_loss_fwd(const void* hidden, int h_dtype, int64_t ldh,
       g.b = static_cast<const uint16_t*>(weight) + v0 * ldw, g.ldb = static_cast<int>(ldw);
     }
     g.cols = static_cast<int>(rows), g.v0 = static_cast<int>(v0);
-    if (space.stored) break;  // (one piece of the vocabulary)
+    if (space.logit_rows > 0) break;  // (one piece of the vocabulary)
     vl_stats<VL_STATS>(g, planes, st.Tp, s);
   }
-  if (space.stored && !thin) {
-    vl_stored_lists(g, l, w_dtype, T, vl_logit_rows(T, vocab), st.Dp, static_cast<int>(top), true, s);
+  if (space.logit_rows > 0 && !thin) {
+    vl_stored_lists(g, l, w_dtype, T, space.logit_rows, st.Dp, static_cast<int>(top), true, s);
   } else if (T > 0) {
     vl_stat(l, T, s);
     if (distill) vl_lists(l, w_dtype, T, s);

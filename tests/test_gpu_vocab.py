@@ -330,6 +330,24 @@ def test_several_pieces_wide_rows_and_split_products(gpu_device, T, V, D, K, dty
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K", [(3, 8), (32, 8), (7, 64), (64, 64)])
+def test_lists_of_few_rows_in_a_large_vocabulary(gpu_device, T, K, dtype):
+    # stored logits of few rows: 1025 tiles of the vocabulary, more than 256 rows of them would fit their bound
+    g = _gen(T + K)
+    V, D = 262208, 48
+    h, w, _ = _operands(g, T, V, D, dtype, gpu_device, pull=False)
+    index = torch.randint(0, V, (T, K), generator=g).to(gpu_device)
+    index[0, :2] = torch.tensor([V - 1, 0])
+    z = 3 * torch.randn(T, K, generator=g).to(gpu_device)
+    up = torch.rand(T, generator=g).to(gpu_device)
+    want = _reference(h, w, index, z, -100, 1.0, 2.0, "none", up)
+    _check(linear_distillation(h, w, index, z, temperature=2.0, reduction="none"), h, w, up, want)
+    with torch.no_grad():
+        only = linear_distillation(h, w, index, z, temperature=2.0, reduction="none")
+    _within(only, *want[0], "loss without gradients")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("far", [60.0, 90.0, 400.0])
 def test_rows_far_from_their_targets(gpu_device, far, dtype):
     # targets (and all listed tokens) whose logits lie far below the others': the exponentials relative to them

@@ -162,6 +162,32 @@ def test_workspaces_stay_bounded():
         assert lib.fmoe_vocab_loss_packs(w, dt, ld, d, planes) == 1
 
 
+def test_workspaces_hold_the_logits_of_few_rows():
+    # the forward of up to 64 rows (up to 32, or 64 where the weight is copied or small) stores a long list's logits: whole
+    # rows of 256-column tiles in fp32, for every row of the call
+    lib = _lib.load()
+    stored = 0
+    for V in (5, 1000, 131071, 131072, 262143, 262144, 262145, 262208, 300001, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, 1 << 22):
+        tiles = (V + 255) // 256
+        for T in (1, 2, 7, 8, 31, 32, 33, 50, 63, 64):
+            for planes, packs in ((1, 0), (1, 1), (3, 1)):
+                size = lambda top: lib.fmoe_vocab_loss_fwd_workspace_bytes(T, 64, V, top, planes, packs)
+                thin = T <= 32 or packs or tiles < 512
+                for top in (5, 8, 1024):
+                    more = size(top) - size(1)
+                    if thin and V <= 1 << 20:
+                        assert T * tiles * 1024 <= more < T * tiles * 1024 + 512, (T, V, planes, packs, top)
+                        stored += 1
+                    else:
+                        assert more == 0, (T, V, planes, packs, top)
+                assert size(4) == size(1)
+    assert stored > 500
+    # more rows: parts of at most 256 MiB, of whole row tiles, or all of the rows
+    for T, V, top in ((65, 600, 900), (300, 32768, 256), (1500, 60000, 800), (1024, 65536, 1024), (100000, 1664, 156)):
+        more = lib.fmoe_vocab_loss_fwd_workspace_bytes(T, 2944, V, top, 1, 0) - lib.fmoe_vocab_loss_fwd_workspace_bytes(T, 2944, V, 1, 1, 0)
+        assert min(T, 256) * ((V + 255) // 256) * 1024 <= more <= 1 << 28, (T, V, top)
+
+
 def test_embedding_refusals():
     with pytest.raises(RuntimeError, match="ROCm device"):
         embedding(torch.zeros(3, dtype=torch.long), torch.randn(4, 64))
