@@ -26,7 +26,7 @@
 // by a power of two each (their largest element to 2^13 .. 2^14) and held as two fp16 numbers, hi + lo: 22 bits of every
 // element down to 2^-17 of its row's largest, and 2^-39 of that below.  lo hi + hi lo + hi hi are added, as three passes
 // over K in one ring.  G spans more: a row's gradient is as precise in its smallest elements, which make up whole rows of dW, so
-// the products with it take three bf16 numbers, hi + mid + lo: 24 bits at any size.  Of the nine products of
+// the products with it take three bf16 numbers, hi + mid + lo: 24 bits of every element down to 2^-109 (bf16 ends at 2^-133).  Of the nine products of
 // such numbers the six largest are added, the smallest first; what is left out is below 2^-22 of the largest.  G is rounded the same way: half a step of bf16,
 // 2^-8 of an element at most, before the elements of a row or column are summed in fp32.
 #include <algorithm>
@@ -353,6 +353,7 @@ struct VlGemm {
   float* sum;           // DH: [Tp][Dp], DW: [vocab][Dp], the sum over the pieces before (add) and for those after (more)
   int add, more;
   const float* row_factor;  // DH: the rows' factors (nullptr: 1)
+  const float* all_factor;  // DW: the product's (nullptr: 1)
   float* split;         // fp32 partial tiles
 };
 
@@ -435,6 +436,11 @@ __device__ __forceinline__ void vl_result8(const VlGemm& a, int n, int row, int 
     float* const s = a.sum + static_cast<int64_t>(row) * a.cols + col;
     if (MODE == VL_DH && a.row_factor) {
       const float f = a.row_factor[row];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * f;
+    }
+    if (MODE == VL_DW && a.all_factor) {
+      const float f = a.all_factor[0];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = v[e] * f;
     }
@@ -1632,6 +1638,11 @@ __device__ __forceinline__ void vl_store_loss(const LossArgs& a, int row, float 
   else a.row_loss[row] = v;
 }
 
+// Gradients at once: the sum of a row's 2^(t - o) beyond which, and beyond whose inverse, its piece is formed in the ordinary
+// way (a loss of 41.6).  Up to it 2^-l H has all of its bits where |h| >= 2^-49 (2^-66 as one bf16 number), and G' W is in
+// range where |w| < 2^66.
+constexpr float kFarSum = 0x1p60f;
+
 // m and l of R rows per workgroup: each of its 1024 / R threads per row joins every so many of the partial
 // sums, in order; then lanes, then waves.
 template <int R>
@@ -1680,7 +1691,7 @@ __global__ __launch_bounds__(1024) void vl_stat_kernel(const LossArgs a) {
     vl_store_loss(a, row, fmaf((m - a.off[row]) + l, kLn2, part) * a.factor);
   }
   a.stat[row] = make_float2(m, l);
-  if (a.flag && !(s < 0x1p100f && s > 0x1p-100f)) a.flag[0] = 1;
+  if (a.flag && !(s < kFarSum && s > 1.0f / kFarSum)) a.flag[0] = 1;
 }
 
 // Distillation, a workgroup per packed row: the teacher's softmax over its list, t of the listed entries (a dot
@@ -1909,11 +1920,12 @@ __global__ __launch_bounds__(256) void vl_fix_kernel(const FixArgs a) {
 
 // ---- gradients at once ---------------------------------------------------------------------------------
 // For a piece of the rows:  G' = 2^(t - o) (PROB, o: the target's t, or the largest listed one),  l = log2 of its
-// sum per row,  G'[r, listed] = 2^l (p - q),  f[r] = w[r] 2^-l,  dH = f (G' W),  dW += G'^T (f H).
-// bf16 has the exponents of fp32, so o need not be the maximum.  Where a row's sum leaves 2^-100 .. 2^100 all the
-// same (a loss of some 70), or is no number, the piece's flag is set, and STATS and GRAD form its statistics and G in
-// the ordinary way (with f[r] = w[r]); else those launches end at once.
-// f H is rounded once more (planes = 1: half a step of bf16 an element, as G).  32768 rows x 2048, vocab 131072: 51.8 ms with
+// sum per row,  G'[r, listed] = 2^l (p - q),  dH = w 2^-l (G' W),  dW += w (G'^T (2^-l H)).  (w, the weight of every row, stays
+// out of the operands: with a small one 2^-l H would lose bits sooner.)
+// bf16 has the exponents of fp32, so o need not be the maximum.  Where a row's sum leaves 2^-60 .. 2^60 all the
+// same (kFarSum), or is no number, the piece's flag is set, and STATS and GRAD form its statistics and G in
+// the ordinary way (with H itself in place of 2^-l H); else those launches end at once.
+// 2^-l H is rounded once more (planes = 1: half a step of bf16 an element, as G).  32768 rows x 2048, vocab 131072: 51.8 ms with
 // the logits formed twice, 39.7 at once.
 
 // o of cross entropy's rows, a wave each.
@@ -1945,20 +1957,22 @@ __global__ __launch_bounds__(256) void vl_off_kernel(const LossArgs a) {
   if (lane == 0) a.off[row] = id < 0 ? 0.0f : acc * a.c;
 }
 
-// f and f H of the piece's rows (zeros in the padding), a wave each.
+// The weight of the rows (all_factor), the factors of the piece's rows of dH, and their 2^-l H (zeros in the padding), a wave
+// each.
 template <int PLANES>
 __global__ __launch_bounds__(256) void vl_factor_kernel(const int* head, int row0, int rows, const float2* stat,
                                                         const int* flag, float factor, int mean, const uint16_t* h,
-                                                        int64_t h_plane, int Dp, float* row_factor, uint16_t* out,
-                                                        int64_t out_plane) {
+                                                        int64_t h_plane, int Dp, float* all_factor, float* row_factor,
+                                                        uint16_t* out, int64_t out_plane) {
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int n = vl_rows_here(head, row0, rows);
+  const float weight = head[0] == 0 ? 0.0f : mean ? factor / static_cast<float>(head[0]) : factor;
+  if (blockIdx.x == 0 && threadIdx.x == 0) all_factor[0] = weight;
   if (row >= pad_rows(n)) return;
-  float f = 0.0f;
+  float f = 1.0f;
   if (row < n) {
-    f = mean ? factor / static_cast<float>(head[0]) : factor;
-    if (flag[0] == 0) f = f * __builtin_amdgcn_exp2f(-stat[row].y);
-    if (lane == 0) row_factor[row] = f;
+    if (flag[0] == 0) f = __builtin_amdgcn_exp2f(-stat[row].y);
+    if (lane == 0) row_factor[row] = weight * f;
   }
   for (int c = lane * 8; c < Dp; c += 512) {
     const int64_t at = static_cast<int64_t>(row) * Dp + c;
@@ -2298,7 +2312,7 @@ int64_t vl_fused_piece(int64_t T, int64_t D, int64_t V, int planes, bool packs) 
 
 struct VlFusedSpace {
   int64_t piece;
-  size_t state, masks, part, row_loss, row_part, off, factor, flag, logits, g, fh, split, sum, bytes = 0;
+  size_t state, masks, part, row_loss, row_part, off, factor, all_factor, flag, logits, g, fh, split, sum, bytes = 0;
   bool stored;  // the logits, for the lists: of a part of the piece at a time
   VlPackSpace pack;
   VlFusedSpace(int64_t T, int64_t D, int64_t V, int64_t top, int planes, bool packs)
@@ -2317,6 +2331,7 @@ struct VlFusedSpace {
     row_part = take(piece * 4);
     off = take(piece * 4);
     factor = take(piece * 4);
+    all_factor = take(4);
     flag = take(4);
     stored = vl_stores_logits(T, D, V, top, planes, true);
     logits = take(stored ? vl_logit_rows(piece, V) * vt * 1024 : 0);
@@ -2542,6 +2557,7 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
   uint16_t* const gbuf = reinterpret_cast<uint16_t*>(ws + space.g);
   uint16_t* const fh = reinterpret_cast<uint16_t*>(ws + space.fh);
   float* const factor = reinterpret_cast<float*>(ws + space.factor);
+  float* const all_factor = reinterpret_cast<float*>(ws + space.all_factor);
   int* const flag = reinterpret_cast<int*>(ws + space.flag);
   const uint16_t *w = static_cast<const uint16_t*>(weight), *w16 = nullptr;
   const float* w_scale = nullptr;
@@ -2614,10 +2630,10 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
     const dim3 wave_rows(static_cast<uint32_t>(ceil_div(pad64(std::max<int64_t>(rows, 1)), 4)));
     if (planes == 1)
       vl_factor_kernel<1><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
-                                                   rows_h, st.plane, Dp, factor, fh, fh_plane);
+                                                   rows_h, st.plane, Dp, all_factor, factor, fh, fh_plane);
     else
       vl_factor_kernel<3><<<wave_rows, 256, 0, s>>>(st.head, g.row0, g.rows, g.stat, flag, fac, reduction == FMOE_REDUCE_MEAN,
-                                                   rows_h, st.plane, Dp, factor, fh, fh_plane);
+                                                   rows_h, st.plane, Dp, all_factor, factor, fh, fh_plane);
     VlGemm h = g;
     h.a = gbuf, h.a_plane = g_plane, h.lda = g.ldg, h.b = w, h.cols = Dp, h.vocab = static_cast<int>(vocab);
     if (d_hidden != nullptr) {
@@ -2626,7 +2642,7 @@ extern "C" int fmoe_vocab_loss_fwd_grad(const void* hidden, int h_dtype, int64_t
       vl_product<VL_DH>(h, planes, mt, dt, ceil_div(vocab, 64), r0 + piece >= T ? st.inv : nullptr, T, s);
     }
     if (d_weight != nullptr) {
-      h.b = fh, h.b_plane = fh_plane, h.ldb = Dp, h.out = d_weight, h.out_dtype = dw_dtype;
+      h.b = fh, h.b_plane = fh_plane, h.ldb = Dp, h.out = d_weight, h.out_dtype = dw_dtype, h.all_factor = all_factor;
       h.sum = reinterpret_cast<float*>(ws + space.sum), h.add = r0 > 0, h.more = piece < T;
       vl_product<VL_DW>(h, planes, vt, dt, ceil_div(rows, 64), nullptr, 0, s);
     }

@@ -62,7 +62,7 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  *   d_hidden = G weight,  d_weight = G^T hidden.
  * planes = 1: operands and G are bf16 (fp32 operands are rounded), sums fp32.  planes = 3: fp32
  * operands (both), whose rows are taken as two scaled fp16 numbers each for the logits (three products) and, like G, as
- * three bf16 numbers for the gradients (the six largest products): fp32 precision; up to 64 rows the logits and d_hidden are fp32 products.
+ * three bf16 numbers for the gradients (the six largest products; 24 bits of elements down to 2^-109): fp32 precision; up to 64 rows the logits and d_hidden are fp32 products.
  * Long lists of a distillation read their logits from a piece of at most 256 MB in the workspace.
  * Deterministic, no atomics.
  *
@@ -97,7 +97,7 @@ int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int w_dtype, in
  * forming the logits twice: a piece of the rows at a time, whose exponentials 2^(s - o), o the logit of the row's
  * target (or the largest listed one), are G up to a factor per row.  Those factors go into d_hidden, and with hidden into
  * the product of d_weight: with planes = 1 the scaled hidden states are rounded to bf16 once more.  Rows whose
- * sum of such exponentials leaves 2^-100 .. 2^100 (or is no number) make their piece be formed in the ordinary way.
+ * sum of such exponentials leaves 2^-60 .. 2^60 (a loss of 41.6; or is no number) make their piece be formed in the ordinary way.
  * d_hidden and d_weight as in fmoe_vocab_loss_bwd.  The size query returns 0 where this form is not taken (up to 64
  * rows; vocabularies of which no piece of 2048 rows fits 2 GiB): FMOE_ERR_SHAPE.  There is no state. */
 size_t fmoe_vocab_loss_grad_workspace_bytes(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes, int packs);

@@ -368,6 +368,37 @@ def test_rows_far_from_their_targets(gpu_device, far, dtype):
     _check(loss, h, w, up, _reference(h, w, index, z, -100, 1.0, 1.0, "mean", up))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [27.0, 41.0, 45.0, 68.0])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("hidden,scale", [(-12, -24), (-26, 0)])
+def test_rows_of_high_loss_with_small_factors(gpu_device, hidden, scale, nats, reduction, dtype):
+    # one row of a high loss, small hidden states (2^hidden) and a small factor of the loss (2^scale) against a large weight: what
+    # d_weight's product takes of the row must not end among the subnormal numbers (at 68 nats the row's factor is 2^-98), and
+    # d_hidden's stays in range
+    g = _gen(int(nats))
+    T, V, D = 100, 700, 64
+    h, w, t = _operands(g, T, V, D, torch.float32, gpu_device, pull=False)
+    t[t == t[17]] = (t[17] + 1) % V
+    t[17] = (t[17] - 1) % V
+    h, w, scale = h.detach() * 2.0 ** hidden, w.detach() * 2.0 ** (-hidden - scale), 2.0 ** scale
+    away = -w[t[17]].double() * (scale / w[t[17]].double().square().sum()) / scale ** 2
+    least, most = 0.0, nats
+    for _ in range(50):  # the multiple of it that has this loss
+        far = (least + most) / 2
+        s = w.double() @ (far * away) * scale
+        least, most = (far, most) if float(torch.logsumexp(s, 0) - s[t[17]]) < nats else (least, far)
+    h[17] = (far * away).float()
+    h, w = (x.to(dtype).requires_grad_(True) for x in (h, w))
+    up = torch.tensor(1.0, device=gpu_device)
+    loss = linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale)
+    _check(loss, h, w, up, _reference(h, w, t[:, None], None, -100, scale, 1.0, reduction, up))
+    index = t[:, None].repeat(1, 2)
+    z = torch.randn(T, 2, generator=g).to(gpu_device)
+    loss = linear_distillation(h, w, index, z, logit_scale=scale, reduction=reduction)
+    _check(loss, h, w, up, _reference(h, w, index, z, -100, scale, 1.0, reduction, up))
+
+
 def test_infinite_operands(gpu_device):
     # a vocabulary row of -infinity (a token that is never taken) against positive hidden states: torch's results
     # from bf16 operands; NaN from fp32 operands, whose parts (infinity less infinity) are no numbers
