@@ -2200,7 +2200,8 @@ struct VlCall {
 int vl_check(const VlCall& a, const void* state, const void* workspace) {
   const bool distill = a.distill();
   if (a.T < 0 || a.dim <= 0 || a.vocab <= 0 || a.top <= 0 || a.index64 < 0 || a.index64 > 1 || a.reduction < 0 ||
-      a.reduction > 2 || (a.planes != 1 && a.planes != 3) || !(a.temperature > 0.0) || (!distill && a.temperature != 1.0))
+      a.reduction > 2 || (a.planes != 1 && a.planes != 3) || !(a.temperature > 0.0) ||
+      (!distill && a.T > 0 && a.temperature != 1.0))  // (without rows there may be no address to tell them apart)
     return FMOE_ERR_INVALID_ARG;
   if (!vl_sizes_ok(a.T, a.dim, a.vocab, a.top, a.planes)) return FMOE_ERR_SHAPE;
   if ((a.T > 1 && (a.ldh < a.dim || a.ldh > (int64_t(1) << 38))) ||

@@ -511,6 +511,20 @@ def test_empty_batch(gpu_device):
     assert gh.shape == (0, 64) and not gw.any()
 
 
+@pytest.mark.parametrize("K", [1, 2, 30])
+def test_empty_batch_of_lists(gpu_device, K):
+    w = torch.randn(100, 64, device=gpu_device, requires_grad=True)
+    h = torch.randn(2, 0, 64, device=gpu_device, requires_grad=True)
+    index = torch.empty(2, 0, K, dtype=torch.long, device=gpu_device)
+    z = torch.empty(2, 0, K, device=gpu_device)
+    for tau in (1.0, 2.0):
+        assert linear_distillation(h, w, index, z, temperature=tau, reduction="none").shape == (2, 0)
+        assert bool(linear_distillation(h, w, index, z, temperature=tau).isnan())
+        loss = linear_distillation(h, w, index, z, temperature=tau, reduction="sum")
+        gh, gw = torch.autograd.grad(loss, [h, w])
+        assert float(loss.detach()) == 0 and gh.shape == (2, 0, 64) and not gw.any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,D", [(48, 192), (200, 192), (200, 101)])
 def test_strided_operands_leading_shapes_and_frozen_parts(gpu_device, T, D, dtype):

@@ -119,6 +119,24 @@ def test_gradients_at_once_and_scale_argument_errors_without_gpu():
     assert scale(count=9) == 1 and scale(count=-1) == 1 and scale(count=0, f=None) == 0
 
 
+def test_calls_without_rows_are_not_refused_for_their_missing_teacher():
+    # an empty tensor has no address, so nothing tells a distillation of no rows, lists of one, from cross entropy: its
+    # temperature passes the check of arguments (the workspace that is too small is what comes next, before any launch)
+    lib = _lib.load()
+    state = lib.fmoe_vocab_loss_state_bytes(0, 64, 1, 1)
+
+    def fwd(T, top, temp, teacher):
+        return lib.fmoe_vocab_loss_fwd(None, 0, 64, FAKE, 0, 64, None, 1, teacher, 1, T, 64, 100, top, -100, 1.0, temp, 1, 1,
+                                       FAKE, FAKE, state, FAKE, 0, None)
+
+    for top in (1, 2, 7):
+        for temp in (1.0, 2.0, 0.5):
+            for teacher in (None, FAKE):
+                assert fwd(0, top, temp, teacher) == 6, (top, temp, teacher)
+            assert fwd(0, top, -temp, None) == 1
+    assert fwd(1, 1, 2.0, None) == 1
+
+
 def test_state_size_is_the_librarys():
     lib = _lib.load()
     for a in [(0, 1, 1, 1), (1, 1, 1, 1), (5, 7, 3, 3), (64, 64, 64, 1), (65, 65, 1, 3), (16384, 768, 1, 1),
