@@ -906,6 +906,8 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
     const int er = el & 15, eg = el >> 4;  // acc[i][j]: row 16 i + er, columns 16 j + 4 eg + 0..3
 
     if constexpr (HALF) {
+      // the scales together first: powers of two, whose product is exact; with one of them alone a large row against a small
+      // one would leave fp32's range
       float rs[FM];
 #pragma unroll
       for (int i = 0; i < FM; ++i) rs[i] = a.a_scale[min(row0 + 16 * i + er, np - 1)];
@@ -916,7 +918,7 @@ __global__ __launch_bounds__(core::NT, 1) void vl_gemm_kernel(const VlGemm a) {
         for (int e = 0; e < 4; ++e) {
           const float cs = a.b_scale[min(col0 + 16 * j + 4 * eg + e, a.cols - 1)];
 #pragma unroll
-          for (int i = 0; i < FM; ++i) acc[i][j][e] = (acc[i][j][e] * rs[i]) * cs;
+          for (int i = 0; i < FM; ++i) acc[i][j][e] = acc[i][j][e] * (rs[i] * cs);
         }
       }
     }

@@ -399,6 +399,18 @@ def test_rows_of_high_loss_with_small_factors(gpu_device, hidden, scale, nats, r
     _check(loss, h, w, up, _reference(h, w, index, z, -100, scale, 1.0, reduction, up))
 
 
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_rows_of_very_different_scales(gpu_device, reduction):
+    # fp32 logits in range, though the hidden states' scale times the products of the scaled rows is not
+    g = _gen(8)
+    T, V, D, scale = 100, 700, 64, 2.0 ** -72
+    h, w, t = _operands(g, T, V, D, torch.float32, gpu_device, pull=False)
+    h, w = ((x.detach() * f).requires_grad_(True) for x, f in ((h, 2.0 ** 112), (w, 2.0 ** -40)))
+    up = torch.rand(T, generator=g).to(gpu_device) if reduction == "none" else torch.tensor(1.0, device=gpu_device)
+    loss = linear_cross_entropy(h, w, t, reduction=reduction, logit_scale=scale)
+    _check(loss, h, w, up, _reference(h, w, t[:, None], None, -100, scale, 1.0, reduction, up))
+
+
 def test_infinite_operands(gpu_device):
     # a vocabulary row of -infinity (a token that is never taken) against positive hidden states: torch's results
     # from bf16 operands; NaN from fp32 operands, whose parts (infinity less infinity) are no numbers
