@@ -1720,7 +1720,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void vl_list_kernel(const LossArgs a) {
   __shared__ float red[4], tq[FMOE_VOCAB_MAX_TOP];
   __shared__ int ti[FMOE_VOCAB_MAX_TOP];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, row = blockIdx.y * gridDim.x + blockIdx.x;
   const bool early = a.row_part != nullptr;  // before the logits' statistics: o of the row, and its part of the loss
   if (early && row == 0 && threadIdx.x == 0) a.flag[0] = 0;
   if (row >= vl_rows_here(a.head, a.row0, a.n_rows)) return;
@@ -2250,7 +2250,9 @@ void vl_stat(const LossArgs& l, int64_t rows, hipStream_t s) {
 }
 
 void vl_lists(const LossArgs& l, int w_dtype, int64_t rows, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(rows));
+  // (a side of the grid stays below 2^32 threads)
+  constexpr int64_t kSide = int64_t(1) << 23;
+  const dim3 grid(static_cast<uint32_t>(std::min(rows, kSide)), static_cast<uint32_t>(ceil_div(rows, kSide)));
   if (w_dtype == FMOE_BF16) vl_list_kernel<FMOE_BF16><<<grid, 256, 0, s>>>(l);
   else vl_list_kernel<FMOE_F32><<<grid, 256, 0, s>>>(l);
 }

@@ -718,6 +718,27 @@ def test_wrappers_give_the_native_calls_results(gpu_device):
             "scale"} <= set(times)
 
 
+def test_as_many_rows_as_a_call_takes(gpu_device):
+    # 2^24 rows: a workgroup for each of their lists is more than one side of a grid holds
+    g = torch.Generator(device=gpu_device).manual_seed(6)
+    T, V, D = 1 << 24, 3, 4
+    h = torch.randn(T, D, device=gpu_device, generator=g).bfloat16()
+    w = torch.randn(V, D, device=gpu_device, generator=g).bfloat16()
+    index = torch.randint(0, V, (T, 2), device=gpu_device, generator=g, dtype=torch.int32)
+    z = torch.randn(T, 2, device=gpu_device, generator=g)
+    up = torch.ones(T, device=gpu_device)
+    _within(linear_distillation(h, w, index, z, temperature=2.0, reduction="none"),
+            *_reference(h, w, index, z, -100, 1.0, 2.0, "none", up)[0], "distillation")
+    target = index[:, 0].contiguous()
+    _within(linear_cross_entropy(h, w, target, reduction="none"),
+            *_reference(h, w, index[:, :1], None, -100, 1.0, 1.0, "none", up)[0], "cross entropy")
+    ids = target.long()
+    assert torch.equal(embedding(target, w), w[ids])
+    leaf = w.clone().requires_grad_(True)
+    dw, = torch.autograd.grad(embedding(ids, leaf), [leaf], torch.ones_like(h))
+    assert torch.equal(dw, torch.bincount(ids, minlength=V).bfloat16()[:, None].expand(V, D))  # (counts below 2^24: exact sums)
+
+
 def test_long_offsets(gpu_device):
     # a weight of more than 2^31 elements (rows at offsets beyond 32 bits), few of them used
     V, D = 1 << 20, 2064
