@@ -29,7 +29,7 @@ outputs y [T,d] (out_dtype), mean [T] and rstd [T] fp32; gradients [dx, dw, db],
 without those of a weight or bias that is not there.
 
 ``fusionllm::embedding_fwd`` / ``embedding_bwd`` and the losses over a vocabulary:
-``vocab_loss_fwd`` (loss, the state for the backward) / ``vocab_loss_bwd`` (d_hidden, d_weight),
+``vocab_loss_fwd`` (loss, the state for the backward) / ``vocab_loss_bwd`` (d_hidden, d_weight, those that are wanted),
 and ``vocab_loss_fwd_grad`` (loss, and the gradients that are wanted, formed at once) with ``scale``.
 """
 from __future__ import annotations
@@ -271,28 +271,38 @@ def _(hidden, weight, index, teacher, ignore_index, logit_scale, temperature, pl
 
 @torch.library.custom_op("fusionllm::vocab_loss_bwd", mutates_args=())
 def vocab_loss_bwd(d_loss: Tensor, hidden: Tensor, weight: Tensor, state: Tensor, top: int, distill: bool,
-                   logit_scale: float, temperature: float, planes: int, reduction: str) -> list[Tensor]:
+                   logit_scale: float, temperature: float, planes: int, reduction: str, need_h: bool = True,
+                   need_w: bool = True) -> list[Tensor]:
+    """The gradients that are wanted; hidden gives its rows and dtype alone (any columns)."""
     with _norm._on_device(weight):
-        return list(K.vocab_loss_bwd(d_loss.contiguous(), _norm._rows(weight), state, hidden.shape[0], top, distill,
-                                     logit_scale, temperature, planes, reduction, hidden.dtype, weight.dtype))
+        out = K.vocab_loss_bwd(d_loss.contiguous(), _norm._rows(weight), state, hidden.shape[0], top, distill, logit_scale,
+                               temperature, planes, reduction, hidden.dtype if need_h else None,
+                               weight.dtype if need_w else None)
+    return [t for t in out if t is not None]
 
 
 @vocab_loss_bwd.register_fake
-def _(d_loss, hidden, weight, state, top, distill, logit_scale, temperature, planes, reduction):
-    return [hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)]
+def _(d_loss, hidden, weight, state, top, distill, logit_scale, temperature, planes, reduction, need_h=True, need_w=True):
+    return ([hidden.new_empty((hidden.shape[0], weight.shape[1]))] if need_h else []) + (
+        [weight.new_empty(weight.shape)] if need_w else [])
 
 
 def _vocab_loss_setup(ctx, inputs, output):
     hidden, weight, index, teacher, _, logit_scale, temperature, planes, reduction = inputs
-    ctx.save_for_backward(hidden, weight, output[1])
+    ctx.save_for_backward(weight, output[1])  # (the state holds the hidden states)
+    ctx.hidden = (hidden.shape[0], hidden.dtype)
     ctx.args = (index.shape[1], teacher is not None, logit_scale, temperature, planes, reduction)
 
 
 def _vocab_loss_backward(ctx, d_loss, *unused):
-    hidden, weight, state = ctx.saved_tensors
-    if d_loss is None:
+    weight, state = ctx.saved_tensors
+    need = ctx.needs_input_grad[:2]
+    if d_loss is None or not any(need):
         return (None,) * 9
-    dh, dw = torch.ops.fusionllm.vocab_loss_bwd(d_loss, hidden, weight, state, *ctx.args)
+    rows, dtype = ctx.hidden
+    grads = iter(torch.ops.fusionllm.vocab_loss_bwd(d_loss, weight.new_empty((rows, 0), dtype=dtype), weight, state,
+                                                    *ctx.args, *need))
+    dh, dw = (next(grads) if n else None for n in need)
     return dh, dw, None, None, None, None, None, None, None
 
 

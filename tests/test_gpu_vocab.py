@@ -684,6 +684,24 @@ def test_compiled(gpu_device, S):
     assert torch.equal(loss, step(ids, w)) and torch.equal(torch.autograd.grad(loss, [w])[0], want)
 
 
+@pytest.mark.parametrize("S,reduction", [(30, "mean"), (70, "mean"), (70, "none")])
+def test_compiled_with_frozen_parts(gpu_device, S, reduction):
+    torch._dynamo.reset()
+    g = _gen(S)
+    h, w, t = _operands(g, S, 300, 64, torch.bfloat16, gpu_device)
+    index, z = _lists(g, S, 300, 4, gpu_device)
+
+    def step(h, w):
+        return (linear_cross_entropy(h, w, t, reduction=reduction) +
+                linear_distillation(h, w, index, z, reduction=reduction)).sum()
+
+    for a, b in ((h, w.detach()), (h.detach(), w), (h, w)):
+        leaves = [x for x in (a, b) if x.requires_grad]
+        want = torch.autograd.grad(step(a, b), leaves)
+        got = torch.autograd.grad(torch.compile(step, fullgraph=True, backend="aot_eager")(a, b), leaves)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_second_derivatives_are_refused(gpu_device):
     h, w, t = _operands(_gen(0), 8, 50, 64, torch.float32, gpu_device)
     gh, = torch.autograd.grad(linear_cross_entropy(h, w, t), [h], create_graph=True)

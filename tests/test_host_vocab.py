@@ -307,6 +307,37 @@ def test_operator_fake_shapes():
             assert (dh.shape, dw.shape, dh.dtype) == ((7, 64), (10, 64), torch.bfloat16)
 
 
+@pytest.mark.parametrize("need_h,need_w", [(True, True), (True, False), (False, True)])
+def test_traced_backward_forms_the_wanted_gradients(need_h, need_w):
+    # of the operators that torch.compile runs: a frozen head or frozen hidden states cost no product, and the hidden states,
+    # which the state holds packed, are not kept a second time
+    from torch.utils._python_dispatch import TorchDispatchMode
+    calls = []
+
+    class Calls(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if func is torch.ops.fusionllm.vocab_loss_bwd.default:
+                calls.append((args, out))
+            return out
+
+    with FakeTensorMode():  # (on the CPU, where autograd runs without a device)
+        h = torch.empty(7, 64, dtype=torch.bfloat16, requires_grad=need_h)
+        w = torch.empty(10, 64, requires_grad=need_w)
+        index = torch.empty(7, 1, dtype=torch.long)
+        loss = torch.ops.fusionllm.vocab_loss_fwd(h, w, index, None, -100, 1.0, 1.0, 1, "none")[0]
+        kept = [t for t in loss.grad_fn.saved_tensors]
+        assert all(t.shape != h.shape for t in kept)
+        with Calls():
+            grads = torch.autograd.grad(loss, [t for t in (h, w) if t.requires_grad], torch.ones_like(loss))
+    (args, out), = calls
+    asked = (*args[10:], True, True)[:2]  # (arguments that have their defaults are left out)
+    assert args[1].shape == (7, 0) and asked == (need_h, need_w)
+    want = [((7, 64), torch.bfloat16)] * need_h + [((10, 64), torch.float32)] * need_w
+    assert [(tuple(t.shape), t.dtype) for t in out] == want
+    assert [(tuple(t.shape), t.dtype) for t in grads] == want
+
+
 def _objects():
     from fusionllm_amd import build
     return [build.BUILD_DIR / "vocab_loss.o", build.BUILD_DIR / "embedding.o"]
