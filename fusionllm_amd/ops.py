@@ -315,7 +315,12 @@ def vocab_loss_fwd_grad(hidden: Tensor, weight: Tensor, index: Tensor, teacher: 
                         need_w: bool) -> list[Tensor]:
     _norm.refuse_tangents("fusionllm::vocab_loss_fwd_grad", hidden, weight)
     with _norm._on_device(weight):
-        out = K.vocab_loss_fwd_grad(_norm._rows(hidden), _norm._rows(weight), index, teacher, ignore_index, logit_scale,
+        w = _norm._rows(weight)
+        if not K.vocab_loss_takes_gradients(*hidden.shape, w.shape[0], planes, K.vocab_loss_packs(w, planes)):
+            # chosen for a weight as it lies in a module; this one's address or stride needs a copy of its rows, which is more
+            # than this form takes
+            w = w.clone(memory_format=torch.contiguous_format)
+        out = K.vocab_loss_fwd_grad(_norm._rows(hidden), w, index, teacher, ignore_index, logit_scale,
                                     temperature, planes, reduction, need_h, need_w)
     return [t for t in out if t is not None]
 

@@ -702,6 +702,22 @@ def test_compiled_with_frozen_parts(gpu_device, S, reduction):
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_compiled_with_a_weight_at_an_odd_address(gpu_device):
+    # a weight (part of a flat buffer) whose copy would be more than gradients formed in the forward allow for: a traced
+    # call, which sees no addresses, has chosen them
+    torch._dynamo.reset()
+    T, V, D = 65, 131072, 8256
+    g = torch.Generator(device=gpu_device).manual_seed(1)
+    flat = torch.empty(V * D + 8, device=gpu_device, dtype=torch.bfloat16).normal_(std=0.02, generator=g)
+    w = flat[1:1 + V * D].view(V, D)
+    h = torch.randn(T, D, device=gpu_device, generator=g).bfloat16().requires_grad_(True)
+    t = torch.randint(0, V, (T,), device=gpu_device, generator=g)
+    want = linear_cross_entropy(h, w.clone(), t)
+    dh, = torch.autograd.grad(want, [h])
+    loss = torch.compile(lambda h, w: linear_cross_entropy(h, w, t), fullgraph=True, backend="aot_eager")(h, w)
+    assert torch.equal(loss, want) and torch.equal(torch.autograd.grad(loss, [h])[0], dh)
+
+
 def test_second_derivatives_are_refused(gpu_device):
     h, w, t = _operands(_gen(0), 8, 50, 64, torch.float32, gpu_device)
     gh, = torch.autograd.grad(linear_cross_entropy(h, w, t), [h], create_graph=True)
