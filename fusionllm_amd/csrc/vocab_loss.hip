@@ -30,6 +30,7 @@
 // such numbers the six largest are added, the smallest first; what is left out is below 2^-22 of the largest.  G is rounded the same way: half a step of bf16,
 // 2^-8 of an element at most, before the elements of a row or column are summed in fp32.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/fusionvocab.h"
@@ -2155,6 +2156,13 @@ bool vl_sizes_ok(int64_t T, int64_t dim, int64_t vocab, int64_t top, int planes)
          vocab * dim <= FMOE_VOCAB_MAX_ELEMENTS && T * top < (int64_t(1) << 31) && (planes == 1 || planes == 3);
 }
 
+// Factors that the kernels hold in fp32: logit_scale / temperature * log2(e), logit_scale * temperature, temperature^2 and
+// 1 / temperature are in range.
+bool vl_factors_ok(double logit_scale, double temperature) {
+  return temperature >= 0x1p-63 && temperature <= 0x1p63 &&
+         std::fabs(logit_scale) * std::max(temperature, 1.0 / temperature) < 0x1p126;
+}
+
 bool vl_packs(const void* weight, int w_dtype, int64_t ldw, int64_t dim, int planes) {
   return planes != 1 || w_dtype != FMOE_BF16 || dim % 64 != 0 || ldw % 8 != 0 || !aligned16(weight);
 }
@@ -2202,7 +2210,7 @@ struct VlCall {
 int vl_check(const VlCall& a, const void* state, const void* workspace) {
   const bool distill = a.distill();
   if (a.T < 0 || a.dim <= 0 || a.vocab <= 0 || a.top <= 0 || a.index64 < 0 || a.index64 > 1 || a.reduction < 0 ||
-      a.reduction > 2 || (a.planes != 1 && a.planes != 3) || !(a.temperature > 0.0) ||
+      a.reduction > 2 || (a.planes != 1 && a.planes != 3) || !vl_factors_ok(a.logit_scale, a.temperature) ||
       (!distill && a.T > 0 && a.temperature != 1.0))  // (without rows there may be no address to tell them apart)
     return FMOE_ERR_INVALID_ARG;
   if (!vl_sizes_ok(a.T, a.dim, a.vocab, a.top, a.planes)) return FMOE_ERR_SHAPE;
@@ -2450,7 +2458,7 @@ extern "C" int fmoe_vocab_loss_bwd(const float* d_loss, const void* weight, int 
                                    void* d_hidden, int dh_dtype, void* d_weight, int dw_dtype, void* workspace,
                                    size_t workspace_bytes, void* stream) {
   if (T < 0 || dim <= 0 || vocab <= 0 || top <= 0 || distill < 0 || distill > 1 || (!distill && top != 1) ||
-      reduction < 0 || reduction > 2 || (planes != 1 && planes != 3) || !(temperature > 0.0) ||
+      reduction < 0 || reduction > 2 || (planes != 1 && planes != 3) || !vl_factors_ok(logit_scale, temperature) ||
       (!distill && temperature != 1.0))
     return FMOE_ERR_INVALID_ARG;
   if (!vl_sizes_ok(T, dim, vocab, top, planes)) return FMOE_ERR_SHAPE;

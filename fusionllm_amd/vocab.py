@@ -211,12 +211,16 @@ def _check_loss(what, hidden, weight, reduction, logit_scale):
 
 def _vocab_loss(what, hidden, weight, index, teacher, ignore_index, logit_scale, temperature, planes, reduction):
     """index and teacher: hidden's leading shape and the list."""
+    logit_scale, temperature = float(logit_scale), float(temperature)
+    if not (2.0 ** -63 <= temperature <= 2.0 ** 63 and
+            abs(logit_scale) * max(temperature, 1.0 / temperature) < 2.0 ** 126):
+        raise ValueError(f"{what}: logit_scale {logit_scale} and temperature {temperature} leave the range of fp32")
     shape = hidden.shape[:-1]
     flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     index = index.reshape(-1, index.shape[-1]).contiguous()
     if teacher is not None:
         teacher = teacher.detach().reshape(index.shape).contiguous()
-    args = (flat, weight, index, teacher, int(ignore_index), float(logit_scale), float(temperature), planes, reduction)
+    args = (flat, weight, index, teacher, int(ignore_index), logit_scale, temperature, planes, reduction)
     if torch.compiler.is_compiling():
         # (the traced form sees no addresses: a weight as it lies in a module)
         packs = planes != 1 or weight.dtype != torch.bfloat16 or weight.shape[1] % 64 != 0 or not weight.is_contiguous()

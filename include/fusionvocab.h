@@ -53,6 +53,7 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  * index [T, top]; an entry whose index is ignore_index, or whose teacher logit is -infinity, is none,
  * and a row without entries has no loss, no gradient, and its hidden state is not read.  An index listed twice
  * counts twice.  Any other index outside 0 .. vocab - 1 makes the row's loss NaN (and with it the gradients).
+ * temperature lies in 2^-63 .. 2^63, and |logit_scale| times it or its inverse below 2^126 (factors in fp32).
  * reduction: loss [T] (0 in rows without entries), or one value, the mean over the rows with entries
  * (NaN where there are none) or their sum.
  *

@@ -280,6 +280,36 @@ def test_loss_refusals():
                 linear_distillation(h, w, index, z.detach(), temperature=bad)
 
 
+def test_factors_outside_fp32_are_refused():
+    # the logits' factor logit_scale / temperature, the gradients' logit_scale * temperature and the loss's temperature^2
+    # are fp32 numbers in the kernels
+    with FakeTensorMode():
+        h, w = torch.empty(3, 64, device="cuda"), torch.empty(10, 64, device="cuda")
+        index, z = torch.empty(3, 5, dtype=torch.long, device="cuda"), torch.empty(3, 5, device="cuda")
+        for bad in (dict(temperature=1e-20), dict(temperature=1e-300), dict(temperature=1e20), dict(logit_scale=-1e38),
+                    dict(logit_scale=1e300), dict(logit_scale=1e25, temperature=1e-15), dict(logit_scale=1e25, temperature=1e15)):
+            with pytest.raises(ValueError, match="fp32"):
+                linear_distillation(h, w, index, z, **bad)
+        with pytest.raises(ValueError, match="fp32"):
+            linear_cross_entropy(h, w, index[:, 0], logit_scale=1e38)
+    lib = _lib.load()
+    big = 1 << 40  # (more than any workspace below; nothing is launched: the loss's address is missing)
+
+    def fwd(scale, temp, teacher=FAKE, grad=False):
+        head = (FAKE, 0, 64, FAKE, 0, 64, FAKE, 1, teacher, 1, 100, 64, 100, 1, -100, scale, temp, 1, 1)
+        if grad:
+            return lib.fmoe_vocab_loss_fwd_grad(*head, FAKE + 2, FAKE, 0, FAKE, 0, FAKE, big, None)
+        return lib.fmoe_vocab_loss_fwd(*head, FAKE + 2, FAKE, big, FAKE, big, None)
+
+    def bwd(scale, temp):
+        return lib.fmoe_vocab_loss_bwd(FAKE + 2, FAKE, 0, 64, 100, 64, 100, 1, 1, scale, temp, 1, 1, FAKE, big, FAKE, 0, FAKE,
+                                       0, FAKE, big, None)
+
+    for scale, temp, rc in ((1.0, 2.0, 3), (-1e3, 1e-3, 3), (1.0, 1e-20, 1), (1.0, 1e20, 1), (1e38, 1.0, 1), (1e25, 1e15, 1),
+                            (1e25, 1e-15, 1), (float("nan"), 1.0, 1), (float("inf"), 1.0, 1)):
+        assert fwd(scale, temp) == fwd(scale, temp, grad=True) == bwd(scale, temp) == rc, (scale, temp)
+
+
 def test_embedding_module_has_torchs_interface():
     a, b = Embedding(12, 8, padding_idx=2, scale=3.0), torch.nn.Embedding(12, 8, padding_idx=2)
     assert isinstance(a, torch.nn.Embedding) and a.scale == 3.0 and a.padding_idx == 2
