@@ -433,6 +433,30 @@ def test_infinite_operands(gpu_device):
     assert float(linear_cross_entropy(hb, wb, t).detach()) == math.inf
 
 
+@pytest.mark.parametrize("T", [1, 20, 50, 64])
+def test_infinite_rows_of_the_vocabulary_in_fp32(gpu_device, T):
+    # up to 64 rows run on fp32 products, so that a row of -infinity against positive hidden states is a token that is never
+    # taken: the losses of the vocabulary without it (a dot product of 64 terms below 1 x 4, twice, and the sums behind it)
+    g = _gen(T)
+    V, D = 300, 64
+    h = (0.01 + 0.9 * torch.rand(T, D, generator=g)).to(gpu_device)
+    w = torch.randn(V, D, generator=g).clamp(-4, 4).to(gpu_device)
+    w[7] = -math.inf
+    t = torch.randint(8, V, (T,), generator=g).to(gpu_device)
+    rest = torch.cat([w[:7], w[8:]]).double()
+    s = h.double() @ rest.T
+    size = (h.double() @ rest.abs().T).amax(1)
+    want = torch.logsumexp(s, 1) - s.gather(1, t[:, None] - 1)[:, 0]
+    _within(linear_cross_entropy(h, w, t, reduction="none"), want,
+            (4 * (6 * D + 16) * size + 64 + 4 * (V / 128 + 8)) * U + 8 * U * (want.abs() + size), "loss")
+    index = torch.stack([t, t.roll(1)], 1)
+    q = torch.softmax(torch.zeros(T, 2, device=gpu_device, dtype=torch.float64), 1)
+    log_p = s - torch.logsumexp(s, 1, keepdim=True)
+    want = (q * (q.log() - log_p.gather(1, index - 1))).sum(1)
+    _within(linear_distillation(h, w, index, torch.zeros(T, 2, device=gpu_device), reduction="none"), want,
+            (4 * (6 * D + 16) * size + 128 + 4 * (V / 128 + 8)) * U + 16 * U * (want.abs() + size), "distillation")
+
+
 @pytest.mark.parametrize("T", [40, 300])
 def test_backward_passes_of_a_graph_that_is_kept(gpu_device, T):
     # gradients formed in the forward are handed out scaled; a second pass gets its own
