@@ -14,7 +14,8 @@
 // up to a factor per row, which is known when the piece's logits are done.  A call with a loss per row, whose weights
 // only the backward brings, reduces a tile's logits to a maximum and a sum of exponentials per row, and forms
 // them again in the backward, a piece of the vocabulary at a time: one product more (8 instead of
-// 6 T V d flops).  Either way the extra memory is bounded by a piece.  All products are bound by the matrix units and run on
+// 6 T V d flops).  The extra memory is that of a piece and what goes by the rows: the packed rows, dH's sums between pieces, and
+// without gradients at once the partial maxima and sums, 8 bytes per row and 128 columns (T V / 16 in all).  All products are bound by the matrix units and run on
 // the main loop of gemm_core.h: 256 x 256 tiles, persistent workgroups, copies in one ring over all
 // of a workgroup's tiles.
 //
@@ -313,9 +314,9 @@ __global__ __launch_bounds__(256) void vl_pack32_kernel(const float* src, int64_
 // LOGITS as STATS, and t of the rows
 // H and G are row-major, so A is K-contiguous but for DW (G^T: read with transposing LDS reads), and B is
 // K-contiguous where logits are formed, and read as it lies, transposing, for DH (W) and DW (H).
-// All are bound by the matrix units.  32768 rows x 2048, vocab 131072, bf16: PROB 1.38 PFLOP/s, DH 1.41, DW 1.29 (it also
+// All are bound by the matrix units.  32768 rows x 2048, vocab 131072, bf16: PROB 1.42 PFLOP/s, DH 1.43, DW 1.29 (it also
 // adds 1 GB of fp32 a piece), where a library product of such sizes reaches 1.42.  At K = 768 (16384 rows, vocab 50021) PROB
-// has only 12 K steps a tile to an epilogue of exponentials and stores, in which the matrix units idle: 1.06; DH 1.25, DW 1.28.
+// has only 12 K steps a tile to an epilogue of exponentials and stores, in which the matrix units idle: 1.07; DH 1.30, DW 1.30.
 enum VlMode { VL_STATS = 0, VL_GRAD = 1, VL_DH = 2, VL_DW = 3, VL_PROB = 4, VL_LOGITS = 5 };
 
 struct VlGemm {
@@ -1352,9 +1353,8 @@ void vl_thin_direct(const VlGemm& a, const RowsArgs& r, const void* weight, int 
 // of four products (column d0 + 4 m + i is row m of product i, so that a lane ends with 16 consecutive columns), and the
 // step's G comes from LDS, four vocabulary rows a lane at a time.  The vocabulary is split over workgroups, and where the
 // rows are short over the waves of one; vl_thin_join_kernel adds their partial rows in order.  Training, vocab 50021 x 1024:
-// 20 rows 457 us with the packed copy, 318; 60 rows 507 and 421.  (bf16 rows of odd lengths this way: 5 rows x 1001 x 50021
-// 195 and 187 us, 20 rows 197 and 211: not taken.)  One workgroup a CU above 16 rows: two would spill (20 rows: 307
-// with two spilled registers).
+// 20 rows 457 us with the packed copy, 307; 60 rows 507 and 408.  (bf16 rows of odd lengths this way: 5 rows x 1001 x 50021
+// 195 and 187 us, 20 rows 197 and 211: not taken.)  One workgroup a CU above 16 rows: two would spill.
 constexpr int kDhRows = 256;  // vocabulary rows whose G is in LDS
 struct ThinDh {
   int across, ranges;  // waves side by side; parts of the vocabulary
@@ -1929,7 +1929,7 @@ __global__ __launch_bounds__(256) void vl_fix_kernel(const FixArgs a) {
 // same (kFarSum), or is no number, the piece's flag is set, and STATS and GRAD form its statistics and G in
 // the ordinary way (with H itself in place of 2^-l H); else those launches end at once.
 // 2^-l H is rounded once more (planes = 1: half a step of bf16 an element, as G).  32768 rows x 2048, vocab 131072: 51.8 ms with
-// the logits formed twice, 39.7 at once.
+// the logits formed twice, 39.4 at once.
 
 // o of cross entropy's rows, a wave each.
 template <int DT>

@@ -65,6 +65,8 @@ int fmoe_embedding_bwd(const void* ids, int index64, const void* dy, int dy_dtyp
  * operands (both), whose rows are taken as two scaled fp16 numbers each for the logits (three products) and, like G, as
  * three bf16 numbers for the gradients (the six largest products; 24 bits of elements down to 2^-109): fp32 precision; up to 64 rows the logits and d_hidden are fp32 products.
  * Long lists of a distillation read their logits from a piece of at most 256 MB in the workspace.
+ * The forward's workspace holds a maximum and a sum per row and 128 columns (T vocab / 16 bytes), the backward's a piece of G (2 GiB,
+ * or 256 columns) and fp32 sums of d_hidden where there are several.
  * Deterministic, no atomics.
  *
  * state keeps what the backward needs (fmoe_vocab_loss_state_bytes); it belongs to one forward call.
